@@ -160,7 +160,7 @@ def prepare(case, seed):
         s["slots"] = torch.randperm(pages * page, device=dev, generator=gen)[:tokens].contiguous()
         for n in ("k", "v"):
             s[n + "_cache"] = torch.zeros(pages, page, heads, d, device=dev, dtype=torch.float8_e4m3fn)
-            s[n + "_scale"] = torch.zeros(pages, page, heads, device=dev, dtype=torch.float32)
+            s[n + "_scale"] = torch.zeros(pages, heads, page, device=dev, dtype=torch.float32)
         return s
     h, hk = case["heads"], case["kv_heads"]
     lengths = _lengths(case)
@@ -186,7 +186,7 @@ def prepare(case, seed):
             s[n + "_scale"] = None
             if case["cache"] == "e4m3":
                 x, s[n + "_scale"] = _quantised(x)
-                s[n + "_scale"] = s[n + "_scale"].contiguous()
+                s[n + "_scale"] = s[n + "_scale"].transpose(1, 2).contiguous()
             s[n + "_cache"] = x
         return s
     if case["packed"]:
@@ -246,10 +246,9 @@ def _own(s):
                                  dtype=s["dtype"])
     if s["op"] == "paged":
         return ops.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["table"], s["seq_lens"],
-                                   cu_seqlens=s["cu"], max_len=case["rows"], k_scale=s["k_scale"],
+                                   cu_seqlens=s["cu"], max_rows=case["rows"], k_scale=s["k_scale"],
                                    v_scale=s["v_scale"])
-    out = prompt_attention(s["q"], s["k"], s["v"], causal=case["causal"], key_mask=s["mask"], cu_seqlens=s["cu"],
-                           max_len=case["high"])
+    out = prompt_attention(s["q"], s["k"], s["v"], causal=case["causal"], key_mask=s["mask"], cu_seqlens=s["cu"])
     if s["op"] == "prompt":
         return out
     return (out.detach(), *torch.autograd.grad(out, (s["q"], s["k"], s["v"]), s["grad"]))
@@ -257,13 +256,14 @@ def _own(s):
 
 def _plain_cache(s):
     slots = s["slots"]
+    at = (slots // s["case"]["page"], slice(None), slots % s["case"]["page"])
     back = []
     for n in ("k", "v"):
         codes, scale = _quantised(s[n])
         flat = s[n + "_cache"].view(torch.uint8).flatten(0, 1)
         flat[slots] = codes.view(torch.uint8)
-        s[n + "_scale"].flatten(0, 1)[slots] = scale
-        read = flat[slots].view(torch.float8_e4m3fn).float() * s[n + "_scale"].flatten(0, 1)[slots][..., None]
+        s[n + "_scale"][at] = scale
+        read = flat[slots].view(torch.float8_e4m3fn).float() * s[n + "_scale"][at][..., None]
         back.append(read.to(s["dtype"]))
     return tuple(back)
 
@@ -352,7 +352,7 @@ def _plain_paged(s):
         x = s[n + "_cache"]
         if s[n + "_scale"] is not None:
             x = x.view(torch.uint8)[s["table"].long()].view(torch.float8_e4m3fn).float()
-            x = x * s[n + "_scale"][s["table"].long()][..., None]
+            x = x * s[n + "_scale"][s["table"].long()].transpose(2, 3)[..., None]
         else:
             x = x[s["table"].long()].float()
         got.append(x.flatten(1, 2).transpose(1, 2))
@@ -391,7 +391,7 @@ def exact(case, seed):
                     c = c[pages].double()
                 else:
                     c = c.view(torch.uint8)[pages].view(torch.float8_e4m3fn).double()
-                    c = c * s[x + "_scale"][pages].double()[..., None]
+                    c = c * s[x + "_scale"][pages].double().transpose(1, 2)[..., None]
                 full[x] = c.reshape(-1, hk, d)[:n]
             i = torch.arange(n - rows, n, device="cuda")
             see = torch.arange(n, device="cuda")[None, :] <= i[:, None]
