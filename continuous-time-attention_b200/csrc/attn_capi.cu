@@ -1,0 +1,290 @@
+// C ABI of the attention and key/value-cache operators: argument checks, the
+// choice of kernel, launches.  Declarations and contracts live in
+// include/cta_stencil.h.
+#include <cstring>
+
+#include "attn.h"
+#include "cta_stencil.h"
+
+namespace cta {
+void set_last_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
+}
+
+using namespace cta;
+
+namespace {
+
+constexpr int kMaxHeadDim = 256;
+
+#define fail(code, ...) (set_last_error(__VA_ARGS__), (code))
+
+int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return CTA_OK;
+  return fail(CTA_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+AttnStrides strides(const int64_t s[3]) { return AttnStrides{s[0], s[1], s[2]}; }
+
+// argument checks shared by both directions; kNothing = an empty call
+constexpr int kNothing = -1;
+int prompt_args(const cta_attention_args* p, AttnArgs& a) {
+  if (p == nullptr) return fail(CTA_EINVAL, "null arguments");
+  if (p->dtype != CTA_F32 && p->dtype != CTA_BF16 && p->dtype != CTA_F16)
+    return fail(CTA_EINVAL, "unsupported dtype code %d", p->dtype);
+  if (p->batch < 0 || p->length < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0)
+    return fail(CTA_EINVAL, "bad shape: batch %lld, length %lld, heads %lld, kv_heads %lld", (long long)p->batch,
+                (long long)p->length, (long long)p->heads, (long long)p->kv_heads);
+  if (p->dim < 1 || p->dim > kMaxHeadDim)
+    return fail(CTA_EINVAL, "head dim must be in 1..%d, got %lld", kMaxHeadDim, (long long)p->dim);
+  if (p->length >= (1LL << 30) || p->batch >= (1LL << 30) || p->heads >= (1LL << 20))
+    return fail(CTA_EUNSUPPORTED, "batch, length and heads must be below 2^30, 2^30 and 2^20");
+  if (p->cu_seqlens != nullptr && p->mask_words != nullptr)
+    return fail(CTA_EINVAL, "a key mask takes padded sequences, not packed ones");
+  if (p->batch == 0 || p->length == 0) return kNothing;
+  if (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr)
+    return fail(CTA_EINVAL, "null tensor pointer");
+  std::memset(&a, 0, sizeof(a));
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.o = p->out;
+  a.lse = p->lse;
+  a.g = p->grad_out;
+  a.delta = p->delta;
+  a.dq = p->dq;
+  a.dk = p->dk;
+  a.dv = p->dv;
+  a.qs = strides(p->q_stride);
+  a.ks = strides(p->k_stride);
+  a.vs = strides(p->v_stride);
+  a.os = strides(p->out_stride);
+  a.gs = strides(p->grad_stride);
+  a.dqs = strides(p->dq_stride);
+  a.dks = strides(p->dk_stride);
+  a.dvs = strides(p->dv_stride);
+  a.cu = p->cu_seqlens;
+  a.mask = p->mask_words;
+  a.mask_words = cta_attention_mask_words_per_row(p->length);
+  a.L = p->length;
+  a.nseq = static_cast<int>(p->batch);
+  a.H = static_cast<int>(p->heads);
+  a.Hk = static_cast<int>(p->kv_heads);
+  a.d = static_cast<int>(p->dim);
+  a.causal = p->causal != 0;
+  a.zero_tail = p->zero_tail != 0;
+  a.scale = p->scale;
+  return CTA_OK;
+}
+
+int cache_args(const cta_kv_cache_args* p, bool write, CacheArgs& a) {
+  if (p == nullptr) return fail(CTA_EINVAL, "null arguments");
+  if (p->dtype != CTA_BF16 && p->dtype != CTA_F16)
+    return fail(CTA_EINVAL, "the cache takes bf16 or fp16 rows, got dtype code %d", p->dtype);
+  if (p->tokens < 0 || p->kv_heads < 1 || p->pages < 0 || p->page_size < 1)
+    return fail(CTA_EINVAL, "bad cache shape");
+  if (p->dim < 16 || p->dim > kMaxHeadDim || p->dim % 16 != 0)
+    return fail(CTA_EINVAL, "the cache's head dim must be a multiple of 16 in 16..%d, got %lld", kMaxHeadDim,
+                (long long)p->dim);
+  if (p->pages * p->page_size >= (1LL << 31) || p->tokens * p->kv_heads >= (1LL << 30))
+    return fail(CTA_EUNSUPPORTED, "slots must be below 2^31, tokens * heads below 2^30");
+  if (p->quantized && (p->k_scale == nullptr || p->v_scale == nullptr))
+    return fail(CTA_EINVAL, "an e4m3 cache needs its scales");
+  if (p->tokens == 0) return kNothing;
+  if (p->k == nullptr || p->v == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->slots == nullptr)
+    return fail(CTA_EINVAL, "null tensor pointer");
+  const int64_t rows = 8, cells = p->quantized ? 16 : 8;  // elements in 16 bytes
+  for (int64_t s : {p->k_stride[0], p->k_stride[1], p->v_stride[0], p->v_stride[1]})
+    if (s % rows != 0) return fail(CTA_EINVAL, "rows must start on 16 bytes");
+  for (int64_t s : {p->k_cache_stride[0], p->k_cache_stride[1], p->k_cache_stride[2], p->v_cache_stride[0],
+                    p->v_cache_stride[1], p->v_cache_stride[2]})
+    if (s % cells != 0) return fail(CTA_EINVAL, "the cache's rows must start on 16 bytes");
+  for (const void* x : {p->k, p->v, (const void*)p->k_cache, (const void*)p->v_cache})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
+  std::memset(&a, 0, sizeof(a));
+  if (write) {
+    a.k_in = p->k;
+    a.v_in = p->v;
+  } else {
+    a.k_out = const_cast<void*>(p->k);
+    a.v_out = const_cast<void*>(p->v);
+  }
+  a.k_sT = p->k_stride[0];
+  a.k_sH = p->k_stride[1];
+  a.v_sT = p->v_stride[0];
+  a.v_sH = p->v_stride[1];
+  a.k_cache = p->k_cache;
+  a.v_cache = p->v_cache;
+  a.kc_sP = p->k_cache_stride[0];
+  a.kc_sS = p->k_cache_stride[1];
+  a.kc_sH = p->k_cache_stride[2];
+  a.vc_sP = p->v_cache_stride[0];
+  a.vc_sS = p->v_cache_stride[1];
+  a.vc_sH = p->v_cache_stride[2];
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.slots = p->slots;
+  a.T = p->tokens;
+  a.n_slots = p->pages * p->page_size;
+  a.page = static_cast<int>(p->page_size);
+  a.Hk = static_cast<int>(p->kv_heads);
+  a.d = static_cast<int>(p->dim);
+  a.quantized = p->quantized != 0;
+  return CTA_OK;
+}
+
+int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
+  if (p == nullptr) return fail(CTA_EINVAL, "null arguments");
+  if (p->dtype != CTA_BF16 && p->dtype != CTA_F16)
+    return fail(CTA_EINVAL, "paged attention takes bf16 or fp16, got dtype code %d", p->dtype);
+  if (p->rows < 0 || p->batch < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0)
+    return fail(CTA_EINVAL, "bad shape: rows %lld, batch %lld, heads %lld, kv_heads %lld", (long long)p->rows,
+                (long long)p->batch, (long long)p->heads, (long long)p->kv_heads);
+  if (p->dim < 16 || p->dim > 128 || p->dim % 16 != 0)
+    return fail(CTA_EINVAL, "paged attention's head dim must be a multiple of 16 in 16..128, got %lld",
+                (long long)p->dim);
+  if (p->page_size < 16 || p->page_size % 16 != 0)
+    return fail(CTA_EINVAL, "the page size must be a multiple of 16, got %lld", (long long)p->page_size);
+  if (p->pages < 0 || p->pages * p->page_size >= (1LL << 31) || p->table_width < 0 ||
+      p->table_width * p->page_size >= (1LL << 31) - 64 || p->rows >= (1LL << 28) || p->batch >= (1LL << 28) ||
+      p->rows * p->heads >= (1LL << 31) - 1)
+    return fail(CTA_EUNSUPPORTED, "slots and table_width * page_size must be below 2^31, rows and batch below 2^28");
+  if (p->max_rows < 1) return fail(CTA_EINVAL, "max_rows must be at least 1");
+  if (p->cu_seqlens == nullptr && p->rows != p->batch)
+    return fail(CTA_EINVAL, "without offsets there is one row per sequence: %lld rows, %lld sequences",
+                (long long)p->rows, (long long)p->batch);
+  if (p->quantized && (p->k_scale == nullptr || p->v_scale == nullptr))
+    return fail(CTA_EINVAL, "an e4m3 cache needs its scales");
+  std::memset(&a, 0, sizeof(a));
+  a.q = p->q;
+  a.o = p->out;
+  a.q_sT = p->q_stride[0];
+  a.q_sH = p->q_stride[1];
+  a.o_sT = p->out_stride[0];
+  a.o_sH = p->out_stride[1];
+  a.k_cache = p->k_cache;
+  a.v_cache = p->v_cache;
+  a.kc_sP = p->k_cache_stride[0];
+  a.kc_sS = p->k_cache_stride[1];
+  a.kc_sH = p->k_cache_stride[2];
+  a.vc_sP = p->v_cache_stride[0];
+  a.vc_sS = p->v_cache_stride[1];
+  a.vc_sH = p->v_cache_stride[2];
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.table = p->block_table;
+  a.table_sB = p->table_stride;
+  a.seq_lens = p->seq_lens;
+  a.cu = p->cu_seqlens;
+  a.T = p->rows;
+  a.B = static_cast<int>(p->batch);
+  a.H = static_cast<int>(p->heads);
+  a.Hk = static_cast<int>(p->kv_heads);
+  a.d = static_cast<int>(p->dim);
+  a.page = static_cast<int>(p->page_size);
+  a.table_width = static_cast<int>(p->table_width);
+  a.n_pages = static_cast<int>(p->pages);
+  a.max_rows = static_cast<int>(p->max_rows < p->rows ? p->max_rows : p->rows);
+  a.scale = p->scale;
+  return CTA_OK;
+}
+
+int64_t split_bytes(int workers, int d) {
+  return 2LL * workers * 16 * ((d <= 64 ? 64 : 128) + 4) * static_cast<int64_t>(sizeof(float));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t cta_attention_mask_words_per_row(int64_t length) { return kMaskHead + (length + 127) / 128 * 4; }
+
+int cta_attention_mask_words(const void* mask, int mask_dtype, int64_t mask_sB, int64_t mask_sL, int64_t B, int64_t L,
+                             uint32_t* words, void* stream) {
+  if (B < 0 || L < 0 || L >= (1LL << 30) || B >= (1LL << 30)) return fail(CTA_EINVAL, "bad mask shape");
+  if (mask_dtype < CTA_MASK_U8 || mask_dtype > CTA_MASK_F16) return fail(CTA_EINVAL, "bad mask dtype %d", mask_dtype);
+  if (B == 0) return CTA_OK;
+  if (mask == nullptr || words == nullptr) return fail(CTA_EINVAL, "null mask pointer");
+  return launched(launch_attn_mask_words(mask, mask_dtype, mask_sB, mask_sL, B, L, words,
+                                         cta_attention_mask_words_per_row(L), static_cast<cudaStream_t>(stream)),
+                  "attention mask launch");
+}
+
+int cta_attention_forward(const cta_attention_args* args, void* stream) {
+  AttnArgs a;
+  const int rc = prompt_args(args, a);
+  if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
+  return launched(launch_attn_simt_fwd(a, args->dtype, static_cast<cudaStream_t>(stream)), "attention forward launch");
+}
+
+int cta_attention_backward(const cta_attention_args* args, void* stream) {
+  AttnArgs a;
+  const int rc = prompt_args(args, a);
+  if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
+  if (a.g == nullptr || a.lse == nullptr || a.delta == nullptr)
+    return fail(CTA_EINVAL, "the backward needs grad_out, lse and the delta scratch");
+  if ((a.dk == nullptr) != (a.dv == nullptr)) return fail(CTA_EINVAL, "dk and dv come together");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = launch_attn_delta(a, args->dtype, st);
+  if (e != cudaSuccess) return launched(e, "attention backward launch");
+  return launched(launch_attn_simt_bwd(a, args->dtype, st), "attention backward launch");
+}
+
+int cta_kv_cache_write(const cta_kv_cache_args* args, void* stream) {
+  CacheArgs a;
+  const int rc = cache_args(args, true, a);
+  if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
+  return launched(launch_cache_write(a, args->dtype, static_cast<cudaStream_t>(stream)), "cache write launch");
+}
+
+int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream) {
+  CacheArgs a;
+  const int rc = cache_args(args, false, a);
+  if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
+  return launched(launch_cache_read(a, args->dtype, static_cast<cudaStream_t>(stream)), "cache read launch");
+}
+
+int64_t cta_paged_attention_workspace_bytes(int64_t rows_per_sequence, int64_t heads, int64_t kv_heads, int64_t dim,
+                                            int dtype, int quantized) {
+  if (kv_heads < 1 || dim < 1) return 0;
+  PagedArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.H = static_cast<int>(heads);
+  a.Hk = static_cast<int>(kv_heads);
+  a.d = static_cast<int>(dim);
+  // the larger of the two row variants, so that any max_rows up to this one fits
+  int workers = 0;
+  for (int64_t rows : {static_cast<int64_t>(1), rows_per_sequence}) {
+    a.max_rows = static_cast<int>(rows);
+    const int w = paged_split_workers(a, dtype, quantized);
+    workers = w > workers ? w : workers;
+  }
+  return split_bytes(workers, a.d);
+}
+
+int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+  PagedArgs a;
+  const int rc = paged_args(args, a);
+  if (rc != CTA_OK) return rc;
+  if (a.T == 0 || a.B == 0) return CTA_OK;
+  if (a.q == nullptr || a.o == nullptr || a.k_cache == nullptr || a.v_cache == nullptr || a.table == nullptr ||
+      a.seq_lens == nullptr)
+    return fail(CTA_EINVAL, "null tensor pointer");
+  const int64_t cells = args->quantized ? 16 : 8;
+  for (int64_t s : {a.q_sT, a.q_sH, a.o_sT, a.o_sH})
+    if (s % 8 != 0) return fail(CTA_EINVAL, "rows must start on 16 bytes");
+  for (int64_t s : {a.kc_sP, a.kc_sS, a.kc_sH, a.vc_sP, a.vc_sS, a.vc_sH})
+    if (s % cells != 0) return fail(CTA_EINVAL, "the cache's rows must start on 16 bytes");
+  for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, static_cast<const void*>(workspace)})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
+  a.workers = paged_split_workers(a, args->dtype, args->quantized);
+  if (workspace == nullptr || workspace_bytes < split_bytes(a.workers, a.d))
+    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)split_bytes(a.workers, a.d),
+                (long long)workspace_bytes);
+  a.part_ml = static_cast<float*>(workspace);
+  a.part_o = a.part_ml + 2LL * a.workers * 16 * 4;
+  return launched(launch_paged_split(a, args->dtype, args->quantized, static_cast<cudaStream_t>(stream)),
+                  "paged attention launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,134 @@
+// Device helpers shared by the attention kernels: which sequence a tile belongs
+// to, the key mask, base-2 exponentials.
+#pragma once
+
+#include "attn.h"
+#include "common.cuh"
+
+namespace cta {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// device-side error code: a page, slot or length outside the cache
+enum : int { kDevBadIndex = 2 };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// A tile of one sequence: rows [row0, row0 + n) of the batch entry / packed row
+// `batch`, the tile's first row at `first` within the sequence.  n == 0: the
+// tile lies behind the last sequence; then tail_index of tail_count such tiles,
+// and row0 is the first row behind the last sequence.
+struct SeqTile {
+  int seq;
+  int batch;
+  int64_t row0;
+  int n;      // length of the sequence
+  int first;  // first row of the tile within it
+  int tail_index, tail_count;
+};
+
+__device__ __forceinline__ void clamp_range(const int32_t* cu, int i, int64_t total, int64_t& begin, int& n) {
+  const int64_t b = min(max(static_cast<int64_t>(__ldg(cu + i)), static_cast<int64_t>(0)), total);
+  const int64_t e = min(max(static_cast<int64_t>(__ldg(cu + i + 1)), b), total);
+  begin = b;
+  n = static_cast<int>(e - b);
+}
+
+// The tile-th tile of `rows` rows.  Called by one whole warp; every lane gets
+// the result.  Packed: the lanes walk the offsets 32 sequences at a time with a
+// prefix sum of the tile counts, so that the host never reads the offsets.
+// Tiles of a sequence are numbered from its end when `backwards` (the last
+// tiles of a causal sequence have the most keys and start first).
+__device__ __forceinline__ SeqTile find_tile(const int32_t* cu, int nseq, int64_t L, int tiles, int tile, int rows,
+                                             bool backwards) {
+  SeqTile t;
+  t.tail_index = t.tail_count = 0;
+  if (cu == nullptr) {
+    t.seq = t.batch = tile / tiles;
+    t.row0 = 0;
+    t.n = static_cast<int>(L);
+    const int i = tile - t.seq * tiles;
+    t.first = (backwards ? tiles - 1 - i : i) * rows;
+    return t;
+  }
+  const int lane = threadIdx.x & 31;
+  t.batch = 0;
+  int before = 0;
+  int64_t end = 0;
+  for (int s0 = 0; s0 < nseq; s0 += 32) {
+    int64_t begin = 0;
+    int n = 0;
+    if (s0 + lane < nseq) clamp_range(cu, s0 + lane, L, begin, n);
+    const int count = (n + rows - 1) / rows;
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (tile < before + total) {
+      const unsigned hit = __ballot_sync(0xffffffffu, tile < before + upto);
+      const int src = __ffs(hit) - 1;
+      t.seq = s0 + src;
+      t.row0 = __shfl_sync(0xffffffffu, begin, src);
+      t.n = __shfl_sync(0xffffffffu, n, src);
+      const int c = __shfl_sync(0xffffffffu, count, src);
+      const int i = tile - before - (__shfl_sync(0xffffffffu, upto, src) - c);
+      t.first = (backwards ? c - 1 - i : i) * rows;
+      return t;
+    }
+    before += total;
+    int64_t e = begin + n;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+    end = max(end, e);
+  }
+  t.seq = nseq;
+  t.row0 = end;
+  t.n = 0;
+  t.first = 0;
+  t.tail_index = tile - before;
+  t.tail_count = tiles - before;
+  return t;
+}
+
+// Upper bound on the tiles of a packed row plus one tile that is always behind
+// the last sequence (it clears the rows there when asked to).
+inline int64_t packed_tiles(int64_t L, int nseq, int rows) { return L / rows + nseq + 1; }
+
+// Sets rows behind the last sequence to zero, head h, `d` elements each.
+template <typename T>
+__device__ __forceinline__ void zero_rows(void* base, const AttnStrides& s, int64_t begin, int64_t end, int h, int d,
+                                          int index, int count) {
+  T* p = static_cast<T*>(base) + h * s.h;
+  for (int64_t r = begin + index; r < end; r += count)
+    for (int c = threadIdx.x; c < d; c += blockDim.x) p[r * s.t + c] = Elem<T>::from_f(0.f);
+}
+
+// First and one past the last valid key of a batch entry.
+__device__ __forceinline__ void mask_range(const AttnArgs& a, int batch, int n, int& lo, int& hi) {
+  lo = 0;
+  hi = n;
+  if (a.mask != nullptr) {
+    const uint32_t* m = a.mask + batch * a.mask_words;
+    lo = static_cast<int>(__ldg(m));
+    hi = min(n, static_cast<int>(__ldg(m + 1)));
+  }
+}
+__device__ __forceinline__ bool mask_key(const uint32_t* m, int j) {
+  return m == nullptr || ((__ldg(m + kMaskHead + (j >> 5)) >> (j & 31)) & 1u);
+}
+
+__device__ __forceinline__ int64_t lse_index(const AttnArgs& a, const SeqTile& t, int h, int row) {
+  return (static_cast<int64_t>(t.batch) * a.H + h) * a.L + t.row0 + row;
+}
+
+}  // namespace cta

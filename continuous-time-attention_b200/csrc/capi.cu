@@ -11,6 +11,7 @@
 #include <mutex>
 #include <string>
 
+#include "attn.h"
 #include "cta_stencil.h"
 #include "kernels.h"
 
@@ -332,8 +333,12 @@ int cta_device_error(int clear) {
   const int a = read_device_error_bld_fwd(clear);
   const int c = read_device_error_bdl(clear);
   const int d = read_device_error_bld_dalpha(clear);
-  if (a < 0 || c < 0 || d < 0) return -1;
-  return a != 0 ? a : (c != 0 ? c : d);
+  const int p = read_device_error_paged(clear);
+  const int k = read_device_error_cache(clear);
+  if (a < 0 || c < 0 || d < 0 || p < 0 || k < 0) return -1;
+  for (int e : {a, c, d, p, k})
+    if (e != 0) return e;
+  return 0;
 }
 
 int cta_set_arithmetic(int mode) {

@@ -11,6 +11,7 @@ operator raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from ctypes import POINTER, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
@@ -95,7 +96,21 @@ _SIGNATURES = {
     "cta_diffusion_shard_bld": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                         c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_void_p]),
+    # the three structs are passed as packed bytes (ATTENTION_ARGS, ...)
+    "cta_attention_forward": (c_int, [c_void_p, c_void_p]),
+    "cta_attention_backward": (c_int, [c_void_p, c_void_p]),
+    "cta_attention_mask_words_per_row": (c_int64, [c_int64]),
+    "cta_attention_mask_words": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "cta_kv_cache_write": (c_int, [c_void_p, c_void_p]),
+    "cta_kv_cache_read": (c_int, [c_void_p, c_void_p]),
+    "cta_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "cta_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
+
+# layouts of cta_attention_args, cta_kv_cache_args and cta_paged_attention_args
+ATTENTION_ARGS = struct.Struct("=12Q24q5q4i2f")
+KV_CACHE_ARGS = struct.Struct("=7Q10q5q2i")
+PAGED_ATTENTION_ARGS = struct.Struct("=9Q11q9q2i2f")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -207,7 +222,8 @@ def ptr_array(tensors) -> ctypes.Array:
 
 
 def device_error(clear: bool = True) -> int:
-    """Device-side error word (0 = ok, 1 = a bounded in-kernel wait timed out)."""
+    """Device-side error word (0 = ok, 1 = a bounded in-kernel wait timed out, 2 = a
+    page, slot or length outside a key/value cache was skipped)."""
     return int(load().cta_device_error(1 if clear else 0))
 
 

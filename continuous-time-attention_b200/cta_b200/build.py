@@ -32,7 +32,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = [
     "bld_fwd_bf16_fm.cu", "bld_fwd_f16_fm.cu", "bld_fwd_bf16.cu", "bld_fwd_f16.cu", "bld_fwd_f32.cu",
     "bld_dalpha_bf16_fm.cu", "bld_dalpha_f16_fm.cu", "bld_dalpha_bf16.cu", "bld_dalpha_f16.cu",
-    "bld_dalpha_f32.cu", "stencil_bdl.cu", "capi.cu", "bld_fwd.cu", "bld_dalpha.cu", "noalloc.cu",
+    "bld_dalpha_f32.cu", "stencil_bdl.cu", "attn_simt.cu", "attn_paged.cu", "kv_cache.cu", "capi.cu", "attn_capi.cu",
+    "bld_fwd.cu", "bld_dalpha.cu", "noalloc.cu",
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = [
@@ -108,20 +109,27 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None, d
     build_dir.mkdir(parents=True, exist_ok=True)
     incs = ["-I", str(INCLUDE), "-I", str(CSRC)] + [f"-D{d}" for d in defines]
 
-    headers = [f for f in _inputs() if f.suffix != ".cu"]
-    newest_header = max((f.stat().st_mtime for f in headers), default=0.0)
+    def newest_input(deps: Path) -> float:
+        # the unit's own inputs, from the compiler's dependency file; a missing one counts as new
+        try:
+            names = deps.read_text().replace("\\\n", " ").split(":", 1)[1].split()
+            return max(Path(n).stat().st_mtime for n in names)
+        except (OSError, IndexError, ValueError):
+            return float("inf")
 
     def compile_one(name: str) -> Path:
         obj = build_dir / (Path(name).stem + ".o")
         # ptxas -v always: its per-kernel report is checked for stack frames
-        cmd = [nvcc, *ARCH_FLAGS, "-Xptxas=-v", *CFLAGS, *incs, "-c", str(CSRC / name), "-o", str(obj)]
+        deps = obj.with_suffix(".d")
+        cmd = [nvcc, *ARCH_FLAGS, "-Xptxas=-v", *CFLAGS, *incs, "-MMD", "-MF", str(deps), "-c", str(CSRC / name),
+               "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
-        # an object is reused when it is newer than its source and every header
-        # and was built by the same command
+        # an object is reused when it is newer than every file it was compiled
+        # from and was built by the same command
         stamp = obj.with_suffix(".cmd")
         if (not force and not verbose and obj.exists() and stamp.exists() and stamp.read_text() == " ".join(cmd)
-                and obj.stat().st_mtime > max((CSRC / name).stat().st_mtime, newest_header)):
+                and obj.stat().st_mtime > newest_input(deps)):
             return obj
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:

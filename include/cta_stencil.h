@@ -48,7 +48,8 @@ int cta_abi_version(void);
 const char* cta_last_error(void);
 
 /* Reads (and optionally clears) the device-side error word of every kernel
- * family: 0 = ok, 1 = a bounded wait inside a kernel timed out.  This call
+ * family: 0 = ok, 1 = a bounded wait inside a kernel timed out, 2 = a page,
+ * slot or length outside a key/value cache was skipped.  This call
  * synchronizes with the device. */
 int cta_device_error(int clear);
 
@@ -283,6 +284,124 @@ int cta_diffusion_shard_bld_dalpha(const void* grad_out, const void* x, void* gr
                                    const void* g_hi_halo, int64_t g_hi_rows, const void* x_lo_halo,
                                    int64_t x_lo_rows, const void* x_hi_halo, int64_t x_hi_rows, int part, int dtype,
                                    int steps, int causal, const float* alpha, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Softmax attention of prompts (no counterpart in the reference, whose models
+ * call torch's nn.TransformerEncoderLayer, src/models/transformers.py:62-72)
+ * ------------------------------------------------------------------------- */
+
+/* out[i] = sum_j P[i, j] v[j],  P[i, :] = softmax over the keys row i sees of
+ * scale * (q[i] . k[j]).  Row i sees key j of its own sequence if the key mask
+ * has bit j and, when causal, j <= i.  A row that sees no key has out = 0,
+ * lse = -inf and takes part in no gradient.
+ *
+ * Padded (cu_seqlens NULL): `batch` sequences of `length` tokens; strides are
+ * {batch, token, head} in elements, the dim axis is contiguous; lse and delta
+ * are [batch, heads, length].  Packed: one row of `length` tokens that holds
+ * `batch` sequences, the i-th in [cu_seqlens[i], cu_seqlens[i + 1]) (DEVICE
+ * int32, batch + 1 entries, from 0, not decreasing); the batch strides are
+ * ignored; lse and delta are [heads, length].  Rows behind the last sequence
+ * keep what they hold in out, or are set to zero with zero_tail != 0; the
+ * gradients there are zero.
+ * heads is a multiple of kv_heads: query head h reads key/value head
+ * h / (heads / kv_heads).  dim: 1..256.  dtype: CTA_F32, CTA_BF16, CTA_F16.
+ * Scores, softmax and sums are fp32; results are rounded once.  16-bit weights
+ * are rounded to 16 bits before they multiply v (and the gradients' products).
+ * Nothing is atomic: results do not depend on timing. */
+typedef struct cta_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                  /* forward: written.  backward: the forward's output */
+  float* lse;                 /* forward: written unless NULL.  backward: read */
+  const void* grad_out;       /* backward only, like the rest of the pointers */
+  float* delta;               /* scratch, laid out as lse */
+  void* dq;                   /* NULL: not wanted */
+  void* dk;                   /* NULL with dv: not wanted */
+  void* dv;
+  const int32_t* cu_seqlens;  /* NULL: padded */
+  const uint32_t* mask_words; /* NULL: every key valid; padded sequences only */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t grad_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  int64_t batch, length, heads, kv_heads, dim;
+  int32_t dtype, causal, zero_tail, reserved;
+  float scale, reserved2;
+} cta_attention_args;
+
+int cta_attention_forward(const cta_attention_args* args, void* stream);
+int cta_attention_backward(const cta_attention_args* args, void* stream);
+
+/* A key mask ([B, L], any listed dtype, non-zero = valid) as the words that the
+ * calls above take: cta_attention_mask_words_per_row(L) words per batch entry. */
+int64_t cta_attention_mask_words_per_row(int64_t length);
+int cta_attention_mask_words(const void* mask, int mask_dtype, int64_t mask_sB, int64_t mask_sL, int64_t B, int64_t L,
+                             uint32_t* words, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged key/value cache (no counterpart in the reference, which leaves the
+ * cache to vLLM)
+ * ------------------------------------------------------------------------- */
+
+/* A cache is k_cache, v_cache: [pages, page_size, kv_heads, dim] with strides
+ * {page, slot, head} (dim contiguous, rows on 16 bytes), in the rows' 16-bit
+ * type, or (quantized) e4m3 codes with fp32 scales k_scale, v_scale
+ * [pages, kv_heads, page_size] contiguous:
+ *   scale = m / 448,  code = e4m3(x * (448 / m)),  m = max(max |x|, 2^-100)
+ * over the dim axis.  Slot s is entry s % page_size of page s / page_size.
+ *
+ * write: row t of k and v ([tokens, kv_heads, dim], strides {token, head}) goes
+ * to slots[t] (DEVICE int64); a negative slot is skipped; slots are distinct
+ * (what a slot named twice holds is undefined).  read: row t of k and v is
+ * written from slots[t], zeros for a negative slot.  A slot past the cache is
+ * skipped (read: zeros) and reported by cta_device_error() as 2.
+ * dim: a multiple of 16 up to 256.  dtype: CTA_BF16, CTA_F16. */
+typedef struct cta_kv_cache_args {
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const int64_t* slots;
+  int64_t k_stride[2], v_stride[2], k_cache_stride[3], v_cache_stride[3];
+  int64_t tokens, kv_heads, dim, pages, page_size;
+  int32_t dtype, quantized;
+} cta_kv_cache_args;
+
+int cta_kv_cache_write(const cta_kv_cache_args* args, void* stream);
+int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
+
+/* Attention of each sequence's newest rows over its cached keys, theirs
+ * included: row r of the n_r rows of sequence b (rows [cu_seqlens[b],
+ * cu_seqlens[b + 1]) of q; cu_seqlens NULL: row b alone) sees keys
+ * j <= seq_lens[b] - n_r + r, key j in slot j % page_size of page
+ * block_table[b, j / page_size].  Rows that see no key are zero; rows of out
+ * behind the last sequence keep what they hold.  max_rows: the longest n_r, as
+ * the host knows it; it only chooses the kernel.  The host reads no device
+ * data.  A page outside the cache or a length past the table counts as no keys
+ * and is reported by cta_device_error() as 2.  page_size: a multiple of 16;
+ * dim: a multiple of 16 up to 128; dtype: CTA_BF16, CTA_F16 (of q and out).
+ * workspace: cta_paged_attention_workspace_bytes(max_rows, ...) bytes on 16,
+ * not shared by calls that may overlap; it needs no clearing. */
+typedef struct cta_paged_attention_args {
+  const void* q;
+  void* out;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  int64_t q_stride[2], out_stride[2], k_cache_stride[3], v_cache_stride[3], table_stride;
+  int64_t rows, batch, heads, kv_heads, dim, pages, page_size, table_width, max_rows;
+  int32_t dtype, quantized;
+  float scale, reserved;
+} cta_paged_attention_args;
+
+int64_t cta_paged_attention_workspace_bytes(int64_t rows_per_sequence, int64_t heads, int64_t kv_heads, int64_t dim,
+                                            int dtype, int quantized);
+int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

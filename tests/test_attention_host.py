@@ -1,0 +1,143 @@
+"""CPU-only checks of the attention and cache operators: refusals before any launch, and the
+oracle against torch's own attention and casts."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle import attention_oracle as A
+
+
+def test_oracle_matches_autograd():
+    gen = torch.Generator().manual_seed(0)
+    q, g = (torch.randn(37, 4, 16, generator=gen, dtype=torch.float64) for _ in range(2))
+    k, v = (torch.randn(37, 2, 16, generator=gen, dtype=torch.float64) for _ in range(2))
+    see = torch.ones(37, 37, dtype=torch.bool).tril()
+    see[:, 5] = False
+    see[0] = False
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    kk, vv = (x.transpose(0, 1).repeat_interleave(2, 0) for x in leaves[1:])
+    s = leaves[0].transpose(0, 1) @ kk.transpose(1, 2) * 0.25
+    p = torch.softmax(s.masked_fill(~see, -1e300), -1) * see.any(-1, keepdim=True)
+    out = (p @ vv).transpose(0, 1)
+    want = torch.autograd.grad(out, leaves, g)
+    got = A.gradients(q, k, v, g, see, 0.25)
+    assert torch.allclose(A.attention(q, k, v, see, 0.25)[0], out, atol=1e-13)
+    for x, y in zip(got, want):
+        assert torch.allclose(x, y, atol=1e-12)
+
+
+def test_oracle_quantises_as_torch_casts():
+    x = torch.randn(500, 3, 64, generator=torch.Generator().manual_seed(1)) * 10
+    codes, scale = A.quantise(x)
+    m = x.abs().amax(-1)
+    cast = (x.double() * (448.0 / m.double())[..., None]).to(torch.float32).to(torch.float8_e4m3fn)
+    assert (codes == cast.double()).float().mean() > 0.9999  # the cast rounds twice
+    assert torch.equal(scale, m.double() / 448)
+
+
+def _qkv(shape=(2, 8), heads=4, kv=2, dim=16, dtype=torch.bfloat16, device="meta"):
+    return (torch.empty(*shape, heads, dim, dtype=dtype, device=device),
+            torch.empty(*shape, kv, dim, dtype=dtype, device=device),
+            torch.empty(*shape, kv, dim, dtype=dtype, device=device))
+
+
+def test_cpu_tensors_are_refused():
+    from cta_b200 import ops
+    from cta_b200.attention import prompt_attention
+
+    q, k, v = _qkv(device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        prompt_attention(q, k, v)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.attention_mask(torch.ones(2, 8))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv_cache_write(q[0], q[0], k, v, torch.zeros(8))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv_cache_read(k, v, torch.zeros(8))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_attention(q[0], k, v, torch.zeros(1, 1), torch.zeros(1))
+
+
+def _null():
+    return ctypes.c_void_p(0)
+
+
+def test_attention_arguments_fail_before_launch():
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def call(fn="cta_attention_forward", pointers=(16,) * 4 + (0,) * 8, batch=1, length=8, heads=4, kv=2, dim=64,
+             dtype=1):
+        args = _lib.ATTENTION_ARGS.pack(*pointers, *(64,) * 24, batch, length, heads, kv, dim, dtype, 0, 0, 0, 0.1, 0.0)
+        return getattr(lib, fn)(args, None), lib.cta_last_error()
+
+    for fn in ("cta_attention_forward", "cta_attention_backward"):
+        assert lib.__getattr__(fn)(None, None) == _lib.CTA_EINVAL
+        for kw, word in ((dict(dtype=7), b"dtype"), (dict(heads=5), b"heads"), (dict(kv=0), b"heads"),
+                         (dict(dim=0), b"head dim"), (dict(dim=257), b"head dim"), (dict(batch=-1), b"shape"),
+                         (dict(length=-1), b"shape"), (dict(pointers=(0,) * 12), b"null"),
+                         (dict(pointers=(16,) * 12), b"key mask")):
+            rc, msg = call(fn, **kw)
+            assert rc == _lib.CTA_EINVAL and word in msg, (fn, kw, msg)
+        assert call(fn, length=1 << 30)[0] == _lib.CTA_EUNSUPPORTED
+        assert call(fn, batch=0)[0] == _lib.CTA_OK and call(fn, length=0)[0] == _lib.CTA_OK
+    # the backward's own inputs; dk without dv
+    assert call("cta_attention_backward")[0] == _lib.CTA_EINVAL
+    rc, msg = call("cta_attention_backward", pointers=(16,) * 9 + (0,) * 3)
+    assert rc == _lib.CTA_EINVAL and b"dk and dv" in msg
+    assert lib.cta_attention_mask_words_per_row(1) == 8
+    assert lib.cta_attention_mask_words_per_row(129) == 12
+    assert lib.cta_attention_mask_words(None, 9, 0, 0, 1, 1, None, None) == _lib.CTA_EINVAL
+    assert lib.cta_attention_mask_words(None, 0, 0, 0, 1, 1, None, None) == _lib.CTA_EINVAL
+
+
+def test_cache_arguments_fail_before_launch():
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def call(fn, pointers=(16,) * 7, rows=(64, 64), cells=(1024, 64, 64), tokens=2, heads=2, dim=64, pages=4, page=16,
+             dtype=1, quantized=0):
+        args = _lib.KV_CACHE_ARGS.pack(*pointers, *rows, *rows, *cells, *cells, tokens, heads, dim, pages, page, dtype,
+                                       quantized)
+        return getattr(lib, fn)(args, None), lib.cta_last_error()
+
+    for fn in ("cta_kv_cache_write", "cta_kv_cache_read"):
+        assert getattr(lib, fn)(None, None) == _lib.CTA_EINVAL
+        for kw, word in ((dict(dtype=0), b"bf16 or fp16"), (dict(dim=24), b"multiple of 16"), (dict(dim=272), b"head dim"),
+                         (dict(heads=0), b"shape"), (dict(page=0), b"shape"), (dict(rows=(60, 64)), b"16 bytes"),
+                         (dict(cells=(1024, 65, 64)), b"16 bytes"), (dict(cells=(1024, 72, 72), quantized=1), b"16 bytes"),
+                         (dict(pointers=(8,) * 7), b"16 bytes"), (dict(pointers=(0,) * 7), b"null"),
+                         (dict(pointers=(16, 16, 16, 16, 0, 16, 16), quantized=1), b"scales")):
+            rc, msg = call(fn, **kw)
+            assert rc == _lib.CTA_EINVAL and word in msg, (fn, kw, msg)
+        assert call(fn, pages=1 << 28)[0] == _lib.CTA_EUNSUPPORTED
+        assert call(fn, tokens=0)[0] == _lib.CTA_OK
+
+
+def test_paged_arguments_fail_before_launch():
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def call(pointers=(16,) * 9, q=(256, 64), cells=(1024, 64, 64), rows=2, batch=2, heads=4, kv=2, dim=64, pages=4,
+             page=16, width=3, max_rows=1, dtype=1, quantized=0, ws=16, ws_bytes=0):
+        args = _lib.PAGED_ATTENTION_ARGS.pack(*pointers, *q, *q, *cells, *cells, width, rows, batch, heads, kv, dim,
+                                              pages, page, width, max_rows, dtype, quantized, 0.1, 0.0)
+        return lib.cta_paged_attention(args, ws, ws_bytes, None), lib.cta_last_error()
+
+    assert lib.cta_paged_attention(None, None, 0, None) == _lib.CTA_EINVAL
+    for kw, word in ((dict(dtype=0), b"bf16 or fp16"), (dict(heads=3), b"heads"), (dict(dim=40), b"head dim"),
+                     (dict(dim=144), b"head dim"), (dict(page=8), b"page size"), (dict(page=40), b"page size"),
+                     (dict(max_rows=0), b"max_rows"), (dict(pointers=(16,) * 8 + (0,), rows=3), b"one row"),
+                     (dict(pointers=(16,) * 4 + (0,) * 5, quantized=1), b"scales"), (dict(pointers=(0,) * 9), b"null"),
+                     (dict(q=(256, 60)), b"16 bytes"), (dict(cells=(1024, 60, 64)), b"16 bytes"),
+                     (dict(pointers=(24,) * 9), b"16 bytes"), (dict(), b"workspace"), (dict(ws=None), b"workspace")):
+        rc, msg = call(**kw)
+        assert rc == _lib.CTA_EINVAL and word in msg, (kw, msg)
+    assert call(width=1 << 28)[0] == _lib.CTA_EUNSUPPORTED
+    assert call(rows=0)[0] == _lib.CTA_OK and call(batch=0)[0] == _lib.CTA_OK

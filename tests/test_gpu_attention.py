@@ -1,0 +1,390 @@
+"""Attention of prompts against its definition in 64 bits (oracle/attention_oracle.py),
+with the bounds derived there."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import attention_oracle as A
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _rand(gen, *shape, dtype):
+    return torch.randn(*shape, generator=gen, dtype=torch.float32).to(dtype).cuda()
+
+
+def _inputs(shape, heads, kv_heads, dim, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    q = _rand(gen, *shape, heads, dim, dtype=dtype)
+    k = _rand(gen, *shape, kv_heads, dim, dtype=dtype)
+    v = _rand(gen, *shape, kv_heads, dim, dtype=dtype)
+    g = _rand(gen, *shape, heads, dim, dtype=dtype)
+    return q, k, v, g
+
+
+def _see(n, causal, valid=None, device="cuda"):
+    see = torch.ones(n, n, dtype=torch.bool, device=device)
+    if causal:
+        see = see.tril()
+    if valid is not None:
+        see = see & valid.to(device)[None, :]
+    return see
+
+
+def _within(got, want, tol, what):
+    got = got.detach().double()
+    assert got.shape == want.shape
+    bad = ~((got - want).abs() <= tol)
+    if bad.any():
+        i = tuple(bad.nonzero()[0].tolist())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off, first at {i}: {got[i].item()} for "
+                             f"{want[i].item()}, bound {tol[i].item()}")
+
+
+def _check_sequence(got, q, k, v, g, see, scale, dtype, what=""):
+    out, dq, dk, dv = got
+    want, _ = A.attention(q, k, v, see, scale)
+    if dq is None:
+        _within(out, want, A.bounds(q, k, v, see, scale, dtype), what + "out")
+        return
+    tol = A.bounds(q, k, v, see, scale, dtype, g)
+    _within(out, want, tol[0], what + "out")
+    for x, y, t, name in zip((dq, dk, dv), A.gradients(q, k, v, g, see, scale), tol[1:], ("dq", "dk", "dv")):
+        _within(x, y, t, what + name)
+
+
+def _run(q, k, v, g, **kw):
+    from cta_b200.attention import prompt_attention
+
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    out = prompt_attention(q, k, v, **kw)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), g)
+    return out.detach(), dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("length", [1, 2, 31, 64, 65, 127, 128, 129, 255, 300, 513])
+def test_padded_lengths(length, causal, dtype):
+    q, k, v, g = _inputs((2, length), 4, 2, 64, dtype, seed=length)
+    got = _run(q, k, v, g, causal=causal)
+    for b in range(2):
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], _see(length, causal), 64**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [1, 7, 8, 16, 24, 32, 40, 64, 72, 80, 96, 104, 128, 136, 192, 256])
+def test_head_dims(dim, dtype):
+    q, k, v, g = _inputs((1, 150), 2, 1, dim, dtype, seed=dim)
+    got = _run(q, k, v, g, causal=True)
+    _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _see(150, True), dim**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 3), (3, 1), (6, 2), (8, 1), (12, 2), (40, 8), (64, 1)])
+def test_head_groups(heads, kv_heads, dtype):
+    q, k, v, g = _inputs((1, 140), heads, kv_heads, 64, dtype, seed=heads)
+    got = _run(q, k, v, g, causal=True)
+    _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _see(140, True), 64**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_packed(dim, causal, dtype):
+    """Ragged sequences, empty ones among them, with rows behind the last sequence."""
+    lengths = [0, 1, 130, 0, 0, 257, 64, 3, 128, 0]
+    total = sum(lengths)
+    q, k, v, g = _inputs((total + 5,), 4, 2, dim, dtype, seed=dim)
+    for x in (q, k, v, g):
+        x[total:] = float("nan")  # nothing there may be read into a sequence
+    cu = torch.tensor([0] + torch.tensor(lengths).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    got = _run(q, k, v, g, causal=causal, cu_seqlens=cu)
+    at = 0
+    for n in lengths:
+        part = slice(at, at + n)
+        if n:
+            _check_sequence([x[part] for x in got], q[part], k[part], v[part], g[part], _see(n, causal), dim**-0.5,
+                            dtype, f"at {at}: ")
+        at += n
+    for x in got:
+        assert (x[total:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_packed_many_sequences(dtype):
+    """More sequences than lanes of a warp."""
+    gen = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, 90, (150,), generator=gen).tolist()
+    q, k, v, g = _inputs((sum(lengths),), 2, 2, 64, dtype, seed=9)
+    cu = torch.tensor([0] + torch.tensor(lengths).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    got = _run(q, k, v, g, causal=True, cu_seqlens=cu)
+    at = 0
+    for n in lengths:
+        part = slice(at, at + n)
+        if n:
+            _check_sequence([x[part] for x in got], q[part], k[part], v[part], g[part], _see(n, True), 0.125, dtype)
+        at += n
+
+
+def test_packed_neighbours_do_not_mix():
+    """A sequence's result does not depend on its neighbours' values, NaN among them."""
+    from cta_b200.attention import prompt_attention
+
+    for dtype in DTYPES:
+        q, k, v, g = _inputs((300,), 2, 2, 64, dtype)
+        cu = torch.tensor([0, 100, 170, 300], dtype=torch.int32, device="cuda")
+        clean = _run(q, k, v, g, causal=False, cu_seqlens=cu)
+        for x in (q, k, v, g):
+            x[:100] = float("nan")
+            x[170:] = float("inf")
+        dirty = _run(q, k, v, g, causal=False, cu_seqlens=cu)
+        for x, y in zip(clean, dirty):
+            assert torch.equal(x[100:170], y[100:170])
+        assert prompt_attention(q, k, v, cu_seqlens=cu)[:100].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("kind", ["right", "left", "holes", "none", "one", "all"])
+def test_key_masks(kind, causal, dtype):
+    n = 300
+    q, k, v, g = _inputs((2, n), 2, 1, 64, dtype, seed=3)
+    valid = torch.zeros(2, n, dtype=torch.bool)
+    if kind == "right":
+        valid[0, :131] = True
+        valid[1, :7] = True
+    elif kind == "left":
+        valid[0, 140:] = True
+        valid[1, 299:] = True
+    elif kind == "holes":
+        valid = torch.rand(2, n, generator=torch.Generator().manual_seed(1)) < 0.4
+        valid[1, 128:256] = False
+    elif kind == "one":
+        valid[0, 130] = True
+        valid[1, 0] = True
+    elif kind == "all":
+        valid[:] = True
+    hidden = ~valid.cuda()
+    k[hidden] = float("nan")  # masked places may hold anything
+    v[hidden] = float("inf")
+    got = _run(q, k, v, g, causal=causal, key_mask=valid.cuda())
+    for b in range(2):
+        see = _see(n, causal, valid[b])
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], see, 0.125, dtype, f"{b}: ")
+        assert (got[2][b][hidden[b]] == 0).all() and (got[3][b][hidden[b]] == 0).all()
+        blind = ~see.any(1)
+        assert (got[0][b][blind] == 0).all() and (got[1][b][blind] == 0).all()
+
+
+@pytest.mark.parametrize("mask_dtype", [torch.bool, torch.uint8, torch.int32, torch.int64, torch.float32, torch.bfloat16])
+def test_mask_types_and_strides(mask_dtype):
+    q, k, v, g = _inputs((2, 70), 2, 2, 32, torch.bfloat16)
+    valid = torch.rand(70, 2, generator=torch.Generator().manual_seed(2)) < 0.5
+    a = _run(q, k, v, g, key_mask=valid.t().contiguous().cuda())
+    b = _run(q, k, v, g, key_mask=valid.to(mask_dtype).cuda().t())
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ["projection", "head_major", "odd_offset", "wide_rows", "last_strided"])
+def test_strides(form, dtype):
+    """Views as models make them give what contiguous copies give, bit for bit."""
+    gen = torch.Generator().manual_seed(4)
+    B, L, H, d = 2, 150, 4, 64
+    if form == "projection":
+        x = _rand(gen, B, L, 3, H, d, dtype=dtype)
+        q, k, v = x.unbind(2)
+    elif form == "head_major":
+        q, k, v = (_rand(gen, B, H, L, d, dtype=dtype).transpose(1, 2) for _ in range(3))
+    elif form == "odd_offset":  # rows that TMA cannot address
+        q, k, v = (_rand(gen, B, L, H, d + 3, dtype=dtype)[..., 1 : d + 1] for _ in range(3))
+    elif form == "wide_rows":
+        q, k, v = (_rand(gen, B, L, H, 2 * d, dtype=dtype)[..., d:] for _ in range(3))
+    else:
+        q, k, v = (_rand(gen, B, L, H, d, 2, dtype=dtype)[..., 0] for _ in range(3))
+    g = _rand(gen, B, H, L, d, dtype=dtype).transpose(1, 2)
+    got = _run(q, k, v, g, causal=True)
+    for b in range(B):
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], _see(L, True), d**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_broadcast_keys(dtype):
+    """Keys and values expanded over the batch (stride 0)."""
+    q, k, v, g = _inputs((3, 80), 2, 2, 64, dtype)
+    k1, v1 = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)
+    got = _run(q, k1, v1, g)
+    for b in range(3):
+        _check_sequence([x[b] for x in got], q[b], k[0], v[0], g[b], _see(80, False), 0.125, dtype)
+    # through autograd the gradient of the one row is the sum
+    from cta_b200.attention import prompt_attention
+
+    leaf = k[:1].detach().requires_grad_(True)
+    prompt_attention(q, leaf.expand(3, -1, -1, -1), v1).backward(g)
+    assert torch.allclose(leaf.grad[0].float(), got[2].float().sum(0), rtol=0.02, atol=0.02)
+
+
+def test_offsets_past_31_bits():
+    """Element offsets above 2^31 within one tensor."""
+    n, d = 200, 64
+    stride = (1 << 24) + 64  # 200 rows of it pass 2^31 elements
+    for dtype in (torch.bfloat16, torch.float32):
+        base = torch.zeros(n * stride, dtype=dtype, device="cuda")
+        q, k, v, g = _inputs((1, n), 1, 1, d, dtype)
+        wide = base.as_strided((1, n, 1, d), (0, stride, d, 1))
+        wide.copy_(k)
+        got = _run(q, wide, v, g, causal=True)
+        want = _run(q, k, v, g, causal=True)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+        del base, wide
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_scores(dtype):
+    """Scores far outside the exponential's range: the maximum is taken off first."""
+    q, k, v, g = _inputs((1, 200), 2, 2, 64, dtype)
+    for scale in (0.0, 3.0, -2.0):
+        got = _run(q, k, v, g, scale=scale)
+        _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _see(200, False), scale, dtype, f"scale {scale}: ")
+
+
+def test_lse():
+    from cta_b200 import ops
+
+    for dtype in DTYPES:
+        q, k, v, _ = _inputs((2, 150), 4, 2, 64, dtype)
+        valid = torch.ones(2, 150, dtype=torch.bool)
+        valid[1, :5] = False
+        out, lse = ops.attention_forward(q, k, v, causal=True, mask_words=ops.attention_mask(valid.cuda()))
+        for b in range(2):
+            _, want = A.attention(q[b], k[b], v[b], _see(150, True, valid[b]), 0.125)
+            assert torch.equal(torch.isinf(lse[b]), torch.isinf(want))
+            fin = torch.isfinite(want)
+            # scores: (d + 4) u |q|.|k| / 8 with |q|.|k| below 64 * 3 * 3; sum and logarithm: 2^-20
+            assert ((lse[b].double() - want)[fin].abs() <= 68 * 2.0**-24 * 72 + 2.0**-20 * (1 + want[fin].abs())).all()
+
+
+def test_only_wanted_gradients():
+    from cta_b200.attention import prompt_attention
+
+    q, k, v, g = _inputs((1, 130), 2, 2, 64, torch.bfloat16)
+    full = _run(q, k, v, g, causal=True)
+    for want in ((0,), (1,), (2,), (0, 2)):
+        t = [x.detach().requires_grad_(i in want) for i, x in enumerate((q, k, v))]
+        got = torch.autograd.grad(prompt_attention(*t, causal=True), [t[i] for i in want], g)
+        for i, x in zip(want, got):
+            assert torch.equal(x, full[1 + i])
+
+
+def test_gradient_against_differences():
+    """fp32: the directional derivative against a central difference of the 64-bit definition."""
+    q, k, v, g = _inputs((1, 90), 2, 1, 32, torch.float32)
+    got = _run(q, k, v, g, causal=True)
+    see = _see(90, True)
+    gen = torch.Generator().manual_seed(8)
+    for i, name in enumerate("qkv"):
+        t = [q[0].double(), k[0].double(), v[0].double()]
+        step = torch.randn(t[i].shape, generator=gen, dtype=torch.float64).cuda()
+        f = []
+        for e in (1e-5, -1e-5):
+            u = list(t)
+            u[i] = t[i] + e * step
+            f.append((A.attention(*u, see, 32**-0.5)[0] * g[0].double()).sum())
+        slope = (f[0] - f[1]) / 2e-5
+        mine = (got[1 + i][0].double() * step).sum()
+        # the difference is off by O(e^2) and 2^-53 / e; the gradient's bound is summed up
+        tol = (A.bounds(q[0], k[0], v[0], see, 32**-0.5, torch.float32, g[0])[1 + i] * step.abs()).sum() + 1e-6
+        assert (mine - slope).abs() <= tol, name
+
+
+def test_twice_the_same():
+    for dtype in DTYPES:
+        q, k, v, g = _inputs((2, 400), 4, 2, 64, dtype)
+        a, b = _run(q, k, v, g, causal=True), _run(q, k, v, g, causal=True)
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_empty():
+    from cta_b200.attention import prompt_attention
+
+    for shape in ((0, 5), (2, 0)):
+        q, k, v, g = _inputs(shape, 2, 2, 64, torch.bfloat16)
+        got = _run(q, k, v, g)
+        assert got[0].shape == (*shape, 2, 64)
+    cu = torch.zeros(4, dtype=torch.int32, device="cuda")
+    q, k, v, _ = _inputs((0,), 2, 2, 64, torch.bfloat16)
+    assert prompt_attention(q, k, v, cu_seqlens=cu).shape == (0, 2, 64)
+    # rows, but all sequences empty
+    q, k, v, _ = _inputs((3,), 2, 2, 64, torch.bfloat16)
+    assert (prompt_attention(q, k, v, cu_seqlens=cu) == 0).all()
+    assert (prompt_attention(q, k, v, cu_seqlens=cu[:1]) == 0).all()
+
+
+def test_out_buffer_keeps_tail():
+    from cta_b200 import ops
+
+    for dtype in DTYPES:
+        q, k, v, _ = _inputs((140,), 2, 2, 64, dtype)
+        cu = torch.tensor([0, 60, 133], dtype=torch.int32, device="cuda")
+        out = torch.full_like(q, 7.0)
+        y, _ = ops.attention_forward(q, k, v, cu_seqlens=cu, out=out)
+        assert y is out and (out[133:] == 7).all()
+        z, _ = ops.attention_forward(q, k, v, cu_seqlens=cu)
+        assert torch.equal(out[:133], z[:133]) and (z[133:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_and_replayed(dtype):
+    """Forward and backward in one CUDA graph, replayed on new inputs."""
+    from cta_b200.attention import prompt_attention
+
+    q, k, v, g = _inputs((2, 200), 4, 2, 64, dtype)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            torch.autograd.grad(prompt_attention(*leaves, causal=True), leaves, g)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = prompt_attention(*leaves, causal=True)
+        grads = torch.autograd.grad(out, leaves, g)
+    q2, k2, v2, g2 = _inputs((2, 200), 4, 2, 64, dtype, seed=77)
+    with torch.no_grad():
+        for x, y in zip(leaves, (q2, k2, v2)):
+            x.copy_(y)
+        g.copy_(g2)
+    graph.replay()
+    want = _run(q2, k2, v2, g2, causal=True)
+    for x, y in zip((out, *grads), want):
+        assert torch.equal(x, y)
+
+
+def test_other_stream():
+    q, k, v, g = _inputs((1, 300), 4, 4, 64, torch.bfloat16)
+    want = _run(q, k, v, g, causal=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _run(q, k, v, g, causal=True)
+    torch.cuda.current_stream().wait_stream(s)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_longer(dim, dtype):
+    """Many tiles on both sides, grouped heads."""
+    q, k, v, g = _inputs((1, 2100), 4, 2, dim, dtype)
+    for causal in (True, False):
+        got = _run(q, k, v, g, causal=causal)
+        _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _see(2100, causal), dim**-0.5, dtype)

@@ -1,0 +1,441 @@
+"""The paged key/value cache and the attention that reads it, against their definitions in
+64 bits (oracle/attention_oracle.py)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import attention_oracle as A
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+E4M3 = torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    from cta_b200 import _lib
+
+    _lib.device_error()
+    yield
+    assert _lib.device_error() == 0
+
+
+def _cache(pages, page, heads, dim, dtype, quantized, fill=None, head_major=False):
+    """(k_cache, v_cache, k_scale, v_scale), filled with NaN as memory never written may be."""
+    def one():
+        shape = (pages, heads, page, dim) if head_major else (pages, page, heads, dim)
+        if quantized:
+            t = torch.full(shape, 0x7F, dtype=torch.uint8, device="cuda").view(E4M3)
+        else:
+            t = torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+        return t.transpose(1, 2) if head_major else t
+
+    scales = [torch.full((pages, heads, page), float("nan"), device="cuda") if quantized else None for _ in range(2)]
+    return one(), one(), *scales
+
+
+def _rows(n, heads, dim, dtype, seed, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    size = torch.exp(spread * torch.randn(n, heads, 1, generator=gen))
+    return (torch.randn(n, heads, dim, generator=gen) * size).to(dtype).cuda()
+
+
+def _codes(cache, slots):
+    """The cache's entries at slots, as 64-bit values."""
+    page = cache.shape[1]
+    if cache.dtype == E4M3:
+        return cache.view(torch.uint8)[slots // page, slots % page].view(E4M3).double()
+    return cache[slots // page, slots % page].double()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_major", [False, True])
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 144, 256])
+@pytest.mark.parametrize("tokens", [1, 3, 64, 1000])
+def test_write_and_read(tokens, dim, head_major, dtype):
+    from cta_b200 import ops
+
+    heads, page, pages = 3, 16, 70
+    k, v = _rows(tokens, heads, dim, dtype, 1, 2.0), _rows(tokens, heads, dim, dtype, 2, 2.0)
+    if tokens >= 64:
+        k[5] = 0  # a row of zeros
+        v[6] *= 2.0**-10
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(3))[:tokens].cuda()
+    others = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    others[slots] = False
+    others = others.nonzero()[:, 0]
+    for quantized in (False, True):
+        kc, vc, ks, vs = _cache(pages, page, heads, dim, dtype, quantized, head_major=head_major)
+        ops.kv_cache_write(k, v, kc, vc, slots, k_scale=ks, v_scale=vs)
+        back = ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs, dtype=dtype)
+        for x, c, s, y in ((k, kc, ks, back[0]), (v, vc, vs, back[1])):
+            assert y.dtype == dtype and y.shape == x.shape
+            assert _codes(c, others).isnan().all()  # nothing else was written
+            if not quantized:
+                assert torch.equal(_codes(c, slots), x.double()) and torch.equal(y, x)
+                continue
+            codes, scale = A.quantise(x)
+            got = s[slots // page, :, slots % page].double()
+            assert ((got - scale).abs() <= 2.0**-24 * scale).all()
+            mine = _codes(c, slots)
+            # x * (448 / m) carries two roundings of 2^-24: a value that close to the middle
+            # between two codes may go to the other
+            m = x.double().abs().amax(-1, keepdim=True).clamp_min(2.0**-100)
+            y64 = x.double() * (448.0 / m)
+            assert ((mine - y64).abs() <= (codes - y64).abs() + 2.0**-22 * y64.abs()).all()
+            want = mine * got[..., None]
+            assert ((y.double() - want).abs() <= want.abs() * (torch.finfo(dtype).eps / 2 + 2.0**-23)
+                    + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all()
+
+
+def test_extreme_rows():
+    """Zeros, the smallest and the largest values, infinities and NaN."""
+    from cta_b200 import ops
+
+    k = torch.zeros(6, 1, 16, dtype=torch.bfloat16, device="cuda")
+    k[1] = torch.finfo(torch.bfloat16).tiny
+    k[2] = torch.finfo(torch.bfloat16).max
+    k[2, 0, 0] *= -1
+    k[3] = float("inf")
+    k[4, 0, 3] = float("nan")
+    k[5] = 2.0**-100
+    slots = torch.arange(6, device="cuda")
+    kc, vc, ks, vs = _cache(1, 16, 1, 16, torch.bfloat16, True)
+    ops.kv_cache_write(k, k, kc, vc, slots, k_scale=ks, v_scale=vs)
+    y = ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs)[0]
+    assert (y[0] == 0).all()
+    assert (y[1].abs() <= 2.0**-100).all()  # below the floor: rounded in steps of the floor's scale
+    assert ((y[2].double() - k[2].double()).abs() <= 2.0**-8 * k[2].double().abs()).all()
+    assert y[3].isnan().all()
+    assert y[4, 0, 3].isnan()
+    assert ((y[5].double() - 2.0**-100).abs() <= 2.0**-107).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_padding_and_bad_slots(quantized):
+    from cta_b200 import _lib, ops
+
+    k = _rows(5, 2, 32, torch.bfloat16, 1)
+    kc, vc, ks, vs = _cache(2, 16, 2, 32, torch.bfloat16, quantized)
+    slots = torch.tensor([3, -1, 31, -7, 0], device="cuda")
+    ops.kv_cache_write(k, k, kc, vc, slots, k_scale=ks, v_scale=vs)
+    assert _lib.device_error() == 0
+    assert int(kc.float().isnan().sum()) == (32 - 3) * 2 * 32
+    y, _ = ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs)
+    assert (y[1] == 0).all() and (y[3] == 0).all() and (y[0] != 0).any()
+    before = [c.clone().view(torch.uint8) for c in (kc, vc)]
+    slots[1] = 32  # past the cache: skipped and reported
+    ops.kv_cache_write(k[1:2], k[1:2], kc, vc, slots[1:2], k_scale=ks, v_scale=vs)
+    assert _lib.device_error() == 2 and _lib.device_error() == 0
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (kc, vc)))
+    y, _ = ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs)
+    assert _lib.device_error() == 2
+    assert (y[1] == 0).all()
+    # int32 slots
+    a = ops.kv_cache_read(kc, vc, torch.tensor([3], dtype=torch.int32, device="cuda"), k_scale=ks, v_scale=vs)[0]
+    assert torch.equal(a[0], y[0])
+
+
+def test_strided_rows():
+    """Rows as views of a fused projection, 16-byte aligned or not."""
+    from cta_b200 import ops
+
+    for off in (0, 3):
+        x = torch.randn(20, 3 * 2 * 64 + 8, device="cuda").to(torch.bfloat16)
+        k = x[:, off : off + 128].view(20, 2, 64)
+        v = x[:, off + 128 : off + 256].view(20, 2, 64)
+        kc, vc, _, _ = _cache(2, 16, 2, 64, torch.bfloat16, False)
+        slots = torch.arange(20, device="cuda")
+        ops.kv_cache_write(k, v, kc, vc, slots)
+        y = ops.kv_cache_read(kc, vc, slots)
+        assert torch.equal(y[0], k) and torch.equal(y[1], v)
+
+
+# ---------------------------------------------------------------------------
+# attention over the cache
+# ---------------------------------------------------------------------------
+class Setup:
+    """Sequences of `lens` keys, the newest `rows` of them queried, in shuffled pages."""
+
+    def __init__(self, lens, rows, heads, kv_heads, dim, page, dtype, quantized, seed=0, head_major=False, spread=0.5,
+                 width=None, tail=0):
+        from cta_b200 import ops
+
+        gen = torch.Generator().manual_seed(seed)
+        self.lens, self.rows = lens, rows
+        counts = [-(-n // page) for n in lens]
+        pages = sum(counts) + 3
+        order = torch.randperm(pages, generator=gen).tolist()
+        width = max([1, *counts]) if width is None else width
+        table = torch.full((len(lens), width), 2**31 - 1, dtype=torch.int32)  # entries past the length are not read
+        self.kc, self.vc, self.ks, self.vs = _cache(pages, page, kv_heads, dim, dtype, quantized, head_major=head_major)
+        self.k, self.v = [], []
+        for b, n in enumerate(lens):
+            mine = [order.pop() for _ in range(counts[b])]
+            table[b, : len(mine)] = torch.tensor(mine, dtype=torch.int32)
+            k, v = _rows(n, kv_heads, dim, dtype, 10 * b + 1 + seed, spread), _rows(n, kv_heads, dim, dtype, 10 * b + 2 + seed, spread)
+            slots = torch.tensor([mine[j // page] * page + j % page for j in range(n)], dtype=torch.int64).cuda()
+            ops.kv_cache_write(k, v, self.kc, self.vc, slots, k_scale=self.ks, v_scale=self.vs)
+            if quantized:  # what the cache holds, exactly
+                at = (slots // page, slice(None), slots % page)
+                k = _codes(self.kc, slots) * self.ks[at].double()[..., None]
+                v = _codes(self.vc, slots) * self.vs[at].double()[..., None]
+            self.k.append(k)
+            self.v.append(v)
+        self.table = table.cuda()
+        self.seq_lens = torch.tensor(lens, dtype=torch.int32).cuda()
+        total = sum(rows)
+        self.q = torch.randn(total + tail, heads, dim, generator=gen).to(dtype).cuda()
+        self.cu = torch.tensor([0] + torch.tensor(rows).cumsum(0).tolist(), dtype=torch.int32).cuda()
+        self.dtype, self.quantized, self.dim = dtype, quantized, dim
+
+    def run(self, **kw):
+        from cta_b200 import ops
+
+        if not all(r == 1 for r in self.rows):
+            kw.setdefault("cu_seqlens", self.cu)
+        kw.setdefault("max_rows", max([1, *self.rows]))
+        return ops.paged_attention(self.q, self.kc, self.vc, self.table, self.seq_lens, k_scale=self.ks,
+                                   v_scale=self.vs, **kw)
+
+    def check(self, out, scale=None):
+        scale = self.dim**-0.5 if scale is None else scale
+        at = 0
+        for b, (n, r) in enumerate(zip(self.lens, self.rows)):
+            q, got = self.q[at : at + r], out[at : at + r].double()
+            at += r
+            if r == 0:
+                continue
+            if n == 0:
+                assert (got == 0).all()
+                continue
+            i = torch.arange(n - r, n, device="cuda")
+            see = torch.arange(n, device="cuda")[None, :] <= i[:, None]
+            want, _ = A.attention(q, self.k[b], self.v[b], see, scale)
+            # e4m3: q is rounded to fp16 after an exact scaling, elements below 2^-14 of the largest to 2^-25 of
+            # it: with d elements that is d 2^-25 of |q||k|, inside the (d + 4) 2^-24 of the scores' bound
+            tol = A.bounds(q, self.k[b], self.v[b], see, scale, self.dtype, kv_error=2.0**-20 if self.quantized else 0.0)
+            bad = ~((got - want).abs() <= tol)
+            assert not bad.any(), (b, n, r, int(bad.sum()), (got - want).abs().max().item(), tol.min().item())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 128])
+def test_decode_dims(dim, quantized, dtype):
+    s = Setup([1, 15, 16, 17, 200, 333], [1] * 6, 8, 2, dim, 16, dtype, quantized, seed=dim)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (2, 2), (3, 1), (5, 1), (8, 8), (16, 2), (9, 1), (16, 1), (17, 1), (40, 2), (71, 1)])
+def test_decode_groups(heads, kv_heads, quantized):
+    s = Setup([40, 300, 1], [1] * 3, heads, kv_heads, 64, 32, torch.bfloat16, quantized, seed=heads)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 128, 256])
+def test_pages(page, quantized):
+    s = Setup([page - 1, page, page + 1, 3 * page + 5, 700], [1, 1, 1, 1, 1], 4, 2, 128, page, torch.bfloat16,
+              quantized, seed=page)
+    s.check(s.run())
+    s = Setup([page - 1, page, page + 1, 3 * page + 5, 700], [3, 16, 1, 40, 200], 4, 2, 128, page, torch.bfloat16,
+              quantized, seed=page)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("rows", [[2, 2, 2], [1, 0, 5], [17, 1, 130], [128, 129, 127], [300, 64, 0], [1, 400, 33]])
+def test_chunks(rows, quantized, dtype):
+    lens = [r + x for r, x in zip(rows, (0, 77, 500))]
+    for heads, kv_heads, dim in ((4, 4, 64), (8, 2, 128), (6, 2, 80)):
+        s = Setup(lens, rows, heads, kv_heads, dim, 16, dtype, quantized, seed=sum(rows))
+        s.check(s.run())
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_lengths_zero_and_short(quantized):
+    """No keys at all; more rows than keys (the first rows see nothing)."""
+    s = Setup([0, 5, 0, 200], [1, 1, 1, 1], 4, 2, 64, 16, torch.bfloat16, quantized)
+    s.check(s.run())
+    s = Setup([0, 3, 50], [2, 3, 7], 4, 2, 64, 16, torch.bfloat16, quantized)
+    s.check(s.run())
+    s.seq_lens[2] = 4
+    out = s.run()
+    rows = out[5:12]
+    assert (rows[:3] == 0).all() and (rows[3:] != 0).any() and torch.isfinite(rows.float()).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_one_long_sequence(quantized):
+    """A single sequence over many workers; another with one very long sequence among short ones."""
+    s = Setup([9000], [1], 4, 1, 128, 16, torch.bfloat16, quantized)
+    s.check(s.run())
+    s = Setup([3, 6000, 17, 1], [1, 1, 1, 1], 8, 2, 64, 64, torch.float16, quantized, width=200)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_many_short_sequences(quantized):
+    gen = torch.Generator().manual_seed(1)
+    lens = torch.randint(1, 60, (150,), generator=gen).tolist()
+    s = Setup(lens, [1] * 150, 4, 4, 64, 16, torch.bfloat16, quantized)
+    s.check(s.run())
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_head_major_cache_and_strided_q(quantized):
+    s = Setup([100, 260], [1, 1], 4, 2, 64, 16, torch.bfloat16, quantized, head_major=True)
+    s.check(s.run())
+    wide = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16, device="cuda")
+    wide[:, 1] = s.q
+    want = s.run()
+    s.q = wide[:, 1]
+    assert torch.equal(s.run(), want)
+    odd = torch.zeros(2, 4, 67, dtype=torch.bfloat16, device="cuda")
+    odd[..., 3:] = s.q
+    s.q = odd[..., 3:]
+    assert torch.equal(s.run(), want)
+
+
+@pytest.mark.parametrize("spread", [6.0])
+def test_e4m3_scales_far_apart(spread):
+    """Scales over many orders of magnitude: neither overflow nor vanish in 16 bits."""
+    for dtype in DTYPES:
+        s = Setup([300, 40], [1, 1], 4, 2, 64, 16, torch.bfloat16, True, spread=0.3)
+        for c in (s.vs,):
+            c *= 2.0**-12
+        s.v = [x * 2.0**-12 for x in s.v]
+        s.check(s.run())
+        s = Setup([300, 40], [1, 1], 4, 2, 64, 16, torch.bfloat16, True, spread=0.3)
+        s.vs *= 2.0**14
+        s.v = [x * 2.0**14 for x in s.v]
+        s.check(s.run())
+        s = Setup([300, 40], [1, 1], 4, 2, 64, 16, torch.bfloat16, True, spread=0.3)
+        s.ks *= 2.0**-9
+        s.k = [x * 2.0**-9 for x in s.k]
+        s.q = s.q * 2.0**12
+        s.check(s.run())
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_rows_behind_the_last_sequence(rows, quantized):
+    s = Setup([100, 300], rows, 4, 2, 64, 16, torch.bfloat16, quantized, tail=3)
+    out = torch.full_like(s.q, 7.0)
+    y = s.run(out=out, cu_seqlens=s.cu)
+    assert y is out and (out[sum(rows):] == 7).all()
+    s.check(out)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_bad_pages_and_lengths(rows, quantized):
+    """Skipped and reported; the other sequence keeps its result."""
+    from cta_b200 import _lib
+
+    s = Setup([100, 300], rows, 4, 2, 64, 16, torch.bfloat16, quantized)
+    want = s.run()
+    good = s.table.clone()
+    for bad in (-1, s.kc.shape[0], 2**31 - 1, -(2**31)):
+        s.table[0, 2] = bad
+        got = s.run()
+        assert _lib.device_error() == 2
+        assert torch.equal(got[rows[0]:], want[rows[0]:])
+        assert torch.isfinite(got.float()).all()
+        s.table.copy_(good)
+    for n in (s.table.shape[1] * 16 + 1, 2**31 - 1, -5):
+        s.seq_lens[0] = n
+        s.table[0] = 0
+        s.run()
+        assert _lib.device_error() == 2
+    s.table.copy_(good)
+    s.seq_lens[0] = 100
+    assert torch.equal(s.run(), want)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+def test_max_rows_is_a_hint(rows):
+    s = Setup([100, 300], rows, 8, 2, 64, 16, torch.bfloat16, False)
+    for hint in (1, 3, 100, 1000):
+        s.check(s.run(max_rows=hint, cu_seqlens=s.cu))
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_large_cache(quantized):
+    """Byte and element offsets past 2^31 and 2^32 in the pool."""
+    from cta_b200 import ops
+
+    page, heads, dim = 128, 8, 128
+    pages = 36000  # 4.7e9 elements
+    dtype = torch.bfloat16
+    t = E4M3 if quantized else dtype
+    kc, vc = (torch.empty(pages, page, heads, dim, dtype=t, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(pages, heads, page, device="cuda") if quantized else None for _ in range(2))
+    mine = [35999, 17000, 3, 33000]
+    n = 4 * page - 5
+    k, v = _rows(n, heads, dim, dtype, 1), _rows(n, heads, dim, dtype, 2)
+    slots = torch.tensor([mine[j // page] * page + j % page for j in range(n)], dtype=torch.int64).cuda()
+    ops.kv_cache_write(k, v, kc, vc, slots, k_scale=ks, v_scale=vs)
+    kr, vr = ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs, dtype=dtype)
+    if not quantized:
+        assert torch.equal(kr, k) and torch.equal(vr, v)
+    small = [0, 1, 2, 3]
+    kc2, vc2, ks2, vs2 = _cache(4, page, heads, dim, dtype, quantized)
+    slots2 = torch.arange(n, device="cuda")
+    ops.kv_cache_write(k, v, kc2, vc2, slots2, k_scale=ks2, v_scale=vs2)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for rows in (1, 200):
+        q = torch.randn(rows, 16, dim, device="cuda").to(dtype)
+        cu = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+        a = ops.paged_attention(q, kc, vc, torch.tensor([mine], dtype=torch.int32, device="cuda"), lens, cu_seqlens=cu,
+                                max_rows=rows, k_scale=ks, v_scale=vs)
+        b = ops.paged_attention(q, kc2, vc2, torch.tensor([small], dtype=torch.int32, device="cuda"), lens,
+                                cu_seqlens=cu, max_rows=rows, k_scale=ks2, v_scale=vs2)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [40, 200, 7]])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_captured_twice_and_replayed_together(rows, quantized):
+    """Two graphs captured on one stream, replayed at the same time on two: each has its own workspace."""
+    s = Setup([1500, 300, 2200], rows, 8, 2, 128, 16, torch.bfloat16, quantized)
+    other = Setup([900, 2000, 800], rows, 8, 2, 128, 16, torch.bfloat16, quantized, seed=5)
+    want, want2 = s.run(), other.run()
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for x in (s, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(x.run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+
+
+def test_twice_the_same():
+    for quantized in (False, True):
+        for rows in ([1, 1, 1], [50, 3, 170]):
+            s = Setup([1500, 300, 2200], rows, 8, 2, 128, 16, torch.bfloat16, quantized)
+            assert torch.equal(s.run(), s.run())
+
+
+def test_no_rows_or_sequences():
+    from cta_b200 import ops
+
+    s = Setup([10], [1], 2, 2, 64, 16, torch.bfloat16, False)
+    assert ops.paged_attention(s.q[:0], s.kc, s.vc, s.table[:0], s.seq_lens[:0]).shape == (0, 2, 64)
+    cu = torch.zeros(2, dtype=torch.int32, device="cuda")
+    out = torch.full_like(s.q, 3.0)
+    ops.paged_attention(s.q, s.kc, s.vc, s.table, s.seq_lens, cu_seqlens=cu, out=out)
+    assert (out == 3).all()
