@@ -104,7 +104,12 @@ struct PagedArgs {
 int paged_split_workers(const PagedArgs& a, int dtype, int quantized);
 cudaError_t launch_paged_split(const PagedArgs& a, int dtype, int quantized, cudaStream_t st);
 
+// tensor-core forms; false = not for these types, sizes or strides (nothing was launched)
+bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
+bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
+
 int read_device_error_paged(int clear);
+int read_device_error_tc_fwd(int clear);
 int read_device_error_cache(int clear);
 
 }  // namespace cta

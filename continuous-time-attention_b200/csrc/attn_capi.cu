@@ -1,9 +1,12 @@
 // C ABI of the attention and key/value-cache operators: argument checks, the
 // choice of kernel, launches.  Declarations and contracts live in
 // include/cta_stencil.h.
-#include <cstring>
+#include <cudaTypedefs.h>
 
-#include "attn.h"
+#include <cstring>
+#include <mutex>
+
+#include "attn_tc.cuh"
 #include "cta_stencil.h"
 
 namespace cta {
@@ -11,6 +14,44 @@ void set_last_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 }
 
 using namespace cta;
+
+namespace {
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+}  // namespace
+
+bool cta::attn_map(CUtensorMap* m, const void* base, int dtype, int64_t nb, int64_t tokens, int64_t heads, int64_t d,
+                   const AttnStrides& s, int box_heads, int box_tokens) {
+  const auto fn = encode_fn();
+  if (fn == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0 || d % 8 != 0) return false;
+  // the stride of an axis of one entry means nothing: any valid one
+  const int64_t row = 2 * d;
+  const int64_t st[3] = {heads == 1 ? row : 2 * s.h, tokens == 1 ? row : 2 * s.t, nb == 1 ? row : 2 * s.b};
+  for (int64_t x : st)
+    if (x <= 0 || x % 16 != 0 || x >= (1LL << 40)) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(nb)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(st[0]), static_cast<cuuint64_t>(st[1]),
+                                 static_cast<cuuint64_t>(st[2])};
+  const cuuint32_t box[4] = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens), 1u};
+  const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+  return fn(m, dtype == CTA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 namespace {
 
@@ -213,7 +254,10 @@ int cta_attention_forward(const cta_attention_args* args, void* stream) {
   AttnArgs a;
   const int rc = prompt_args(args, a);
   if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
-  return launched(launch_attn_simt_fwd(a, args->dtype, static_cast<cudaStream_t>(stream)), "attention forward launch");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (!launch_attn_tc_fwd(a, args->dtype, st, &e)) e = launch_attn_simt_fwd(a, args->dtype, st);
+  return launched(e, "attention forward launch");
 }
 
 int cta_attention_backward(const cta_attention_args* args, void* stream) {
@@ -277,14 +321,19 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
     if (s % cells != 0) return fail(CTA_EINVAL, "the cache's rows must start on 16 bytes");
   for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // more rows than one operand of the split kernel holds: the tensor-core kernel
+  cudaError_t e = cudaSuccess;
+  if (!args->quantized && static_cast<int64_t>(a.max_rows) * (a.H / a.Hk) > 16 &&
+      launch_paged_tc(a, args->dtype, st, &e))
+    return launched(e, "paged attention launch");
   a.workers = paged_split_workers(a, args->dtype, args->quantized);
   if (workspace == nullptr || workspace_bytes < split_bytes(a.workers, a.d))
     return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)split_bytes(a.workers, a.d),
                 (long long)workspace_bytes);
   a.part_ml = static_cast<float*>(workspace);
   a.part_o = a.part_ml + 2LL * a.workers * 16 * 4;
-  return launched(launch_paged_split(a, args->dtype, args->quantized, static_cast<cudaStream_t>(stream)),
-                  "paged attention launch");
+  return launched(launch_paged_split(a, args->dtype, args->quantized, st), "paged attention launch");
 }
 
 }  // extern "C"

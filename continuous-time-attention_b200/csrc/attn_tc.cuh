@@ -1,0 +1,153 @@
+// tcgen05 building blocks of the attention kernels: tensor memory, matrix
+// descriptors, 4-D TMA boxes, bounded barrier waits.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace cta {
+namespace tc {
+
+__device__ __forceinline__ void alloc(uint32_t* dst, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void dealloc(uint32_t addr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// the barrier completes one arrival when all MMAs issued so far by this thread are done
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+
+// 32 columns of this warp's 32 tensor-memory lanes, one lane per thread
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Shared-memory operand with the 128-byte swizzle: rows of 128 bytes (64 16-bit
+// elements), groups of 8 rows 1024 bytes apart.
+//   K-major (the contraction index runs along the 128 bytes): the 1024 is the
+//     stride offset, the leading offset is unused;
+//   MN-major (the contraction index counts rows): the 1024 separates groups of 8
+//     rows along the contraction, the leading offset separates the 64-element
+//     blocks of the other index.
+__device__ __forceinline__ uint64_t desc_base(uint32_t lead_bytes) {
+  return (static_cast<uint64_t>((lead_bytes >> 4) & 0x3fff) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc(uint64_t base, uint32_t addr) {
+  return base | static_cast<uint64_t>((addr & 0x3ffff) >> 4);
+}
+
+// kind::f16 instruction descriptor: fp32 accumulator, A and B of type T, M = 128
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn_major, bool a_mn_major = false) {
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (static_cast<uint32_t>(a_mn_major) << 15) |
+         (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+
+// C[128 x N] (+)= A[128 x DP] B[N x DP]^T, both K-major in shared memory; the
+// 64-column halves of A and B lie a_half and b_half bytes apart.  One thread.
+template <int DP>
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t a_half, uint32_t b, uint32_t b_half,
+                                           uint32_t id, bool accumulate = false) {
+  const uint64_t base = desc_base(16);
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k) {
+    const uint32_t off = (k & 3) * 32;
+    mma_ss(d, desc(base, a + (k >> 2) * a_half + off), desc(base, b + (k >> 2) * b_half + off), id,
+           accumulate || k > 0);
+  }
+}
+// C[128 x N] (+)= A[tmem, 128 x KEYS] B[KEYS x N], B MN-major (rows are the
+// contraction index), its 64-column blocks b_half bytes apart.  One thread.
+template <int KEYS>
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t b_half, uint32_t id,
+                                           bool accumulate) {
+  const uint64_t base = desc_base(b_half);
+#pragma unroll
+  for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, a + 8 * k, desc(base, b + k * 2048), id, accumulate || k > 0);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const typename Elem<T>::Pair p = Elem<T>::pack(make_float2(lo, hi));
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+}  // namespace tc
+
+// Host: a 4-D map over a [batch, token, head, dim] tensor of 16-bit elements with
+// a box of 64 x box_heads x box_tokens x 1.  False when TMA cannot address it.
+bool attn_map(CUtensorMap* m, const void* base, int dtype, int64_t nb, int64_t tokens, int64_t heads, int64_t d,
+              const AttnStrides& s, int box_heads, int box_tokens);
+
+}  // namespace cta

@@ -335,8 +335,10 @@ int cta_device_error(int clear) {
   const int d = read_device_error_bld_dalpha(clear);
   const int p = read_device_error_paged(clear);
   const int k = read_device_error_cache(clear);
-  if (a < 0 || c < 0 || d < 0 || p < 0 || k < 0) return -1;
-  for (int e : {a, c, d, p, k})
+  const int f = read_device_error_tc_fwd(clear);
+  for (int e : {a, c, d, p, k, f})
+    if (e < 0) return -1;
+  for (int e : {a, c, d, p, k, f})
     if (e != 0) return e;
   return 0;
 }
