@@ -106,10 +106,13 @@ cudaError_t launch_paged_split(const PagedArgs& a, int dtype, int quantized, cud
 
 // tensor-core forms; false = not for these types, sizes or strides (nothing was launched)
 bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
+bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
+int attn_pack(int group);  // heads of a group that one row tile holds: its largest power of two
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
 
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);
+int read_device_error_tc_bwd(int clear);
 int read_device_error_cache(int clear);
 
 }  // namespace cta

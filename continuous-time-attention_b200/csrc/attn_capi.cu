@@ -268,9 +268,9 @@ int cta_attention_backward(const cta_attention_args* args, void* stream) {
     return fail(CTA_EINVAL, "the backward needs grad_out, lse and the delta scratch");
   if ((a.dk == nullptr) != (a.dv == nullptr)) return fail(CTA_EINVAL, "dk and dv come together");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = launch_attn_delta(a, args->dtype, st);
-  if (e != cudaSuccess) return launched(e, "attention backward launch");
-  return launched(launch_attn_simt_bwd(a, args->dtype, st), "attention backward launch");
+  cudaError_t e = launch_attn_delta(a, args->dtype, st);
+  if (e == cudaSuccess && !launch_attn_tc_bwd(a, args->dtype, st, &e)) e = launch_attn_simt_bwd(a, args->dtype, st);
+  return launched(e, "attention backward launch");
 }
 
 int cta_kv_cache_write(const cta_kv_cache_args* args, void* stream) {

@@ -110,14 +110,42 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t a_ha
            accumulate || k > 0);
   }
 }
-// C[128 x N] (+)= A[tmem, 128 x KEYS] B[KEYS x N], B MN-major (rows are the
-// contraction index), its 64-column blocks b_half bytes apart.  One thread.
-template <int KEYS>
+// C[128 x N] (+)= A[tmem, 128 x 128] B[128 x N], B MN-major (rows are the
+// contraction index), its 64-column blocks b_half bytes apart.  The second half
+// of A's contraction index starts HALF tensor-memory columns after the first
+// (32 when A is dense).  One thread.
+template <int HALF = 32>
 __device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t b_half, uint32_t id,
                                            bool accumulate) {
   const uint64_t base = desc_base(b_half);
 #pragma unroll
-  for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, a + 8 * k, desc(base, b + k * 2048), id, accumulate || k > 0);
+  for (int k = 0; k < 8; ++k)
+    mma_ts(d, a + 8 * (k & 3) + HALF * (k >> 2), desc(base, b + k * 2048), id, accumulate || k > 0);
+}
+
+// zero the 128-byte rows of a 128-row tile (HALVES blocks of 64 columns, 16 KB
+// apart) whose bit in w is clear, before an MMA reads them: what lies there may
+// be NaN, and a zero weight times NaN is NaN.  Whole warp.
+template <int HALVES>
+__device__ __forceinline__ void clear_rows(uint32_t tile, const uint32_t (&w)[4]) {
+  const int lane = threadIdx.x & 31;
+  for (int r = lane >> 3; r < 128; r += 4)
+    if (!((w[r >> 5] >> (r & 31)) & 1u))
+#pragma unroll
+      for (int c = 0; c < HALVES; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * 16384 + r * 128 + (lane & 7) * 16), "r"(0u)
+                     : "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+__device__ __forceinline__ bool all_set(const uint32_t (&w)[4]) { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
+// bit c of word i: c + 32 i < count
+__device__ __forceinline__ void first_bits(int count, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int left = count - 32 * i;
+    w[i] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  }
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,

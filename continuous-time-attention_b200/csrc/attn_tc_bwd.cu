@@ -1,0 +1,676 @@
+// Attention backward on the tensor cores, 16-bit tensors.
+//
+//   P = exp(c Q K^T - lse),  dS = P o (dO V^T - delta)
+//   dQ = c dS K,   dK = c dS^T Q,   dV = P^T dO
+//
+// Two kernels, one that owns 128 query rows (dQ) and one that owns 128 keys (dK,
+// dV).  Both recompute the scores, so seven products of a tile pair are done
+// where five would do; in exchange every gradient has one owner that sums in
+// tensor memory in a fixed order: no atomics, no fp32 scratch for dQ, results
+// that do not depend on timing, and the heads that share keys are summed in
+// place.  Rows are (token, head) pairs as in the forward.
+//
+//   warps 0-7  weights: two warpgroups take 64 columns each of a 128 x 128 tile
+//   warp 8     MMAs      warp 9  TMA loads      warp 10  lse and delta (keys' kernel)
+//
+// Weights and score gradients go back to tensor memory as 16-bit A operands over
+// the columns their fp32 sources came from, so a tile pair crosses shared memory
+// only as Q, K, V and dO.  The MMA warp keeps the pipe busy across the two
+// dependent halves of a step: the next scores run while dS is computed, the
+// next dO V^T while the next P is.
+//
+// Bound by the products at dim 128 (7 x 512 cycles per tile pair against 2 x
+// 1024 of exponentials), by the exponentials at dim 64.
+#include <algorithm>
+
+#include "attn_tc.cuh"
+
+namespace cta {
+
+__device__ int g_tc_bwd_error;
+
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kRows = 128;
+
+struct BwdArgs {
+  AttnArgs a;
+  int pack, tile_tokens;
+  int vec_dq, vec_dk, vec_dv;  // rows of the gradient are on 16 bytes
+};
+
+template <int DP>
+struct Layout {
+  static constexpr int kHalf = kRows * 128;
+  static constexpr int kTile = kHalf * (DP / 64);
+  static constexpr int kStages = 4;  // tiles of the other side in flight
+  static constexpr int kSmem = (2 + kStages) * kTile + 1024;
+};
+
+// a 128-row tile of gradients from tensor memory; one thread per row
+template <typename T, int DP>
+__device__ __forceinline__ void store_grad(uint32_t addr, T* out, int d, float mul, bool live, bool vec, bool any) {
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c) {
+    uint32_t o[32];
+    if (any) {
+      tc::ld32(addr + 32 * c, o);
+      tc::wait_ld();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0u;
+    }
+    if (!live) continue;
+    if (vec) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8)
+        if (32 * c + e < d) {
+          uint4 x;
+          uint32_t* xp = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            xp[y] = tc::pack2<T>(__uint_as_float(o[e + 2 * y]) * mul, __uint_as_float(o[e + 2 * y + 1]) * mul);
+          *reinterpret_cast<uint4*>(out + 32 * c + e) = x;
+        }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (32 * c + e < d) out[32 * c + e] = Elem<T>::from_f(__uint_as_float(o[e]) * mul);
+    }
+  }
+}
+
+// the row's share of the sums: a row that sees no key, or lies outside, has weight zero everywhere
+__device__ __forceinline__ bool blind(float neg_lse2) { return neg_lse2 == neg_inf(); }
+__device__ __forceinline__ float neg_lse2_of(float lse) { return lse == neg_inf() ? neg_inf() : -lse * kLog2e; }
+
+// ---------------------------------------------------------------------------
+// dQ
+// ---------------------------------------------------------------------------
+struct DqBars {
+  uint64_t q_full, kv_full[4], kv_empty[4], s_full[2], dp_full, dp_read, ds_full, done;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_dq_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
+                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ BwdArgs f) {
+  using L = Layout<DP>;
+  constexpr int NS = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ DqBars bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ SeqTile s_tile;
+  const AttnArgs& a = f.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int blocks = a.H / f.pack;
+  const int h0 = static_cast<int>(blockIdx.x % blocks) * f.pack, hk = h0 / (a.H / a.Hk);
+
+  if (warp == 0) {
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal);
+    if (lane == 0) s_tile = x;
+  } else if (warp == 8) {
+    tc::alloc(&s_tmem, 512);
+  } else if (warp == 9 && lane == 0) {
+    mbar_init(&bars.q_full, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&bars.kv_full[i], 1);
+      mbar_init(&bars.kv_empty[i], 1);
+    }
+    mbar_init(&bars.s_full[0], 1);
+    mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.dp_read, 256);
+    mbar_init(&bars.ds_full, 256);
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const SeqTile t = s_tile;
+  const uint32_t tmem = s_tmem;
+  const uint32_t t_dp = tmem + 256, t_dq = tmem + 384;  // scores: columns 0 and 128
+
+  int lo = 0, hi = t.n;
+  mask_range(a, t.batch, t.n, lo, hi);
+  const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
+  const int j_lo = lo / kRows;
+  int end = hi;
+  if (a.causal) end = min(end, t.first + f.tile_tokens);
+  const int steps = t.first < t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
+
+  auto key_words = [&](int j, uint32_t (&w)[4]) {
+    const int j0 = (j_lo + j) * kRows;
+    tc::first_bits(t.n - j0, w);
+    if (mask != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (w[i] != 0u) w[i] &= __ldg(mask + kMaskHead + (j0 >> 5) + i);
+    }
+  };
+
+  if (warp == 9) {
+    bool ok = true;
+    int issued = 0;
+    if (steps > 0 && lane == 0) {
+      mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
+      for (int c = 0; c < DP / 64; ++c) {
+        tc::tma_load_4d(smem + c * L::kHalf, &qmap, &bars.q_full, 64 * c, h0, static_cast<int>(t.row0) + t.first,
+                        t.batch);
+        tc::tma_load_4d(smem + L::kTile + c * L::kHalf, &gmap, &bars.q_full, 64 * c, h0,
+                        static_cast<int>(t.row0) + t.first, t.batch);
+      }
+    }
+    for (int x = 0; x < 2 * steps; ++x) {
+      const int stage = x % NS;
+      if (x >= NS) ok = mbar_wait_bounded(&bars.kv_empty[stage], ((x / NS) - 1) & 1);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
+        for (int c = 0; c < DP / 64; ++c)
+          tc::tma_load_4d(smem + (2 + stage) * L::kTile + c * L::kHalf, (x & 1) ? &vmap : &kmap, &bars.kv_full[stage],
+                          64 * c, hk, static_cast<int>(t.row0) + (j_lo + (x >> 1)) * kRows, t.batch);
+      }
+      issued = x + 1;
+    }
+    if (!ok) {
+      atomicExch(&g_tc_bwd_error, kDevTimeout);
+      for (int x = max(0, issued - NS); x < issued; ++x) mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1);
+    }
+  } else if (warp == 8) {
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
+    const bool leader = tc::elect_one();
+    bool ok = steps == 0 || mbar_wait_bounded(&bars.q_full, 0);
+    auto kv_wait = [&](int x) {
+      ok = ok && mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1);
+      tc::fence_after();
+    };
+    auto kv_addr = [&](int x) { return smem + (2 + x % NS) * L::kTile; };
+    auto scores = [&](int j) {
+      kv_wait(2 * j);
+      uint32_t w[4];
+      key_words(j, w);
+      if (ok && !tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j), w);
+      if (ok && leader) {
+        tc::product_nt<DP>(tmem + (j & 1) * 128, smem, L::kHalf, kv_addr(2 * j), L::kHalf, id_s);
+        tc::commit(&bars.s_full[j & 1]);
+      }
+      __syncwarp();
+    };
+    auto grads = [&](int j) {
+      kv_wait(2 * j + 1);
+      if (ok && leader) {
+        tc::product_nt<DP>(t_dp, smem + L::kTile, L::kHalf, kv_addr(2 * j + 1), L::kHalf, id_s);
+        tc::commit(&bars.dp_full);
+        tc::commit(&bars.kv_empty[(2 * j + 1) % NS]);
+      }
+      __syncwarp();
+    };
+    if (steps > 0 && ok) {
+      scores(0);
+      if (ok) grads(0);
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      if (j + 1 < steps) {
+        scores(j + 1);
+        ok = ok && mbar_wait_bounded(&bars.dp_read, j & 1);
+        tc::fence_after();
+        if (ok) grads(j + 1);
+      }
+      ok = ok && mbar_wait_bounded(&bars.ds_full, j & 1);
+      tc::fence_after();
+      if (ok && leader) {
+        tc::product_tn<64>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), L::kHalf, id_o, j > 0);
+        tc::commit(&bars.kv_empty[(2 * j) % NS]);
+        if (j + 1 == steps) tc::commit(&bars.done);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+  } else if (warp < 8) {
+    const int half = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int tok = t.first + row / f.pack, h = h0 + row % f.pack;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const bool live = tok < t.n;
+    const float c2 = a.scale * kLog2e;
+    const float nl = live ? neg_lse2_of(a.lse[lse_index(a, t, h, tok)]) : neg_inf();
+    const float delta = live ? a.delta[lse_index(a, t, h, tok)] : 0.f;
+    const bool none = blind(nl);
+    const int limit = a.causal ? tok : t.n - 1;
+    bool ok = true;
+    for (int j = 0; j < steps && ok; ++j) {
+      const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + half * 64;
+      ok = mbar_wait_bounded(&bars.s_full[j & 1], (j >> 1) & 1);
+      if (!ok) break;
+      tc::fence_after();
+      uint32_t s[2][32], dp[2][32];
+      tc::ld32(s_addr, s[0]);
+      tc::ld32(s_addr + 32, s[1]);
+      tc::wait_ld();
+      const int j0 = (j_lo + j) * kRows + half * 64;
+      uint32_t w[4];
+      key_words(j, w);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float2 x = fma2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), f2(c2), f2(nl));
+          s[c][e] = __float_as_uint(ex2(x.x));
+          s[c][e + 1] = __float_as_uint(ex2(x.y));
+        }
+      ok = mbar_wait_bounded(&bars.dp_full, j & 1);
+      if (!ok) break;
+      tc::fence_after();
+      tc::ld32(t_dp + lanes + half * 64, dp[0]);
+      tc::ld32(t_dp + lanes + half * 64 + 32, dp[1]);
+      tc::wait_ld();
+      tc::fence_before();
+      tc::arrive(&bars.dp_read);
+      const bool whole = tc::all_set(w) && !none && (!a.causal || j0 + 63 <= t.first + (warp & 3) * 32 / f.pack);
+      // whole is uniform but for `none`
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t ds[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = mul2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
+                                add2(make_float2(__uint_as_float(dp[c][e]), __uint_as_float(dp[c][e + 1])), f2(-delta)));
+          dp[c][e] = __float_as_uint(x.x);
+          dp[c][e + 1] = __float_as_uint(x.y);
+        }
+        if (!whole) {
+          const int left = none ? 0 : limit - j0 - 32 * c + 1;
+          const uint32_t see = (half == 0 ? w[c] : w[2 + c]) &
+                               (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((see >> e) & 1u)) dp[c][e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          ds[e] = tc::pack2<T>(__uint_as_float(dp[c][2 * e]), __uint_as_float(dp[c][2 * e + 1]));
+        tc::st16(s_addr + 16 * c, ds);
+      }
+      tc::wait_st();
+      tc::fence_before();
+      tc::arrive(&bars.ds_full);
+    }
+    if (ok && steps > 0) ok = mbar_wait_bounded(&bars.done, 0);
+    tc::fence_after();
+    if (!ok) {
+      if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+    } else if (t.first < t.n) {
+      if (half == 0) {
+        T* out = static_cast<T*>(a.dq) + t.batch * a.dqs.b + (t.row0 + tok) * a.dqs.t + h * a.dqs.h;
+        store_grad<T, DP>(t_dq + lanes, out, a.d, a.scale, live, f.vec_dq, steps > 0);
+      }
+    } else if (a.cu != nullptr && t.n == 0 && half == 0) {
+      for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
+        for (int x = threadIdx.x; x < a.d * f.pack; x += kRows)
+          static_cast<T*>(a.dq)[r * a.dqs.t + (h0 + x / a.d) * a.dqs.h + x % a.d] = Elem<T>::from_f(0.f);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV: the tiles are transposed, rows are keys and columns are query rows
+// ---------------------------------------------------------------------------
+struct DkvBars {
+  uint64_t kv_full, q_full[2], q_empty[2], stat_full[2], s_full, p_full, dp_full, ds_full, done;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
+                       const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const __grid_constant__ BwdArgs f) {
+  using L = Layout<DP>;
+  constexpr int NS = L::kStages / 2;  // (Q, dO) pairs in flight
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ DkvBars bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ SeqTile s_tile;
+  __shared__ __align__(16) float s_stat[2][2][kRows];  // [stage][-lse2, -delta][row]
+  const AttnArgs& a = f.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
+
+  if (warp == 0) {
+    // the first keys of a causal sequence meet the most rows: forwards is heaviest first
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false);
+    if (lane == 0) s_tile = x;
+  } else if (warp == 8) {
+    tc::alloc(&s_tmem, 512);
+  } else if (warp == 9 && lane == 0) {
+    mbar_init(&bars.kv_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.q_full[i], 1);
+      mbar_init(&bars.q_empty[i], 1);
+      mbar_init(&bars.stat_full[i], 32);
+    }
+    mbar_init(&bars.s_full, 1);
+    mbar_init(&bars.p_full, 256);
+    mbar_init(&bars.dp_full, 1);
+    mbar_init(&bars.ds_full, 256);
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const SeqTile t = s_tile;
+  const uint32_t tmem = s_tmem;
+  const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+
+  const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
+  int lo, hi;
+  mask_range(a, t.batch, t.n, lo, hi);
+  // row tiles that meet these keys, for each block of heads of the group
+  const int i_lo = a.causal ? t.first / f.tile_tokens : 0;
+  const int per_head = max(0, (t.n + f.tile_tokens - 1) / f.tile_tokens - i_lo);
+  const bool some = t.first < min(t.n, hi) && t.first + kRows > lo;  // any valid key
+  const int steps = some ? per_head * (group / f.pack) : 0;
+  auto head_of = [&](int s) { return hk * group + s / per_head * f.pack; };
+  auto first_of = [&](int s) { return (i_lo + s % per_head) * f.tile_tokens; };
+
+  if (warp == 9) {
+    bool ok = true;
+    int issued = 0;
+    if (steps > 0 && lane == 0) {
+      mbar_arrive_expect_tx(&bars.kv_full, 2 * L::kTile);
+      for (int c = 0; c < DP / 64; ++c) {
+        tc::tma_load_4d(smem + c * L::kHalf, &kmap, &bars.kv_full, 64 * c, hk, static_cast<int>(t.row0) + t.first,
+                        t.batch);
+        tc::tma_load_4d(smem + L::kTile + c * L::kHalf, &vmap, &bars.kv_full, 64 * c, hk,
+                        static_cast<int>(t.row0) + t.first, t.batch);
+      }
+    }
+    for (int s = 0; s < steps; ++s) {
+      const int stage = s % NS;
+      if (s >= NS) ok = mbar_wait_bounded(&bars.q_empty[stage], ((s / NS) - 1) & 1);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars.q_full[stage], 2 * L::kTile);
+        const int row = static_cast<int>(t.row0) + first_of(s);
+        for (int c = 0; c < DP / 64; ++c) {
+          tc::tma_load_4d(smem + (2 + 2 * stage) * L::kTile + c * L::kHalf, &qmap, &bars.q_full[stage], 64 * c,
+                          head_of(s), row, t.batch);
+          tc::tma_load_4d(smem + (3 + 2 * stage) * L::kTile + c * L::kHalf, &gmap, &bars.q_full[stage], 64 * c,
+                          head_of(s), row, t.batch);
+        }
+      }
+      issued = s + 1;
+    }
+    if (!ok) {
+      atomicExch(&g_tc_bwd_error, kDevTimeout);
+      for (int s = max(0, issued - NS); s < issued; ++s) mbar_wait_bounded(&bars.q_full[s % NS], (s / NS) & 1);
+    }
+  } else if (warp == 10) {
+    bool ok = true;
+    for (int s = 0; s < steps; ++s) {
+      const int stage = s % NS;
+      float nl[4], dl[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = lane + 32 * i;
+        const int tok = first_of(s) + r / f.pack, h = head_of(s) + r % f.pack;
+        nl[i] = tok < t.n ? neg_lse2_of(__ldg(a.lse + lse_index(a, t, h, tok))) : neg_inf();
+        dl[i] = tok < t.n ? -__ldg(a.delta + lse_index(a, t, h, tok)) : 0.f;
+        if (blind(nl[i])) dl[i] = 0.f;
+      }
+      if (s >= NS) ok = mbar_wait_bounded(&bars.q_empty[stage], ((s / NS) - 1) & 1);
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s_stat[stage][0][lane + 32 * i] = nl[i];
+        s_stat[stage][1][lane + 32 * i] = dl[i];
+      }
+      tc::arrive(&bars.stat_full[stage]);
+    }
+  } else if (warp == 8) {
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
+    const bool leader = tc::elect_one();
+    bool ok = steps == 0 || mbar_wait_bounded(&bars.kv_full, 0);
+    auto q_addr = [&](int s) { return smem + (2 + 2 * (s % NS)) * L::kTile; };
+    auto scores = [&](int s) {
+      ok = ok && mbar_wait_bounded(&bars.q_full[s % NS], (s / NS) & 1);
+      tc::fence_after();
+      // packed: rows of the next sequence in a tile that reaches past this one
+      const int rows = (t.n - first_of(s)) * f.pack;
+      if (ok && rows < kRows) {
+        uint32_t w[4];
+        tc::first_bits(rows, w);
+        tc::clear_rows<DP / 64>(q_addr(s), w);
+        tc::clear_rows<DP / 64>(q_addr(s) + L::kTile, w);
+      }
+      if (ok && leader) {
+        tc::product_nt<DP>(tmem, smem, L::kHalf, q_addr(s), L::kHalf, id_s);
+        tc::commit(&bars.s_full);
+      }
+      __syncwarp();
+    };
+    auto grads = [&](int s) {
+      if (ok && leader) {
+        tc::product_nt<DP>(t_dp, smem + L::kTile, L::kHalf, q_addr(s) + L::kTile, L::kHalf, id_s);
+        tc::commit(&bars.dp_full);
+      }
+      __syncwarp();
+    };
+    if (steps > 0) {
+      scores(0);
+      grads(0);
+    }
+    for (int s = 0; s < steps && ok; ++s) {
+      ok = mbar_wait_bounded(&bars.p_full, s & 1);
+      tc::fence_after();
+      if (ok && leader) tc::product_tn<64>(t_dv, tmem, q_addr(s) + L::kTile, L::kHalf, id_o, s > 0);
+      __syncwarp();
+      if (s + 1 < steps) scores(s + 1);
+      ok = ok && mbar_wait_bounded(&bars.ds_full, s & 1);
+      tc::fence_after();
+      if (ok && leader) {
+        tc::product_tn<64>(t_dk, t_dp, q_addr(s), L::kHalf, id_o, s > 0);
+        tc::commit(&bars.q_empty[s % NS]);
+        if (s + 1 == steps) tc::commit(&bars.done);
+      }
+      __syncwarp();
+      if (s + 1 < steps) grads(s + 1);
+    }
+    if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+  } else if (warp < 8) {
+    const int half = warp >> 2;
+    const int key = t.first + (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const bool valid = key < t.n && (mask == nullptr || mask_key(mask, key));
+    const float c2 = a.scale * kLog2e;
+    bool ok = true;
+    for (int s = 0; s < steps && ok; ++s) {
+      const int stage = s % NS;
+      const uint32_t s_addr = tmem + lanes + half * 64, d_addr = t_dp + lanes + half * 64;
+      ok = mbar_wait_bounded(&bars.stat_full[stage], (s / NS) & 1) && mbar_wait_bounded(&bars.s_full, s & 1);
+      if (!ok) break;
+      tc::fence_after();
+      uint32_t p[2][32];
+      tc::ld32(s_addr, p[0]);
+      tc::ld32(s_addr + 32, p[1]);
+      tc::wait_ld();
+      // causal: the first row of this half that sees the key; 64 = none
+      int from = 0;
+      if (a.causal) from = min(max((key - first_of(s)) * f.pack - half * 64, 0), 64);
+      if (!valid) from = 64;
+      const float4* nl = reinterpret_cast<const float4*>(&s_stat[stage][0][half * 64]);
+      const float4* dl = reinterpret_cast<const float4*>(&s_stat[stage][1][half * 64]);
+      const bool masked = __any_sync(0xffffffffu, from > 0);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 b = nl[(32 * c + e) / 4];
+          float2 x = fma2(make_float2(__uint_as_float(p[c][e]), __uint_as_float(p[c][e + 1])), f2(c2), make_float2(b.x, b.y));
+          float2 y = fma2(make_float2(__uint_as_float(p[c][e + 2]), __uint_as_float(p[c][e + 3])), f2(c2), make_float2(b.z, b.w));
+          p[c][e] = __float_as_uint(ex2(x.x));
+          p[c][e + 1] = __float_as_uint(ex2(x.y));
+          p[c][e + 2] = __float_as_uint(ex2(y.x));
+          p[c][e + 3] = __float_as_uint(ex2(y.y));
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e < from) p[c][e] = 0u;
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = tc::pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
+        tc::st16(s_addr + 16 * c, w);
+      }
+      tc::wait_st();
+      tc::fence_before();
+      tc::arrive(&bars.p_full);
+
+      ok = mbar_wait_bounded(&bars.dp_full, s & 1);
+      if (!ok) break;
+      tc::fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t d[32], w[16];
+        tc::ld32(d_addr + 32 * c, d);
+        tc::wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 b = dl[(32 * c + e) / 4];
+          const float2 x = mul2(make_float2(__uint_as_float(p[c][e]), __uint_as_float(p[c][e + 1])),
+                                add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), make_float2(b.x, b.y)));
+          const float2 y = mul2(make_float2(__uint_as_float(p[c][e + 2]), __uint_as_float(p[c][e + 3])),
+                                add2(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), make_float2(b.z, b.w)));
+          w[e / 2] = tc::pack2<T>(x.x, x.y);
+          w[e / 2 + 1] = tc::pack2<T>(y.x, y.y);
+        }
+        if (masked) {
+          // dO V^T of a key that is not there may be NaN
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (32 * c + 2 * e < from) w[e] &= 0xffff0000u;
+            if (32 * c + 2 * e + 1 < from) w[e] &= 0x0000ffffu;
+          }
+        }
+        // over columns 0-15 (16-31) of this half's 64, both already read when c = 0
+        if (c == 0) {
+          tc::st16(d_addr, w);
+        } else {
+          tc::st16(d_addr + 16, w);
+        }
+      }
+      tc::wait_st();
+      tc::fence_before();
+      tc::arrive(&bars.ds_full);
+    }
+    if (ok && steps > 0) ok = mbar_wait_bounded(&bars.done, 0);
+    tc::fence_after();
+    if (!ok) {
+      if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+    } else if (t.first < t.n) {
+      const bool live = key < t.n;
+      if (half == 0) {
+        T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
+        store_grad<T, DP>(t_dv + lanes, out, a.d, 1.f, live, f.vec_dv, steps > 0);
+      } else {
+        T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
+        store_grad<T, DP>(t_dk + lanes, out, a.d, a.scale, live, f.vec_dk, steps > 0);
+      }
+    } else if (a.cu != nullptr && t.n == 0) {
+      T* base = static_cast<T*>(half == 0 ? a.dv : a.dk) + hk * (half == 0 ? a.dvs.h : a.dks.h);
+      const int64_t st = half == 0 ? a.dvs.t : a.dks.t;
+      for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
+        for (int x = threadIdx.x & 127; x < a.d; x += kRows) base[r * st + x] = Elem<T>::from_f(0.f);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == 8) tc::dealloc(tmem, 512);
+}
+
+bool on16(const void* p, const AttnStrides& s, int64_t nb, int64_t heads) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s.t % 8 == 0 && (heads == 1 || s.h % 8 == 0) &&
+         (nb == 1 || s.b % 8 == 0);
+}
+
+int64_t count_tiles(AttnArgs& a, int rows) {
+  if (a.cu != nullptr) {
+    a.tiles = static_cast<int>(packed_tiles(a.L, a.nseq, rows));
+    return a.tiles;
+  }
+  a.tiles = static_cast<int>((a.L + rows - 1) / rows);
+  return static_cast<int64_t>(a.tiles) * a.nseq;
+}
+
+template <typename K>
+cudaError_t launch(K kernel, int smem, int64_t ctas, const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k,
+                   const CUtensorMap& v, const BwdArgs& f, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(q, g, k, v, f);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP>
+cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k, const CUtensorMap& v, BwdArgs f,
+                cudaStream_t st) {
+  if (f.a.dk != nullptr) {
+    const int64_t tiles = count_tiles(f.a, kRows);
+    const cudaError_t e =
+        launch(attn_tc_dkv_kernel<T, DP>, Layout<DP>::kSmem, tiles * f.a.Hk, q, g, k, v, f, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (f.a.dq == nullptr) return cudaSuccess;
+  const int64_t tiles = count_tiles(f.a, f.tile_tokens);
+  return launch(attn_tc_dq_kernel<T, DP>, Layout<DP>::kSmem, tiles * (f.a.H / f.pack), q, g, k, v, f, st);
+}
+
+}  // namespace
+
+bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e) {
+  if (dtype == kF32 || a.d % 8 != 0 || a.d > 128 || !(a.scale > 0.f)) return false;
+  BwdArgs f = {};
+  f.a = a;
+  f.pack = attn_pack(a.H / a.Hk);
+  f.tile_tokens = kRows / f.pack;
+  const int64_t nb = a.cu != nullptr ? 1 : a.nseq;
+  CUtensorMap q, g, k, v;
+  if (!attn_map(&q, a.q, dtype, nb, a.L, a.H, a.d, a.qs, f.pack, f.tile_tokens) ||
+      !attn_map(&g, a.g, dtype, nb, a.L, a.H, a.d, a.gs, f.pack, f.tile_tokens) ||
+      !attn_map(&k, a.k, dtype, nb, a.L, a.Hk, a.d, a.ks, 1, kRows) ||
+      !attn_map(&v, a.v, dtype, nb, a.L, a.Hk, a.d, a.vs, 1, kRows))
+    return false;
+  f.vec_dq = a.dq != nullptr && on16(a.dq, a.dqs, nb, a.H);
+  f.vec_dk = a.dk != nullptr && on16(a.dk, a.dks, nb, a.Hk);
+  f.vec_dv = a.dv != nullptr && on16(a.dv, a.dvs, nb, a.Hk);
+  if (dtype == kBF16)
+    *e = a.d <= 64 ? run<__nv_bfloat16, 64>(q, g, k, v, f, st) : run<__nv_bfloat16, 128>(q, g, k, v, f, st);
+  else
+    *e = a.d <= 64 ? run<__half, 64>(q, g, k, v, f, st) : run<__half, 128>(q, g, k, v, f, st);
+  return true;
+}
+
+int read_device_error_tc_bwd(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tc_bwd_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v != 0) {
+    const int z = 0;
+    cudaMemcpyToSymbol(g_tc_bwd_error, &z, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace cta

@@ -19,8 +19,9 @@
 // not per tile; P stays below 2^8, the sum and O are fp32, and the quotient is
 // exact in which reference was used.
 //
-// Bound by the exponentials: 128 x 128 of them per tile take 1024 cycles of the
-// SM's 16-per-cycle unit against 512 cycles of MMA at dim 128.
+// Bound by the exponentials and the products alike: 128 x 128 exponentials take
+// 1024 cycles of the SM's 16-per-cycle unit, the two products of a tile 1024
+// cycles at dim 128 (512 at dim 64).
 #include <algorithm>
 
 #include "attn_tc.cuh"
@@ -134,11 +135,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // bit c of word w: key 32 w + c of tile j is one of the sequence's and valid
   auto key_words = [&](int j, uint32_t (&w)[4]) {
     const int j0 = (j_lo + j) * kRows;
+    tc::first_bits(n - j0, w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int left = n - j0 - 32 * i;
-      w[i] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-      if (mask != nullptr && left > 0) w[i] &= __ldg(mask + kMaskHead + (j0 >> 5) + i);
+      if (mask != nullptr && n - j0 - 32 * i > 0) w[i] &= __ldg(mask + kMaskHead + (j0 >> 5) + i);
       if constexpr (PAGED) {
         const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&s_boxes[j & 15]);
 #pragma unroll
@@ -240,24 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // values of keys that are not there or not valid may hold anything: a zero weight times NaN is NaN
       uint32_t w[4];
       key_words(j, w);
-      if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-        const uint32_t v = kv_addr(2 * j + 1);
-        for (int r = lane >> 3; r < kRows; r += 4)
-          if (!((w[r >> 5] >> (r & 31)) & 1u))
-            for (int c = 0; c < DP / 64; ++c)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + c * L::kHalf + r * 128 + (lane & 7) * 16),
-                           "r"(0u)
-                           : "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
+      if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
       const bool more = j + 1 < all;
       for (int i = 0; i < 2 && ok; ++i) {
         if (j < steps[i]) {
           ok = mbar_wait_bounded(&bars.p_full[i], j & 1);
           tc::fence_after();
           if (ok && leader) {
-            tc::product_tn<kRows>(tmem + 2 * kRows + i * DP, tmem + i * kRows, kv_addr(2 * j + 1), L::kHalf, id_o, j > 0);
+            tc::product_tn(tmem + 2 * kRows + i * DP, tmem + i * kRows, kv_addr(2 * j + 1), L::kHalf, id_o, j > 0);
             if (j + 1 == steps[i]) tc::commit(&bars.o_full[i]);
           }
         }
@@ -299,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t w[4];
       key_words(j, w);
       // warp-uniform: does every row of the warp see all 128 keys?
-      const bool whole = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu &&
+      const bool whole = tc::all_set(w) &&
                          (!a.causal || j0 + kRows - 1 <= first[i] + (warp & 3) * 32 / f.pack + shift);
       if (!whole) {
 #pragma unroll

@@ -336,9 +336,10 @@ int cta_device_error(int clear) {
   const int p = read_device_error_paged(clear);
   const int k = read_device_error_cache(clear);
   const int f = read_device_error_tc_fwd(clear);
-  for (int e : {a, c, d, p, k, f})
+  const int b = read_device_error_tc_bwd(clear);
+  for (int e : {a, c, d, p, k, f, b})
     if (e < 0) return -1;
-  for (int e : {a, c, d, p, k, f})
+  for (int e : {a, c, d, p, k, f, b})
     if (e != 0) return e;
   return 0;
 }
