@@ -2,6 +2,8 @@
 // to, the key mask, base-2 exponentials.
 #pragma once
 
+#include <atomic>
+
 #include "attn.h"
 #include "common.cuh"
 
@@ -103,6 +105,20 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* cu, int nseq, int64_
 // Upper bound on the tiles of a packed row plus one tile that is always behind
 // the last sequence (it clears the rows there when asked to).
 inline int64_t packed_tiles(int64_t L, int nseq, int rows) { return L / rows + nseq + 1; }
+
+// Dynamic shared memory above 48 KB has to be allowed, once per kernel and device.
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};  // one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 // Sets rows behind the last sequence to zero, head h, `d` elements each.
 template <typename T>

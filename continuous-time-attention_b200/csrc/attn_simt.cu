@@ -21,19 +21,67 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kPad = 4;
 
+// VEC consecutive elements as fp32
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[VEC]) {
+  if constexpr (VEC == 1) {
+    x[0] = Elem<T>::to_f(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const float2 a = Elem<T>::unpack(*reinterpret_cast<const typename Elem<T>::Pair*>(&v.x));
+    const float2 b = Elem<T>::unpack(*reinterpret_cast<const typename Elem<T>::Pair*>(&v.y));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+  }
+}
+
 // rows [first, first + ROWS) of a head into shared memory as fp32; rows outside
-// [0, n) and invalid keys are zero, so that no NaN of theirs meets a zero weight
+// [0, n) and invalid keys (clear bits of `valid`, row first + r is bit r) are
+// zero, so that no NaN of theirs meets a zero weight.  BATCH loads in flight.
+template <typename T, int ROWS, int DP, int VEC>
+__device__ __forceinline__ void load_rows_vec(float* dst, const T* p, int64_t stride, int first, int n, int d,
+                                              uint64_t valid) {
+  constexpr int kItems = ROWS * DP / VEC / kThreads, kBatch = kItems < 8 ? kItems : 8;
+#pragma unroll 1
+  for (int i0 = 0; i0 < kItems; i0 += kBatch) {
+    float x[kBatch][VEC];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = (i0 + i) * kThreads + threadIdx.x;
+      const int r = at / (DP / VEC), c = at % (DP / VEC) * VEC, j = first + r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[i][e] = 0.f;
+      if (j < n && c < d && ((valid >> r) & 1u)) load_vec<T, VEC>(p + static_cast<int64_t>(j) * stride + c, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = (i0 + i) * kThreads + threadIdx.x;
+      float* o = dst + at / (DP / VEC) * (DP + kPad) + at % (DP / VEC) * VEC;
+      if constexpr (VEC == 4) *reinterpret_cast<float4*>(o) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+      else o[0] = x[i][0];
+    }
+  }
+}
+
 template <typename T, int ROWS, int DP>
 __device__ __forceinline__ void load_rows(float* dst, const void* base, const AttnStrides& s, const SeqTile& t, int h,
-                                          int first, int n, int d, const uint32_t* mask) {
+                                          int first, int n, int d, uint64_t valid) {
   const T* p = static_cast<const T*>(base) + t.batch * s.b + t.row0 * s.t + h * s.h;
-  for (int i = threadIdx.x; i < ROWS * DP; i += kThreads) {
-    const int r = i / DP, c = i - r * DP;
-    const int j = first + r;
-    float x = 0.f;
-    if (j < n && c < d && mask_key(mask, j)) x = Elem<T>::to_f(p[static_cast<int64_t>(j) * s.t + c]);
-    dst[r * (DP + kPad) + c] = x;
-  }
+  if (((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(s.t * sizeof(T))) & (4 * sizeof(T) - 1)) == 0 && d % 4 == 0)
+    load_rows_vec<T, ROWS, DP, 4>(dst, p, s.t, first, n, d, valid);
+  else
+    load_rows_vec<T, ROWS, DP, 1>(dst, p, s.t, first, n, d, valid);
+}
+
+// validity of the ROWS (32 or 64) keys from `first` (a multiple of 32)
+template <int ROWS>
+__device__ __forceinline__ uint64_t valid_keys(const uint32_t* mask, int first, int n) {
+  if (mask == nullptr) return ~0ull;
+  uint64_t w = first < n ? __ldg(mask + kMaskHead + (first >> 5)) : 0u;
+  if (ROWS == 64 && first + 32 < n) w |= static_cast<uint64_t>(__ldg(mask + kMaskHead + (first >> 5) + 1)) << 32;
+  return w;
 }
 
 // acc[r][c] = A[ty + 16 r] . B[tx + 8 c] over DP; rows of A and B are DP + kPad apart
@@ -153,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
   int lo, hi;
   mask_range(a, t.batch, t.n, lo, hi);
   if (a.causal) hi = min(hi, t.first + kSimtRows);
-  load_rows<T, kSimtRows, DP>(Q, a.q, a.qs, t, h, t.first, t.n, a.d, nullptr);
+  load_rows<T, kSimtRows, DP>(Q, a.q, a.qs, t, h, t.first, t.n, a.d, ~0ull);
   float m[R], l[R];
   float4 acc[R][DC];
 #pragma unroll
@@ -166,8 +214,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
   const float c2 = a.scale * kLog2e;
   for (int j0 = lo / KT * KT; j0 < hi; j0 += KT) {
     __syncthreads();
-    load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, mask);
-    load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, j0, t.n, a.d, mask);
+    const uint64_t valid = valid_keys<KT>(mask, j0, t.n);
+    load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, valid);
+    load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, j0, t.n, a.d, valid);
     __syncthreads();
     float s[R][C];
     mm_nt<R, C, DP>(s, Q, K, ty, tx);
@@ -178,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int j = j0 + tx + 8 * c;
-        const bool see = j < t.n && (!a.causal || j <= i) && mask_key(mask, j);
+        const bool see = j < t.n && (!a.causal || j <= i) && ((valid >> (tx + 8 * c)) & 1u);
         s[r][c] = see ? s[r][c] * c2 : neg_inf();
         top = fmaxf(top, s[r][c]);
       }
@@ -243,8 +292,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
   int lo, hi;
   mask_range(a, t.batch, t.n, lo, hi);
   if (a.causal) hi = min(hi, t.first + kSimtRows);
-  load_rows<T, kSimtRows, DP>(Q, a.q, a.qs, t, h, t.first, t.n, a.d, nullptr);
-  load_rows<T, kSimtRows, DP>(G, a.g, a.gs, t, h, t.first, t.n, a.d, nullptr);
+  load_rows<T, kSimtRows, DP>(Q, a.q, a.qs, t, h, t.first, t.n, a.d, ~0ull);
+  load_rows<T, kSimtRows, DP>(G, a.g, a.gs, t, h, t.first, t.n, a.d, ~0ull);
   float lse2[R], delta[R];
   float4 acc[R][DC];
 #pragma unroll
@@ -258,8 +307,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
   const float c2 = a.scale * kLog2e;
   for (int j0 = lo / KT * KT; j0 < hi; j0 += KT) {
     __syncthreads();
-    load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, mask);
-    load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, j0, t.n, a.d, mask);
+    const uint64_t valid = valid_keys<KT>(mask, j0, t.n);
+    load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, valid);
+    load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, j0, t.n, a.d, valid);
     __syncthreads();
     float s[R][C], dp[R][C];
     mm_nt<R, C, DP>(s, Q, K, ty, tx);
@@ -269,7 +319,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int i = t.first + ty + 16 * r, j = j0 + tx + 8 * c;
-        const bool see = i < t.n && j < t.n && (!a.causal || j <= i) && mask_key(mask, j) && lse2[r] != neg_inf();
+        const bool see = i < t.n && j < t.n && (!a.causal || j <= i) && ((valid >> (tx + 8 * c)) & 1u) &&
+                         lse2[r] != neg_inf();
         float p, ds;
         weight_grad(s[r][c], dp[r][c], lse2[r], delta[r], c2, see, p, ds);
         P[(ty + 16 * r) * (KT + kPad) + tx + 8 * c] = ds;
@@ -306,14 +357,15 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   }
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
-  load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, t.first, t.n, a.d, mask);
-  load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, t.first, t.n, a.d, mask);
+  const uint64_t valid = valid_keys<KT>(mask, t.first, t.n);
+  load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, t.first, t.n, a.d, valid);
+  load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, t.first, t.n, a.d, valid);
   bool key[R];
   float4 dk[R][DC], dv[R][DC];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int j = t.first + ty + 16 * r;
-    key[r] = j < t.n && mask_key(mask, j);
+    key[r] = j < t.n && ((valid >> (ty + 16 * r)) & 1u);
 #pragma unroll
     for (int x = 0; x < DC; ++x) dk[r][x] = dv[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
@@ -321,8 +373,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     for (int i0 = a.causal ? t.first : 0; i0 < t.n; i0 += QT) {
       __syncthreads();
-      load_rows<T, QT, DP>(Q, a.q, a.qs, t, h, i0, t.n, a.d, nullptr);
-      load_rows<T, QT, DP>(G, a.g, a.gs, t, h, i0, t.n, a.d, nullptr);
+      load_rows<T, QT, DP>(Q, a.q, a.qs, t, h, i0, t.n, a.d, ~0ull);
+      load_rows<T, QT, DP>(G, a.g, a.gs, t, h, i0, t.n, a.d, ~0ull);
       if (threadIdx.x < QT) {
         const int i = i0 + threadIdx.x;
         s_lse[threadIdx.x] = i < t.n ? a.lse[lse_index(a, t, h, i)] * kLog2e : neg_inf();
@@ -360,22 +412,39 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   store_rows<T, R, DC>(a.dv, a.dvs, t, hk, dv, one, a.d, ty, tx);
 }
 
-// delta_i = sum_d g_i o_i, one warp per (row, head)
-template <typename T>
+// delta_i = sum_d g_i o_i.  GROUP lanes per (row, head), 16 bytes of each tensor per lane and step (VEC elements;
+// one element where rows do not start on 16 bytes): bound by HBM, two tensors read once.
+template <typename T, int GROUP, int VEC>
 __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t rows) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (w >= rows) return;
-  const int h = static_cast<int>(w % a.H);
-  const int64_t r = w / a.H;
-  const int64_t b = r / a.L, i = r - b * a.L;
-  const T* o = static_cast<const T*>(a.o) + b * a.os.b + i * a.os.t + h * a.os.h;
-  const T* g = static_cast<const T*>(a.g) + b * a.gs.b + i * a.gs.t + h * a.gs.h;
+  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / GROUP;
+  const int lane = threadIdx.x % GROUP;
   float s = 0.f;
-  for (int c = lane; c < a.d; c += 32) s = fmaf(Elem<T>::to_f(o[c]), Elem<T>::to_f(g[c]), s);
+  int64_t at = 0;
+  if (w < rows) {
+    const int64_t r = w / a.H;
+    const int h = static_cast<int>(w - r * a.H);
+    const int64_t b = a.cu != nullptr ? 0 : r / a.L, i = r - b * a.L;
+    at = (b * a.H + h) * a.L + i;
+    const T* o = static_cast<const T*>(a.o) + b * a.os.b + i * a.os.t + h * a.os.h;
+    const T* g = static_cast<const T*>(a.g) + b * a.gs.b + i * a.gs.t + h * a.gs.h;
+    for (int c = lane * VEC; c < a.d; c += GROUP * VEC) {
+      if constexpr (VEC == 1) {
+        s = fmaf(Elem<T>::to_f(o[c]), Elem<T>::to_f(g[c]), s);
+      } else {
+        float x[4], y[4];
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-  if (lane == 0) a.delta[(b * a.H + h) * a.L + i] = s;
+        for (int e = 0; e < VEC; e += 4) {
+          load_vec<T, 4>(o + c + e, x);
+          load_vec<T, 4>(g + c + e, y);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) s = fmaf(x[z], y[z], s);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int x = GROUP / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+  if (lane == 0 && w < rows) a.delta[at] = s;
 }
 
 // key mask words: one CTA per batch entry
@@ -408,13 +477,13 @@ __global__ void attn_mask_words_kernel(const void* mask, int dtype, int64_t sB, 
   if (threadIdx.x < kMaskHead) w[threadIdx.x] = threadIdx.x == 0 ? s_lo : threadIdx.x == 1 ? s_hi : 0u;
 }
 
-template <typename K>
-cudaError_t launch(K kernel, const AttnArgs& a, int64_t ctas, size_t smem, cudaStream_t st) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+// smem is the same for every launch of a kernel
+template <auto Kernel>
+cudaError_t launch(const AttnArgs& a, int64_t ctas, size_t smem, cudaStream_t st) {
+  const cudaError_t e = allow_smem<Kernel>(static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(a);
+  Kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -432,7 +501,7 @@ cudaError_t fwd(AttnArgs a, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
   const size_t smem = sizeof(float) * ((kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
   const int64_t tiles = count_tiles(a, kSimtRows);
-  return launch(attn_simt_fwd_kernel<T, DP>, a, tiles * a.H, smem, st);
+  return launch<attn_simt_fwd_kernel<T, DP>>(a, tiles * a.H, smem, st);
 }
 
 template <typename T, int DP>
@@ -441,13 +510,13 @@ cudaError_t bwd(AttnArgs a, cudaStream_t st) {
   if (a.dq != nullptr) {
     const size_t smem = sizeof(float) * ((2 * kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
     const int64_t tiles = count_tiles(a, kSimtRows);
-    const cudaError_t e = launch(attn_simt_dq_kernel<T, DP>, a, tiles * a.H, smem, st);
+    const cudaError_t e = launch<attn_simt_dq_kernel<T, DP>>(a, tiles * a.H, smem, st);
     if (e != cudaSuccess) return e;
   }
   if (a.dk == nullptr) return cudaSuccess;
   const size_t smem = sizeof(float) * (4 * KT * (DP + kPad) + KT * (KT + kPad));
   const int64_t tiles = count_tiles(a, KT);
-  return launch(attn_simt_dkv_kernel<T, DP>, a, tiles * a.Hk, smem, st);
+  return launch<attn_simt_dkv_kernel<T, DP>>(a, tiles * a.Hk, smem, st);
 }
 
 template <typename T>
@@ -475,18 +544,35 @@ cudaError_t launch_attn_simt_bwd(const AttnArgs& a, int dtype, cudaStream_t st) 
   }
 }
 
-cudaError_t launch_attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
+namespace {
+template <typename T>
+bool rows_on16(const void* p, const AttnStrides& s) {
+  return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>((s.b | s.t | s.h) * sizeof(T))) % 16 == 0;
+}
+
+template <typename T>
+cudaError_t delta(const AttnArgs& a, cudaStream_t st) {
+  constexpr int kVec = 16 / sizeof(T);
   const int64_t rows = (a.cu != nullptr ? a.L : a.L * a.nseq) * a.H;
-  const int64_t ctas = (rows * 32 + 255) / 256;
-  if (ctas == 0) return cudaSuccess;
+  const bool vec = a.d % kVec == 0 && rows_on16<T>(a.o, a.os) && rows_on16<T>(a.g, a.gs);
+  const int group = vec && a.d <= 8 * kVec ? 8 : vec && a.d <= 16 * kVec ? 16 : 32;
+  const int64_t ctas = (rows * group + 255) / 256;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const unsigned grid = static_cast<unsigned>(ctas);
-  switch (dtype) {
-    case kF32: attn_delta_kernel<float><<<grid, 256, 0, st>>>(a, rows); break;
-    case kBF16: attn_delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, rows); break;
-    default: attn_delta_kernel<__half><<<grid, 256, 0, st>>>(a, rows); break;
-  }
+  if (!vec) attn_delta_kernel<T, 32, 1><<<grid, 256, 0, st>>>(a, rows);
+  else if (group == 8) attn_delta_kernel<T, 8, kVec><<<grid, 256, 0, st>>>(a, rows);
+  else if (group == 16) attn_delta_kernel<T, 16, kVec><<<grid, 256, 0, st>>>(a, rows);
+  else attn_delta_kernel<T, 32, kVec><<<grid, 256, 0, st>>>(a, rows);
   return cudaGetLastError();
+}
+}  // namespace
+
+cudaError_t launch_attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
+  switch (dtype) {
+    case kF32: return delta<float>(a, st);
+    case kBF16: return delta<__nv_bfloat16>(a, st);
+    default: return delta<__half>(a, st);
+  }
 }
 
 cudaError_t launch_attn_mask_words(const void* mask, int mask_dtype, int64_t sB, int64_t sL, int64_t B, int64_t L,

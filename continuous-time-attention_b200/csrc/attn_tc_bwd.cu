@@ -614,13 +614,13 @@ int64_t count_tiles(AttnArgs& a, int rows) {
   return static_cast<int64_t>(a.tiles) * a.nseq;
 }
 
-template <typename K>
-cudaError_t launch(K kernel, int smem, int64_t ctas, const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k,
+template <auto Kernel>
+cudaError_t launch(int smem, int64_t ctas, const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k,
                    const CUtensorMap& v, const BwdArgs& f, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_smem<Kernel>(smem);
   if (e != cudaSuccess) return e;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(q, g, k, v, f);
+  Kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(q, g, k, v, f);
   return cudaGetLastError();
 }
 
@@ -630,12 +630,12 @@ cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k
   if (f.a.dk != nullptr) {
     const int64_t tiles = count_tiles(f.a, kRows);
     const cudaError_t e =
-        launch(attn_tc_dkv_kernel<T, DP>, Layout<DP>::kSmem, tiles * f.a.Hk, q, g, k, v, f, st);
+        launch<attn_tc_dkv_kernel<T, DP>>(Layout<DP>::kSmem, tiles * f.a.Hk, q, g, k, v, f, st);
     if (e != cudaSuccess) return e;
   }
   if (f.a.dq == nullptr) return cudaSuccess;
   const int64_t tiles = count_tiles(f.a, f.tile_tokens);
-  return launch(attn_tc_dq_kernel<T, DP>, Layout<DP>::kSmem, tiles * (f.a.H / f.pack), q, g, k, v, f, st);
+  return launch<attn_tc_dq_kernel<T, DP>>(Layout<DP>::kSmem, tiles * (f.a.H / f.pack), q, g, k, v, f, st);
 }
 
 }  // namespace

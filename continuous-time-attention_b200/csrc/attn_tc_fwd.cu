@@ -408,11 +408,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int DP, bool PAGED>
 cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int64_t ctas,
                    cudaStream_t st) {
-  const auto kernel = attn_tc_fwd_kernel<T, DP, PAGED>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DP>::kSmem);
+  const cudaError_t e = allow_smem<attn_tc_fwd_kernel<T, DP, PAGED>>(Layout<DP>::kSmem);
   if (e != cudaSuccess) return e;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  kernel<<<static_cast<unsigned>(ctas), kThreads, Layout<DP>::kSmem, st>>>(q, k, v, f);
+  attn_tc_fwd_kernel<T, DP, PAGED><<<static_cast<unsigned>(ctas), kThreads, Layout<DP>::kSmem, st>>>(q, k, v, f);
   return cudaGetLastError();
 }
 

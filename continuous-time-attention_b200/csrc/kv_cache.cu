@@ -22,7 +22,7 @@ namespace {
 constexpr float kE4m3Max = 448.f;
 constexpr float kLeastMax = 7.888609052210118e-31f;  // 2^-100
 constexpr int kThreads = 256;
-constexpr int kRowsPerGroup = 2;
+constexpr int kRowsPerGroup = 4;
 
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
   uint16_t lo, hi;

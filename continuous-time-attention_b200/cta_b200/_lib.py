@@ -214,6 +214,20 @@ class on_device:
         return False
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def enqueue(fn, t: torch.Tensor, *args) -> None:
+    """fn(*args, stream) on t's device and its current stream; raises on a non-zero status."""
+    if _current_device() == t.get_device():
+        rc = fn(*args, stream_ptr(t))
+    else:
+        with on_device(t):
+            rc = fn(*args, stream_ptr(t))
+    if rc:
+        check(rc)
+
+
 def ptr_array(tensors) -> ctypes.Array:
     arr = (c_void_p * MAX_STEPS)()
     for i, t in enumerate(tensors):

@@ -68,4 +68,5 @@ def prompt_attention(
         words = ops.attention_mask(key_mask)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal), scale)
-    return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens)[0]
+    return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens,
+                                 need_lse=False)[0]

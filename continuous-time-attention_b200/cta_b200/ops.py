@@ -529,18 +529,14 @@ def bld_forward_pool(
 # ---------------------------------------------------------------------------
 # attention of prompts
 # ---------------------------------------------------------------------------
-def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
 def _same_kind(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
 
 
-def _device_ints(t: torch.Tensor, name: str, device: torch.device, dtype: torch.dtype) -> torch.Tensor:
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
+def _device_ints(t: torch.Tensor, name: str, like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}")
     if t.dtype != dtype:
         if t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
@@ -548,11 +544,23 @@ def _device_ints(t: torch.Tensor, name: str, device: torch.device, dtype: torch.
     return t
 
 
-def _offsets(cu: torch.Tensor, device: torch.device) -> torch.Tensor:
+def _offsets(cu: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     if cu.dim() != 1 or cu.numel() < 1:
         raise ValueError("cu_seqlens must have shape (sequences + 1,)")
-    cu = _device_ints(cu, "cu_seqlens", device, torch.int32)
+    if cu.dtype != torch.int32 or cu.device != like.device:
+        cu = _device_ints(cu, "cu_seqlens", like, torch.int32)
     return cu if cu.is_contiguous() else cu.contiguous()
+
+
+def _on16(t: torch.Tensor) -> bool:
+    """The last axis is contiguous, and every row starts on 16 bytes and on its own."""
+    s = t.stride()
+    if s[-1] != 1 or t.data_ptr() & 15:
+        return False
+    es = t.element_size()
+    if t.is_contiguous():
+        return t.shape[-1] * es & 15 == 0  # the other strides are multiples of a row
+    return all(n <= 1 or (x > 0 and x * es & 15 == 0) for x, n in zip(s[:-1], t.shape))
 
 
 def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
@@ -563,46 +571,69 @@ def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
         raise ValueError("key_mask must have shape (B, L)")
     B, L = key_mask.shape
     m, code, sB, sL = _mask_args(key_mask, B, L, key_mask.device)
-    lib = _lib.load()
-    words = torch.empty(B, lib.cta_attention_mask_words_per_row(L), dtype=torch.int32, device=key_mask.device)
-    with _lib.on_device(key_mask):
-        rc = lib.cta_attention_mask_words(_lib.ptr(m), code, sB, sL, B, L, _lib.ptr(words), _lib.stream_ptr(key_mask))
-    _lib.check(rc)
+    words = torch.empty((B, _mask_row_words(L)), dtype=torch.int32, device=key_mask.device)
+    _lib.enqueue(_lib.load().cta_attention_mask_words, key_mask, m.data_ptr(), code, sB, sL, B, L, words.data_ptr())
     return words
 
 
-def _attention_shapes(q, k, v, cu_seqlens, mask_words, scale):
-    """Checked inputs and the sizes: (q, k, v, cu, sequences, length, heads, kv_heads, dim, scale)."""
+def _attention_inputs(q, k, v, cu_seqlens, mask_words, scale):
+    """Checked inputs and sizes: (q, k, v, cu or None, (sequences, length, heads, kv_heads, dim), dtype code, scale)."""
     _require_cuda(q, "q")
+    dtype, device = q.dtype, q.device
+    code = _lib.dtype_code(dtype)
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+        _same_kind(k, "k", q)
+        _same_kind(v, "v", q)
+    shape, kshape = q.shape, k.shape
     rank = 4 if cu_seqlens is None else 3
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != rank:
-            raise ValueError(f"{name} must have shape " + ("(B, L, heads, dim)" if rank == 4 else "(T, heads, dim)"))
-    _same_kind(k, "k", q)
-    _same_kind(v, "v", q)
-    if k.shape != v.shape or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not go together")
-    heads, dim = q.shape[-2:]
-    kv_heads = k.shape[-2]
+    if len(shape) != rank:
+        raise ValueError("q must have shape " + ("(B, L, heads, dim)" if rank == 4 else "(T, heads, dim)"))
+    if kshape != v.shape or len(kshape) != rank or kshape[:-2] != shape[:-2] or kshape[-1] != shape[-1]:
+        raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)} do not go together")
+    length, heads, dim = shape[-3:]
+    kv_heads = kshape[-2]
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    length = q.shape[-3]
     cu = None
     if cu_seqlens is None:
-        sequences = q.shape[0]
-        if mask_words is not None and (mask_words.dtype != torch.int32 or mask_words.device != q.device
-                                       or not mask_words.is_contiguous() or tuple(mask_words.shape)
-                                       != (sequences, _lib.load().cta_attention_mask_words_per_row(length))):
+        sequences = shape[0]
+        if mask_words is not None and (mask_words.dtype != torch.int32 or mask_words.device != device
+                                       or not mask_words.is_contiguous()
+                                       or mask_words.shape != (sequences, _mask_row_words(length))):
             raise ValueError("mask_words must come from attention_mask() of a (B, L) mask")
     else:
         if mask_words is not None:
             raise ValueError("a key mask takes padded sequences, not packed ones")
-        cu = _offsets(cu_seqlens, q.device)
-        sequences = cu.numel() - 1
-    if scale is None:
-        scale = dim**-0.5
-    return (_last_contiguous(q), _last_contiguous(k), _last_contiguous(v), cu, sequences, length, heads, kv_heads, dim,
-            float(scale))
+        cu = _offsets(cu_seqlens, q)
+        sequences = cu.shape[0] - 1
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()
+            and (code == 0 or dim & 7 or not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15)):
+        q, k, v = _attention_rows(q, code), _attention_rows(k, code), _attention_rows(v, code)
+    return q, k, v, cu, (sequences, length, heads, kv_heads, dim), code, dim**-0.5 if scale is None else float(scale)
+
+
+def _mask_row_words(length: int) -> int:
+    """cta_attention_mask_words_per_row: a header of 4 words, then one bit per key in blocks of 128."""
+    return 4 + (length + 127) // 128 * 4
+
+
+def _attention_rows(t: torch.Tensor, code: int) -> torch.Tensor:
+    """t with a contiguous last axis and, in 16 bits, rows that the tensor-core kernels can
+    load: other views are copied (head dims that are no multiple of 8 take the plain kernels)."""
+    if t.stride(-1) == 1 and (code == 0 or t.shape[-1] & 7 or _on16(t)):
+        return t
+    return _own_rows(t)
+
+
+def _own_rows(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous copy that starts on 16 bytes."""
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _new(like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of like's shape (empty_like is the cheaper call)."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype,
+                                                                           device=like.device)
 
 
 def _strides3(t: Optional[torch.Tensor]):
@@ -612,8 +643,7 @@ def _strides3(t: Optional[torch.Tensor]):
     return s[:3] if len(s) == 4 else (0, s[0], s[1])
 
 
-def _full_like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+_NO_STRIDES = (0,) * 12
 
 
 def attention_forward(
@@ -626,26 +656,29 @@ def attention_forward(
     mask_words: Optional[torch.Tensor] = None,
     cu_seqlens: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
+    need_lse: bool = True,
 ):
     """Softmax attention of prompts, one launch: (out, lse).
 
     Padded: q [B, L, heads, dim], k and v [B, L, kv_heads, dim], optionally the
     words of a key mask (attention_mask).  Packed: [T, heads, dim] with device
-    cu_seqlens (int32, sequences + 1).  Any strides with a contiguous last axis.
-    Rows that see no key are zero.  Packed rows behind the last sequence keep
-    what `out` holds; in an output allocated here they are zero.  `lse` (fp32,
-    [B, heads, L] or [heads, T]) is what attention_backward takes."""
-    q, k, v, cu, n, length, heads, kv_heads, dim, scale = _attention_shapes(q, k, v, cu_seqlens, mask_words, scale)
-    zero_tail = out is None
-    o = _out(out, q.shape, q)
-    lse = torch.empty((n, heads, length) if cu is None else (heads, length), dtype=torch.float32, device=q.device)
+    cu_seqlens (int32, sequences + 1).  float32, bfloat16, float16; dim up to
+    256; any strides (views that TMA cannot address are copied first).  Rows
+    that see no key are zero.  Packed rows behind the last sequence keep what
+    `out` holds; in an output allocated here they are zero.  `lse` (fp32,
+    [B, heads, L] or [heads, T]; None without need_lse) is what
+    attention_backward takes."""
+    q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
+    o = _new(q) if out is None else _out(out, q.shape, q)
+    lse = None
+    if need_lse:
+        n, length, heads = sizes[:3]
+        lse = torch.empty((n, heads, length) if cu is None else (heads, length), dtype=torch.float32, device=q.device)
     args = _lib.ATTENTION_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, _lib.ptr(cu),
-        _lib.ptr(mask_words), *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(o), *(0,) * 12, n, length,
-        heads, kv_heads, dim, _lib.dtype_code(q.dtype), int(causal), int(zero_tail), 0, scale, 0.0)
-    with _lib.on_device(q):
-        rc = _lib.load().cta_attention_forward(args, _lib.stream_ptr(q))
-    _lib.check(rc)
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
+        0 if cu is None else cu.data_ptr(), 0 if mask_words is None else mask_words.data_ptr(), *_strides3(q),
+        *_strides3(k), *_strides3(v), *_strides3(o), *_NO_STRIDES, *sizes, code, bool(causal), out is None, 0, scale, 0.0)
+    _lib.enqueue(_lib.load().cta_attention_forward, q, args)
     return o, lse
 
 
@@ -665,75 +698,84 @@ def attention_backward(
     need_dkv: bool = True,
 ):
     """(dq, dk, dv) of attention_forward from its out and lse; None for what is not wanted."""
-    q, k, v, cu, n, length, heads, kv_heads, dim, scale = _attention_shapes(q, k, v, cu_seqlens, mask_words, scale)
+    q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
+    n, length, heads = sizes[:3]
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"grad_out and out must be {tuple(q.shape)}")
-    _same_kind(grad_out, "grad_out", q)
-    _same_kind(out, "out", q)
+    if grad_out.dtype != q.dtype or out.dtype != q.dtype or grad_out.device != q.device or out.device != q.device:
+        _same_kind(grad_out, "grad_out", q)
+        _same_kind(out, "out", q)
     shape = (n, heads, length) if cu is None else (heads, length)
-    if tuple(lse.shape) != shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+    if lse.shape != shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 {shape} on {q.device}")
-    g, o = _last_contiguous(grad_out), _last_contiguous(out)
-    dq = _full_like(q) if need_dq else None
-    dk = _full_like(k) if need_dkv else None
-    dv = _full_like(v) if need_dkv else None
+    g, o = _attention_rows(grad_out, code), _attention_rows(out, code)
+    dq = _new(q) if need_dq else None
+    dk = _new(k) if need_dkv else None
+    dv = _new(v) if need_dkv else None
     delta = torch.empty_like(lse)
     args = _lib.ATTENTION_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), g.data_ptr(), delta.data_ptr(),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(cu), _lib.ptr(mask_words), *_strides3(q), *_strides3(k),
-        *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), n, length, heads,
-        kv_heads, dim, _lib.dtype_code(q.dtype), int(causal), 0, 0, scale, 0.0)
-    with _lib.on_device(q):
-        rc = _lib.load().cta_attention_backward(args, _lib.stream_ptr(q))
-    _lib.check(rc)
+        *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), *sizes, code,
+        bool(causal), 0, 0, scale, 0.0)
+    _lib.enqueue(_lib.load().cta_attention_backward, q, args)
     return dq, dk, dv
 
 
 # ---------------------------------------------------------------------------
 # paged key/value cache
 # ---------------------------------------------------------------------------
-def _on16(t: torch.Tensor) -> bool:
-    """The last axis is contiguous and every row starts on 16 bytes."""
-    es = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n <= 1 or s * es % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])))
-
-
 def _row_strides(t: torch.Tensor):
-    """Strides of all axes but the last; 0 for an axis of one entry, whose stride means nothing."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+    """Strides of all axes but the last; an axis of one entry, whose own stride means nothing, counts 0 or
+    what it would have in a fresh tensor."""
+    if t.is_contiguous():
+        shape = t.shape
+        if len(shape) == 3:
+            return shape[1] * shape[2], shape[2]
+        return shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]
+    return tuple(x if n > 1 else 0 for x, n in zip(t.stride(), t.shape[:-1]))
 
 
-def _cache_shapes(k_cache, v_cache, k_scale, v_scale, dtype, device):
+def _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, like):
     """Checked cache: (pages, page_size, kv_heads, dim, quantized)."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape, kind = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have one shape (pages, page_size, kv_heads, dim)")
-    quantized = k_cache.dtype == torch.float8_e4m3fn
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.device != device or t.dtype != k_cache.dtype or not (quantized or t.dtype == dtype):
-            raise ValueError(f"{name} must be {dtype} or float8_e4m3fn on {device}, got {t.dtype} on {t.device}")
-        if not _on16(t):
-            raise ValueError(f"{name} must have a contiguous last axis and rows that start on 16 bytes")
-    pages, page, heads, dim = k_cache.shape
-    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if not quantized:
-            if t is not None:
-                raise ValueError(f"{name} goes with a float8_e4m3fn cache")
-        elif (t is None or tuple(t.shape) != (pages, heads, page) or t.dtype != torch.float32 or t.device != device
-              or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 {(pages, heads, page)} on {device}")
+    quantized = kind == torch.float8_e4m3fn
+    device = like.device
+    if (not quantized and kind != dtype) or v_cache.dtype != kind or k_cache.device != device or (
+            v_cache.device != device):
+        raise ValueError(f"k_cache and v_cache must be {dtype} or float8_e4m3fn on {device}, got {kind} on "
+                         f"{k_cache.device} and {v_cache.dtype} on {v_cache.device}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
+            and shape[3] & 15 == 0) and not (_on16(k_cache) and _on16(v_cache)):
+        raise ValueError("k_cache and v_cache must have a contiguous last axis and rows that start on 16 bytes")
+    pages, page, heads, dim = shape
+    if quantized:
+        want = (pages, heads, page)
+        for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if (t is None or t.shape != want or t.dtype != torch.float32 or t.device != device
+                    or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous float32 {want} on {device}")
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("k_scale and v_scale go with a float8_e4m3fn cache")
     return pages, page, heads, dim, quantized
 
 
-def _cache_call(name, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes):
+def _slots(slots: torch.Tensor, n: Optional[int], like: torch.Tensor) -> torch.Tensor:
+    if slots.dim() != 1 or (n is not None and slots.shape[0] != n):
+        raise ValueError("slots must have shape (T,)")
+    slots = _device_ints(slots, "slots", like, torch.int64)
+    return slots if slots.is_contiguous() else slots.contiguous()
+
+
+def _cache_call(fn, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes):
     pages, page, heads, dim, quantized = sizes
     args = _lib.KV_CACHE_ARGS.pack(
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
         slots.data_ptr(), *_row_strides(k), *_row_strides(v), *_row_strides(k_cache), *_row_strides(v_cache),
-        k.shape[0], heads, dim, pages, page, _lib.dtype_code(k.dtype), int(quantized))
-    with _lib.on_device(k):
-        rc = getattr(_lib.load(), name)(args, _lib.stream_ptr(k))
-    _lib.check(rc)
+        slots.shape[0], heads, dim, pages, page, _lib.dtype_code(k.dtype), quantized)
+    _lib.enqueue(fn, k, args)
 
 
 def kv_cache_write(
@@ -758,22 +800,14 @@ def kv_cache_write(
     _require_cuda(k, "k")
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError("k and v must have one shape (T, kv_heads, dim)")
-    _lib.dtype_code(k.dtype)
     _same_kind(v, "v", k)
-    sizes = _cache_shapes(k_cache, v_cache, k_scale, v_scale, k.dtype, k.device)
+    sizes = _cache_sizes(k_cache, v_cache, k_scale, v_scale, k.dtype, k)
     if k.shape[1:] != k_cache.shape[2:]:
         raise ValueError(f"k {tuple(k.shape)} does not fit a cache {tuple(k_cache.shape)}")
-    slots = _slots(slots, k.shape[0], k.device)
-    k = k if _on16(k) else k.contiguous()
-    v = v if _on16(v) else v.contiguous()
-    _cache_call("cta_kv_cache_write", k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
-
-
-def _slots(slots: torch.Tensor, n: Optional[int], device: torch.device) -> torch.Tensor:
-    if slots.dim() != 1 or (n is not None and slots.shape[0] != n):
-        raise ValueError("slots must have shape (T,)")
-    slots = _device_ints(slots, "slots", device, torch.int64)
-    return slots if slots.is_contiguous() else slots.contiguous()
+    slots = _slots(slots, k.shape[0], k)
+    k = k if _on16(k) else _own_rows(k)
+    v = v if _on16(v) else _own_rows(v)
+    _cache_call(_lib.load().cta_kv_cache_write, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
 
 
 def kv_cache_read(
@@ -790,11 +824,12 @@ def kv_cache_read(
     _require_cuda(k_cache, "k_cache")
     if dtype is None:
         dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
-    _lib.dtype_code(dtype)
-    sizes = _cache_shapes(k_cache, v_cache, k_scale, v_scale, dtype, k_cache.device)
-    slots = _slots(slots, None, k_cache.device)
-    k, v = (torch.empty(slots.shape[0], sizes[2], sizes[3], dtype=dtype, device=k_cache.device) for _ in range(2))
-    _cache_call("cta_kv_cache_read", k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
+    sizes = _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, k_cache)
+    slots = _slots(slots, None, k_cache)
+    # both in one allocation
+    both = torch.empty((2, slots.shape[0], sizes[2], sizes[3]), dtype=dtype, device=k_cache.device)
+    k, v = both.unbind(0)
+    _cache_call(_lib.load().cta_kv_cache_read, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
     return k, v
 
 
@@ -829,46 +864,50 @@ def paged_attention(
     _require_cuda(q, "q")
     if q.dim() != 3:
         raise ValueError("q must have shape (T, heads, dim)")
-    dcode = _lib.dtype_code(q.dtype)
-    pages, page, kv_heads, dim, quantized = _cache_shapes(k_cache, v_cache, k_scale, v_scale, q.dtype, q.device)
-    rows, heads = q.shape[:2]
-    if q.shape[2] != dim or heads < 1 or kv_heads < 1 or heads % kv_heads:
+    code = _lib.dtype_code(q.dtype)
+    pages, page, kv_heads, dim, quantized = _cache_sizes(k_cache, v_cache, k_scale, v_scale, q.dtype, q)
+    rows, heads, q_dim = q.shape
+    if q_dim != dim or heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not go with a cache {tuple(k_cache.shape)}")
-    table = _device_ints(block_table, "block_table", q.device, torch.int32)
-    if table.dim() != 2 or seq_lens.dim() != 1 or table.shape[0] != seq_lens.shape[0]:
+    table, lens = block_table, seq_lens
+    if table.dtype != torch.int32 or table.device != q.device:
+        table = _device_ints(table, "block_table", q, torch.int32)
+    if lens.dtype != torch.int32 or lens.device != q.device:
+        lens = _device_ints(lens, "seq_lens", q, torch.int32)
+    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
         raise ValueError("block_table must have shape (B, width), seq_lens (B,)")
     if table.stride(1) != 1:
         table = table.contiguous()
-    lens = _device_ints(seq_lens, "seq_lens", q.device, torch.int32)
     if not lens.is_contiguous():
         lens = lens.contiguous()
     batch = lens.shape[0]
     cu = None
     if cu_seqlens is not None:
-        cu = _offsets(cu_seqlens, q.device)
+        cu = _offsets(cu_seqlens, q)
         if cu.numel() != batch + 1:
             raise ValueError(f"cu_seqlens must have {batch + 1} entries, got {cu.numel()}")
-    q = q if _on16(q) else q.contiguous()
-    o = _out(out, q.shape, q)
-    if not _on16(o):
-        raise ValueError("out must have rows that start on 16 bytes")
-    if scale is None:
-        scale = dim**-0.5
+    if not _on16(q):
+        q = _own_rows(q)
+    if out is None:
+        o = _new(q)
+    else:
+        o = _out(out, q.shape, q)
+        if not _on16(o):
+            raise ValueError("out must have rows that start on 16 bytes")
     lib = _lib.load()
     max_rows = int(max_rows)
-    key = (q.device.index, dcode, quantized, dim, heads // kv_heads, min(max_rows, 16))
-    with _lib.on_device(q):
-        nbytes = _PAGED_BYTES.get(key)
-        if nbytes is None:
-            nbytes = lib.cta_paged_attention_workspace_bytes(max_rows, heads, kv_heads, dim, dcode, int(quantized))
-            _PAGED_BYTES[key] = nbytes
-        # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        args = _lib.PAGED_ATTENTION_ARGS.pack(
-            q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
-            table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o),
-            *_row_strides(k_cache), *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages,
-            page, table.shape[1], max_rows, dcode, int(quantized), float(scale), 0.0)
-        rc = lib.cta_paged_attention(args, ws.data_ptr(), nbytes, _lib.stream_ptr(q))
-    _lib.check(rc)
+    key = (q.get_device(), code, quantized, dim, heads // kv_heads, min(max_rows, 16))
+    nbytes = _PAGED_BYTES.get(key)
+    if nbytes is None:
+        with _lib.on_device(q):
+            nbytes = lib.cta_paged_attention_workspace_bytes(max_rows, heads, kv_heads, dim, code, int(quantized))
+        _PAGED_BYTES[key] = nbytes
+    # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _lib.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
+        table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o), *_row_strides(k_cache),
+        *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, table.shape[1],
+        max_rows, code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
+    _lib.enqueue(lib.cta_paged_attention, q, args, ws.data_ptr(), nbytes)
     return o
