@@ -7,14 +7,16 @@
 // What bounds it: HBM, 2 Hk (2 d) bytes per key (e4m3: 2 Hk (d + 4)).  So the
 // design keeps loads in flight and does nothing else:
 //
-// * The rows of all query heads that share a key/value head form one 16-row
-//   (8-row, when no more are live) operand of mma.m16n8k16, whose B fragments
-//   the lanes load straight from the pages, 16 bytes each, without shared
-//   memory.  A contraction may take its index in any order, so the lane that
-//   holds key n of a B fragment takes the eight (e4m3: sixteen) elements that
-//   one load brings as its share of two (four) k16 steps, and Q is laid out to
-//   match; in P V the n index is permuted the same way and undone in the
-//   output's address.  tcgen05 would need 128 rows where there are 1 to 16.
+// * The products are transposed: K Q^T and V^T P^T, keys (dims) along the 16 of
+//   mma.m16n8k16 and the rows of all query heads that share a key/value head
+//   along the 8, so that 8 rows fill the instruction.  The lanes load the A
+//   fragments straight from the pages, 16 bytes each, without shared memory: a
+//   contraction may take its index in any order, so the lane that holds a key
+//   takes the eight (e4m3: sixteen) elements that one load brings as its share
+//   of two (four) k16 steps, and Q is laid out to match; in V^T P^T the m index
+//   is permuted so that a lane ends with the consecutive elements it loaded.
+//   The weights change sides by a transposing move.  tcgen05 would need 128 rows
+//   where there are 1 to 16.
 // * Every warp is a worker.  The 16-key groups of all (sequence, row tile, head)
 //   segments form one list, cut into equal runs, one per worker, whatever the
 //   lengths are; the host never reads them.  A worker that holds only a part
@@ -41,8 +43,10 @@ constexpr int kThreads = 128;
 constexpr int kGroup = 16;      // keys per step of a warp
 constexpr int kMinGroups = 2;   // groups a worker gets at least
 constexpr int kPartRows = 16;
-// fp16 weights carry 2^14: what is lost to subnormals is below 2^-39 of the largest
-constexpr float kHalfShift = 14.f;
+// the references that weights are relative to move when a weight would pass 2^kLazy
+constexpr float kLazy = 8.f;
+// fp16 weights carry 2^7, and so stay below 2^15; what is lost to subnormals is below 2^-32 of the reference
+constexpr float kHalfShift = 7.f;
 
 template <typename M> struct Mma;
 template <> struct Mma<__half> {
@@ -159,19 +163,28 @@ __device__ __forceinline__ Seg find_segment(const PagedArgs& a, int64_t u, int t
   }
 }
 
+// 8 x 8 of 16-bit values across the warp, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// ROWS: 8 or 16 rows per segment
 template <typename T, bool FP8, int DP, int ROWS>
-__global__ void __launch_bounds__(kThreads, DP == 128 ? 2 : ROWS == 8 ? 4 : 3)
+__global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3) : (DP == 64 ? 3 : 2))
     paged_split_kernel(const __grid_constant__ PagedArgs a) {
   using M = typename std::conditional<FP8, __half, T>::type;
   constexpr bool kHalf = std::is_same<M, __half>::value;
-  constexpr int R = ROWS / 8;                 // rows per lane
-  constexpr int KS = DP / 16;                 // k16 steps of Q K^T
+  constexpr float kShift = kHalf ? kHalfShift : 0.f;
+  constexpr int NR = ROWS / 8;                // n8 tiles of rows
+  constexpr int KS = DP / 16;                 // k16 steps of K Q^T
   constexpr int KE = FP8 ? 16 : 8;            // elements of one key load
   constexpr int KL = DP / (4 * KE);           // key loads per lane and key
   constexpr int VE = FP8 && DP == 128 ? 16 : 8;  // elements of one value load
   constexpr int VL = DP / (8 * VE);           // value loads per lane and key
   constexpr int VW = FP8 ? VE / 4 : VE / 2;   // 32-bit words of one value load
-  constexpr int NT = DP / 8;                  // n8 tiles of the output
+  constexpr int MT = DP / 16;                 // m16 tiles of the output
 
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, quad = lane & 3, oct = lane >> 2;
@@ -189,18 +202,17 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 2 : ROWS == 8 ? 4 : 3)
     const Seg g = find_segment(a, u, ROWS);
     const int count = static_cast<int>(min(u_end - u, static_cast<int64_t>(g.groups - g.group)));
 
-    // Q fragments, and each row's last visible key
-    uint32_t qf[KS][R][2];
-    float c2[R];
-    int last[R];
+    // Q as the B operand: row oct of each n8 tile
+    uint32_t qf[KS][NR][2];
+    float c2[NR][2];
+    int last[NR][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < NR; ++r) {
       const int i = g.tile * ROWS + oct + 8 * r;
       const int tok = i / group;
       const bool live = tok < g.rows;
-      last[r] = live ? g.n - g.rows + tok : -1;
       const T* q = static_cast<const T*>(a.q) + (g.row0 + tok) * a.q_sT + (g.hk * group + i - tok * group) * a.q_sH;
-      float top = 0.f;
+      float top = 0.f, mul = a.scale * kLog2e;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int c = FP8 ? 64 * (k / 4) + 16 * quad + 4 * (k % 4) : 32 * (k / 2) + 8 * quad + 4 * (k % 2);
@@ -214,14 +226,13 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 2 : ROWS == 8 ? 4 : 3)
           top = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))), top);
         }
       }
-      c2[r] = a.scale * kLog2e;
       if constexpr (FP8 && !std::is_same<T, __half>::value) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the power of two at the row's largest element, kept where it and its reciprocal are normal
         const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 2), 252);
         const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        c2[r] *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+        mul *= __uint_as_float(static_cast<uint32_t>(e) << 23);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -230,78 +241,79 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 2 : ROWS == 8 ? 4 : 3)
             qf[k][r][i2] = Mma<__half>::pack(x.x * down, x.y * down);
           }
       }
+      const int see = live ? g.n - g.rows + tok : -1;
+      // scores and weights hold rows 2 quad, 2 quad + 1
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        c2[r][e] = __shfl_sync(0xffffffffu, mul, 4 * (2 * quad + e));
+        last[r][e] = __shfl_sync(0xffffffffu, see, 4 * (2 * quad + e));
+      }
     }
 
-    float o[NT][4];
-    float m[R], l[R], mv[R];  // running maximum of the scores, sum of weights, maximum of the weighted values
+    float o[MT][NR][4];
+    float m[NR][2], l[NR][2], mv[NR][2];  // reference of the weights, their sum, reference of the weighted values
 #pragma unroll
-    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int r = 0; r < R; ++r) m[r] = mv[r] = neg_inf(), l[r] = 0.f;
+      for (int r = 0; r < NR; ++r) o[t][r][0] = o[t][r][1] = o[t][r][2] = o[t][r][3] = 0.f;
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[r][e] = mv[r][e] = neg_inf(), l[r][e] = 0.f;
 
     const int32_t* table = a.table + g.b * a.table_sB;
-    auto page_of = [&](int grp) -> int {
-      // the page of a group, -1 if the table's entry lies outside the cache
-      if (grp >= g.group + count || grp * kGroup >= g.n) return -1;
-      const int p = __ldg(table + grp * kGroup / a.page);
+    const int per_page = a.page / kGroup;
+    auto page_at = [&](int index) -> int {
+      // the index-th page of the sequence, -1 if the table's entry lies outside the cache
+      if (index * a.page >= g.n) return -1;
+      const int p = __ldg(table + index);
       if (p < 0 || p >= a.n_pages) {
         if (lane == 0) atomicExch(&g_paged_error, kDevBadIndex);
         return -1;
       }
       return p;
     };
+    using C = typename std::conditional<FP8, uint8_t, T>::type;
+    const C* k_base = static_cast<const C*>(a.k_cache) + g.hk * a.kc_sH + KE * quad;
+    const C* v_base = static_cast<const C*>(a.v_cache) + g.hk * a.vc_sH + VE * oct;
     uint4 kf[2][KL];
-    float ks[2][2], vs[2][2];
+    float ks[2], vs[2];
     uint32_t vf[4][VL][VW];
-    auto load_keys = [&](int grp, int p) {
+    auto load_keys = [&](int grp, int p, int slot) {
+      const C* at = k_base + p * a.kc_sP + (slot + oct) * a.kc_sS;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int j = grp * kGroup + 8 * t + oct;
-        const bool ok = p >= 0 && j < g.n;
-        const int64_t at = p * a.kc_sP + (j % a.page) * a.kc_sS + g.hk * a.kc_sH;
+        const bool ok = p >= 0 && grp * kGroup + 8 * t + oct < g.n;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
-          const int c = 4 * KE * i + KE * quad;
           kf[t][i] = make_uint4(0u, 0u, 0u, 0u);
-          if (ok && c < a.d) {
-            if constexpr (FP8) kf[t][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.k_cache) + at + c));
-            else kf[t][i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_cache) + at + c));
-          }
+          if (ok && 4 * KE * i + KE * quad < a.d)
+            kf[t][i] = __ldg(reinterpret_cast<const uint4*>(at + 8 * t * a.kc_sS + 4 * KE * i));
+        }
+        if constexpr (FP8) {
+          const int64_t x = (static_cast<int64_t>(p) * a.Hk + g.hk) * a.page + slot + 8 * t + oct;
+          ks[t] = ok ? __ldg(a.k_scale + x) : 1.f;
+          vs[t] = ok ? __ldg(a.v_scale + x) : 1.f;
         }
       }
     };
-    auto load_scales = [&](int grp, int p) {
-      if constexpr (FP8) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = grp * kGroup + 8 * t + 2 * quad + e;
-            const bool ok = p >= 0 && j < g.n;
-            const int64_t at = (static_cast<int64_t>(p) * a.Hk + g.hk) * a.page + j % a.page;
-            ks[t][e] = ok ? __ldg(a.k_scale + at) : 1.f;
-            vs[t][e] = ok ? __ldg(a.v_scale + at) : 1.f;
-          }
-      }
-    };
-    auto load_values = [&](int grp, int p) {
+    auto load_values = [&](int grp, int p, int slot) {
+      const C* at = v_base + p * a.vc_sP + (slot + 2 * quad) * a.vc_sS;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = grp * kGroup + 2 * quad + (i & 1) + 8 * (i >> 1);
-        const bool ok = p >= 0 && j < g.n;
-        const int64_t at = p * a.vc_sP + (j % a.page) * a.vc_sS + g.hk * a.vc_sH;
+        const int k = (i & 1) + 8 * (i >> 1);
+        const bool ok = p >= 0 && grp * kGroup + 2 * quad + k < g.n;
 #pragma unroll
         for (int x = 0; x < VL; ++x) {
-          const int c = 8 * VE * x + VE * oct;
 #pragma unroll
           for (int w = 0; w < VW; ++w) vf[i][x][w] = 0u;
-          if (ok && c < a.d) {
+          if (ok && 8 * VE * x + VE * oct < a.d) {
+            const C* q = at + k * a.vc_sS + 8 * VE * x;
             if constexpr (VW == 4) {
-              const uint4 w = FP8 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.v_cache) + at + c))
-                                  : __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v_cache) + at + c));
+              const uint4 w = __ldg(reinterpret_cast<const uint4*>(q));
               vf[i][x][0] = w.x, vf[i][x][1] = w.y, vf[i][x][2] = w.z, vf[i][x][3] = w.w;
             } else {
-              const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v_cache) + at + c));
+              const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
               vf[i][x][0] = w.x, vf[i][x][1] = w.y;
             }
           }
@@ -309,187 +321,198 @@ __global__ void __launch_bounds__(kThreads, DP == 128 ? 2 : ROWS == 8 ? 4 : 3)
       }
     };
 
-    int p_now = page_of(g.group), p_next = page_of(g.group + 1);
-    load_keys(g.group, p_now);
-    load_scales(g.group, p_now);
-    load_values(g.group, p_now);
+    // the group's page and its first slot there, now and one group on; the page after that is on its way
+    int index = g.group / per_page;
+    int slot = (g.group - index * per_page) * kGroup;
+    int page = page_at(index), page_on = page_at(index + 1);
+    load_keys(g.group, page, slot);
+    load_values(g.group, page, slot);
     for (int it = 0; it < count; ++it) {
       const int grp = g.group + it;
-      const int p_after = page_of(grp + 2);
-      // scores of 16 keys
-      float s[2][4];
+      const bool here = page >= 0;
+      // where the next group lies
+      int slot_next = slot + kGroup, page_next = page;
+      if (slot_next == a.page) {
+        slot_next = 0;
+        page_next = page_on;
+        ++index;
+        if (it + 1 < count) page_on = page_at(index + 1);
+      }
+      // scores: 16 keys x ROWS
+      float s[NR][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      for (int r = 0; r < NR; ++r) {
+        s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
+      }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t qa[4];
-          qa[0] = qf[k][0][0];
-          qa[2] = qf[k][0][1];
-          qa[1] = R == 2 ? qf[k][R - 1][0] : 0u;
-          qa[3] = R == 2 ? qf[k][R - 1][1] : 0u;
-          uint32_t b0, b1;
+      for (int k = 0; k < KS; ++k) {
+        uint32_t ka[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
           if constexpr (FP8) {
             const uint4 w = kf[t][k / 4];
             const uint32_t x = k % 4 == 0 ? w.x : k % 4 == 1 ? w.y : k % 4 == 2 ? w.z : w.w;
-            b0 = e4m3x2_to_half2(x);
-            b1 = e4m3x2_to_half2(x >> 16);
+            ka[t] = e4m3x2_to_half2(x);
+            ka[2 + t] = e4m3x2_to_half2(x >> 16);
           } else {
             const uint4 w = kf[t][k / 2];
-            b0 = k % 2 == 0 ? w.x : w.z;
-            b1 = k % 2 == 0 ? w.y : w.w;
+            ka[t] = k % 2 == 0 ? w.x : w.z;
+            ka[2 + t] = k % 2 == 0 ? w.y : w.w;
           }
-          Mma<M>::run(s[t], qa, b0, b1);
         }
+#pragma unroll
+        for (int r = 0; r < NR; ++r) Mma<M>::run(s[r], ka, qf[k][r][0], qf[k][r][1]);
       }
-      float ksc[2][2], vsc[2][2];
+      float ksc[2], vl2[2];
       if constexpr (FP8) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) ksc[t][e] = ks[t][e], vsc[t][e] = vs[t][e];
+        for (int t = 0; t < 2; ++t) ksc[t] = ks[t], vl2[t] = __log2f(vs[t]);
       }
-      if (it + 1 < count) {
-        load_keys(grp + 1, p_next);
-        load_scales(grp + 1, p_next);
-      }
-      // softmax
-      uint32_t pf[4];
-      pf[1] = pf[3] = 0u;
+      if (it + 1 < count) load_keys(grp + 1, page_next, slot_next);
+
+      // weights of keys oct, oct + 8 in rows 2 quad, 2 quad + 1
+      uint32_t pf[NR][2];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float y[2][2], z[2][2];
-        float top = m[r], topv = mv[r];
+      for (int r = 0; r < NR; ++r) {
+        float y[2][2], z[2][2], top[2], topv[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 2; ++e) {
+          top[e] = m[r][e];
+          topv[e] = mv[r][e];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = grp * kGroup + 8 * t + 2 * quad + e;
-            const bool see = j <= last[r] && p_now >= 0;
-            float x = s[t][2 * r + e] * c2[r];
-            if constexpr (FP8) x *= ksc[t][e];
+          for (int t = 0; t < 2; ++t) {
+            float x = s[r][2 * t + e] * c2[r][e];
+            if constexpr (FP8) x *= ksc[t];
+            const bool see = here && grp * kGroup + 8 * t + oct <= last[r][e];
             y[t][e] = see ? x : neg_inf();
-            top = fmaxf(top, y[t][e]);
+            top[e] = fmaxf(top[e], y[t][e]);
             if constexpr (FP8) {
-              z[t][e] = see ? x + __log2f(vsc[t][e]) : neg_inf();
-              topv = fmaxf(topv, z[t][e]);
+              z[t][e] = see ? x + vl2[t] : neg_inf();
+              topv[e] = fmaxf(topv[e], z[t][e]);
             }
           }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float base = top == neg_inf() ? 0.f : top;
-        float basev = base;
-        if constexpr (FP8) {
-          topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
-          topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
-          basev = topv == neg_inf() ? 0.f : topv;
-        } else {
-          topv = top;
+          if constexpr (!FP8) topv[e] = top[e];
         }
-        float sum = 0.f, w[2][2];
+        // the references move for the whole warp, when some weight would pass 2^kLazy (or there was none)
+        bool move = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 2; ++e)
+          move |= (top[e] > m[r][e] && !(top[e] - m[r][e] <= kLazy)) || (topv[e] > mv[r][e] && !(topv[e] - mv[r][e] <= kLazy));
+        if (__any_sync(0xffffffffu, move)) {
+          float shrink[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
+              if constexpr (FP8) topv[e] = fmaxf(topv[e], __shfl_xor_sync(0xffffffffu, topv[e], x));
+            }
+            if constexpr (!FP8) topv[e] = top[e];
+            // a reference of -inf moves with weights and sums that are all zero
+            l[r][e] *= m[r][e] == top[e] ? 1.f : ex2(m[r][e] - top[e]);
+            shrink[e] = mv[r][e] == topv[e] ? 1.f : ex2(mv[r][e] - topv[e]);
+            m[r][e] = top[e];
+            mv[r][e] = topv[e];
+          }
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][r][e] *= shrink[e & 1];
+        }
+        float w[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base = m[r][e] == neg_inf() ? 0.f : m[r][e];
+          const float basev = mv[r][e] == neg_inf() ? 0.f : mv[r][e] - kShift;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
             const float p = ex2(y[t][e] - base);
-            sum += p;
-            if constexpr (FP8) w[t][e] = ex2(z[t][e] - basev + kHalfShift);
-            else if constexpr (kHalf) w[t][e] = ex2(y[t][e] - base + kHalfShift);
+            l[r][e] += p;
+            if constexpr (FP8) w[t][e] = ex2(z[t][e] - basev);
+            else if constexpr (kHalf) w[t][e] = ex2(y[t][e] - basev);
             else w[t][e] = p;
           }
-        l[r] = fmaf(l[r], ex2(m[r] - base), sum);
-        const float shrink = ex2(mv[r] - basev);
-        m[r] = top;
-        if (__any_sync(0xffffffffu, topv != mv[r])) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            o[t][2 * r] *= shrink;
-            o[t][2 * r + 1] *= shrink;
-          }
         }
-        mv[r] = topv;
-        pf[r] = Mma<M>::pack(w[0][0], w[0][1]);
-        pf[2 + r] = Mma<M>::pack(w[1][0], w[1][1]);
+        pf[r][0] = transpose8(Mma<M>::pack(w[0][0], w[0][1]));
+        pf[r][1] = transpose8(Mma<M>::pack(w[1][0], w[1][1]));
       }
-      // P V
+      // V^T P^T: m16 tile t holds elements 2 t, 2 t + 1 of each lane's load
 #pragma unroll
       for (int x = 0; x < VL; ++x) {
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           if constexpr (FP8) {
-            // four columns per word: bytes of the two keys of a fragment side by side
+            // four elements per word: bytes of the two keys of a fragment side by side
             const uint32_t lo0 = __byte_perm(vf[0][x][w], vf[1][x][w], 0x5140), hi0 = __byte_perm(vf[0][x][w], vf[1][x][w], 0x7362);
             const uint32_t lo1 = __byte_perm(vf[2][x][w], vf[3][x][w], 0x5140), hi1 = __byte_perm(vf[2][x][w], vf[3][x][w], 0x7362);
-            const int t = x * VE + 4 * w;
-            Mma<M>::run(o[t], pf, e4m3x2_to_half2(lo0), e4m3x2_to_half2(lo1));
-            Mma<M>::run(o[t + 1], pf, e4m3x2_to_half2(lo0 >> 16), e4m3x2_to_half2(lo1 >> 16));
-            Mma<M>::run(o[t + 2], pf, e4m3x2_to_half2(hi0), e4m3x2_to_half2(hi1));
-            Mma<M>::run(o[t + 3], pf, e4m3x2_to_half2(hi0 >> 16), e4m3x2_to_half2(hi1 >> 16));
+            const int t = x * VE / 2 + 2 * w;
+            const uint32_t v0[4] = {e4m3x2_to_half2(lo0), e4m3x2_to_half2(lo0 >> 16), e4m3x2_to_half2(lo1), e4m3x2_to_half2(lo1 >> 16)};
+            const uint32_t v1[4] = {e4m3x2_to_half2(hi0), e4m3x2_to_half2(hi0 >> 16), e4m3x2_to_half2(hi1), e4m3x2_to_half2(hi1 >> 16)};
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              Mma<M>::run(o[t][r], v0, pf[r][0], pf[r][1]);
+              Mma<M>::run(o[t + 1][r], v1, pf[r][0], pf[r][1]);
+            }
           } else {
-            const int t = x * VE + 2 * w;
-            Mma<M>::run(o[t], pf, __byte_perm(vf[0][x][w], vf[1][x][w], 0x5410),
-                        __byte_perm(vf[2][x][w], vf[3][x][w], 0x5410));
-            Mma<M>::run(o[t + 1], pf, __byte_perm(vf[0][x][w], vf[1][x][w], 0x7632),
-                        __byte_perm(vf[2][x][w], vf[3][x][w], 0x7632));
+            const int t = x * VE / 2 + w;
+            const uint32_t v0[4] = {__byte_perm(vf[0][x][w], vf[1][x][w], 0x5410), __byte_perm(vf[0][x][w], vf[1][x][w], 0x7632),
+                                    __byte_perm(vf[2][x][w], vf[3][x][w], 0x5410), __byte_perm(vf[2][x][w], vf[3][x][w], 0x7632)};
+#pragma unroll
+            for (int r = 0; r < NR; ++r) Mma<M>::run(o[t][r], v0, pf[r][0], pf[r][1]);
           }
         }
       }
-      if (it + 1 < count) load_values(grp + 1, p_next);
-      p_now = p_next;
-      p_next = p_after;
+      if (it + 1 < count) load_values(grp + 1, page_next, slot_next);
+      page = page_next;
+      slot = slot_next;
     }
 
     // this run's share of the segment
     const bool whole = count == g.groups;
-    const int64_t slot = 2 * static_cast<int64_t>(worker) + (first ? 0 : 1);
+    const int64_t part = 2 * static_cast<int64_t>(worker) + (first ? 0 : 1);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float sum = l[r];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int i = g.tile * ROWS + oct + 8 * r;
-      const int tok = i / group;
-      if (tok >= g.rows) continue;
-      // column VE (8 x) + VE (2 quad + e) + j of n8 tile VE x + j
-      if (whole) {
-        float mul = 0.f;
-        if (sum > 0.f || sum != sum) mul = __fdividef(ex2((FP8 ? mv[r] - m[r] : 0.f) - (kHalf ? kHalfShift : 0.f)), sum);
-        T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (g.hk * group + i - tok * group) * a.o_sH;
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int x = 0; x < VL; ++x)
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[r][e];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 8 * VE * x + VE * (2 * quad + e);
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const int row = 8 * r + 2 * quad + e;
+        const int i = g.tile * ROWS + row, tok = i / group;
+        if (tok >= g.rows) continue;
+        if (whole) {
+          float mul = 0.f;
+          if (sum > 0.f || sum != sum) mul = __fdividef(ex2((FP8 ? mv[r][e] - m[r][e] : 0.f) - kShift), sum);
+          T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (g.hk * group + i - tok * group) * a.o_sH;
+#pragma unroll
+          for (int x = 0; x < VL; ++x) {
+            const int c = 8 * VE * x + VE * oct;
             if (c < a.d) {
 #pragma unroll
-              for (int j = 0; j < VE; j += 8) {
+              for (int j = 0; j < VE / 2; j += 4) {
                 uint4 w;
                 uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
                 for (int y = 0; y < 4; ++y)
-                  wp[y] = Mma<T>::pack(o[VE * x + j + 2 * y][2 * r + e] * mul, o[VE * x + j + 2 * y + 1][2 * r + e] * mul);
-                *reinterpret_cast<uint4*>(out + c + j) = w;
+                  wp[y] = Mma<T>::pack(o[x * VE / 2 + j + y][r][e] * mul, o[x * VE / 2 + j + y][r][2 + e] * mul);
+                *reinterpret_cast<uint4*>(out + c + 2 * j) = w;
               }
             }
           }
-      } else {
-        float* po = a.part_o + (slot * kPartRows + oct + 8 * r) * DP;
+        } else {
+          float* po = a.part_o + (part * kPartRows + row) * DP;
 #pragma unroll
-        for (int x = 0; x < VL; ++x)
+          for (int x = 0; x < VL; ++x)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 8 * VE * x + VE * (2 * quad + e);
-#pragma unroll
-            for (int j = 0; j < VE; j += 4)
-              *reinterpret_cast<float4*>(po + c + j) =
-                  make_float4(o[VE * x + j][2 * r + e], o[VE * x + j + 1][2 * r + e], o[VE * x + j + 2][2 * r + e],
-                              o[VE * x + j + 3][2 * r + e]);
-          }
-        if (quad == 0)
-          *reinterpret_cast<float4*>(a.part_ml + (slot * kPartRows + oct + 8 * r) * 4) =
-              make_float4(m[r], sum, mv[r], 0.f);
+            for (int j = 0; j < VE / 2; j += 2) {
+              const int t = x * VE / 2 + j;
+              *reinterpret_cast<float4*>(po + 8 * VE * x + VE * oct + 2 * j) =
+                  make_float4(o[t][r][e], o[t][r][2 + e], o[t + 1][r][e], o[t + 1][r][2 + e]);
+            }
+          if (oct == 0)
+            *reinterpret_cast<float4*>(a.part_ml + (part * kPartRows + row) * 4) = make_float4(m[r][e], sum, mv[r][e], 0.f);
+        }
       }
-    }
     u += count;
     first = false;
   }

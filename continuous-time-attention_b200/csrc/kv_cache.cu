@@ -9,8 +9,8 @@
 // by s in 32 bits and rounds once to the tensor's type.
 //
 // Bound by HBM: 2 d bytes read and d + 4 (2 d) written per row.  Each lane
-// moves 16 bytes of the 16-bit row; kRowsPerGroup rows per group of lanes are
-// in flight together.
+// moves 16 bytes of the 16-bit row; kHeads rows per group of lanes are in flight
+// together.
 #include "attn_common.cuh"
 
 namespace cta {
@@ -22,7 +22,7 @@ namespace {
 constexpr float kE4m3Max = 448.f;
 constexpr float kLeastMax = 7.888609052210118e-31f;  // 2^-100
 constexpr int kThreads = 256;
-constexpr int kRowsPerGroup = 4;
+constexpr int kHeads = 4;  // rows of a token per group of lanes
 
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
   uint16_t lo, hi;
@@ -57,59 +57,88 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// GROUP lanes hold one row of at most 8 GROUP elements.  gridDim.y: 0 keys, 1 values.
+// A group of GROUP lanes holds a row of at most 8 GROUP elements and takes
+// kHeads consecutive heads of one token: the slot and its page are found once,
+// the rows' loads are in flight together, and the divisions of all of them are
+// one, each lane doing one row's.  gridDim.y: 0 keys, 1 values.
+struct Place {
+  unsigned t;   // token
+  int h0;       // first head
+  bool any;     // there is such a token
+  int64_t slot;
+};
+template <int GROUP>
+__device__ __forceinline__ Place place(const CacheArgs& a) {
+  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
+  const unsigned blocks = (a.Hk + kHeads - 1) / kHeads;
+  Place p;
+  p.t = group / blocks;
+  p.h0 = static_cast<int>(group - p.t * blocks) * kHeads;
+  p.any = p.t < static_cast<unsigned>(a.T);
+  p.slot = p.any ? __ldg(a.slots + p.t) : -1;
+  return p;
+}
+// past the cache: reported, and treated as padding
+__device__ __forceinline__ bool in_cache(const CacheArgs& a, int64_t slot, bool report) {
+  if (slot >= a.n_slots && report) atomicExch(&g_cache_error, kDevBadIndex);
+  return slot >= 0 && slot < a.n_slots;
+}
+
 template <typename T, int GROUP, bool QUANT>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_constant__ CacheArgs a) {
   const bool second = blockIdx.y != 0;
   const T* in = static_cast<const T*>(second ? a.v_in : a.k_in);
   const int64_t sT = second ? a.v_sT : a.k_sT, sH = second ? a.v_sH : a.k_sH;
   const int64_t cP = second ? a.vc_sP : a.kc_sP, cS = second ? a.vc_sS : a.kc_sS, cH = second ? a.vc_sH : a.kc_sH;
-  void* cache = second ? a.v_cache : a.k_cache;
-  float* scale = second ? a.v_scale : a.k_scale;
-  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
-  const unsigned groups = gridDim.x * (kThreads / GROUP);
-  const int c = (threadIdx.x % GROUP) * 8;
-  const unsigned rows = static_cast<unsigned>(a.T) * a.Hk;  // < 2^30, checked by the caller
-  uint4 x[kRowsPerGroup];
-  int64_t slot[kRowsPerGroup];
+  const int lane = threadIdx.x % GROUP, c = lane * 8;
+  const Place at = place<GROUP>(a);
+  uint4 x[kHeads];
 #pragma unroll
-  for (int i = 0; i < kRowsPerGroup; ++i) {
-    const unsigned r = group + i * groups;
+  for (int i = 0; i < kHeads; ++i) {
     x[i] = make_uint4(0u, 0u, 0u, 0u);
-    slot[i] = -1;
-    if (r < rows) {
-      const unsigned t = r / a.Hk;
-      slot[i] = __ldg(a.slots + t);
-      if (c < a.d) x[i] = __ldg(reinterpret_cast<const uint4*>(in + static_cast<int64_t>(t) * sT + (r - t * a.Hk) * sH + c));
-    }
+    if (at.any && at.h0 + i < a.Hk && c < a.d)
+      x[i] = __ldg(reinterpret_cast<const uint4*>(in + at.t * sT + (at.h0 + i) * sH + c));
   }
+  const bool keep = in_cache(a, at.slot, lane == 0);
+  const unsigned page = static_cast<unsigned>(at.slot) / a.page, slot = static_cast<unsigned>(at.slot) - page * a.page;
+  const int64_t base = page * cP + slot * cS + at.h0 * cH + c;
+  if constexpr (QUANT) {
+    uint8_t* cache = static_cast<uint8_t*>(second ? a.v_cache : a.k_cache);
+    float* scale = second ? a.v_scale : a.k_scale;
+    float m[kHeads];
 #pragma unroll
-  for (int i = 0; i < kRowsPerGroup; ++i) {
-    const unsigned r = group + i * groups;
-    const int h = r % a.Hk;
-    const bool bad = slot[i] >= a.n_slots;
-    if (bad && c == 0) atomicExch(&g_cache_error, kDevBadIndex);
-    const bool keep = slot[i] >= 0 && !bad;  // a negative slot is padding
-    const int64_t p = static_cast<unsigned>(slot[i]) / a.page, s = slot[i] - p * a.page;  // n_slots < 2^31
-    if constexpr (QUANT) {
+    for (int i = 0; i < kHeads; ++i) {
       float f[8];
       unpack8<T>(x[i], f);
-      float m = kLeastMax;
+      m[i] = kLeastMax;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(f[e]));
+      for (int e = 0; e < 8; ++e) m[i] = fmaxf(m[i], fabsf(f[e]));
 #pragma unroll
-      for (int o = 1; o < GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float up = __fdiv_rn(kE4m3Max, m);
-      if (keep && c < a.d) {
-        uint2 code;
-        code.x = to_e4m3x4(f[0] * up, f[1] * up, f[2] * up, f[3] * up);
-        code.y = to_e4m3x4(f[4] * up, f[5] * up, f[6] * up, f[7] * up);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + p * cP + s * cS + h * cH + c) = code;
-        if (c == 0) scale[(p * a.Hk + h) * a.page + s] = __fdiv_rn(m, kE4m3Max);
-      }
-    } else if (keep && c < a.d) {
-      *reinterpret_cast<uint4*>(static_cast<T*>(cache) + p * cP + s * cS + h * cH + c) = x[i];
+      for (int o = 1; o < GROUP; o <<= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
     }
+    // lane i of the first kHeads: 448 / m[i], lane kHeads + i: m[i] / 448
+    float mine = m[0];
+#pragma unroll
+    for (int i = 1; i < kHeads; ++i) mine = (lane % kHeads) == i ? m[i] : mine;
+    const bool up = (lane / kHeads) % 2 == 0;
+    const float ratio = __fdiv_rn(up ? kE4m3Max : mine, up ? mine : kE4m3Max);
+    if (keep && lane >= kHeads && lane < 2 * kHeads && at.h0 + lane - kHeads < a.Hk)
+      scale[(static_cast<int64_t>(page) * a.Hk + at.h0 + lane - kHeads) * a.page + slot] = ratio;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      const float r = __shfl_sync(0xffffffffu, ratio, i, GROUP);
+      float f[8];
+      unpack8<T>(x[i], f);
+      uint2 code;
+      code.x = to_e4m3x4(f[0] * r, f[1] * r, f[2] * r, f[3] * r);
+      code.y = to_e4m3x4(f[4] * r, f[5] * r, f[6] * r, f[7] * r);
+      if (keep && c < a.d && at.h0 + i < a.Hk) *reinterpret_cast<uint2*>(cache + base + i * cH) = code;
+    }
+  } else {
+    T* cache = static_cast<T*>(second ? a.v_cache : a.k_cache);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (keep && c < a.d && at.h0 + i < a.Hk) *reinterpret_cast<uint4*>(cache + base + i * cH) = x[i];
   }
 }
 
@@ -119,44 +148,31 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   T* out = static_cast<T*>(second ? a.v_out : a.k_out);
   const int64_t sT = second ? a.v_sT : a.k_sT, sH = second ? a.v_sH : a.k_sH;
   const int64_t cP = second ? a.vc_sP : a.kc_sP, cS = second ? a.vc_sS : a.kc_sS, cH = second ? a.vc_sH : a.kc_sH;
-  const void* cache = second ? a.v_cache : a.k_cache;
-  const float* scale = second ? a.v_scale : a.k_scale;
-  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
-  const unsigned groups = gridDim.x * (kThreads / GROUP);
-  const int c = (threadIdx.x % GROUP) * 8;
-  if (c >= a.d) return;
-  const unsigned rows = static_cast<unsigned>(a.T) * a.Hk;  // < 2^30, checked by the caller
-  uint4 x[kRowsPerGroup];
-  float mul[kRowsPerGroup];
+  const int lane = threadIdx.x % GROUP, c = lane * 8;
+  const Place at = place<GROUP>(a);
+  if (!at.any || c >= a.d) return;
+  const bool have = in_cache(a, at.slot, lane == 0);
+  const unsigned page = static_cast<unsigned>(at.slot) / a.page, slot = static_cast<unsigned>(at.slot) - page * a.page;
+  const int64_t base = page * cP + slot * cS + at.h0 * cH + c;
+  uint4 x[kHeads];
+  float mul[kHeads];
 #pragma unroll
-  for (int i = 0; i < kRowsPerGroup; ++i) {
-    const unsigned r = group + i * groups;
+  for (int i = 0; i < kHeads; ++i) {
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     mul[i] = 0.f;
-    if (r >= rows) continue;
-    const unsigned t = r / a.Hk;
-    const int64_t slot = __ldg(a.slots + t);
-    const int h = r - t * a.Hk;
-    if (slot >= a.n_slots) {
-      if (c == 0) atomicExch(&g_cache_error, kDevBadIndex);
-    } else if (slot >= 0) {
-      const int64_t p = static_cast<unsigned>(slot) / a.page, s = slot - p * a.page;
-      const int64_t at = p * cP + s * cS + h * cH + c;
-      if constexpr (QUANT) {
-        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(cache) + at);
-        x[i].x = w.x;
-        x[i].y = w.y;
-        mul[i] = scale[(p * a.Hk + h) * a.page + s];
-      } else {
-        x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(cache) + at);
-      }
+    if (!have || at.h0 + i >= a.Hk) continue;
+    if constexpr (QUANT) {
+      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(second ? a.v_cache : a.k_cache) + base + i * cH);
+      x[i].x = w.x;
+      x[i].y = w.y;
+      mul[i] = (second ? a.v_scale : a.k_scale)[(static_cast<int64_t>(page) * a.Hk + at.h0 + i) * a.page + slot];
+    } else {
+      x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(second ? a.v_cache : a.k_cache) + base + i * cH);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRowsPerGroup; ++i) {
-    const unsigned r = group + i * groups;
-    if (r >= rows) continue;
-    const unsigned t = r / a.Hk;
+  for (int i = 0; i < kHeads; ++i) {
+    if (at.h0 + i >= a.Hk) continue;
     uint4 y = x[i];
     if constexpr (QUANT) {
       float f[8];
@@ -169,14 +185,14 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
       }
       y = pack8<T>(f);
     }
-    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * sT + (r - t * a.Hk) * sH + c) = y;
+    *reinterpret_cast<uint4*>(out + at.t * sT + (at.h0 + i) * sH + c) = y;
   }
 }
 
 template <typename T, int GROUP>
 cudaError_t launch(const CacheArgs& a, bool write, cudaStream_t st) {
-  const int64_t per_cta = static_cast<int64_t>(kThreads / GROUP) * kRowsPerGroup;
-  const int64_t ctas = (a.T * a.Hk + per_cta - 1) / per_cta;
+  const int64_t groups = a.T * ((a.Hk + kHeads - 1) / kHeads);
+  const int64_t ctas = (groups + kThreads / GROUP - 1) / (kThreads / GROUP);
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(ctas), 2u);
   if (write) {
