@@ -17,7 +17,25 @@ __device__ __forceinline__ void dealloc(uint32_t addr, uint32_t cols) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for this thread's tensor-memory loads.  The registers they fill pass
+// through an empty statement behind the wait, so that no use of them can be
+// scheduled before it: to the compiler a load's result is there at once.
+__device__ __forceinline__ void arrived(uint32_t (&r)[16]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+__device__ __forceinline__ void arrived(uint32_t (&r)[32]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+               "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+               "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+               "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]));
+  asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+template <typename... R>
+__device__ __forceinline__ void wait_ld(R&... r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  (arrived(r), ...);
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // the barrier completes one arrival when all MMAs issued so far by this thread are done
 __device__ __forceinline__ void commit(uint64_t* bar) {
@@ -35,6 +53,14 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
@@ -110,16 +136,16 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t a_ha
            accumulate || k > 0);
   }
 }
-// C[128 x N] (+)= A[tmem, 128 x 128] B[128 x N], B MN-major (rows are the
-// contraction index), its 64-column blocks b_half bytes apart.  The second half
-// of A's contraction index starts HALF tensor-memory columns after the first
-// (32 when A is dense).  One thread.
-template <int HALF = 32>
+// C[128 x N] (+)= A[tmem, 128 x KEYS] B[KEYS x N], B MN-major (rows are the
+// contraction index), its 64-column blocks b_half bytes apart.  The second 64 of
+// A's contraction index start HALF tensor-memory columns after the first.  One
+// thread.
+template <int KEYS, int HALF = 32>
 __device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t b_half, uint32_t id,
                                            bool accumulate) {
   const uint64_t base = desc_base(b_half);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < KEYS / 16; ++k)
     mma_ts(d, a + 8 * (k & 3) + HALF * (k >> 2), desc(base, b + k * 2048), id, accumulate || k > 0);
 }
 
@@ -163,6 +189,50 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+
+// Asks for the index of a CTA of this grid that has not started yet, which then
+// never starts: a running CTA goes on with its work instead of leaving the SM.
+// 16 bytes arrive at `resp` on the barrier.
+__device__ __forceinline__ void steal(void* resp, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_addr(resp)),
+               "r"(smem_addr(bar))
+               : "memory");
+}
+// the index, or -1 when every CTA has started
+__device__ __forceinline__ int stolen(const void* resp) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\tld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_addr(resp))
+      : "memory");
+  fence_proxy_async_smem();  // the next answer overwrites it
+  return ok ? static_cast<int>(x) : -1;
+}
+
+// named barrier of `threads` threads, and the same with an OR of their votes
+__device__ __forceinline__ void sync_of(int id, int threads) {
+  asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool any_of(int id, int threads, bool vote) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred.aligned q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(vote))
+      : "memory");
+  return r != 0;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <typename T>

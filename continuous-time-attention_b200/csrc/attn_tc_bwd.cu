@@ -56,7 +56,7 @@ __device__ __forceinline__ void store_grad(uint32_t addr, T* out, int d, float m
     uint32_t o[32];
     if (any) {
       tc::ld32(addr + 32 * c, o);
-      tc::wait_ld();
+      tc::wait_ld(o);
     } else {
 #pragma unroll
       for (int e = 0; e < 32; ++e) o[e] = 0u;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && mbar_wait_bounded(&bars.ds_full, j & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<64>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), L::kHalf, id_o, j > 0);
+        tc::product_tn<128, 64>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), L::kHalf, id_o, j > 0);
         tc::commit(&bars.kv_empty[(2 * j) % NS]);
         if (j + 1 == steps) tc::commit(&bars.done);
       }
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t s[2][32], dp[2][32];
       tc::ld32(s_addr, s[0]);
       tc::ld32(s_addr + 32, s[1]);
-      tc::wait_ld();
+      tc::wait_ld(s[0], s[1]);
       const int j0 = (j_lo + j) * kRows + half * 64;
       uint32_t w[4];
       key_words(j, w);
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after();
       tc::ld32(t_dp + lanes + half * 64, dp[0]);
       tc::ld32(t_dp + lanes + half * 64 + 32, dp[1]);
-      tc::wait_ld();
+      tc::wait_ld(dp[0], dp[1]);
       tc::fence_before();
       tc::arrive(&bars.dp_read);
       const bool whole = tc::all_set(w) && !none && (!a.causal || j0 + 63 <= t.first + (warp & 3) * 32 / f.pack);
@@ -473,13 +473,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < steps && ok; ++s) {
       ok = mbar_wait_bounded(&bars.p_full, s & 1);
       tc::fence_after();
-      if (ok && leader) tc::product_tn<64>(t_dv, tmem, q_addr(s) + L::kTile, L::kHalf, id_o, s > 0);
+      if (ok && leader) tc::product_tn<128, 64>(t_dv, tmem, q_addr(s) + L::kTile, L::kHalf, id_o, s > 0);
       __syncwarp();
       if (s + 1 < steps) scores(s + 1);
       ok = ok && mbar_wait_bounded(&bars.ds_full, s & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<64>(t_dk, t_dp, q_addr(s), L::kHalf, id_o, s > 0);
+        tc::product_tn<128, 64>(t_dk, t_dp, q_addr(s), L::kHalf, id_o, s > 0);
         tc::commit(&bars.q_empty[s % NS]);
         if (s + 1 == steps) tc::commit(&bars.done);
       }
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t p[2][32];
       tc::ld32(s_addr, p[0]);
       tc::ld32(s_addr + 32, p[1]);
-      tc::wait_ld();
+      tc::wait_ld(p[0], p[1]);
       // causal: the first row of this half that sees the key; 64 = none
       int from = 0;
       if (a.causal) from = min(max((key - first_of(s)) * f.pack - half * 64, 0), 64);
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 2; ++c) {
         uint32_t d[32], w[16];
         tc::ld32(d_addr + 32 * c, d);
-        tc::wait_ld();
+        tc::wait_ld(d);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 b = dl[(32 * c + e) / 4];

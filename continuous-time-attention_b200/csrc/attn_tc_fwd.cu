@@ -8,12 +8,18 @@
 // are read for all of them at once.
 //
 //   warps 0-3, 4-7   softmax of tile 0 and 1: a thread holds one row
-//   warp 8           issues the MMAs        warp 9   issues the TMA loads
+//   warp 8   issues the MMAs    warp 9   issues the TMA loads    warp 10   finds the work
 //
-// Per 128 keys and tile:  S = Q K^T into 128 columns of tensor memory; each
-// softmax thread reads its row, P = exp2(c S - m) goes back as 16-bit into the
-// same columns; O += P V with P read from tensor memory as the A operand.  While
-// one tile's softmax runs, the other tile's products do.  The running maximum
+// The grid has a CTA for each pair of tiles; a CTA that has finished one takes
+// over another that has not started (cluster launch control), so that the loads
+// and the first scores of the next pair run under the last weights and the
+// output of this one, and the setup is paid once per SM.
+//
+// Per 64 keys and tile:  S = Q K^T into one of two buffers of 64 tensor-memory
+// columns; each softmax thread reads its row, P = exp2(c S - m) goes back as
+// 16-bit into the same columns; O += P V with P read from tensor memory as the A
+// operand.  With two buffers the next scores are ready when a step's weights are
+// done, so the softmax warps never wait for the products.  The running maximum
 // that P is relative to moves only when it has grown by more than 2^8, so O is
 // rescaled (tensor memory -> registers -> tensor memory) a few times per row and
 // not per tile; P stays below 2^8, the sum and O are fp32, and the quotient is
@@ -32,7 +38,8 @@ __device__ int g_tc_fwd_error;
 
 namespace {
 
-constexpr int kThreads = 384;  // three warpgroups; warps 10 and 11 idle
+constexpr int kThreads = 640;  // five warpgroups; warp 19 idles
+constexpr int kSoftmaxWarps = 16;
 constexpr int kRows = 128;  // rows of a tile, and keys of a step
 constexpr float kLazy = 8.f;
 
@@ -57,7 +64,17 @@ struct Layout {
 };
 
 struct Bars {
-  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2];
+  uint64_t item_full, item_taken, answer;
+};
+
+// One piece of work: two row tiles of one block of heads.
+struct Item {
+  SeqTile t;
+  int h0, hk;  // first query head, key/value head
+  int n;       // keys of the sequence
+  int lo, hi;  // first and one past the last that may be valid
+  bool last;   // there is no more work
 };
 
 template <typename T, int DP, bool PAGED>
@@ -69,31 +86,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
-  __shared__ SeqTile s_tile;
+  __shared__ Item s_item;
+  __shared__ __align__(16) uint4 s_answer;
+  __shared__ float s_max[2][2][kRows], s_sum[2][2][kRows];  // [tile][half of the keys][row]
   __shared__ uint32_t s_boxes[16];  // paged: which boxes of a key tile were loaded
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  const int blocks = a.H / f.pack;
-  const int hb = blockIdx.x % blocks;
-  const int h0 = hb * f.pack, hk = h0 / (a.H / a.Hk);
 
-  if (warp == 0) {
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, 2 * f.tile_tokens, a.causal);
-    if (lane == 0) s_tile = x;
-  } else if (warp == 8) {
+  if (warp == kSoftmaxWarps) {
     tc::alloc(&s_tmem, 512);
-  } else if (warp == 9 && lane == 0) {
+  } else if (warp == kSoftmaxWarps + 1 && lane == 0) {
     mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_empty, 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.kv_full[i], 1);
       mbar_init(&bars.kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], kRows);
+      mbar_init(&bars.p_full[i], 2 * kRows);
       mbar_init(&bars.o_full[i], 1);
     }
+    mbar_init(&bars.item_full, 1);
+    mbar_init(&bars.item_taken, kSoftmaxWarps + 2);
+    mbar_init(&bars.answer, 1);
     fence_mbar_init();
     prefetch_tmap(&qmap);
     prefetch_tmap(&kmap);
@@ -102,82 +119,141 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const SeqTile t = s_tile;
   const uint32_t tmem = s_tmem;
 
-  // keys: [lo, hi) of the sequence, n of them, row i sees j <= i + shift when causal
-  int n = t.n, lo = 0, hi = t.n;
-  bool bad_length = false;
-  if constexpr (PAGED) {
-    if (t.first < t.n) {
-      n = __ldg(f.seq_lens + t.seq);
-      const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
-      bad_length = n < 0 || n > most;
-      n = n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(n), most));
+  // the it-th piece of work, for the warps that work on it; false: a wait ran out
+  auto read_item = [&](int it, Item& x) -> bool {
+    if (!mbar_wait_bounded(&bars.item_full, it & 1)) return false;
+    x = s_item;
+    __syncwarp();
+    return true;
+  };
+  auto taken = [&] {
+    if (lane == 0) tc::arrive(&bars.item_taken);
+  };
+  auto take = [&](int it, Item& x) -> bool {
+    if (!read_item(it, x)) return false;
+    taken();
+    return true;
+  };
+  // steps of 128 keys of the two tiles; j_lo: the first
+  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j_lo, int& shift) {
+    shift = PAGED ? x.n - x.t.n : 0;
+    j_lo = x.lo / kRows;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      first[i] = x.t.first + i * f.tile_tokens;
+      int end = x.hi;
+      if (a.causal) end = min(end, min(first[i] + f.tile_tokens, x.t.n) + shift);
+      steps[i] = first[i] < x.t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
     }
-    hi = n;
-  } else {
-    mask_range(a, t.batch, t.n, lo, hi);
-  }
-  const int shift = PAGED ? n - t.n : 0;
-  const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
-  const int j_lo = lo / kRows;
-  int steps[2], first[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    first[i] = t.first + i * f.tile_tokens;
-    int end = hi;
-    if (a.causal) end = min(end, min(first[i] + f.tile_tokens, t.n) + shift);
-    steps[i] = first[i] < t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
-  }
-  const int all = max(steps[0], steps[1]);
-
-  // bit c of word w: key 32 w + c of tile j is one of the sequence's and valid
-  auto key_words = [&](int j, uint32_t (&w)[4]) {
-    const int j0 = (j_lo + j) * kRows;
+  };
+  // bit c of word i: key 32 i + c of the tile at j0 is one of the sequence's and valid; `kt`: running number of the tile
+  auto key_words = [&](int n, const uint32_t* mask, int j0, int kt, uint32_t (&w)[4]) {
     tc::first_bits(n - j0, w);
+    if constexpr (PAGED) {
+      const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&s_boxes[kt & 15]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (mask != nullptr && n - j0 - 32 * i > 0) w[i] &= __ldg(mask + kMaskHead + (j0 >> 5) + i);
-      if constexpr (PAGED) {
-        const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&s_boxes[j & 15]);
+      for (int i = 0; i < 8; ++i)
+        if (!((boxes >> i) & 1u)) w[i >> 1] &= (i & 1) == 0 ? 0xffff0000u : 0x0000ffffu;
+    } else if (mask != nullptr) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          if (!((boxes >> (2 * i + b)) & 1u)) w[i] &= b == 0 ? 0xffff0000u : 0x0000ffffu;
-      }
+      for (int i = 0; i < 4; ++i)
+        if (n - j0 - 32 * i > 0) w[i] &= __ldg(mask + (j0 >> 5) + i);
     }
   };
 
-  // 384 threads x 168 registers at launch = 2 x 128 x 208 + 128 x 88
-  if (warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-   if (warp == 9) {
+  // 640 threads x 96 registers at launch = 4 x 128 x 104 + 128 x 64
+  if (warp >= kSoftmaxWarps) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+   if (warp == kSoftmaxWarps + 2) {
+    // ---------------- which work ----------------
+    // The grid has a CTA per piece of work; a CTA that is done goes on with one that has not started.
+    const int blocks = a.H / f.pack;
+    bool ok = true;
+    int id = blockIdx.x;
+    for (int it = 0; ok; ++it) {
+      if (it > 0) {
+        // Every warp has begun the piece before, and its loads are all on their way.  Asked for
+        // earlier, pieces of different lengths would be dealt out before it is known who is free:
+        // 4 chunks over 1500 to 8192 keys took 315 us instead of 200.
+        ok = mbar_wait_bounded(&bars.item_taken, (it - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.answer, 16);
+          tc::steal(&s_answer, &bars.answer);
+        }
+        ok = mbar_wait_bounded(&bars.answer, (it - 1) & 1);
+        if (!ok) break;
+        id = tc::stolen(&s_answer);
+      }
+      Item x = {};
+      x.last = id < 0;
+      if (id >= 0) {
+        const int hb = id % blocks;
+        x.h0 = hb * f.pack;
+        x.hk = x.h0 / (a.H / a.Hk);
+        x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal);
+        x.n = x.hi = x.t.n;
+        if constexpr (PAGED) {
+          if (x.t.first < x.t.n) {
+            x.n = __ldg(f.seq_lens + x.t.seq);
+            const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
+            if ((x.n < 0 || x.n > most) && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
+            x.n = x.n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(x.n), most));
+          }
+          x.hi = x.n;
+        } else {
+          mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
+        }
+      }
+      if (lane == 0) {
+        s_item = x;
+        tc::arrive(&bars.item_full);
+      }
+      __syncwarp();
+      if (id < 0) break;
+    }
+    if (!ok && lane == 0) atomicExch(&g_tc_fwd_error, kDevTimeout);
+   } else if (warp == kSoftmaxWarps + 1) {
     // ---------------- loads ----------------
     bool ok = true;
-    int issued = 0;
-    if (bad_length && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
-    if (all > 0) {
+    int kv = 0, nq = 0;  // tiles loaded so far, Q loads so far
+    for (int it = 0; ok; ++it) {
+      Item x;
+      ok = read_item(it, x);
+      if (!ok || x.last) break;
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
+      const int all = max(steps[0], steps[1]);
+      if (all == 0) {
+        taken();
+        continue;
+      }
+      if (nq > 0) ok = mbar_wait_bounded(&bars.q_empty, (nq - 1) & 1);
+      if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
         for (int i = 0; i < 2; ++i)
           for (int c = 0; c < DP / 64; ++c)
-            tc::tma_load_4d(smem + i * L::kTile + c * L::kHalf, &qmap, &bars.q_full, 64 * c, h0,
-                            static_cast<int>(t.row0) + first[i], t.batch);
+            tc::tma_load_4d(smem + i * L::kTile + c * L::kHalf, &qmap, &bars.q_full, 64 * c, x.h0,
+                            static_cast<int>(x.t.row0) + first[i], x.t.batch);
       }
-      for (int x = 0; x < 2 * all && ok; ++x) {
-        const int stage = x % NS;
-        if (x >= NS) ok = mbar_wait_bounded(&bars.kv_empty[stage], ((x / NS) - 1) & 1);
+      ++nq;
+      for (int y = 0; y < 2 * all; ++y) {
+        const int stage = kv % NS;
+        if (kv >= NS) ok = mbar_wait_bounded(&bars.kv_empty[stage], ((kv / NS) - 1) & 1);
         if (!ok) break;
-        const CUtensorMap* map = (x & 1) ? &vmap : &kmap;
+        const CUtensorMap* map = (y & 1) ? &vmap : &kmap;
         const uint32_t dst = smem + (2 + stage) * L::kTile;
-        const int j0 = (j_lo + (x >> 1)) * kRows;
+        const int j0 = (j_lo + (y >> 1)) * kRows;
         if constexpr (PAGED) {
           // one lane per box; a box outside the sequence or the cache is left out
           const int boxes = kRows / f.box;
           const int key = j0 + lane * f.box;
           int page = -1;
-          if (lane < boxes && key < n) {
-            page = __ldg(f.table + t.seq * f.table_sB + key / f.page);
+          if (lane < boxes && key < x.n) {
+            page = __ldg(f.table + x.t.seq * f.table_sB + key / f.page);
             if (page < 0 || page >= f.n_pages) {
               atomicExch(&g_tc_fwd_error, kDevBadIndex);
               page = -1;
@@ -190,219 +266,276 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int per = f.box / 16;
             for (int b = 0; b < boxes; ++b)
               if ((got >> b) & 1u) bits |= ((1u << per) - 1u) << (b * per);
-            *reinterpret_cast<volatile uint32_t*>(&s_boxes[(x >> 1) & 15]) = bits;
+            *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kv >> 1) & 15]) = bits;
             mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64));
           }
           __syncwarp();
           if (page >= 0)
             for (int c = 0; c < DP / 64; ++c)
-              tc::tma_load_4d(dst + c * L::kHalf + lane * f.box * 128, map, &bars.kv_full[stage], 64 * c, hk,
+              tc::tma_load_4d(dst + c * L::kHalf + lane * f.box * 128, map, &bars.kv_full[stage], 64 * c, x.hk,
                               key % f.page, page);
         } else if (lane == 0) {
           mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
           for (int c = 0; c < DP / 64; ++c)
-            tc::tma_load_4d(dst + c * L::kHalf, map, &bars.kv_full[stage], 64 * c, hk,
-                            static_cast<int>(t.row0) + j0, t.batch);
+            tc::tma_load_4d(dst + c * L::kHalf, map, &bars.kv_full[stage], 64 * c, x.hk,
+                            static_cast<int>(x.t.row0) + j0, x.t.batch);
         }
-        issued = x + 1;
+        ++kv;
       }
-      // nothing may still be in flight when the CTA ends: the MMA warp has waited for all of it unless a wait ran out
-      if (!ok) {
-        atomicExch(&g_tc_fwd_error, kDevTimeout);
-        for (int x = max(0, issued - NS); x < issued; ++x) mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1);
-      }
+      taken();
     }
-  } else if (warp == 8) {
+    // nothing may still be in flight when the CTA ends: the MMA warp has waited for all of it unless a wait ran out
+    if (!ok) {
+      atomicExch(&g_tc_fwd_error, kDevTimeout);
+      for (int y = max(0, kv - NS); y < kv; ++y) mbar_wait_bounded(&bars.kv_full[y % NS], (y / NS) & 1);
+      if (nq > 0) mbar_wait_bounded(&bars.q_full, (nq - 1) & 1);
+    }
+   } else if (warp == kSoftmaxWarps) {
     // ---------------- products ----------------
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
-    bool ok = all == 0 || mbar_wait_bounded(&bars.q_full, 0);
-    auto kv_wait = [&](int x) { ok = ok && mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1); };
-    auto kv_addr = [&](int x) { return smem + (2 + x % NS) * L::kTile; };
-    auto scores = [&](int i, int j) {
-      if (leader) {
-        tc::product_nt<DP>(tmem + i * kRows, smem + i * L::kTile, L::kHalf, kv_addr(2 * j), L::kHalf, id_s);
-        tc::commit(&bars.s_full[i]);
-      }
-    };
-    if (all > 0) {
+    bool ok = true;
+    int kv = 0, nq = 0, ns[2] = {0, 0};  // running numbers: tiles, Q loads, steps of each row tile
+    for (int it = 0; ok; ++it) {
+      Item x;
+      ok = take(it, x);
+      if (!ok || x.last) break;
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
+      const int all = max(steps[0], steps[1]);
+      if (all == 0) continue;
+      ok = mbar_wait_bounded(&bars.q_full, nq & 1);
+      ++nq;
+      const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
+      auto kv_wait = [&](int y) { ok = ok && mbar_wait_bounded(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
+      auto kv_addr = [&](int y) { return smem + (2 + (kv + y) % NS) * L::kTile; };
+      auto scores = [&](int i, int j) {
+        if (leader) {
+          tc::product_nt<DP>(tmem + i * kRows, smem + i * L::kTile, L::kHalf, kv_addr(2 * j), L::kHalf, id_s);
+          tc::commit(&bars.s_full[i]);
+        }
+      };
       kv_wait(0);
       tc::fence_after();
       if (ok) {
         for (int i = 0; i < 2; ++i)
           if (steps[i] > 0) scores(i, 0);
-        if (leader) tc::commit(&bars.kv_empty[0]);
+        if (leader) {
+          tc::commit(&bars.kv_empty[kv % NS]);
+          if (all == 1) tc::commit(&bars.q_empty);
+        }
       }
-    }
-    for (int j = 0; j < all && ok; ++j) {
-      kv_wait(2 * j + 1);
-      if (!ok) break;
-      // values of keys that are not there or not valid may hold anything: a zero weight times NaN is NaN
-      uint32_t w[4];
-      key_words(j, w);
-      if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
-      const bool more = j + 1 < all;
-      for (int i = 0; i < 2 && ok; ++i) {
-        if (j < steps[i]) {
-          ok = mbar_wait_bounded(&bars.p_full[i], j & 1);
-          tc::fence_after();
-          if (ok && leader) {
-            tc::product_tn(tmem + 2 * kRows + i * DP, tmem + i * kRows, kv_addr(2 * j + 1), L::kHalf, id_o, j > 0);
-            if (j + 1 == steps[i]) tc::commit(&bars.o_full[i]);
+      for (int j = 0; j < all && ok; ++j) {
+        kv_wait(2 * j + 1);
+        if (!ok) break;
+        // values of keys that are not there or not valid may hold anything
+        uint32_t w[4];
+        key_words(x.n, mask, (j_lo + j) * kRows, (kv >> 1) + j, w);
+        if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
+        const bool more = j + 1 < all;
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j < steps[i]) {
+            ok = mbar_wait_bounded(&bars.p_full[i], ns[i] & 1);
+            tc::fence_after();
+            if (ok && leader) {
+              tc::product_tn<128, 64>(tmem + 2 * kRows + i * DP, tmem + i * kRows, kv_addr(2 * j + 1), L::kHalf, id_o,
+                                      j > 0);
+              if (j + 1 == steps[i]) tc::commit(&bars.o_full[i]);
+            }
+            __syncwarp();
+            ++ns[i];
+          }
+          if (j + 1 < steps[i]) {
+            kv_wait(2 * j + 2);
+            tc::fence_after();
+            if (ok) scores(i, j + 1);
           }
         }
-        if (j + 1 < steps[i]) {
-          kv_wait(2 * j + 2);
-          tc::fence_after();
-          if (ok) scores(i, j + 1);
+        if (ok && leader) {
+          tc::commit(&bars.kv_empty[(kv + 2 * j + 1) % NS]);
+          if (more) tc::commit(&bars.kv_empty[(kv + 2 * j + 2) % NS]);
+          if (j + 2 == all) tc::commit(&bars.q_empty);  // the last scores are on their way
         }
+        __syncwarp();
       }
-      if (ok && leader) {
-        tc::commit(&bars.kv_empty[(2 * j + 1) % NS]);
-        if (more) tc::commit(&bars.kv_empty[(2 * j + 2) % NS]);
-      }
-      __syncwarp();
+      kv += 2 * all;
     }
     if (!ok && lane == 0) atomicExch(&g_tc_fwd_error, kDevTimeout);
    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ---------------- softmax ----------------
-    const int i = warp >> 2;
+    const int i = warp >> 3, half = (warp >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
-    const int tok = first[i] + row / f.pack, h = h0 + row % f.pack;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + i * kRows, o_addr = tmem + lanes + 2 * kRows + i * DP;
+    const uint32_t s_addr = tmem + lanes + i * kRows + half * 64;
+    const uint32_t o_addr = tmem + lanes + 2 * kRows + i * DP + half * (DP / 2);
     const float c2 = a.scale * kLog2e;
-    const int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
-    float m = neg_inf(), sum = 0.f;
     bool ok = true;
-    for (int j = 0; j < steps[i]; ++j) {
-      ok = mbar_wait_bounded(&bars.s_full[i], j & 1);
-      if (!ok) break;
-      tc::fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tc::ld32(s_addr + 32 * c, s[c]);
-      tc::wait_ld();
-      const int j0 = (j_lo + j) * kRows;
-      uint32_t w[4];
-      key_words(j, w);
-      // warp-uniform: does every row of the warp see all 128 keys?
-      const bool whole = tc::all_set(w) &&
-                         (!a.causal || j0 + kRows - 1 <= first[i] + (warp & 3) * 32 / f.pack + shift);
-      if (!whole) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int left = limit - j0 - 32 * c + 1;
-          const uint32_t see = w[c] & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((see >> e) & 1u)) s[c][e] = 0xff800000u;
-        }
+    int ns = 0, no = 0, kt = 0;  // running numbers: steps, outputs, key tiles
+    for (int it = 0; ok; ++it) {
+      Item x;
+      ok = take(it, x);
+      if (!ok || x.last) break;
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
+      const int mine = i == 0 ? first[0] : first[1], count = i == 0 ? steps[0] : steps[1];
+      const int all = max(steps[0], steps[1]);
+      if (!PAGED && a.cu != nullptr && a.zero_tail && warp < 4 && x.t.n == 0) {
+        // a tile behind the last sequence clears rows there
+        for (int64_t r = x.t.row0 + x.t.tail_index; r < a.L; r += x.t.tail_count)
+          for (int y = threadIdx.x; y < a.d * f.pack; y += kRows)
+            static_cast<T*>(a.o)[r * a.os.t + (x.h0 + y / a.d) * a.os.h + y % a.d] = Elem<T>::from_f(0.f);
       }
-      float top[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        top[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) top[c] = fmaxf(top[c], __uint_as_float(s[c][e]));
+      if (mine >= x.t.n) {
+        kt += all;
+        continue;
       }
-      const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-      // move the reference when it has grown by more than kLazy (or there was none)
-      const bool move = now > m && !((now - m) * c2 <= kLazy);
-      if (__any_sync(0xffffffffu, move)) {
-        const float shrink = move ? ex2((m - now) * c2) : 1.f;
-        if (move) {
-          sum *= shrink;
-          m = now;
-        }
-        if (j > 0) {
-          // the scores' barrier also covers the previous O += P V
+      const int n = x.n;
+      const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
+      const int tok = mine + row / f.pack, h = x.h0 + row % f.pack;
+      const bool live = tok < x.t.n;
+      const int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
+      const int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
+      T* out = static_cast<T*>(a.o) + x.t.batch * a.os.b + (x.t.row0 + tok) * a.os.t + h * a.os.h;
+      float* lse = live && half == 0 && a.lse != nullptr ? a.lse + lse_index(a, x.t, h, tok) : nullptr;
+      float m = neg_inf(), sum = 0.f;
+      for (int j = 0; j < count; ++j, ++ns) {
+        // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
+        // the named barriers below see all their warps.
+        ok = ok && mbar_wait_bounded(&bars.s_full[i], ns & 1);
+        tc::fence_after();
+        const int j0 = (j_lo + j) * kRows;
+        uint32_t s[2][32];
+        tc::ld32(s_addr, s[0]);
+        tc::ld32(s_addr + 32, s[1]);
+        // warp-uniform: every row of the warp sees all keys of the tile
+        bool whole = j0 + kRows <= n && mask == nullptr && (!a.causal || j0 + kRows - 1 <= limit_all);
+        if constexpr (PAGED) whole = whole && *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kt + j) & 15]) == 0xffu;
+        tc::wait_ld(s[0], s[1]);
+        if (!whole) {
+          uint32_t w[4];
+          key_words(n, mask, j0, kt + j, w);
 #pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tc::ld32(o_addr + 32 * c, o);
-            tc::wait_ld();
+          for (int c = 0; c < 2; ++c) {
+            const int left = limit - j0 - 64 * half - 32 * c + 1;
+            const uint32_t see = (half == 0 ? w[c] : w[2 + c]) &
+                                 (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-            tc::st32(o_addr + 32 * c, o);
+            for (int e = 0; e < 32; ++e)
+              if (!((see >> e) & 1u)) s[c][e] = 0xff800000u;
           }
         }
-      }
-      const float base = m == neg_inf() ? 0.f : -m * c2;
-      const float2 c2v = f2(c2), bv = f2(base);
-      float2 part = f2(0.f), part2 = f2(0.f);
+        float t[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t p[16];
+        for (int c = 0; c < 4; ++c) {
+          t[c] = __uint_as_float(s[c >> 1][16 * (c & 1)]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 x = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), c2v, bv);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          if (e & 1) part2 = add2(part2, x);
-          else part = add2(part, x);
-          p[e] = tc::pack2<T>(x.x, x.y);
+          for (int e = 1; e < 15; e += 2)
+            t[c] = tc::max3(t[c], __uint_as_float(s[c >> 1][16 * (c & 1) + e]), __uint_as_float(s[c >> 1][16 * (c & 1) + e + 1]));
+          t[c] = fmaxf(t[c], __uint_as_float(s[c >> 1][16 * (c & 1) + 15]));
         }
-        tc::st16(s_addr + 16 * c, p);
-      }
-      part = add2(part, part2);
-      sum += part.x + part.y;
-      tc::wait_st();
-      tc::fence_before();
-      tc::arrive(&bars.p_full[i]);
-    }
-    const bool live = tok < t.n && row / f.pack < f.tile_tokens;
-    if (ok && steps[i] > 0) ok = mbar_wait_bounded(&bars.o_full[i], 0);
-    tc::fence_after();
-    if (!ok) {
-      if (lane == 0) atomicExch(&g_tc_fwd_error, kDevTimeout);
-    } else if (first[i] < t.n) {
-      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays
-      T* out = static_cast<T*>(a.o) + t.batch * a.os.b + (t.row0 + tok) * a.os.t + h * a.os.h;
+        float top = tc::max3(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]), m);
+        // The reference of a row moves when one of its halves has grown by more than kLazy past it (or
+        // there was none): one barrier with a vote per step, and the halves' maxima only then.
+        if (tc::any_of(1 + i, 2 * kRows, top > m && !((top - m) * c2 <= kLazy))) {
+          s_max[i][half][row] = top;
+          tc::sync_of(1 + i, 2 * kRows);
+          top = fmaxf(top, s_max[i][half ^ 1][row]);
+          const bool move = top > m && !((top - m) * c2 <= kLazy);
+          const float shrink = move ? ex2((m - top) * c2) : 1.f;
+          if (move) {
+            sum *= shrink;
+            m = top;
+          }
+          if (j > 0 && __any_sync(0xffffffffu, move)) {
+            // the scores' barrier also covers the previous O += P V; each half has its half of the columns
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[16];
+              tc::ld16(o_addr + 16 * c, o);
+              tc::wait_ld(o);
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+              tc::st16(o_addr + 16 * c, o);
+            }
+          }
+        }
+        const float base = m == neg_inf() ? 0.f : -m * c2;
+        const float2 c2v = f2(c2), bv = f2(base);
+        float2 part = f2(0.f), part2 = f2(0.f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 y = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), c2v, bv);
+            y.x = ex2(y.x);
+            y.y = ex2(y.y);
+            if (e & 1) part2 = add2(part2, y);
+            else part = add2(part, y);
+            p[e] = tc::pack2<T>(y.x, y.y);
+          }
+          // over this half's own scores: the other half may not have read its yet
+          tc::st16(s_addr + 16 * c, p);
+        }
+        part = add2(part, part2);
+        sum += part.x + part.y;
+        tc::wait_st();
+        tc::fence_before();
+        tc::arrive(&bars.p_full[i]);
+      }
+      kt += all;
+      if (count > 0) {
+        ok = ok && mbar_wait_bounded(&bars.o_full[i], no & 1);
+        ++no;
+        tc::fence_after();
+        s_sum[i][half][row] = sum;
+        if (tc::any_of(1 + i, 2 * kRows, !ok)) {
+          ok = false;
+          break;  // all warps of the tile
+        }
+        sum += s_sum[i][half ^ 1][row];
+      }
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const int col = half * (DP / 2) + 32 * c;
         uint32_t o[32];
-        if (steps[i] > 0) {
+        if (count > 0) {
           tc::ld32(o_addr + 32 * c, o);
-          tc::wait_ld();
+          tc::wait_ld(o);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
-        if (live) {
-          if (f.vec_out) {
+        if (!live) continue;
+        if (f.vec_out) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (32 * c + e < a.d) {
-                uint4 x;
-                uint32_t* xp = reinterpret_cast<uint32_t*>(&x);
+          for (int e = 0; e < 32; e += 8)
+            if (col + e < a.d) {
+              uint4 v;
+              uint32_t* vp = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  xp[y] = tc::pack2<T>(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
-                *reinterpret_cast<uint4*>(out + 32 * c + e) = x;
-              }
-          } else {
+              for (int y = 0; y < 4; ++y)
+                vp[y] = tc::pack2<T>(__uint_as_float(o[e + 2 * y]) * inv, __uint_as_float(o[e + 2 * y + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + col + e) = v;
+            }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e < a.d) out[32 * c + e] = Elem<T>::from_f(__uint_as_float(o[e]) * inv);
-          }
+          for (int e = 0; e < 32; ++e)
+            if (col + e < a.d) out[col + e] = Elem<T>::from_f(__uint_as_float(o[e]) * inv);
         }
       }
-      if (live && a.lse != nullptr)
-        a.lse[lse_index(a, t, h, tok)] = sum == 0.f ? neg_inf() : (m * c2 + log2f(sum)) * kLn2;
-    } else if (!PAGED && a.cu != nullptr && a.zero_tail && i == 0 && t.n == 0) {
-      // a tile behind the last sequence clears rows there
-      for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
-        for (int x = threadIdx.x; x < a.d * f.pack; x += kRows)
-          static_cast<T*>(a.o)[r * a.os.t + (h0 + x / a.d) * a.os.h + x % a.d] = Elem<T>::from_f(0.f);
+      if (lse != nullptr) *lse = sum == 0.f ? neg_inf() : (m * c2 + log2f(sum)) * kLn2;
+      tc::fence_before();  // O has been read before the next piece's first weights are announced
     }
+    if (!ok && lane == 0) atomicExch(&g_tc_fwd_error, kDevTimeout);
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::dealloc(tmem, 512);
+  if (warp == kSoftmaxWarps) tc::dealloc(tmem, 512);
 }
 
 template <typename T, int DP, bool PAGED>
