@@ -90,12 +90,12 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
 //   MN-major (the contraction index counts rows): the 1024 separates groups of 8
 //     rows along the contraction, the leading offset separates the 64-element
 //     blocks of the other index.
-__device__ __forceinline__ uint64_t desc_base(uint32_t lead_bytes) {
-  return (static_cast<uint64_t>((lead_bytes >> 4) & 0x3fff) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc(uint64_t base, uint32_t addr) {
-  return base | static_cast<uint64_t>((addr & 0x3ffff) >> 4);
+// The address and the leading offset make up the low word, the rest is constant:
+// a product's descriptors differ by additions to the low word (address / 16).
+// Built from 64-bit values instead, each MMA took about 80 cycles to issue.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead_bytes) {
+  return ((addr & 0x3ffffu) >> 4) | ((lead_bytes >> 4) << 16);
 }
 
 // kind::f16 instruction descriptor: fp32 accumulator, A and B of type T, M = 128
@@ -107,46 +107,42 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn_major, bool
 }
 
 // D[tmem] (+)= A[smem] B[smem]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate))
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate)), "n"(kDescHigh)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate))
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(static_cast<uint32_t>(accumulate)), "n"(kDescHigh)
       : "memory");
 }
 
-// C[128 x N] (+)= A[128 x DP] B[N x DP]^T, both K-major in shared memory; the
-// 64-column halves of A and B lie a_half and b_half bytes apart.  One thread.
-template <int DP>
-__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t a_half, uint32_t b, uint32_t b_half,
-                                           uint32_t id, bool accumulate = false) {
-  const uint64_t base = desc_base(16);
+// C[128 x N] = A[128 x DP] B[N x DP]^T, both K-major in shared memory; the
+// 64-column halves of A and B lie HALF bytes apart.  One thread.
+template <int DP, int HALF = 16384>
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, uint32_t id) {
+  const uint32_t al = desc_low(a, 16), bl = desc_low(b, 16);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
-    const uint32_t off = (k & 3) * 32;
-    mma_ss(d, desc(base, a + (k >> 2) * a_half + off), desc(base, b + (k >> 2) * b_half + off), id,
-           accumulate || k > 0);
+    const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+    mma_ss(d, al + off, bl + off, id, k > 0);
   }
 }
-// C[128 x N] (+)= A[tmem, 128 x KEYS] B[KEYS x N], B MN-major (rows are the
-// contraction index), its 64-column blocks b_half bytes apart.  The second 64 of
-// A's contraction index start HALF tensor-memory columns after the first.  One
-// thread.
-template <int KEYS, int HALF = 32>
-__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t b_half, uint32_t id,
-                                           bool accumulate) {
-  const uint64_t base = desc_base(b_half);
+// C[128 x N] (+)= A[tmem, 128 x 128] B[128 x N], B MN-major (rows are the
+// contraction index), its 64-column blocks 16 KB apart.  The second 64 of A's
+// contraction index start 64 tensor-memory columns after the first.  One thread.
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accumulate) {
+  const uint32_t bl = desc_low(b, 16384);
 #pragma unroll
-  for (int k = 0; k < KEYS / 16; ++k)
-    mma_ts(d, a + 8 * (k & 3) + HALF * (k >> 2), desc(base, b + k * 2048), id, accumulate || k > 0);
+  for (int k = 0; k < 8; ++k)
+    mma_ts(d, a + 8 * (k & 3) + 64 * (k >> 2), bl + k * (2048 >> 4), id, accumulate || k > 0);
 }
 
 // zero the 128-byte rows of a 128-row tile (HALVES blocks of 64 columns, 16 KB
@@ -181,6 +177,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+// Bounded wait on an mbarrier phase, false after about a second.  The timer is
+// read only when some tries have failed: reading it costs a few hundred cycles,
+// which a wait that is on the critical path would pay after every failed try.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity);
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");

@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.s_full[0], 1);
     mbar_init(&bars.s_full[1], 1);
     mbar_init(&bars.dp_full, 1);
-    mbar_init(&bars.dp_read, 256);
-    mbar_init(&bars.ds_full, 256);
+    mbar_init(&bars.dp_read, 8);
+    mbar_init(&bars.ds_full, 8);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int x = 0; x < 2 * steps; ++x) {
       const int stage = x % NS;
-      if (x >= NS) ok = mbar_wait_bounded(&bars.kv_empty[stage], ((x / NS) - 1) & 1);
+      if (x >= NS) ok = tc::wait(&bars.kv_empty[stage], ((x / NS) - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
@@ -179,14 +179,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) {
       atomicExch(&g_tc_bwd_error, kDevTimeout);
-      for (int x = max(0, issued - NS); x < issued; ++x) mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1);
+      for (int x = max(0, issued - NS); x < issued; ++x) tc::wait(&bars.kv_full[x % NS], (x / NS) & 1);
     }
   } else if (warp == 8) {
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
-    bool ok = steps == 0 || mbar_wait_bounded(&bars.q_full, 0);
+    bool ok = steps == 0 || tc::wait(&bars.q_full, 0);
     auto kv_wait = [&](int x) {
-      ok = ok && mbar_wait_bounded(&bars.kv_full[x % NS], (x / NS) & 1);
+      ok = ok && tc::wait(&bars.kv_full[x % NS], (x / NS) & 1);
       tc::fence_after();
     };
     auto kv_addr = [&](int x) { return smem + (2 + x % NS) * L::kTile; };
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       key_words(j, w);
       if (ok && !tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j), w);
       if (ok && leader) {
-        tc::product_nt<DP>(tmem + (j & 1) * 128, smem, L::kHalf, kv_addr(2 * j), L::kHalf, id_s);
+        tc::product_nt<DP>(tmem + (j & 1) * 128, smem, kv_addr(2 * j), id_s);
         tc::commit(&bars.s_full[j & 1]);
       }
       __syncwarp();
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto grads = [&](int j) {
       kv_wait(2 * j + 1);
       if (ok && leader) {
-        tc::product_nt<DP>(t_dp, smem + L::kTile, L::kHalf, kv_addr(2 * j + 1), L::kHalf, id_s);
+        tc::product_nt<DP>(t_dp, smem + L::kTile, kv_addr(2 * j + 1), id_s);
         tc::commit(&bars.dp_full);
         tc::commit(&bars.kv_empty[(2 * j + 1) % NS]);
       }
@@ -217,14 +217,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = 0; j < steps && ok; ++j) {
       if (j + 1 < steps) {
         scores(j + 1);
-        ok = ok && mbar_wait_bounded(&bars.dp_read, j & 1);
+        ok = ok && tc::wait(&bars.dp_read, j & 1);
         tc::fence_after();
         if (ok) grads(j + 1);
       }
-      ok = ok && mbar_wait_bounded(&bars.ds_full, j & 1);
+      ok = ok && tc::wait(&bars.ds_full, j & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<128, 64>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), L::kHalf, id_o, j > 0);
+        tc::product_tn(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), id_o, j > 0);
         tc::commit(&bars.kv_empty[(2 * j) % NS]);
         if (j + 1 == steps) tc::commit(&bars.done);
       }
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
       const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + half * 64;
-      ok = mbar_wait_bounded(&bars.s_full[j & 1], (j >> 1) & 1);
+      ok = tc::wait(&bars.s_full[j & 1], (j >> 1) & 1);
       if (!ok) break;
       tc::fence_after();
       uint32_t s[2][32], dp[2][32];
@@ -263,14 +263,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           s[c][e] = __float_as_uint(ex2(x.x));
           s[c][e + 1] = __float_as_uint(ex2(x.y));
         }
-      ok = mbar_wait_bounded(&bars.dp_full, j & 1);
+      ok = tc::wait(&bars.dp_full, j & 1);
       if (!ok) break;
       tc::fence_after();
       tc::ld32(t_dp + lanes + half * 64, dp[0]);
       tc::ld32(t_dp + lanes + half * 64 + 32, dp[1]);
       tc::wait_ld(dp[0], dp[1]);
       tc::fence_before();
-      tc::arrive(&bars.dp_read);
+      __syncwarp();
+      if (lane == 0) tc::arrive(&bars.dp_read);
       const bool whole = tc::all_set(w) && !none && (!a.causal || j0 + 63 <= t.first + (warp & 3) * 32 / f.pack);
       // whole is uniform but for `none`
 #pragma unroll
@@ -298,9 +299,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::wait_st();
       tc::fence_before();
-      tc::arrive(&bars.ds_full);
+      __syncwarp();
+      if (lane == 0) tc::arrive(&bars.ds_full);
     }
-    if (ok && steps > 0) ok = mbar_wait_bounded(&bars.done, 0);
+    if (ok && steps > 0) ok = tc::wait(&bars.done, 0);
     tc::fence_after();
     if (!ok) {
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
@@ -359,9 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.stat_full[i], 32);
     }
     mbar_init(&bars.s_full, 1);
-    mbar_init(&bars.p_full, 256);
+    mbar_init(&bars.p_full, 8);
     mbar_init(&bars.dp_full, 1);
-    mbar_init(&bars.ds_full, 256);
+    mbar_init(&bars.ds_full, 8);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < steps; ++s) {
       const int stage = s % NS;
-      if (s >= NS) ok = mbar_wait_bounded(&bars.q_empty[stage], ((s / NS) - 1) & 1);
+      if (s >= NS) ok = tc::wait(&bars.q_empty[stage], ((s / NS) - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bars.q_full[stage], 2 * L::kTile);
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) {
       atomicExch(&g_tc_bwd_error, kDevTimeout);
-      for (int s = max(0, issued - NS); s < issued; ++s) mbar_wait_bounded(&bars.q_full[s % NS], (s / NS) & 1);
+      for (int s = max(0, issued - NS); s < issued; ++s) tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
     }
   } else if (warp == 10) {
     bool ok = true;
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         dl[i] = tok < t.n ? -__ldg(a.delta + lse_index(a, t, h, tok)) : 0.f;
         if (blind(nl[i])) dl[i] = 0.f;
       }
-      if (s >= NS) ok = mbar_wait_bounded(&bars.q_empty[stage], ((s / NS) - 1) & 1);
+      if (s >= NS) ok = tc::wait(&bars.q_empty[stage], ((s / NS) - 1) & 1);
       if (!ok) break;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -440,10 +442,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 8) {
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
-    bool ok = steps == 0 || mbar_wait_bounded(&bars.kv_full, 0);
+    bool ok = steps == 0 || tc::wait(&bars.kv_full, 0);
     auto q_addr = [&](int s) { return smem + (2 + 2 * (s % NS)) * L::kTile; };
     auto scores = [&](int s) {
-      ok = ok && mbar_wait_bounded(&bars.q_full[s % NS], (s / NS) & 1);
+      ok = ok && tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
       tc::fence_after();
       // packed: rows of the next sequence in a tile that reaches past this one
       const int rows = (t.n - first_of(s)) * f.pack;
@@ -454,14 +456,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::clear_rows<DP / 64>(q_addr(s) + L::kTile, w);
       }
       if (ok && leader) {
-        tc::product_nt<DP>(tmem, smem, L::kHalf, q_addr(s), L::kHalf, id_s);
+        tc::product_nt<DP>(tmem, smem, q_addr(s), id_s);
         tc::commit(&bars.s_full);
       }
       __syncwarp();
     };
     auto grads = [&](int s) {
       if (ok && leader) {
-        tc::product_nt<DP>(t_dp, smem + L::kTile, L::kHalf, q_addr(s) + L::kTile, L::kHalf, id_s);
+        tc::product_nt<DP>(t_dp, smem + L::kTile, q_addr(s) + L::kTile, id_s);
         tc::commit(&bars.dp_full);
       }
       __syncwarp();
@@ -471,15 +473,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       grads(0);
     }
     for (int s = 0; s < steps && ok; ++s) {
-      ok = mbar_wait_bounded(&bars.p_full, s & 1);
+      ok = tc::wait(&bars.p_full, s & 1);
       tc::fence_after();
-      if (ok && leader) tc::product_tn<128, 64>(t_dv, tmem, q_addr(s) + L::kTile, L::kHalf, id_o, s > 0);
+      if (ok && leader) tc::product_tn(t_dv, tmem, q_addr(s) + L::kTile, id_o, s > 0);
       __syncwarp();
       if (s + 1 < steps) scores(s + 1);
-      ok = ok && mbar_wait_bounded(&bars.ds_full, s & 1);
+      ok = ok && tc::wait(&bars.ds_full, s & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<128, 64>(t_dk, t_dp, q_addr(s), L::kHalf, id_o, s > 0);
+        tc::product_tn(t_dk, t_dp, q_addr(s), id_o, s > 0);
         tc::commit(&bars.q_empty[s % NS]);
         if (s + 1 == steps) tc::commit(&bars.done);
       }
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < steps && ok; ++s) {
       const int stage = s % NS;
       const uint32_t s_addr = tmem + lanes + half * 64, d_addr = t_dp + lanes + half * 64;
-      ok = mbar_wait_bounded(&bars.stat_full[stage], (s / NS) & 1) && mbar_wait_bounded(&bars.s_full, s & 1);
+      ok = tc::wait(&bars.stat_full[stage], (s / NS) & 1) && tc::wait(&bars.s_full, s & 1);
       if (!ok) break;
       tc::fence_after();
       uint32_t p[2][32];
@@ -535,9 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::wait_st();
       tc::fence_before();
-      tc::arrive(&bars.p_full);
+      __syncwarp();
+      if (lane == 0) tc::arrive(&bars.p_full);
 
-      ok = mbar_wait_bounded(&bars.dp_full, s & 1);
+      ok = tc::wait(&bars.dp_full, s & 1);
       if (!ok) break;
       tc::fence_after();
 #pragma unroll
@@ -572,9 +575,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::wait_st();
       tc::fence_before();
-      tc::arrive(&bars.ds_full);
+      __syncwarp();
+      if (lane == 0) tc::arrive(&bars.ds_full);
     }
-    if (ok && steps > 0) ok = mbar_wait_bounded(&bars.done, 0);
+    if (ok && steps > 0) ok = tc::wait(&bars.done, 0);
     tc::fence_after();
     if (!ok) {
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);

@@ -7,19 +7,18 @@
 // has fewer tokens (less of a causal diagonal is computed in vain) and the keys
 // are read for all of them at once.
 //
-//   warps 0-3, 4-7   softmax of tile 0 and 1: a thread holds one row
-//   warp 8   issues the MMAs    warp 9   issues the TMA loads    warp 10   finds the work
+//   warps 0-7, 8-15   softmax of tile 0 and 1: two threads per row, 64 keys each
+//   warps 16, 19   MMAs of tile 0 and 1    warp 17   TMA loads    warp 18   finds the work
 //
 // The grid has a CTA for each pair of tiles; a CTA that has finished one takes
 // over another that has not started (cluster launch control), so that the loads
 // and the first scores of the next pair run under the last weights and the
 // output of this one, and the setup is paid once per SM.
 //
-// Per 64 keys and tile:  S = Q K^T into one of two buffers of 64 tensor-memory
-// columns; each softmax thread reads its row, P = exp2(c S - m) goes back as
-// 16-bit into the same columns; O += P V with P read from tensor memory as the A
-// operand.  With two buffers the next scores are ready when a step's weights are
-// done, so the softmax warps never wait for the products.  The running maximum
+// Per 128 keys and tile:  S = Q K^T into 128 columns of tensor memory; each
+// softmax thread reads its half row, P = exp2(c S - m) goes back as 16-bit into
+// the same columns; O += P V with P read from tensor memory as the A operand.
+// While one tile's softmax runs, the other tile's products do.  The running maximum
 // that P is relative to moves only when it has grown by more than 2^8, so O is
 // rescaled (tensor memory -> registers -> tensor memory) a few times per row and
 // not per tile; P stays below 2^8, the sum and O are fp32, and the quotient is
@@ -38,7 +37,7 @@ __device__ int g_tc_fwd_error;
 
 namespace {
 
-constexpr int kThreads = 640;  // five warpgroups; warp 19 idles
+constexpr int kThreads = 640;  // five warpgroups
 constexpr int kSoftmaxWarps = 16;
 constexpr int kRows = 128;  // rows of a tile, and keys of a step
 constexpr float kLazy = 8.f;
@@ -64,7 +63,7 @@ struct Layout {
 };
 
 struct Bars {
-  uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_full[2];
   uint64_t item_full, item_taken, answer;
 };
 
@@ -83,6 +82,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FwdArgs f) {
   using L = Layout<DP>;
   constexpr int NS = L::kStages;
+  // Half of a step's weights are announced too, which wakes the waiting MMA warp ahead of time: 402
+  // instead of 454 us at 8192 keys, 16 heads of 64, but 534 instead of 503 at 128.
+  constexpr bool kEarly = DP == 64;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -98,18 +100,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::alloc(&s_tmem, 512);
   } else if (warp == kSoftmaxWarps + 1 && lane == 0) {
     mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 1);
+    mbar_init(&bars.q_empty, 2);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.kv_full[i], 1);
-      mbar_init(&bars.kv_empty[i], 1);
+      mbar_init(&bars.kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 2 * kRows);
+      mbar_init(&bars.p_half[i], kSoftmaxWarps / 2);
+      mbar_init(&bars.p_full[i], kSoftmaxWarps / 2);
       mbar_init(&bars.o_full[i], 1);
     }
     mbar_init(&bars.item_full, 1);
-    mbar_init(&bars.item_taken, kSoftmaxWarps + 2);
+    mbar_init(&bars.item_taken, kSoftmaxWarps + 3);
     mbar_init(&bars.answer, 1);
     fence_mbar_init();
     prefetch_tmap(&qmap);
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // the it-th piece of work, for the warps that work on it; false: a wait ran out
   auto read_item = [&](int it, Item& x) -> bool {
-    if (!mbar_wait_bounded(&bars.item_full, it & 1)) return false;
+    if (!tc::wait(&bars.item_full, it & 1)) return false;
     x = s_item;
     __syncwarp();
     return true;
@@ -177,13 +180,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Every warp has begun the piece before, and its loads are all on their way.  Asked for
         // earlier, pieces of different lengths would be dealt out before it is known who is free:
         // 4 chunks over 1500 to 8192 keys took 315 us instead of 200.
-        ok = mbar_wait_bounded(&bars.item_taken, (it - 1) & 1);
+        ok = tc::wait(&bars.item_taken, (it - 1) & 1);
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&bars.answer, 16);
           tc::steal(&s_answer, &bars.answer);
         }
-        ok = mbar_wait_bounded(&bars.answer, (it - 1) & 1);
+        ok = tc::wait(&bars.answer, (it - 1) & 1);
         if (!ok) break;
         id = tc::stolen(&s_answer);
       }
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         taken();
         continue;
       }
-      if (nq > 0) ok = mbar_wait_bounded(&bars.q_empty, (nq - 1) & 1);
+      if (nq > 0) ok = tc::wait(&bars.q_empty, (nq - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bars.q_full, 2 * L::kTile);
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++nq;
       for (int y = 0; y < 2 * all; ++y) {
         const int stage = kv % NS;
-        if (kv >= NS) ok = mbar_wait_bounded(&bars.kv_empty[stage], ((kv / NS) - 1) & 1);
+        if (kv >= NS) ok = tc::wait(&bars.kv_empty[stage], ((kv / NS) - 1) & 1);
         if (!ok) break;
         const CUtensorMap* map = (y & 1) ? &vmap : &kmap;
         const uint32_t dst = smem + (2 + stage) * L::kTile;
@@ -287,74 +290,74 @@ __global__ void __launch_bounds__(kThreads, 1)
     // nothing may still be in flight when the CTA ends: the MMA warp has waited for all of it unless a wait ran out
     if (!ok) {
       atomicExch(&g_tc_fwd_error, kDevTimeout);
-      for (int y = max(0, kv - NS); y < kv; ++y) mbar_wait_bounded(&bars.kv_full[y % NS], (y / NS) & 1);
-      if (nq > 0) mbar_wait_bounded(&bars.q_full, (nq - 1) & 1);
+      for (int y = max(0, kv - NS); y < kv; ++y) tc::wait(&bars.kv_full[y % NS], (y / NS) & 1);
+      if (nq > 0) tc::wait(&bars.q_full, (nq - 1) & 1);
     }
-   } else if (warp == kSoftmaxWarps) {
+   } else {
     // ---------------- products ----------------
+    // One warp per row tile: a successful wait costs a hundred cycles or more, and with one warp for
+    // both tiles those of one tile delayed the other's products (562 instead of 503 us at 8192 keys,
+    // 16 heads of 128, 477 instead of 402 at 64).  Both free a key tile.
+    const int i = warp == kSoftmaxWarps ? 0 : 1;
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
     bool ok = true;
-    int kv = 0, nq = 0, ns[2] = {0, 0};  // running numbers: tiles, Q loads, steps of each row tile
+    int kv = 0, nq = 0, ns = 0;  // running numbers: tiles, Q loads, steps of this row tile
+    const uint32_t t_s = tmem + i * kRows, t_o = tmem + 2 * kRows + i * DP, q = smem + i * L::kTile;
     for (int it = 0; ok; ++it) {
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
       int first[2], steps[2], j_lo, shift;
       plan(x, first, steps, j_lo, shift);
-      const int all = max(steps[0], steps[1]);
+      const int all = max(steps[0], steps[1]), mine = i == 0 ? steps[0] : steps[1];
       if (all == 0) continue;
-      ok = mbar_wait_bounded(&bars.q_full, nq & 1);
+      ok = tc::wait(&bars.q_full, nq & 1);
       ++nq;
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
-      auto kv_wait = [&](int y) { ok = ok && mbar_wait_bounded(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
+      auto kv_wait = [&](int y) { ok = ok && tc::wait(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
       auto kv_addr = [&](int y) { return smem + (2 + (kv + y) % NS) * L::kTile; };
-      auto scores = [&](int i, int j) {
-        if (leader) {
-          tc::product_nt<DP>(tmem + i * kRows, smem + i * L::kTile, L::kHalf, kv_addr(2 * j), L::kHalf, id_s);
-          tc::commit(&bars.s_full[i]);
-        }
+      // scores of step j into the tile's buffer; keys are released by the step's end
+      auto scores = [&](int j) {
+        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), id_s);
+        tc::commit(&bars.s_full[i]);
+        if (j + 1 == mine) tc::commit(&bars.q_empty);
       };
       kv_wait(0);
       tc::fence_after();
-      if (ok) {
-        for (int i = 0; i < 2; ++i)
-          if (steps[i] > 0) scores(i, 0);
-        if (leader) {
-          tc::commit(&bars.kv_empty[kv % NS]);
-          if (all == 1) tc::commit(&bars.q_empty);
-        }
+      if (ok && leader) {
+        if (mine > 0) scores(0);
+        else tc::commit(&bars.q_empty);
+        tc::commit(&bars.kv_empty[kv % NS]);
       }
+      __syncwarp();
       for (int j = 0; j < all && ok; ++j) {
         kv_wait(2 * j + 1);
+        if (j + 1 < all) kv_wait(2 * j + 2);
         if (!ok) break;
-        // values of keys that are not there or not valid may hold anything
-        uint32_t w[4];
-        key_words(x.n, mask, (j_lo + j) * kRows, (kv >> 1) + j, w);
-        if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
-        const bool more = j + 1 < all;
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j < steps[i]) {
-            ok = mbar_wait_bounded(&bars.p_full[i], ns[i] & 1);
-            tc::fence_after();
-            if (ok && leader) {
-              tc::product_tn<128, 64>(tmem + 2 * kRows + i * DP, tmem + i * kRows, kv_addr(2 * j + 1), L::kHalf, id_o,
-                                      j > 0);
-              if (j + 1 == steps[i]) tc::commit(&bars.o_full[i]);
-            }
-            __syncwarp();
-            ++ns[i];
+        if (j < mine) {
+          // values of keys that are not there or not valid may hold anything
+          uint32_t w[4];
+          const int j0 = (j_lo + j) * kRows;
+          if (PAGED || mask != nullptr || j0 + kRows > x.n) {
+            key_words(x.n, mask, j0, (kv >> 1) + j, w);
+            if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
           }
-          if (j + 1 < steps[i]) {
-            kv_wait(2 * j + 2);
-            tc::fence_after();
-            if (ok) scores(i, j + 1);
+          // (Issuing the products of half the keys ahead of the others was tried: it costs more than it
+          // hides, 643 instead of 534 us at 8192 keys, 16 heads of 128.)
+          if (kEarly) ok = tc::wait(&bars.p_half[i], ns & 1);
+          ok = ok && tc::wait(&bars.p_full[i], ns & 1);
+          tc::fence_after();
+          if (ok && leader) {
+            tc::product_tn(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            if (j + 1 == mine) tc::commit(&bars.o_full[i]);
+            else scores(j + 1);
           }
+          ++ns;
         }
         if (ok && leader) {
           tc::commit(&bars.kv_empty[(kv + 2 * j + 1) % NS]);
-          if (more) tc::commit(&bars.kv_empty[(kv + 2 * j + 2) % NS]);
-          if (j + 2 == all) tc::commit(&bars.q_empty);  // the last scores are on their way
+          if (j + 1 < all) tc::commit(&bars.kv_empty[(kv + 2 * j + 2) % NS]);
         }
         __syncwarp();
       }
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < count; ++j, ++ns) {
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
-        ok = ok && mbar_wait_bounded(&bars.s_full[i], ns & 1);
+        ok = ok && tc::wait(&bars.s_full[i], ns & 1);
         tc::fence_after();
         const int j0 = (j_lo + j) * kRows;
         uint32_t s[2][32];
@@ -478,16 +481,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // over this half's own scores: the other half may not have read its yet
           tc::st16(s_addr + 16 * c, p);
+          tc::wait_st();
+          tc::fence_before();
+          __syncwarp();
+          // one arrival per warp: 256 of them would queue up at the barrier
+          if (c == 0 && kEarly && lane == 0) tc::arrive(&bars.p_half[i]);
+          if (c == 1 && lane == 0) tc::arrive(&bars.p_full[i]);
         }
         part = add2(part, part2);
         sum += part.x + part.y;
-        tc::wait_st();
-        tc::fence_before();
-        tc::arrive(&bars.p_full[i]);
       }
       kt += all;
       if (count > 0) {
-        ok = ok && mbar_wait_bounded(&bars.o_full[i], no & 1);
+        ok = ok && tc::wait(&bars.o_full[i], no & 1);
         ++no;
         tc::fence_after();
         s_sum[i][half][row] = sum;
