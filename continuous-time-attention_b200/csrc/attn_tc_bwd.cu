@@ -10,8 +10,8 @@
 // that do not depend on timing, and the heads that share keys are summed in
 // place.  Rows are (token, head) pairs as in the forward.
 //
-//   warps 0-7  weights: two warpgroups take 64 columns each of a 128 x 128 tile
-//   warp 8     MMAs      warp 9  TMA loads      warp 10  lse and delta (keys' kernel)
+//   warps 0-15  weights: four warpgroups take 32 columns each of a 128 x 128 tile
+//   warp 16     MMAs      warp 17  TMA loads      warp 18  lse and delta (keys' kernel)
 //
 // Weights and score gradients go back to tensor memory as 16-bit A operands over
 // the columns their fp32 sources came from, so a tile pair crosses shared memory
@@ -31,7 +31,8 @@ __device__ int g_tc_bwd_error;
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;  // five warpgroups; the last has a warp or two to spare
+constexpr int kWeightWarps = 16;
 constexpr int kRows = 128;
 
 struct BwdArgs {
@@ -44,39 +45,40 @@ template <int DP>
 struct Layout {
   static constexpr int kHalf = kRows * 128;
   static constexpr int kTile = kHalf * (DP / 64);
-  static constexpr int kStages = 4;  // tiles of the other side in flight
+  static constexpr int kStages = DP == 128 ? 4 : 8;  // tiles of the other side in flight
   static constexpr int kSmem = (2 + kStages) * kTile + 1024;
 };
 
-// a 128-row tile of gradients from tensor memory; one thread per row
-template <typename T, int DP>
-__device__ __forceinline__ void store_grad(uint32_t addr, T* out, int d, float mul, bool live, bool vec, bool any) {
+// COLS columns of a gradient's row from tensor memory, the first of them column c0 of d
+template <typename T, int COLS>
+__device__ __forceinline__ void store_grad(uint32_t addr, T* out, int c0, int d, float mul, bool live, bool vec, bool any) {
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
-    uint32_t o[32];
+  for (int c = 0; c < COLS / 16; ++c) {
+    uint32_t o[16];
     if (any) {
-      tc::ld32(addr + 32 * c, o);
+      tc::ld16(addr + 16 * c, o);
       tc::wait_ld(o);
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0u;
+      for (int e = 0; e < 16; ++e) o[e] = 0u;
     }
     if (!live) continue;
+    const int at = c0 + 16 * c;
     if (vec) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 8)
-        if (32 * c + e < d) {
+      for (int e = 0; e < 16; e += 8)
+        if (at + e < d) {
           uint4 x;
           uint32_t* xp = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             xp[y] = tc::pack2<T>(__uint_as_float(o[e + 2 * y]) * mul, __uint_as_float(o[e + 2 * y + 1]) * mul);
-          *reinterpret_cast<uint4*>(out + 32 * c + e) = x;
+          *reinterpret_cast<uint4*>(out + at + e) = x;
         }
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if (32 * c + e < d) out[32 * c + e] = Elem<T>::from_f(__uint_as_float(o[e]) * mul);
+      for (int e = 0; e < 16; ++e)
+        if (at + e < d) out[at + e] = Elem<T>::from_f(__uint_as_float(o[e]) * mul);
     }
   }
 }
@@ -89,7 +91,7 @@ __device__ __forceinline__ float neg_lse2_of(float lse) { return lse == neg_inf(
 // dQ
 // ---------------------------------------------------------------------------
 struct DqBars {
-  uint64_t q_full, kv_full[4], kv_empty[4], s_full[2], dp_full, dp_read, ds_full, done;
+  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], dp_full, dp_read, ds_full[2], done;
 };
 
 template <typename T, int DP>
@@ -112,9 +114,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal);
     if (lane == 0) s_tile = x;
-  } else if (warp == 8) {
+  } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
-  } else if (warp == 9 && lane == 0) {
+  } else if (warp == kWeightWarps + 1 && lane == 0) {
     mbar_init(&bars.q_full, 1);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.kv_full[i], 1);
@@ -123,8 +125,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.s_full[0], 1);
     mbar_init(&bars.s_full[1], 1);
     mbar_init(&bars.dp_full, 1);
-    mbar_init(&bars.dp_read, 8);
-    mbar_init(&bars.ds_full, 8);
+    mbar_init(&bars.dp_read, kWeightWarps);
+    mbar_init(&bars.ds_full[0], kWeightWarps);
+    mbar_init(&bars.ds_full[1], kWeightWarps);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  if (warp == 9) {
+  if (warp == kWeightWarps + 1) {
     bool ok = true;
     int issued = 0;
     if (steps > 0 && lane == 0) {
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       atomicExch(&g_tc_bwd_error, kDevTimeout);
       for (int x = max(0, issued - NS); x < issued; ++x) tc::wait(&bars.kv_full[x % NS], (x / NS) & 1);
     }
-  } else if (warp == 8) {
+  } else if (warp == kWeightWarps) {
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
     bool ok = steps == 0 || tc::wait(&bars.q_full, 0);
@@ -192,9 +195,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto kv_addr = [&](int x) { return smem + (2 + x % NS) * L::kTile; };
     auto scores = [&](int j) {
       kv_wait(2 * j);
-      uint32_t w[4];
-      key_words(j, w);
-      if (ok && !tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j), w);
+      if (mask != nullptr || (j_lo + j + 1) * kRows > t.n) {
+        uint32_t w[4];
+        key_words(j, w);
+        if (ok && !tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j), w);
+      }
       if (ok && leader) {
         tc::product_nt<DP>(tmem + (j & 1) * 128, smem, kv_addr(2 * j), id_s);
         tc::commit(&bars.s_full[j & 1]);
@@ -221,18 +226,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after();
         if (ok) grads(j + 1);
       }
-      ok = ok && tc::wait(&bars.ds_full, j & 1);
+      ok = ok && tc::wait(&bars.ds_full[j & 1], (j >> 1) & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), id_o, j > 0);
+        tc::product_tn<32>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), id_o, j > 0);
         tc::commit(&bars.kv_empty[(2 * j) % NS]);
         if (j + 1 == steps) tc::commit(&bars.done);
       }
       __syncwarp();
     }
     if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
-  } else if (warp < 8) {
-    const int half = warp >> 2;
+  } else if (warp < kWeightWarps) {
+    const int part = warp >> 2;  // columns [32 part, 32 part + 32) of each tile
     const int row = (warp & 3) * 32 + lane;
     const int tok = t.first + row / f.pack, h = h0 + row % f.pack;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -242,76 +247,67 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float delta = live ? a.delta[lse_index(a, t, h, tok)] : 0.f;
     const bool none = blind(nl);
     const int limit = a.causal ? tok : t.n - 1;
+    const int limit_all = t.first + (warp & 3) * 32 / f.pack;  // causal: last key all rows of the warp see
+    const bool any_blind = __any_sync(0xffffffffu, none);
     bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
-      const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + half * 64;
+      const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + part * 32;
       ok = tc::wait(&bars.s_full[j & 1], (j >> 1) & 1);
       if (!ok) break;
       tc::fence_after();
-      uint32_t s[2][32], dp[2][32];
-      tc::ld32(s_addr, s[0]);
-      tc::ld32(s_addr + 32, s[1]);
-      tc::wait_ld(s[0], s[1]);
-      const int j0 = (j_lo + j) * kRows + half * 64;
-      uint32_t w[4];
-      key_words(j, w);
+      uint32_t s[32], dp[32];
+      tc::ld32(s_addr, s);
+      const int j0 = (j_lo + j) * kRows;
+      const bool whole = j0 + kRows <= t.n && mask == nullptr && !any_blind && (!a.causal || j0 + kRows - 1 <= limit_all);
+      tc::wait_ld(s);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float2 x = fma2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), f2(c2), f2(nl));
-          s[c][e] = __float_as_uint(ex2(x.x));
-          s[c][e + 1] = __float_as_uint(ex2(x.y));
-        }
+      for (int e = 0; e < 32; e += 2) {
+        const float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2(c2), f2(nl));
+        s[e] = __float_as_uint(ex2(x.x));
+        s[e + 1] = __float_as_uint(ex2(x.y));
+      }
       ok = tc::wait(&bars.dp_full, j & 1);
       if (!ok) break;
       tc::fence_after();
-      tc::ld32(t_dp + lanes + half * 64, dp[0]);
-      tc::ld32(t_dp + lanes + half * 64 + 32, dp[1]);
-      tc::wait_ld(dp[0], dp[1]);
+      tc::ld32(t_dp + lanes + part * 32, dp);
+      tc::wait_ld(dp);
       tc::fence_before();
       __syncwarp();
       if (lane == 0) tc::arrive(&bars.dp_read);
-      const bool whole = tc::all_set(w) && !none && (!a.causal || j0 + 63 <= t.first + (warp & 3) * 32 / f.pack);
-      // whole is uniform but for `none`
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t ds[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float2 x = mul2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])),
-                                add2(make_float2(__uint_as_float(dp[c][e]), __uint_as_float(dp[c][e + 1])), f2(-delta)));
-          dp[c][e] = __float_as_uint(x.x);
-          dp[c][e + 1] = __float_as_uint(x.y);
-        }
-        if (!whole) {
-          const int left = none ? 0 : limit - j0 - 32 * c + 1;
-          const uint32_t see = (half == 0 ? w[c] : w[2 + c]) &
-                               (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((see >> e) & 1u)) dp[c][e] = 0u;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          ds[e] = tc::pack2<T>(__uint_as_float(dp[c][2 * e]), __uint_as_float(dp[c][2 * e + 1]));
-        tc::st16(s_addr + 16 * c, ds);
+      for (int e = 0; e < 32; e += 2) {
+        const float2 x = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                              add2(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), f2(-delta)));
+        dp[e] = __float_as_uint(x.x);
+        dp[e + 1] = __float_as_uint(x.y);
       }
+      if (!whole) {
+        uint32_t w[4];
+        key_words(j, w);
+        const int left = none ? 0 : limit - j0 - 32 * part + 1;
+        const uint32_t see = (part == 0 ? w[0] : part == 1 ? w[1] : part == 2 ? w[2] : w[3]) &
+                             (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!((see >> e) & 1u)) dp[e] = 0u;
+      }
+      uint32_t ds[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ds[e] = tc::pack2<T>(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1]));
+      tc::st16(s_addr, ds);
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::arrive(&bars.ds_full);
+      if (lane == 0) tc::arrive(&bars.ds_full[j & 1]);
     }
     if (ok && steps > 0) ok = tc::wait(&bars.done, 0);
     tc::fence_after();
     if (!ok) {
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
     } else if (t.first < t.n) {
-      if (half == 0) {
-        T* out = static_cast<T*>(a.dq) + t.batch * a.dqs.b + (t.row0 + tok) * a.dqs.t + h * a.dqs.h;
-        store_grad<T, DP>(t_dq + lanes, out, a.d, a.scale, live, f.vec_dq, steps > 0);
-      }
-    } else if (a.cu != nullptr && t.n == 0 && half == 0) {
+      T* out = static_cast<T*>(a.dq) + t.batch * a.dqs.b + (t.row0 + tok) * a.dqs.t + h * a.dqs.h;
+      store_grad<T, DP / 4>(t_dq + lanes + part * (DP / 4), out, part * (DP / 4), a.d, a.scale, live, f.vec_dq, steps > 0);
+    } else if (a.cu != nullptr && t.n == 0 && part == 0) {
       for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
         for (int x = threadIdx.x; x < a.d * f.pack; x += kRows)
           static_cast<T*>(a.dq)[r * a.dqs.t + (h0 + x / a.d) * a.dqs.h + x % a.d] = Elem<T>::from_f(0.f);
@@ -320,14 +316,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::dealloc(tmem, 512);
+  if (warp == kWeightWarps) tc::dealloc(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
 // dK, dV: the tiles are transposed, rows are keys and columns are query rows
 // ---------------------------------------------------------------------------
 struct DkvBars {
-  uint64_t kv_full, q_full[2], q_empty[2], stat_full[2], s_full, p_full, dp_full, ds_full, done;
+  uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], p_full[2], dp_full, ds_full, done;
 };
 
 template <typename T, int DP>
@@ -341,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DkvBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ SeqTile s_tile;
-  __shared__ __align__(16) float s_stat[2][2][kRows];  // [stage][-lse2, -delta][row]
+  __shared__ __align__(16) float s_stat[NS][2][kRows];  // [stage][-lse2, -delta][row]
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -351,19 +347,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the first keys of a causal sequence meet the most rows: forwards is heaviest first
     const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false);
     if (lane == 0) s_tile = x;
-  } else if (warp == 8) {
+  } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
-  } else if (warp == 9 && lane == 0) {
+  } else if (warp == kWeightWarps + 1 && lane == 0) {
     mbar_init(&bars.kv_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.q_empty[i], 1);
-      mbar_init(&bars.stat_full[i], 32);
+      mbar_init(&bars.g_full[i], 1);
+      mbar_init(&bars.g_empty[i], 1);
+      mbar_init(&bars.stat_full[i], 1);
     }
-    mbar_init(&bars.s_full, 1);
-    mbar_init(&bars.p_full, 8);
+    mbar_init(&bars.s_full[0], 1);
+    mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.p_full[0], kWeightWarps);
+    mbar_init(&bars.p_full[1], kWeightWarps);
     mbar_init(&bars.dp_full, 1);
-    mbar_init(&bars.ds_full, 8);
+    mbar_init(&bars.ds_full, kWeightWarps);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
@@ -372,7 +372,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const SeqTile t = s_tile;
   const uint32_t tmem = s_tmem;
-  const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 256 + DP;
+  // Scores: one buffer of 128 columns at dim 128, where the four accumulators fill tensor memory, two at 64
+  constexpr int NB = DP == 64 ? 2 : 1;
+  const uint32_t t_dp = tmem + NB * 128, t_dv = t_dp + 128, t_dk = t_dv + DP;
 
   const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
   int lo, hi;
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto head_of = [&](int s) { return hk * group + s / per_head * f.pack; };
   auto first_of = [&](int s) { return (i_lo + s % per_head) * f.tile_tokens; };
 
-  if (warp == 9) {
+  if (warp == kWeightWarps + 1) {
     bool ok = true;
     int issued = 0;
     if (steps > 0 && lane == 0) {
@@ -397,27 +399,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                         static_cast<int>(t.row0) + t.first, t.batch);
       }
     }
-    for (int s = 0; s < steps; ++s) {
-      const int stage = s % NS;
-      if (s >= NS) ok = tc::wait(&bars.q_empty[stage], ((s / NS) - 1) & 1);
+    for (int x = 0; x < 2 * steps; ++x) {
+      // Q and dO of a step by turns, each given back when its last product is done
+      const int s = x >> 1, stage = s % NS;
+      uint64_t* full = (x & 1) ? &bars.g_full[stage] : &bars.q_full[stage];
+      if (s >= NS) ok = tc::wait((x & 1) ? &bars.g_empty[stage] : &bars.q_empty[stage], ((s / NS) - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bars.q_full[stage], 2 * L::kTile);
-        const int row = static_cast<int>(t.row0) + first_of(s);
-        for (int c = 0; c < DP / 64; ++c) {
-          tc::tma_load_4d(smem + (2 + 2 * stage) * L::kTile + c * L::kHalf, &qmap, &bars.q_full[stage], 64 * c,
-                          head_of(s), row, t.batch);
-          tc::tma_load_4d(smem + (3 + 2 * stage) * L::kTile + c * L::kHalf, &gmap, &bars.q_full[stage], 64 * c,
-                          head_of(s), row, t.batch);
-        }
+        mbar_arrive_expect_tx(full, L::kTile);
+        for (int c = 0; c < DP / 64; ++c)
+          tc::tma_load_4d(smem + (2 + 2 * stage + (x & 1)) * L::kTile + c * L::kHalf, (x & 1) ? &gmap : &qmap, full, 64 * c,
+                          head_of(s), static_cast<int>(t.row0) + first_of(s), t.batch);
       }
-      issued = s + 1;
+      issued = x + 1;
     }
     if (!ok) {
       atomicExch(&g_tc_bwd_error, kDevTimeout);
-      for (int s = max(0, issued - NS); s < issued; ++s) tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
+      for (int x = max(0, issued - 2 * NS); x < issued; ++x)
+        tc::wait((x & 1) ? &bars.g_full[(x >> 1) % NS] : &bars.q_full[(x >> 1) % NS], ((x >> 1) / NS) & 1);
     }
-  } else if (warp == 10) {
+  } else if (warp == kWeightWarps + 2) {
     bool ok = true;
     for (int s = 0; s < steps; ++s) {
       const int stage = s % NS;
@@ -437,31 +438,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_stat[stage][0][lane + 32 * i] = nl[i];
         s_stat[stage][1][lane + 32 * i] = dl[i];
       }
-      tc::arrive(&bars.stat_full[stage]);
+      __syncwarp();
+      if (lane == 0) tc::arrive(&bars.stat_full[stage]);
     }
-  } else if (warp == 8) {
+  } else if (warp == kWeightWarps) {
     constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
     bool ok = steps == 0 || tc::wait(&bars.kv_full, 0);
     auto q_addr = [&](int s) { return smem + (2 + 2 * (s % NS)) * L::kTile; };
+    // packed: rows of the next sequence in a tile that reaches past this one
+    auto clear_behind = [&](int s, uint32_t tile) {
+      const int rows = (t.n - first_of(s)) * f.pack;
+      if (ok && a.cu != nullptr && rows < kRows) {
+        uint32_t w[4];
+        tc::first_bits(rows, w);
+        tc::clear_rows<DP / 64>(tile, w);
+      }
+    };
     auto scores = [&](int s) {
       ok = ok && tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
       tc::fence_after();
-      // packed: rows of the next sequence in a tile that reaches past this one
-      const int rows = (t.n - first_of(s)) * f.pack;
-      if (ok && rows < kRows) {
-        uint32_t w[4];
-        tc::first_bits(rows, w);
-        tc::clear_rows<DP / 64>(q_addr(s), w);
-        tc::clear_rows<DP / 64>(q_addr(s) + L::kTile, w);
-      }
+      clear_behind(s, q_addr(s));
       if (ok && leader) {
-        tc::product_nt<DP>(tmem, smem, q_addr(s), id_s);
-        tc::commit(&bars.s_full);
+        tc::product_nt<DP>(tmem + (s % NB) * 128, smem, q_addr(s), id_s);
+        tc::commit(&bars.s_full[s % NB]);
       }
       __syncwarp();
     };
     auto grads = [&](int s) {
+      ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
+      tc::fence_after();
+      clear_behind(s, q_addr(s) + L::kTile);
       if (ok && leader) {
         tc::product_nt<DP>(t_dp, smem + L::kTile, q_addr(s) + L::kTile, id_s);
         tc::commit(&bars.dp_full);
@@ -473,15 +480,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       grads(0);
     }
     for (int s = 0; s < steps && ok; ++s) {
-      ok = tc::wait(&bars.p_full, s & 1);
+      if (NB == 2 && s + 1 < steps) scores(s + 1);  // its buffer's weights went into dV at step s - 1
+      ok = ok && tc::wait(&bars.p_full[s & 1], (s >> 1) & 1);
       tc::fence_after();
-      if (ok && leader) tc::product_tn(t_dv, tmem, q_addr(s) + L::kTile, id_o, s > 0);
+      if (ok && leader) {
+        tc::product_tn<32>(t_dv, tmem + (s % NB) * 128, q_addr(s) + L::kTile, id_o, s > 0);
+        tc::commit(&bars.g_empty[s % NS]);  // its dO V^T was done before
+      }
       __syncwarp();
-      if (s + 1 < steps) scores(s + 1);
+      if (NB == 1 && s + 1 < steps) scores(s + 1);
       ok = ok && tc::wait(&bars.ds_full, s & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn(t_dk, t_dp, q_addr(s), id_o, s > 0);
+        tc::product_tn<32>(t_dk, t_dp, q_addr(s), id_o, s > 0);
         tc::commit(&bars.q_empty[s % NS]);
         if (s + 1 == steps) tc::commit(&bars.done);
       }
@@ -489,8 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (s + 1 < steps) grads(s + 1);
     }
     if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
-  } else if (warp < 8) {
-    const int half = warp >> 2;
+  } else if (warp < kWeightWarps) {
+    const int part = warp >> 2;  // columns [32 part, 32 part + 32) of each tile
     const int key = t.first + (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool valid = key < t.n && (mask == nullptr || mask_key(mask, key));
@@ -498,81 +509,68 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int s = 0; s < steps && ok; ++s) {
       const int stage = s % NS;
-      const uint32_t s_addr = tmem + lanes + half * 64, d_addr = t_dp + lanes + half * 64;
-      ok = tc::wait(&bars.stat_full[stage], (s / NS) & 1) && tc::wait(&bars.s_full, s & 1);
+      const uint32_t s_addr = tmem + lanes + (s % NB) * 128 + part * 32, d_addr = t_dp + lanes + part * 32;
+      ok = tc::wait(&bars.stat_full[stage], (s / NS) & 1) && tc::wait(&bars.s_full[s % NB], (s / NB) & 1);
       if (!ok) break;
       tc::fence_after();
-      uint32_t p[2][32];
-      tc::ld32(s_addr, p[0]);
-      tc::ld32(s_addr + 32, p[1]);
-      tc::wait_ld(p[0], p[1]);
-      // causal: the first row of this half that sees the key; 64 = none
+      uint32_t p[32], w[16];
+      tc::ld32(s_addr, p);
+      // causal: the first row of this part that sees the key; 32 = none
       int from = 0;
-      if (a.causal) from = min(max((key - first_of(s)) * f.pack - half * 64, 0), 64);
-      if (!valid) from = 64;
-      const float4* nl = reinterpret_cast<const float4*>(&s_stat[stage][0][half * 64]);
-      const float4* dl = reinterpret_cast<const float4*>(&s_stat[stage][1][half * 64]);
+      if (a.causal) from = min(max((key - first_of(s)) * f.pack - part * 32, 0), 32);
+      if (!valid) from = 32;
+      const float4* nl = reinterpret_cast<const float4*>(&s_stat[stage][0][part * 32]);
+      const float4* dl = reinterpret_cast<const float4*>(&s_stat[stage][1][part * 32]);
       const bool masked = __any_sync(0xffffffffu, from > 0);
+      tc::wait_ld(p);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 b = nl[(32 * c + e) / 4];
-          float2 x = fma2(make_float2(__uint_as_float(p[c][e]), __uint_as_float(p[c][e + 1])), f2(c2), make_float2(b.x, b.y));
-          float2 y = fma2(make_float2(__uint_as_float(p[c][e + 2]), __uint_as_float(p[c][e + 3])), f2(c2), make_float2(b.z, b.w));
-          p[c][e] = __float_as_uint(ex2(x.x));
-          p[c][e + 1] = __float_as_uint(ex2(x.y));
-          p[c][e + 2] = __float_as_uint(ex2(y.x));
-          p[c][e + 3] = __float_as_uint(ex2(y.y));
-        }
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (32 * c + e < from) p[c][e] = 0u;
-        }
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = tc::pack2<T>(__uint_as_float(p[c][2 * e]), __uint_as_float(p[c][2 * e + 1]));
-        tc::st16(s_addr + 16 * c, w);
+      for (int e = 0; e < 32; e += 4) {
+        const float4 b = nl[e / 4];
+        const float2 x = fma2(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), f2(c2), make_float2(b.x, b.y));
+        const float2 y = fma2(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])), f2(c2), make_float2(b.z, b.w));
+        p[e] = __float_as_uint(ex2(x.x));
+        p[e + 1] = __float_as_uint(ex2(x.y));
+        p[e + 2] = __float_as_uint(ex2(y.x));
+        p[e + 3] = __float_as_uint(ex2(y.y));
       }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (e < from) p[e] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) w[e] = tc::pack2<T>(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
+      tc::st16(s_addr, w);
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::arrive(&bars.p_full);
+      if (lane == 0) tc::arrive(&bars.p_full[s & 1]);
 
       ok = tc::wait(&bars.dp_full, s & 1);
       if (!ok) break;
       tc::fence_after();
+      uint32_t d[32];
+      tc::ld32(d_addr, d);
+      tc::wait_ld(d);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t d[32], w[16];
-        tc::ld32(d_addr + 32 * c, d);
-        tc::wait_ld(d);
+      for (int e = 0; e < 32; e += 4) {
+        const float4 b = dl[e / 4];
+        const float2 x = mul2(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])),
+                              add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), make_float2(b.x, b.y)));
+        const float2 y = mul2(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])),
+                              add2(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), make_float2(b.z, b.w)));
+        w[e / 2] = tc::pack2<T>(x.x, x.y);
+        w[e / 2 + 1] = tc::pack2<T>(y.x, y.y);
+      }
+      if (masked) {
+        // dO V^T of a key that is not there may be NaN
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 b = dl[(32 * c + e) / 4];
-          const float2 x = mul2(make_float2(__uint_as_float(p[c][e]), __uint_as_float(p[c][e + 1])),
-                                add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), make_float2(b.x, b.y)));
-          const float2 y = mul2(make_float2(__uint_as_float(p[c][e + 2]), __uint_as_float(p[c][e + 3])),
-                                add2(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), make_float2(b.z, b.w)));
-          w[e / 2] = tc::pack2<T>(x.x, x.y);
-          w[e / 2 + 1] = tc::pack2<T>(y.x, y.y);
-        }
-        if (masked) {
-          // dO V^T of a key that is not there may be NaN
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (32 * c + 2 * e < from) w[e] &= 0xffff0000u;
-            if (32 * c + 2 * e + 1 < from) w[e] &= 0x0000ffffu;
-          }
-        }
-        // over columns 0-15 (16-31) of this half's 64, both already read when c = 0
-        if (c == 0) {
-          tc::st16(d_addr, w);
-        } else {
-          tc::st16(d_addr + 16, w);
+        for (int e = 0; e < 16; ++e) {
+          if (2 * e < from) w[e] &= 0xffff0000u;
+          if (2 * e + 1 < from) w[e] &= 0x0000ffffu;
         }
       }
+      tc::st16(d_addr, w);
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
@@ -584,16 +582,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
     } else if (t.first < t.n) {
       const bool live = key < t.n;
-      if (half == 0) {
+      const int c0 = (part & 1) * (DP / 2);  // parts 0, 1: dV, parts 2, 3: dK, half of the columns each
+      if (part < 2) {
         T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
-        store_grad<T, DP>(t_dv + lanes, out, a.d, 1.f, live, f.vec_dv, steps > 0);
+        store_grad<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, 1.f, live, f.vec_dv, steps > 0);
       } else {
         T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
-        store_grad<T, DP>(t_dk + lanes, out, a.d, a.scale, live, f.vec_dk, steps > 0);
+        store_grad<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, a.scale, live, f.vec_dk, steps > 0);
       }
-    } else if (a.cu != nullptr && t.n == 0) {
-      T* base = static_cast<T*>(half == 0 ? a.dv : a.dk) + hk * (half == 0 ? a.dvs.h : a.dks.h);
-      const int64_t st = half == 0 ? a.dvs.t : a.dks.t;
+    } else if (a.cu != nullptr && t.n == 0 && part < 2) {
+      T* base = static_cast<T*>(part == 0 ? a.dv : a.dk) + hk * (part == 0 ? a.dvs.h : a.dks.h);
+      const int64_t st = part == 0 ? a.dvs.t : a.dks.t;
       for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
         for (int x = threadIdx.x & 127; x < a.d; x += kRows) base[r * st + x] = Elem<T>::from_f(0.f);
     }
@@ -601,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::dealloc(tmem, 512);
+  if (warp == kWeightWarps) tc::dealloc(tmem, 512);
 }
 
 bool on16(const void* p, const AttnStrides& s, int64_t nb, int64_t heads) {

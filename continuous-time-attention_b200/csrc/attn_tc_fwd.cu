@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && tc::wait(&bars.p_full[i], ns & 1);
           tc::fence_after();
           if (ok && leader) {
-            tc::product_tn(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
             if (j + 1 == mine) tc::commit(&bars.o_full[i]);
             else scores(j + 1);
           }
