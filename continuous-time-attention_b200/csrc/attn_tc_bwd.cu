@@ -11,13 +11,14 @@
 // place.  Rows are (token, head) pairs as in the forward.
 //
 //   warps 0-15  weights: four warpgroups take 32 columns each of a 128 x 128 tile
-//   warp 16     MMAs      warp 17  TMA loads      warp 18  lse and delta (keys' kernel)
+//   warp 16  MMAs of the scores and of dO V^T    warp 17  TMA loads
+//   dQ:      warp 18  MMAs of dQ
+//   dK, dV:  warp 18  lse and delta              warp 19  MMAs of dV and dK
 //
 // Weights and score gradients go back to tensor memory as 16-bit A operands over
 // the columns their fp32 sources came from, so a tile pair crosses shared memory
-// only as Q, K, V and dO.  The MMA warp keeps the pipe busy across the two
-// dependent halves of a step: the next scores run while dS is computed, the
-// next dO V^T while the next P is.
+// only as Q, K, V and dO.  The next scores run while dS is computed, the next
+// dO V^T while the next P is.
 //
 // Bound by the products at dim 128 (7 x 512 cycles per tile pair against 2 x
 // 1024 of exponentials), by the exponentials at dim 64.
@@ -45,8 +46,12 @@ template <int DP>
 struct Layout {
   static constexpr int kHalf = kRows * 128;
   static constexpr int kTile = kHalf * (DP / 64);
-  static constexpr int kStages = DP == 128 ? 4 : 8;  // tiles of the other side in flight
+  // tiles of the other side in flight: a key tile is held until its dQ is done, and with four of 32 KB
+  // the next but one came too late (dQ at 8192 keys, 16 heads of 128: 4090 cycles a step)
+  static constexpr int kStages = DP == 128 ? 5 : 8;
   static constexpr int kSmem = (2 + kStages) * kTile + 1024;
+  static constexpr int kPairs = DP == 128 ? 2 : 4;  // (Q, dO) pairs of the keys' kernel
+  static constexpr int kSmemKv = (2 + 2 * kPairs) * kTile + 1024;
 };
 
 // COLS columns of a gradient's row from tensor memory, the first of them column c0 of d
@@ -91,7 +96,7 @@ __device__ __forceinline__ float neg_lse2_of(float lse) { return lse == neg_inf(
 // dQ
 // ---------------------------------------------------------------------------
 struct DqBars {
-  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], dp_full, dp_read, ds_full[2], done;
+  uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], s_free[2], dp_full, dp_read, ds_full[2], done;
 };
 
 template <typename T, int DP>
@@ -124,6 +129,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bars.s_full[0], 1);
     mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.s_free[0], 1);
+    mbar_init(&bars.s_free[1], 1);
     mbar_init(&bars.dp_full, 1);
     mbar_init(&bars.dp_read, kWeightWarps);
     mbar_init(&bars.ds_full[0], kWeightWarps);
@@ -185,51 +192,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int x = max(0, issued - NS); x < issued; ++x) tc::wait(&bars.kv_full[x % NS], (x / NS) & 1);
     }
   } else if (warp == kWeightWarps) {
-    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
+    // scores and dO V^T; another warp issues dQ: every wait takes a hundred cycles or two, and one warp
+    // for all three was what the steps waited for
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false);
     const bool leader = tc::elect_one();
     bool ok = steps == 0 || tc::wait(&bars.q_full, 0);
-    auto kv_wait = [&](int x) {
-      ok = ok && tc::wait(&bars.kv_full[x % NS], (x / NS) & 1);
-      tc::fence_after();
-    };
-    auto kv_addr = [&](int x) { return smem + (2 + x % NS) * L::kTile; };
-    auto scores = [&](int j) {
-      kv_wait(2 * j);
-      if (mask != nullptr || (j_lo + j + 1) * kRows > t.n) {
+    for (int j = 0; j < steps && ok; ++j) {
+      const uint32_t k = smem + (2 + (2 * j) % NS) * L::kTile, v = smem + (2 + (2 * j + 1) % NS) * L::kTile;
+      ok = tc::wait(&bars.kv_full[(2 * j) % NS], ((2 * j) / NS) & 1);
+      if (ok && (mask != nullptr || (j_lo + j + 1) * kRows > t.n)) {
         uint32_t w[4];
         key_words(j, w);
-        if (ok && !tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j), w);
+        if (!tc::all_set(w)) tc::clear_rows<DP / 64>(k, w);
       }
+      // the score gradients of step j - 2 lie in the buffer until they are in dQ
+      if (j >= 2) ok = ok && tc::wait(&bars.s_free[j & 1], ((j >> 1) - 1) & 1);
+      tc::fence_after();
       if (ok && leader) {
-        tc::product_nt<DP>(tmem + (j & 1) * 128, smem, kv_addr(2 * j), id_s);
+        tc::product_nt<DP>(tmem + (j & 1) * 128, smem, k, id_s);
         tc::commit(&bars.s_full[j & 1]);
       }
       __syncwarp();
-    };
-    auto grads = [&](int j) {
-      kv_wait(2 * j + 1);
+      ok = ok && tc::wait(&bars.kv_full[(2 * j + 1) % NS], ((2 * j + 1) / NS) & 1);
+      if (j >= 1) ok = ok && tc::wait(&bars.dp_read, (j - 1) & 1);
+      tc::fence_after();
       if (ok && leader) {
-        tc::product_nt<DP>(t_dp, smem + L::kTile, kv_addr(2 * j + 1), id_s);
+        tc::product_nt<DP>(t_dp, smem + L::kTile, v, id_s);
         tc::commit(&bars.dp_full);
         tc::commit(&bars.kv_empty[(2 * j + 1) % NS]);
       }
       __syncwarp();
-    };
-    if (steps > 0 && ok) {
-      scores(0);
-      if (ok) grads(0);
     }
+    if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+  } else if (warp == kWeightWarps + 2) {
+    constexpr uint32_t id_o = tc::idesc<T>(DP, true);
+    const bool leader = tc::elect_one();
+    bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
-      if (j + 1 < steps) {
-        scores(j + 1);
-        ok = ok && tc::wait(&bars.dp_read, j & 1);
-        tc::fence_after();
-        if (ok) grads(j + 1);
-      }
-      ok = ok && tc::wait(&bars.ds_full[j & 1], (j >> 1) & 1);
+      ok = tc::wait(&bars.ds_full[j & 1], (j >> 1) & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<32>(t_dq, tmem + (j & 1) * 128, kv_addr(2 * j), id_o, j > 0);
+        tc::product_tn<32>(t_dq, tmem + (j & 1) * 128, smem + (2 + (2 * j) % NS) * L::kTile, id_o, j > 0);
+        tc::commit(&bars.s_free[j & 1]);
         tc::commit(&bars.kv_empty[(2 * j) % NS]);
         if (j + 1 == steps) tc::commit(&bars.done);
       }
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // dK, dV: the tiles are transposed, rows are keys and columns are query rows
 // ---------------------------------------------------------------------------
 struct DkvBars {
-  uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], p_full[2], dp_full, ds_full, done;
+  uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], s_free[2], p_full[2], dp_full, dp_free, ds_full, done;
 };
 
 template <typename T, int DP>
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ BwdArgs f) {
   using L = Layout<DP>;
-  constexpr int NS = L::kStages / 2;  // (Q, dO) pairs in flight
+  constexpr int NS = L::kPairs;  // (Q, dO) pairs in flight
   extern __shared__ uint8_t smem_raw[];
   __shared__ DkvBars bars;
   __shared__ uint32_t s_tmem;
@@ -360,6 +364,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bars.s_full[0], 1);
     mbar_init(&bars.s_full[1], 1);
+    mbar_init(&bars.s_free[0], 1);
+    mbar_init(&bars.s_free[1], 1);
+    mbar_init(&bars.dp_free, 1);
     mbar_init(&bars.p_full[0], kWeightWarps);
     mbar_init(&bars.p_full[1], kWeightWarps);
     mbar_init(&bars.dp_full, 1);
@@ -442,62 +449,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) tc::arrive(&bars.stat_full[stage]);
     }
   } else if (warp == kWeightWarps) {
-    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
+    // K Q^T and V dO^T; another warp issues the gradients' products
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false);
     const bool leader = tc::elect_one();
     bool ok = steps == 0 || tc::wait(&bars.kv_full, 0);
-    auto q_addr = [&](int s) { return smem + (2 + 2 * (s % NS)) * L::kTile; };
-    // packed: rows of the next sequence in a tile that reaches past this one
-    auto clear_behind = [&](int s, uint32_t tile) {
+    for (int s = 0; s < steps && ok; ++s) {
+      const uint32_t q = smem + (2 + 2 * (s % NS)) * L::kTile, g = q + L::kTile;
+      ok = tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
+      // packed: rows of the next sequence in a tile that reaches past this one, in both tensors before
+      // anything is made of either
       const int rows = (t.n - first_of(s)) * f.pack;
-      if (ok && a.cu != nullptr && rows < kRows) {
+      if (a.cu != nullptr && rows < kRows) {
+        ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
         uint32_t w[4];
         tc::first_bits(rows, w);
-        tc::clear_rows<DP / 64>(tile, w);
+        if (ok) {
+          tc::clear_rows<DP / 64>(q, w);
+          tc::clear_rows<DP / 64>(g, w);
+        }
       }
-    };
-    auto scores = [&](int s) {
-      ok = ok && tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
+      // the weights of the step before in this buffer lie there until they are in dV
+      if (s >= NB) ok = ok && tc::wait(&bars.s_free[s % NB], ((s / NB) - 1) & 1);
       tc::fence_after();
-      clear_behind(s, q_addr(s));
       if (ok && leader) {
-        tc::product_nt<DP>(tmem + (s % NB) * 128, smem, q_addr(s), id_s);
+        tc::product_nt<DP>(tmem + (s % NB) * 128, smem, q, id_s);
         tc::commit(&bars.s_full[s % NB]);
       }
       __syncwarp();
-    };
-    auto grads = [&](int s) {
       ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
+      if (s >= 1) ok = ok && tc::wait(&bars.dp_free, (s - 1) & 1);
       tc::fence_after();
-      clear_behind(s, q_addr(s) + L::kTile);
       if (ok && leader) {
-        tc::product_nt<DP>(t_dp, smem + L::kTile, q_addr(s) + L::kTile, id_s);
+        tc::product_nt<DP>(t_dp, smem + L::kTile, g, id_s);
         tc::commit(&bars.dp_full);
       }
       __syncwarp();
-    };
-    if (steps > 0) {
-      scores(0);
-      grads(0);
     }
+    if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
+  } else if (warp == kWeightWarps + 3) {
+    constexpr uint32_t id_o = tc::idesc<T>(DP, true);
+    const bool leader = tc::elect_one();
+    bool ok = true;
     for (int s = 0; s < steps && ok; ++s) {
-      if (NB == 2 && s + 1 < steps) scores(s + 1);  // its buffer's weights went into dV at step s - 1
-      ok = ok && tc::wait(&bars.p_full[s & 1], (s >> 1) & 1);
+      const uint32_t q = smem + (2 + 2 * (s % NS)) * L::kTile, g = q + L::kTile;
+      ok = tc::wait(&bars.p_full[s & 1], (s >> 1) & 1) && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<32>(t_dv, tmem + (s % NB) * 128, q_addr(s) + L::kTile, id_o, s > 0);
-        tc::commit(&bars.g_empty[s % NS]);  // its dO V^T was done before
+        tc::product_tn<32>(t_dv, tmem + (s % NB) * 128, g, id_o, s > 0);
+        tc::commit(&bars.s_free[s % NB]);
       }
       __syncwarp();
-      if (NB == 1 && s + 1 < steps) scores(s + 1);
       ok = ok && tc::wait(&bars.ds_full, s & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<32>(t_dk, t_dp, q_addr(s), id_o, s > 0);
+        tc::product_tn<32>(t_dk, t_dp, q, id_o, s > 0);
+        tc::commit(&bars.dp_free);
         tc::commit(&bars.q_empty[s % NS]);
+        tc::commit(&bars.g_empty[s % NS]);  // dO V^T was done before the score gradients
         if (s + 1 == steps) tc::commit(&bars.done);
       }
       __syncwarp();
-      if (s + 1 < steps) grads(s + 1);
     }
     if (!ok && lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
   } else if (warp < kWeightWarps) {
@@ -633,7 +644,7 @@ cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k
   if (f.a.dk != nullptr) {
     const int64_t tiles = count_tiles(f.a, kRows);
     const cudaError_t e =
-        launch<attn_tc_dkv_kernel<T, DP>>(Layout<DP>::kSmem, tiles * f.a.Hk, q, g, k, v, f, st);
+        launch<attn_tc_dkv_kernel<T, DP>>(Layout<DP>::kSmemKv, tiles * f.a.Hk, q, g, k, v, f, st);
     if (e != cudaSuccess) return e;
   }
   if (f.a.dq == nullptr) return cudaSuccess;
