@@ -262,7 +262,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t s[32], dp[32];
       tc::ld32(s_addr, s);
       const int j0 = (j_lo + j) * kRows;
-      const bool whole = j0 + kRows <= t.n && mask == nullptr && !any_blind && (!a.causal || j0 + kRows - 1 <= limit_all);
+      bool whole = j0 + kRows <= t.n && !any_blind && (!a.causal || j0 + kRows - 1 <= limit_all);
+      uint32_t w[4];
+      if (mask != nullptr || !whole) {
+        key_words(j, w);
+        whole = whole && tc::all_set(w);
+      }
       tc::wait_ld(s);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
@@ -286,8 +291,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         dp[e + 1] = __float_as_uint(x.y);
       }
       if (!whole) {
-        uint32_t w[4];
-        key_words(j, w);
         const int left = none ? 0 : limit - j0 - 32 * part + 1;
         const uint32_t see = (part == 0 ? w[0] : part == 1 ? w[1] : part == 2 ? w[2] : w[3]) &
                              (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);

@@ -413,12 +413,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::ld32(s_addr, s[0]);
         tc::ld32(s_addr + 32, s[1]);
         // warp-uniform: every row of the warp sees all keys of the tile
-        bool whole = j0 + kRows <= n && mask == nullptr && (!a.causal || j0 + kRows - 1 <= limit_all);
-        if constexpr (PAGED) whole = whole && *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kt + j) & 15]) == 0xffu;
+        bool whole = j0 + kRows <= n && (!a.causal || j0 + kRows - 1 <= limit_all);
+        uint32_t w[4];
+        if (PAGED || mask != nullptr || !whole) {
+          key_words(n, mask, j0, kt + j, w);
+          whole = whole && tc::all_set(w);
+        }
         tc::wait_ld(s[0], s[1]);
         if (!whole) {
-          uint32_t w[4];
-          key_words(n, mask, j0, kt + j, w);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int left = limit - j0 - 64 * half - 32 * c + 1;

@@ -6,6 +6,7 @@ Modules
   pde_layers                   : DiffusionPDELayer & co. (src/models/pde_layers.py)
   transformers                 : PDE Transformer models (src/models/transformers.py)
   serving_vllm                 : CtaConfig / CtaPostAttnMixer (src/cta/serving_vllm.py)
+  attention                    : softmax attention of prompts, with gradients
   sharded                      : L-sharded stencil over NCCL for very long sequences
   ops                          : single-launch functional wrappers over the C ABI
   build                        : nvcc build of libcta_stencil.so

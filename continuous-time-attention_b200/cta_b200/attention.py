@@ -46,21 +46,25 @@ def prompt_attention(
     causal: bool = False,
     scale: Optional[float] = None,
     key_mask: Optional[torch.Tensor] = None,
+    mask_words: Optional[torch.Tensor] = None,
     cu_seqlens: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """softmax(scale * q k^T) v over the keys each row sees, differentiable in q, k, v.
 
     Padded: q [B, L, heads, dim], k and v [B, L, kv_heads, dim]; ``key_mask``
-    [B, L] (any mask dtype, non-zero = valid) hides padding.  Packed: [T, heads,
-    dim] with ``cu_seqlens`` (device int32, sequences + 1 offsets).  ``causal``:
+    [B, L] (any mask dtype, non-zero = valid) hides padding, or ``mask_words``,
+    its form from ``ops.attention_mask``, made once for several layers.  Packed:
+    [T, heads, dim] with ``cu_seqlens`` (device int32, sequences + 1 offsets).  ``causal``:
     row i sees keys j <= i of its sequence.  ``scale`` defaults to dim**-0.5.
 
     A row that sees no key is zero and has no gradient, as are packed rows
     behind the last sequence.  Masked keys may hold anything, infinities and NaN
     included; a NaN or infinity in the k or v of a valid token may also reach
     earlier rows of its sequence."""
-    words = None
+    words = mask_words
     if key_mask is not None:
+        if words is not None:
+            raise ValueError("give key_mask or mask_words, not both")
         if q.dim() != 4 or cu_seqlens is not None or key_mask.shape != q.shape[:2]:
             raise ValueError("key_mask must be (B, L) for padded q, k, v")
         if key_mask.device != q.device:

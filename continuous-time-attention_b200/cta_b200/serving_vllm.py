@@ -16,6 +16,9 @@ What changes:
   * every step count 1..8 is fused (the reference fuses only {1, 2, 4, 8} and
     loops single steps, rounding each, otherwise); ``fuse_any_steps=False``
     restores the reference's per-step rounding for the other counts.
+``CtaPostAttnMixer.attend`` is the layer's attention together with the mixer: it
+writes the batch's new keys and values into the paged cache (16-bit, or
+quantised to e4m3), attends over it and mixes, from the same metadata object.
 The kernels are the only compute path: ``use_triton`` is kept for config
 compatibility and a CPU tensor raises ``ValueError``.
 """
@@ -170,6 +173,51 @@ class CtaPostAttnMixer(nn.Module):
         if residual is not None and not fused:
             out = residual + out
         return out
+
+    def attend(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        *,
+        attn_metadata: object,
+        scale: Optional[float] = None,
+        k_scale: Optional[torch.Tensor] = None,
+        v_scale: Optional[torch.Tensor] = None,
+        is_prefill: Optional[bool] = None,
+        residual: Optional[torch.Tensor] = None,
+    ) -> torch.Tensor:
+        """Attention of a packed batch over the paged cache, then the mixer: [T, heads * dim].
+
+        q [T, heads, dim], k and v [T, kv_heads, dim] are the batch's new rows,
+        prompts, chunks of prompts and single decode tokens alike.
+        ``attn_metadata`` (vLLM 0.22's names) gives ``slot_mapping`` (where k and
+        v go in the cache, negative = nowhere), ``block_table``, ``seq_lens``
+        (the new tokens counted) and ``query_start_loc``, all on the device, and
+        ``max_query_len`` on the host.  The cache is [pages, page_size, kv_heads,
+        dim], in q's type or float8_e4m3fn with scales [pages, kv_heads,
+        page_size] (``ops.kv_cache_write``, ``ops.paged_attention``).  No device
+        data is read on the host.  Rows behind the last sequence come back
+        undefined, as the mixer leaves them; ``residual`` as for ``forward``."""
+        for name in ("slot_mapping", "block_table", "seq_lens", "query_start_loc"):
+            if getattr(attn_metadata, name, None) is None:
+                raise ValueError(f"attn_metadata has no {name}")
+        if q.dim() != 3:
+            raise ValueError("q must have shape (T, heads, dim)")
+        max_rows = _max_query_len(attn_metadata)
+        if max_rows is None:
+            raise ValueError("attn_metadata has no max_query_len")
+        slots = attn_metadata.slot_mapping
+        if slots.dim() != 1 or slots.shape[0] < k.shape[0]:
+            raise ValueError("slot_mapping must have an entry for every row of k")
+        ops.kv_cache_write(k, v, k_cache, v_cache, slots[: k.shape[0]], k_scale=k_scale, v_scale=v_scale)
+        out = ops.paged_attention(q, k_cache, v_cache, attn_metadata.block_table, attn_metadata.seq_lens,
+                                  cu_seqlens=self._device_qsl(attn_metadata.query_start_loc, q.device),
+                                  max_rows=max(1, max_rows), scale=scale, k_scale=k_scale, v_scale=v_scale)
+        return self.forward(out.view(q.shape[0], -1), attn_metadata=attn_metadata, is_prefill=is_prefill,
+                            residual=residual)
 
     def _mix(self, x, *, attn_metadata, is_prefill, residual):
         """(output, residual already added)."""

@@ -8,12 +8,23 @@ same forward.  The Transformer parts are stock PyTorch modules, exactly as in
 the reference; the only change is that the ``pde_steps`` refinement layers
 after each Transformer layer run as ONE fused launch forward and one backward
 (:124-133, :309-317), with no layout transposes for ``pde_layout="bld"``.
+
+``attention="fused"`` (default ``"torch"``: the stock modules, as above) runs the
+layers' attention on ``cta_b200.attention.prompt_attention``: same parameters,
+no L x L mask or scores in memory, forward or backward.  Two things differ from
+the stock modules: the attention weights themselves are not dropped out (the
+layers' other dropouts stay), and a row that sees no valid token (left padding
+under the causal mask) gets zeros from its attention, where softmax over nothing
+gives NaN.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
+from . import ops
+from .attention import prompt_attention
 from .pde_layers import (
     _DiffusionFamilyLayer,
     _TwoCoefficientLayer,
@@ -50,6 +61,31 @@ def _refine(x: torch.Tensor, pde_list: nn.ModuleList, layout: str, attention_mas
     return diffusion_pde_stack(x, pde_list, attention_mask=attention_mask)
 
 
+class _FusedAttentionLayer(nn.TransformerEncoderLayer):
+    """A post-norm encoder layer (same parameters and names) whose attention runs fused."""
+
+    def forward(self, x, mask_words, causal):  # type: ignore[override]
+        att = self.self_attn
+        B, L, E = x.shape
+        qkv = F.linear(x, att.in_proj_weight, att.in_proj_bias).view(B, L, 3, att.num_heads, E // att.num_heads)
+        q, k, v = qkv.unbind(2)
+        a = prompt_attention(q, k, v, causal=causal, mask_words=mask_words).reshape(B, L, E)
+        x = self.norm1(x + self.dropout1(att.out_proj(a)))
+        return self.norm2(x + self._ff_block(x))
+
+
+def _encoder_layers(attention, embed_dim, num_heads, hidden_dim, num_layers, dropout):
+    if attention not in ("torch", "fused"):
+        raise ValueError(f"attention must be 'torch' or 'fused', got {attention!r}")
+    cls = _FusedAttentionLayer if attention == "fused" else nn.TransformerEncoderLayer
+    return nn.ModuleList(
+        [
+            cls(d_model=embed_dim, nhead=num_heads, dim_feedforward=hidden_dim, dropout=dropout, batch_first=True)
+            for _ in range(num_layers)
+        ]
+    )
+
+
 class PDETransformerClassifier(nn.Module):
     """Sequence classifier with PDE refinement after every layer (transformers.py:35-142)."""
 
@@ -66,20 +102,15 @@ class PDETransformerClassifier(nn.Module):
         pde_layout: str = "bld",
         max_length=512,
         dropout=0.1,
+        attention: str = "torch",
         **pde_kwargs,
     ):
         super().__init__()
         self.embedding = nn.Embedding(vocab_size, embed_dim)
         self.pos_encoder = nn.Parameter(torch.randn(1, max_length, embed_dim))
         self.dropout = nn.Dropout(dropout)
-        self.transformer_layers = nn.ModuleList(
-            [
-                nn.TransformerEncoderLayer(
-                    d_model=embed_dim, nhead=num_heads, dim_feedforward=hidden_dim, dropout=dropout, batch_first=True
-                )
-                for _ in range(num_layers)
-            ]
-        )
+        self.attention = attention
+        self.transformer_layers = _encoder_layers(attention, embed_dim, num_heads, hidden_dim, num_layers, dropout)
         self.pde_layout = pde_layout
         self.pde_layers = nn.ModuleList(
             [
@@ -96,10 +127,17 @@ class PDETransformerClassifier(nn.Module):
         seq_len = x.size(1)
         x = x + self.pos_encoder[:, :seq_len, :]
         x = self.dropout(x)
-        padding_mask = attention_mask == 0
+        fused = self.attention == "fused"
+        if fused:
+            words = ops.attention_mask(attention_mask)
+        else:
+            padding_mask = attention_mask == 0
         n = len(self.transformer_layers)
         for i, (transformer_layer, pde_list) in enumerate(zip(self.transformer_layers, self.pde_layers)):
-            x = transformer_layer(x, src_key_padding_mask=padding_mask)
+            if fused:
+                x = transformer_layer(x, words, False)
+            else:
+                x = transformer_layer(x, src_key_padding_mask=padding_mask)
             if (i == n - 1 and self.pde_layout == "bld" and len(pde_list) > 0 and x.size(1) >= 3
                     and all(isinstance(l, _DiffusionFamilyLayer) and not l.causal for l in pde_list)):
                 # the last refinement and the masked mean pool in one pass
@@ -126,20 +164,15 @@ class PDETransformerLM(nn.Module):
         pde_layout: str = "bld",
         max_length=512,
         dropout=0.1,
+        attention: str = "torch",
         **pde_kwargs,
     ):
         super().__init__()
         self.embedding = nn.Embedding(vocab_size, embed_dim)
         self.pos_encoder = nn.Parameter(torch.randn(1, max_length, embed_dim))
         self.dropout = nn.Dropout(dropout)
-        self.transformer_layers = nn.ModuleList(
-            [
-                nn.TransformerEncoderLayer(
-                    d_model=embed_dim, nhead=num_heads, dim_feedforward=hidden_dim, dropout=dropout, batch_first=True
-                )
-                for _ in range(num_layers)
-            ]
-        )
+        self.attention = attention
+        self.transformer_layers = _encoder_layers(attention, embed_dim, num_heads, hidden_dim, num_layers, dropout)
         self.pde_layout = pde_layout
         self.pde_layers = nn.ModuleList(
             [
@@ -159,10 +192,17 @@ class PDETransformerLM(nn.Module):
         seq_len = x.size(1)
         x = x + self.pos_encoder[:, :seq_len, :]
         x = self.dropout(x)
-        padding_mask = torch.zeros_like(attention_mask, dtype=torch.float32)
-        padding_mask = padding_mask.masked_fill(attention_mask == 0, float("-inf"))
-        causal_mask = generate_causal_mask(seq_len, device=x.device)
+        fused = self.attention == "fused"
+        if fused:
+            words = ops.attention_mask(attention_mask)
+        else:
+            padding_mask = torch.zeros_like(attention_mask, dtype=torch.float32)
+            padding_mask = padding_mask.masked_fill(attention_mask == 0, float("-inf"))
+            causal_mask = generate_causal_mask(seq_len, device=x.device)
         for transformer_layer, pde_list in zip(self.transformer_layers, self.pde_layers):
-            x = transformer_layer(x, src_mask=causal_mask, src_key_padding_mask=padding_mask)
+            if fused:
+                x = transformer_layer(x, words, True)
+            else:
+                x = transformer_layer(x, src_mask=causal_mask, src_key_padding_mask=padding_mask)
             x = _refine(x, pde_list, self.pde_layout, attention_mask)
         return self.fc(x)
