@@ -98,6 +98,7 @@ struct PagedArgs {
   int workers;
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
+  int expanded;    // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages
 };
 
 // workers (warps) of the split kernel on the current device, and its launch
@@ -109,6 +110,9 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
 bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
 int attn_pack(int group);  // heads of a group that one row tile holds: its largest power of two
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
+// e4m3 caches: the pages that the table names, as 16-bit rows in page order (page i of sequence b is page
+// b * table_width + i), for the tensor-core kernel
+cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, cudaStream_t st);
 
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);

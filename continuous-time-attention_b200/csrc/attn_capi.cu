@@ -3,6 +3,7 @@
 // include/cta_stencil.h.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 
@@ -229,6 +230,31 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
   return CTA_OK;
 }
 
+// The tensor-core kernel takes 128 (row, head) pairs at once but has a CTA per pair of such tiles only;
+// the split kernel takes 16, reads the keys again for each 16, and fills the GPU whatever the shape.
+// Measured (32/8 heads of 128, B200): a 16-row tile costs the split kernel 0.11 ns per key, a pass of
+// the other kernel over one wave of its CTAs 15 ns per key, i.e. as much as 137 such tiles.  One
+// sequence of 8192 keys: 64 rows 96 us split, 142 us on tensor cores; 128 rows 179 and 144 us.  8
+// sequences of 4096: 8 rows 65 and 69 us, 16 rows 112 and 70 us.  Over an e4m3 cache the pages have to
+// be expanded first: 32 sequences of 2048, 8 rows 121 and 139 us, 16 rows 225 and 140 us.
+bool tensor_cores_pay(const PagedArgs& a) {
+  const int64_t group = a.H / a.Hk, pack = attn_pack(static_cast<int>(group));
+  if (a.cu == nullptr || a.max_rows * group <= 16 || !(a.scale > 0.f)) return false;
+  const int64_t b = a.B;
+  const int64_t tiles = std::max(b, (a.T * group + 15) / 16) * a.Hk;
+  const int64_t ctas = std::max(b, (a.T * pack + 255) / 256) * (a.H / pack);
+  return tiles > (a.k_scale != nullptr ? 256 : 128) * ((ctas + 147) / 148);
+}
+
+// 16-bit copy of the pages that the table can name, k then v; 0 where that is too much to ask for
+constexpr int64_t kMostExpanded = 1LL << 31;
+int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64_t d) {
+  const int64_t slots = b * width * page;
+  if (slots >= (1LL << 24) || slots * hk >= (1LL << 26)) return 0;
+  const int64_t bytes = slots * hk * d * 4;
+  return bytes <= kMostExpanded ? bytes : 0;
+}
+
 int64_t split_bytes(int workers, int d) {
   return 2LL * workers * 16 * ((d <= 64 ? 64 : 128) + 4) * static_cast<int64_t>(sizeof(float));
 }
@@ -287,22 +313,15 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream) {
   return launched(launch_cache_read(a, args->dtype, static_cast<cudaStream_t>(stream)), "cache read launch");
 }
 
-int64_t cta_paged_attention_workspace_bytes(int64_t rows_per_sequence, int64_t heads, int64_t kv_heads, int64_t dim,
-                                            int dtype, int quantized) {
-  if (kv_heads < 1 || dim < 1) return 0;
+int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args) {
   PagedArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.H = static_cast<int>(heads);
-  a.Hk = static_cast<int>(kv_heads);
-  a.d = static_cast<int>(dim);
-  // the larger of the two row variants, so that any max_rows up to this one fits
-  int workers = 0;
-  for (int64_t rows : {static_cast<int64_t>(1), rows_per_sequence}) {
-    a.max_rows = static_cast<int>(rows);
-    const int w = paged_split_workers(a, dtype, quantized);
-    workers = w > workers ? w : workers;
+  if (paged_args(args, a) != CTA_OK || a.T == 0 || a.B == 0) return 0;
+  if (tensor_cores_pay(a)) {
+    if (!args->quantized) return 0;
+    const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
+    if (bytes > 0) return bytes;
   }
-  return split_bytes(workers, a.d);
+  return split_bytes(paged_split_workers(a, args->dtype, args->quantized), a.d);
 }
 
 int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes,
@@ -322,15 +341,30 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
   for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // more rows than one operand of the split kernel holds: the tensor-core kernel
+  const int64_t need = cta_paged_attention_workspace_bytes(args);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
   cudaError_t e = cudaSuccess;
-  if (!args->quantized && static_cast<int64_t>(a.max_rows) * (a.H / a.Hk) > 16 &&
-      launch_paged_tc(a, args->dtype, st, &e))
-    return launched(e, "paged attention launch");
+  if (tensor_cores_pay(a)) {
+    const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
+    if (!args->quantized) {
+      if (launch_paged_tc(a, args->dtype, st, &e)) return launched(e, "paged attention launch");
+      return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");
+    }
+    if (bytes > 0) {
+      PagedArgs x = a;
+      char* k = static_cast<char*>(workspace);
+      char* v = k + bytes / 2;
+      e = launch_cache_expand(a, args->dtype, k, v, st);
+      if (e != cudaSuccess) return launched(e, "paged attention launch");
+      x.k_cache = k;
+      x.v_cache = v;
+      x.expanded = 1;
+      if (launch_paged_tc(x, args->dtype, st, &e)) return launched(e, "paged attention launch");
+      return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");
+    }
+  }
   a.workers = paged_split_workers(a, args->dtype, args->quantized);
-  if (workspace == nullptr || workspace_bytes < split_bytes(a.workers, a.d))
-    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)split_bytes(a.workers, a.d),
-                (long long)workspace_bytes);
   a.part_ml = static_cast<float*>(workspace);
   a.part_o = a.part_ml + 2LL * a.workers * 16 * 4;
   return launched(launch_paged_split(a, args->dtype, args->quantized, st), "paged attention launch");

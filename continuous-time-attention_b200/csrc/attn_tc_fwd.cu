@@ -1,6 +1,9 @@
 // Attention forward on the tensor cores: whole prompts, and chunks of rows over
 // a 16-bit paged cache.
 //
+// An e4m3 cache is first expanded to 16-bit pages (kv_cache.cu): one more rounding
+// of k and v, 2^-9 in bf16, like that of the weights.
+//
 // A CTA owns two 128-row tiles of one block of heads.  A row is a (token, head)
 // pair: where query heads share a key/value head, the largest power of two of
 // them that divides the group goes into one tile, token by token, so that a tile
@@ -51,6 +54,7 @@ struct FwdArgs {
   int64_t table_sB;
   const int32_t* seq_lens;
   int table_width, page, n_pages, box;  // box: keys per TMA box
+  int expanded;  // page i of sequence b is page b * table_width + i (the table still says which are valid)
   int vec_out;       // rows of the output are on 16 bytes
 };
 
@@ -260,6 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (page < 0 || page >= f.n_pages) {
               atomicExch(&g_tc_fwd_error, kDevBadIndex);
               page = -1;
+            } else if (f.expanded) {
+              page = x.t.seq * f.table_width + key / f.page;
             }
           }
           const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
@@ -625,12 +631,18 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
   f.table_width = p.table_width;
   f.page = p.page;
   f.n_pages = p.n_pages;
+  f.expanded = p.expanded;
   f.box = std::min(p.page & -p.page, kRows);  // the largest power of two that divides a page
   f.vec_out = 1;
+  // expanded pages are contiguous
+  const int64_t pages = p.expanded ? static_cast<int64_t>(p.B) * p.table_width : p.n_pages;
+  const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
+  const AttnStrides ks = p.expanded ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
+  const AttnStrides vs = p.expanded ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
   CUtensorMap q, k, v;
   if (!attn_map(&q, p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) ||
-      !attn_map(&k, p.k_cache, dtype, p.n_pages, p.page, p.Hk, p.d, AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH}, 1, f.box) ||
-      !attn_map(&v, p.v_cache, dtype, p.n_pages, p.page, p.Hk, p.d, AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH}, 1, f.box))
+      !attn_map(&k, p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) ||
+      !attn_map(&v, p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box))
     return false;
   const int64_t tiles = packed_tiles(p.T, p.B, 2 * f.tile_tokens);
   a.tiles = static_cast<int>(tiles);

@@ -189,6 +189,49 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   }
 }
 
+// code * scale of the pages of each sequence, in order, as 16-bit rows
+template <typename T>
+__global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out) {
+  constexpr int GROUP = 16;
+  const bool second = blockIdx.y != 0;
+  const unsigned blocks = (a.Hk + kHeads - 1) / kHeads;
+  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
+  const unsigned slots = static_cast<unsigned>(a.table_width) * a.page;  // per sequence
+  const unsigned row = group / blocks, b = row / slots, j = row - b * slots;
+  const int h0 = static_cast<int>(group - row * blocks) * kHeads, c = threadIdx.x % GROUP * 8;
+  if (b >= static_cast<unsigned>(a.B) || c >= a.d) return;
+  const int n = __ldg(a.seq_lens + b);
+  if (n < 0 || j >= static_cast<unsigned>(n)) return;
+  const int page = __ldg(a.table + b * a.table_sB + j / a.page);
+  if (page < 0 || page >= a.n_pages) return;  // reported by the kernel that reads them, which leaves them out
+  const unsigned slot = j % a.page;
+  const uint8_t* in = static_cast<const uint8_t*>(second ? a.v_cache : a.k_cache) + c +
+                      page * (second ? a.vc_sP : a.kc_sP) + slot * (second ? a.vc_sS : a.kc_sS);
+  const int64_t sH = second ? a.vc_sH : a.kc_sH;
+  const float* scale = (second ? a.v_scale : a.k_scale) + static_cast<int64_t>(page) * a.Hk * a.page + slot;
+  T* out = (second ? v_out : k_out) + static_cast<int64_t>(row) * a.Hk * a.d + c;
+  uint2 w[kHeads];
+  float mul[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i)
+    if (h0 + i < a.Hk) {
+      w[i] = __ldg(reinterpret_cast<const uint2*>(in + (h0 + i) * sH));
+      mul[i] = __ldg(scale + (h0 + i) * a.page);
+    }
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i)
+    if (h0 + i < a.Hk) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = from_e4m3x2(static_cast<uint16_t>((e < 2 ? w[i].x : w[i].y) >> (16 * (e & 1))));
+        f[2 * e] = v.x * mul[i];
+        f[2 * e + 1] = v.y * mul[i];
+      }
+      *reinterpret_cast<uint4*>(out + (h0 + i) * a.d) = pack8<T>(f);
+    }
+}
+
 template <typename T, int GROUP>
 cudaError_t launch(const CacheArgs& a, bool write, cudaStream_t st) {
   const int64_t groups = a.T * ((a.Hk + kHeads - 1) / kHeads);
@@ -216,6 +259,19 @@ cudaError_t dispatch(const CacheArgs& a, int dtype, bool write, cudaStream_t st)
 
 cudaError_t launch_cache_write(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, true, st); }
 cudaError_t launch_cache_read(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, false, st); }
+
+cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, cudaStream_t st) {
+  const int64_t groups = static_cast<int64_t>(p.B) * p.table_width * p.page * ((p.Hk + kHeads - 1) / kHeads);
+  const int64_t ctas = (groups * 16 + kThreads - 1) / kThreads;
+  if (groups >= (1LL << 28)) return cudaErrorInvalidConfiguration;  // the caller's limit keeps it below
+  const dim3 grid(static_cast<unsigned>(ctas), 2u);
+  if (ctas == 0) return cudaSuccess;
+  if (dtype == kBF16)
+    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+  else
+    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__half*>(k), static_cast<__half*>(v));
+  return cudaGetLastError();
+}
 
 int read_device_error_cache(int clear) {
   int v = 0;

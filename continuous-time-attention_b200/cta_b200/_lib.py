@@ -103,7 +103,7 @@ _SIGNATURES = {
     "cta_attention_mask_words": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "cta_kv_cache_write": (c_int, [c_void_p, c_void_p]),
     "cta_kv_cache_read": (c_int, [c_void_p, c_void_p]),
-    "cta_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "cta_paged_attention_workspace_bytes": (c_int64, [c_void_p]),
     "cta_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
 }
 

@@ -833,9 +833,6 @@ def kv_cache_read(
     return k, v
 
 
-_PAGED_BYTES: dict = {}  # workspace bytes by what they depend on
-
-
 def paged_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -856,7 +853,8 @@ def paged_attention(
     q [T, heads, dim]; cu_seqlens (int32, B + 1) gives the rows of each of the B
     sequences, None one row each (decode).  seq_lens [B] (int32) counts all keys
     of a sequence, block_table [B, width] (int32) lists its pages.  Row r of n_r
-    sees keys j <= seq_len - n_r + r.  max_rows, the longest n_r as the host
+    sees keys j <= seq_len - n_r + r.  Chunks over an e4m3 cache may be computed
+    from a 16-bit copy of the keys and values.  max_rows, the longest n_r as the host
     knows it, only chooses the kernel.  No device data is read on the host.
     Rows that see no key are zero; rows behind the last sequence are not
     written.  A page outside the cache or a length past the table counts as no
@@ -895,19 +893,17 @@ def paged_attention(
         if not _on16(o):
             raise ValueError("out must have rows that start on 16 bytes")
     lib = _lib.load()
-    max_rows = int(max_rows)
-    key = (q.get_device(), code, quantized, dim, heads // kv_heads, min(max_rows, 16))
-    nbytes = _PAGED_BYTES.get(key)
-    if nbytes is None:
-        with _lib.on_device(q):
-            nbytes = lib.cta_paged_attention_workspace_bytes(max_rows, heads, kv_heads, dim, code, int(quantized))
-        _PAGED_BYTES[key] = nbytes
-    # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     args = _lib.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
         table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o), *_row_strides(k_cache),
         *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, table.shape[1],
-        max_rows, code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
-    _lib.enqueue(lib.cta_paged_attention, q, args, ws.data_ptr(), nbytes)
+        int(max_rows), code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
+    if _lib._current_device() == q.get_device():
+        nbytes = lib.cta_paged_attention_workspace_bytes(args)
+    else:
+        with _lib.on_device(q):
+            nbytes = lib.cta_paged_attention_workspace_bytes(args)
+    # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.enqueue(lib.cta_paged_attention, q, args, _lib.ptr(ws), nbytes)
     return o

@@ -381,8 +381,10 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
  * data.  A page outside the cache or a length past the table counts as no keys
  * and is reported by cta_device_error() as 2.  page_size: a multiple of 16;
  * dim: a multiple of 16 up to 128; dtype: CTA_BF16, CTA_F16 (of q and out).
- * workspace: cta_paged_attention_workspace_bytes(max_rows, ...) bytes on 16,
- * not shared by calls that may overlap; it needs no clearing. */
+ * Chunks over an e4m3 cache may be computed from a 16-bit copy of k and v.
+ * workspace: cta_paged_attention_workspace_bytes(args) bytes (sizes, types and
+ * strides of args count, not its pointers; 0 = none) on 16, not shared by calls
+ * that may overlap; it needs no clearing. */
 typedef struct cta_paged_attention_args {
   const void* q;
   void* out;
@@ -399,8 +401,7 @@ typedef struct cta_paged_attention_args {
   float scale, reserved;
 } cta_paged_attention_args;
 
-int64_t cta_paged_attention_workspace_bytes(int64_t rows_per_sequence, int64_t heads, int64_t kv_heads, int64_t dim,
-                                            int dtype, int quantized);
+int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args);
 int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -214,9 +214,12 @@ class Setup:
             i = torch.arange(n - r, n, device="cuda")
             see = torch.arange(n, device="cuda")[None, :] <= i[:, None]
             want, _ = A.attention(q, self.k[b], self.v[b], see, scale)
-            # e4m3: q is rounded to fp16 after an exact scaling, elements below 2^-14 of the largest to 2^-25 of
-            # it: with d elements that is d 2^-25 of |q||k|, inside the (d + 4) 2^-24 of the scores' bound
-            tol = A.bounds(q, self.k[b], self.v[b], see, scale, self.dtype, kv_error=2.0**-20 if self.quantized else 0.0)
+            # e4m3, few rows: q is rounded to fp16 after an exact scaling, elements below 2^-14 of the largest to
+            # 2^-25 of it: with d elements that is d 2^-25 of |q||k|, inside the (d + 4) 2^-24 of the scores'
+            # bound.  More rows than one operand holds: k and v may first be rounded to 16 bits, half a step.
+            many = max(self.rows) * (q.shape[1] // self.k[b].shape[1]) > 16
+            kv_error = 0.0 if not self.quantized else torch.finfo(self.dtype).eps / 2 if many else 2.0**-20
+            tol = A.bounds(q, self.k[b], self.v[b], see, scale, self.dtype, kv_error=kv_error)
             bad = ~((got - want).abs() <= tol)
             assert not bad.any(), (b, n, r, int(bad.sum()), (got - want).abs().max().item(), tol.min().item())
 
@@ -257,17 +260,36 @@ def test_chunks(rows, quantized, dtype):
         s.check(s.run())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("rows", [[64, 64, 64], [1, 0, 300], [17, 1, 130], [128, 129, 127], [300, 64, 0], [1, 400, 33]])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(32, 8, 128, 16), (24, 8, 64, 48), (32, 32, 80, 128), (64, 4, 32, 64)])
+def test_chunks_of_many_heads(heads, kv_heads, dim, page, rows, quantized, dtype):
+    """Enough rows and heads for the tensor-core kernel."""
+    lens = [r + x for r, x in zip(rows, (0, 77, 500))]
+    s = Setup(lens, rows, heads, kv_heads, dim, page, dtype, quantized, seed=sum(rows), tail=2)
+    out = torch.full_like(s.q, 7.0)
+    s.run(out=out)
+    s.check(out)
+    assert (out[sum(rows):] == 7).all()
+    if dim == 128 and not quantized:
+        # any scale, the signs of it too
+        s.check(s.run(scale=0.02), 0.02)
+        s.check(s.run(scale=-0.02), -0.02)
+
+
 @pytest.mark.parametrize("quantized", [False, True])
 def test_lengths_zero_and_short(quantized):
     """No keys at all; more rows than keys (the first rows see nothing)."""
     s = Setup([0, 5, 0, 200], [1, 1, 1, 1], 4, 2, 64, 16, torch.bfloat16, quantized)
     s.check(s.run())
-    s = Setup([0, 3, 50], [2, 3, 7], 4, 2, 64, 16, torch.bfloat16, quantized)
-    s.check(s.run())
-    s.seq_lens[2] = 4
-    out = s.run()
-    rows = out[5:12]
-    assert (rows[:3] == 0).all() and (rows[3:] != 0).any() and torch.isfinite(rows.float()).all()
+    for more in (0, 150):  # split and tensor-core kernels
+        s = Setup([0, 3, 50 + more], [2, 3, 7 + more], 32, 8, 64, 16, torch.bfloat16, quantized)
+        s.check(s.run())
+        s.seq_lens[2] = 4 + more
+        out = s.run()
+        rows = out[5:12 + more]
+        assert (rows[:3] == 0).all() and (rows[3:] != 0).any() and torch.isfinite(rows.float()).all()
 
 
 @pytest.mark.parametrize("quantized", [False, True])
@@ -325,7 +347,7 @@ def test_e4m3_scales_far_apart(spread):
 @pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
 @pytest.mark.parametrize("quantized", [False, True])
 def test_rows_behind_the_last_sequence(rows, quantized):
-    s = Setup([100, 300], rows, 4, 2, 64, 16, torch.bfloat16, quantized, tail=3)
+    s = Setup([100, 300], rows, 32, 8, 64, 16, torch.bfloat16, quantized, tail=3)
     out = torch.full_like(s.q, 7.0)
     y = s.run(out=out, cu_seqlens=s.cu)
     assert y is out and (out[sum(rows):] == 7).all()
@@ -338,7 +360,7 @@ def test_bad_pages_and_lengths(rows, quantized):
     """Skipped and reported; the other sequence keeps its result."""
     from cta_b200 import _lib
 
-    s = Setup([100, 300], rows, 4, 2, 64, 16, torch.bfloat16, quantized)
+    s = Setup([100, 300], rows, 32, 8, 64, 16, torch.bfloat16, quantized)
     want = s.run()
     good = s.table.clone()
     for bad in (-1, s.kc.shape[0], 2**31 - 1, -(2**31)):
@@ -360,7 +382,7 @@ def test_bad_pages_and_lengths(rows, quantized):
 
 @pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
 def test_max_rows_is_a_hint(rows):
-    s = Setup([100, 300], rows, 8, 2, 64, 16, torch.bfloat16, False)
+    s = Setup([100, 300], rows, 32, 8, 64, 16, torch.bfloat16, False)
     for hint in (1, 3, 100, 1000):
         s.check(s.run(max_rows=hint, cu_seqlens=s.cu))
 
@@ -389,7 +411,7 @@ def test_large_cache(quantized):
     slots2 = torch.arange(n, device="cuda")
     ops.kv_cache_write(k, v, kc2, vc2, slots2, k_scale=ks2, v_scale=vs2)
     lens = torch.tensor([n], dtype=torch.int32, device="cuda")
-    for rows in (1, 200):
+    for rows in (1, 400):
         q = torch.randn(rows, 16, dim, device="cuda").to(dtype)
         cu = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
         a = ops.paged_attention(q, kc, vc, torch.tensor([mine], dtype=torch.int32, device="cuda"), lens, cu_seqlens=cu,
@@ -403,8 +425,8 @@ def test_large_cache(quantized):
 @pytest.mark.parametrize("quantized", [False, True])
 def test_captured_twice_and_replayed_together(rows, quantized):
     """Two graphs captured on one stream, replayed at the same time on two: each has its own workspace."""
-    s = Setup([1500, 300, 2200], rows, 8, 2, 128, 16, torch.bfloat16, quantized)
-    other = Setup([900, 2000, 800], rows, 8, 2, 128, 16, torch.bfloat16, quantized, seed=5)
+    s = Setup([1500, 300, 2200], rows, 32, 8, 128, 16, torch.bfloat16, quantized)
+    other = Setup([900, 2000, 800], rows, 32, 8, 128, 16, torch.bfloat16, quantized, seed=5)
     want, want2 = s.run(), other.run()
     side = torch.cuda.Stream()
     graphs, outs = [], []
@@ -426,7 +448,7 @@ def test_captured_twice_and_replayed_together(rows, quantized):
 def test_twice_the_same():
     for quantized in (False, True):
         for rows in ([1, 1, 1], [50, 3, 170]):
-            s = Setup([1500, 300, 2200], rows, 8, 2, 128, 16, torch.bfloat16, quantized)
+            s = Setup([1500, 300, 2200], rows, 32, 8, 128, 16, torch.bfloat16, quantized)
             assert torch.equal(s.run(), s.run())
 
 
