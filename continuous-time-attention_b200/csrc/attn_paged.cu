@@ -17,9 +17,11 @@
 //   is permuted so that a lane ends with the consecutive elements it loaded.
 //   The weights change sides by a transposing move.  tcgen05 would need 128 rows
 //   where there are 1 to 16.
-// * Every warp is a worker.  The 16-key groups of all (sequence, row tile, head)
-//   segments form one list, cut into equal runs, one per worker, whatever the
-//   lengths are; the host never reads them.  A worker that holds only a part
+// * Every warp is a worker.  The 16-key groups of all (sequence, row tile)
+//   segments form one list, cut into equal runs, one per worker of a key/value
+//   head, whatever the lengths are; the host never reads them.  The workers of
+//   all heads walk the list side by side, so that the rows of a token, which lie
+//   next to each other, are read at about the same time.  A worker that holds only a part
 //   of a segment leaves (maximum, sum, weighted values) in 32 bits, and a second
 //   kernel, launched as a programmatic dependent, joins the parts of a segment
 //   in worker order.  Nothing is atomic, so results do not depend on timing.
@@ -31,6 +33,8 @@
 // element, which loses only what is below 2^-24 of that element.  The key's
 // scale multiplies the score in 32 bits.  The value's scale joins the weight,
 // whose own running maximum keeps weight * scale within fp16 for any scales.
+#include <algorithm>
+
 #include "attn_common.cuh"
 
 namespace cta {
@@ -80,7 +84,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
 
 // rows of a segment: `tile` consecutive (row, head of the group) pairs
 struct Seg {
-  int b, tile, hk;
+  int b, tile;
   int n, rows;         // keys and rows of the sequence
   int64_t row0;        // its first row in q
   int group, groups;   // first group of this call and groups of the segment
@@ -109,7 +113,7 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b, int tile_
   }
   s.tiles = (s.rows * (a.H / a.Hk) + tile_rows - 1) / tile_rows;
   s.groups = max(1, (n + kGroup - 1) / kGroup);  // a sequence without keys still writes its zeros
-  s.units = static_cast<int64_t>(s.tiles) * a.Hk * s.groups;
+  s.units = static_cast<int64_t>(s.tiles) * s.groups;
   return s;
 }
 
@@ -125,8 +129,9 @@ __device__ __forceinline__ int64_t total_units(const PagedArgs& a, int tile_rows
   return warp_sum(u);
 }
 
-__device__ __forceinline__ int active_workers(const PagedArgs& a, int64_t units) {
-  return static_cast<int>(min(static_cast<int64_t>(a.workers), max(static_cast<int64_t>(1), units / kMinGroups)));
+// workers per key/value head, of a.workers / Hk
+__device__ __forceinline__ int active_shares(const PagedArgs& a, int64_t units) {
+  return static_cast<int>(min(static_cast<int64_t>(a.workers / a.Hk), max(static_cast<int64_t>(1), units / kMinGroups)));
 }
 
 // the segment that holds unit u (u < total); whole warp
@@ -154,8 +159,7 @@ __device__ __forceinline__ Seg find_segment(const PagedArgs& a, int64_t u, int t
       const int64_t first = before + __shfl_sync(0xffffffffu, upto - s.units, src);
       const int64_t seg = (u - first) / g.groups;
       g.group = static_cast<int>((u - first) - seg * g.groups);
-      g.hk = static_cast<int>(seg % a.Hk);
-      g.tile = static_cast<int>(seg / a.Hk);
+      g.tile = static_cast<int>(seg);
       g.start = first + seg * g.groups;
       return g;
     }
@@ -191,10 +195,11 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
   const int worker = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t units = total_units(a, ROWS);
   if (units == 0) return;
-  const int workers = active_workers(a, units);
-  if (worker >= workers) return;
-  int64_t u = units * worker / workers;
-  const int64_t u_end = units * (worker + 1) / workers;
+  const int shares = active_shares(a, units);
+  const int hk = worker % a.Hk, share = worker / a.Hk;
+  if (share >= shares) return;
+  int64_t u = units * share / shares;
+  const int64_t u_end = units * (share + 1) / shares;
   bool first = true;
   const int group = a.H / a.Hk;
 
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       const int i = g.tile * ROWS + oct + 8 * r;
       const int tok = i / group;
       const bool live = tok < g.rows;
-      const T* q = static_cast<const T*>(a.q) + (g.row0 + tok) * a.q_sT + (g.hk * group + i - tok * group) * a.q_sH;
+      const T* q = static_cast<const T*>(a.q) + (g.row0 + tok) * a.q_sT + (hk * group + i - tok * group) * a.q_sH;
       float top = 0.f, mul = a.scale * kLog2e;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -250,6 +255,14 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       }
     }
 
+    // Last key that every row of the tile sees.  Rows behind the sequence's last count as seeing all: theirs are
+    // not written.  (So do rows that see nothing; then no other row of the tile sees 16 keys.)
+    int least = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) least = min(least, last[r][e] < 0 ? 0x7fffffff : last[r][e]);
+    least = __reduce_min_sync(0xffffffffu, least);
     float o[MT][NR][4];
     float m[NR][2], l[NR][2], mv[NR][2];  // reference of the weights, their sum, reference of the weighted values
 #pragma unroll
@@ -274,13 +287,29 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       return p;
     };
     using C = typename std::conditional<FP8, uint8_t, T>::type;
-    const C* k_base = static_cast<const C*>(a.k_cache) + g.hk * a.kc_sH + KE * quad;
-    const C* v_base = static_cast<const C*>(a.v_cache) + g.hk * a.vc_sH + VE * oct;
+    const C* k_base = static_cast<const C*>(a.k_cache) + hk * a.kc_sH + KE * quad;
+    const C* v_base = static_cast<const C*>(a.v_cache) + hk * a.vc_sH + VE * oct;
     uint4 kf[2][KL];
     float ks[2], vs[2];
     uint32_t vf[4][VL][VW];
+    // A group that lies in the cache and the sequence whole, of full rows, loads without conditions
+    const bool full_rows = a.d == DP;
     auto load_keys = [&](int grp, int p, int slot) {
       const C* at = k_base + p * a.kc_sP + (slot + oct) * a.kc_sS;
+      const int64_t x = FP8 ? (static_cast<int64_t>(p) * a.Hk + hk) * a.page + slot + oct : 0;
+      if (full_rows && p >= 0 && (grp + 1) * kGroup <= g.n) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int i = 0; i < KL; ++i) kf[t][i] = __ldg(reinterpret_cast<const uint4*>(at + 4 * KE * i));
+          if constexpr (FP8) {
+            ks[t] = __ldg(a.k_scale + x + 8 * t);
+            vs[t] = __ldg(a.v_scale + x + 8 * t);
+          }
+          at += 8 * a.kc_sS;
+        }
+        return;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const bool ok = p >= 0 && grp * kGroup + 8 * t + oct < g.n;
@@ -291,14 +320,31 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
             kf[t][i] = __ldg(reinterpret_cast<const uint4*>(at + 8 * t * a.kc_sS + 4 * KE * i));
         }
         if constexpr (FP8) {
-          const int64_t x = (static_cast<int64_t>(p) * a.Hk + g.hk) * a.page + slot + 8 * t + oct;
-          ks[t] = ok ? __ldg(a.k_scale + x) : 1.f;
-          vs[t] = ok ? __ldg(a.v_scale + x) : 1.f;
+          ks[t] = ok ? __ldg(a.k_scale + x + 8 * t) : 1.f;
+          vs[t] = ok ? __ldg(a.v_scale + x + 8 * t) : 1.f;
         }
+      }
+    };
+    auto load_row = [&](uint32_t (&w)[VW], const C* q) {
+      if constexpr (VW == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(q));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
+        w[0] = v.x, w[1] = v.y;
       }
     };
     auto load_values = [&](int grp, int p, int slot) {
       const C* at = v_base + p * a.vc_sP + (slot + 2 * quad) * a.vc_sS;
+      if (full_rows && p >= 0 && (grp + 1) * kGroup <= g.n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int x = 0; x < VL; ++x) load_row(vf[i][x], at + 8 * VE * x);
+          at += (i == 1 ? 7 : 1) * a.vc_sS;  // keys 2 quad + {0, 1, 8, 9}
+        }
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = (i & 1) + 8 * (i >> 1);
@@ -307,16 +353,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
         for (int x = 0; x < VL; ++x) {
 #pragma unroll
           for (int w = 0; w < VW; ++w) vf[i][x][w] = 0u;
-          if (ok && 8 * VE * x + VE * oct < a.d) {
-            const C* q = at + k * a.vc_sS + 8 * VE * x;
-            if constexpr (VW == 4) {
-              const uint4 w = __ldg(reinterpret_cast<const uint4*>(q));
-              vf[i][x][0] = w.x, vf[i][x][1] = w.y, vf[i][x][2] = w.z, vf[i][x][3] = w.w;
-            } else {
-              const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
-              vf[i][x][0] = w.x, vf[i][x][1] = w.y;
-            }
-          }
+          if (ok && 8 * VE * x + VE * oct < a.d) load_row(vf[i][x], at + k * a.vc_sS + 8 * VE * x);
         }
       }
     };
@@ -370,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       }
       if (it + 1 < count) load_keys(grp + 1, page_next, slot_next);
 
+      const bool all_see = here && (grp + 1) * kGroup <= least + 1;
       // weights of keys oct, oct + 8 in rows 2 quad, 2 quad + 1
       uint32_t pf[NR][2];
 #pragma unroll
@@ -383,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
           for (int t = 0; t < 2; ++t) {
             float x = s[r][2 * t + e] * c2[r][e];
             if constexpr (FP8) x *= ksc[t];
-            const bool see = here && grp * kGroup + 8 * t + oct <= last[r][e];
+            const bool see = all_see || (here && grp * kGroup + 8 * t + oct <= last[r][e]);
             y[t][e] = see ? x : neg_inf();
             top[e] = fmaxf(top[e], y[t][e]);
             if constexpr (FP8) {
@@ -483,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
         if (whole) {
           float mul = 0.f;
           if (sum > 0.f || sum != sum) mul = __fdividef(ex2((FP8 ? mv[r][e] - m[r][e] : 0.f) - kShift), sum);
-          T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (g.hk * group + i - tok * group) * a.o_sH;
+          T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (hk * group + i - tok * group) * a.o_sH;
 #pragma unroll
           for (int x = 0; x < VL; ++x) {
             const int c = 8 * VE * x + VE * oct;
@@ -554,14 +592,14 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   const SeqInfo s = seq_info(a, b, ROWS);
   const int i = first_row * group + (h - hk * group);
   const int tile = i / ROWS, r = i - tile * ROWS;
-  const int64_t u0 = before + (static_cast<int64_t>(tile) * a.Hk + hk) * s.groups, u1 = u0 + s.groups;
-  const int64_t workers = active_workers(a, units);
+  const int64_t u0 = before + static_cast<int64_t>(tile) * s.groups, u1 = u0 + s.groups;
+  const int64_t workers = active_shares(a, units);
   const int64_t w0 = ((u0 + 1) * workers - 1) / units, w1 = (u1 * workers - 1) / units;
   if (w0 == w1) return;  // one worker held it all and wrote the output
   const int parts = static_cast<int>(w1 - w0 + 1);
   auto slot_of = [&](int x) -> int64_t {
     const int64_t w = w0 + x;
-    return 2 * w + (x == 0 && units * w / workers < u0 ? 1 : 0);
+    return 2 * (w * a.Hk + hk) + (x == 0 && units * w / workers < u0 ? 1 : 0);
   };
   constexpr int V = DP / 32;
   float m = neg_inf(), l = 0.f, mv = neg_inf(), o[V];
@@ -627,12 +665,12 @@ struct Split {
         n = 1;
       per_sm = n;
     }
-    return per_sm * num_sms_here() * (kThreads / 32);
+    return per_sm * num_sms_here() * (kThreads / 32);  // what the GPU holds at a time
   }
   static cudaError_t run(const PagedArgs& a, cudaStream_t st) {
     constexpr bool kHalf = FP8 || std::is_same<T, __half>::value;
     paged_split_kernel<T, FP8, DP, ROWS>
-        <<<static_cast<unsigned>(a.workers / (kThreads / 32)), kThreads, 0, st>>>(a);
+        <<<static_cast<unsigned>((a.workers + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     // about as many warps as a segment has parts when all are equally long
@@ -677,7 +715,9 @@ auto with_variant(const PagedArgs& a, int dtype, int quantized, G&& g) {
 }  // namespace
 
 int paged_split_workers(const PagedArgs& a, int dtype, int quantized) {
-  return with_variant<Split>(a, dtype, quantized, [](auto f) { return f.workers(); });
+  // the same number for every head, one at least
+  const int all = with_variant<Split>(a, dtype, quantized, [](auto f) { return f.workers(); });
+  return std::max(1, all / a.Hk) * a.Hk;
 }
 
 cudaError_t launch_paged_split(const PagedArgs& a, int dtype, int quantized, cudaStream_t st) {

@@ -219,8 +219,9 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 def enqueue(fn, t: torch.Tensor, *args) -> None:
     """fn(*args, stream) on t's device and its current stream; raises on a non-zero status."""
-    if _current_device() == t.get_device():
-        rc = fn(*args, stream_ptr(t))
+    device = t.get_device()
+    if _current_device() == device and _raw_stream is not None:
+        rc = fn(*args, _raw_stream(device))
     else:
         with on_device(t):
             rc = fn(*args, stream_ptr(t))

@@ -545,22 +545,23 @@ def _device_ints(t: torch.Tensor, name: str, like: torch.Tensor, dtype: torch.dt
 
 
 def _offsets(cu: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
-    if cu.dim() != 1 or cu.numel() < 1:
+    shape = cu.shape
+    if len(shape) != 1 or shape[0] < 1:
         raise ValueError("cu_seqlens must have shape (sequences + 1,)")
-    if cu.dtype != torch.int32 or cu.device != like.device:
+    if cu.dtype != torch.int32 or cu.get_device() != like.get_device():
         cu = _device_ints(cu, "cu_seqlens", like, torch.int32)
     return cu if cu.is_contiguous() else cu.contiguous()
 
 
 def _on16(t: torch.Tensor) -> bool:
     """The last axis is contiguous, and every row starts on 16 bytes and on its own."""
-    s = t.stride()
-    if s[-1] != 1 or t.data_ptr() & 15:
+    if t.data_ptr() & 15:
         return False
     es = t.element_size()
     if t.is_contiguous():
         return t.shape[-1] * es & 15 == 0  # the other strides are multiples of a row
-    return all(n <= 1 or (x > 0 and x * es & 15 == 0) for x, n in zip(s[:-1], t.shape))
+    s = t.stride()
+    return s[-1] == 1 and all(n <= 1 or (x > 0 and x * es & 15 == 0) for x, n in zip(s[:-1], t.shape))
 
 
 def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
@@ -578,10 +579,12 @@ def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
 
 def _attention_inputs(q, k, v, cu_seqlens, mask_words, scale):
     """Checked inputs and sizes: (q, k, v, cu or None, (sequences, length, heads, kv_heads, dim), dtype code, scale)."""
-    _require_cuda(q, "q")
-    dtype, device = q.dtype, q.device
+    device = q.get_device()  # plain numbers: comparing device objects costs several times as much
+    if device < 0:
+        _require_cuda(q, "q")
+    dtype = q.dtype
     code = _lib.dtype_code(dtype)
-    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+    if k.dtype != dtype or v.dtype != dtype or k.get_device() != device or v.get_device() != device:
         _same_kind(k, "k", q)
         _same_kind(v, "v", q)
     shape, kshape = q.shape, k.shape
@@ -597,7 +600,7 @@ def _attention_inputs(q, k, v, cu_seqlens, mask_words, scale):
     cu = None
     if cu_seqlens is None:
         sequences = shape[0]
-        if mask_words is not None and (mask_words.dtype != torch.int32 or mask_words.device != device
+        if mask_words is not None and (mask_words.dtype != torch.int32 or mask_words.get_device() != device
                                        or not mask_words.is_contiguous()
                                        or mask_words.shape != (sequences, _mask_row_words(length))):
             raise ValueError("mask_words must come from attention_mask() of a (B, L) mask")
@@ -702,11 +705,13 @@ def attention_backward(
     n, length, heads = sizes[:3]
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"grad_out and out must be {tuple(q.shape)}")
-    if grad_out.dtype != q.dtype or out.dtype != q.dtype or grad_out.device != q.device or out.device != q.device:
+    device = q.get_device()
+    if (grad_out.dtype != q.dtype or out.dtype != q.dtype or grad_out.get_device() != device
+            or out.get_device() != device):
         _same_kind(grad_out, "grad_out", q)
         _same_kind(out, "out", q)
     shape = (n, heads, length) if cu is None else (heads, length)
-    if lse.shape != shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+    if lse.shape != shape or lse.dtype != torch.float32 or lse.get_device() != device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 {shape} on {q.device}")
     g, o = _attention_rows(grad_out, code), _attention_rows(out, code)
     dq = _new(q) if need_dq else None
@@ -742,10 +747,10 @@ def _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, like):
     if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have one shape (pages, page_size, kv_heads, dim)")
     quantized = kind == torch.float8_e4m3fn
-    device = like.device
-    if (not quantized and kind != dtype) or v_cache.dtype != kind or k_cache.device != device or (
-            v_cache.device != device):
-        raise ValueError(f"k_cache and v_cache must be {dtype} or float8_e4m3fn on {device}, got {kind} on "
+    device = like.get_device()
+    if (not quantized and kind != dtype) or v_cache.dtype != kind or k_cache.get_device() != device or (
+            v_cache.get_device() != device):
+        raise ValueError(f"k_cache and v_cache must be {dtype} or float8_e4m3fn on {like.device}, got {kind} on "
                          f"{k_cache.device} and {v_cache.dtype} on {v_cache.device}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and not (k_cache.data_ptr() | v_cache.data_ptr()) & 15
             and shape[3] & 15 == 0) and not (_on16(k_cache) and _on16(v_cache)):
@@ -754,18 +759,20 @@ def _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, like):
     if quantized:
         want = (pages, heads, page)
         for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-            if (t is None or t.shape != want or t.dtype != torch.float32 or t.device != device
+            if (t is None or t.shape != want or t.dtype != torch.float32 or t.get_device() != device
                     or not t.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous float32 {want} on {device}")
+                raise ValueError(f"{name} must be a contiguous float32 {want} on {like.device}")
     elif k_scale is not None or v_scale is not None:
         raise ValueError("k_scale and v_scale go with a float8_e4m3fn cache")
     return pages, page, heads, dim, quantized
 
 
 def _slots(slots: torch.Tensor, n: Optional[int], like: torch.Tensor) -> torch.Tensor:
-    if slots.dim() != 1 or (n is not None and slots.shape[0] != n):
+    shape = slots.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n):
         raise ValueError("slots must have shape (T,)")
-    slots = _device_ints(slots, "slots", like, torch.int64)
+    if slots.dtype != torch.int64 or slots.get_device() != like.get_device():
+        slots = _device_ints(slots, "slots", like, torch.int64)
     return slots if slots.is_contiguous() else slots.contiguous()
 
 
@@ -797,14 +804,17 @@ def kv_cache_write(
     page s // page_size.  A negative slot is skipped (padding rows); the others
     must be distinct.  A slot past the cache is skipped and reported by
     ``_lib.device_error()``."""
-    _require_cuda(k, "k")
-    if k.dim() != 3 or k.shape != v.shape:
+    if k.get_device() < 0:
+        _require_cuda(k, "k")
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape:
         raise ValueError("k and v must have one shape (T, kv_heads, dim)")
-    _same_kind(v, "v", k)
+    if v.dtype != k.dtype or v.get_device() != k.get_device():
+        _same_kind(v, "v", k)
     sizes = _cache_sizes(k_cache, v_cache, k_scale, v_scale, k.dtype, k)
-    if k.shape[1:] != k_cache.shape[2:]:
-        raise ValueError(f"k {tuple(k.shape)} does not fit a cache {tuple(k_cache.shape)}")
-    slots = _slots(slots, k.shape[0], k)
+    if shape[1] != sizes[2] or shape[2] != sizes[3]:
+        raise ValueError(f"k {tuple(shape)} does not fit a cache {tuple(k_cache.shape)}")
+    slots = _slots(slots, shape[0], k)
     k = k if _on16(k) else _own_rows(k)
     v = v if _on16(v) else _own_rows(v)
     _cache_call(_lib.load().cta_kv_cache_write, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
@@ -821,7 +831,8 @@ def kv_cache_read(
 ):
     """The rows k, v [T, kv_heads, dim] that slots [T] hold, as `dtype` (bf16 / fp16; None:
     the cache's own type, bf16 for e4m3); zeros for a negative slot.  One launch."""
-    _require_cuda(k_cache, "k_cache")
+    if k_cache.get_device() < 0:
+        _require_cuda(k_cache, "k_cache")
     if dtype is None:
         dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
     sizes = _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, k_cache)
@@ -859,31 +870,35 @@ def paged_attention(
     Rows that see no key are zero; rows behind the last sequence are not
     written.  A page outside the cache or a length past the table counts as no
     keys and is reported by ``_lib.device_error()``."""
-    _require_cuda(q, "q")
-    if q.dim() != 3:
+    device = q.get_device()
+    if device < 0:
+        _require_cuda(q, "q")
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("q must have shape (T, heads, dim)")
     code = _lib.dtype_code(q.dtype)
     pages, page, kv_heads, dim, quantized = _cache_sizes(k_cache, v_cache, k_scale, v_scale, q.dtype, q)
-    rows, heads, q_dim = q.shape
+    rows, heads, q_dim = shape
     if q_dim != dim or heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"q {tuple(q.shape)} does not go with a cache {tuple(k_cache.shape)}")
     table, lens = block_table, seq_lens
-    if table.dtype != torch.int32 or table.device != q.device:
+    if table.dtype != torch.int32 or table.get_device() != device:
         table = _device_ints(table, "block_table", q, torch.int32)
-    if lens.dtype != torch.int32 or lens.device != q.device:
+    if lens.dtype != torch.int32 or lens.get_device() != device:
         lens = _device_ints(lens, "seq_lens", q, torch.int32)
-    if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
+    tshape, lshape = table.shape, lens.shape
+    if len(tshape) != 2 or len(lshape) != 1 or tshape[0] != lshape[0]:
         raise ValueError("block_table must have shape (B, width), seq_lens (B,)")
     if table.stride(1) != 1:
         table = table.contiguous()
     if not lens.is_contiguous():
         lens = lens.contiguous()
-    batch = lens.shape[0]
+    batch = lshape[0]
     cu = None
     if cu_seqlens is not None:
         cu = _offsets(cu_seqlens, q)
-        if cu.numel() != batch + 1:
-            raise ValueError(f"cu_seqlens must have {batch + 1} entries, got {cu.numel()}")
+        if cu.shape[0] != batch + 1:
+            raise ValueError(f"cu_seqlens must have {batch + 1} entries, got {cu.shape[0]}")
     if not _on16(q):
         q = _own_rows(q)
     if out is None:
@@ -896,9 +911,9 @@ def paged_attention(
     args = _lib.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
         table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o), *_row_strides(k_cache),
-        *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, table.shape[1],
+        *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, tshape[1],
         int(max_rows), code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
-    if _lib._current_device() == q.get_device():
+    if _lib._current_device() == device:
         nbytes = lib.cta_paged_attention_workspace_bytes(args)
     else:
         with _lib.on_device(q):
