@@ -47,16 +47,18 @@ __device__ __forceinline__ void clamp_range(const int32_t* cu, int i, int64_t to
 // the result.  Packed: the lanes walk the offsets 32 sequences at a time with a
 // prefix sum of the tile counts, so that the host never reads the offsets.
 // Tiles of a sequence are numbered from its end when `backwards` (the last
-// tiles of a causal sequence have the most keys and start first).
+// tiles of a causal sequence have the most keys and start first).  Not packed:
+// `across` takes the same tile of all sequences, then the next, and otherwise
+// one sequence follows the other.
 __device__ __forceinline__ SeqTile find_tile(const int32_t* cu, int nseq, int64_t L, int tiles, int tile, int rows,
-                                             bool backwards) {
+                                             bool backwards, bool across) {
   SeqTile t;
   t.tail_index = t.tail_count = 0;
   if (cu == nullptr) {
-    t.seq = t.batch = tile / tiles;
+    const int i = across ? tile / nseq : tile % tiles;
+    t.seq = t.batch = across ? tile % nseq : tile / tiles;
     t.row0 = 0;
     t.n = static_cast<int>(L);
-    const int i = tile - t.seq * tiles;
     t.first = (backwards ? tiles - 1 - i : i) * rows;
     return t;
   }
@@ -118,6 +120,36 @@ cudaError_t allow_smem(int bytes) {
   e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return e;
+}
+
+inline int num_sms_here() {
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
+  return v;
+}
+
+// Launches a kernel.  `beside`: its CTAs may start as soon as all of the kernel in
+// front of it in the stream have started (that one calls pdl_launch_dependents,
+// and this one reads nothing of it), so that they fill the SMs that its last CTAs
+// leave idle; every CTA calls pdl_wait before it ends, so that the stream goes on
+// only when both are done.
+template <auto Kernel, typename... Args>
+cudaError_t launch_grid(bool beside, int64_t ctas, int threads, int smem, cudaStream_t st, const Args&... args) {
+  const cudaError_t e = allow_smem<Kernel>(smem);
+  if (e != cudaSuccess) return e;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, Kernel, args...);
 }
 
 // Sets rows behind the last sequence to zero, head h, `d` elements each.

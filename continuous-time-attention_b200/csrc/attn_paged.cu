@@ -574,7 +574,7 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
     int n;
     clamp_range(a.cu, 0, a.T, begin, n);
     if (row < begin) return;
-    const SeqTile t = find_tile(a.cu, a.B, a.T, static_cast<int>(a.T) + 1, static_cast<int>(row - begin), 1, false);
+    const SeqTile t = find_tile(a.cu, a.B, a.T, static_cast<int>(a.T) + 1, static_cast<int>(row - begin), 1, false, false);
     if (t.n == 0) return;  // behind the last sequence
     b = t.seq;
     first_row = t.first;
@@ -645,13 +645,6 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
 #pragma unroll
   for (int e = 0; e < V; ++e)
     if (lane + 32 * e < a.d) out[lane + 32 * e] = Elem<T>::from_f(o[e] * mul);
-}
-
-int num_sms_here() {
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
-  return v;
 }
 
 template <typename T, bool FP8, int DP, int ROWS>

@@ -172,7 +172,7 @@ __device__ __forceinline__ float sum8(float x) {
 __device__ __forceinline__ SeqTile block_tile(const AttnArgs& a, int tile, int rows, bool backwards) {
   __shared__ SeqTile t;
   if (threadIdx.x < 32) {
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, tile, rows, backwards);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, tile, rows, backwards, a.causal);
     if (threadIdx.x == 0) t = x;
   }
   __syncthreads();
@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
   const SeqTile t = block_tile(a, blockIdx.x / a.H, kSimtRows, a.causal);
   if (t.first >= t.n) {
     if (a.cu != nullptr) zero_rows<T>(a.dq, a.dqs, t.row0, a.L, h, a.d, t.tail_index, t.tail_count);
+    pdl_wait();
     return;
   }
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
@@ -332,6 +333,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
 #pragma unroll
   for (int r = 0; r < R; ++r) mul[r] = a.scale;
   store_rows<T, R, DC>(a.dq, a.dqs, t, h, acc, mul, a.d, ty, tx);
+  pdl_wait();  // launched beside dK and dV
 }
 
 // owns KT keys of one key/value head; rows of the score tile are keys, columns are queries
@@ -346,6 +348,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   float* P = G + QT * (DP + kPad);
   __shared__ float s_lse[QT], s_delta[QT];
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
+  pdl_launch_dependents();  // dQ's CTAs may follow
   // early keys of a causal sequence meet the most queries: forwards is heaviest first
   const SeqTile t = block_tile(a, blockIdx.x / a.Hk, KT, false);
   if (t.first >= t.n) {
@@ -477,16 +480,6 @@ __global__ void attn_mask_words_kernel(const void* mask, int dtype, int64_t sB, 
   if (threadIdx.x < kMaskHead) w[threadIdx.x] = threadIdx.x == 0 ? s_lo : threadIdx.x == 1 ? s_hi : 0u;
 }
 
-// smem is the same for every launch of a kernel
-template <auto Kernel>
-cudaError_t launch(const AttnArgs& a, int64_t ctas, size_t smem, cudaStream_t st) {
-  const cudaError_t e = allow_smem<Kernel>(static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  Kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(a);
-  return cudaGetLastError();
-}
-
 int64_t count_tiles(AttnArgs& a, int rows) {
   if (a.cu != nullptr) {
     a.tiles = static_cast<int>(packed_tiles(a.L, a.nseq, rows));
@@ -496,27 +489,28 @@ int64_t count_tiles(AttnArgs& a, int rows) {
   return static_cast<int64_t>(a.tiles) * a.nseq;
 }
 
+// shared memory is the same for every launch of a kernel
 template <typename T, int DP>
 cudaError_t fwd(AttnArgs a, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
-  const size_t smem = sizeof(float) * ((kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
+  constexpr int smem = sizeof(float) * ((kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
   const int64_t tiles = count_tiles(a, kSimtRows);
-  return launch<attn_simt_fwd_kernel<T, DP>>(a, tiles * a.H, smem, st);
+  return launch_grid<attn_simt_fwd_kernel<T, DP>>(false, tiles * a.H, kThreads, smem, st, a);
 }
 
 template <typename T, int DP>
 cudaError_t bwd(AttnArgs a, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
-  if (a.dq != nullptr) {
-    const size_t smem = sizeof(float) * ((2 * kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
-    const int64_t tiles = count_tiles(a, kSimtRows);
-    const cudaError_t e = launch<attn_simt_dq_kernel<T, DP>>(a, tiles * a.H, smem, st);
+  if (a.dk != nullptr) {
+    constexpr int smem = sizeof(float) * (4 * KT * (DP + kPad) + KT * (KT + kPad));
+    const int64_t tiles = count_tiles(a, KT);
+    const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP>>(false, tiles * a.Hk, kThreads, smem, st, a);
     if (e != cudaSuccess) return e;
   }
-  if (a.dk == nullptr) return cudaSuccess;
-  const size_t smem = sizeof(float) * (4 * KT * (DP + kPad) + KT * (KT + kPad));
-  const int64_t tiles = count_tiles(a, KT);
-  return launch<attn_simt_dkv_kernel<T, DP>>(a, tiles * a.Hk, smem, st);
+  if (a.dq == nullptr) return cudaSuccess;
+  constexpr int smem = sizeof(float) * ((2 * kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
+  const int64_t tiles = count_tiles(a, kSimtRows);
+  return launch_grid<attn_simt_dq_kernel<T, DP>>(a.dk != nullptr, tiles * a.H, kThreads, smem, st, a);
 }
 
 template <typename T>

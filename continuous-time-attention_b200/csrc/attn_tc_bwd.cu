@@ -39,7 +39,7 @@ constexpr int kRows = 128;
 struct BwdArgs {
   AttnArgs a;
   int pack, tile_tokens;
-  int vec_dq, vec_dk, vec_dv;  // rows of the gradient are on 16 bytes
+  int wide_dq, wide_dk, wide_dv;  // alignment of the gradients' rows, see store_rows
 };
 
 template <int DP>
@@ -53,40 +53,6 @@ struct Layout {
   static constexpr int kPairs = DP == 128 ? 2 : 4;  // (Q, dO) pairs of the keys' kernel
   static constexpr int kSmemKv = (2 + 2 * kPairs) * kTile + 1024;
 };
-
-// COLS columns of a gradient's row from tensor memory, the first of them column c0 of d
-template <typename T, int COLS>
-__device__ __forceinline__ void store_grad(uint32_t addr, T* out, int c0, int d, float mul, bool live, bool vec, bool any) {
-#pragma unroll
-  for (int c = 0; c < COLS / 16; ++c) {
-    uint32_t o[16];
-    if (any) {
-      tc::ld16(addr + 16 * c, o);
-      tc::wait_ld(o);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] = 0u;
-    }
-    if (!live) continue;
-    const int at = c0 + 16 * c;
-    if (vec) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 8)
-        if (at + e < d) {
-          uint4 x;
-          uint32_t* xp = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            xp[y] = tc::pack2<T>(__uint_as_float(o[e + 2 * y]) * mul, __uint_as_float(o[e + 2 * y + 1]) * mul);
-          *reinterpret_cast<uint4*>(out + at + e) = x;
-        }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (at + e < d) out[at + e] = Elem<T>::from_f(__uint_as_float(o[e]) * mul);
-    }
-  }
-}
 
 // the row's share of the sums: a row that sees no key, or lies outside, has weight zero everywhere
 __device__ __forceinline__ bool blind(float neg_lse2) { return neg_lse2 == neg_inf(); }
@@ -117,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h0 = static_cast<int>(blockIdx.x % blocks) * f.pack, hk = h0 / (a.H / a.Hk);
 
   if (warp == 0) {
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal, a.causal);
     if (lane == 0) s_tile = x;
   } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
@@ -313,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
     } else if (t.first < t.n) {
       T* out = static_cast<T*>(a.dq) + t.batch * a.dqs.b + (t.row0 + tok) * a.dqs.t + h * a.dqs.h;
-      store_grad<T, DP / 4>(t_dq + lanes + part * (DP / 4), out, part * (DP / 4), a.d, a.scale, live, f.vec_dq, steps > 0);
+      tc::store_rows<T, DP / 4>(t_dq + lanes + part * (DP / 4), out, part * (DP / 4), a.d, a.scale, live, f.wide_dq, steps > 0);
     } else if (a.cu != nullptr && t.n == 0 && part == 0) {
       for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
         for (int x = threadIdx.x; x < a.d * f.pack; x += kRows)
@@ -324,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
+  pdl_wait();  // launched beside dK and dV
 }
 
 // ---------------------------------------------------------------------------
@@ -349,10 +316,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
+  pdl_launch_dependents();  // dQ's CTAs may follow
 
   if (warp == 0) {
     // the first keys of a causal sequence meet the most rows: forwards is heaviest first
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false, a.causal);
     if (lane == 0) s_tile = x;
   } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
@@ -599,10 +567,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c0 = (part & 1) * (DP / 2);  // parts 0, 1: dV, parts 2, 3: dK, half of the columns each
       if (part < 2) {
         T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
-        store_grad<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, 1.f, live, f.vec_dv, steps > 0);
+        tc::store_rows<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, 1.f, live, f.wide_dv, steps > 0);
       } else {
         T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
-        store_grad<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, a.scale, live, f.vec_dk, steps > 0);
+        tc::store_rows<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, a.scale, live, f.wide_dk, steps > 0);
       }
     } else if (a.cu != nullptr && t.n == 0 && part < 2) {
       T* base = static_cast<T*>(part == 0 ? a.dv : a.dk) + hk * (part == 0 ? a.dvs.h : a.dks.h);
@@ -617,11 +585,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
 }
 
-bool on16(const void* p, const AttnStrides& s, int64_t nb, int64_t heads) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s.t % 8 == 0 && (heads == 1 || s.h % 8 == 0) &&
-         (nb == 1 || s.b % 8 == 0);
-}
-
 int64_t count_tiles(AttnArgs& a, int rows) {
   if (a.cu != nullptr) {
     a.tiles = static_cast<int>(packed_tiles(a.L, a.nseq, rows));
@@ -631,28 +594,19 @@ int64_t count_tiles(AttnArgs& a, int rows) {
   return static_cast<int64_t>(a.tiles) * a.nseq;
 }
 
-template <auto Kernel>
-cudaError_t launch(int smem, int64_t ctas, const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k,
-                   const CUtensorMap& v, const BwdArgs& f, cudaStream_t st) {
-  const cudaError_t e = allow_smem<Kernel>(smem);
-  if (e != cudaSuccess) return e;
-  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  Kernel<<<static_cast<unsigned>(ctas), kThreads, smem, st>>>(q, g, k, v, f);
-  return cudaGetLastError();
-}
-
 template <typename T, int DP>
 cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k, const CUtensorMap& v, BwdArgs f,
                 cudaStream_t st) {
   if (f.a.dk != nullptr) {
     const int64_t tiles = count_tiles(f.a, kRows);
     const cudaError_t e =
-        launch<attn_tc_dkv_kernel<T, DP>>(Layout<DP>::kSmemKv, tiles * f.a.Hk, q, g, k, v, f, st);
+        launch_grid<attn_tc_dkv_kernel<T, DP>>(false, tiles * f.a.Hk, kThreads, Layout<DP>::kSmemKv, st, q, g, k, v, f);
     if (e != cudaSuccess) return e;
   }
   if (f.a.dq == nullptr) return cudaSuccess;
   const int64_t tiles = count_tiles(f.a, f.tile_tokens);
-  return launch<attn_tc_dq_kernel<T, DP>>(Layout<DP>::kSmem, tiles * (f.a.H / f.pack), q, g, k, v, f, st);
+  return launch_grid<attn_tc_dq_kernel<T, DP>>(f.a.dk != nullptr, tiles * (f.a.H / f.pack), kThreads, Layout<DP>::kSmem,
+                                               st, q, g, k, v, f);
 }
 
 }  // namespace
@@ -670,9 +624,9 @@ bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
       !attn_map(&k, a.k, dtype, nb, a.L, a.Hk, a.d, a.ks, 1, kRows) ||
       !attn_map(&v, a.v, dtype, nb, a.L, a.Hk, a.d, a.vs, 1, kRows))
     return false;
-  f.vec_dq = a.dq != nullptr && on16(a.dq, a.dqs, nb, a.H);
-  f.vec_dk = a.dk != nullptr && on16(a.dk, a.dks, nb, a.Hk);
-  f.vec_dv = a.dv != nullptr && on16(a.dv, a.dvs, nb, a.Hk);
+  f.wide_dq = row_alignment(a.dq, a.dqs, nb, a.H);
+  f.wide_dk = row_alignment(a.dk, a.dks, nb, a.Hk);
+  f.wide_dv = row_alignment(a.dv, a.dvs, nb, a.Hk);
   if (dtype == kBF16)
     *e = a.d <= 64 ? run<__nv_bfloat16, 64>(q, g, k, v, f, st) : run<__nv_bfloat16, 128>(q, g, k, v, f, st);
   else
