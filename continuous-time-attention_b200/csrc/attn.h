@@ -20,6 +20,7 @@ struct AttnArgs {
   const void* q;
   const void* k;
   const void* v;
+  void* low;         // 16-bit: what rounding o lost, times low_scale<T>(), rows {L * H * d, H * d, d}; or nullptr
   void* o;           // forward: output.  backward: the forward's output (read)
   float* lse;        // [nseq, H, L] dense, [H, L] packed; natural logarithm, -inf for a row without keys
   const void* g;     // backward: gradient of the output

@@ -90,6 +90,7 @@ int prompt_args(const cta_attention_args* p, AttnArgs& a) {
   a.k = p->k;
   a.v = p->v;
   a.o = p->out;
+  a.low = p->dtype == CTA_F32 ? nullptr : p->out_low;
   a.lse = p->lse;
   a.g = p->grad_out;
   a.delta = p->delta;

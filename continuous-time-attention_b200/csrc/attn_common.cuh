@@ -152,6 +152,19 @@ cudaError_t launch_grid(bool beside, int64_t ctas, int threads, int smem, cudaSt
   return cudaLaunchKernelEx(&cfg, Kernel, args...);
 }
 
+// The backward takes delta = sum_d g * o from an o that rounding has moved.  The
+// error, up to 2^-9 |g| |o| in bf16, is the same for all keys of a row; it is small
+// beside the rounding of the single P (dP - delta) in long rows, but not where few
+// keys make o large: over sequences of 1 to 16 tokens the gradients were 2 to 3 times
+// as far off as one rounding of them.  So a training forward keeps o's lost part.
+// In fp16 it is scaled, or it would be subnormal for |o| < 2^-3.
+template <typename T> __host__ __device__ constexpr float low_scale() { return 1.f; }
+template <> __host__ __device__ constexpr float low_scale<__half>() { return 2048.f; }
+template <typename T>
+__device__ __forceinline__ float lost(float x) {
+  return (x - Elem<T>::to_f(Elem<T>::from_f(x))) * low_scale<T>();
+}
+
 // Sets rows behind the last sequence to zero, head h, `d` elements each.
 template <typename T>
 __device__ __forceinline__ void zero_rows(void* base, const AttnStrides& s, int64_t begin, int64_t end, int h, int d,

@@ -138,7 +138,7 @@ __device__ __forceinline__ void mm_nn(float4 (&acc)[R][DC], const float* P, cons
   }
 }
 
-template <typename T, int R, int DC>
+template <typename T, int R, int DC, bool LOW = false>
 __device__ __forceinline__ void store_rows(void* base, const AttnStrides& s, const SeqTile& t, int h,
                                            const float4 (&acc)[R][DC], const float (&mul)[R], int d, int ty, int tx) {
   T* p = static_cast<T*>(base) + t.batch * s.b + t.row0 * s.t + h * s.h;
@@ -152,7 +152,7 @@ __device__ __forceinline__ void store_rows(void* base, const AttnStrides& s, con
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int c = 4 * tx + 32 * x + e;
-        if (c < d) p[static_cast<int64_t>(i) * s.t + c] = Elem<T>::from_f(v[e] * mul[r]);
+        if (c < d) p[static_cast<int64_t>(i) * s.t + c] = Elem<T>::from_f(LOW ? lost<T>(v[e] * mul[r]) : v[e] * mul[r]);
       }
     }
   }
@@ -263,6 +263,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
       a.lse[lse_index(a, t, h, i)] = l[r] == 0.f ? neg_inf() : (m[r] + log2f(l[r])) * kLn2;
   }
   store_rows<T, R, DC>(a.o, a.os, t, h, acc, inv, a.d, ty, tx);
+  if (!std::is_same<T, float>::value && a.low != nullptr)
+    store_rows<T, R, DC, true>(a.low, AttnStrides{a.L * a.H * a.d, static_cast<int64_t>(a.H) * a.d, a.d}, t, h, acc, inv,
+                               a.d, ty, tx);
 }
 
 // weights and d(scores) of a tile pair from the scores s and the products dp = dO.V
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   store_rows<T, R, DC>(a.dv, a.dvs, t, hk, dv, one, a.d, ty, tx);
 }
 
-// delta_i = sum_d g_i o_i.  GROUP lanes per (row, head), 16 bytes of each tensor per lane and step (VEC elements;
+// delta_i = sum_d g_i o_i, o_i with what its rounding lost where that was kept.  GROUP lanes per (row, head), 16 bytes of each tensor per lane and step (VEC elements;
 // one element where rows do not start on 16 bytes): bound by HBM, two tensors read once.
 template <typename T, int GROUP, int VEC>
 __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t rows) {
@@ -430,17 +433,25 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t ro
     at = (b * a.H + h) * a.L + i;
     const T* o = static_cast<const T*>(a.o) + b * a.os.b + i * a.os.t + h * a.os.h;
     const T* g = static_cast<const T*>(a.g) + b * a.gs.b + i * a.gs.t + h * a.gs.h;
+    const T* low = a.low != nullptr ? static_cast<const T*>(a.low) + w * a.d : nullptr;
     for (int c = lane * VEC; c < a.d; c += GROUP * VEC) {
       if constexpr (VEC == 1) {
-        s = fmaf(Elem<T>::to_f(o[c]), Elem<T>::to_f(g[c]), s);
+        float x = Elem<T>::to_f(o[c]);
+        if (low != nullptr) x = fmaf(Elem<T>::to_f(low[c]), 1.f / low_scale<T>(), x);
+        s = fmaf(x, Elem<T>::to_f(g[c]), s);
       } else {
-        float x[4], y[4];
+        float x[4], y[4], z[4];
 #pragma unroll
         for (int e = 0; e < VEC; e += 4) {
           load_vec<T, 4>(o + c + e, x);
           load_vec<T, 4>(g + c + e, y);
+          if (low != nullptr) {
+            load_vec<T, 4>(low + c + e, z);
 #pragma unroll
-          for (int z = 0; z < 4; ++z) s = fmaf(x[z], y[z], s);
+            for (int w4 = 0; w4 < 4; ++w4) x[w4] = fmaf(z[w4], 1.f / low_scale<T>(), x[w4]);
+          }
+#pragma unroll
+          for (int w4 = 0; w4 < 4; ++w4) s = fmaf(x[w4], y[w4], s);
         }
       }
     }
@@ -548,7 +559,8 @@ template <typename T>
 cudaError_t delta(const AttnArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
   const int64_t rows = (a.cu != nullptr ? a.L : a.L * a.nseq) * a.H;
-  const bool vec = a.d % kVec == 0 && rows_on16<T>(a.o, a.os) && rows_on16<T>(a.g, a.gs);
+  const bool vec = a.d % kVec == 0 && rows_on16<T>(a.o, a.os) && rows_on16<T>(a.g, a.gs) &&
+                   reinterpret_cast<uintptr_t>(a.low) % 16 == 0;
   const int group = vec && a.d <= 8 * kVec ? 8 : vec && a.d <= 16 * kVec ? 16 : 32;
   const int64_t ctas = (rows * group + 255) / 256;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;

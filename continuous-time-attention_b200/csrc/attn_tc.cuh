@@ -251,13 +251,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 
 // Writes N columns, from `col` on, of the rows that a warp's lanes have in tensor
 // memory (one row per lane), times `scale`; `any` false: zeros.  `wide` is the
-// alignment of the output's rows in bytes, 32 or 16, or 0 for neither.
+// alignment of the output's rows in bytes, 32 or 16, or 0 for neither.  LOW
+// writes what rounding loses instead (see lost()).
 //
 // With one row per lane a store touches 32 rows, and the SM takes the rows one
 // after another.  So up to four lanes exchange their 32-byte pieces first, and a
 // store writes 64 or 128 bytes each of 16 or 8 rows: prompts of 1024 tokens, 32/8
 // heads of 128, causal, take 281 us instead of 328 with 16 bytes per lane and 302 with 32.
-template <typename T, int N>
+template <typename T, int N, bool LOW = false>
 __device__ __forceinline__ void store_rows(uint32_t taddr, T* out, int col, int d, float scale, bool live, int wide,
                                            bool any) {
   constexpr int NC = N / 16;  // pieces of a lane
@@ -276,7 +277,10 @@ __device__ __forceinline__ void store_rows(uint32_t taddr, T* out, int col, int 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      v[c][e] = pack2<T>(__uint_as_float(o[2 * e]) * scale, __uint_as_float(o[2 * e + 1]) * scale);
+    {
+      const float x = __uint_as_float(o[2 * e]) * scale, y = __uint_as_float(o[2 * e + 1]) * scale;
+      v[c][e] = LOW ? pack2<T>(lost<T>(x), lost<T>(y)) : pack2<T>(x, y);
+    }
   }
   if (wide == 0) {
     if (!live) return;

@@ -56,7 +56,7 @@ struct FwdArgs {
   const int32_t* seq_lens;
   int table_width, page, n_pages, box;  // box: keys per TMA box
   int expanded;  // page i of sequence b is page b * table_width + i (the table still says which are valid)
-  int wide_out;      // alignment of the output's rows, see store_rows
+  int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
 };
 
 template <int DP>
@@ -514,6 +514,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays
       tc::store_rows<T, DP / 2>(o_addr, out, half * (DP / 2), a.d, inv, live, f.wide_out, count > 0);
+      if (!PAGED && a.low != nullptr) {
+        T* low = static_cast<T*>(a.low) + ((x.t.batch * a.L + x.t.row0 + tok) * a.H + h) * a.d;
+        tc::store_rows<T, DP / 2, true>(o_addr, low, half * (DP / 2), a.d, inv, live, f.wide_low, count > 0);
+      }
       if (lse != nullptr) *lse = sum == 0.f ? neg_inf() : (m * c2 + log2f(sum)) * kLn2;
       tc::fence_before();  // O has been read before the next piece's first weights are announced
     }
@@ -558,6 +562,7 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
       !attn_map(&v, a.v, dtype, nb, a.L, a.Hk, a.d, a.vs, 1, kRows))
     return false;
   f.wide_out = row_alignment(a.o, a.os, nb, a.H);
+  f.wide_low = row_alignment(a.low, AttnStrides{a.L * a.H * a.d, static_cast<int64_t>(a.H) * a.d, a.d}, nb, a.H);
   int64_t tiles;
   const int rows = 2 * f.tile_tokens;
   if (a.cu != nullptr) {

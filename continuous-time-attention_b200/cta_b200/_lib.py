@@ -108,7 +108,7 @@ _SIGNATURES = {
 }
 
 # layouts of cta_attention_args, cta_kv_cache_args and cta_paged_attention_args
-ATTENTION_ARGS = struct.Struct("=12Q24q5q4i2f")
+ATTENTION_ARGS = struct.Struct("=13Q24q5q4i2f")
 KV_CACHE_ARGS = struct.Struct("=7Q10q5q2i")
 PAGED_ATTENTION_ARGS = struct.Struct("=9Q11q9q2i2f")
 

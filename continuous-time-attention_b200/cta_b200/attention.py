@@ -20,9 +20,12 @@ __all__ = ["prompt_attention"]
 class _PromptAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale):
+        low = None
+        if q.dtype != torch.float32:
+            low = torch.empty_like(q, memory_format=torch.contiguous_format)
         out, lse = ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=mask_words,
-                                         cu_seqlens=cu_seqlens)
-        ctx.save_for_backward(q, k, v, out, lse, mask_words, cu_seqlens)
+                                         cu_seqlens=cu_seqlens, out_low=low)
+        ctx.save_for_backward(q, k, v, out, low, lse, mask_words, cu_seqlens)
         ctx.causal = causal
         ctx.scale = scale
         return out
@@ -30,11 +33,11 @@ class _PromptAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, mask_words, cu_seqlens = ctx.saved_tensors
+        q, k, v, out, low, lse, mask_words, cu_seqlens = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq, dk, dv = ops.attention_backward(grad_out, q, k, v, out, lse, causal=ctx.causal, scale=ctx.scale,
                                             mask_words=mask_words, cu_seqlens=cu_seqlens, need_dq=need_q,
-                                            need_dkv=need_k or need_v)
+                                            need_dkv=need_k or need_v, out_low=low)
         return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 

@@ -649,6 +649,16 @@ def _strides3(t: Optional[torch.Tensor]):
 _NO_STRIDES = (0,) * 12
 
 
+def _low(low: Optional[torch.Tensor], q: torch.Tensor) -> int:
+    if low is None:
+        return 0
+    if (low.shape != q.shape or low.dtype != q.dtype or low.get_device() != q.get_device() or not low.is_contiguous()
+            or q.dtype == torch.float32):
+        raise ValueError(f"out_low must be contiguous, of a 16-bit type and like q: {tuple(q.shape)}, {q.dtype} on "
+                         f"{q.device}")
+    return low.data_ptr()
+
+
 def attention_forward(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -660,6 +670,7 @@ def attention_forward(
     cu_seqlens: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
     need_lse: bool = True,
+    out_low: Optional[torch.Tensor] = None,
 ):
     """Softmax attention of prompts, one launch: (out, lse).
 
@@ -670,7 +681,10 @@ def attention_forward(
     that see no key are zero.  Packed rows behind the last sequence keep what
     `out` holds; in an output allocated here they are zero.  `lse` (fp32,
     [B, heads, L] or [heads, T]; None without need_lse) is what
-    attention_backward takes."""
+    attention_backward takes.  `out_low`, for 16-bit types a contiguous tensor
+    like out, receives what rounding out lost (in float16 times 2048): given to
+    attention_backward too, it spares the gradients of rows with few keys the
+    error of that rounding."""
     q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
     o = _new(q) if out is None else _out(out, q.shape, q)
     lse = None
@@ -678,7 +692,7 @@ def attention_forward(
         n, length, heads = sizes[:3]
         lse = torch.empty((n, heads, length) if cu is None else (heads, length), dtype=torch.float32, device=q.device)
     args = _lib.ATTENTION_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _low(out_low, q), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
         0 if cu is None else cu.data_ptr(), 0 if mask_words is None else mask_words.data_ptr(), *_strides3(q),
         *_strides3(k), *_strides3(v), *_strides3(o), *_NO_STRIDES, *sizes, code, bool(causal), out is None, 0, scale, 0.0)
     _lib.enqueue(_lib.load().cta_attention_forward, q, args)
@@ -699,8 +713,10 @@ def attention_backward(
     cu_seqlens: Optional[torch.Tensor] = None,
     need_dq: bool = True,
     need_dkv: bool = True,
+    out_low: Optional[torch.Tensor] = None,
 ):
-    """(dq, dk, dv) of attention_forward from its out and lse; None for what is not wanted."""
+    """(dq, dk, dv) of attention_forward from its out, lse and, if it wrote one, out_low; None for what is not
+    wanted."""
     q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
     n, length, heads = sizes[:3]
     if grad_out.shape != q.shape or out.shape != q.shape:
@@ -719,7 +735,8 @@ def attention_backward(
     dv = _new(v) if need_dkv else None
     delta = torch.empty_like(lse)
     args = _lib.ATTENTION_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), g.data_ptr(), delta.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _low(out_low, q), lse.data_ptr(), g.data_ptr(),
+        delta.data_ptr(),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(cu), _lib.ptr(mask_words), *_strides3(q), *_strides3(k),
         *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), *sizes, code,
         bool(causal), 0, 0, scale, 0.0)

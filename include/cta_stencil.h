@@ -313,6 +313,9 @@ typedef struct cta_attention_args {
   const void* k;
   const void* v;
   void* out;                  /* forward: written.  backward: the forward's output */
+  void* out_low;              /* 16-bit types: what rounding out lost (fp16: times 2048), [B, L, heads, dim] or
+                               * [T, heads, dim] contiguous.  forward: written unless NULL.  backward: read unless
+                               * NULL; without it short rows' gradients lose up to a bit and a half */
   float* lse;                 /* forward: written unless NULL.  backward: read */
   const void* grad_out;       /* backward only, like the rest of the pointers */
   float* delta;               /* scratch, laid out as lse */

@@ -70,7 +70,7 @@ def test_attention_arguments_fail_before_launch():
 
     lib = _lib.load()
 
-    def call(fn="cta_attention_forward", pointers=(16,) * 4 + (0,) * 8, batch=1, length=8, heads=4, kv=2, dim=64,
+    def call(fn="cta_attention_forward", pointers=(16,) * 4 + (0,) * 9, batch=1, length=8, heads=4, kv=2, dim=64,
              dtype=1):
         args = _lib.ATTENTION_ARGS.pack(*pointers, *(64,) * 24, batch, length, heads, kv, dim, dtype, 0, 0, 0, 0.1, 0.0)
         return getattr(lib, fn)(args, None), lib.cta_last_error()
@@ -79,15 +79,15 @@ def test_attention_arguments_fail_before_launch():
         assert lib.__getattr__(fn)(None, None) == _lib.CTA_EINVAL
         for kw, word in ((dict(dtype=7), b"dtype"), (dict(heads=5), b"heads"), (dict(kv=0), b"heads"),
                          (dict(dim=0), b"head dim"), (dict(dim=257), b"head dim"), (dict(batch=-1), b"shape"),
-                         (dict(length=-1), b"shape"), (dict(pointers=(0,) * 12), b"null"),
-                         (dict(pointers=(16,) * 12), b"key mask")):
+                         (dict(length=-1), b"shape"), (dict(pointers=(0,) * 13), b"null"),
+                         (dict(pointers=(16,) * 13), b"key mask")):
             rc, msg = call(fn, **kw)
             assert rc == _lib.CTA_EINVAL and word in msg, (fn, kw, msg)
         assert call(fn, length=1 << 30)[0] == _lib.CTA_EUNSUPPORTED
         assert call(fn, batch=0)[0] == _lib.CTA_OK and call(fn, length=0)[0] == _lib.CTA_OK
     # the backward's own inputs; dk without dv
     assert call("cta_attention_backward")[0] == _lib.CTA_EINVAL
-    rc, msg = call("cta_attention_backward", pointers=(16,) * 9 + (0,) * 3)
+    rc, msg = call("cta_attention_backward", pointers=(16,) * 10 + (0,) * 3)
     assert rc == _lib.CTA_EINVAL and b"dk and dv" in msg
     assert lib.cta_attention_mask_words_per_row(1) == 8
     assert lib.cta_attention_mask_words_per_row(129) == 12

@@ -388,3 +388,47 @@ def test_longer(dim, dtype):
     for causal in (True, False):
         got = _run(q, k, v, g, causal=causal)
         _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _see(2100, causal), dim**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,dim", [(8, 64), (4, 128), (2, 200), (3, 20)])
+def test_output_that_rounds_far(heads, dim, dtype):
+    # Two keys of equal score with values a and a + step, a step of the type apart: the output a + step / 2 rounds
+    # by half a step, which is all of dP - delta.  dS = -+ step / 4 per unit of the gradient.
+    step = 2.0
+    a = 2.0 / torch.finfo(dtype).eps
+    q = torch.zeros(3, 2, heads, dim, dtype=dtype, device="cuda")
+    k = torch.randn(3, 2, heads, dim, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    v = torch.zeros_like(q)
+    v[:, 0, :, 0], v[:, 1, :, 0] = a, a + step
+    g = torch.zeros_like(q)
+    g[..., 0] = 1.0
+    dq = _run(q, k, v, g)[1].double()
+    want = dim**-0.5 * step / 4 * (k[:, 1:] - k[:, :1].double()).expand(-1, 2, -1, -1)
+    # Relative to |dS| = step / 4, as large as a * eps / 8: P and delta, both of a few fp32 roundings (lse, the
+    # exponential, the sum over dim: 2^-21 in all), err by 2^-21 a = 2^-18 / eps of it.  dS and dq are rounded
+    # once more (eps / 2 each).  The terms of the two keys add up.
+    eps = torch.finfo(dtype).eps
+    tol = dim**-0.5 * step / 4 * (2.0**-18 / eps + eps / 2) * (k.double().abs().sum(1, keepdim=True)) + eps / 2 * want.abs()
+    tol = tol + torch.finfo(dtype).smallest_normal * eps
+    _within(dq, want, tol.expand_as(want), "dq")
+
+
+def test_low_part_refusals():
+    from cta_b200 import ops
+
+    q, k, v, _ = (x.cuda() for x in _inputs((2, 5), 2, 2, 32, torch.bfloat16, seed=0))
+    for low in (q.float(), q[:, :4], torch.empty(2, 5, 2, 64, dtype=q.dtype, device="cuda")[..., :32], q.cpu()):
+        with pytest.raises(ValueError, match="out_low"):
+            ops.attention_forward(q, k, v, out_low=low)
+    with pytest.raises(ValueError, match="out_low"):
+        ops.attention_forward(q.float(), k.float(), v.float(), out_low=q.float())
+    low = torch.full_like(q, float("nan"))
+    out, lse = ops.attention_forward(q, k, v, out_low=low)
+    with pytest.raises(ValueError, match="out_low"):
+        ops.attention_backward(q, q, k, v, out, lse, out_low=low[:1])
+    # out + low is the output with 16 bits more or less: within the weights' error of the formula's, below one rounding
+    see = _see(5, False)
+    want, _ = A.attention(q[0], k[0], v[0], see, 32**-0.5)
+    tol = A.bounds(q[0], k[0], v[0], see, 32**-0.5, q.dtype) - 2.0**-9 * (1 - 2.0**-7) * want.abs()
+    _within(out[0].double() + low[0].double(), want, tol, "out + low")
