@@ -99,7 +99,10 @@ struct PagedArgs {
   int workers;
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
-  int expanded;    // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages
+  // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these the fractions of the
+  // scales [B, Hk, residue_row(table_width * page)]; else nullptr
+  const float* k_res;
+  const float* v_res;
 };
 
 // workers (warps) of the split kernel on the current device, and its launch
@@ -113,7 +116,10 @@ int attn_pack(int group);  // heads of a group that one row tile holds: its larg
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
 // e4m3 caches: the pages that the table names, as 16-bit rows in page order (page i of sequence b is page
 // b * table_width + i), for the tensor-core kernel
-cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, cudaStream_t st);
+cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
+                                cudaStream_t st);
+// fractions of a sequence's scales per head, in whole key tiles
+__host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots + 127) / 128 * 128; }
 
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);

@@ -237,7 +237,8 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
 // the other kernel over one wave of its CTAs 15 ns per key, i.e. as much as 137 such tiles.  One
 // sequence of 8192 keys: 64 rows 96 us split, 142 us on tensor cores; 128 rows 179 and 144 us.  8
 // sequences of 4096: 8 rows 65 and 69 us, 16 rows 112 and 70 us.  Over an e4m3 cache the pages have to
-// be expanded first: 32 sequences of 2048, 8 rows 121 and 139 us, 16 rows 225 and 140 us.
+// be expanded first: 32 sequences of 2048, 8 rows 119 and 198 us, 16 rows 225 and 199 us; one of
+// 8192 keys, 512 rows: 675 and 295 us.
 bool tensor_cores_pay(const PagedArgs& a) {
   const int64_t group = a.H / a.Hk, pack = attn_pack(static_cast<int>(group));
   if (a.cu == nullptr || a.max_rows * group <= 16 || !(a.scale > 0.f)) return false;
@@ -247,12 +248,13 @@ bool tensor_cores_pay(const PagedArgs& a) {
   return tiles > (a.k_scale != nullptr ? 256 : 128) * ((ctas + 147) / 148);
 }
 
-// 16-bit copy of the pages that the table can name, k then v; 0 where that is too much to ask for
+// 16-bit copy of the pages that the table can name, k then v, and the fractions of their scales; 0 where that is too
+// much to ask for
 constexpr int64_t kMostExpanded = 1LL << 31;
 int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64_t d) {
   const int64_t slots = b * width * page;
   if (slots >= (1LL << 24) || slots * hk >= (1LL << 26)) return 0;
-  const int64_t bytes = slots * hk * d * 4;
+  const int64_t bytes = slots * hk * d * 4 + b * residue_row(width * page) * hk * 8;
   return bytes <= kMostExpanded ? bytes : 0;
 }
 
@@ -355,12 +357,16 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
     if (bytes > 0) {
       PagedArgs x = a;
       char* k = static_cast<char*>(workspace);
-      char* v = k + bytes / 2;
-      e = launch_cache_expand(a, args->dtype, k, v, st);
+      const int64_t part = static_cast<int64_t>(a.B) * a.table_width * a.page * a.Hk * a.d * 2;
+      char* v = k + part;
+      float* k_res = reinterpret_cast<float*>(v + part);
+      float* v_res = k_res + a.B * residue_row(static_cast<int64_t>(a.table_width) * a.page) * a.Hk;
+      e = launch_cache_expand(a, args->dtype, k, v, k_res, v_res, st);
       if (e != cudaSuccess) return launched(e, "paged attention launch");
       x.k_cache = k;
       x.v_cache = v;
-      x.expanded = 1;
+      x.k_res = k_res;
+      x.v_res = v_res;
       if (launch_paged_tc(x, args->dtype, st, &e)) return launched(e, "paged attention launch");
       return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");
     }

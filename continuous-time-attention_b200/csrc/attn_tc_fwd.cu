@@ -1,8 +1,13 @@
 // Attention forward on the tensor cores: whole prompts, and chunks of rows over
 // a 16-bit paged cache.
 //
-// An e4m3 cache is first expanded to 16-bit pages (kv_cache.cu): one more rounding
-// of k and v, 2^-9 in bf16, like that of the weights.
+// An e4m3 cache is first expanded to 16-bit pages (kv_cache.cu) that hold codes
+// times the power of two below their scale, which 16 bits represent exactly.  The
+// rest of the scale, in [1, 2), multiplies the key's scores and, after the sum of
+// the weights, its weights.  That costs the softmax more than a 16-bit cache does
+// (512 rows over 8192 keys, 32/8 heads of 128: 295 and 142 us); with k and v times
+// their whole scale, rounded to 16 bits, the call took 157 us, but fp16 outputs
+// were twice as far off as one rounding of them, and are 1.4 times now.
 //
 // A CTA owns two 128-row tiles of one block of heads.  A row is a (token, head)
 // pair: where query heads share a key/value head, the largest power of two of
@@ -55,7 +60,10 @@ struct FwdArgs {
   int64_t table_sB;
   const int32_t* seq_lens;
   int table_width, page, n_pages, box;  // box: keys per TMA box
-  int expanded;  // page i of sequence b is page b * table_width + i (the table still says which are valid)
+  // SCALED: page i of sequence b is page b * table_width + i (the table still says which are valid), and these are
+  // the scales' fractions
+  const float* k_res;
+  const float* v_res;
   int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
 };
 
@@ -81,7 +89,7 @@ struct Item {
   bool last;   // there is no more work
 };
 
-template <typename T, int DP, bool PAGED>
+template <typename T, int DP, bool PAGED, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FwdArgs f) {
@@ -265,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (page < 0 || page >= f.n_pages) {
               atomicExch(&g_tc_fwd_error, kDevBadIndex);
               page = -1;
-            } else if (f.expanded) {
+            } else if (SCALED) {
               page = x.t.seq * f.table_width + key / f.page;
             }
           }
@@ -409,16 +417,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
       T* out = static_cast<T*>(a.o) + x.t.batch * a.os.b + (x.t.row0 + tok) * a.os.t + h * a.os.h;
       float* lse = live && half == 0 && a.lse != nullptr ? a.lse + lse_index(a, x.t, h, tok) : nullptr;
+      // the first fraction of this half's keys
+      int res = SCALED ? (x.t.seq * a.Hk + x.hk) * static_cast<int>(residue_row(f.table_width * f.page)) +
+                             j_lo * kRows + 64 * half
+                       : 0;
       float m = neg_inf(), sum = 0.f;
-      for (int j = 0; j < count; ++j, ++ns) {
+      for (int j = 0; j < count; ++j, ++ns, res += SCALED ? kRows : 0) {
+        if (SCALED && lane < 4)  // two lines each of the step's fractions
+          asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 2 ? f.k_res : f.v_res) + res + 32 * (lane & 1)));
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
         ok = ok && tc::wait(&bars.s_full[i], ns & 1);
         tc::fence_after();
         const int j0 = (j_lo + j) * kRows;
         uint32_t s[2][32];
-        tc::ld32(s_addr, s[0]);
-        tc::ld32(s_addr + 32, s[1]);
+        if (!SCALED) {
+          tc::ld32(s_addr, s[0]);
+          tc::ld32(s_addr + 32, s[1]);
+        }
         // warp-uniform: every row of the warp sees all keys of the tile
         bool whole = j0 + kRows <= n && (!a.causal || j0 + kRows - 1 <= limit_all);
         uint32_t w[4];
@@ -426,26 +442,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           key_words(n, mask, j0, kt + j, w);
           whole = whole && tc::all_set(w);
         }
-        tc::wait_ld(s[0], s[1]);
-        if (!whole) {
+        if (!SCALED) tc::wait_ld(s[0], s[1]);
+        // Fractions of the scales, 32 keys at a time: the scores are read from tensor memory once for the maximum and
+        // once for the weights, which leaves registers for eight loads.  Bound by those loads (128 bits to each of
+        // 32 lanes at 128 bytes a cycle); with one read of both they wait for one another instead, 205 and 199 us
+        // for 32 chunks of 16 rows over 2048 keys.
+        auto scale = [&](int c, uint32_t (&x)[32]) {
+          tc::ld32(s_addr + 32 * c, x);
+          float4 r[8];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int left = limit - j0 - 64 * half - 32 * c + 1;
-            const uint32_t see = (half == 0 ? w[c] : w[2 + c]) &
-                                 (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+          for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.k_res + res + 32 * c) + e);
+          tc::wait_ld(x);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((see >> e) & 1u)) s[c][e] = 0xff800000u;
+          for (int e = 0; e < 8; ++e) {
+            const float2 lo = mul2(make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])),
+                                   make_float2(r[e].x, r[e].y));
+            const float2 hi = mul2(make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])),
+                                   make_float2(r[e].z, r[e].w));
+            x[4 * e] = __float_as_uint(lo.x);
+            x[4 * e + 1] = __float_as_uint(lo.y);
+            x[4 * e + 2] = __float_as_uint(hi.x);
+            x[4 * e + 3] = __float_as_uint(hi.y);
           }
-        }
+        };
+        auto hide = [&](int c, uint32_t (&x)[32]) {
+          const int left = limit - j0 - 64 * half - 32 * c + 1;
+          const uint32_t see =
+              (half == 0 ? w[c] : w[2 + c]) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((see >> e) & 1u)) x[e] = 0xff800000u;
+        };
         float t[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          t[c] = __uint_as_float(s[c >> 1][16 * (c & 1)]);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t(&x)[32] = s[SCALED ? 0 : c];
+          if (SCALED) scale(c, x);
+          if (!whole) hide(c, x);
 #pragma unroll
-          for (int e = 1; e < 15; e += 2)
-            t[c] = tc::max3(t[c], __uint_as_float(s[c >> 1][16 * (c & 1) + e]), __uint_as_float(s[c >> 1][16 * (c & 1) + e + 1]));
-          t[c] = fmaxf(t[c], __uint_as_float(s[c >> 1][16 * (c & 1) + 15]));
+          for (int y = 0; y < 2; ++y) {
+            float& z = t[2 * c + y];
+            z = __uint_as_float(x[16 * y]);
+#pragma unroll
+            for (int e = 1; e < 15; e += 2)
+              z = tc::max3(z, __uint_as_float(x[16 * y + e]), __uint_as_float(x[16 * y + e + 1]));
+            z = fmaxf(z, __uint_as_float(x[16 * y + 15]));
+          }
         }
         float top = tc::max3(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]), m);
         // The reference of a row moves when one of its halves has grown by more than kLazy past it (or
@@ -479,13 +521,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t p[16];
+          uint32_t(&x)[32] = s[SCALED ? 0 : c];
+          float4 r[SCALED ? 8 : 1];
+          if constexpr (SCALED) {
+            scale(c, x);
+            if (!whole) hide(c, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float2 y = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), c2v, bv);
+            float2 y = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2v, bv);
             y.x = ex2(y.x);
             y.y = ex2(y.y);
             if (e & 1) part2 = add2(part2, y);
             else part = add2(part, y);
+            if constexpr (SCALED) {
+              const float4& z = r[e / 2];
+              y = mul2(y, (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y));
+            }
             p[e] = tc::pack2<T>(y.x, y.y);
           }
           // over this half's own scores: the other half may not have read its yet
@@ -529,20 +583,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kSoftmaxWarps) tc::dealloc(tmem, 512);
 }
 
-template <typename T, int DP, bool PAGED>
+template <typename T, int DP, bool PAGED, bool SCALED>
 cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int64_t ctas,
                    cudaStream_t st) {
-  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
+  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED, SCALED>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
 }
 
-template <bool PAGED>
+template <bool PAGED, bool SCALED>
 cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int dtype,
                      int64_t ctas, cudaStream_t st) {
   if (dtype == kBF16)
-    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED>(q, k, v, f, ctas, st)
-                       : launch<__nv_bfloat16, 128, PAGED>(q, k, v, f, ctas, st);
-  return f.a.d <= 64 ? launch<__half, 64, PAGED>(q, k, v, f, ctas, st)
-                     : launch<__half, 128, PAGED>(q, k, v, f, ctas, st);
+    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
+                       : launch<__nv_bfloat16, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
+  return f.a.d <= 64 ? launch<__half, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
+                     : launch<__half, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
 }
 
 }  // namespace
@@ -577,7 +631,7 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   // the keys' sake (24 such sequences, 32/8 heads, 3072 pieces: 281 and 266 us).
   const int64_t pieces = tiles * (a.H / f.pack);
   f.across = a.causal && pieces <= 12 * num_sms_here();
-  *e = dispatch<false>(q, k, v, f, dtype, pieces, st);
+  *e = dispatch<false, false>(q, k, v, f, dtype, pieces, st);
   return true;
 }
 
@@ -605,14 +659,15 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
   f.table_width = p.table_width;
   f.page = p.page;
   f.n_pages = p.n_pages;
-  f.expanded = p.expanded;
+  f.k_res = p.k_res;
+  f.v_res = p.v_res;
   f.box = std::min(p.page & -p.page, kRows);  // the largest power of two that divides a page
   f.wide_out = row_alignment(a.o, a.os, 1, a.H);
   // expanded pages are contiguous
-  const int64_t pages = p.expanded ? static_cast<int64_t>(p.B) * p.table_width : p.n_pages;
+  const int64_t pages = p.k_res != nullptr ? static_cast<int64_t>(p.B) * p.table_width : p.n_pages;
   const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
-  const AttnStrides ks = p.expanded ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
-  const AttnStrides vs = p.expanded ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
+  const AttnStrides ks = p.k_res != nullptr ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
+  const AttnStrides vs = p.k_res != nullptr ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
   CUtensorMap q, k, v;
   if (!attn_map(&q, p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) ||
       !attn_map(&k, p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) ||
@@ -620,7 +675,9 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
     return false;
   const int64_t tiles = packed_tiles(p.T, p.B, 2 * f.tile_tokens);
   a.tiles = static_cast<int>(tiles);
-  *e = dispatch<true>(q, k, v, f, dtype, tiles * (p.H / f.pack), st);
+  const int64_t pieces = tiles * (p.H / f.pack);
+  *e = p.k_res != nullptr ? dispatch<true, true>(q, k, v, f, dtype, pieces, st)
+                          : dispatch<true, false>(q, k, v, f, dtype, pieces, st);
   return true;
 }
 

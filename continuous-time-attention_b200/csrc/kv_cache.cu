@@ -189,21 +189,34 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   }
 }
 
-// code * scale of the pages of each sequence, in order, as 16-bit rows
+// codes of the pages of each sequence, in order, as 16-bit rows: each times the power of two below its scale, whose
+// fraction goes into k_res and v_res (attn_tc_fwd.cu says why)
 template <typename T>
-__global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out) {
+__global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out,
+                                                                float* k_res, float* v_res) {
   constexpr int GROUP = 16;
   const bool second = blockIdx.y != 0;
   const unsigned blocks = (a.Hk + kHeads - 1) / kHeads;
   const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
   const unsigned slots = static_cast<unsigned>(a.table_width) * a.page;  // per sequence
   const unsigned row = group / blocks, b = row / slots, j = row - b * slots;
-  const int h0 = static_cast<int>(group - row * blocks) * kHeads, c = threadIdx.x % GROUP * 8;
-  if (b >= static_cast<unsigned>(a.B) || c >= a.d) return;
+  const int h0 = static_cast<int>(group - row * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
+  if (b >= static_cast<unsigned>(a.B)) return;
+  // the scales' fractions of this key, and behind the last key up to the row's end
+  const int64_t res_row = residue_row(slots);
+  float* res = (second ? v_res : k_res) + (static_cast<int64_t>(b) * a.Hk + h0) * res_row;
+  if (j + 1 == slots)
+    for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i)
+      for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
+  if (c >= a.d) return;
   const int n = __ldg(a.seq_lens + b);
-  if (n < 0 || j >= static_cast<unsigned>(n)) return;
-  const int page = __ldg(a.table + b * a.table_sB + j / a.page);
-  if (page < 0 || page >= a.n_pages) return;  // reported by the kernel that reads them, which leaves them out
+  const int page = n < 0 || j >= static_cast<unsigned>(n) ? -1 : __ldg(a.table + b * a.table_sB + j / a.page);
+  if (page < 0 || page >= a.n_pages) {
+    // not there, or reported by the kernel that reads the pages, which leaves it out
+    if (lane == 0)
+      for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i) res[i * res_row + j] = 1.f;
+    return;
+  }
   const unsigned slot = j % a.page;
   const uint8_t* in = static_cast<const uint8_t*>(second ? a.v_cache : a.k_cache) + c +
                       page * (second ? a.vc_sP : a.kc_sP) + slot * (second ? a.vc_sS : a.kc_sS);
@@ -221,12 +234,16 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
 #pragma unroll
   for (int i = 0; i < kHeads; ++i)
     if (h0 + i < a.Hk) {
+      // sign and exponent of the scale go into the element, which stays exact, its fraction beside it
+      const uint32_t bits = __float_as_uint(mul[i]);
+      const float pow = __uint_as_float(bits & 0xff800000u);
+      if (lane == 0) res[i * res_row + j] = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
       float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 v = from_e4m3x2(static_cast<uint16_t>((e < 2 ? w[i].x : w[i].y) >> (16 * (e & 1))));
-        f[2 * e] = v.x * mul[i];
-        f[2 * e + 1] = v.y * mul[i];
+        f[2 * e] = v.x * pow;
+        f[2 * e + 1] = v.y * pow;
       }
       *reinterpret_cast<uint4*>(out + (h0 + i) * a.d) = pack8<T>(f);
     }
@@ -260,16 +277,19 @@ cudaError_t dispatch(const CacheArgs& a, int dtype, bool write, cudaStream_t st)
 cudaError_t launch_cache_write(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, true, st); }
 cudaError_t launch_cache_read(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, false, st); }
 
-cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, cudaStream_t st) {
+cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
+                                cudaStream_t st) {
   const int64_t groups = static_cast<int64_t>(p.B) * p.table_width * p.page * ((p.Hk + kHeads - 1) / kHeads);
   const int64_t ctas = (groups * 16 + kThreads - 1) / kThreads;
   if (groups >= (1LL << 28)) return cudaErrorInvalidConfiguration;  // the caller's limit keeps it below
   const dim3 grid(static_cast<unsigned>(ctas), 2u);
   if (ctas == 0) return cudaSuccess;
   if (dtype == kBF16)
-    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v),
+                                                   k_res, v_res);
   else
-    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__half*>(k), static_cast<__half*>(v));
+    cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__half*>(k), static_cast<__half*>(v), k_res,
+                                                   v_res);
   return cudaGetLastError();
 }
 

@@ -384,7 +384,7 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
  * data.  A page outside the cache or a length past the table counts as no keys
  * and is reported by cta_device_error() as 2.  page_size: a multiple of 16;
  * dim: a multiple of 16 up to 128; dtype: CTA_BF16, CTA_F16 (of q and out).
- * Chunks over an e4m3 cache may be computed from a 16-bit copy of k and v.
+ * Chunks over an e4m3 cache may be computed from a copy of the codes in 16 bits.
  * workspace: cta_paged_attention_workspace_bytes(args) bytes (sizes, types and
  * strides of args count, not its pointers; 0 = none) on 16, not shared by calls
  * that may overlap; it needs no clearing. */
