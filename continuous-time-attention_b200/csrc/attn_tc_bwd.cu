@@ -21,7 +21,10 @@
 // dO V^T while the next P is.
 //
 // Bound by the products at dim 128 (7 x 512 cycles per tile pair against 2 x
-// 1024 of exponentials), by the exponentials at dim 64.
+// 1024 of exponentials), by the exponentials at dim 64.  Measured, 8192 tokens, 16
+// heads, not causal: dim 128 dQ 640 us, dK and dV 960, 1230 TFLOP/s of the seven
+// products; dim 64 464 and 640, 870.  Both in one call take 1566 and 1099: dQ's CTAs
+// start while the last ones of dK and dV run.
 #include <algorithm>
 
 #include "attn_tc.cuh"

@@ -7,7 +7,9 @@
  *     x[i] <- x[i] + alpha * ((x[i+1] - 2 x[i]) + x[i-1])      (fp32 math)
  * applied `steps` times along the sequence axis with the copy boundary (first
  * and last row unchanged), its causal variant, attention-mask handling, packed
- * variable-length sequences, and the adjoint (backward) with d(alpha).
+ * variable-length sequences, and the adjoint (backward) with d(alpha).  Beside
+ * it stands softmax attention: prompts forward and backward, a paged key/value
+ * cache, and attention of new rows over that cache.
  *
  * Conventions
  *   - All tensors are device pointers owned by the caller; the library never
