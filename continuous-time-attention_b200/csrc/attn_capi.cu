@@ -82,7 +82,8 @@ int prompt_args(const cta_attention_args* p, AttnArgs& a) {
     return fail(CTA_EUNSUPPORTED, "batch, length and heads must be below 2^30, 2^30 and 2^20");
   if (p->cu_seqlens != nullptr && p->mask_words != nullptr)
     return fail(CTA_EINVAL, "a key mask takes padded sequences, not packed ones");
-  if (p->batch == 0 || p->length == 0) return kNothing;
+  // packed rows without sequences all lie behind the last one and may have to be cleared
+  if ((p->batch == 0 && p->cu_seqlens == nullptr) || p->length == 0) return kNothing;
   if (p->q == nullptr || p->k == nullptr || p->v == nullptr || p->out == nullptr)
     return fail(CTA_EINVAL, "null tensor pointer");
   std::memset(&a, 0, sizeof(a));

@@ -432,3 +432,15 @@ def test_low_part_refusals():
     want, _ = A.attention(q[0], k[0], v[0], see, 32**-0.5)
     tol = A.bounds(q[0], k[0], v[0], see, 32**-0.5, q.dtype) - 2.0**-9 * (1 - 2.0**-7) * want.abs()
     _within(out[0].double() + low[0].double(), want, tol, "out + low")
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 20)])
+def test_rows_without_sequences(dtype, dim):
+    """Packed rows of no sequence are zero and have no gradient, whatever the memory held before."""
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, k, v, g = (x.cuda() for x in _inputs((70,), 4, 2, dim, dtype))
+    for _ in range(3):
+        held = [torch.full_like(x, float("nan")) for x in (q, q, q, k, k, k)]
+        del held
+        for x in _run(q, k, v, g, cu_seqlens=cu):
+            assert (x == 0).all()
