@@ -129,8 +129,10 @@ int cache_args(const cta_kv_cache_args* p, bool write, CacheArgs& a) {
   if (p->dim < 16 || p->dim > kMaxHeadDim || p->dim % 16 != 0)
     return fail(CTA_EINVAL, "the cache's head dim must be a multiple of 16 in 16..%d, got %lld", kMaxHeadDim,
                 (long long)p->dim);
-  if (p->pages * p->page_size >= (1LL << 31) || p->tokens * p->kv_heads >= (1LL << 30))
-    return fail(CTA_EUNSUPPORTED, "slots must be below 2^31, tokens * heads below 2^30");
+  // the kernels number up to 32 lanes per token and four heads in 32 bits
+  if (p->pages >= (1LL << 31) || p->page_size >= (1LL << 31) || p->pages * p->page_size >= (1LL << 31) ||
+      p->tokens >= (1LL << 27) || p->kv_heads >= (1LL << 20) || p->tokens * ((p->kv_heads + 3) / 4) >= (1LL << 27))
+    return fail(CTA_EUNSUPPORTED, "slots must be below 2^31, tokens * ceil(heads / 4) below 2^27, heads below 2^20");
   if (p->quantized && (p->k_scale == nullptr || p->v_scale == nullptr))
     return fail(CTA_EINVAL, "an e4m3 cache needs its scales");
   if (p->tokens == 0) return kNothing;
@@ -188,10 +190,14 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
                 (long long)p->dim);
   if (p->page_size < 16 || p->page_size % 16 != 0)
     return fail(CTA_EINVAL, "the page size must be a multiple of 16, got %lld", (long long)p->page_size);
-  if (p->pages < 0 || p->pages * p->page_size >= (1LL << 31) || p->table_width < 0 ||
-      p->table_width * p->page_size >= (1LL << 31) - 64 || p->rows >= (1LL << 28) || p->batch >= (1LL << 28) ||
-      p->rows * p->heads >= (1LL << 31) - 1)
-    return fail(CTA_EUNSUPPORTED, "slots and table_width * page_size must be below 2^31, rows and batch below 2^28");
+  // key numbers, a tile past the last one included, and (row, head) pairs are 32-bit
+  constexpr int64_t most = (1LL << 31) - 256;
+  if (p->pages < 0 || p->pages >= most || p->page_size >= most || p->pages * p->page_size >= most ||
+      p->table_width < 0 || p->table_width >= most || p->table_width * p->page_size >= most || p->rows >= (1LL << 28) ||
+      p->batch >= (1LL << 28) || p->heads >= (1LL << 20) || p->rows * p->heads >= most)
+    return fail(CTA_EUNSUPPORTED,
+                "slots, table_width * page_size and rows * heads must be below 2^31 - 256, rows and batch below 2^28, "
+                "heads below 2^20");
   if (p->max_rows < 1) return fail(CTA_EINVAL, "max_rows must be at least 1");
   if (p->cu_seqlens == nullptr && p->rows != p->batch)
     return fail(CTA_EINVAL, "without offsets there is one row per sequence: %lld rows, %lld sequences",

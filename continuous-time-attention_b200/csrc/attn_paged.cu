@@ -655,15 +655,15 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
 template <typename T, bool FP8, int DP, int ROWS>
 struct Split {
   static int workers() {
-    static int per_sm = 0;  // the same on every device: a property of the code
-    if (per_sm == 0) {
-      int n = 0;
+    static std::atomic<int> per_sm{0};  // the same on every device: a property of the code
+    int n = per_sm.load(std::memory_order_relaxed);
+    if (n == 0) {
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_split_kernel<T, FP8, DP, ROWS>, kThreads, 0) !=
               cudaSuccess || n <= 0)
         n = 1;
-      per_sm = n;
+      per_sm.store(n, std::memory_order_relaxed);
     }
-    return per_sm * num_sms_here() * (kThreads / 32);  // what the GPU holds at a time
+    return n * num_sms_here() * (kThreads / 32);  // what the GPU holds at a time
   }
   static cudaError_t run(const PagedArgs& a, cudaStream_t st) {
     constexpr bool kHalf = FP8 || std::is_same<T, __half>::value;

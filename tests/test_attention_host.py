@@ -141,3 +141,29 @@ def test_paged_arguments_fail_before_launch():
         assert rc == _lib.CTA_EINVAL and word in msg, (kw, msg)
     assert call(width=1 << 28)[0] == _lib.CTA_EUNSUPPORTED
     assert call(rows=0)[0] == _lib.CTA_OK and call(batch=0)[0] == _lib.CTA_OK
+
+
+def test_sizes_past_the_kernels_numbers_are_refused():
+    """Index arithmetic of the kernels is 32-bit in places: sizes past it are refused before any launch."""
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def cache(tokens, heads, pages=4, page=16):
+        args = _lib.KV_CACHE_ARGS.pack(*(16,) * 7, *(64,) * 4, *(64,) * 6, tokens, heads, 64, pages, page, 1, 1)
+        return lib.cta_kv_cache_write(args, None)
+
+    def paged(width=4, page=16, pages=4, rows=2, heads=4):
+        args = _lib.PAGED_ATTENTION_ARGS.pack(*(16,) * 9, *(64,) * 4, *(64,) * 6, width, rows, rows, heads, 2, 64, pages,
+                                              page, width, 1, 1, 0, 0.1, 0.0)
+        return lib.cta_paged_attention(args, None, 0, None)
+
+    # 2^27 groups of up to 32 lanes are 2^32 threads
+    assert cache(1 << 27, 1) == _lib.CTA_EUNSUPPORTED
+    assert cache(1 << 25, 13) == _lib.CTA_EUNSUPPORTED
+    assert cache(2, 2, pages=1 << 40, page=1 << 40) == _lib.CTA_EUNSUPPORTED
+    # a tile of 128 keys past the last one still has a number
+    assert paged(width=(1 << 27) - 8) == _lib.CTA_EUNSUPPORTED
+    assert paged(width=1 << 40, page=1 << 40) == _lib.CTA_EUNSUPPORTED
+    assert paged(pages=1 << 40, page=1 << 40) == _lib.CTA_EUNSUPPORTED
+    assert paged(rows=1 << 27, heads=16) == _lib.CTA_EUNSUPPORTED
