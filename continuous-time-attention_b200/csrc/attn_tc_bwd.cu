@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
       // packed: rows of the next sequence in a tile that reaches past this one, in both tensors before
       // anything is made of either
-      const int rows = (t.n - first_of(s)) * f.pack;
+      const int rows = min(t.n - first_of(s), kRows) * f.pack;
       if (a.cu != nullptr && rows < kRows) {
         ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
         uint32_t w[4];
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::ld32(s_addr, p);
       // causal: the first row of this part that sees the key; 32 = none
       int from = 0;
-      if (a.causal) from = min(max((key - first_of(s)) * f.pack - part * 32, 0), 32);
+      if (a.causal) from = min(max(max(key - first_of(s), -1) * f.pack - part * 32, 0), 32);
       if (!valid) from = 32;
       const float4* nl = reinterpret_cast<const float4*>(&s_stat[stage][0][part * 32]);
       const float4* dl = reinterpret_cast<const float4*>(&s_stat[stage][1][part * 32]);
