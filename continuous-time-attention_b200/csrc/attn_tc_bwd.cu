@@ -23,7 +23,7 @@
 // Bound by the products at dim 128 (7 x 512 cycles per tile pair against 2 x
 // 1024 of exponentials), by the exponentials at dim 64.  Measured, 8192 tokens, 16
 // heads, not causal: dim 128 dQ 640 us, dK and dV 960, 1230 TFLOP/s of the seven
-// products; dim 64 464 and 640, 870.  Both in one call take 1566 and 1099: dQ's CTAs
+// products; dim 64 464 and 600, 900.  Both in one call take 1566 and 1090: dQ's CTAs
 // start while the last ones of dK and dV run.
 #include <algorithm>
 
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // dK, dV: the tiles are transposed, rows are keys and columns are query rows
 // ---------------------------------------------------------------------------
 struct DkvBars {
-  uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], s_free[2], p_full[2], dp_full, dp_free, ds_full, done;
+  uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], s_free[2], p_full[2], dp_full, dp_free, ds_full[2], done;
 };
 
 template <typename T, int DP>
@@ -318,6 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  // With two score buffers dS goes beside P, into the columns that P leaves of its scores', and the next dO V^T can
+  // start once this one has been read; with one it goes over dO V^T, so that the next scores wait for dV only.
+  constexpr bool kBeside = DP == 64;
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
   pdl_launch_dependents();  // dQ's CTAs may follow
 
@@ -340,11 +343,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.s_full[1], 1);
     mbar_init(&bars.s_free[0], 1);
     mbar_init(&bars.s_free[1], 1);
-    mbar_init(&bars.dp_free, 1);
+    mbar_init(&bars.dp_free, kBeside ? kWeightWarps : 1);
     mbar_init(&bars.p_full[0], kWeightWarps);
     mbar_init(&bars.p_full[1], kWeightWarps);
     mbar_init(&bars.dp_full, 1);
-    mbar_init(&bars.ds_full, kWeightWarps);
+    mbar_init(&bars.ds_full[0], kWeightWarps);
+    mbar_init(&bars.ds_full[1], kWeightWarps);
     mbar_init(&bars.done, 1);
     fence_mbar_init();
   }
@@ -470,14 +474,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after();
       if (ok && leader) {
         tc::product_tn<32>(t_dv, tmem + (s % NB) * 128, g, id_o, s > 0);
-        tc::commit(&bars.s_free[s % NB]);
+        if (!kBeside) tc::commit(&bars.s_free[s % NB]);
       }
       __syncwarp();
-      ok = ok && tc::wait(&bars.ds_full, s & 1);
+      ok = ok && tc::wait(&bars.ds_full[s & 1], (s >> 1) & 1);
       tc::fence_after();
       if (ok && leader) {
-        tc::product_tn<32>(t_dk, t_dp, q, id_o, s > 0);
-        tc::commit(&bars.dp_free);
+        tc::product_tn<32>(t_dk, kBeside ? tmem + (s % NB) * 128 + 16 : t_dp, q, id_o, s > 0);
+        tc::commit(kBeside ? &bars.s_free[s % NB] : &bars.dp_free);
         tc::commit(&bars.q_empty[s % NS]);
         tc::commit(&bars.g_empty[s % NS]);  // dO V^T was done before the score gradients
         if (s + 1 == steps) tc::commit(&bars.done);
@@ -537,6 +541,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t d[32];
       tc::ld32(d_addr, d);
       tc::wait_ld(d);
+      if (kBeside) {
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::arrive(&bars.dp_free);
+      }
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 b = dl[e / 4];
@@ -555,11 +564,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (2 * e + 1 < from) w[e] &= 0x0000ffffu;
         }
       }
-      tc::st16(d_addr, w);
+      tc::st16(kBeside ? s_addr + 16 : d_addr, w);
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
-      if (lane == 0) tc::arrive(&bars.ds_full);
+      if (lane == 0) tc::arrive(&bars.ds_full[s & 1]);
     }
     if (ok && steps > 0) ok = tc::wait(&bars.done, 0);
     tc::fence_after();
