@@ -47,11 +47,13 @@ __device__ __forceinline__ void clamp_range(const int32_t* cu, int i, int64_t to
 // the result.  Packed: the lanes walk the offsets 32 sequences at a time with a
 // prefix sum of the tile counts, so that the host never reads the offsets.
 // Tiles of a sequence are numbered from its end when `backwards` (the last
-// tiles of a causal sequence have the most keys and start first).  Not packed:
-// `across` takes the same tile of all sequences, then the next, and otherwise
-// one sequence follows the other.
+// tiles of a causal sequence have the most keys and start first).  Otherwise
+// one sequence follows the other, unless `across`: not packed, the same tile of all
+// sequences comes before the next; packed, up to 32 sequences come by descending
+// `weight` (their rows if that is null), so that the longest pieces of work do not
+// come last.
 __device__ __forceinline__ SeqTile find_tile(const int32_t* cu, int nseq, int64_t L, int tiles, int tile, int rows,
-                                             bool backwards, bool across) {
+                                             bool backwards, bool across, const int32_t* weight = nullptr) {
   SeqTile t;
   t.tail_index = t.tail_count = 0;
   if (cu == nullptr) {
@@ -66,20 +68,30 @@ __device__ __forceinline__ SeqTile find_tile(const int32_t* cu, int nseq, int64_
   t.batch = 0;
   int before = 0;
   int64_t end = 0;
+  const bool ranked = across && nseq > 1 && nseq <= 32;
   for (int s0 = 0; s0 < nseq; s0 += 32) {
     int64_t begin = 0;
     int n = 0;
     if (s0 + lane < nseq) clamp_range(cu, s0 + lane, L, begin, n);
     const int count = (n + rows - 1) / rows;
-    int upto = count;
+    int upto = count, total;
+    if (ranked) {
+      const int w = lane < nseq && weight != nullptr ? __ldg(weight + lane) : n;
+      total = __reduce_add_sync(0xffffffffu, count);
+      for (int i = 0; i < nseq; ++i) {
+        const int wi = __shfl_sync(0xffffffffu, w, i), ci = __shfl_sync(0xffffffffu, count, i);
+        if (wi > w || (wi == w && i < lane)) upto += ci;
+      }
+    } else {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      total = __shfl_sync(0xffffffffu, upto, 31);
     }
-    const int total = __shfl_sync(0xffffffffu, upto, 31);
     if (tile < before + total) {
-      const unsigned hit = __ballot_sync(0xffffffffu, tile < before + upto);
+      const unsigned hit = __ballot_sync(0xffffffffu, tile < before + upto && tile >= before + upto - count);
       const int src = __ffs(hit) - 1;
       t.seq = s0 + src;
       t.row0 = __shfl_sync(0xffffffffu, begin, src);

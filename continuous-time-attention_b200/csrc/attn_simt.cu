@@ -176,7 +176,8 @@ __device__ __forceinline__ float sum8(float x) {
 __device__ __forceinline__ SeqTile block_tile(const AttnArgs& a, int tile, int rows, bool backwards) {
   __shared__ SeqTile t;
   if (threadIdx.x < 32) {
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, tile, rows, backwards, a.causal);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, tile, rows, backwards,
+                                a.causal || a.cu != nullptr);
     if (threadIdx.x == 0) t = x;
   }
   __syncthreads();

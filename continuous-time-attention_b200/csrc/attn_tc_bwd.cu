@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h0 = static_cast<int>(blockIdx.x % blocks) * f.pack, hk = h0 / (a.H / a.Hk);
 
   if (warp == 0) {
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal, a.causal);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / blocks, f.tile_tokens, a.causal,
+                                a.causal || a.cu != nullptr);
     if (lane == 0) s_tile = x;
   } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
@@ -326,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // the first keys of a causal sequence meet the most rows: forwards is heaviest first
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false, a.causal);
+    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false,
+                                a.causal || a.cu != nullptr);
     if (lane == 0) s_tile = x;
   } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);

@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int hb = id % blocks;
         x.h0 = hb * f.pack;
         x.hk = x.h0 / (a.H / a.Hk);
-        x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across);
+        x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
+                        f.seq_lens);
         x.n = x.hi = x.t.n;
         if constexpr (PAGED) {
           if (x.t.first < x.t.n) {
@@ -632,7 +633,7 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   // 1024, 16/4 heads of 128, 1024 pieces: 106 and 112 us); with much of it a sequence's pieces stay together for
   // the keys' sake (24 such sequences, 32/8 heads, 3072 pieces: 281 and 266 us).
   const int64_t pieces = tiles * (a.H / f.pack);
-  f.across = a.causal && pieces <= 12 * num_sms_here();
+  f.across = a.cu != nullptr || (a.causal && pieces <= 12 * num_sms_here());
   *e = dispatch<false, false>(q, k, v, f, dtype, pieces, st);
   return true;
 }
@@ -658,6 +659,7 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
   f.table = p.table;
   f.table_sB = p.table_sB;
   f.seq_lens = p.seq_lens;
+  f.across = 1;
   f.table_width = p.table_width;
   f.page = p.page;
   f.n_pages = p.n_pages;
