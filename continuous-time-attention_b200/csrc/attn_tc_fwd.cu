@@ -447,9 +447,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!SCALED) tc::wait_ld(s[0], s[1]);
         // Fractions of the scales, 32 keys at a time: the scores are read from tensor memory once for the maximum and
-        // once for the weights, which leaves registers for eight loads.  Bound by those loads (128 bits to each of
-        // 32 lanes at 128 bytes a cycle); with one read of both they wait for one another instead, 205 and 199 us
-        // for 32 chunks of 16 rows over 2048 keys.
+        // once for the weights, which leaves registers for eight loads.  Bound by issue (77 % of the cycles of a busy
+        // SM); with one read of both the loads wait for one another instead, 205 and 199 us for 32 chunks of 16
+        // rows over 2048 keys.
         auto scale = [&](int c, uint32_t (&x)[32]) {
           tc::ld32(s_addr + 32 * c, x);
           float4 r[8];
