@@ -20,24 +20,24 @@ __all__ = ["prompt_attention"]
 class _PromptAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale):
-        low = None
-        if q.dtype != torch.float32:
-            low = torch.empty_like(q, memory_format=torch.contiguous_format)
-        out, lse = ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=mask_words,
-                                         cu_seqlens=cu_seqlens, out_low=low)
-        ctx.save_for_backward(q, k, v, out, low, lse, mask_words, cu_seqlens)
-        ctx.causal = causal
-        ctx.scale = scale
+        q, k, v, cu, sizes, code, scale = ops._attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
+        out = ops._new(q)
+        # what rounding the output loses: delta of rows with few keys needs it
+        low = torch.empty_like(out) if code != 0 else None
+        lse = ops._attention_forward(q, k, v, out, 0 if low is None else low.data_ptr(), cu, mask_words, causal, scale,
+                                     sizes, code, True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, mask_words, cu)
+        ctx.plan = (causal, scale, sizes, code)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, low, lse, mask_words, cu_seqlens = ctx.saved_tensors
+        # the forward has checked what was saved
+        q, k, v, out, low, lse, mask_words, cu = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = ops.attention_backward(grad_out, q, k, v, out, lse, causal=ctx.causal, scale=ctx.scale,
-                                            mask_words=mask_words, cu_seqlens=cu_seqlens, need_dq=need_q,
-                                            need_dkv=need_k or need_v, out_low=low)
+        dq, dk, dv = ops._attention_backward(grad_out, q, k, v, out, 0 if low is None else low.data_ptr(), lse, cu,
+                                             mask_words, *ctx.plan, need_q, need_k or need_v)
         return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 

@@ -687,16 +687,22 @@ def attention_forward(
     error of that rounding."""
     q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
     o = _new(q) if out is None else _out(out, q.shape, q)
+    return o, _attention_forward(q, k, v, o, _low(out_low, q), cu, mask_words, causal, scale, sizes, code, need_lse,
+                                 out is None)
+
+
+def _attention_forward(q, k, v, o, low, cu, mask_words, causal, scale, sizes, code, need_lse, zero_tail):
+    """attention_forward of inputs that have been checked into o; `low` is an address or 0.  Returns lse."""
     lse = None
     if need_lse:
         n, length, heads = sizes[:3]
         lse = torch.empty((n, heads, length) if cu is None else (heads, length), dtype=torch.float32, device=q.device)
     args = _lib.ATTENTION_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _low(out_low, q), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low, 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
         0 if cu is None else cu.data_ptr(), 0 if mask_words is None else mask_words.data_ptr(), *_strides3(q),
-        *_strides3(k), *_strides3(v), *_strides3(o), *_NO_STRIDES, *sizes, code, bool(causal), out is None, 0, scale, 0.0)
+        *_strides3(k), *_strides3(v), *_strides3(o), *_NO_STRIDES, *sizes, code, bool(causal), zero_tail, 0, scale, 0.0)
     _lib.enqueue(_lib.load().cta_attention_forward, q, args)
-    return o, lse
+    return lse
 
 
 def attention_backward(
@@ -729,14 +735,22 @@ def attention_backward(
     shape = (n, heads, length) if cu is None else (heads, length)
     if lse.shape != shape or lse.dtype != torch.float32 or lse.get_device() != device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 {shape} on {q.device}")
+    return _attention_backward(grad_out, q, k, v, out, _low(out_low, q), lse, cu, mask_words, causal, scale, sizes, code,
+                               need_dq, need_dkv)
+
+
+def _attention_backward(grad_out, q, k, v, out, low, lse, cu, mask_words, causal, scale, sizes, code, need_dq, need_dkv):
+    """attention_backward of inputs that have been checked; `low` is an address or 0."""
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()
+            and (code == 0 or sizes[4] & 7 or not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15)):
+        q, k, v = _attention_rows(q, code), _attention_rows(k, code), _attention_rows(v, code)
     g, o = _attention_rows(grad_out, code), _attention_rows(out, code)
     dq = _new(q) if need_dq else None
     dk = _new(k) if need_dkv else None
     dv = _new(v) if need_dkv else None
     delta = torch.empty_like(lse)
     args = _lib.ATTENTION_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _low(out_low, q), lse.data_ptr(), g.data_ptr(),
-        delta.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low, lse.data_ptr(), g.data_ptr(), delta.data_ptr(),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(cu), _lib.ptr(mask_words), *_strides3(q), *_strides3(k),
         *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), *sizes, code,
         bool(causal), 0, 0, scale, 0.0)
