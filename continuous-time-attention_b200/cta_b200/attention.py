@@ -70,7 +70,7 @@ def prompt_attention(
             raise ValueError("give key_mask or mask_words, not both")
         if q.dim() != 4 or cu_seqlens is not None or key_mask.shape != q.shape[:2]:
             raise ValueError("key_mask must be (B, L) for padded q, k, v")
-        if key_mask.device != q.device:
+        if key_mask.get_device() != q.get_device():
             raise ValueError(f"key_mask on {key_mask.device}, expected {q.device}")
         words = ops.attention_mask(key_mask)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

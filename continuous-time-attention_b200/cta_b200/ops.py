@@ -567,13 +567,16 @@ def _on16(t: torch.Tensor) -> bool:
 def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
     """A key mask [B, L] (any mask dtype, non-zero = valid) as the words that
     attention_forward and attention_backward take; one launch."""
-    _require_cuda(key_mask, "key_mask")
+    if key_mask.get_device() < 0:
+        _require_cuda(key_mask, "key_mask")
     if key_mask.dim() != 2:
         raise ValueError("key_mask must have shape (B, L)")
     B, L = key_mask.shape
-    m, code, sB, sL = _mask_args(key_mask, B, L, key_mask.device)
+    dtype = key_mask.dtype
+    code = _lib.mask_code(torch.uint8 if dtype == torch.bool else dtype)  # a bool is a byte
     words = torch.empty((B, _mask_row_words(L)), dtype=torch.int32, device=key_mask.device)
-    _lib.enqueue(_lib.load().cta_attention_mask_words, key_mask, m.data_ptr(), code, sB, sL, B, L, words.data_ptr())
+    _lib.enqueue(_lib.load().cta_attention_mask_words, key_mask, key_mask.data_ptr(), code, *key_mask.stride(), B, L,
+                 words.data_ptr())
     return words
 
 
