@@ -444,3 +444,31 @@ def test_rows_without_sequences(dtype, dim):
         del held
         for x in _run(q, k, v, g, cu_seqlens=cu):
             assert (x == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_streams_at_once(dtype):
+    """Calls that run side by side give what they give alone, bit for bit: the gradients' kernels of one call also run
+    beside each other, and those of the next call of a stream start only when both are done."""
+    from cta_b200 import ops
+
+    sets = [[x.cuda() for x in _inputs((2, n), 8, 2, 64, dtype, seed=n)] for n in (700, 333)]
+
+    def call(q, k, v, g):
+        o, lse = ops.attention_forward(q, k, v, causal=True)
+        return (o, lse, *ops.attention_backward(g, q, k, v, o, lse, causal=True))
+
+    alone = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(6):
+        for i, (s, stream) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(stream):
+                x = call(*s)
+                got[i].append(tuple(y.clone() for y in x))  # reads the gradients right behind their kernels
+    torch.cuda.synchronize()
+    for want, all_of in zip(alone, got):
+        for x in all_of:
+            for a, b in zip(want, x):
+                assert torch.equal(a, b)

@@ -460,3 +460,24 @@ def test_no_rows_or_sequences():
     out = torch.full_like(s.q, 3.0)
     ops.paged_attention(s.q, s.kc, s.vc, s.table, s.seq_lens, cu_seqlens=cu, out=out)
     assert (out == 3).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_two_streams_at_once(quantized):
+    """Decode and a chunk side by side give what they give alone, bit for bit."""
+    from cta_b200 import ops
+
+    sets = [Setup([900, 33, 2100], [1, 1, 1], 8, 2, 128, 16, torch.bfloat16, quantized),
+            Setup([1500, 700], [300, 260], 8, 2, 128, 32, torch.bfloat16, quantized)]
+    alone = [s.run() for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(6):
+        for i, (s, stream) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(s.run().clone())
+    torch.cuda.synchronize()
+    for want, all_of in zip(alone, got):
+        for x in all_of:
+            assert torch.equal(want, x)
