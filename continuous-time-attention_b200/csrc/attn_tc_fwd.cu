@@ -631,7 +631,7 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   }
   // Causal: with little work the long pieces of all sequences go first, else the ends are uneven (16 sequences of
   // 1024, 16/4 heads of 128, 1024 pieces: 106 and 112 us); with much of it a sequence's pieces stay together for
-  // the keys' sake (24 such sequences, 32/8 heads, 3072 pieces: 281 and 266 us).
+  // the keys' sake (24 such sequences, 32/8 heads, three times the pieces: 281 and 266 us).
   const int64_t pieces = tiles * (a.H / f.pack);
   f.across = a.cu != nullptr || (a.causal && pieces <= 12 * num_sms_here());
   *e = dispatch<false, false>(q, k, v, f, dtype, pieces, st);
