@@ -260,13 +260,16 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       }
     }
 
-    // Last key that every row of the tile sees.  Rows behind the sequence's last count as seeing all: theirs are
-    // not written.  (So do rows that see nothing; then no other row of the tile sees 16 keys.)
+    // Last key that every row of the tile sees, -1 if one of them sees none.  Rows behind the sequence's last do not
+    // count: theirs are not written.
     int least = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) least = min(least, last[r][e] < 0 ? 0x7fffffff : last[r][e]);
+      for (int e = 0; e < 2; ++e) {
+        const bool counts = (g.tile * ROWS + 2 * quad + e + 8 * r) / group < g.rows;
+        if (counts) least = min(least, max(last[r][e], -1));
+      }
     least = __reduce_min_sync(0xffffffffu, least);
     float o[MT][NR][4];
     float m[NR][2], l[NR][2], mv[NR][2];  // reference of the weights, their sum, reference of the weighted values
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
       }
       if (it + 1 < count) load_keys(grp + 1, page_next, slot_next);
 
-      const bool all_see = here && (grp + 1) * kGroup <= least + 1;
+      const bool all_see = here && grp * kGroup + kGroup - 1 <= least;
       // weights of keys oct, oct + 8 in rows 2 quad, 2 quad + 1
       uint32_t pf[NR][2];
 #pragma unroll

@@ -481,3 +481,16 @@ def test_two_streams_at_once(quantized):
     for want, all_of in zip(alone, got):
         for x in all_of:
             assert torch.equal(want, x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,rows,hint", [(32, 8, 8, 8), (8, 8, 24, 1), (16, 2, 40, 1), (4, 4, 40, 40)])
+@pytest.mark.parametrize("keys", [1, 3, 4, 7, 17])
+def test_tiles_whose_rows_all_see_nothing(keys, heads, kv_heads, rows, hint, quantized, dtype):
+    """So many more rows than keys that whole tiles of 8 or 16 (row, head) pairs see none of the keys there are."""
+    s = Setup([keys, 200], [rows, 1], heads, kv_heads, 64, 16, dtype, quantized, seed=keys)
+    out = s.run(max_rows=hint)
+    blind = max(0, rows - keys)
+    assert (out[:blind] == 0).all()
+    s.check(out)
