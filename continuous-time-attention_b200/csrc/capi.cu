@@ -602,7 +602,8 @@ int cta_diffusion_fwd_bld_residual(const void* x, const void* residual, void* y,
                                    int64_t x_sB, int64_t x_sL, int64_t r_sB, int64_t r_sL, int64_t y_sB,
                                    int64_t y_sL, int dtype, int steps, const float* alpha, const void* mask,
                                    int mask_dtype, int64_t mask_sB, int64_t mask_sL, void* stream) {
-  if (residual == nullptr) return fail(CTA_EINVAL, "null residual pointer");
+  // an empty tensor has no address
+  if (residual == nullptr && B != 0 && L != 0 && D != 0) return fail(CTA_EINVAL, "null residual pointer");
   return fwd_bld_impl(x, residual, y, B, L, D, x_sB, x_sL, r_sB, r_sL, y_sB, y_sL, dtype, steps, 0, alpha, nullptr,
                       0, mask, mask_dtype, mask_sB, mask_sL, stream);
 }
@@ -774,7 +775,7 @@ int cta_diffusion_fwd_varlen_residual(const void* x, const void* residual, void*
                                       int64_t x_sL, int64_t r_sL, int64_t y_sL, const int32_t* cu_seqlens,
                                       int64_t nseq, int64_t max_len, int pad_to_max, int dtype, int steps,
                                       float alpha, void* stream) {
-  if (residual == nullptr) return fail(CTA_EINVAL, "null residual pointer");
+  if (residual == nullptr && total_rows != 0 && D != 0) return fail(CTA_EINVAL, "null residual pointer");
   return fwd_varlen_impl(x, residual, y, total_rows, D, x_sL, r_sL, y_sL, cu_seqlens, nseq, max_len, pad_to_max,
                          dtype, steps, alpha, stream);
 }

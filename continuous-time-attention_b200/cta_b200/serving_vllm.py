@@ -216,7 +216,7 @@ class CtaPostAttnMixer(nn.Module):
         out = ops.paged_attention(q, k_cache, v_cache, attn_metadata.block_table, attn_metadata.seq_lens,
                                   cu_seqlens=self._device_qsl(attn_metadata.query_start_loc, q.device),
                                   max_rows=max(1, max_rows), scale=scale, k_scale=k_scale, v_scale=v_scale)
-        return self.forward(out.view(q.shape[0], -1), attn_metadata=attn_metadata, is_prefill=is_prefill,
+        return self.forward(out.flatten(1), attn_metadata=attn_metadata, is_prefill=is_prefill,
                             residual=residual)
 
     def _mix(self, x, *, attn_metadata, is_prefill, residual):

@@ -219,3 +219,26 @@ def test_decode_step_captured():
             md.block_table[:, : nmd.block_table.shape[1]].copy_(nmd.block_table)
         graph.replay()
         server.check(out.view(-1, 8, 64), q, new)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_attend_without_rows(quantized):
+    """A step without tokens (an idle rank): no row out, nothing written."""
+    from cta_b200.serving_vllm import CtaConfig, CtaPostAttnMixer
+
+    for enabled in (False, True):
+        mixer = CtaPostAttnMixer(CtaConfig(enabled=enabled))
+        server = Server(8, 2, 64, 16, 20, torch.bfloat16, quantized)
+        md, q, k, v = server.batch({0: 40}, 0)
+        before = server.kc.clone().view(torch.uint8)
+        for starts, lens, longest in (([0], 0, 0), ([0, 0], 1, 0), ([0, 0], 1, 5)):
+            md.query_start_loc = torch.tensor(starts, dtype=torch.int32, device="cuda")
+            md.block_table, md.seq_lens = md.block_table[:lens], torch.full((lens,), 7, dtype=torch.int32, device="cuda")
+            if lens == 1:
+                md.block_table = torch.zeros(1, 3, dtype=torch.int32, device="cuda")
+            md.max_query_len, md.slot_mapping = longest, torch.zeros(0, dtype=torch.int64, device="cuda")
+            for residual in (None, torch.zeros(0, 512, dtype=torch.bfloat16, device="cuda")):
+                out = mixer.attend(q[:0], k[:0], v[:0], server.kc, server.vc, attn_metadata=md, k_scale=server.ks,
+                                   v_scale=server.vs, residual=residual)
+                assert out.shape == (0, 512)
+        assert torch.equal(before, server.kc.view(torch.uint8))
