@@ -325,7 +325,9 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream) {
 
 int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args) {
   PagedArgs a;
-  if (paged_args(args, a) != CTA_OK || a.T == 0 || a.B == 0) return 0;
+  const int rc = paged_args(args, a);
+  if (rc != CTA_OK) return -rc;
+  if (a.T == 0 || a.B == 0) return 0;
   if (tensor_cores_pay(a)) {
     if (!args->quantized) return 0;
     const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);

@@ -904,6 +904,13 @@ def paged_attention(
     Rows that see no key are zero; rows behind the last sequence are not
     written.  A page outside the cache or a length past the table counts as no
     keys and is reported by ``_lib.device_error()``."""
+    return _paged_launch(*_paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale,
+                                      v_scale, out))
+
+
+def _paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale, v_scale, out):
+    """All checks of paged_attention, and what its launch takes: (q, out, arguments, bytes of workspace, the tensors
+    that the arguments point to)."""
     device = q.get_device()
     if device < 0:
         _require_cuda(q, "q")
@@ -952,7 +959,13 @@ def paged_attention(
     else:
         with _lib.on_device(q):
             nbytes = lib.cta_paged_attention_workspace_bytes(args)
+    if nbytes < 0:
+        _lib.check(-nbytes)
+    return q, o, args, nbytes, (k_cache, v_cache, k_scale, v_scale, table, lens, cu)
+
+
+def _paged_launch(q, o, args, nbytes, _held):
     # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.enqueue(lib.cta_paged_attention, q, args, _lib.ptr(ws), nbytes)
+    _lib.enqueue(_lib.load().cta_paged_attention, q, args, _lib.ptr(ws), nbytes)
     return o

@@ -212,10 +212,12 @@ class CtaPostAttnMixer(nn.Module):
         slots = attn_metadata.slot_mapping
         if slots.dim() != 1 or slots.shape[0] < k.shape[0]:
             raise ValueError("slot_mapping must have an entry for every row of k")
+        # refused, if at all, before the cache is touched
+        plan = ops._paged_plan(q, k_cache, v_cache, attn_metadata.block_table, attn_metadata.seq_lens,
+                               self._device_qsl(attn_metadata.query_start_loc, q.device), max(1, max_rows), scale, k_scale,
+                               v_scale, None)
         ops.kv_cache_write(k, v, k_cache, v_cache, slots[: k.shape[0]], k_scale=k_scale, v_scale=v_scale)
-        out = ops.paged_attention(q, k_cache, v_cache, attn_metadata.block_table, attn_metadata.seq_lens,
-                                  cu_seqlens=self._device_qsl(attn_metadata.query_start_loc, q.device),
-                                  max_rows=max(1, max_rows), scale=scale, k_scale=k_scale, v_scale=v_scale)
+        out = ops._paged_launch(*plan)
         return self.forward(out.flatten(1), attn_metadata=attn_metadata, is_prefill=is_prefill,
                             residual=residual)
 

@@ -388,8 +388,9 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
  * dim: a multiple of 16 up to 128; dtype: CTA_BF16, CTA_F16 (of q and out).
  * Chunks over an e4m3 cache may be computed from a copy of the codes in 16 bits.
  * workspace: cta_paged_attention_workspace_bytes(args) bytes (sizes, types and
- * strides of args count, not its pointers; 0 = none) on 16, not shared by calls
- * that may overlap; it needs no clearing. */
+ * strides of args count, of its pointers only which are NULL; 0 = none; negative:
+ * minus the status with which the call would refuse the arguments) on 16, not
+ * shared by calls that may overlap; it needs no clearing. */
 typedef struct cta_paged_attention_args {
   const void* q;
   void* out;

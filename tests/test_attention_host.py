@@ -167,3 +167,21 @@ def test_sizes_past_the_kernels_numbers_are_refused():
     assert paged(width=1 << 40, page=1 << 40) == _lib.CTA_EUNSUPPORTED
     assert paged(pages=1 << 40, page=1 << 40) == _lib.CTA_EUNSUPPORTED
     assert paged(rows=1 << 27, heads=16) == _lib.CTA_EUNSUPPORTED
+
+
+def test_paged_workspace_size_of_refused_arguments():
+    """Minus the status that the call itself returns, with its message."""
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def size(dim=64, page=16, width=3):
+        args = _lib.PAGED_ATTENTION_ARGS.pack(*(16,) * 9, 256, 64, 256, 64, *(1024, 64, 64) * 2, width, 2, 2, 4, 2, dim, 4,
+                                              page, width, 1, 1, 0, 0.1, 0.0)
+        return lib.cta_paged_attention_workspace_bytes(args), lib.cta_last_error()
+
+    assert size()[0] > 0
+    for kw, status, word in ((dict(dim=144), _lib.CTA_EINVAL, b"head dim"), (dict(page=24), _lib.CTA_EINVAL, b"page size"),
+                             (dict(width=1 << 28), _lib.CTA_EUNSUPPORTED, b"2^31")):
+        rc, msg = size(**kw)
+        assert rc == -status and word in msg, (kw, rc, msg)

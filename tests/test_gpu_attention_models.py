@@ -242,3 +242,34 @@ def test_attend_without_rows(quantized):
                                    v_scale=server.vs, residual=residual)
                 assert out.shape == (0, 512)
         assert torch.equal(before, server.kc.view(torch.uint8))
+
+
+def test_attend_refuses_before_it_writes():
+    """Whatever the attention refuses is refused before the cache is touched."""
+    from cta_b200.serving_vllm import CtaConfig, CtaPostAttnMixer
+
+    mixer = CtaPostAttnMixer(CtaConfig(enabled=False))
+
+    def refused(server, md, q, k, v, match, **kw):
+        before = [c.clone().view(torch.uint8) for c in (server.kc, server.vc)]
+        with pytest.raises(ValueError, match=match):
+            mixer.attend(q, k, v, server.kc, server.vc, attn_metadata=md, k_scale=server.ks, v_scale=server.vs, **kw)
+        assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (server.kc, server.vc)))
+
+    for quantized in (False, True):
+        for dim in (144, 256):  # the cache takes them, the attention does not
+            server = Server(4, 2, dim, 16, 20, torch.bfloat16, quantized)
+            refused(server, *server.batch({0: 40}, 0), "head dim")
+        server = Server(4, 2, 64, 8, 20, torch.bfloat16, quantized)
+        refused(server, *server.batch({0: 40}, 0), "page size")
+        server = Server(4, 2, 64, 16, 20, torch.bfloat16, quantized)
+        md, q, k, v = server.batch({0: 40, 1: 3}, 0)
+        refused(server, md, q[:, :3], k, v, "does not go with")
+        refused(server, md, torch.cat([q, q], -1), k, v, "does not go with")
+        refused(server, md, q.float(), k, v, "must be|bf16 or fp16")
+        for name, value, match in (("block_table", md.block_table[:1], "block_table"),
+                                   ("seq_lens", md.seq_lens.float(), "seq_lens"),
+                                   ("query_start_loc", md.query_start_loc[:2], "cu_seqlens")):
+            bad = SimpleNamespace(**vars(md))
+            setattr(bad, name, value)
+            refused(server, bad, q, k, v, match)
