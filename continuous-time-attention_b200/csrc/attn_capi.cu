@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "attn_tc.cuh"
@@ -133,10 +134,12 @@ int cache_args(const cta_kv_cache_args* p, bool write, CacheArgs& a) {
   if (p->pages >= (1LL << 31) || p->page_size >= (1LL << 31) || p->pages * p->page_size >= (1LL << 31) ||
       p->tokens >= (1LL << 27) || p->kv_heads >= (1LL << 20) || p->tokens * ((p->kv_heads + 3) / 4) >= (1LL << 27))
     return fail(CTA_EUNSUPPORTED, "slots must be below 2^31, tokens * ceil(heads / 4) below 2^27, heads below 2^20");
-  if (p->quantized && (p->k_scale == nullptr || p->v_scale == nullptr))
+  if (p->quantized && p->pages > 0 && (p->k_scale == nullptr || p->v_scale == nullptr))
     return fail(CTA_EINVAL, "an e4m3 cache needs its scales");
   if (p->tokens == 0) return kNothing;
-  if (p->k == nullptr || p->v == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->slots == nullptr)
+  // a pool without pages has no address
+  if (p->k == nullptr || p->v == nullptr || p->slots == nullptr ||
+      (p->pages > 0 && (p->k_cache == nullptr || p->v_cache == nullptr)))
     return fail(CTA_EINVAL, "null tensor pointer");
   const int64_t rows = 8, cells = p->quantized ? 16 : 8;  // elements in 16 bytes
   for (int64_t s : {p->k_stride[0], p->k_stride[1], p->v_stride[0], p->v_stride[1]})
@@ -202,7 +205,7 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
   if (p->cu_seqlens == nullptr && p->rows != p->batch)
     return fail(CTA_EINVAL, "without offsets there is one row per sequence: %lld rows, %lld sequences",
                 (long long)p->rows, (long long)p->batch);
-  if (p->quantized && (p->k_scale == nullptr || p->v_scale == nullptr))
+  if (p->quantized && p->pages > 0 && (p->k_scale == nullptr || p->v_scale == nullptr))
     return fail(CTA_EINVAL, "an e4m3 cache needs its scales");
   std::memset(&a, 0, sizeof(a));
   a.q = p->q;
@@ -219,8 +222,8 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
   a.vc_sP = p->v_cache_stride[0];
   a.vc_sS = p->v_cache_stride[1];
   a.vc_sH = p->v_cache_stride[2];
-  a.k_scale = p->k_scale;
-  a.v_scale = p->v_scale;
+  a.k_scale = p->quantized ? p->k_scale : nullptr;
+  a.v_scale = p->quantized ? p->v_scale : nullptr;
   a.table = p->block_table;
   a.table_sB = p->table_stride;
   a.seq_lens = p->seq_lens;
@@ -246,7 +249,23 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
 // sequences of 4096: 8 rows 65 and 69 us, 16 rows 112 and 70 us.  Over an e4m3 cache the pages have to
 // be expanded first: 32 sequences of 2048, 8 rows 119 and 198 us, 16 rows 225 and 199 us; one of
 // 8192 keys, 512 rows: 675 and 295 us.
+//
+// What TMA cannot address, a pool without pages among it, is for the split kernel.
+bool tma_strides(std::initializer_list<int64_t> elements) {
+  for (int64_t s : elements)
+    if (s <= 0 || s >= (1LL << 39)) return false;
+  return true;
+}
+bool tma_can_address(const PagedArgs& a) {
+  // an axis of one entry has no stride
+  const auto axis = [](int64_t entries, int64_t stride) { return entries == 1 ? int64_t{8} : stride; };
+  if (!tma_strides({axis(a.T, a.q_sT), axis(a.H, a.q_sH)})) return false;
+  if (a.k_scale != nullptr) return true;  // the expanded copy is what TMA reads
+  return a.n_pages > 0 && tma_strides({axis(a.n_pages, a.kc_sP), axis(a.page, a.kc_sS), axis(a.Hk, a.kc_sH),
+                                       axis(a.n_pages, a.vc_sP), axis(a.page, a.vc_sS), axis(a.Hk, a.vc_sH)});
+}
 bool tensor_cores_pay(const PagedArgs& a) {
+  if (!tma_can_address(a)) return false;
   const int64_t group = a.H / a.Hk, pack = attn_pack(static_cast<int>(group));
   if (a.cu == nullptr || a.max_rows * group <= 16 || !(a.scale > 0.f)) return false;
   const int64_t b = a.B;
@@ -342,8 +361,9 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
   const int rc = paged_args(args, a);
   if (rc != CTA_OK) return rc;
   if (a.T == 0 || a.B == 0) return CTA_OK;
-  if (a.q == nullptr || a.o == nullptr || a.k_cache == nullptr || a.v_cache == nullptr || a.table == nullptr ||
-      a.seq_lens == nullptr)
+  // a pool without pages and a table without entries have no address
+  if (a.q == nullptr || a.o == nullptr || (a.n_pages > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
+      (a.table == nullptr && a.table_width > 0) || a.seq_lens == nullptr)
     return fail(CTA_EINVAL, "null tensor pointer");
   const int64_t cells = args->quantized ? 16 : 8;
   for (int64_t s : {a.q_sT, a.q_sH, a.o_sT, a.o_sH})

@@ -185,3 +185,22 @@ def test_paged_workspace_size_of_refused_arguments():
                              (dict(width=1 << 28), _lib.CTA_EUNSUPPORTED, b"2^31")):
         rc, msg = size(**kw)
         assert rc == -status and word in msg, (kw, rc, msg)
+
+
+def test_paged_kernel_goes_by_what_tma_addresses():
+    """Chunks take the tensor-core kernel, which needs no workspace over a 16-bit cache; with strides that a tensor map
+    cannot hold, or no pages, the split kernel, which does."""
+    from cta_b200 import _lib
+
+    lib = _lib.load()
+
+    def size(q=(2048, 64), cells=(8192, 512, 64), pages=100, heads=32):
+        args = _lib.PAGED_ATTENTION_ARGS.pack(*(16,) * 9, *q, *q, *cells, *cells, 64, 512, 1, heads, 8, 64, pages, 16, 64,
+                                              512, 1, 0, 0.1, 0.0)
+        return lib.cta_paged_attention_workspace_bytes(args)
+
+    assert size() == 0
+    assert size(pages=0) > 0
+    assert size(pages=1, cells=(0, 512, 64)) == 0  # an axis of one entry has no stride
+    for kw in (dict(q=(0, 64)), dict(q=(2048, -64)), dict(cells=(1 << 39, 512, 64)), dict(cells=(8192, 0, 64))):
+        assert size(**kw) > 0, kw

@@ -494,3 +494,29 @@ def test_tiles_whose_rows_all_see_nothing(keys, heads, kv_heads, rows, hint, qua
     blind = max(0, rows - keys)
     assert (out[:blind] == 0).all()
     s.check(out)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_empty_pool(quantized):
+    """A cache without pages, or a view of none: every sequence is without keys, by whatever kernel the rows choose."""
+    from cta_b200 import _lib, ops
+
+    for rows in ([1, 1], [40, 200]):
+        s = Setup([rows[0], rows[1]], rows, 32, 8, 64, 16, torch.bfloat16, quantized)
+        for empty in (lambda t: t[:0], torch.empty_like):
+            kc, vc, ks, vs = (None if t is None else empty(t[:0]) for t in (s.kc, s.vc, s.ks, s.vs))
+            s.kc, s.vc, s.ks, s.vs = kc, vc, ks, vs
+            s.seq_lens.zero_()
+            assert (s.run(cu_seqlens=s.cu, out=torch.full_like(s.q, 7.0)) == 0).all()
+            s.seq_lens.fill_(5)  # pages that are not there: skipped and reported
+            assert (s.run(cu_seqlens=s.cu, out=torch.full_like(s.q, 7.0)) == 0).all()
+            assert _lib.device_error() == 2
+            slots = torch.full((3,), -1, device="cuda")
+            new = torch.ones(3, 8, 64, dtype=torch.bfloat16, device="cuda")
+            ops.kv_cache_write(new, new, kc, vc, slots, k_scale=ks, v_scale=vs)
+            assert all((x == 0).all() for x in ops.kv_cache_read(kc, vc, slots, k_scale=ks, v_scale=vs))
+            slots[1] = 0
+            ops.kv_cache_write(new, new, kc, vc, slots, k_scale=ks, v_scale=vs)
+            assert _lib.device_error() == 2
+    s = Setup([0, 0], [40, 200], 32, 8, 64, 16, torch.bfloat16, quantized, width=0)  # a table without entries
+    assert s.table.numel() == 0 and (s.run() == 0).all()
