@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -41,6 +42,13 @@ class _PromptAttention(torch.autograd.Function):
         return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
+def _tangents(*tensors: torch.Tensor) -> bool:
+    """Whether one carries a forward-mode tangent: such a call goes through the function, which refuses it.
+    Outside of a dual level, a look at its number (unpack_dual takes 0.4 us a tensor)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def prompt_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -63,7 +71,7 @@ def prompt_attention(
     A row that sees no key is zero and has no gradient, as are packed rows
     behind the last sequence.  Masked keys may hold anything, infinities and NaN
     included; a NaN or infinity in the k or v of a valid token may also reach
-    earlier rows of its sequence."""
+    earlier rows of its sequence.  Forward-mode differentiation raises."""
     words = mask_words
     if key_mask is not None:
         if words is not None:
@@ -73,7 +81,7 @@ def prompt_attention(
         if key_mask.get_device() != q.get_device():
             raise ValueError(f"key_mask on {key_mask.device}, expected {q.device}")
         words = ops.attention_mask(key_mask)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _tangents(q, k, v):
         return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal), scale)
     return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens,
                                  need_lse=False)[0]

@@ -472,3 +472,22 @@ def test_two_streams_at_once(dtype):
         for x in all_of:
             for a, b in zip(want, x):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_forward_mode_raises(dtype):
+    """A tangent is refused, as by the framework's other operators, and not dropped."""
+    import torch.autograd.forward_ad as fw
+
+    from cta_b200.attention import prompt_attention
+
+    q, k, v, g = _inputs((1, 40), 2, 2, 64, dtype)
+    for i in range(3):
+        for grad in (True, False):
+            with fw.dual_level(), torch.set_grad_enabled(grad):
+                t = [q, k, v]
+                t[i] = fw.make_dual(t[i], g)
+                with pytest.raises(RuntimeError, match="forward mode AD"):
+                    prompt_attention(*t)
+    with fw.dual_level():  # inside a level, without a tangent
+        assert torch.equal(prompt_attention(q, k, v), prompt_attention(q, k, v))
