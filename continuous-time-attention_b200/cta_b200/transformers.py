@@ -89,6 +89,8 @@ def _encoder_layers(attention, embed_dim, num_heads, hidden_dim, num_layers, dro
 class PDETransformerClassifier(nn.Module):
     """Sequence classifier with PDE refinement after every layer (transformers.py:35-142)."""
 
+    attention = "torch"  # of objects saved whole before there was a choice
+
     def __init__(
         self,
         vocab_size,
@@ -151,6 +153,8 @@ class PDETransformerClassifier(nn.Module):
 
 class PDETransformerLM(nn.Module):
     """Language model with causal PDE refinement after every layer (transformers.py:220-320)."""
+
+    attention = "torch"  # of objects saved whole before there was a choice
 
     def __init__(
         self,

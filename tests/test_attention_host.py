@@ -204,3 +204,16 @@ def test_paged_kernel_goes_by_what_tma_addresses():
     assert size(pages=1, cells=(0, 512, 64)) == 0  # an axis of one entry has no stride
     for kw in (dict(q=(0, 64)), dict(q=(2048, -64)), dict(cells=(1 << 39, 512, 64)), dict(cells=(8192, 0, 64))):
         assert size(**kw) > 0, kw
+
+
+def test_models_saved_whole_before_the_choice_of_attention():
+    """A model object from before there was a choice has no such attribute and runs as it did."""
+    from cta_b200 import transformers as T
+
+    for cls, kw in ((T.PDETransformerLM, {}), (T.PDETransformerClassifier, dict(num_classes=3))):
+        net = cls(vocab_size=11, embed_dim=16, num_heads=2, hidden_dim=16, num_layers=1, pde_steps=0, max_length=32, **kw)
+        net.eval()
+        ids, mask = torch.randint(0, 11, (2, 9)), torch.ones(2, 9, dtype=torch.long)
+        want = net(ids, mask)
+        net.__dict__.pop("attention", None)
+        assert torch.equal(net(ids, mask), want)
