@@ -61,16 +61,34 @@ def _refine(x: torch.Tensor, pde_list: nn.ModuleList, layout: str, attention_mas
     return diffusion_pde_stack(x, pde_list, attention_mask=attention_mask)
 
 
-class _FusedAttentionLayer(nn.TransformerEncoderLayer):
-    """A post-norm encoder layer (same parameters and names) whose attention runs fused."""
+class _FusedSelfAttention(nn.MultiheadAttention):
+    """The layers' attention module (same parameters and names), running fused."""
 
     def forward(self, x, mask_words, causal):  # type: ignore[override]
-        att = self.self_attn
         B, L, E = x.shape
-        qkv = F.linear(x, att.in_proj_weight, att.in_proj_bias).view(B, L, 3, att.num_heads, E // att.num_heads)
+        qkv = F.linear(x, self.in_proj_weight, self.in_proj_bias).view(B, L, 3, self.num_heads, E // self.num_heads)
         q, k, v = qkv.unbind(2)
-        a = prompt_attention(q, k, v, causal=causal, mask_words=mask_words).reshape(B, L, E)
-        x = self.norm1(x + self.dropout1(att.out_proj(a)))
+        return self.out_proj(prompt_attention(q, k, v, causal=causal, mask_words=mask_words).reshape(B, L, E))
+
+
+class _FusedAttentionLayer(nn.TransformerEncoderLayer):
+    """A post-norm encoder layer (same parameters and names) whose attention runs fused, as a
+    call of its ``self_attn``, so that hooks there see it."""
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self._fuse()
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._fuse()  # saved whole by a version that kept the stock module
+
+    def _fuse(self):
+        # the stock module with another forward: the parameters are drawn once, as in a stock layer
+        self.self_attn.__class__ = _FusedSelfAttention
+
+    def forward(self, x, mask_words, causal):  # type: ignore[override]
+        x = self.norm1(x + self.dropout1(self.self_attn(x, mask_words, causal)))
         return self.norm2(x + self._ff_block(x))
 
 

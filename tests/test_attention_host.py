@@ -217,3 +217,87 @@ def test_models_saved_whole_before_the_choice_of_attention():
         want = net(ids, mask)
         net.__dict__.pop("attention", None)
         assert torch.equal(net(ids, mask), want)
+
+
+def _plain_prompt_attention(q, k, v, *, causal=False, mask_words=None):
+    """What the CPU has in place of the kernel; ``mask_words``: the mask itself."""
+    s = torch.einsum("bihd,bjhd->bhij", q, k) * q.shape[-1] ** -0.5
+    see = mask_words[:, None, None, :] != 0
+    if causal:
+        see = see & torch.ones(s.shape[-2:], dtype=torch.bool).tril()
+    return torch.einsum("bhij,bjhd->bihd", torch.softmax(s.masked_fill(~see, -1e30), -1), v)
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    from cta_b200 import transformers as T
+
+    monkeypatch.setattr(T, "prompt_attention", _plain_prompt_attention)
+    monkeypatch.setattr(T.ops, "attention_mask", lambda mask: mask)
+    return T
+
+
+KW = dict(vocab_size=11, embed_dim=16, num_heads=2, hidden_dim=16, num_layers=2, pde_steps=0, max_length=32, dropout=0.0)
+
+
+def test_fused_attention_runs_through_its_module(plain):
+    """The attention of a layer is the call of its ``self_attn``: hooks there fire, and what they do counts."""
+    torch.manual_seed(0)
+    stock = plain.PDETransformerLM(**KW)
+    torch.manual_seed(0)
+    net = plain.PDETransformerLM(attention="fused", **KW)
+    for (a, x), (b, y) in zip(stock.state_dict().items(), net.state_dict().items()):
+        assert a == b and torch.equal(x, y)  # the same draws under the same names
+    ids, mask = torch.randint(0, 11, (2, 9)), torch.ones(2, 9, dtype=torch.long)
+    want = stock(ids, mask)
+    assert (net(ids, mask) - want).abs().max() <= 1e-5 * want.abs().max()
+    att = net.transformer_layers[0].self_attn
+    assert isinstance(att, torch.nn.MultiheadAttention)
+    seen = []
+    handles = [att.register_forward_pre_hook(lambda m, args: seen.append("before")),
+               att.register_forward_hook(lambda m, args, out: seen.append("after")),
+               att.out_proj.register_forward_hook(lambda m, args, out: seen.append("out_proj"))]
+    net(ids, mask)
+    assert seen == ["before", "out_proj", "after"]
+    for h in handles:
+        h.remove()
+    # a weight that a hook recomputes
+    half = att.register_forward_pre_hook(lambda m, args: (m.in_proj_weight.data.mul_(0.5), None)[1])
+    net(ids, mask)
+    half.remove()
+    with torch.no_grad():
+        stock.transformer_layers[0].self_attn.in_proj_weight.mul_(0.5)
+    want = stock(ids, mask)
+    assert (net(ids, mask) - want).abs().max() <= 1e-5 * want.abs().max()
+
+
+def test_gradients_reach_the_fused_attention(plain):
+    torch.manual_seed(0)
+    stock = plain.PDETransformerClassifier(num_classes=3, **KW)
+    net = plain.PDETransformerClassifier(num_classes=3, attention="fused", **KW)
+    net.load_state_dict(stock.state_dict())
+    ids, mask = torch.randint(0, 11, (2, 9)), torch.ones(2, 9, dtype=torch.long)
+    mask[1, 5:] = 0
+    for x in (stock, net):
+        x.train()
+        x(ids, mask).square().sum().backward()
+    for (n, a), b in zip(stock.named_parameters(), net.parameters()):
+        assert (a.grad - b.grad).abs().max() <= 1e-4 * a.grad.abs().max() + 1e-7, n
+
+
+def test_fused_models_are_saved_and_copied_whole(plain, tmp_path):
+    """Copies and pickles keep the fused module; one that was saved with the stock module in its place gets it."""
+    import copy
+
+    torch.manual_seed(0)
+    net = plain.PDETransformerLM(attention="fused", **KW)
+    ids, mask = torch.randint(0, 11, (2, 9)), torch.ones(2, 9, dtype=torch.long)
+    want = net(ids, mask)
+    old = copy.deepcopy(net)
+    for layer in old.transformer_layers:
+        layer.self_attn.__class__ = torch.nn.MultiheadAttention
+    for i, x in enumerate((net, old)):
+        torch.save(x, tmp_path / f"{i}.pt")
+        back = torch.load(tmp_path / f"{i}.pt", weights_only=False)
+        assert torch.equal(back(ids, mask), want)
+    assert torch.equal(copy.deepcopy(net)(ids, mask), want)
