@@ -616,10 +616,11 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
 #pragma unroll 4
   for (int x = warp; x < parts; x += warps) {
     const int64_t at = slot_of(x) * kPartRows + r;
-    const float4 ml = __ldg(reinterpret_cast<const float4*>(a.part_ml + at * 4));
+    // ordinary loads: the parts are written while this kernel may already be there
+    const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml + at * 4));
     float po[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) po[e] = __ldg(a.part_o + at * DP + lane + 32 * e);
+    for (int e = 0; e < V; ++e) po[e] = __ldcg(a.part_o + at * DP + lane + 32 * e);
     const float top = fmaxf(m, ml.x), topv = fmaxf(mv, ml.z);
     const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
     l = l * ex2(m - base) + ml.y * ex2(ml.x - base);
