@@ -381,11 +381,17 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
     for (int x = 0; x < DC; ++x) dk[r][x] = dv[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float c2 = a.scale * kLog2e;
+  int lo, hi;
+  mask_range(a, t.batch, t.n, lo, hi);
+  // rows that see no key, up to the first valid one, may hold anything
+  const int from = lo >= hi ? t.n : a.causal ? lo : 0;
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
     for (int i0 = a.causal ? t.first : 0; i0 < t.n; i0 += QT) {
+      if (from >= i0 + QT) continue;
+      const uint64_t seeing = from > i0 ? ~0ull << (from - i0) : ~0ull;
       __syncthreads();
-      load_rows<T, QT, DP>(Q, a.q, a.qs, t, h, i0, t.n, a.d, ~0ull);
-      load_rows<T, QT, DP>(G, a.g, a.gs, t, h, i0, t.n, a.d, ~0ull);
+      load_rows<T, QT, DP>(Q, a.q, a.qs, t, h, i0, t.n, a.d, seeing);
+      load_rows<T, QT, DP>(G, a.g, a.gs, t, h, i0, t.n, a.d, seeing);
       if (threadIdx.x < QT) {
         const int i = i0 + threadIdx.x;
         s_lse[threadIdx.x] = i < t.n ? a.lse[lse_index(a, t, h, i)] * kLog2e : neg_inf();

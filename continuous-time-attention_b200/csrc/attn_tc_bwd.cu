@@ -436,13 +436,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < steps && ok; ++s) {
       const uint32_t q = smem + (2 + 2 * (s % NS)) * L::kTile, g = q + L::kTile;
       ok = tc::wait(&bars.q_full[s % NS], (s / NS) & 1);
-      // packed: rows of the next sequence in a tile that reaches past this one, in both tensors before
-      // anything is made of either
+      // Packed: rows of the next sequence in a tile that reaches past this one; causal behind a mask: rows up to the
+      // first valid key, which see none and may hold anything.  In both tensors before anything is made of either.
       const int rows = min(t.n - first_of(s), kRows) * f.pack;
-      if (a.cu != nullptr && rows < kRows) {
+      const int blind_rows = a.causal ? min(lo - first_of(s), kRows) * f.pack : 0;
+      if ((a.cu != nullptr && rows < kRows) || blind_rows > 0) {
         ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
-        uint32_t w[4];
+        uint32_t w[4], x[4];
         tc::first_bits(rows, w);
+        tc::first_bits(blind_rows, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] &= ~x[i];
         if (ok) {
           tc::clear_rows<DP / 64>(q, w);
           tc::clear_rows<DP / 64>(g, w);

@@ -491,3 +491,27 @@ def test_forward_mode_raises(dtype):
                     prompt_attention(*t)
     with fw.dual_level():  # inside a level, without a tangent
         assert torch.equal(prompt_attention(q, k, v), prompt_attention(q, k, v))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 2, 1), (128, 4, 4), (72, 8, 1), (20, 2, 2), (160, 2, 1)])
+def test_rows_that_see_nothing_take_no_part(dim, heads, kv_heads, dtype):
+    """Left padding, causal: q and the output's gradient of rows that see no key may hold anything, NaN included,
+    and reach no gradient."""
+    n = 300
+    q, k, v, g = _inputs((3, n), heads, kv_heads, dim, dtype, seed=dim)
+    valid = torch.ones(3, n, dtype=torch.bool)
+    valid[0, :140] = False
+    valid[1, :5] = False
+    valid[1, 9] = False
+    valid[2] = False
+    hidden = ~valid.cuda()
+    blind = hidden.cumprod(1).bool()
+    k[hidden], v[hidden] = float("nan"), float("inf")
+    q[blind], g[blind] = float("nan"), float("inf")
+    got = _run(q, k, v, g, causal=True, key_mask=valid.cuda())
+    clean_q, clean_g = q.masked_fill(blind[..., None, None], 0), g.masked_fill(blind[..., None, None], 0)
+    for b in range(3):
+        _check_sequence([x[b] for x in got], clean_q[b], k[b], v[b], clean_g[b], _see(n, True, valid[b]), dim**-0.5, dtype,
+                        f"{b}: ")
+        assert (got[0][b][blind[b]] == 0).all() and (got[1][b][blind[b]] == 0).all()
