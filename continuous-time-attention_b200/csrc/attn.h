@@ -67,7 +67,7 @@ struct CacheArgs {
   void* k_cache;
   void* v_cache;
   int64_t kc_sP, kc_sS, kc_sH, vc_sP, vc_sS, vc_sH;  // page, slot in page, head
-  float* k_scale;  // e4m3 caches: [pages, page, Hk] contiguous
+  float* k_scale;  // e4m3 caches: [pages, Hk, page] contiguous
   float* v_scale;
   const int64_t* slots;
   int64_t T, n_slots;
@@ -99,8 +99,9 @@ struct PagedArgs {
   int workers;
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
-  // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these the fractions of the
-  // scales [B, Hk, residue_row(table_width * page)]; else nullptr
+  // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these what it left out of their
+  // elements [B, Hk, residue_row(table_width * page)]: the fractions of the scales in bf16, the key's scale and the
+  // logarithm (base 2) of the value's in fp16; else nullptr
   const float* k_res;
   const float* v_res;
 };
@@ -118,7 +119,7 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
 // b * table_width + i), for the tensor-core kernel
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
                                 cudaStream_t st);
-// fractions of a sequence's scales per head, in whole key tiles
+// entries of k_res and v_res for a sequence and head, in whole key tiles
 __host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots + 127) / 128 * 128; }
 
 int read_device_error_paged(int clear);

@@ -247,8 +247,8 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
 // the other kernel over one wave of its CTAs 15 ns per key, i.e. as much as 137 such tiles.  One
 // sequence of 8192 keys: 64 rows 96 us split, 142 us on tensor cores; 128 rows 179 and 144 us.  8
 // sequences of 4096: 8 rows 65 and 69 us, 16 rows 112 and 70 us.  Over an e4m3 cache the pages have to
-// be expanded first: 32 sequences of 2048, 8 rows 119 and 198 us, 16 rows 225 and 199 us; one of
-// 8192 keys, 512 rows: 675 and 295 us.
+// be expanded first: 32 sequences of 2048, 8 rows 119 and 198 us, 16 rows 225 and 199 us (fp16 232); one of
+// 8192 keys, 512 rows: 675 and 299 us (fp16 408).
 //
 // What TMA cannot address, a pool without pages among it, is for the split kernel.
 bool tma_strides(std::initializer_list<int64_t> elements) {
@@ -274,8 +274,8 @@ bool tensor_cores_pay(const PagedArgs& a) {
   return tiles > (a.k_scale != nullptr ? 256 : 128) * ((ctas + 147) / 148);
 }
 
-// 16-bit copy of the pages that the table can name, k then v, and the fractions of their scales; 0 where that is too
-// much to ask for
+// 16-bit copy of the pages that the table can name, k then v, and what goes beside them; 0 where that is too much to
+// ask for
 constexpr int64_t kMostExpanded = 1LL << 31;
 int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64_t d) {
   const int64_t slots = b * width * page;

@@ -1,13 +1,16 @@
 // Attention forward on the tensor cores: whole prompts, and chunks of rows over
 // a 16-bit paged cache.
 //
-// An e4m3 cache is first expanded to 16-bit pages (kv_cache.cu) that hold codes
-// times the power of two below their scale, which 16 bits represent exactly.  The
-// rest of the scale, in [1, 2), multiplies the key's scores and, after the sum of
-// the weights, its weights.  That costs the softmax more than a 16-bit cache does
-// (512 rows over 8192 keys, 32/8 heads of 128: 295 and 142 us); with k and v times
-// their whole scale, rounded to 16 bits, the call took 157 us, but fp16 outputs
-// were twice as far off as one rounding of them, and are 1.4 times now.
+// An e4m3 cache is first expanded to 16-bit pages (kv_cache.cu) whose elements are exact.
+// bf16: codes times the power of two below their scale; the rest of the scale, in [1, 2),
+// multiplies the key's scores and, after the sum of the weights, its weights.  fp16, which
+// does not reach as far as scales do: the codes alone; the key's scale multiplies the scores,
+// and the value's joins the weight's exponent, relative to a running maximum of its own, so
+// that any scales are right (with powers of two in the elements, as in bf16, scales from 256 on
+// were infinite, and codes under scales below 2^-15 rounded).  Both cost the softmax more than a
+// 16-bit cache does: 512 rows over 8192 keys, 32/8 heads of 128, take 143 us over 16 bits,
+// 299 in bf16 and 408 in fp16 over e4m3; with k and v times their whole scale, rounded to 16
+// bits, the call took 157 us, but fp16 outputs were twice as far off as one rounding of them.
 //
 // A CTA owns two 128-row tiles of one block of heads.  A row is a (token, head)
 // pair: where query heads share a key/value head, the largest power of two of
@@ -51,6 +54,8 @@ constexpr int kThreads = 640;  // five warpgroups
 constexpr int kSoftmaxWarps = 16;
 constexpr int kRows = 128;  // rows of a tile, and keys of a step
 constexpr float kLazy = 8.f;
+// fp16 weights carry 2^7, and so stay below 2^15; what is lost to subnormals is below 2^-32 of the reference
+constexpr float kHalfShift = 7.f;
 
 struct FwdArgs {
   AttnArgs a;
@@ -63,7 +68,7 @@ struct FwdArgs {
   const int32_t* seq_lens;
   int table_width, page, n_pages, box;  // box: keys per TMA box
   // SCALED: page i of sequence b is page b * table_width + i (the table still says which are valid), and these are
-  // the scales' fractions
+  // what the expansion left out of its elements, see launch_cache_expand
   const float* k_res;
   const float* v_res;
   int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
@@ -100,12 +105,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Half of a step's weights are announced too, which wakes the waiting MMA warp ahead of time: 402
   // instead of 454 us at 8192 keys, 16 heads of 64, but 534 instead of 503 at 128.
   constexpr bool kEarly = DP == 64;
+  // Over an expanded e4m3 cache in fp16 the value's scale joins the weight, whose own running reference keeps the
+  // product within fp16 for any scales.
+  constexpr bool kWeighted = SCALED && std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
   __shared__ Item s_item;
   __shared__ __align__(16) uint4 s_answer;
   __shared__ float s_max[2][2][kRows], s_sum[2][2][kRows];  // [tile][half of the keys][row]
+  __shared__ float s_maxv[kWeighted ? 2 : 1][2][kWeighted ? kRows : 1];
   __shared__ uint32_t s_boxes[16];  // paged: which boxes of a key tile were loaded
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -425,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                              j_lo * kRows + 64 * half
                        : 0;
       float m = neg_inf(), sum = 0.f;
+      float mv = neg_inf();  // kWeighted: the reference of weight * scale, as an exponent of two
       for (int j = 0; j < count; ++j, ++ns, res += SCALED ? kRows : 0) {
         if (SCALED && lane < 4)  // two lines each of the step's fractions
           asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 2 ? f.k_res : f.v_res) + res + 32 * (lane & 1)));
@@ -476,12 +486,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e)
             if (!((see >> e) & 1u)) x[e] = 0xff800000u;
         };
-        float t[4];
+        float t[4], topv = mv;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t(&x)[32] = s[SCALED ? 0 : c];
           if (SCALED) scale(c, x);
           if (!whole) hide(c, x);
+          if constexpr (kWeighted) {
+            // score + logarithm of the value's scale
+            float4 r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 lo = fma2(make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])), f2(c2),
+                                     make_float2(r[e].x, r[e].y));
+              const float2 hi = fma2(make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])), f2(c2),
+                                     make_float2(r[e].z, r[e].w));
+              topv = tc::max3(tc::max3(lo.x, lo.y, hi.x), hi.y, topv);
+            }
+          }
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             float& z = t[2 * c + y];
@@ -495,13 +519,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         float top = tc::max3(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]), m);
         // The reference of a row moves when one of its halves has grown by more than kLazy past it (or
         // there was none): one barrier with a vote per step, and the halves' maxima only then.
-        if (tc::any_of(1 + i, 2 * kRows, top > m && !((top - m) * c2 <= kLazy))) {
+        auto far = [&] {
+          return (top > m && !((top - m) * c2 <= kLazy)) || (kWeighted && topv > mv && !(topv - mv <= kLazy));
+        };
+        if (tc::any_of(1 + i, 2 * kRows, far())) {
           s_max[i][half][row] = top;
+          if constexpr (kWeighted) s_maxv[i][half][row] = topv;
           tc::sync_of(1 + i, 2 * kRows);
           top = fmaxf(top, s_max[i][half ^ 1][row]);
-          const bool move = top > m && !((top - m) * c2 <= kLazy);
-          const float shrink = move ? ex2((m - top) * c2) : 1.f;
-          if (move) {
+          if constexpr (kWeighted) topv = fmaxf(topv, s_maxv[i][half ^ 1][row]);
+          const bool move = far();
+          float shrink = 1.f;
+          if constexpr (kWeighted) {
+            if (move) {
+              if (top > m) sum *= ex2((m - top) * c2);
+              if (topv > mv) shrink = ex2(mv - topv);
+              m = fmaxf(m, top);
+              mv = fmaxf(mv, topv);
+            }
+          } else if (move) {
+            shrink = ex2((m - top) * c2);
             sum *= shrink;
             m = top;
           }
@@ -520,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float base = m == neg_inf() ? 0.f : -m * c2;
         const float2 c2v = f2(c2), bv = f2(base);
+        const float2 vv = f2(mv == neg_inf() ? 0.f : kHalfShift - mv);
         float2 part = f2(0.f), part2 = f2(0.f);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -534,14 +572,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float2 y = fma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2v, bv);
+            const float2 score = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+            float2 y = fma2(score, c2v, bv);
             y.x = ex2(y.x);
             y.y = ex2(y.y);
             if (e & 1) part2 = add2(part2, y);
             else part = add2(part, y);
             if constexpr (SCALED) {
               const float4& z = r[e / 2];
-              y = mul2(y, (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y));
+              const float2 of_value = (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
+              if constexpr (kWeighted) {
+                y = fma2(score, c2v, add2(of_value, vv));
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+              } else {
+                y = mul2(y, of_value);
+              }
             }
             p[e] = tc::pack2<T>(y.x, y.y);
           }
@@ -569,7 +615,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         sum += s_sum[i][half ^ 1][row];
       }
-      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays
+      // the factor between the references, which a scale past 2^120 takes out of fp32's range, and fp16's anyway
+      const float unit = kWeighted ? ex2(fminf(mv - kHalfShift - m * c2, 127.f)) : 1.f;
+      const float inv = sum > 0.f ? unit / sum : sum == 0.f ? 0.f : sum;  // NaN stays
       tc::store_rows<T, DP / 2>(o_addr, out, half * (DP / 2), a.d, inv, live, f.wide_out, count > 0);
       if (!PAGED && a.low != nullptr) {
         T* low = static_cast<T*>(a.low) + ((x.t.batch * a.L + x.t.row0 + tok) * a.H + h) * a.d;

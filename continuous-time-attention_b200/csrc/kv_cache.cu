@@ -190,8 +190,9 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   }
 }
 
-// codes of the pages of each sequence, in order, as 16-bit rows: each times the power of two below its scale, whose
-// fraction goes into k_res and v_res (attn_tc_fwd.cu says why)
+// Codes of the pages of each sequence, in order, as exact 16-bit rows.  bf16, whose exponents reach as far as fp32's:
+// each times the power of two below its scale, whose fraction goes into k_res and v_res.  fp16: the codes alone, and
+// beside them the key's scale and the logarithm of the value's (attn_tc_fwd.cu says why).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out,
                                                                 float* k_res, float* v_res) {
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
   const unsigned row = group / blocks, b = row / slots, j = row - b * slots;
   const int h0 = static_cast<int>(group - row * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
   if (b >= static_cast<unsigned>(a.B)) return;
-  // the scales' fractions of this key, and behind the last key up to the row's end
+  // what goes beside this key, and behind the last key up to the row's end
   const int64_t res_row = residue_row(slots);
   float* res = (second ? v_res : k_res) + (static_cast<int64_t>(b) * a.Hk + h0) * res_row;
   if (j + 1 == slots)
@@ -235,10 +236,16 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
 #pragma unroll
   for (int i = 0; i < kHeads; ++i)
     if (h0 + i < a.Hk) {
-      // sign and exponent of the scale go into the element, which stays exact, its fraction beside it
-      const uint32_t bits = __float_as_uint(mul[i]);
-      const float pow = __uint_as_float(bits & 0xff800000u);
-      if (lane == 0) res[i * res_row + j] = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+      float pow = 1.f, rest;
+      if constexpr (std::is_same<T, __half>::value) {
+        // an infinite scale must not make a NaN of a weight that is zero
+        rest = second ? fminf(__log2f(mul[i]), 128.f) : mul[i];
+      } else {
+        const uint32_t bits = __float_as_uint(mul[i]);
+        pow = __uint_as_float(bits & 0xff800000u);
+        rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+      }
+      if (lane == 0) res[i * res_row + j] = rest;
       float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

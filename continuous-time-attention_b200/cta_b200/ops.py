@@ -898,9 +898,10 @@ def paged_attention(
     q [T, heads, dim]; cu_seqlens (int32, B + 1) gives the rows of each of the B
     sequences, None one row each (decode).  seq_lens [B] (int32) counts all keys
     of a sequence, block_table [B, width] (int32) lists its pages.  Row r of n_r
-    sees keys j <= seq_len - n_r + r.  Chunks over an e4m3 cache may be computed
-    from a copy of the codes in 16 bits, in a workspace.  max_rows, the longest n_r as the host
-    knows it, only chooses the kernel.  No device data is read on the host.
+    sees keys j <= seq_len - n_r + r.  Scales may be positive normal numbers of any size.
+    Chunks over an e4m3 cache may be computed from a copy of the codes in 16 bits, in a
+    workspace of up to 2 GiB.  max_rows, the longest n_r as the host knows it, only chooses
+    the kernel.  No device data is read on the host.
     Rows that see no key are zero; rows behind the last sequence are not
     written.  A page outside the cache or a length past the table counts as no
     keys and is reported by ``_lib.device_error()``."""

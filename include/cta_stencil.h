@@ -386,7 +386,8 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
  * data.  A page outside the cache or a length past the table counts as no keys
  * and is reported by cta_device_error() as 2.  page_size: a multiple of 16;
  * dim: a multiple of 16 up to 128; dtype: CTA_BF16, CTA_F16 (of q and out).
- * Chunks over an e4m3 cache may be computed from a copy of the codes in 16 bits.
+ * Chunks over an e4m3 cache may be computed from a copy of the codes in 16 bits
+ * (a workspace of up to 2^31 bytes).  Scales are positive normal numbers of any size.
  * workspace: cta_paged_attention_workspace_bytes(args) bytes (sizes, types and
  * strides of args count, of its pointers only which are NULL; 0 = none; negative:
  * minus the status with which the call would refuse the arguments) on 16, not

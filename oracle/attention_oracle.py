@@ -68,9 +68,11 @@ def gradients(q, k, v, g, see, scale):
             _fold(torch.matmul(p.transpose(1, 2), gh), hk))
 
 
-def bounds(q, k, v, see, scale, dtype, g=None, kv_error=0.0):
+def bounds(q, k, v, see, scale, dtype, g=None, kv_error=0.0, weight_step=None, grad_steps=None):
     """Tolerances of out, or with g of (out, dq, dk, dv).  kv_error: a relative error that k
-    and v already carry on their way into the products."""
+    and v already carry on their way into the products.  weight_step: the error of a weight that
+    is too small for its type, grad_steps: of (P, dS) in the gradients' products; by default fp16's
+    smallest step, and nothing in the other types, whose exponents reach as far as fp32's."""
     u = 2.0**-24
     w = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
     r = torch.finfo(dtype).eps / 2
@@ -87,7 +89,10 @@ def bounds(q, k, v, see, scale, dtype, g=None, kv_error=0.0):
     # a result below the type's normal range is rounded to its smallest step; a weight too
     step = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     tiny = step if dtype == torch.float16 else 0.0
-    low = tiny * torch.matmul(see.double().expand_as(p), vh.abs())
+    if weight_step is None:
+        weight_step = tiny
+    p_step, ds_step = (tiny, tiny) if grad_steps is None else grad_steps
+    low = weight_step * torch.matmul(see.double().expand_as(p), vh.abs())
     tol = tol + step + low
     if g is None:
         return tol.transpose(0, 1)
@@ -96,11 +101,11 @@ def bounds(q, k, v, see, scale, dtype, g=None, kv_error=0.0):
     ds = p * (dp - (gh * out).sum(-1, keepdim=True))
     t_delta = (gh.abs() * tol).sum(-1, keepdim=True) + (d + 4) * u * (gh * out).abs().sum(-1, keepdim=True)
     t_dp = (d + 4) * u * torch.matmul(gh.abs(), vh.abs().transpose(1, 2))
-    t_ds = ds.abs() * e_p + p * (t_dp + t_delta) + tiny * see
+    t_ds = ds.abs() * e_p + p * (t_dp + t_delta) + ds_step * see
     m = q.shape[0]
     t_dq = abs(scale) * torch.matmul(t_ds + sums * ds.abs(), kh.abs())
     t_dk = abs(scale) * torch.matmul((t_ds + (m + 8) * u * ds.abs()).transpose(1, 2), qh.abs())
-    t_dv = torch.matmul((p * (e_p + (m + 8) * u) + tiny * see).transpose(1, 2), gh.abs())
+    t_dv = torch.matmul((p * (e_p + (m + 8) * u) + p_step * see).transpose(1, 2), gh.abs())
     dq, dk, dv = gradients(q, k, v, g, see, scale)
     return (tol.transpose(0, 1), t_dq.transpose(0, 1) + r * dq.abs() + step, _fold(t_dk, hk) + r * dk.abs() + step,
             _fold(t_dv, hk) + r * dv.abs() + step)

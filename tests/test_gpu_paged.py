@@ -520,3 +520,82 @@ def test_empty_pool(quantized):
             assert _lib.device_error() == 2
     s = Setup([0, 0], [40, 200], 32, 8, 64, 16, torch.bfloat16, quantized, width=0)  # a table without entries
     assert s.table.numel() == 0 and (s.run() == 0).all()
+
+
+def _rescaled(s, ks=1.0, vs=1.0, q=1.0):
+    """Other scales over the same codes: powers of two, so that the cache's values stay known exactly."""
+    s.ks *= ks
+    s.vs *= vs
+    s.k, s.v = [x * ks for x in s.k], [x * vs for x in s.v]
+    s.q = s.q * q
+
+
+def _check_scaled(s, out):
+    """Against the definition, with no allowance for what 16 bits cannot hold of a weight but this: weight times
+    value's scale is held relative to the largest of them so far, with a smallest step of 2^-31 of it (fp16:
+    2^-24, shifted by 2^7), so each key is off by at most 2^-32 of the row's largest weight * scale, times its
+    code, 448 at most and 448 in the largest element of each row.  A scale that joins a weight through its
+    logarithm (up to 64 here, 2^-24 of it) moves it by 2^-18."""
+    at = 0
+    for b, (n, r) in enumerate(zip(s.lens, s.rows)):
+        q, got = s.q[at : at + r], out[at : at + r].double()
+        at += r
+        see = torch.arange(n, device="cuda")[None, :] <= torch.arange(n - r, n, device="cuda")[:, None]
+        scale = s.dim**-0.5
+        want, _ = A.attention(q, s.k[b], s.v[b], see, scale)
+        assert want.abs().max() < torch.finfo(s.dtype).max
+        tol = A.bounds(q, s.k[b], s.v[b], see, scale, s.dtype, kv_error=2.0**-20, weight_step=0.0)
+        p, _ = A.weights(q, s.k[b], see, scale)
+        v = s.v[b].abs().transpose(0, 1).repeat_interleave(q.shape[1] // s.v[b].shape[1], 0)  # [H, n, dim]
+        most = (p * v.amax(-1)[:, None]).amax(-1, keepdim=True)
+        tol = tol + (n * 2.0**-32 * most + 2.0**-18 * torch.matmul(p, v)).transpose(0, 1)
+        bad = ~((got - want).abs() <= tol)
+        assert not bad.any(), (b, n, r, int(bad.sum()), (got - want).abs().max().item(), want.abs().max().item())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("written", DTYPES)
+def test_e4m3_scales_outside_the_type(written, dim, rows, dtype):
+    """Scales that fp32 holds and fp16 does not, codes times them included: decode and chunks alike, whatever type
+    the cache was written from."""
+    def setup(**kw):
+        s = Setup([300, 250], rows, 32, 8, dim, 16, written, True, **kw)
+        s.q, s.dtype = s.q.to(dtype), dtype
+        return s
+
+    for kw in (dict(ks=2.0**19, q=2.0**-19), dict(ks=2.0**17, q=2.0**-14), dict(ks=2.0**-13, q=2.0**12),
+               dict(ks=2.0**-40, q=2.0**13), dict(vs=2.0**-10), dict(vs=2.0**-17), dict(vs=2.0**11),
+               dict(ks=2.0**-13, q=2.0**11, vs=2.0**9)):
+        s = setup()
+        _rescaled(s, **kw)
+        _check_scaled(s, s.run())
+    # rows of different size in one sequence, as a whole far down and up
+    for vs in (1.0, 2.0**-10, 2.0**4):
+        s = setup(spread=1.5, seed=3)
+        _rescaled(s, vs=vs)
+        _check_scaled(s, s.run())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+def test_e4m3_large_values_of_little_weight(rows, dtype):
+    """Every fourth key has values 2^17 times the others', past fp16, and a weight that makes up for it."""
+    from cta_b200 import ops
+
+    s = Setup([300, 250], rows, 32, 8, 64, 16, dtype, True, seed=4)
+    s.q = s.q.abs() + 1
+    page = s.kc.shape[1]
+    # their scores are about -115 * 0.85 / 8 = -12, a weight of 2^-17.6
+    for b, n in enumerate(s.lens):
+        j = torch.arange(0, n, 4, device="cuda")
+        slots = s.table[b].long()[j // page] * page + j % page
+        far = -(0.7 + 0.3 * torch.rand(len(j), 8, 64, generator=torch.Generator().manual_seed(b))).cuda().to(dtype)
+        ops.kv_cache_write(far, s.v[b][j].to(dtype), s.kc, s.vc, slots, k_scale=s.ks, v_scale=s.vs)
+        at = (slots // page, slice(None), slots % page)
+        s.vs[at] *= 2.0**17
+        s.k[b][j] = _codes(s.kc, slots) * s.ks[at].double()[..., None]
+        s.v[b][j] = _codes(s.vc, slots) * s.vs[at].double()[..., None]
+    assert s.v[0].abs().max() > torch.finfo(torch.float16).max
+    _check_scaled(s, s.run())
