@@ -38,6 +38,10 @@ namespace {
 constexpr int kThreads = 640;  // five warpgroups; the last has a warp or two to spare
 constexpr int kWeightWarps = 16;
 constexpr int kRows = 128;
+// In fp16 the P of dV carries 2^14: of thousands of keys it would lie among the type's subnormal numbers (one of
+// 41891 equal weights was 1.2e-3 off), and with 2^14 what is lost is below 2^-39.  P is at most 1, but for the
+// rounding of scores and lse.
+constexpr float kHalfShift = 14.f, kHalfUnit = 0x1p-14f;
 
 struct BwdArgs {
   AttnArgs a;
@@ -315,13 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DkvBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ SeqTile s_tile;
-  __shared__ __align__(16) float s_stat[NS][2][kRows];  // [stage][-lse2, -delta][row]
+  __shared__ __align__(16) float s_stat[NS][2][kRows];  // [stage][-lse2, -delta, fp16: + 14, * 2^-14][row]
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
   // With two score buffers dS goes beside P, into the columns that P leaves of its scores', and the next dO V^T can
   // start once this one has been read; with one it goes over dO V^T, so that the next scores wait for dV only.
   constexpr bool kBeside = DP == 64;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
   pdl_launch_dependents();  // dQ's CTAs may follow
 
@@ -417,6 +422,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         nl[i] = tok < t.n ? neg_lse2_of(__ldg(a.lse + lse_index(a, t, h, tok))) : neg_inf();
         dl[i] = tok < t.n ? -__ldg(a.delta + lse_index(a, t, h, tok)) : 0.f;
         if (blind(nl[i])) dl[i] = 0.f;
+        if constexpr (kHalf) {
+          nl[i] += kHalfShift;
+          dl[i] *= kHalfUnit;
+        }
       }
       if (s >= NS) ok = tc::wait(&bars.q_empty[stage], ((s / NS) - 1) & 1);
       if (!ok) break;
@@ -501,6 +510,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool valid = key < t.n && (mask == nullptr || mask_key(mask, key));
     const float c2 = a.scale * kLog2e;
+    auto less_delta = [](float2 dp, float2 neg_delta) {
+      if constexpr (kHalf) return fma2(dp, f2(kHalfUnit), neg_delta);
+      else return add2(dp, neg_delta);
+    };
     bool ok = true;
     for (int s = 0; s < steps && ok; ++s) {
       const int stage = s % NS;
@@ -556,9 +569,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e = 0; e < 32; e += 4) {
         const float4 b = dl[e / 4];
         const float2 x = mul2(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])),
-                              add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), make_float2(b.x, b.y)));
+                              less_delta(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), make_float2(b.x, b.y)));
         const float2 y = mul2(make_float2(__uint_as_float(p[e + 2]), __uint_as_float(p[e + 3])),
-                              add2(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), make_float2(b.z, b.w)));
+                              less_delta(make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3])), make_float2(b.z, b.w)));
         w[e / 2] = tc::pack2<T>(x.x, x.y);
         w[e / 2 + 1] = tc::pack2<T>(y.x, y.y);
       }
@@ -585,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c0 = (part & 1) * (DP / 2);  // parts 0, 1: dV, parts 2, 3: dK, half of the columns each
       if (part < 2) {
         T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
-        tc::store_rows<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, 1.f, live, f.wide_dv, steps > 0);
+        tc::store_rows<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, kHalf ? kHalfUnit : 1.f, live, f.wide_dv, steps > 0);
       } else {
         T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
         tc::store_rows<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, a.scale, live, f.wide_dk, steps > 0);

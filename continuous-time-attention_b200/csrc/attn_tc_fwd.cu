@@ -56,6 +56,7 @@ constexpr int kRows = 128;  // rows of a tile, and keys of a step
 constexpr float kLazy = 8.f;
 // fp16 weights carry 2^7, and so stay below 2^15; what is lost to subnormals is below 2^-32 of the reference
 constexpr float kHalfShift = 7.f;
+static_assert(kHalfShift == 7.f, "lse takes 2^-7 of the sum");
 
 struct FwdArgs {
   AttnArgs a;
@@ -108,6 +109,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Over an expanded e4m3 cache in fp16 the value's scale joins the weight, whose own running reference keeps the
   // product within fp16 for any scales.
   constexpr bool kWeighted = SCALED && std::is_same<T, __half>::value;
+  constexpr float kShift = std::is_same<T, __half>::value && !SCALED ? kHalfShift : 0.f;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float base = m == neg_inf() ? 0.f : -m * c2;
+        const float base = m == neg_inf() ? 0.f : kShift - m * c2;
         const float2 c2v = f2(c2), bv = f2(base);
         const float2 vv = f2(mv == neg_inf() ? 0.f : kHalfShift - mv);
         float2 part = f2(0.f), part2 = f2(0.f);
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         T* low = static_cast<T*>(a.low) + ((x.t.batch * a.L + x.t.row0 + tok) * a.H + h) * a.d;
         tc::store_rows<T, DP / 2, true>(o_addr, low, half * (DP / 2), a.d, inv, live, f.wide_low, count > 0);
       }
-      if (lse != nullptr) *lse = sum == 0.f ? neg_inf() : (m * c2 + log2f(sum)) * kLn2;
+      if (lse != nullptr) *lse = sum == 0.f ? neg_inf() : (m * c2 + log2f(kShift == 0.f ? sum : sum * 0x1p-7f)) * kLn2;
       tc::fence_before();  // O has been read before the next piece's first weights are announced
     }
     if (!ok && lane == 0) atomicExch(&g_tc_fwd_error, kDevTimeout);

@@ -515,3 +515,45 @@ def test_rows_that_see_nothing_take_no_part(dim, heads, kv_heads, dtype):
         _check_sequence([x[b] for x in got], clean_q[b], k[b], v[b], clean_g[b], _see(n, True, valid[b]), dim**-0.5, dtype,
                         f"{b}: ")
         assert (got[0][b][blind[b]] == 0).all() and (got[1][b][blind[b]] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_equal_weights_of_little_size(dim, dtype):
+    """41891 keys of equal weight: 1 / 41891 is 400.497 steps of fp16's smallest, 1.2e-3 off when rounded to one.  dV
+    is then the same everywhere, the sum of g over 41891."""
+    n, m = 41891, 64
+    q = torch.zeros(1, n, 1, dim, dtype=dtype, device="cuda")
+    k, v = (torch.randn(1, n, 1, dim, generator=torch.Generator().manual_seed(i)).to(dtype).cuda() for i in (1, 2))
+    g = torch.zeros_like(q)
+    g[0, 1000 : 1000 + m] = (torch.rand(m, 1, dim, generator=torch.Generator().manual_seed(3)) * 64 + 32).to(dtype).cuda()
+    dv = _run(q, k, v, g)[3].double()
+    want = (g.double().sum(1, keepdim=True) / n).expand_as(dv)
+    # P and dv are rounded once each; m terms are summed in fp32; lse = 10.6 and the sum of n weights, each 1 exactly,
+    # (its logarithm 15.4) are rounded a few times, by 3e-6 in all; the exponential is off by 2^-21
+    eps = torch.finfo(dtype).eps
+    tol = want * (eps + (m + 8) * 2.0**-24 + 2.0**-18) + torch.finfo(dtype).smallest_normal * eps
+    _within(dv, want, tol, "dv")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_weights_beside_a_large_one(dim, dtype):
+    """One key of weight 1 and value 0, 4000 of weight exp(-11.4453125) = 179.507 steps of fp16's smallest."""
+    from cta_b200.attention import prompt_attention
+
+    n, dot = 4001, -11.4453125
+    q = torch.zeros(1, n, 2, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    k = torch.zeros_like(q)
+    k[:, 1:, :, 0] = dot
+    v = torch.ones_like(q)
+    v[:, 0] = 0.0
+    out = prompt_attention(q, k, v, scale=1.0).double()
+    w = torch.exp(torch.tensor(k[0, 1, 0, 0].item(), dtype=torch.float64)).item()
+    want = torch.full_like(out, 4000 * w / (1 + 4000 * w))
+    # weights and output are rounded once each; the exponential 2^-21, the scores 2^-24 * 11.4 * 4, the sums below
+    # (n / 64 + 80) 2^-24 of themselves: every 64 weights are added by themselves first
+    eps = torch.finfo(dtype).eps
+    _within(out, want, want * (eps + 2.0**-20 + 50 * 2.0**-24 + (n / 64 + 80) * 2.0**-24), "out")
+
