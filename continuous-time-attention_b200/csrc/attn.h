@@ -25,6 +25,8 @@ struct AttnArgs {
   float* lse;        // [nseq, H, L] dense, [H, L] packed; natural logarithm, -inf for a row without keys
   const void* g;     // backward: gradient of the output
   float* delta;      // backward scratch, laid out as lse: sum_d g * o
+  float* g_norm;     // fp16 on tensor cores, else nullptr: |g| of each row, laid out as lse
+  float* v_norm;     // and |v| of each key, [nseq, Hk, L] dense, [Hk, L] packed, 0 for a masked one
   void* dq;
   void* dk;
   void* dv;

@@ -322,6 +322,12 @@ int cta_attention_backward(const cta_attention_args* args, void* stream) {
   if (a.g == nullptr || a.lse == nullptr || a.delta == nullptr)
     return fail(CTA_EINVAL, "the backward needs grad_out, lse and the delta scratch");
   if ((a.dk == nullptr) != (a.dv == nullptr)) return fail(CTA_EINVAL, "dk and dv come together");
+  if (args->delta_planes < 0) return fail(CTA_EINVAL, "delta_planes must not be negative");
+  if (args->dtype == CTA_F16 && args->delta_planes >= 3 && a.d <= 128) {
+    const int64_t plane = (a.cu != nullptr ? 1 : a.nseq) * static_cast<int64_t>(a.H) * a.L;
+    a.g_norm = a.delta + plane;
+    a.v_norm = a.g_norm + plane;
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_attn_delta(a, args->dtype, st);
   if (e == cudaSuccess && !launch_attn_tc_bwd(a, args->dtype, st, &e)) e = launch_attn_simt_bwd(a, args->dtype, st);

@@ -429,28 +429,46 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   store_rows<T, R, DC>(a.dv, a.dvs, t, hk, dv, one, a.d, ty, tx);
 }
 
-// delta_i = sum_d g_i o_i, o_i with what its rounding lost where that was kept.  GROUP lanes per (row, head), 16 bytes of each tensor per lane and step (VEC elements;
-// one element where rows do not start on 16 bytes): bound by HBM, two or three tensors read once; 8 x 1024 tokens, 32
-// heads of 128 in bf16, two tensors: 40 us, 3.4 TB/s.
+// delta_i = sum_d g_i o_i, o_i with what its rounding lost where that was kept.  GROUP lanes per (row, head), 16 bytes
+// of each tensor per lane and step (VEC elements; one element where rows do not start on 16 bytes): bound by HBM, two
+// or three tensors read once; 8 x 1024 tokens, 32 heads of 128 in bf16, two tensors: 40 us, 3.4 TB/s.
+// For fp16 gradients on tensor cores it also leaves |g_i| and, of the first groups one key each, |v_j|: 55 us there
+// with 8 key/value heads, 45 without the norms (groups of their own for the keys: 57); 16 x 512 tokens, 8 heads of 64: 11 and 7.
 template <typename T, int GROUP, int VEC>
-__global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t rows) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 6 : 5) attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t rows, int64_t keys) {
   const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / GROUP;
   const int lane = threadIdx.x % GROUP;
-  float s = 0.f;
-  int64_t at = 0;
+  const bool norms = std::is_same<T, __half>::value && a.g_norm != nullptr;
+  float s = 0.f, g2 = 0.f, v2 = 0.f;
+  int64_t at = 0, key_at = 0, key_b = 0, key_i = 0;
+  // token and head of the x-th row of a tensor with `heads`, and its place in [batch, heads, token]
+  auto place = [&](int64_t x, int heads, int64_t& b, int64_t& i, int& h) {
+    const int64_t r = x / heads;
+    h = static_cast<int>(x - r * heads);
+    b = a.cu != nullptr ? 0 : r / a.L;
+    i = r - b * a.L;
+    return (b * heads + h) * a.L + i;
+  };
   if (w < rows) {
-    const int64_t r = w / a.H;
-    const int h = static_cast<int>(w - r * a.H);
-    const int64_t b = a.cu != nullptr ? 0 : r / a.L, i = r - b * a.L;
-    at = (b * a.H + h) * a.L + i;
+    int64_t b, i;
+    int h, hk = 0;
+    at = place(w, a.H, b, i, h);
     const T* o = static_cast<const T*>(a.o) + b * a.os.b + i * a.os.t + h * a.os.h;
     const T* g = static_cast<const T*>(a.g) + b * a.gs.b + i * a.gs.t + h * a.gs.h;
     const T* low = a.low != nullptr ? static_cast<const T*>(a.low) + w * a.d : nullptr;
+    const T* v = nullptr;
+    if (norms && w < keys) {
+      key_at = place(w, a.Hk, key_b, key_i, hk);
+      v = static_cast<const T*>(a.v) + key_b * a.vs.b + key_i * a.vs.t + hk * a.vs.h;
+    }
     for (int c = lane * VEC; c < a.d; c += GROUP * VEC) {
       if constexpr (VEC == 1) {
         float x = Elem<T>::to_f(o[c]);
         if (low != nullptr) x = fmaf(Elem<T>::to_f(low[c]), 1.f / low_scale<T>(), x);
-        s = fmaf(x, Elem<T>::to_f(g[c]), s);
+        const float y = Elem<T>::to_f(g[c]), z = v != nullptr ? Elem<T>::to_f(v[c]) : 0.f;
+        s = fmaf(x, y, s);
+        g2 = fmaf(y, y, g2);
+        v2 = fmaf(z, z, v2);
       } else {
         float x[4], y[4], z[4];
 #pragma unroll
@@ -464,13 +482,36 @@ __global__ void attn_delta_kernel(const __grid_constant__ AttnArgs a, int64_t ro
           }
 #pragma unroll
           for (int w4 = 0; w4 < 4; ++w4) s = fmaf(x[w4], y[w4], s);
+          if (norms) {
+#pragma unroll
+            for (int w4 = 0; w4 < 4; ++w4) g2 = fmaf(y[w4], y[w4], g2);
+          }
+          if (v != nullptr) {
+            load_vec<T, 4>(v + c + e, z);
+#pragma unroll
+            for (int w4 = 0; w4 < 4; ++w4) v2 = fmaf(z[w4], z[w4], v2);
+          }
         }
       }
     }
   }
 #pragma unroll
-  for (int x = GROUP / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-  if (lane == 0 && w < rows) a.delta[at] = s;
+  for (int x = GROUP / 2; x > 0; x >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (norms) {
+      g2 += __shfl_xor_sync(0xffffffffu, g2, x);
+      v2 += __shfl_xor_sync(0xffffffffu, v2, x);
+    }
+  }
+  if (lane != 0 || w >= rows) return;
+  a.delta[at] = s;
+  if (!norms) return;
+  // what may hold anything does not count: masked keys, infinities and NaN
+  const float inf = __int_as_float(0x7f800000);
+  a.g_norm[at] = g2 < inf ? sqrtf(g2) : 0.f;
+  if (w >= keys) return;
+  const uint32_t* mask = a.mask != nullptr ? a.mask + key_b * a.mask_words : nullptr;
+  a.v_norm[key_at] = mask_key(mask, static_cast<int>(key_i)) && v2 < inf ? sqrtf(v2) : 0.f;
 }
 
 // key mask words: one CTA per batch entry
@@ -570,17 +611,18 @@ bool rows_on16(const void* p, const AttnStrides& s) {
 template <typename T>
 cudaError_t delta(const AttnArgs& a, cudaStream_t st) {
   constexpr int kVec = 16 / sizeof(T);
-  const int64_t rows = (a.cu != nullptr ? a.L : a.L * a.nseq) * a.H;
+  const int64_t tokens = a.cu != nullptr ? a.L : a.L * a.nseq;
+  const int64_t rows = tokens * a.H, keys = a.v_norm != nullptr ? tokens * a.Hk : 0;
   const bool vec = a.d % kVec == 0 && rows_on16<T>(a.o, a.os) && rows_on16<T>(a.g, a.gs) &&
-                   reinterpret_cast<uintptr_t>(a.low) % 16 == 0;
+                   reinterpret_cast<uintptr_t>(a.low) % 16 == 0 && (keys == 0 || rows_on16<T>(a.v, a.vs));
   const int group = vec && a.d <= 8 * kVec ? 8 : vec && a.d <= 16 * kVec ? 16 : 32;
   const int64_t ctas = (rows * group + 255) / 256;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const unsigned grid = static_cast<unsigned>(ctas);
-  if (!vec) attn_delta_kernel<T, 32, 1><<<grid, 256, 0, st>>>(a, rows);
-  else if (group == 8) attn_delta_kernel<T, 8, kVec><<<grid, 256, 0, st>>>(a, rows);
-  else if (group == 16) attn_delta_kernel<T, 16, kVec><<<grid, 256, 0, st>>>(a, rows);
-  else attn_delta_kernel<T, 32, kVec><<<grid, 256, 0, st>>>(a, rows);
+  if (!vec) attn_delta_kernel<T, 32, 1><<<grid, 256, 0, st>>>(a, rows, keys);
+  else if (group == 8) attn_delta_kernel<T, 8, kVec><<<grid, 256, 0, st>>>(a, rows, keys);
+  else if (group == 16) attn_delta_kernel<T, 16, kVec><<<grid, 256, 0, st>>>(a, rows, keys);
+  else attn_delta_kernel<T, 32, kVec><<<grid, 256, 0, st>>>(a, rows, keys);
   return cudaGetLastError();
 }
 }  // namespace

@@ -43,6 +43,28 @@ constexpr int kRows = 128;
 // rounding of scores and lse.
 constexpr float kHalfShift = 14.f, kHalfUnit = 0x1p-14f;
 
+// fp16 holds nothing below 2^-25, and dS of thousands of keys lies there as soon as the output's gradient is small,
+// while its sums dQ and dK do not.  So dS is multiplied by the power of two that takes its bound, |g| |v| + |delta|,
+// to 2^14..2^15 (dQ: row by row; dK, dV: for all rows that meet the CTA's keys), and the sums are multiplied back: what
+// is lost of a dS is below 2^-39 of that bound.  The attn_delta_kernel leaves the norms.
+__device__ __forceinline__ int unit_exponent(float bound) {
+  return max(-100, min(100, 14 + 127 - static_cast<int>(__float_as_uint(bound) >> 23)));
+}
+__device__ __forceinline__ float pow2(int n) { return __uint_as_float(static_cast<uint32_t>(127 + n) << 23); }
+__device__ __forceinline__ float finite(float x) { return fabsf(x) < __int_as_float(0x7f800000) ? fabsf(x) : 0.f; }
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+// maximum of |x| over [begin, end), by the weight warps; each thread gets its share's
+__device__ __forceinline__ float most_of(const float* x, int begin, int end) {
+  float m = 0.f;
+#pragma unroll 4
+  for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += 32 * kWeightWarps) m = fmaxf(m, finite(__ldg(x + i)));
+  return m;
+}
+
 struct BwdArgs {
   AttnArgs a;
   int pack, tile_tokens;
@@ -79,8 +101,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ BwdArgs f) {
   using L = Layout<DP>;
   constexpr int NS = L::kStages;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   __shared__ DqBars bars;
+  __shared__ float s_most[kHalf ? kWeightWarps : 1];
   __shared__ uint32_t s_tmem;
   __shared__ SeqTile s_tile;
   const AttnArgs& a = f.a;
@@ -227,6 +251,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int limit = a.causal ? tok : t.n - 1;
     const int limit_all = t.first + (warp & 3) * 32 / f.pack;  // causal: last key all rows of the warp see
     const bool any_blind = __any_sync(0xffffffffu, none);
+    // fp16: the row's power of two
+    int unit = 0;
+    if constexpr (kHalf) {
+      const float* v = a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0;
+      const float mine = warp_max(steps > 0 ? most_of(v, lo, end) : 0.f);
+      if (lane == 0) s_most[warp] = mine;
+      tc::sync_of(1, 32 * kWeightWarps);
+      const float most = warp_max(s_most[lane % kWeightWarps]);
+      unit = live ? unit_exponent(finite(a.g_norm[lse_index(a, t, h, tok)]) * most + finite(delta)) : 0;
+    }
+    const float up = pow2(unit), neg_delta = -delta * up;
+    auto less_delta = [&](float2 x) {
+      if constexpr (kHalf) return fma2(x, f2(up), f2(neg_delta));
+      else return add2(x, f2(-delta));
+    };
     bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
       const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + part * 32;
@@ -260,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 x = mul2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
-                              add2(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), f2(-delta)));
+                              less_delta(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]))));
         dp[e] = __float_as_uint(x.x);
         dp[e + 1] = __float_as_uint(x.y);
       }
@@ -287,7 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) atomicExch(&g_tc_bwd_error, kDevTimeout);
     } else if (t.first < t.n) {
       T* out = static_cast<T*>(a.dq) + t.batch * a.dqs.b + (t.row0 + tok) * a.dqs.t + h * a.dqs.h;
-      tc::store_rows<T, DP / 4>(t_dq + lanes + part * (DP / 4), out, part * (DP / 4), a.d, a.scale, live, f.wide_dq, steps > 0);
+      tc::store_rows<T, DP / 4>(t_dq + lanes + part * (DP / 4), out, part * (DP / 4), a.d, kHalf ? a.scale * pow2(-unit) : a.scale, live, f.wide_dq,
+                                    steps > 0);
     } else if (a.cu != nullptr && t.n == 0 && part == 0) {
       for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
         for (int x = threadIdx.x; x < a.d * f.pack; x += kRows)
@@ -319,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ DkvBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ SeqTile s_tile;
-  __shared__ __align__(16) float s_stat[NS][2][kRows];  // [stage][-lse2, -delta, fp16: + 14, * 2^-14][row]
+  __shared__ __align__(16) float s_stat[NS][2][kRows];  // [stage][-lse2, -delta, fp16: + 14, * its unit][row]
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -327,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // start once this one has been read; with one it goes over dO V^T, so that the next scores wait for dV only.
   constexpr bool kBeside = DP == 64;
   constexpr bool kHalf = std::is_same<T, __half>::value;
+  __shared__ float s_most[kHalf ? 3 : 1][kHalf ? kWeightWarps : 1];  // |g|, |delta|, |v|
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
   pdl_launch_dependents();  // dQ's CTAs may follow
 
@@ -379,6 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto head_of = [&](int s) { return hk * group + s / per_head * f.pack; };
   auto first_of = [&](int s) { return (i_lo + s % per_head) * f.tile_tokens; };
 
+  // fp16: the exponent of the CTA's power of two; the weight warps and the warp of the statistics
+  auto unit_of = [&] {
+    tc::sync_of(1, 32 * (kWeightWarps + 1));
+    const int w = kHalf ? lane % kWeightWarps : 0;
+    return unit_exponent(warp_max(s_most[0][w]) * warp_max(s_most[kHalf ? 2 : 0][w]) + warp_max(s_most[kHalf ? 1 : 0][w]));
+  };
+
   if (warp == kWeightWarps + 1) {
     bool ok = true;
     int issued = 0;
@@ -412,6 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kWeightWarps + 2) {
     bool ok = true;
+    float down = 1.f;
+    if constexpr (kHalf) down = pow2(unit_of() - static_cast<int>(kHalfShift));
     for (int s = 0; s < steps; ++s) {
       const int stage = s % NS;
       float nl[4], dl[4];
@@ -424,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (blind(nl[i])) dl[i] = 0.f;
         if constexpr (kHalf) {
           nl[i] += kHalfShift;
-          dl[i] *= kHalfUnit;
+          dl[i] *= down;
         }
       }
       if (s >= NS) ok = tc::wait(&bars.q_empty[stage], ((s / NS) - 1) & 1);
@@ -510,8 +560,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool valid = key < t.n && (mask == nullptr || mask_key(mask, key));
     const float c2 = a.scale * kLog2e;
-    auto less_delta = [](float2 dp, float2 neg_delta) {
-      if constexpr (kHalf) return fma2(dp, f2(kHalfUnit), neg_delta);
+    int unit = 0;
+    if constexpr (kHalf) {
+      float m[3] = {0.f, 0.f, 0.f};
+      if (steps > 0) {
+        const int from = a.causal ? max(t.first, lo) : 0;  // rows that see a key
+        for (int h = hk * group; h < (hk + 1) * group; ++h) {
+          m[0] = fmaxf(m[0], most_of(a.g_norm + lse_index(a, t, h, 0), from, t.n));
+          m[1] = fmaxf(m[1], most_of(a.delta + lse_index(a, t, h, 0), from, t.n));
+        }
+        m[2] = most_of(a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0, t.first, min(t.n, t.first + kRows));
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        m[i] = warp_max(m[i]);
+        if (lane == 0) s_most[i][warp] = m[i];
+      }
+      unit = unit_of();
+    }
+    const float up = pow2(unit - static_cast<int>(kHalfShift));
+    auto less_delta = [&](float2 dp, float2 neg_delta) {
+      if constexpr (kHalf) return fma2(dp, f2(up), neg_delta);
       else return add2(dp, neg_delta);
     };
     bool ok = true;
@@ -601,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::store_rows<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, kHalf ? kHalfUnit : 1.f, live, f.wide_dv, steps > 0);
       } else {
         T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
-        tc::store_rows<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, a.scale, live, f.wide_dk, steps > 0);
+        tc::store_rows<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, kHalf ? a.scale * pow2(-unit) : a.scale, live, f.wide_dk, steps > 0);
       }
     } else if (a.cu != nullptr && t.n == 0 && part < 2) {
       T* base = static_cast<T*>(part == 0 ? a.dv : a.dk) + hk * (part == 0 ? a.dvs.h : a.dks.h);
@@ -643,7 +712,7 @@ cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k
 }  // namespace
 
 bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e) {
-  if (dtype == kF32 || a.d % 8 != 0 || a.d > 128 || !(a.scale > 0.f)) return false;
+  if (dtype == kF32 || a.d % 8 != 0 || a.d > 128 || !(a.scale > 0.f) || (dtype == kF16 && a.g_norm == nullptr)) return false;
   BwdArgs f = {};
   f.a = a;
   f.pack = attn_pack(a.H / a.Hk);

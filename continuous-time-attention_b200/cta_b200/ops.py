@@ -751,12 +751,14 @@ def _attention_backward(grad_out, q, k, v, out, low, lse, cu, mask_words, causal
     dq = _new(q) if need_dq else None
     dk = _new(k) if need_dkv else None
     dv = _new(v) if need_dkv else None
-    delta = torch.empty_like(lse)
+    # fp16 on tensor cores: beside delta the norms that scale its score gradients
+    planes = 3 if code == 2 else 1
+    delta = torch.empty_like(lse) if planes == 1 else torch.empty((planes, *lse.shape), dtype=lse.dtype, device=lse.device)
     args = _lib.ATTENTION_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low, lse.data_ptr(), g.data_ptr(), delta.data_ptr(),
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(cu), _lib.ptr(mask_words), *_strides3(q), *_strides3(k),
         *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), *sizes, code,
-        bool(causal), 0, 0, scale, 0.0)
+        bool(causal), 0, planes, scale, 0.0)
     _lib.enqueue(_lib.load().cta_attention_backward, q, args)
     return dq, dk, dv
 

@@ -320,7 +320,7 @@ typedef struct cta_attention_args {
                                * NULL; without it short rows' gradients lose up to a bit and a half */
   float* lse;                 /* forward: written unless NULL.  backward: read */
   const void* grad_out;       /* backward only, like the rest of the pointers */
-  float* delta;               /* scratch, laid out as lse */
+  float* delta;               /* scratch, laid out as lse, delta_planes times one after the other */
   void* dq;                   /* NULL: not wanted */
   void* dk;                   /* NULL with dv: not wanted */
   void* dv;
@@ -329,7 +329,9 @@ typedef struct cta_attention_args {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
   int64_t grad_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   int64_t batch, length, heads, kv_heads, dim;
-  int32_t dtype, causal, zero_tail, reserved;
+  int32_t dtype, causal, zero_tail;
+  int32_t delta_planes;       /* backward: 0 or 1: one.  3 in fp16 lets the tensor cores do it; with one the FP32
+                               * pipe does, which takes many times as long */
   float scale, reserved2;
 } cta_attention_args;
 

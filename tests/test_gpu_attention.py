@@ -557,3 +557,85 @@ def test_small_weights_beside_a_large_one(dim, dtype):
     eps = torch.finfo(dtype).eps
     _within(out, want, want * (eps + 2.0**-20 + 50 * 2.0**-24 + (n / 64 + 80) * 2.0**-24), "out")
 
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", [1.0, 2.0**-13, 2.0**-17, 2.0**8])
+def test_fp16_gradients_of_any_size(size, causal, dim):
+    """P (dP - delta) over thousands of keys lies far below fp16's smallest step when the output's gradient is small;
+    the sums over it do not.  Only what the gradients' own type cannot hold may be lost: the bounds here allow
+    no step of fp16 per key, but 2^-39 of the largest weight for P and of 2 |g| |v| for dS."""
+    n = 4200
+    q, k, v, g = _inputs((1, n), 2, 1, dim, torch.float16, seed=dim)
+    q, g = (q * 0.5).half(), (g * size).half()
+    got = _run(q, k, v, g, causal=causal)
+    see = _see(n, causal)
+    q, k, v, g = (x[0] for x in (q, k, v, g))
+    most = 2 * g.double().norm(dim=-1).max() * v.double().norm(dim=-1).max()
+    tol = A.bounds(q, k, v, see, dim**-0.5, torch.float16, g, weight_step=2.0**-31, grad_steps=(2.0**-39, 2.0**-39 * most))
+    for x, y, t, name in zip(got[1:], A.gradients(q, k, v, g, see, dim**-0.5), tol[1:], ("dq", "dk", "dv")):
+        _within(x[0], y, t, name)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp16_gradients_of_other_sequences_and_rows(dim):
+    """Sizes that differ by 2^20 between sequences, padded and packed, and between the heads of a batch: each keeps its
+    own precision.  Values of masked keys and of rows behind the last sequence count for nothing."""
+    n = 700
+    sizes = [2.0**-14, 1.0, 2.0**6]
+    q, k, v, g = _inputs((3, n), 4, 2, dim, torch.float16, seed=dim)
+    g = (g * torch.tensor(sizes, device="cuda")[:, None, None, None]).half()
+    v[1, :, 1] *= 2.0**8
+    valid = torch.ones(3, n, dtype=torch.bool, device="cuda")
+    valid[:, 600:] = False
+    v[:, 600:], k[:, 600:] = 60000.0, float("nan")
+
+    def check(got, what, part):
+        for b in range(3):
+            m = 600 if part else n
+            x = [t[b][:m] for t in (q, k, v, g)]
+            see = _see(m, True)
+            most = 2 * x[3].double().norm(dim=-1).max() * x[2].double().norm(dim=-1).amax(0)
+            per_head = most.repeat_interleave(2)[:, None, None]
+            tol = A.bounds(*x[:3], see, dim**-0.5, torch.float16, x[3], weight_step=2.0**-31,
+                           grad_steps=(2.0**-39, 2.0**-39 * per_head))
+            for y, w, t, name in zip(got[1:], A.gradients(*x, see, dim**-0.5), tol[1:], ("dq", "dk", "dv")):
+                _within(y[b][:m], w, t, f"{what}, {b}: {name}")
+
+    g[:, 600:] = 0
+    check(_run(q, k, v, g, causal=True, key_mask=valid), "padded", True)
+    packed = [torch.cat([x[:, :600].flatten(0, 1), torch.full_like(x[0, :9], 60000.0)]) for x in (q, k, v, g)]
+    cu = torch.tensor([0, 600, 1200, 1800], dtype=torch.int32, device="cuda")
+    got = _run(*packed, causal=True, cu_seqlens=cu)
+    check([x[:1800].unflatten(0, (3, 600)) for x in got], "packed", True)
+    assert all((x[1800:] == 0).all() for x in got)
+
+
+def test_fp16_backward_with_one_plane_of_scratch():
+    """Through the C interface with room for delta alone: the plain kernels, within the same bounds."""
+    from cta_b200 import _lib, ops
+
+    n, d = 300, 64
+    q, k, v, g = _inputs((1, n), 4, 2, d, torch.float16)
+    out, lse = ops.attention_forward(q, k, v, causal=True)
+    grads = [torch.empty_like(x) for x in (q, k, v)]
+    delta = torch.full((2, *lse.shape), 7.0, device="cuda")
+
+    def strides(t):
+        return t.stride()[:3]
+
+    for planes in (0, 1, 2):
+        args = _lib.ATTENTION_ARGS.pack(
+            *(t.data_ptr() for t in (q, k, v, out)), 0, lse.data_ptr(), g.data_ptr(), delta.data_ptr(),
+            *(t.data_ptr() for t in grads), 0, 0, *strides(q), *strides(k), *strides(v), *strides(out), *strides(g),
+            *(x for t in grads for x in strides(t)), 1, n, 4, 2, d, 2, 1, 0, planes, d**-0.5, 0.0)
+        _lib.enqueue(_lib.load().cta_attention_backward, q, args)
+        assert (delta[1] == 7).all()
+        see = _see(n, True)
+        tol = A.bounds(q[0], k[0], v[0], see, d**-0.5, q.dtype, g[0])
+        for x, y, t, name in zip(grads, A.gradients(q[0], k[0], v[0], g[0], see, d**-0.5), tol[1:], ("dq", "dk", "dv")):
+            _within(x[0], y, t, name)
+    bad = bytearray(args)
+    bad[-12:-8] = (-1).to_bytes(4, "little", signed=True)
+    assert _lib.load().cta_attention_backward(bytes(bad), None) == _lib.CTA_EINVAL
