@@ -61,6 +61,13 @@ def _refine(x: torch.Tensor, pde_list: nn.ModuleList, layout: str, attention_mas
     return diffusion_pde_stack(x, pde_list, attention_mask=attention_mask)
 
 
+def _key_words(attention_mask: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """The mask as the fused attention takes it; its words alone do not tell a length from the next."""
+    if attention_mask.shape != x.shape[:2]:
+        raise ValueError(f"attention_mask must be {tuple(x.shape[:2])}, got {tuple(attention_mask.shape)}")
+    return ops.attention_mask(attention_mask)
+
+
 class _FusedSelfAttention(nn.MultiheadAttention):
     """The layers' attention module (same parameters and names), running fused."""
 
@@ -149,7 +156,7 @@ class PDETransformerClassifier(nn.Module):
         x = self.dropout(x)
         fused = self.attention == "fused"
         if fused:
-            words = ops.attention_mask(attention_mask)
+            words = _key_words(attention_mask, x)
         else:
             padding_mask = attention_mask == 0
         n = len(self.transformer_layers)
@@ -216,7 +223,7 @@ class PDETransformerLM(nn.Module):
         x = self.dropout(x)
         fused = self.attention == "fused"
         if fused:
-            words = ops.attention_mask(attention_mask)
+            words = _key_words(attention_mask, x)
         else:
             padding_mask = torch.zeros_like(attention_mask, dtype=torch.float32)
             padding_mask = padding_mask.masked_fill(attention_mask == 0, float("-inf"))

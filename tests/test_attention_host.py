@@ -301,3 +301,12 @@ def test_fused_models_are_saved_and_copied_whole(plain, tmp_path):
         back = torch.load(tmp_path / f"{i}.pt", weights_only=False)
         assert torch.equal(back(ids, mask), want)
     assert torch.equal(copy.deepcopy(net)(ids, mask), want)
+
+
+def test_fused_models_refuse_a_mask_of_another_length(plain):
+    for cls, kw in ((plain.PDETransformerLM, {}), (plain.PDETransformerClassifier, dict(num_classes=3))):
+        net = cls(attention="fused", **KW, **kw)
+        ids = torch.randint(0, 11, (2, 9))
+        for shape in ((2, 8), (2, 10), (1, 9), (2, 9, 1)):
+            with pytest.raises(ValueError, match="attention_mask"):
+                net(ids, torch.ones(*shape, dtype=torch.long))
