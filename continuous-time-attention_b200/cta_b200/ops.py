@@ -835,8 +835,8 @@ def kv_cache_write(
     cache [pages, page_size, kv_heads, dim], in place; one launch.
 
     The cache holds the rows' type, or float8_e4m3fn codes with fp32 scales
-    [pages, kv_heads, page_size]: scale = m / 448 and code = e4m3(x * (448 / m))
-    with m = max(max|x|, 2**-100) over the row.  Slot s is entry s % page_size of
+    [pages, kv_heads, page_size]: scale = m / 448 and code = e4m3(448 x / m), the
+    nearest to the exact quotient, with m = max(max|x|, 2**-100) over the row.  Slot s is entry s % page_size of
     page s // page_size.  A negative slot is skipped (padding rows); the others
     must be distinct.  A slot past the cache is skipped and reported by
     ``_lib.device_error()``."""

@@ -353,7 +353,8 @@ int cta_attention_mask_words(const void* mask, int mask_dtype, int64_t mask_sB, 
  * {page, slot, head} (dim contiguous, rows on 16 bytes), in the rows' 16-bit
  * type, or (quantized) e4m3 codes with fp32 scales k_scale, v_scale
  * [pages, kv_heads, page_size] contiguous:
- *   scale = m / 448,  code = e4m3(x * (448 / m)),  m = max(max |x|, 2^-100)
+ *   scale = m / 448,  code = e4m3(448 x / m),  m = max(max |x|, 2^-100)
+ * (each code the nearest to the exact quotient, ties to even)
  * over the dim axis.  Slot s is entry s % page_size of page s / page_size.
  *
  * write: row t of k and v ([tokens, kv_heads, dim], strides {token, head}) goes

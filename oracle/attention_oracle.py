@@ -115,7 +115,7 @@ def quantise(x):
     """(codes as the values they stand for, scales) of an e4m3 cache row: 64 bits, ties to even."""
     x = x.detach().double()
     m = x.abs().amax(-1).clamp_min(2.0**-100)
-    y = x * (448.0 / m)[..., None]
+    y = x * 448.0 / m[..., None]  # a tie stays one: the product is exact
     size = y.abs().clamp_min(2.0**-6)
     e = torch.frexp(size).exponent - 1
     step = torch.ldexp(torch.ones_like(size), e - 3)

@@ -599,3 +599,38 @@ def test_e4m3_large_values_of_little_weight(rows, dtype):
         s.v[b][j] = _codes(s.vc, slots) * s.vs[at].double()[..., None]
     assert s.v[0].abs().max() > torch.finfo(torch.float16).max
     _check_scaled(s, s.run())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_codes_are_the_nearest(dtype):
+    """Every element's code is the e4m3 number nearest to x * 448 / m, ties to the even one.  In 64 bits x * 448 is exact
+    and the quotient exact to 2^-53, while a quotient that is no tie lies 2^-17 or further from one: x * 448 and
+    the tie times m are whole numbers of at most 17 bits."""
+    from cta_b200 import ops
+
+    bits = 7 if dtype == torch.bfloat16 else 10
+    # all fractions of x against the fractions of m: those with ties (m = 7 i) and others
+    fractions = torch.arange(2**bits, 2 ** (bits + 1), dtype=torch.float64)
+    mine = fractions if bits == 7 else torch.cat([fractions[fractions % 7 == 0][::4], fractions[::31]])
+    binades = 17 if bits == 7 else 14
+    x = (fractions[None, :] * 2.0 ** -torch.arange(binades, dtype=torch.float64)[:, None]).flatten()
+    per = 255
+    x = torch.cat([x, x[: -len(x) % per]]).view(-1, per)
+    x[:, ::2] *= -1
+    for scale in ((2.0**-106, 2.0**-7, 1.0, 2.0**120) if bits == 7 else (2.0**-10, 2.0**5)):
+        rows = []
+        for m in mine:
+            keep = torch.where(x.abs() > m, x / 2, x)
+            rows.append(torch.cat([torch.full((len(x), 1), m.item(), dtype=torch.float64), keep], 1))
+        wide = torch.cat(rows) * scale
+        k = wide.to(dtype)
+        wide = k.double()  # fp16's subnormal numbers are rounded here
+        n = len(k)
+        k = k.cuda()[:, None]
+        kc, vc, ks, vs = _cache(-(-n // 16), 16, 1, 256, dtype, True)
+        slots = torch.arange(n, device="cuda")
+        ops.kv_cache_write(k, -k, kc, vc, slots, k_scale=ks, v_scale=vs)
+        codes, scales = A.quantise(k)
+        assert torch.equal(_codes(kc, slots), codes)
+        assert torch.equal(_codes(vc, slots), -codes)
+        assert torch.equal(ks[slots // 16, :, slots % 16], scales.float())
