@@ -245,8 +245,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const bool live = tok < t.n;
     const float c2 = a.scale * kLog2e;
-    const float nl = live ? neg_lse2_of(a.lse[lse_index(a, t, h, tok)]) : neg_inf();
-    const float delta = live ? a.delta[lse_index(a, t, h, tok)] : 0.f;
+    // all of these loads are on their way before the first is used
+    const int64_t at = live ? lse_index(a, t, h, tok) : 0;
+    const float lse = live ? a.lse[at] : neg_inf(), delta = live ? a.delta[at] : 0.f;
+    float norm = 0.f, most = 0.f;
+    if constexpr (kHalf) {
+      norm = live ? a.g_norm[at] : 0.f;
+      if (steps > 0) most = most_of(a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0, lo, end);
+    }
+    const float nl = neg_lse2_of(lse);
     const bool none = blind(nl);
     const int limit = a.causal ? tok : t.n - 1;
     const int limit_all = t.first + (warp & 3) * 32 / f.pack;  // causal: last key all rows of the warp see
@@ -254,12 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // fp16: the row's power of two
     int unit = 0;
     if constexpr (kHalf) {
-      const float* v = a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0;
-      const float mine = warp_max(steps > 0 ? most_of(v, lo, end) : 0.f);
-      if (lane == 0) s_most[warp] = mine;
+      most = warp_max(most);
+      if (lane == 0) s_most[warp] = most;
+      __syncwarp();
       tc::sync_of(1, 32 * kWeightWarps);
-      const float most = warp_max(s_most[lane % kWeightWarps]);
-      unit = live ? unit_exponent(finite(a.g_norm[lse_index(a, t, h, tok)]) * most + finite(delta)) : 0;
+      most = warp_max(s_most[lane % kWeightWarps]);  // by the whole warp, its rows behind the sequence too
+      unit = live ? unit_exponent(finite(norm) * most + finite(delta)) : 0;
     }
     const float up = pow2(unit), neg_delta = -delta * up;
     auto less_delta = [&](float2 x) {
@@ -565,9 +572,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m[3] = {0.f, 0.f, 0.f};
       if (steps > 0) {
         const int from = a.causal ? max(t.first, lo) : 0;  // rows that see a key
-        for (int h = hk * group; h < (hk + 1) * group; ++h) {
-          m[0] = fmaxf(m[0], most_of(a.g_norm + lse_index(a, t, h, 0), from, t.n));
-          m[1] = fmaxf(m[1], most_of(a.delta + lse_index(a, t, h, 0), from, t.n));
+        // four heads at a time: one after the other, their loads wait for one another (delta, dK and dV of 8 x 1024 tokens,
+        // 32/8 heads of 128: 237 us instead of 225)
+        for (int h = 0; h < group; h += 4) {
+          const int64_t at = lse_index(a, t, hk * group + h, 0);
+          for (int i = from + static_cast<int>(threadIdx.x); i < t.n; i += 32 * kWeightWarps) {
+            float g[4], d[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              g[x] = h + x < group ? __ldg(a.g_norm + at + x * a.L + i) : 0.f;
+              d[x] = h + x < group ? __ldg(a.delta + at + x * a.L + i) : 0.f;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              m[0] = fmaxf(m[0], finite(g[x]));
+              m[1] = fmaxf(m[1], finite(d[x]));
+            }
+          }
         }
         m[2] = most_of(a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0, t.first, min(t.n, t.first + kRows));
       }
@@ -576,6 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         m[i] = warp_max(m[i]);
         if (lane == 0) s_most[i][warp] = m[i];
       }
+      __syncwarp();
       unit = unit_of();
     }
     const float up = pow2(unit - static_cast<int>(kHalfShift));

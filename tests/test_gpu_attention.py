@@ -639,3 +639,44 @@ def test_fp16_backward_with_one_plane_of_scratch():
     bad = bytearray(args)
     bad[-12:-8] = (-1).to_bytes(4, "little", signed=True)
     assert _lib.load().cta_attention_backward(bytes(bad), None) == _lib.CTA_EINVAL
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp16_captured_and_on_two_streams(dim):
+    """fp16's backward, whose scratch holds the norms too: captured and replayed on new inputs, and beside another call
+    of other sizes, bit for bit."""
+    from cta_b200.attention import prompt_attention
+
+    first, second = _inputs((2, 300), 4, 2, dim, torch.float16), _inputs((2, 300), 4, 2, dim, torch.float16, seed=5)
+    second[3].mul_(2.0**-12)
+    want = [_run(*x, causal=True) for x in (first, second)]
+    held = [x.clone() for x in first]
+    leaves = [x.requires_grad_(True) for x in held[:3]]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(prompt_attention(*leaves, causal=True), leaves, held[3])
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = prompt_attention(*leaves, causal=True)
+        grads = torch.autograd.grad(out, leaves, held[3])
+    for inputs, expected in zip((second, first), reversed(want)):
+        with torch.no_grad():
+            for x, y in zip((*leaves, held[3]), inputs):
+                x.copy_(y)
+        graph.replay()
+        for x, y in zip((out, *grads), expected):
+            assert torch.equal(x, y)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, (inputs, st) in enumerate(zip((first, second), streams)):
+            with torch.cuda.stream(st):
+                got[i].append(_run(*inputs, causal=True))
+    torch.cuda.synchronize()
+    for expected, all_of in zip(want, got):
+        for x in all_of:
+            for a, b in zip(x, expected):
+                assert torch.equal(a, b)

@@ -634,3 +634,27 @@ def test_codes_are_the_nearest(dtype):
         assert torch.equal(_codes(kc, slots), codes)
         assert torch.equal(_codes(vc, slots), -codes)
         assert torch.equal(ks[slots // 16, :, slots % 16], scales.float())
+
+
+def test_fp16_chunks_over_e4m3_captured_together():
+    """Chunks whose expansion lies in a workspace of their own: two graphs replayed at the same time, bit for bit."""
+    sets = [Setup(lens, [40, 200, 7], 32, 8, 128, 16, torch.float16, True, seed=i)
+            for i, lens in enumerate(([1500, 300, 2200], [900, 2000, 800]))]
+    _rescaled(sets[1], vs=2.0**6)
+    want = [s.run() for s in sets]
+    assert all(torch.equal(s.run(), x) for s, x in zip(sets, want))
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(s.run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(outs, want):
+        assert torch.equal(x, y)
