@@ -28,9 +28,10 @@
 // * The next group's keys load while this group's softmax runs, the next
 //   values while the next scores run.
 //
-// Measured, 32/8 heads of 128, 64 sequences of 512 to 8192 keys: 16-bit 176 us, 6.4
-// TB/s, 98 % of what a copy reaches; e4m3 134 us, 4.3 TB/s, bound by issue (a code
-// is converted before it is multiplied).  One sequence of 777 keys: 11 us, the
+// Measured, 32/8 heads of 128, 64 sequences of 512 to 8192 keys: 16-bit 178 us, 6.2
+// TB/s, 95 % of what a copy reaches; e4m3 135 us, 4.2 TB/s (a code is converted before
+// it is multiplied, and 15 warps an SM do not hide that behind the loads: HBM is busy
+// half the time, and instructions issue in 41 % of the cycles).  One sequence of 777 keys: 11 us, the
 // latency of two launches and of a chain of loads.
 //
 // e4m3: the codes are exact in fp16, so both products run in fp16 whatever the

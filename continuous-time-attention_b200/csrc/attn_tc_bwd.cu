@@ -22,9 +22,10 @@
 //
 // Bound by the products at dim 128 (7 x 512 cycles per tile pair against 2 x
 // 1024 of exponentials), by the exponentials at dim 64.  Measured, 8192 tokens, 16
-// heads, not causal: dim 128 dQ 640 us, dK and dV 960, 1230 TFLOP/s of the seven
-// products; dim 64 464 and 600, 900.  Both in one call take 1566 and 1090: dQ's CTAs
-// start while the last ones of dK and dV run.
+// heads, not causal, bf16: dim 128 dQ 658 us, dK and dV 990, 1170 TFLOP/s of the seven
+// products; dim 64 406 and 537, 1020.  Both in one call, delta included, take 1655 and
+// 941: dQ's CTAs start while the last ones of dK and dV run.  fp16, with its bounds,
+// 1678 and 976.
 #include <algorithm>
 
 #include "attn_tc.cuh"

@@ -37,9 +37,10 @@
 //
 // Bound by the exponentials and the products alike: 128 x 128 exponentials take
 // 1024 cycles of the SM's 16-per-cycle unit, the two products of a tile 1024
-// cycles at dim 128 (512 at dim 64).  Measured, 8192 tokens: 16 heads of 128 510 us,
-// 1080 TFLOP/s; 32/8 heads of 128, causal, 445 us, 1235; 16 heads of 64 400 us, 687.
-// 4 chunks of 512 rows over 1500 to 8192 cached keys, 32/8 heads of 128: 197 us.
+// cycles at dim 128 (512 at dim 64).  Measured, 8192 tokens: 16 heads of 128 514 us,
+// 1070 TFLOP/s; 32/8 heads of 128, causal, 457 us, 1203; 16 heads of 64 426 us, 645
+// (runs on other boards: 503 to 510, 445, 400).
+// 4 chunks of 512 rows over 1500 to 8192 cached keys, 32/8 heads of 128: 162 us.
 #include <algorithm>
 
 #include "attn_tc.cuh"
