@@ -65,13 +65,14 @@ def prompt_attention(
     Padded: q [B, L, heads, dim], k and v [B, L, kv_heads, dim]; ``key_mask``
     [B, L] (any mask dtype, non-zero = valid) hides padding, or ``mask_words``,
     its form from ``ops.attention_mask``, made once for several layers.  Packed:
-    [T, heads, dim] with ``cu_seqlens`` (device int32, sequences + 1 offsets).  ``causal``:
+    [T, heads, dim] with ``cu_seqlens`` (device int32, sequences + 1 offsets from 0, not decreasing).  ``causal``:
     row i sees keys j <= i of its sequence.  ``scale`` defaults to dim**-0.5.
 
     A row that sees no key is zero and has no gradient, as are packed rows
-    behind the last sequence.  Masked keys may hold anything, infinities and NaN
-    included; a NaN or infinity in the k or v of a valid token may also reach
-    earlier rows of its sequence.  Forward-mode differentiation raises."""
+    behind the last sequence.  Masked keys and such rows may hold anything,
+    infinities and NaN included; a NaN or infinity in the k or v of a valid token may
+    also reach earlier rows of its sequence, one in the q or the output gradient of
+    a row the gradients of later keys.  Forward-mode differentiation raises."""
     words = mask_words
     if key_mask is not None:
         if words is not None:

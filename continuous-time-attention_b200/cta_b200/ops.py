@@ -905,7 +905,8 @@ def paged_attention(
     workspace of up to 2 GiB.  max_rows, the longest n_r as the host knows it, only chooses
     the kernel.  No device data is read on the host.
     Rows that see no key are zero; rows behind the last sequence are not
-    written.  A page outside the cache or a length past the table counts as no
+    written.  A NaN or infinity in the v of a cached token may also reach earlier
+    rows of this call.  A page outside the cache or a length past the table counts as no
     keys and is reported by ``_lib.device_error()``."""
     return _paged_launch(*_paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale,
                                       v_scale, out))
