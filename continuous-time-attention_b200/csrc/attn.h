@@ -41,6 +41,7 @@ struct AttnArgs {
   int zero_tail;  // packed: rows behind the last sequence are set to zero (else left as they are)
   float scale;
   int tiles;  // tiles of the launch per (packed) row or per sequence (dense)
+  int window, sinks;  // see Reach; window 0 = every key up to the row's own
 };
 
 // Key mask words of one batch entry: {first valid key, one past the last valid
@@ -79,6 +80,19 @@ struct CacheArgs {
 cudaError_t launch_cache_write(const CacheArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_cache_read(const CacheArgs& a, int dtype, cudaStream_t st);
 
+// New rows rotated by their positions: q [T, H, d] into q_out, k into the cache with v.
+struct RotaryArgs {
+  CacheArgs cache;
+  const void* q;
+  void* q_out;
+  int64_t q_sT, q_sH, o_sT, o_sH;
+  const int64_t* positions;
+  const void* table;  // [positions_end, 2 * pairs]: cosines, then sines
+  int64_t table_sP, positions_end;
+  int H, pairs, interleaved;
+};
+cudaError_t launch_rotary_write(const RotaryArgs& r, int dtype, bool table16, cudaStream_t st);
+
 struct PagedArgs {
   const void* q;  // [T, H, d]
   void* o;
@@ -97,6 +111,8 @@ struct PagedArgs {
   int page, table_width, n_pages;
   int max_rows;  // longest chunk (host)
   float scale;
+  int window, sinks;  // see Reach; window 0 = every key up to the row's own
+  int skip;           // split kernel: keys from here on, a multiple of 16
   // split over the keys: one worker per warp
   int workers;
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32

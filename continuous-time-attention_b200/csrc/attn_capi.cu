@@ -181,6 +181,25 @@ int cache_args(const cta_kv_cache_args* p, bool write, CacheArgs& a) {
   return CTA_OK;
 }
 
+// A sliding window and the first keys that stay visible, as the kernels take them.  A window that reaches over all of
+// `length` keys, whatever the sinks, is none.
+int window_args(int64_t window, int64_t sinks, int64_t length, int& w, int& s) {
+  if (window < 0 || sinks < 0) return fail(CTA_EINVAL, "window and sinks must not be negative");
+  if (window == 0 && sinks != 0) return fail(CTA_EINVAL, "sinks go with a window");
+  w = s = 0;
+  if (window == 0 || window >= length || sinks >= length - window) return CTA_OK;
+  w = static_cast<int>(window);  // both below `length`
+  s = static_cast<int>(sinks);
+  return CTA_OK;
+}
+int prompt_window(const cta_attention_args* p, int64_t window, int64_t sinks, AttnArgs& a) {
+  if (p != nullptr && window > 0 && !p->causal) return fail(CTA_EINVAL, "a window needs the causal mask");
+  const int rc = prompt_args(p, a);
+  if (rc != CTA_OK && rc != kNothing) return rc;
+  const int wrc = window_args(window, sinks, p->length, a.window, a.sinks);
+  return wrc != CTA_OK ? wrc : rc;
+}
+
 int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
   if (p == nullptr) return fail(CTA_EINVAL, "null arguments");
   if (p->dtype != CTA_BF16 && p->dtype != CTA_F16)
@@ -241,6 +260,17 @@ int paged_args(const cta_paged_attention_args* p, PagedArgs& a) {
   return CTA_OK;
 }
 
+int paged_window(const cta_paged_attention_args* p, int64_t window, int64_t sinks, PagedArgs& a) {
+  const int rc = paged_args(p, a);
+  if (rc != CTA_OK) return rc;
+  const int64_t keys = p->table_width * p->page_size;
+  const int wrc = window_args(window, sinks, keys, a.window, a.sinks);
+  if (wrc != CTA_OK) return wrc;
+  if (a.window > 0 && keys >= (1LL << 30))  // the split kernel counts groups past the last key
+    return fail(CTA_EUNSUPPORTED, "table_width * page_size must be below 2^30 with a window");
+  return CTA_OK;
+}
+
 // The tensor-core kernel takes 128 (row, head) pairs at once but has a CTA per pair of such tiles only;
 // the split kernel takes 16, reads the keys again for each 16, and fills the GPU whatever the shape.
 // Measured (32/8 heads of 128, B200): a 16-row tile costs the split kernel 0.11 ns per key, a pass of
@@ -265,7 +295,7 @@ bool tma_can_address(const PagedArgs& a) {
                                        axis(a.n_pages, a.vc_sP), axis(a.page, a.vc_sS), axis(a.Hk, a.vc_sH)});
 }
 bool tensor_cores_pay(const PagedArgs& a) {
-  if (!tma_can_address(a)) return false;
+  if (a.window > 0 || !tma_can_address(a)) return false;
   const int64_t group = a.H / a.Hk, pack = attn_pack(static_cast<int>(group));
   if (a.cu == nullptr || a.max_rows * group <= 16 || !(a.scale > 0.f)) return false;
   const int64_t b = a.B;
@@ -306,18 +336,34 @@ int cta_attention_mask_words(const void* mask, int mask_dtype, int64_t mask_sB, 
 }
 
 int cta_attention_forward(const cta_attention_args* args, void* stream) {
+  return cta_window_attention_forward(args, 0, 0, stream);
+}
+
+int cta_window_attention_forward(const cta_attention_args* args, int64_t window, int64_t sinks, void* stream) {
   AttnArgs a;
-  const int rc = prompt_args(args, a);
+  const int rc = prompt_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (!launch_attn_tc_fwd(a, args->dtype, st, &e)) e = launch_attn_simt_fwd(a, args->dtype, st);
+  if (a.window > 0 || !launch_attn_tc_fwd(a, args->dtype, st, &e)) e = launch_attn_simt_fwd(a, args->dtype, st);
   return launched(e, "attention forward launch");
 }
 
 int cta_attention_backward(const cta_attention_args* args, void* stream) {
+  return cta_window_attention_backward(args, 0, 0, nullptr, 0, stream);
+}
+
+int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int64_t window, int64_t sinks) {
   AttnArgs a;
-  const int rc = prompt_args(args, a);
+  const int rc = prompt_window(args, window, sinks, a);
+  if (rc != CTA_OK) return rc == kNothing ? 0 : -rc;
+  return 0;
+}
+
+int cta_window_attention_backward(const cta_attention_args* args, int64_t window, int64_t sinks, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  AttnArgs a;
+  const int rc = prompt_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
   if (a.g == nullptr || a.lse == nullptr || a.delta == nullptr)
     return fail(CTA_EINVAL, "the backward needs grad_out, lse and the delta scratch");
@@ -330,7 +376,7 @@ int cta_attention_backward(const cta_attention_args* args, void* stream) {
   }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_attn_delta(a, args->dtype, st);
-  if (e == cudaSuccess && !launch_attn_tc_bwd(a, args->dtype, st, &e)) e = launch_attn_simt_bwd(a, args->dtype, st);
+  if (e == cudaSuccess && (a.window > 0 || !launch_attn_tc_bwd(a, args->dtype, st, &e))) e = launch_attn_simt_bwd(a, args->dtype, st);
   return launched(e, "attention backward launch");
 }
 
@@ -348,9 +394,59 @@ int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream) {
   return launched(launch_cache_read(a, args->dtype, static_cast<cudaStream_t>(stream)), "cache read launch");
 }
 
+int cta_rotary_cache_write(const cta_kv_cache_args* args, const cta_rotary_args* rotary, void* stream) {
+  RotaryArgs r;
+  std::memset(&r, 0, sizeof(r));
+  const int rc = cache_args(args, true, r.cache);
+  if (rc != CTA_OK && rc != kNothing) return rc;
+  const cta_rotary_args* p = rotary;
+  if (p == nullptr) return fail(CTA_EINVAL, "null arguments");
+  if (p->heads < 1 || p->heads >= (1LL << 20)) return fail(CTA_EINVAL, "heads must be in 1..2^20 - 1");
+  if (p->rotary_dim < 16 || p->rotary_dim % 16 != 0 || p->rotary_dim > args->dim)
+    return fail(CTA_EINVAL, "rotary_dim must be a multiple of 16 in 16..%lld, got %lld", (long long)args->dim,
+                (long long)p->rotary_dim);
+  if (p->table_dtype != CTA_F32 && p->table_dtype != args->dtype)
+    return fail(CTA_EINVAL, "the table is fp32 or of the rows' type, got dtype code %d", p->table_dtype);
+  if (p->positions_end < 0) return fail(CTA_EINVAL, "bad table shape");
+  const int64_t blocks = (p->heads + 3) / 4 + 2 * ((args->kv_heads + 3) / 4);
+  if (args->tokens * blocks >= (1LL << 27))
+    return fail(CTA_EUNSUPPORTED, "tokens * ceil(heads / 4), of q, k and v, must be below 2^27");
+  if (rc == kNothing) return CTA_OK;
+  if (p->q == nullptr || p->q_out == nullptr || p->positions == nullptr || (p->table == nullptr && p->positions_end > 0))
+    return fail(CTA_EINVAL, "null tensor pointer");
+  for (int64_t s : {p->q_stride[0], p->q_stride[1], p->q_out_stride[0], p->q_out_stride[1]})
+    if (s % 8 != 0) return fail(CTA_EINVAL, "rows must start on 16 bytes");
+  if (p->table_stride % (p->table_dtype == CTA_F32 ? 4 : 8) != 0) return fail(CTA_EINVAL, "the table's rows must start on 16 bytes");
+  for (const void* x : {p->q, static_cast<const void*>(p->q_out), p->table})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
+  r.q = p->q;
+  r.q_out = p->q_out;
+  r.q_sT = p->q_stride[0];
+  r.q_sH = p->q_stride[1];
+  r.o_sT = p->q_out_stride[0];
+  r.o_sH = p->q_out_stride[1];
+  r.positions = p->positions;
+  r.table = p->table;
+  r.table_sP = p->table_stride;
+  r.positions_end = p->positions_end;
+  r.H = static_cast<int>(p->heads);
+  r.pairs = static_cast<int>(p->rotary_dim / 2);
+  r.interleaved = p->interleaved != 0;
+  return launched(launch_rotary_write(r, args->dtype, p->table_dtype != CTA_F32, static_cast<cudaStream_t>(stream)),
+                  "rotary cache write launch");
+}
+
 int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args) {
+  return cta_window_paged_attention_workspace_bytes(args, 0, 0);
+}
+
+int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream) {
+  return cta_window_paged_attention(args, 0, 0, workspace, workspace_bytes, stream);
+}
+
+int64_t cta_window_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t window, int64_t sinks) {
   PagedArgs a;
-  const int rc = paged_args(args, a);
+  const int rc = paged_window(args, window, sinks, a);
   if (rc != CTA_OK) return -rc;
   if (a.T == 0 || a.B == 0) return 0;
   if (tensor_cores_pay(a)) {
@@ -361,10 +457,10 @@ int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args
   return split_bytes(paged_split_workers(a, args->dtype, args->quantized), a.d);
 }
 
-int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes,
-                        void* stream) {
+int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t window, int64_t sinks, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   PagedArgs a;
-  const int rc = paged_args(args, a);
+  const int rc = paged_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc;
   if (a.T == 0 || a.B == 0) return CTA_OK;
   // a pool without pages and a table without entries have no address
@@ -379,7 +475,7 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
   for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t need = cta_paged_attention_workspace_bytes(args);
+  const int64_t need = cta_window_paged_attention_workspace_bytes(args, window, sinks);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
   cudaError_t e = cudaSuccess;
@@ -410,6 +506,17 @@ int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, i
   a.part_ml = static_cast<float*>(workspace);
   a.part_o = a.part_ml + 2LL * a.workers * 16 * 4;
   return launched(launch_paged_split(a, args->dtype, args->quantized, st), "paged attention launch");
+}
+
+int64_t cta_prefix_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t shared_prefix) {
+  if (shared_prefix < 0) return -fail(CTA_EINVAL, "shared_prefix must not be negative");
+  return cta_window_paged_attention_workspace_bytes(args, 0, 0);
+}
+
+int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t shared_prefix, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  if (shared_prefix < 0) return fail(CTA_EINVAL, "shared_prefix must not be negative");
+  return cta_window_paged_attention(args, 0, 0, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -200,6 +200,18 @@ __device__ __forceinline__ bool mask_key(const uint32_t* m, int j) {
   return m == nullptr || ((__ldg(m + kMaskHead + (j >> 5)) >> (j & 31)) & 1u);
 }
 
+// Sliding window: the causal row at place i sees the keys j <= i that lie in its
+// window, j > i - window, or among the first ones, j < sink_end.
+struct Reach {
+  int window, sink_end;
+  __device__ __forceinline__ int first(int i) const { return i - window + 1; }
+  __device__ __forceinline__ bool sees(int i, int j) const { return j > i - window || j < sink_end; }
+};
+// of a batch entry whose first valid key is `lo`: padding on the left does not count
+__device__ __forceinline__ Reach reach_of(const AttnArgs& a, int lo) {
+  return Reach{a.window, a.sinks > 0 ? lo + a.sinks : 0};
+}
+
 __device__ __forceinline__ int64_t lse_index(const AttnArgs& a, const SeqTile& t, int h, int row) {
   return (static_cast<int64_t>(t.batch) * a.H + h) * a.L + t.row0 + row;
 }

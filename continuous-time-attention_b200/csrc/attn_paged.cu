@@ -101,6 +101,26 @@ struct SeqInfo {
   int n, rows, tiles, groups;
   int64_t row0, units;
 };
+
+// CUT: a segment takes only some of the sequence's groups: those of the first `sinks` keys, and from the one on that
+// holds the first key in the window of the tile's first row (or from `skip` on) as many as its rows' windows can touch.
+// A page between the two is not read, nor is its entry in the table.
+constexpr int kNoWindow = 1 << 30;
+__device__ __forceinline__ int cut_window(const PagedArgs& a) { return a.window > 0 ? a.window : kNoWindow; }
+__device__ __forceinline__ int sink_groups(const PagedArgs& a, int n) { return (min(a.sinks, n) + kGroup - 1) / kGroup; }
+// groups that the windows of one tile's rows touch at most
+__device__ __forceinline__ int window_groups(const PagedArgs& a, int rows, int tile_rows) {
+  const int group = a.H / a.Hk;
+  const int tokens = min(rows, (tile_rows + group - 2) / group + 1);
+  return (cut_window(a) + tokens - 1 + 2 * (kGroup - 1)) / kGroup;
+}
+// the first group behind those of the first keys, for the tile whose first row is `tok`
+__device__ __forceinline__ int first_window_group(const PagedArgs& a, int n, int rows, int tok) {
+  const int low = n - rows + tok - cut_window(a) + 1;
+  return max(max(low, 0) / kGroup, max(sink_groups(a, n), a.skip / kGroup));
+}
+
+template <bool CUT>
 __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b, int tile_rows) {
   SeqInfo s{0, 0, 0, 0, 0, 0};
   if (b >= a.B) return s;
@@ -118,7 +138,9 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedArgs& a, int b, int tile_
     s.rows = 1;
   }
   s.tiles = (s.rows * (a.H / a.Hk) + tile_rows - 1) / tile_rows;
-  s.groups = max(1, (n + kGroup - 1) / kGroup);  // a sequence without keys still writes its zeros
+  s.groups = (n + kGroup - 1) / kGroup;
+  if constexpr (CUT) s.groups = min(s.groups - a.skip / kGroup, sink_groups(a, n) + window_groups(a, s.rows, tile_rows));
+  s.groups = max(1, s.groups);  // a sequence without keys still writes its zeros
   s.units = static_cast<int64_t>(s.tiles) * s.groups;
   return s;
 }
@@ -129,9 +151,10 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
   return x;
 }
 
+template <bool CUT>
 __device__ __forceinline__ int64_t total_units(const PagedArgs& a, int tile_rows) {
   int64_t u = 0;
-  for (int b = threadIdx.x & 31; b < a.B; b += 32) u += seq_info(a, b, tile_rows).units;
+  for (int b = threadIdx.x & 31; b < a.B; b += 32) u += seq_info<CUT>(a, b, tile_rows).units;
   return warp_sum(u);
 }
 
@@ -141,11 +164,12 @@ __device__ __forceinline__ int active_shares(const PagedArgs& a, int64_t units) 
 }
 
 // the segment that holds unit u (u < total); whole warp
+template <bool CUT>
 __device__ __forceinline__ Seg find_segment(const PagedArgs& a, int64_t u, int tile_rows) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
   for (int b0 = 0;; b0 += 32) {
-    const SeqInfo s = seq_info(a, b0 + lane, tile_rows);
+    const SeqInfo s = seq_info<CUT>(a, b0 + lane, tile_rows);
     int64_t upto = s.units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -181,8 +205,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 // ROWS: 8 or 16 rows per segment
-template <typename T, bool FP8, int DP, int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3) : (DP == 64 ? 3 : 2))
+template <typename T, bool FP8, int DP, int ROWS, bool CUT>
+__global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 64 ? 4 : 3) : (DP == 64 ? 3 : 2))
     paged_split_kernel(const __grid_constant__ PagedArgs a) {
   using M = typename std::conditional<FP8, __half, T>::type;
   constexpr bool kHalf = std::is_same<M, __half>::value;
@@ -199,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, quad = lane & 3, oct = lane >> 2;
   const int worker = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int64_t units = total_units(a, ROWS);
+  const int64_t units = total_units<CUT>(a, ROWS);
   if (units == 0) return;
   const int shares = active_shares(a, units);
   const int hk = worker % a.Hk, share = worker / a.Hk;
@@ -210,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
   const int group = a.H / a.Hk;
 
   while (u < u_end) {
-    const Seg g = find_segment(a, u, ROWS);
+    const Seg g = find_segment<CUT>(a, u, ROWS);
     const int count = static_cast<int>(min(u_end - u, static_cast<int64_t>(g.groups - g.group)));
 
     // Q as the B operand: row oct of each n8 tile
@@ -263,15 +287,21 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
 
     // Last key that every row of the tile sees, -1 if one of them sees none.  Rows behind the sequence's last do not
     // count: theirs are not written.
-    int least = 0x7fffffff;
+    int least = 0x7fffffff, most = -1;
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const bool counts = (g.tile * ROWS + 2 * quad + e + 8 * r) / group < g.rows;
         if (counts) least = min(least, max(last[r][e], -1));
+        if (CUT && counts) most = max(most, last[r][e]);
       }
     least = __reduce_min_sync(0xffffffffu, least);
+    // CUT: the first key that every row's window holds, and the groups as they are numbered here
+    const int window = CUT ? cut_window(a) : 0, sinks = CUT ? sink_groups(a, g.n) : 0;
+    if constexpr (CUT) most = __reduce_max_sync(0xffffffffu, most) - window + 1;
+    const int from = CUT ? first_window_group(a, g.n, g.rows, g.tile * ROWS / group) : 0;
+    auto group_at = [&](int i) { return CUT ? (i < sinks ? i : from + i - sinks) : i; };
     float o[MT][NR][4];
     float m[NR][2], l[NR][2], mv[NR][2];  // reference of the weights, their sum, reference of the weighted values
 #pragma unroll
@@ -368,21 +398,33 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
     };
 
     // the group's page and its first slot there, now and one group on; the page after that is on its way
-    int index = g.group / per_page;
-    int slot = (g.group - index * per_page) * kGroup;
-    int page = page_at(index), page_on = page_at(index + 1);
-    load_keys(g.group, page, slot);
-    load_values(g.group, page, slot);
+    int index = group_at(g.group) / per_page;
+    int slot = (group_at(g.group) - index * per_page) * kGroup;
+    // CUT: the page after this one, if the groups that follow reach it
+    auto page_after = [&](int i) -> int {
+      if (CUT && (index + 1) * per_page > (i < sinks ? sinks - 1 : from + g.groups - 1 - sinks)) return -1;
+      return page_at(index + 1);
+    };
+    int page = page_at(index), page_on = page_after(g.group);
+    load_keys(group_at(g.group), page, slot);
+    load_values(group_at(g.group), page, slot);
     for (int it = 0; it < count; ++it) {
-      const int grp = g.group + it;
+      const int grp = group_at(g.group + it), grp_next = group_at(g.group + it + 1);
       const bool here = page >= 0;
       // where the next group lies
       int slot_next = slot + kGroup, page_next = page;
-      if (slot_next == a.page) {
+      if (CUT && g.group + it + 1 == sinks) {
+        if (it + 1 < count) {
+          index = from / per_page;
+          slot_next = (from - index * per_page) * kGroup;
+          page_next = page_at(index);
+          page_on = page_after(sinks);
+        }
+      } else if (slot_next == a.page) {
         slot_next = 0;
         page_next = page_on;
         ++index;
-        if (it + 1 < count) page_on = page_at(index + 1);
+        if (it + 1 < count) page_on = page_after(g.group + it + 1);
       }
       // scores: 16 keys x ROWS
       float s[NR][4];
@@ -414,9 +456,10 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
 #pragma unroll
         for (int t = 0; t < 2; ++t) ksc[t] = ks[t], vl2[t] = __log2f(vs[t]);
       }
-      if (it + 1 < count) load_keys(grp + 1, page_next, slot_next);
+      if (it + 1 < count) load_keys(grp_next, page_next, slot_next);
 
-      const bool all_see = here && grp * kGroup + kGroup - 1 <= least;
+      const bool all_see = here && grp * kGroup + kGroup - 1 <= least &&
+                           (!CUT || grp * kGroup >= most || (grp + 1) * kGroup <= a.sinks);
       // weights of keys oct, oct + 8 in rows 2 quad, 2 quad + 1
       uint32_t pf[NR][2];
 #pragma unroll
@@ -430,7 +473,8 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
           for (int t = 0; t < 2; ++t) {
             float x = s[r][2 * t + e] * c2[r][e];
             if constexpr (FP8) x *= ksc[t];
-            const bool see = all_see || (here && grp * kGroup + 8 * t + oct <= last[r][e]);
+            const int key = grp * kGroup + 8 * t + oct;
+            const bool see = all_see || (here && key <= last[r][e] && (!CUT || key > last[r][e] - window || key < a.sinks));
             y[t][e] = see ? x : neg_inf();
             top[e] = fmaxf(top[e], y[t][e]);
             if constexpr (FP8) {
@@ -509,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
           }
         }
       }
-      if (it + 1 < count) load_values(grp + 1, page_next, slot_next);
+      if (it + 1 < count) load_values(grp_next, page_next, slot_next);
       page = page_next;
       slot = slot_next;
     }
@@ -568,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? (FP8 || DP == 64 ? 4 : 3
 // Joins the parts of one (row, head): the warps of the CTA take the parts in turn, then join theirs in order.
 constexpr int kMaxJoinWarps = 16;
 
-template <typename T, bool HALF, int DP, int ROWS>
+template <typename T, bool HALF, int DP, int ROWS, bool CUT>
 __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   __shared__ float s_ml[kMaxJoinWarps][4];
   __shared__ float s_o[kMaxJoinWarps][DP];
@@ -592,13 +636,13 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   // its segment: units before the sequence, and all units
   int64_t before = 0, units = 0;
   for (int s = lane; s < a.B; s += 32) {
-    const int64_t x = seq_info(a, s, ROWS).units;
+    const int64_t x = seq_info<CUT>(a, s, ROWS).units;
     units += x;
     if (s < b) before += x;
   }
   before = warp_sum(before);
   units = warp_sum(units);
-  const SeqInfo s = seq_info(a, b, ROWS);
+  const SeqInfo s = seq_info<CUT>(a, b, ROWS);
   const int i = first_row * group + (h - hk * group);
   const int tile = i / ROWS, r = i - tile * ROWS;
   const int64_t u0 = before + static_cast<int64_t>(tile) * s.groups, u1 = u0 + s.groups;
@@ -657,13 +701,13 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
     if (lane + 32 * e < a.d) out[lane + 32 * e] = Elem<T>::from_f(o[e] * mul);
 }
 
-template <typename T, bool FP8, int DP, int ROWS>
+template <typename T, bool FP8, int DP, int ROWS, bool CUT>
 struct Split {
   static int workers() {
     static std::atomic<int> per_sm{0};  // the same on every device: a property of the code
     int n = per_sm.load(std::memory_order_relaxed);
     if (n == 0) {
-      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_split_kernel<T, FP8, DP, ROWS>, kThreads, 0) !=
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_split_kernel<T, FP8, DP, ROWS, CUT>, kThreads, 0) !=
               cudaSuccess || n <= 0)
         n = 1;
       per_sm.store(n, std::memory_order_relaxed);
@@ -672,7 +716,7 @@ struct Split {
   }
   static cudaError_t run(const PagedArgs& a, cudaStream_t st) {
     constexpr bool kHalf = FP8 || std::is_same<T, __half>::value;
-    paged_split_kernel<T, FP8, DP, ROWS>
+    paged_split_kernel<T, FP8, DP, ROWS, CUT>
         <<<static_cast<unsigned>((a.workers + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -690,18 +734,22 @@ struct Split {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kHalf, DP, ROWS>, a);
+    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kHalf, DP, ROWS, CUT>, a);
   }
 };
 
 // rows of the operand: 8 when no sequence has more (row, head) pairs per key/value head
-template <template <typename, bool, int, int> class F, typename G>
+template <template <typename, bool, int, int, bool> class F, typename G>
 auto with_variant(const PagedArgs& a, int dtype, int quantized, G&& g) {
   const bool few = static_cast<int64_t>(a.max_rows) * (a.H / a.Hk) <= 8;
-  auto by_rows = [&](auto t, auto fp8, auto dp) {
+  auto by_cut = [&](auto t, auto fp8, auto dp, auto rows) {
     using T = decltype(t);
-    if (few) return g(F<T, decltype(fp8)::value, decltype(dp)::value, 8>());
-    return g(F<T, decltype(fp8)::value, decltype(dp)::value, 16>());
+    if (a.window > 0 || a.skip > 0) return g(F<T, decltype(fp8)::value, decltype(dp)::value, decltype(rows)::value, true>());
+    return g(F<T, decltype(fp8)::value, decltype(dp)::value, decltype(rows)::value, false>());
+  };
+  auto by_rows = [&](auto t, auto fp8, auto dp) {
+    if (few) return by_cut(t, fp8, dp, std::integral_constant<int, 8>());
+    return by_cut(t, fp8, dp, std::integral_constant<int, 16>());
   };
   auto by_dim = [&](auto t, auto fp8) {
     if (a.d <= 64) return by_rows(t, fp8, std::integral_constant<int, 64>());

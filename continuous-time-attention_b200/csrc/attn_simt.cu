@@ -191,7 +191,8 @@ __device__ __forceinline__ SeqTile block_tile(const AttnArgs& a, int tile, int r
 // keys per tile: 64, and 32 at head dim 256, where the tiles of four tensors have to fit shared memory
 template <int DP> struct SimtTile { static constexpr int KT = DP == 256 ? 32 : 64; };
 
-template <typename T, int DP>
+// WINDOW: rows see the keys of Reach; tiles between the first keys and the tile's window are passed over
+template <typename T, int DP, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int KT = SimtTile<DP>::KT, C = KT / 8, DC = DP / 32, R = kSimtRows / 16;
   extern __shared__ float4 smem_raw[];
@@ -221,7 +222,12 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
     for (int x = 0; x < DC; ++x) acc[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float c2 = a.scale * kLog2e;
+  const Reach reach = reach_of(a, lo);
   for (int j0 = lo / KT * KT; j0 < hi; j0 += KT) {
+    if (WINDOW && j0 >= reach.sink_end && j0 + KT <= reach.first(t.first)) {
+      j0 = reach.first(t.first) / KT * KT;
+      if (j0 >= hi) break;
+    }
     __syncthreads();
     const uint64_t valid = valid_keys<KT>(mask, j0, t.n);
     load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, valid);
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_fwd_kernel(const __grid_co
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int j = j0 + tx + 8 * c;
-        const bool see = j < t.n && (!a.causal || j <= i) && ((valid >> (tx + 8 * c)) & 1u);
+        const bool see = j < t.n && (!a.causal || j <= i) && (!WINDOW || reach.sees(i, j)) && ((valid >> (tx + 8 * c)) & 1u);
         s[r][c] = see ? s[r][c] * c2 : neg_inf();
         top = fmaxf(top, s[r][c]);
       }
@@ -284,7 +290,7 @@ __device__ __forceinline__ void weight_grad(float s, float dp, float lse2, float
   ds = see ? p * (dp - delta) : 0.f;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int KT = SimtTile<DP>::KT, C = KT / 8, DC = DP / 32, R = kSimtRows / 16;
   extern __shared__ float4 smem_raw[];
@@ -318,7 +324,12 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
     for (int x = 0; x < DC; ++x) acc[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float c2 = a.scale * kLog2e;
+  const Reach reach = reach_of(a, lo);
   for (int j0 = lo / KT * KT; j0 < hi; j0 += KT) {
+    if (WINDOW && j0 >= reach.sink_end && j0 + KT <= reach.first(t.first)) {
+      j0 = reach.first(t.first) / KT * KT;
+      if (j0 >= hi) break;
+    }
     __syncthreads();
     const uint64_t valid = valid_keys<KT>(mask, j0, t.n);
     load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, j0, t.n, a.d, valid);
@@ -332,8 +343,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int i = t.first + ty + 16 * r, j = j0 + tx + 8 * c;
-        const bool see = i < t.n && j < t.n && (!a.causal || j <= i) && ((valid >> (tx + 8 * c)) & 1u) &&
-                         lse2[r] != neg_inf();
+        const bool see = i < t.n && j < t.n && (!a.causal || j <= i) && (!WINDOW || reach.sees(i, j)) &&
+                         ((valid >> (tx + 8 * c)) & 1u) && lse2[r] != neg_inf();
         float p, ds;
         weight_grad(s[r][c], dp[r][c], lse2[r], delta[r], c2, see, p, ds);
         P[(ty + 16 * r) * (KT + kPad) + tx + 8 * c] = ds;
@@ -349,7 +360,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
 }
 
 // owns KT keys of one key/value head; rows of the score tile are keys, columns are queries
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int KT = SimtTile<DP>::KT, QT = KT, C = QT / 8, DC = DP / 32, R = KT / 16;
   extern __shared__ float4 smem_raw[];
@@ -389,10 +400,22 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   mask_range(a, t.batch, t.n, lo, hi);
   // rows that see no key, up to the first valid one, may hold anything
   const int from = lo >= hi ? t.n : a.causal ? lo : 0;
+  const Reach reach = reach_of(a, lo);
+  // rows behind the windows that hold the last of these keys see none of them, unless it is one of the first
+  const int end = WINDOW && t.first >= reach.sink_end ? min(t.n, t.first + KT - 1 + reach.window) : t.n;
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
-    for (int i0 = a.causal ? t.first : 0; i0 < t.n; i0 += QT) {
+    for (int i0 = a.causal ? t.first : 0; i0 < end; i0 += QT) {
       if (from >= i0 + QT) continue;
-      const uint64_t seeing = from > i0 ? ~0ull << (from - i0) : ~0ull;
+      uint64_t seeing = from > i0 ? ~0ull << (from - i0) : ~0ull;
+      if constexpr (WINDOW) {
+        // a window may lie on masked keys alone: such a row sees nothing and may hold anything, as the padding may
+#pragma unroll
+        for (int x = 0; x < QT; x += 32) {
+          const int i = i0 + x + static_cast<int>(threadIdx.x & 31);
+          const unsigned some = __ballot_sync(0xffffffffu, i < t.n && a.lse[lse_index(a, t, h, i)] != neg_inf());
+          seeing &= ~(static_cast<uint64_t>(~some) << x);
+        }
+      }
       __syncthreads();
       load_rows<T, QT, DP>(Q, a.q, a.qs, t, h, i0, t.n, a.d, seeing);
       load_rows<T, QT, DP>(G, a.g, a.gs, t, h, i0, t.n, a.d, seeing);
@@ -410,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           const int q = tx + 8 * c, i = i0 + q, j = t.first + ty + 16 * r;
-          const bool see = key[r] && i < t.n && (!a.causal || j <= i) && s_lse[q] != neg_inf();
+          const bool see = key[r] && i < t.n && (!a.causal || j <= i) && (!WINDOW || reach.sees(i, j)) && s_lse[q] != neg_inf();
           float p;
           weight_grad(s[r][c], dp[r][c], s_lse[q], s_delta[q], c2, see, p, dp[r][c]);
           P[(ty + 16 * r) * (QT + kPad) + q] = p;
@@ -558,34 +581,38 @@ int64_t count_tiles(AttnArgs& a, int rows) {
 }
 
 // shared memory is the same for every launch of a kernel
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 cudaError_t fwd(AttnArgs a, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
   constexpr int smem = sizeof(float) * ((kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
   const int64_t tiles = count_tiles(a, kSimtRows);
-  return launch_grid<attn_simt_fwd_kernel<T, DP>>(false, tiles * a.H, kThreads, smem, st, a);
+  return launch_grid<attn_simt_fwd_kernel<T, DP, WINDOW>>(false, tiles * a.H, kThreads, smem, st, a);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 cudaError_t bwd(AttnArgs a, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
   if (a.dk != nullptr) {
     constexpr int smem = sizeof(float) * (4 * KT * (DP + kPad) + KT * (KT + kPad));
     const int64_t tiles = count_tiles(a, KT);
-    const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP>>(false, tiles * a.Hk, kThreads, smem, st, a);
+    const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP, WINDOW>>(false, tiles * a.Hk, kThreads, smem, st, a);
     if (e != cudaSuccess) return e;
   }
   if (a.dq == nullptr) return cudaSuccess;
   constexpr int smem = sizeof(float) * ((2 * kSimtRows + 2 * KT) * (DP + kPad) + kSimtRows * (KT + kPad));
   const int64_t tiles = count_tiles(a, kSimtRows);
-  return launch_grid<attn_simt_dq_kernel<T, DP>>(a.dk != nullptr, tiles * a.H, kThreads, smem, st, a);
+  return launch_grid<attn_simt_dq_kernel<T, DP, WINDOW>>(a.dk != nullptr, tiles * a.H, kThreads, smem, st, a);
 }
 
+template <typename T, bool WINDOW>
+cudaError_t dispatch_dim(const AttnArgs& a, bool backward, cudaStream_t st) {
+  if (a.d <= 64) return backward ? bwd<T, 64, WINDOW>(a, st) : fwd<T, 64, WINDOW>(a, st);
+  if (a.d <= 128) return backward ? bwd<T, 128, WINDOW>(a, st) : fwd<T, 128, WINDOW>(a, st);
+  return backward ? bwd<T, 256, WINDOW>(a, st) : fwd<T, 256, WINDOW>(a, st);
+}
 template <typename T>
 cudaError_t dispatch(const AttnArgs& a, bool backward, cudaStream_t st) {
-  if (a.d <= 64) return backward ? bwd<T, 64>(a, st) : fwd<T, 64>(a, st);
-  if (a.d <= 128) return backward ? bwd<T, 128>(a, st) : fwd<T, 128>(a, st);
-  return backward ? bwd<T, 256>(a, st) : fwd<T, 256>(a, st);
+  return a.window > 0 ? dispatch_dim<T, true>(a, backward, st) : dispatch_dim<T, false>(a, backward, st);
 }
 
 }  // namespace

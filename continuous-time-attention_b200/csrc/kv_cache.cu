@@ -302,10 +302,207 @@ cudaError_t dispatch(const CacheArgs& a, int dtype, bool write, cudaStream_t st)
   return wide ? launch<__half, 32>(a, write, st) : launch<__half, 16>(a, write, st);
 }
 
+
+// ---------------------------------------------------------------------------
+// rotation by position, on the way into the cache
+// ---------------------------------------------------------------------------
+// The first 2 P elements of a row of q or k are P pairs, (x_i, x_{P + i}), or interleaved (x_{2i}, x_{2i + 1}); pair i of
+// a token at position p turns by the angle whose cosine and sine the table holds in [p, i] and [p, P + i]:
+//   (a, b) -> (a cos - b sin, b cos + a sin)
+// in fp32, rounded once: to q's type, the cache's type, or e4m3 straight from fp32 (an intermediate 16-bit row would
+// round twice).
+//
+// A lane takes 16 elements of a row as two pieces of 16 bytes that hold whole pairs: pieces l and l + P / 8, or 2 l and
+// 2 l + 1; the elements behind the pairs go by in the same steps.  So no pair is split between lanes, and out may be q
+// itself.  GROUP lanes hold a row and take kHeads heads of one token, for which the angles are loaded once.
+//
+// Its floor is HBM: q read and written, k and v read, the cache written.
+template <typename T, bool TABLE16>
+__device__ __forceinline__ void load_turn(const void* table, int64_t at, float (&x)[8]) {
+  if constexpr (TABLE16) {
+    unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(table) + at)), x);
+  } else {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(table) + at);
+    const float4 lo = __ldg(p), hi = __ldg(p + 1);
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+    x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+  }
+}
+
+template <typename T, int GROUP, bool QUANT, bool TABLE16>
+__global__ void __launch_bounds__(kThreads) rotary_write_kernel(const __grid_constant__ RotaryArgs r) {
+  const CacheArgs& a = r.cache;
+  const int lane = threadIdx.x % GROUP;
+  const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
+  const unsigned q_blocks = (r.H + kHeads - 1) / kHeads, k_blocks = (a.Hk + kHeads - 1) / kHeads;
+  const unsigned blocks = q_blocks + 2 * k_blocks;
+  const unsigned t = group / blocks, block = group - t * blocks;
+  const bool any = t < static_cast<unsigned>(a.T);
+  // 0: q, 1: k, 2: v
+  const int what = block < q_blocks ? 0 : block < q_blocks + k_blocks ? 1 : 2;
+  const int heads = what == 0 ? r.H : a.Hk;
+  const int h0 = static_cast<int>(what == 0 ? block : what == 1 ? block - q_blocks : block - q_blocks - k_blocks) * kHeads;
+  const int pairs = r.pairs;
+  const bool turns = what != 2 && lane * 8 < pairs;  // this lane's elements are pairs
+  const int c0 = turns && !r.interleaved ? 8 * lane : 16 * lane;
+  const int c1 = turns && !r.interleaved ? 8 * lane + pairs : 16 * lane + 8;
+  const bool live = any && 16 * lane < a.d;
+  const T* in = static_cast<const T*>(what == 0 ? r.q : what == 1 ? a.k_in : a.v_in);
+  const int64_t sT = what == 0 ? r.q_sT : what == 1 ? a.k_sT : a.v_sT, sH = what == 0 ? r.q_sH : what == 1 ? a.k_sH : a.v_sH;
+  const int64_t slot_at = any ? __ldg(a.slots + t) : -1;
+  const int64_t pos = any ? __ldg(r.positions + t) : -1;
+  uint4 x0[kHeads], x1[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    x0[i] = x1[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (live && h0 + i < heads) {
+      const T* row = in + t * sT + (h0 + i) * sH;
+      x0[i] = *reinterpret_cast<const uint4*>(row + c0);
+      x1[i] = *reinterpret_cast<const uint4*>(row + c1);
+    }
+  }
+  // a position outside the table: reported; q's row is zero, the token is not written
+  const bool placed = pos >= 0 && pos < r.positions_end;
+  if (any && !placed && slot_at >= 0 && lane == 0) atomicExch(&g_cache_error, kDevBadIndex);
+  float cs[8] = {}, sn[8] = {};
+  if (turns && placed) {
+    load_turn<T, TABLE16>(r.table, pos * r.table_sP + 8 * lane, cs);
+    load_turn<T, TABLE16>(r.table, pos * r.table_sP + pairs + 8 * lane, sn);
+  }
+  auto rotated = [&](int i, float (&f)[16]) {
+    float u[8], w[8];
+    unpack8<T>(x0[i], u);
+    unpack8<T>(x1[i], w);
+    if (turns && r.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = __fmaf_rn(u[2 * e], cs[e], -u[2 * e + 1] * sn[e]);
+        f[2 * e + 1] = __fmaf_rn(u[2 * e + 1], cs[e], u[2 * e] * sn[e]);
+        f[8 + 2 * e] = __fmaf_rn(w[2 * e], cs[4 + e], -w[2 * e + 1] * sn[4 + e]);
+        f[9 + 2 * e] = __fmaf_rn(w[2 * e + 1], cs[4 + e], w[2 * e] * sn[4 + e]);
+      }
+    } else if (turns) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = __fmaf_rn(u[e], cs[e], -w[e] * sn[e]);
+        f[8 + e] = __fmaf_rn(w[e], cs[e], u[e] * sn[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = u[e], f[8 + e] = w[e];
+    }
+  };
+  auto halves = [&](const float (&f)[16], uint4& lo, uint4& hi) {
+    float u[8], w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = f[e], w[e] = f[8 + e];
+    lo = pack8<T>(u);
+    hi = pack8<T>(w);
+  };
+  if (what == 0) {
+    T* out = static_cast<T*>(r.q_out);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      float f[16];
+      rotated(i, f);
+      uint4 lo, hi;
+      halves(f, lo, hi);
+      if (!placed) lo = hi = make_uint4(0u, 0u, 0u, 0u);
+      if (live && h0 + i < heads) {
+        T* row = out + t * r.o_sT + (h0 + i) * r.o_sH;
+        *reinterpret_cast<uint4*>(row + c0) = lo;
+        *reinterpret_cast<uint4*>(row + c1) = hi;
+      }
+    }
+    return;
+  }
+  const bool second = what == 2;
+  const bool keep = in_cache(a, slot_at, any && lane == 0) && placed && live;
+  const unsigned page = static_cast<unsigned>(slot_at) / a.page, slot = static_cast<unsigned>(slot_at) - page * a.page;
+  const int64_t cH = second ? a.vc_sH : a.kc_sH;
+  const int64_t base = page * (second ? a.vc_sP : a.kc_sP) + slot * (second ? a.vc_sS : a.kc_sS) + h0 * cH;
+  if constexpr (QUANT) {
+    uint8_t* cache = static_cast<uint8_t*>(second ? a.v_cache : a.k_cache);
+    float* scale = second ? a.v_scale : a.k_scale;
+    // the lanes of this row; others of the warp may have a row of q and be gone
+    const unsigned members = (GROUP == 32 ? 0xffffffffu : (1u << (GROUP & 31)) - 1u) << (threadIdx.x & 31 & ~(GROUP - 1));
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      float f[16];
+      rotated(i, f);
+      float m = kLeastMax;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(f[e]));
+#pragma unroll
+      for (int o = 1; o < GROUP; o <<= 1) m = fmaxf(m, __shfl_xor_sync(members, m, o));
+      // as in cache_write_kernel
+      const float rec = __fdiv_rn(1.f, fraction(m));
+      const float2 rr = f2(rec), div = f2(-fraction(m));
+      const float2 num = f2(__uint_as_float(((262u - (__float_as_uint(m) >> 23)) << 23) | 0x600000u));
+      float2 y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 z = mul2(make_float2(f[2 * e], f[2 * e + 1]), num), q0 = mul2(z, rr);
+        y[e] = fma2(fma2(q0, div, z), rr, q0);
+      }
+      if (keep && h0 + i < heads) {
+        uint2 lo, hi;
+        lo.x = to_e4m3x4(y[0].x, y[0].y, y[1].x, y[1].y);
+        lo.y = to_e4m3x4(y[2].x, y[2].y, y[3].x, y[3].y);
+        hi.x = to_e4m3x4(y[4].x, y[4].y, y[5].x, y[5].y);
+        hi.y = to_e4m3x4(y[6].x, y[6].y, y[7].x, y[7].y);
+        uint8_t* row = cache + base + i * cH;
+        *reinterpret_cast<uint2*>(row + c0) = lo;
+        *reinterpret_cast<uint2*>(row + c1) = hi;
+        if (lane == 0) scale[(static_cast<int64_t>(page) * a.Hk + h0 + i) * a.page + slot] = __fdiv_rn(m, kE4m3Max);
+      }
+    }
+  } else {
+    T* cache = static_cast<T*>(second ? a.v_cache : a.k_cache);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      uint4 lo = x0[i], hi = x1[i];
+      if (!second) {
+        float f[16];
+        rotated(i, f);
+        halves(f, lo, hi);
+      }
+      if (keep && h0 + i < heads) {
+        T* row = cache + base + i * cH;
+        *reinterpret_cast<uint4*>(row + c0) = lo;
+        *reinterpret_cast<uint4*>(row + c1) = hi;
+      }
+    }
+  }
+}
+
+template <typename T, int GROUP>
+cudaError_t launch_rotary(const RotaryArgs& r, bool table16, cudaStream_t st) {
+  const int64_t blocks = (r.H + kHeads - 1) / kHeads + 2 * ((r.cache.Hk + kHeads - 1) / kHeads);
+  const int64_t ctas = (r.cache.T * blocks * GROUP + kThreads - 1) / kThreads;
+  if (ctas > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (r.cache.quantized) {
+    if (table16) rotary_write_kernel<T, GROUP, true, true><<<grid, kThreads, 0, st>>>(r);
+    else rotary_write_kernel<T, GROUP, true, false><<<grid, kThreads, 0, st>>>(r);
+  } else {
+    if (table16) rotary_write_kernel<T, GROUP, false, true><<<grid, kThreads, 0, st>>>(r);
+    else rotary_write_kernel<T, GROUP, false, false><<<grid, kThreads, 0, st>>>(r);
+  }
+  return cudaGetLastError();
+}
+
 }  // namespace
 
 cudaError_t launch_cache_write(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, true, st); }
 cudaError_t launch_cache_read(const CacheArgs& a, int dtype, cudaStream_t st) { return dispatch(a, dtype, false, st); }
+
+cudaError_t launch_rotary_write(const RotaryArgs& r, int dtype, bool table16, cudaStream_t st) {
+  // 16 elements per lane
+  if (dtype == kBF16)
+    return r.cache.d > 128 ? launch_rotary<__nv_bfloat16, 16>(r, table16, st) : launch_rotary<__nv_bfloat16, 8>(r, table16, st);
+  return r.cache.d > 128 ? launch_rotary<__half, 16>(r, table16, st) : launch_rotary<__half, 8>(r, table16, st);
+}
 
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
                                 cudaStream_t st) {

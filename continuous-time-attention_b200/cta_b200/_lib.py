@@ -96,7 +96,7 @@ _SIGNATURES = {
     "cta_diffusion_shard_bld": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                         c_int64, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_float,
                                         c_void_p]),
-    # the three structs are passed as packed bytes (ATTENTION_ARGS, ...)
+    # the four structs are passed as packed bytes (ATTENTION_ARGS, ...)
     "cta_attention_forward": (c_int, [c_void_p, c_void_p]),
     "cta_attention_backward": (c_int, [c_void_p, c_void_p]),
     "cta_attention_mask_words_per_row": (c_int64, [c_int64]),
@@ -105,12 +105,21 @@ _SIGNATURES = {
     "cta_kv_cache_read": (c_int, [c_void_p, c_void_p]),
     "cta_paged_attention_workspace_bytes": (c_int64, [c_void_p]),
     "cta_paged_attention": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "cta_window_attention_forward": (c_int, [c_void_p, c_int64, c_int64, c_void_p]),
+    "cta_window_attention_workspace_bytes": (c_int64, [c_void_p, c_int64, c_int64]),
+    "cta_window_attention_backward": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "cta_window_paged_attention_workspace_bytes": (c_int64, [c_void_p, c_int64, c_int64]),
+    "cta_window_paged_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "cta_prefix_paged_attention_workspace_bytes": (c_int64, [c_void_p, c_int64]),
+    "cta_prefix_paged_attention": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "cta_rotary_cache_write": (c_int, [c_void_p, c_void_p, c_void_p]),
 }
 
-# layouts of cta_attention_args, cta_kv_cache_args and cta_paged_attention_args
+# layouts of cta_attention_args, cta_kv_cache_args, cta_paged_attention_args and cta_rotary_args
 ATTENTION_ARGS = struct.Struct("=13Q24q5q4i2f")
 KV_CACHE_ARGS = struct.Struct("=7Q10q5q2i")
 PAGED_ATTENTION_ARGS = struct.Struct("=9Q11q9q2i2f")
+ROTARY_ARGS = struct.Struct("=4Q5q3q2i")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -238,7 +247,8 @@ def ptr_array(tensors) -> ctypes.Array:
 
 def device_error(clear: bool = True) -> int:
     """Device-side error word (0 = ok, 1 = a bounded in-kernel wait timed out, 2 = a
-    page, slot or length outside a key/value cache was skipped)."""
+    page, slot or length outside a key/value cache, or a position outside the table of
+    angles, was skipped)."""
     return int(load().cta_device_error(1 if clear else 0))
 
 

@@ -4,7 +4,7 @@
 (``cta_b200.transformers``, ``attention="fused"``) and of packed prefill
 batches, whose output the mixer (``cta_b200.serving_vllm``) refines: padded
 [B, L, heads, dim] with a key mask, or packed [T, heads, dim] with offsets;
-causal or not; grouped key/value heads; float32, bfloat16, float16.
+causal or not, or causal within a sliding window whose first tokens stay visible; grouped key/value heads; float32, bfloat16, float16.
 """
 from __future__ import annotations
 
@@ -20,15 +20,15 @@ __all__ = ["prompt_attention"]
 
 class _PromptAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale):
+    def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale, reach):
         q, k, v, cu, sizes, code, scale = ops._attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
         out = ops._new(q)
         # what rounding the output loses: delta of rows with few keys needs it
         low = torch.empty_like(out) if code != 0 else None
         lse = ops._attention_forward(q, k, v, out, 0 if low is None else low.data_ptr(), cu, mask_words, causal, scale,
-                                     sizes, code, True, True)
+                                     sizes, code, True, True, reach)
         ctx.save_for_backward(q, k, v, out, low, lse, mask_words, cu)
-        ctx.plan = (causal, scale, sizes, code)
+        ctx.plan = (causal, scale, reach, sizes, code)
         return out
 
     @staticmethod
@@ -39,7 +39,7 @@ class _PromptAttention(torch.autograd.Function):
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq, dk, dv = ops._attention_backward(grad_out, q, k, v, out, 0 if low is None else low.data_ptr(), lse, cu,
                                              mask_words, *ctx.plan, need_q, need_k or need_v)
-        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None, None
 
 
 def _tangents(*tensors: torch.Tensor) -> bool:
@@ -59,6 +59,8 @@ def prompt_attention(
     key_mask: Optional[torch.Tensor] = None,
     mask_words: Optional[torch.Tensor] = None,
     cu_seqlens: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """softmax(scale * q k^T) v over the keys each row sees, differentiable in q, k, v.
 
@@ -66,13 +68,16 @@ def prompt_attention(
     [B, L] (any mask dtype, non-zero = valid) hides padding, or ``mask_words``,
     its form from ``ops.attention_mask``, made once for several layers.  Packed:
     [T, heads, dim] with ``cu_seqlens`` (device int32, sequences + 1 offsets from 0, not decreasing).  ``causal``:
-    row i sees keys j <= i of its sequence.  ``scale`` defaults to dim**-0.5.
+    row i sees keys j <= i of its sequence; with ``window`` only those with j > i - window
+    and the first ``sinks`` ones of its sequence (of a padded one with a mask: from
+    its first valid token on).  ``scale`` defaults to dim**-0.5.
 
     A row that sees no key is zero and has no gradient, as are packed rows
     behind the last sequence.  Masked keys and such rows may hold anything,
     infinities and NaN included; a NaN or infinity in the k or v of a valid token may
-    also reach earlier rows of its sequence, one in the q or the output gradient of
-    a row the gradients of later keys.  Forward-mode differentiation raises."""
+    also reach rows of its sequence that do not see it, one in the q or the output
+    gradient of a row the gradients of keys that it does not see.  Forward-mode differentiation raises."""
+    reach = ops._window(window, sinks, causal)
     words = mask_words
     if key_mask is not None:
         if words is not None:
@@ -83,6 +88,6 @@ def prompt_attention(
             raise ValueError(f"key_mask on {key_mask.device}, expected {q.device}")
         words = ops.attention_mask(key_mask)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _tangents(q, k, v):
-        return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal), scale)
+        return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal), scale, reach)
     return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens,
-                                 need_lse=False)[0]
+                                 need_lse=False, window=window, sinks=sinks)[0]

@@ -9,6 +9,7 @@ sequence length < 3) with the reference's aliasing rules before calling here.
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Sequence, Union
 
 import torch
@@ -618,6 +619,23 @@ def _attention_inputs(q, k, v, cu_seqlens, mask_words, scale):
     return q, k, v, cu, (sequences, length, heads, kv_heads, dim), code, dim**-0.5 if scale is None else float(scale)
 
 
+def _window(window, sinks, causal: bool = True):
+    """Checked (window, sinks) as the library takes them, (0, 0) without a window."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks go with a window")
+        return 0, 0
+    w, s = operator.index(window), operator.index(sinks)
+    if w < 1 or s < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {w} and {s}")
+    if not causal:
+        raise ValueError("a window needs causal=True")
+    return min(w, _FAR), min(s, _FAR)
+
+
+_FAR = 1 << 40  # more keys than any call has
+
+
 def _mask_row_words(length: int) -> int:
     """cta_attention_mask_words_per_row: a header of 4 words, then one bit per key in blocks of 128."""
     return 4 + (length + 127) // 128 * 4
@@ -674,6 +692,8 @@ def attention_forward(
     out: Optional[torch.Tensor] = None,
     need_lse: bool = True,
     out_low: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ):
     """Softmax attention of prompts, one launch: (out, lse).
 
@@ -687,14 +707,19 @@ def attention_forward(
     attention_backward takes.  `out_low`, for 16-bit types a contiguous tensor
     like out, receives what rounding out lost (in float16 times 2048): given to
     attention_backward too, it spares the gradients of rows with few keys the
-    error of that rounding."""
+    error of that rounding.
+
+    `window` (causal only): row i sees the last `window` keys, j > i - window, and the
+    first `sinks` ones of its sequence (with a key mask, from its first valid key on);
+    what no row of a tile sees costs nothing."""
+    reach = _window(window, sinks, causal)
     q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
     o = _new(q) if out is None else _out(out, q.shape, q)
     return o, _attention_forward(q, k, v, o, _low(out_low, q), cu, mask_words, causal, scale, sizes, code, need_lse,
-                                 out is None)
+                                 out is None, reach)
 
 
-def _attention_forward(q, k, v, o, low, cu, mask_words, causal, scale, sizes, code, need_lse, zero_tail):
+def _attention_forward(q, k, v, o, low, cu, mask_words, causal, scale, sizes, code, need_lse, zero_tail, reach=(0, 0)):
     """attention_forward of inputs that have been checked into o; `low` is an address or 0.  Returns lse."""
     lse = None
     if need_lse:
@@ -704,7 +729,10 @@ def _attention_forward(q, k, v, o, low, cu, mask_words, causal, scale, sizes, co
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low, 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, 0,
         0 if cu is None else cu.data_ptr(), 0 if mask_words is None else mask_words.data_ptr(), *_strides3(q),
         *_strides3(k), *_strides3(v), *_strides3(o), *_NO_STRIDES, *sizes, code, bool(causal), zero_tail, 0, scale, 0.0)
-    _lib.enqueue(_lib.load().cta_attention_forward, q, args)
+    if reach[0]:
+        _lib.enqueue(_lib.load().cta_window_attention_forward, q, args, *reach)
+    else:
+        _lib.enqueue(_lib.load().cta_attention_forward, q, args)
     return lse
 
 
@@ -723,9 +751,12 @@ def attention_backward(
     need_dq: bool = True,
     need_dkv: bool = True,
     out_low: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ):
     """(dq, dk, dv) of attention_forward from its out, lse and, if it wrote one, out_low; None for what is not
     wanted."""
+    reach = _window(window, sinks, causal)
     q, k, v, cu, sizes, code, scale = _attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
     n, length, heads = sizes[:3]
     if grad_out.shape != q.shape or out.shape != q.shape:
@@ -738,11 +769,12 @@ def attention_backward(
     shape = (n, heads, length) if cu is None else (heads, length)
     if lse.shape != shape or lse.dtype != torch.float32 or lse.get_device() != device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 {shape} on {q.device}")
-    return _attention_backward(grad_out, q, k, v, out, _low(out_low, q), lse, cu, mask_words, causal, scale, sizes, code,
-                               need_dq, need_dkv)
+    return _attention_backward(grad_out, q, k, v, out, _low(out_low, q), lse, cu, mask_words, causal, scale, reach, sizes,
+                               code, need_dq, need_dkv)
 
 
-def _attention_backward(grad_out, q, k, v, out, low, lse, cu, mask_words, causal, scale, sizes, code, need_dq, need_dkv):
+def _attention_backward(grad_out, q, k, v, out, low, lse, cu, mask_words, causal, scale, reach, sizes, code, need_dq,
+                        need_dkv):
     """attention_backward of inputs that have been checked; `low` is an address or 0."""
     if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()
             and (code == 0 or sizes[4] & 7 or not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15)):
@@ -759,8 +791,26 @@ def _attention_backward(grad_out, q, k, v, out, low, lse, cu, mask_words, causal
         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(cu), _lib.ptr(mask_words), *_strides3(q), *_strides3(k),
         *_strides3(v), *_strides3(o), *_strides3(g), *_strides3(dq), *_strides3(dk), *_strides3(dv), *sizes, code,
         bool(causal), 0, planes, scale, 0.0)
-    _lib.enqueue(_lib.load().cta_attention_backward, q, args)
+    if not reach[0]:
+        _lib.enqueue(_lib.load().cta_attention_backward, q, args)
+        return dq, dk, dv
+    lib = _lib.load()
+    nbytes = _workspace_bytes(lib.cta_window_attention_workspace_bytes, q, args, *reach)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.enqueue(lib.cta_window_attention_backward, q, args, *reach, _lib.ptr(ws), nbytes)
     return dq, dk, dv
+
+
+def _workspace_bytes(query, t: torch.Tensor, *args) -> int:
+    """query(*args) on t's device; raises what the call itself would."""
+    if _lib._current_device() == t.get_device():
+        nbytes = query(*args)
+    else:
+        with _lib.on_device(t):
+            nbytes = query(*args)
+    if nbytes < 0:
+        _lib.check(-nbytes)
+    return nbytes
 
 
 # ---------------------------------------------------------------------------
@@ -856,6 +906,110 @@ def kv_cache_write(
     _cache_call(_lib.load().cta_kv_cache_write, k, v, k_cache, v_cache, slots, k_scale, v_scale, sizes)
 
 
+def rotary_cache_write(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """kv_cache_write of keys that are rotated by their positions on the way; returns the
+    queries rotated too.  One launch.
+
+    q [T, heads, dim], k and v [T, kv_heads, dim] (bf16 / fp16), slots [T] and positions [T]
+    (int64); the cache as for ``kv_cache_write``.  cos_sin [positions, rotary_dim], float32 or
+    q's type, holds the cosines of a position's rotary_dim / 2 angles, then the sines
+    (``rotary_table``).  The first rotary_dim elements of a row (a multiple of 16) are
+    pairs, elements i and rotary_dim / 2 + i, or with ``interleaved`` 2 i and 2 i + 1;
+    pair (a, b) becomes (a cos - b sin, b cos + a sin).  fp32, rounded once; an e4m3 cache
+    takes scale and codes from the unrounded row.
+
+    ``out`` receives the queries and may be q itself.  A negative slot leaves the cache
+    alone (padding rows; their queries are rotated all the same), the others must be
+    distinct.  A slot past the cache is skipped; a token whose position is
+    outside of cos_sin has a zero query and is not written.  Both are reported by
+    ``_lib.device_error()``, the position only where the slot is not negative."""
+    return _rotary_launch(*_rotary_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved, k_scale,
+                                        v_scale, out))
+
+
+def _rotary_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved, k_scale, v_scale, out):
+    """All checks of rotary_cache_write but the library's own, and what its launch takes."""
+    device = q.get_device()
+    if device < 0:
+        _require_cuda(q, "q")
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 3 or len(kshape) != 3 or kshape != v.shape or kshape[0] != shape[0] or kshape[2] != shape[2]:
+        raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)} must be (T, heads, dim) of one T and dim")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.get_device() != device or v.get_device() != device:
+        _same_kind(k, "k", q)
+        _same_kind(v, "v", q)
+    code = _lib.dtype_code(q.dtype)
+    pages, page, kv_heads, dim, quantized = _cache_sizes(k_cache, v_cache, k_scale, v_scale, q.dtype, q)
+    if kshape[1] != kv_heads or kshape[2] != dim:
+        raise ValueError(f"k {tuple(kshape)} does not fit a cache {tuple(k_cache.shape)}")
+    slots = _slots(slots, shape[0], q)
+    if positions.dim() != 1 or positions.shape[0] != shape[0]:
+        raise ValueError("positions must have shape (T,)")
+    if positions.dtype != torch.int64 or positions.get_device() != device:
+        positions = _device_ints(positions, "positions", q, torch.int64)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if cos_sin.dim() != 2 or cos_sin.dtype not in (torch.float32, q.dtype) or cos_sin.get_device() != device:
+        raise ValueError(f"cos_sin must have shape (positions, rotary_dim), float32 or {q.dtype} on {q.device}, got "
+                         f"{tuple(cos_sin.shape)}, {cos_sin.dtype} on {cos_sin.device}")
+    if not _on16(cos_sin):
+        raise ValueError("cos_sin must have a contiguous last axis and rows that start on 16 bytes")
+    q, k, v = (x if _on16(x) else _own_rows(x) for x in (q, k, v))
+    if out is None:
+        o = _new(q)
+    else:
+        o = _out(out, shape, q)
+        if not _on16(o):
+            raise ValueError("out must have rows that start on 16 bytes")
+    cache = _lib.KV_CACHE_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
+        slots.data_ptr(), *_row_strides(k), *_row_strides(v), *_row_strides(k_cache), *_row_strides(v_cache), shape[0],
+        kv_heads, dim, pages, page, code, quantized)
+    rotary = _lib.ROTARY_ARGS.pack(
+        q.data_ptr(), o.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), *_row_strides(q), *_row_strides(o),
+        cos_sin.stride(0) if cos_sin.shape[0] > 1 else 0, shape[1], cos_sin.shape[1], cos_sin.shape[0],
+        _lib.dtype_code(cos_sin.dtype), bool(interleaved))
+    return q, o, cache, rotary, (k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, cos_sin)
+
+
+def _rotary_launch(q, o, cache, rotary, _held):
+    _lib.enqueue(_lib.load().cta_rotary_cache_write, q, cache, rotary)
+    return o
+
+
+def rotary_table(
+    positions: int,
+    rotary_dim: int,
+    *,
+    base: float = 10000.0,
+    dtype: torch.dtype = torch.float32,
+    device: Union[str, torch.device] = "cuda",
+) -> torch.Tensor:
+    """cos_sin [positions, rotary_dim] for ``rotary_cache_write``: the cosines, then the sines, of
+    position / base**(2 i / rotary_dim), from angles in 64 bits (a position of 10^5 has
+    no digits left behind the point of a turn in fp32), rounded once."""
+    if positions < 0 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"positions must not be negative and rotary_dim even, got {positions} and {rotary_dim}")
+    half = rotary_dim // 2
+    turn = float(base) ** (-torch.arange(half, dtype=torch.float64, device=device) / half)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * turn
+    return torch.cat([angle.cos(), angle.sin()], dim=1).to(dtype)
+
+
 def kv_cache_read(
     k_cache: torch.Tensor,
     v_cache: torch.Tensor,
@@ -893,6 +1047,9 @@ def paged_attention(
     k_scale: Optional[torch.Tensor] = None,
     v_scale: Optional[torch.Tensor] = None,
     out: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
+    shared_prefix: int = 0,
 ) -> torch.Tensor:
     """Attention of each sequence's newest rows over its keys and values in a paged cache
     (16-bit, or e4m3 with scales), those of the rows themselves included.
@@ -907,14 +1064,29 @@ def paged_attention(
     Rows that see no key are zero; rows behind the last sequence are not
     written.  A NaN or infinity in the v of a cached token may also reach earlier
     rows of this call.  A page outside the cache or a length past the table counts as no
-    keys and is reported by ``_lib.device_error()``."""
+    keys and is reported by ``_lib.device_error()``.
+
+    `window`: the row whose last key is j0 sees the keys j <= j0 with j > j0 - window, and
+    the first `sinks` keys.  Pages that no row sees are not read, and their entries in
+    the table may hold anything: an engine may have freed them.
+
+    `shared_prefix`: the batch's sequences all begin with the same keys, and the rows of
+    block_table name the same pages for the first shared_prefix of them (a page that
+    they fill in part does not count).  Where that pays they are read once for all
+    rows; it changes what the call costs, and its sums' order, not what it computes.
+    With a window it is not used."""
     return _paged_launch(*_paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale,
-                                      v_scale, out))
+                                      v_scale, out, window, sinks, shared_prefix))
 
 
-def _paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale, v_scale, out):
-    """All checks of paged_attention, and what its launch takes: (q, out, arguments, bytes of workspace, the tensors
-    that the arguments point to)."""
+def _paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale, v_scale, out,
+                window=None, sinks=0, shared_prefix=0):
+    """All checks of paged_attention, and what its launch takes: (q, out, the library's call, its arguments, bytes of
+    workspace, the tensors that the arguments point to)."""
+    reach = _window(window, sinks)
+    prefix = operator.index(shared_prefix)
+    if prefix < 0:
+        raise ValueError(f"shared_prefix must not be negative, got {prefix}")
     device = q.get_device()
     if device < 0:
         _require_cuda(q, "q")
@@ -958,18 +1130,18 @@ def _paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows
         table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o), *_row_strides(k_cache),
         *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, tshape[1],
         int(max_rows), code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
-    if _lib._current_device() == device:
-        nbytes = lib.cta_paged_attention_workspace_bytes(args)
+    if reach[0]:
+        fn, query, args = lib.cta_window_paged_attention, lib.cta_window_paged_attention_workspace_bytes, (args, *reach)
+    elif prefix:
+        fn, query, args = lib.cta_prefix_paged_attention, lib.cta_prefix_paged_attention_workspace_bytes, (args, prefix)
     else:
-        with _lib.on_device(q):
-            nbytes = lib.cta_paged_attention_workspace_bytes(args)
-    if nbytes < 0:
-        _lib.check(-nbytes)
-    return q, o, args, nbytes, (k_cache, v_cache, k_scale, v_scale, table, lens, cu)
+        fn, query, args = lib.cta_paged_attention, lib.cta_paged_attention_workspace_bytes, (args,)
+    nbytes = _workspace_bytes(query, q, *args)
+    return q, o, fn, args, nbytes, (k_cache, v_cache, k_scale, v_scale, table, lens, cu)
 
 
-def _paged_launch(q, o, args, nbytes, _held):
+def _paged_launch(q, o, fn, args, nbytes, _held):
     # a buffer of the caching allocator per call: calls on other streams and captured graphs have their own
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.enqueue(_lib.load().cta_paged_attention, q, args, _lib.ptr(ws), nbytes)
+    _lib.enqueue(fn, q, *args, _lib.ptr(ws), nbytes)
     return o

@@ -188,6 +188,12 @@ class CtaPostAttnMixer(nn.Module):
         v_scale: Optional[torch.Tensor] = None,
         is_prefill: Optional[bool] = None,
         residual: Optional[torch.Tensor] = None,
+        positions: Optional[torch.Tensor] = None,
+        cos_sin: Optional[torch.Tensor] = None,
+        interleaved: bool = False,
+        window: Optional[int] = None,
+        sinks: int = 0,
+        shared_prefix: int = 0,
     ) -> torch.Tensor:
         """Attention of a packed batch over the paged cache, then the mixer: [T, heads * dim].
 
@@ -200,7 +206,13 @@ class CtaPostAttnMixer(nn.Module):
         dim], in q's type or float8_e4m3fn with scales [pages, kv_heads,
         page_size] (``ops.kv_cache_write``, ``ops.paged_attention``).  No device
         data is read on the host.  Rows behind the last sequence come back
-        undefined, as the mixer leaves them; ``residual`` as for ``forward``."""
+        undefined, as the mixer leaves them; ``residual`` as for ``forward``.
+
+        ``positions`` [T] with ``cos_sin`` (and ``interleaved``) rotate q and k by
+        their positions on the way (``ops.rotary_cache_write``; q itself is left as
+        it is).  ``window`` and ``sinks`` limit what a row sees, ``shared_prefix``
+        says how many keys all sequences begin with (vLLM's
+        ``common_prefix_len``): see ``ops.paged_attention``."""
         for name in ("slot_mapping", "block_table", "seq_lens", "query_start_loc"):
             if getattr(attn_metadata, name, None) is None:
                 raise ValueError(f"attn_metadata has no {name}")
@@ -213,10 +225,24 @@ class CtaPostAttnMixer(nn.Module):
         if slots.dim() != 1 or slots.shape[0] < k.shape[0]:
             raise ValueError("slot_mapping must have an entry for every row of k")
         # refused, if at all, before the cache is touched
+        slots = slots[: k.shape[0]]
+        if positions is not None:
+            if cos_sin is None:
+                raise ValueError("positions go with cos_sin")
+            if positions.dim() != 1 or positions.shape[0] < q.shape[0]:
+                raise ValueError("positions must have an entry for every row of q")
+            rotary = ops._rotary_plan(q, k, v, k_cache, v_cache, slots, positions[: q.shape[0]], cos_sin, interleaved,
+                                      k_scale, v_scale, None)
+            q = rotary[1]
+        elif cos_sin is not None:
+            raise ValueError("cos_sin goes with positions")
         plan = ops._paged_plan(q, k_cache, v_cache, attn_metadata.block_table, attn_metadata.seq_lens,
                                self._device_qsl(attn_metadata.query_start_loc, q.device), max(1, max_rows), scale, k_scale,
-                               v_scale, None)
-        ops.kv_cache_write(k, v, k_cache, v_cache, slots[: k.shape[0]], k_scale=k_scale, v_scale=v_scale)
+                               v_scale, None, window, sinks, shared_prefix)
+        if positions is not None:
+            ops._rotary_launch(*rotary)
+        else:
+            ops.kv_cache_write(k, v, k_cache, v_cache, slots, k_scale=k_scale, v_scale=v_scale)
         out = ops._paged_launch(*plan)
         return self.forward(out.flatten(1), attn_metadata=attn_metadata, is_prefill=is_prefill,
                             residual=residual)

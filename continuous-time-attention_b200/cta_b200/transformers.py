@@ -15,9 +15,12 @@ no L x L mask or scores in memory, forward or backward.  Two things differ from
 the stock modules: the attention weights themselves are not dropped out (the
 layers' other dropouts stay), and a row that sees no valid token (left padding
 under the causal mask) gets zeros from its attention, where softmax over nothing
-gives NaN.
+gives NaN.  The language model's ``attention_window=W, attention_sinks=S`` (fused
+only) limit each token's attention to the last W tokens and the first S valid ones.
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -71,11 +74,14 @@ def _key_words(attention_mask: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
 class _FusedSelfAttention(nn.MultiheadAttention):
     """The layers' attention module (same parameters and names), running fused."""
 
+    reach = {}  # window and sinks, where the model has them
+
     def forward(self, x, mask_words, causal):  # type: ignore[override]
         B, L, E = x.shape
         qkv = F.linear(x, self.in_proj_weight, self.in_proj_bias).view(B, L, 3, self.num_heads, E // self.num_heads)
         q, k, v = qkv.unbind(2)
-        return self.out_proj(prompt_attention(q, k, v, causal=causal, mask_words=mask_words).reshape(B, L, E))
+        return self.out_proj(prompt_attention(q, k, v, causal=causal, mask_words=mask_words, **self.reach)
+                             .reshape(B, L, E))
 
 
 class _FusedAttentionLayer(nn.TransformerEncoderLayer):
@@ -194,14 +200,22 @@ class PDETransformerLM(nn.Module):
         max_length=512,
         dropout=0.1,
         attention: str = "torch",
+        attention_window: Optional[int] = None,
+        attention_sinks: int = 0,
         **pde_kwargs,
     ):
         super().__init__()
+        ops._window(attention_window, attention_sinks)
+        if attention_window is not None and attention != "fused":
+            raise ValueError("attention_window needs attention='fused'")
         self.embedding = nn.Embedding(vocab_size, embed_dim)
         self.pos_encoder = nn.Parameter(torch.randn(1, max_length, embed_dim))
         self.dropout = nn.Dropout(dropout)
         self.attention = attention
         self.transformer_layers = _encoder_layers(attention, embed_dim, num_heads, hidden_dim, num_layers, dropout)
+        if attention_window is not None:
+            for layer in self.transformer_layers:
+                layer.self_attn.reach = {"window": attention_window, "sinks": attention_sinks}
         self.pde_layout = pde_layout
         self.pde_layers = nn.ModuleList(
             [

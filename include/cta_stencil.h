@@ -338,6 +338,20 @@ typedef struct cta_attention_args {
 int cta_attention_forward(const cta_attention_args* args, void* stream);
 int cta_attention_backward(const cta_attention_args* args, void* stream);
 
+/* The same with a sliding window (causal != 0): row i sees key j <= i if j > i -
+ * window or if key j is one of its sequence's first `sinks` keys (of a padded
+ * sequence with a key mask: the first sinks from its first valid key on).
+ * window 0: no window, and no sinks.  Tiles that no row of a tile sees are
+ * passed over.  backward: workspace is
+ * cta_window_attention_workspace_bytes(args, window, sinks) bytes on 16 (sizes
+ * and types of args count, of its pointers only which are NULL; 0 = none;
+ * negative: minus the status with which the call would refuse), not shared by
+ * calls that may overlap; it needs no clearing. */
+int cta_window_attention_forward(const cta_attention_args* args, int64_t window, int64_t sinks, void* stream);
+int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int64_t window, int64_t sinks);
+int cta_window_attention_backward(const cta_attention_args* args, int64_t window, int64_t sinks, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 /* A key mask ([B, L], any listed dtype, non-zero = valid) as the words that the
  * calls above take: cta_attention_mask_words_per_row(L) words per batch entry. */
 int64_t cta_attention_mask_words_per_row(int64_t length);
@@ -379,6 +393,31 @@ typedef struct cta_kv_cache_args {
 int cta_kv_cache_write(const cta_kv_cache_args* args, void* stream);
 int cta_kv_cache_read(const cta_kv_cache_args* args, void* stream);
 
+/* cta_kv_cache_write of rows that are rotated by their positions on the way, with
+ * the queries beside them.  The first rotary_dim = 2 P elements of each row of k
+ * (args) and of q ([tokens, heads, dim], args->dim, args->dtype) are P pairs,
+ * elements i and P + i, or interleaved != 0: 2 i and 2 i + 1; of the token at
+ * position p (positions[t], DEVICE int64) pair i = (a, b) becomes
+ *   (a cos - b sin, b cos + a sin),  cos = table[p, i],  sin = table[p, P + i]
+ * in fp32, rounded once to where it goes: q_out (which may be q), the 16-bit
+ * cache, or e4m3, whose scale and codes are those of the unrounded row.  v is
+ * written as it is.  table: [positions_end, rotary_dim], fp32 or args->dtype, last
+ * axis contiguous, rows on 16 bytes.  A negative slot leaves the cache alone; q is
+ * rotated all the same.  A position outside the table writes zeros to q_out and
+ * nothing to the cache, and is reported by cta_device_error() as 2 unless the
+ * slot is negative.  rotary_dim: a multiple of 16 up to dim. */
+typedef struct cta_rotary_args {
+  const void* q;
+  void* q_out;
+  const int64_t* positions;
+  const void* table;
+  int64_t q_stride[2], q_out_stride[2], table_stride;
+  int64_t heads, rotary_dim, positions_end;
+  int32_t table_dtype, interleaved;
+} cta_rotary_args;
+
+int cta_rotary_cache_write(const cta_kv_cache_args* args, const cta_rotary_args* rotary, void* stream);
+
 /* Attention of each sequence's newest rows over its cached keys, theirs
  * included: row r of the n_r rows of sequence b (rows [cu_seqlens[b],
  * cu_seqlens[b + 1]) of q; cu_seqlens NULL: row b alone) sees keys
@@ -413,6 +452,23 @@ typedef struct cta_paged_attention_args {
 
 int64_t cta_paged_attention_workspace_bytes(const cta_paged_attention_args* args);
 int cta_paged_attention(const cta_paged_attention_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same with a sliding window: the row whose last key is j0 sees keys j <= j0
+ * with j > j0 - window or j < sinks.  window 0: no window, and no sinks.  Pages
+ * that no row sees are not read, and their entries in the table may hold
+ * anything. */
+int64_t cta_window_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t window, int64_t sinks);
+int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t window, int64_t sinks, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* The same for a batch whose sequences all begin with the same keys: the rows of
+ * block_table name the same pages for the first shared_prefix keys (>= 0; a last
+ * page that they fill in part does not count), and those are read once for all
+ * rows where that pays.  It changes the cost and the order of the sums, not what
+ * is computed.  Sequences may end within the prefix. */
+int64_t cta_prefix_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t shared_prefix);
+int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t shared_prefix, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
