@@ -122,6 +122,11 @@ struct PagedArgs {
   // logarithm (base 2) of the value's in fp16; else nullptr
   const float* k_res;
   const float* v_res;
+  int64_t expanded_pages;
+  // shared prefix of `skip` keys: its sums over prefix_splits parts of prefix_chunk keys, for every row of q
+  int prefix_splits, prefix_chunk;
+  float* prefix_o;   // [splits, T, H, dim rounded up to 64 or 128] fp32
+  float* prefix_ml;  // [splits, T, H, 4] as part_ml
 };
 
 // workers (warps) of the split kernel on the current device, and its launch
@@ -133,6 +138,9 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
 bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
 int attn_pack(int group);  // heads of a group that one row tile holds: its largest power of two
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
+// sums of all rows over the first `skip` keys of the table's first row
+int64_t prefix_tiles(const PagedArgs& p);  // CTAs for each part
+bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
 // e4m3 caches: the pages that the table names, as 16-bit rows in page order (page i of sequence b is page
 // b * table_width + i), for the tensor-core kernel
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,

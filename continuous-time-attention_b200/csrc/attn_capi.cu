@@ -295,7 +295,7 @@ bool tma_can_address(const PagedArgs& a) {
                                        axis(a.n_pages, a.vc_sP), axis(a.page, a.vc_sS), axis(a.Hk, a.vc_sH)});
 }
 bool tensor_cores_pay(const PagedArgs& a) {
-  if (a.window > 0 || !tma_can_address(a)) return false;
+  if (!tma_can_address(a)) return false;
   const int64_t group = a.H / a.Hk, pack = attn_pack(static_cast<int>(group));
   if (a.cu == nullptr || a.max_rows * group <= 16 || !(a.scale > 0.f)) return false;
   const int64_t b = a.B;
@@ -345,7 +345,7 @@ int cta_window_attention_forward(const cta_attention_args* args, int64_t window,
   if (rc != CTA_OK) return rc == kNothing ? CTA_OK : rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (a.window > 0 || !launch_attn_tc_fwd(a, args->dtype, st, &e)) e = launch_attn_simt_fwd(a, args->dtype, st);
+  if (!launch_attn_tc_fwd(a, args->dtype, st, &e)) e = launch_attn_simt_fwd(a, args->dtype, st);
   return launched(e, "attention forward launch");
 }
 
@@ -498,6 +498,7 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
       x.v_cache = v;
       x.k_res = k_res;
       x.v_res = v_res;
+      x.expanded_pages = static_cast<int64_t>(a.B) * a.table_width;
       if (launch_paged_tc(x, args->dtype, st, &e)) return launched(e, "paged attention launch");
       return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");
     }

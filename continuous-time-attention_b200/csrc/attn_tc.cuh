@@ -173,6 +173,9 @@ __device__ __forceinline__ void first_bits(int count, uint32_t (&w)[4]) {
   }
 }
 
+// the bits of a word from number x on
+__device__ __forceinline__ uint32_t bits_from(int x) { return x <= 0 ? 0xffffffffu : x >= 32 ? 0u : 0xffffffffu << x; }
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
                                             int c3) {
   asm volatile(

@@ -63,6 +63,7 @@ struct FwdArgs {
   AttnArgs a;
   int pack;          // heads per tile row block
   int tile_tokens;   // kRows / pack
+  int warp_span;     // tokens from a warp's first row to its last
   int across;        // order of the work, see find_tile
   // paged keys
   const int32_t* table;
@@ -74,7 +75,15 @@ struct FwdArgs {
   const float* k_res;
   const float* v_res;
   int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
+  // shared prefix: `splits` parts of `chunk` keys (whole tiles), whose sums go to part_o [splits, rows, heads, DP] and
+  // part_ml [splits, rows, heads, 4] as the split kernel leaves them (attn_paged.cu)
+  int splits, chunk, prefix;
+  float* part_o;
+  float* part_ml;
 };
+
+// What the rows see.  kPrefix: all rows of a batch over the pages that it begins with.
+enum Form : int { kPlain = 0, kWindow = 1, kPrefix = 2 };
 
 template <int DP>
 struct Layout {
@@ -98,7 +107,30 @@ struct Item {
   bool last;   // there is no more work
 };
 
-template <typename T, int DP, bool PAGED, bool SCALED>
+// kPrefix: the last key that row `tok` sees, by its own sequence's length; rows behind the last sequence do not count
+__device__ __forceinline__ int last_key(const FwdArgs& f, int tok) {
+  const AttnArgs& a = f.a;
+  int b = tok, from = tok, rows = 1;
+  if (a.cu != nullptr) {
+    // the last sequence that begins at or before the row
+    int lo = 0, hi = a.nseq;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.cu + mid + 1) > tok) hi = mid;
+      else lo = mid + 1;
+    }
+    if (lo == a.nseq) return 0x7fffffff;
+    b = lo;
+    int64_t begin;
+    clamp_range(a.cu, b, a.L, begin, rows);
+    from = static_cast<int>(begin);
+  }
+  const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
+  const int n = static_cast<int>(min(static_cast<int64_t>(max(__ldg(f.seq_lens + b), 0)), most));
+  return n - rows + tok - from;
+}
+
+template <typename T, int DP, bool PAGED, bool SCALED, int FORM>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FwdArgs f) {
@@ -166,17 +198,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     taken();
     return true;
   };
-  // steps of 128 keys of the two tiles; j_lo: the first
-  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j_lo, int& shift) {
-    shift = PAGED ? x.n - x.t.n : 0;
-    j_lo = x.lo / kRows;
+  // steps of 128 keys of the two tiles; j0: the first key of the first
+  // kWindow: the tiles between the first keys and `from`, where the windows begin, are passed over
+  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j0, int& from, int& shift) {
+    shift = PAGED && FORM != kPrefix ? x.n - x.t.n : 0;
+    int tile = x.lo / kRows, jump = 1 << 30, gap = 0;
+    from = 0;
+    if constexpr (FORM == kWindow) {
+      const int window_tile = max(tile, max(x.t.first + shift - a.window + 1, 0) / kRows);
+      if (a.sinks == 0) {
+        tile = window_tile;
+      } else {
+        const int sink_tiles = (x.lo + a.sinks + kRows - 1) / kRows;
+        if (window_tile > sink_tiles) jump = sink_tiles - tile, gap = window_tile - sink_tiles;
+      }
+      from = window_tile * kRows;
+    }
+    j0 = tile * kRows;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       first[i] = x.t.first + i * f.tile_tokens;
       int end = x.hi;
       if (a.causal) end = min(end, min(first[i] + f.tile_tokens, x.t.n) + shift);
-      steps[i] = first[i] < x.t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
+      int n = (end + kRows - 1) / kRows - tile;
+      if (FORM == kWindow && n > jump) n = max(jump, n - gap);
+      steps[i] = first[i] < x.t.n ? max(0, n) : 0;
     }
+  };
+  // first keys that stay visible to all: those before this one
+  auto sinks_of = [&](const Item& x) { return FORM == kWindow && a.sinks > 0 ? x.lo + a.sinks : 0; };
+  // to the next tile
+  auto advance = [&](int& j0, int from, const Item& x) {
+    j0 += kRows;
+    if (FORM == kWindow && j0 >= sinks_of(x)) j0 = max(j0, from);
   };
   // bit c of word i: key 32 i + c of the tile at j0 is one of the sequence's and valid; `kt`: running number of the tile
   auto key_words = [&](int n, const uint32_t* mask, int j0, int kt, uint32_t (&w)[4]) {
@@ -223,6 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int hb = id % blocks;
         x.h0 = hb * f.pack;
         x.hk = x.h0 / (a.H / a.Hk);
+        if constexpr (FORM == kPrefix) {
+          const int y = id / blocks, part = y % f.splits;
+          x.t.n = static_cast<int>(a.L);
+          x.t.first = y / f.splits * 2 * f.tile_tokens;
+          x.lo = part * f.chunk;
+          x.n = x.hi = min(f.prefix, x.lo + f.chunk);
+        } else {
         x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
                         f.seq_lens);
         x.n = x.hi = x.t.n;
@@ -236,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           x.hi = x.n;
         } else {
           mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
+        }
         }
       }
       if (lane == 0) {
@@ -254,8 +316,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = read_item(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j_lo, shift;
-      plan(x, first, steps, j_lo, shift);
+      int first[2], steps[2], j0, from, shift;
+      plan(x, first, steps, j0, from, shift);
       const int all = max(steps[0], steps[1]);
       if (all == 0) {
         taken();
@@ -277,13 +339,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const CUtensorMap* map = (y & 1) ? &vmap : &kmap;
         const uint32_t dst = smem + (2 + stage) * L::kTile;
-        const int j0 = (j_lo + (y >> 1)) * kRows;
         if constexpr (PAGED) {
           // one lane per box; a box outside the sequence or the cache is left out
           const int boxes = kRows / f.box;
           const int key = j0 + lane * f.box;
           int page = -1;
-          if (lane < boxes && key < x.n) {
+          // no row's window reaches it: the page may be gone
+          const bool reached = FORM != kWindow || key < a.sinks || key + f.box > x.t.first + shift - a.window + 1;
+          if (lane < boxes && key < x.n && reached) {
             page = __ldg(f.table + x.t.seq * f.table_sB + key / f.page);
             if (page < 0 || page >= f.n_pages) {
               atomicExch(&g_tc_fwd_error, kDevBadIndex);
@@ -313,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::tma_load_4d(dst + c * L::kHalf, map, &bars.kv_full[stage], 64 * c, x.hk,
                             static_cast<int>(x.t.row0) + j0, x.t.batch);
         }
+        if (y & 1) advance(j0, from, x);
         ++kv;
       }
       taken();
@@ -338,8 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j_lo, shift;
-      plan(x, first, steps, j_lo, shift);
+      int first[2], steps[2], j0, from, shift;
+      plan(x, first, steps, j0, from, shift);
       const int all = max(steps[0], steps[1]), mine = i == 0 ? steps[0] : steps[1];
       if (all == 0) continue;
       ok = tc::wait(&bars.q_full, nq & 1);
@@ -361,14 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::commit(&bars.kv_empty[kv % NS]);
       }
       __syncwarp();
-      for (int j = 0; j < all && ok; ++j) {
+      for (int j = 0; j < all && ok; ++j, advance(j0, from, x)) {
         kv_wait(2 * j + 1);
         if (j + 1 < all) kv_wait(2 * j + 2);
         if (!ok) break;
         if (j < mine) {
           // values of keys that are not there or not valid may hold anything
           uint32_t w[4];
-          const int j0 = (j_lo + j) * kRows;
           if (PAGED || mask != nullptr || j0 + kRows > x.n) {
             key_words(x.n, mask, j0, (kv >> 1) + j, w);
             if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
@@ -410,8 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j_lo, shift;
-      plan(x, first, steps, j_lo, shift);
+      int first[2], steps[2], j0, from, shift;
+      plan(x, first, steps, j0, from, shift);
       const int mine = i == 0 ? first[0] : first[1], count = i == 0 ? steps[0] : steps[1];
       const int all = max(steps[0], steps[1]);
       if (!PAGED && a.cu != nullptr && a.zero_tail && warp < 4 && x.t.n == 0) {
@@ -428,31 +491,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
       const int tok = mine + row / f.pack, h = x.h0 + row % f.pack;
       const bool live = tok < x.t.n;
-      const int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
-      const int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
+      int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
+      int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
+      if constexpr (FORM == kPrefix) {
+        // of its own sequence, which may end here
+        limit = live ? min(n - 1, last_key(f, tok)) : n - 1;
+        limit_all = __reduce_min_sync(0xffffffffu, limit);
+      }
       T* out = static_cast<T*>(a.o) + x.t.batch * a.os.b + (x.t.row0 + tok) * a.os.t + h * a.os.h;
       float* lse = live && half == 0 && a.lse != nullptr ? a.lse + lse_index(a, x.t, h, tok) : nullptr;
+      const int sink_end = sinks_of(x);
       // the first fraction of this half's keys
-      int res = SCALED ? (x.t.seq * a.Hk + x.hk) * static_cast<int>(residue_row(f.table_width * f.page)) +
-                             j_lo * kRows + 64 * half
-                       : 0;
+      int res = SCALED ? (x.t.seq * a.Hk + x.hk) * static_cast<int>(residue_row(f.table_width * f.page)) + j0 + 64 * half : 0;
       float m = neg_inf(), sum = 0.f;
       float mv = neg_inf();  // kWeighted: the reference of weight * scale, as an exponent of two
-      for (int j = 0; j < count; ++j, ++ns, res += SCALED ? kRows : 0) {
+      auto next = [&] {
+        const int before = j0;
+        advance(j0, from, x);
+        if (SCALED) res += j0 - before;
+      };
+      for (int j = 0; j < count; ++j, ++ns, next()) {
         if (SCALED && lane < 4)  // two lines each of the step's fractions
           asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 2 ? f.k_res : f.v_res) + res + 32 * (lane & 1)));
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
         ok = ok && tc::wait(&bars.s_full[i], ns & 1);
         tc::fence_after();
-        const int j0 = (j_lo + j) * kRows;
         uint32_t s[2][32];
         if (!SCALED) {
           tc::ld32(s_addr, s[0]);
           tc::ld32(s_addr + 32, s[1]);
         }
         // warp-uniform: every row of the warp sees all keys of the tile
-        bool whole = j0 + kRows <= n && (!a.causal || j0 + kRows - 1 <= limit_all);
+        bool whole = j0 + kRows <= n && ((FORM != kPrefix && !a.causal) || j0 + kRows - 1 <= limit_all) &&
+                     (FORM != kWindow || j0 > limit_all + f.warp_span - a.window || j0 + kRows <= sink_end);
         uint32_t w[4];
         if (PAGED || mask != nullptr || !whole) {
           key_words(n, mask, j0, kt + j, w);
@@ -483,8 +555,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         auto hide = [&](int c, uint32_t (&x)[32]) {
           const int left = limit - j0 - 64 * half - 32 * c + 1;
-          const uint32_t see =
+          uint32_t see =
               (half == 0 ? w[c] : w[2 + c]) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+          if constexpr (FORM == kWindow) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - j0 - 64 * half - 32 * c);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!((see >> e) & 1u)) x[e] = 0xff800000u;
@@ -618,6 +691,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         sum += s_sum[i][half ^ 1][row];
       }
+      if constexpr (FORM == kPrefix) {
+        // The part's sums as they are.  The join takes it that values of half products carry 2^7; bf16 weights over e4m3
+        // codes do not.
+        constexpr float kUnit = SCALED && !kWeighted ? 128.f : 1.f;
+        const int64_t at = (static_cast<int64_t>(x.lo / f.chunk) * a.L + tok) * a.H + h;
+        float* to = f.part_o + at * DP + half * (DP / 2);
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[16];
+          tc::ld16(o_addr + 16 * c, o);
+          tc::wait_ld(o);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<float4*>(to + 16 * c + e) =
+                  make_float4(__uint_as_float(o[e]) * kUnit, __uint_as_float(o[e + 1]) * kUnit,
+                              __uint_as_float(o[e + 2]) * kUnit, __uint_as_float(o[e + 3]) * kUnit);
+          }
+        }
+        if (live && half == 0)
+          *reinterpret_cast<float4*>(f.part_ml + at * 4) =
+              make_float4(m * c2, kShift == 0.f ? sum : sum * 0x1p-7f, kWeighted ? mv : m * c2, 0.f);
+        tc::fence_before();
+        continue;
+      }
       // the factor between the references, which a scale past 2^120 takes out of fp32's range, and fp16's anyway
       const float unit = kWeighted ? ex2(fminf(mv - kHalfShift - m * c2, 127.f)) : 1.f;
       const float inv = sum > 0.f ? unit / sum : sum == 0.f ? 0.f : sum;  // NaN stays
@@ -637,20 +735,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kSoftmaxWarps) tc::dealloc(tmem, 512);
 }
 
-template <typename T, int DP, bool PAGED, bool SCALED>
+template <typename T, int DP, bool PAGED, bool SCALED, int FORM>
 cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int64_t ctas,
                    cudaStream_t st) {
-  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED, SCALED>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
+  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED, SCALED, FORM>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
 }
 
-template <bool PAGED, bool SCALED>
+template <bool PAGED, bool SCALED, int FORM>
 cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int dtype,
                      int64_t ctas, cudaStream_t st) {
   if (dtype == kBF16)
-    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
-                       : launch<__nv_bfloat16, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
-  return f.a.d <= 64 ? launch<__half, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
-                     : launch<__half, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
+    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED, SCALED, FORM>(q, k, v, f, ctas, st)
+                       : launch<__nv_bfloat16, 128, PAGED, SCALED, FORM>(q, k, v, f, ctas, st);
+  return f.a.d <= 64 ? launch<__half, 64, PAGED, SCALED, FORM>(q, k, v, f, ctas, st)
+                     : launch<__half, 128, PAGED, SCALED, FORM>(q, k, v, f, ctas, st);
 }
 
 }  // namespace
@@ -663,6 +761,7 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   f.a = a;
   f.pack = attn_pack(a.H / a.Hk);
   f.tile_tokens = kRows / f.pack;
+  f.warp_span = 31 / f.pack;
   const int64_t nb = a.cu != nullptr ? 1 : a.nseq;
   CUtensorMap q, k, v;
   if (!attn_map(&q, a.q, dtype, nb, a.L, a.H, a.d, a.qs, f.pack, f.tile_tokens) ||
@@ -685,13 +784,16 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   // the keys' sake (24 such sequences, 32/8 heads, three times the pieces: 281 and 266 us).
   const int64_t pieces = tiles * (a.H / f.pack);
   f.across = a.cu != nullptr || (a.causal && pieces <= 12 * num_sms_here());
-  *e = dispatch<false, false>(q, k, v, f, dtype, pieces, st);
+  *e = a.window > 0 ? dispatch<false, false, kWindow>(q, k, v, f, dtype, pieces, st)
+                    : dispatch<false, false, kPlain>(q, k, v, f, dtype, pieces, st);
   return true;
 }
 
-bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
-  if (!(p.scale > 0.f) || p.cu == nullptr) return false;
-  FwdArgs f = {};
+namespace {
+
+// what chunks and prefixes have in common: the tensors and the pages
+bool paged_maps(const PagedArgs& p, int dtype, FwdArgs& f, CUtensorMap (&maps)[3]) {
+  if (!(p.scale > 0.f)) return false;
   AttnArgs& a = f.a;
   a.q = p.q;
   a.o = p.o;
@@ -703,36 +805,71 @@ bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t
   a.H = p.H;
   a.Hk = p.Hk;
   a.d = p.d;
-  a.causal = 1;
   a.scale = p.scale;
   f.pack = attn_pack(p.H / p.Hk);
   f.tile_tokens = kRows / f.pack;
+  f.warp_span = 31 / f.pack;
   f.table = p.table;
   f.table_sB = p.table_sB;
   f.seq_lens = p.seq_lens;
-  f.across = 1;
   f.table_width = p.table_width;
   f.page = p.page;
   f.n_pages = p.n_pages;
   f.k_res = p.k_res;
   f.v_res = p.v_res;
   f.box = std::min(p.page & -p.page, kRows);  // the largest power of two that divides a page
-  f.wide_out = row_alignment(a.o, a.os, 1, a.H);
   // expanded pages are contiguous
-  const int64_t pages = p.k_res != nullptr ? static_cast<int64_t>(p.B) * p.table_width : p.n_pages;
+  const int64_t pages = p.k_res != nullptr ? p.expanded_pages : p.n_pages;
   const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
   const AttnStrides ks = p.k_res != nullptr ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
   const AttnStrides vs = p.k_res != nullptr ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
-  CUtensorMap q, k, v;
-  if (!attn_map(&q, p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) ||
-      !attn_map(&k, p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) ||
-      !attn_map(&v, p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box))
-    return false;
+  return attn_map(&maps[0], p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) &&
+         attn_map(&maps[1], p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) &&
+         attn_map(&maps[2], p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box);
+}
+
+}  // namespace
+
+bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
+  if (p.cu == nullptr) return false;
+  FwdArgs f = {};
+  CUtensorMap m[3];
+  if (!paged_maps(p, dtype, f, m)) return false;
+  f.a.causal = 1;
+  f.a.window = p.window;
+  f.a.sinks = p.sinks;
+  f.across = 1;
+  f.wide_out = row_alignment(f.a.o, f.a.os, 1, f.a.H);
   const int64_t tiles = packed_tiles(p.T, p.B, 2 * f.tile_tokens);
-  a.tiles = static_cast<int>(tiles);
+  f.a.tiles = static_cast<int>(tiles);
   const int64_t pieces = tiles * (p.H / f.pack);
-  *e = p.k_res != nullptr ? dispatch<true, true>(q, k, v, f, dtype, pieces, st)
-                          : dispatch<true, false>(q, k, v, f, dtype, pieces, st);
+  if (p.window > 0)
+    *e = p.k_res != nullptr ? dispatch<true, true, kWindow>(m[0], m[1], m[2], f, dtype, pieces, st)
+                            : dispatch<true, false, kWindow>(m[0], m[1], m[2], f, dtype, pieces, st);
+  else
+    *e = p.k_res != nullptr ? dispatch<true, true, kPlain>(m[0], m[1], m[2], f, dtype, pieces, st)
+                            : dispatch<true, false, kPlain>(m[0], m[1], m[2], f, dtype, pieces, st);
+  return true;
+}
+
+// row tiles of 256 (row, head) pairs
+int64_t prefix_tiles(const PagedArgs& p) {
+  const int64_t rows = 2 * (kRows / attn_pack(p.H / p.Hk));
+  return (p.T + rows - 1) / rows * (p.H / attn_pack(p.H / p.Hk));
+}
+
+bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
+  FwdArgs f = {};
+  CUtensorMap m[3];
+  if (!paged_maps(p, dtype, f, m)) return false;
+  f.splits = p.prefix_splits;
+  f.chunk = p.prefix_chunk;
+  f.prefix = p.skip;
+  f.part_o = p.prefix_o;
+  f.part_ml = p.prefix_ml;
+  const int64_t pieces = prefix_tiles(p) * f.splits;
+  *e = p.k_res != nullptr ? dispatch<true, true, kPrefix>(m[0], m[1], m[2], f, dtype, pieces, st)
+                          : dispatch<true, false, kPrefix>(m[0], m[1], m[2], f, dtype, pieces, st);
   return true;
 }
 

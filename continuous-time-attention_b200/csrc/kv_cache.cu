@@ -234,7 +234,18 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
       for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
   if (c >= a.d) return;
   const int n = __ldg(a.seq_lens + b);
-  const int page = n < 0 || j >= static_cast<unsigned>(n) ? -1 : __ldg(a.table + b * a.table_sB + j / a.page);
+  bool there = n >= 0 && j < static_cast<unsigned>(n);
+  if (a.window > 0) {
+    // Left out where no row's window reaches, but for boxes that the reader loads whole: what lies beside a key that
+    // counts meets a zero weight, and must not be NaN.
+    const int box = min(a.page & -a.page, 128);
+    int64_t begin;
+    int rows;
+    clamp_range(a.cu, b, a.T, begin, rows);
+    const int at = static_cast<int>(j) / box * box;
+    there = there && (at < a.sinks || at + box > n - rows - a.window + 1);
+  }
+  const int page = there ? __ldg(a.table + b * a.table_sB + j / a.page) : -1;
   if (page < 0 || page >= a.n_pages) {
     // not there, or reported by the kernel that reads the pages, which leaves it out
     if (lane == 0)
