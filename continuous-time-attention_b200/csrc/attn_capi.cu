@@ -357,7 +357,7 @@ int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int
   AttnArgs a;
   const int rc = prompt_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc == kNothing ? 0 : -rc;
-  return 0;
+  return a.dk != nullptr ? far_bytes(a, args->dtype) : 0;
 }
 
 int cta_window_attention_backward(const cta_attention_args* args, int64_t window, int64_t sinks, void* workspace,
@@ -374,9 +374,13 @@ int cta_window_attention_backward(const cta_attention_args* args, int64_t window
     a.g_norm = a.delta + plane;
     a.v_norm = a.g_norm + plane;
   }
+  const int64_t need = a.dk != nullptr ? far_bytes(a, args->dtype) : 0;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CTA_EINVAL, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_attn_delta(a, args->dtype, st);
-  if (e == cudaSuccess && (a.window > 0 || !launch_attn_tc_bwd(a, args->dtype, st, &e))) e = launch_attn_simt_bwd(a, args->dtype, st);
+  if (e == cudaSuccess && !launch_attn_tc_bwd(a, args->dtype, workspace, st, &e)) e = launch_attn_simt_bwd(a, args->dtype, st);
   return launched(e, "attention backward launch");
 }
 

@@ -70,7 +70,16 @@ struct BwdArgs {
   AttnArgs a;
   int pack, tile_tokens;
   int wide_dq, wide_dk, wide_dv;  // alignment of the gradients' rows, see store_rows
+  // window: the far rows' share of the first keys, see kFar
+  float* far;
+  int chunk, sink_tiles, far_keys;
 };
+
+// What the rows see.  kWindow: a key's rows end with its window, and the sequence's first keys, which all rows see,
+// would meet many times as many as the others.  So their rows behind the window are kFar's, another launch of the
+// dK, dV kernel: a CTA per `chunk` rows, key tile and head leaves its sums in `far` in 32 bits, and the tile's own CTA
+// adds them in order.
+enum Form : int { kPlain = 0, kWindow = 1, kFar = 2 };
 
 template <int DP>
 struct Layout {
@@ -95,7 +104,7 @@ struct DqBars {
   uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], s_free[2], dp_full, dp_read, ds_full[2], done;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_dq_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
                       const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -147,13 +156,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   int lo = 0, hi = t.n;
   mask_range(a, t.batch, t.n, lo, hi);
   const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
-  const int j_lo = lo / kRows;
+  int j_lo = lo / kRows;
   int end = hi;
   if (a.causal) end = min(end, t.first + f.tile_tokens);
-  const int steps = t.first < t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
+  // window: from step `jump` on, `gap` tiles further; those between the first keys and the rows' windows are passed over
+  const int sink_end = WINDOW && a.sinks > 0 ? lo + a.sinks : 0;
+  const int window_lo = WINDOW ? max(lo, t.first - a.window + 1) : lo;  // first key of the first row's window
+  int jump = 1 << 30, gap = 0;
+  if constexpr (WINDOW) {
+    const int sink_tiles = (sink_end + kRows - 1) / kRows;
+    if (a.sinks == 0) j_lo = window_lo / kRows;
+    else if (window_lo / kRows > sink_tiles) jump = sink_tiles - j_lo, gap = window_lo / kRows - sink_tiles;
+  }
+  int steps = (end + kRows - 1) / kRows - j_lo;
+  if (WINDOW && steps > jump) steps = max(jump, steps - gap);
+  steps = t.first < t.n ? max(0, steps) : 0;
+  auto first_key = [&](int j) { return (j_lo + j + (WINDOW && j >= jump ? gap : 0)) * kRows; };
 
   auto key_words = [&](int j, uint32_t (&w)[4]) {
-    const int j0 = (j_lo + j) * kRows;
+    const int j0 = first_key(j);
     tc::first_bits(t.n - j0, w);
     if (mask != nullptr) {
 #pragma unroll
@@ -182,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
         for (int c = 0; c < DP / 64; ++c)
           tc::tma_load_4d(smem + (2 + stage) * L::kTile + c * L::kHalf, (x & 1) ? &vmap : &kmap, &bars.kv_full[stage],
-                          64 * c, hk, static_cast<int>(t.row0) + (j_lo + (x >> 1)) * kRows, t.batch);
+                          64 * c, hk, static_cast<int>(t.row0) + first_key(x >> 1), t.batch);
       }
       issued = x + 1;
     }
@@ -199,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = 0; j < steps && ok; ++j) {
       const uint32_t k = smem + (2 + (2 * j) % NS) * L::kTile, v = smem + (2 + (2 * j + 1) % NS) * L::kTile;
       ok = tc::wait(&bars.kv_full[(2 * j) % NS], ((2 * j) / NS) & 1);
-      if (ok && (mask != nullptr || (j_lo + j + 1) * kRows > t.n)) {
+      if (ok && (mask != nullptr || first_key(j) + kRows > t.n)) {
         uint32_t w[4];
         key_words(j, w);
         if (!tc::all_set(w)) tc::clear_rows<DP / 64>(k, w);
@@ -252,7 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     float norm = 0.f, most = 0.f;
     if constexpr (kHalf) {
       norm = live ? a.g_norm[at] : 0.f;
-      if (steps > 0) most = most_of(a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0, lo, end);
+      if (steps > 0) {
+        const float* norms = a.v_norm + (static_cast<int64_t>(t.batch) * a.Hk + hk) * a.L + t.row0;
+        most = most_of(norms, window_lo, end);
+        if (WINDOW && sink_end > lo) most = fmaxf(most, most_of(norms, lo, min(min(sink_end, window_lo), end)));
+      }
     }
     const float nl = neg_lse2_of(lse);
     const bool none = blind(nl);
@@ -282,8 +307,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after();
       uint32_t s[32], dp[32];
       tc::ld32(s_addr, s);
-      const int j0 = (j_lo + j) * kRows;
-      bool whole = j0 + kRows <= t.n && !any_blind && (!a.causal || j0 + kRows - 1 <= limit_all);
+      const int j0 = first_key(j);
+      bool whole = j0 + kRows <= t.n && !any_blind && (!a.causal || j0 + kRows - 1 <= limit_all) &&
+                   (!WINDOW || j0 > limit_all + 31 / f.pack - a.window || j0 + kRows <= sink_end);
       uint32_t w[4];
       if (mask != nullptr || !whole) {
         key_words(j, w);
@@ -313,8 +339,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!whole) {
         const int left = none ? 0 : limit - j0 - 32 * part + 1;
-        const uint32_t see = (part == 0 ? w[0] : part == 1 ? w[1] : part == 2 ? w[2] : w[3]) &
-                             (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+        uint32_t see = (part == 0 ? w[0] : part == 1 ? w[1] : part == 2 ? w[2] : w[3]) &
+                       (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
+        if constexpr (WINDOW) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - j0 - 32 * part);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
           if (!((see >> e) & 1u)) dp[e] = 0u;
@@ -356,7 +383,7 @@ struct DkvBars {
   uint64_t kv_full, q_full[4], q_empty[4], g_full[4], g_empty[4], stat_full[4], s_full[2], s_free[2], p_full[2], dp_full, dp_free, ds_full[2], done;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int FORM>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_dkv_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap gmap,
                        const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -381,8 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // the first keys of a causal sequence meet the most rows: forwards is heaviest first
-    const SeqTile x = find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false,
-                                a.causal || a.cu != nullptr);
+    const SeqTile x = FORM == kFar ? find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk / f.sink_tiles, f.chunk, false, false)
+                                   : find_tile(a.cu, a.nseq, a.L, a.tiles, blockIdx.x / a.Hk, kRows, false,
+                                               a.causal || a.cu != nullptr);
     if (lane == 0) s_tile = x;
   } else if (warp == kWeightWarps) {
     tc::alloc(&s_tmem, 512);
@@ -411,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const SeqTile t = s_tile;
+  SeqTile t = s_tile;
   const uint32_t tmem = s_tmem;
   // Scores: one buffer of 128 columns at dim 128, where the four accumulators fill tensor memory, two at 64
   constexpr int NB = DP == 64 ? 2 : 1;
@@ -421,10 +449,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   int lo, hi;
   mask_range(a, t.batch, t.n, lo, hi);
   // row tiles that meet these keys, for each block of heads of the group
-  const int i_lo = a.causal ? t.first / f.tile_tokens : 0;
-  const int per_head = max(0, (t.n + f.tile_tokens - 1) / f.tile_tokens - i_lo);
-  const bool some = t.first < min(t.n, hi) && t.first + kRows > lo;  // any valid key
+  int row_from = a.causal ? t.first : 0, row_to = t.n;
+  bool some = t.first < min(t.n, hi) && t.first + kRows > lo;  // any valid key
+  const int sink_end = FORM != kPlain && a.sinks > 0 ? lo + a.sinks : 0;
+  int far_from = 0;  // the first of the far rows of a tile that holds first keys
+  if constexpr (FORM != kPlain) {
+    const int chunk_from = t.first;
+    if constexpr (FORM == kFar) t.first = (lo / kRows + static_cast<int>(blockIdx.x) / a.Hk % f.sink_tiles) * kRows;
+    far_from = (min(t.n, t.first + kRows - 1 + a.window) + f.tile_tokens - 1) / f.tile_tokens * f.tile_tokens;
+    if constexpr (FORM == kFar) {
+      row_from = max(chunk_from, far_from);
+      row_to = min(chunk_from + f.chunk, t.n);
+      some = t.first < min(min(t.n, hi), sink_end) && row_from < row_to;
+    } else {
+      row_to = min(t.n, far_from);
+    }
+  }
+  const int i_lo = row_from / f.tile_tokens;
+  const int per_head = max(0, (row_to + f.tile_tokens - 1) / f.tile_tokens - i_lo);
   const int steps = some ? per_head * (group / f.pack) : 0;
+  // the sums of the far rows of chunk c over the first keys of this tile: dV, then dK, [far_keys][2][DP]
+  auto far_at = [&](int chunk) {
+    const int64_t slot = a.cu != nullptr ? (t.row0 + static_cast<int64_t>(chunk) * f.chunk) / f.chunk + t.row0 / (a.window + kRows)
+                                         : static_cast<int64_t>(t.batch) * ((a.L + f.chunk - 1) / f.chunk) + chunk;
+    return f.far + ((slot * f.sink_tiles + (t.first / kRows - lo / kRows)) * a.Hk + hk) * f.far_keys * 2 * DP;
+  };
   auto head_of = [&](int s) { return hk * group + s / per_head * f.pack; };
   auto first_of = [&](int s) { return (i_lo + s % per_head) * f.tile_tokens; };
 
@@ -507,14 +556,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       // first valid key, which see none and may hold anything.  In both tensors before anything is made of either.
       const int rows = min(t.n - first_of(s), kRows) * f.pack;
       const int blind_rows = a.causal ? min(lo - first_of(s), kRows) * f.pack : 0;
-      if ((a.cu != nullptr && rows < kRows) || blind_rows > 0) {
+      // a window may lie on masked keys alone: such rows are anywhere
+      const bool scattered = FORM != kPlain && mask != nullptr && a.sinks == 0;
+      if ((a.cu != nullptr && rows < kRows) || blind_rows > 0 || scattered) {
         ok = ok && tc::wait(&bars.g_full[s % NS], (s / NS) & 1);
         uint32_t w[4], x[4];
         tc::first_bits(rows, w);
         tc::first_bits(blind_rows, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] &= ~x[i];
-        if (ok) {
+        if (scattered) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = lane + 32 * i, tok = first_of(s) + r / f.pack;
+            w[i] &= __ballot_sync(0xffffffffu, tok < t.n && a.lse[lse_index(a, t, head_of(s) + r % f.pack, tok)] != neg_inf());
+          }
+        }
+        if (ok && !tc::all_set(w)) {
           tc::clear_rows<DP / 64>(q, w);
           tc::clear_rows<DP / 64>(g, w);
         }
@@ -572,17 +630,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (kHalf) {
       float m[3] = {0.f, 0.f, 0.f};
       if (steps > 0) {
-        const int from = a.causal ? max(t.first, lo) : 0;  // rows that see a key
+        const int from = a.causal ? max(row_from, lo) : 0;  // rows that see a key
+        const bool scattered = FORM != kPlain && mask != nullptr && a.sinks == 0;
         // four heads at a time: one after the other, their loads wait for one another (delta, dK and dV of 8 x 1024 tokens,
         // 32/8 heads of 128: 237 us instead of 225)
         for (int h = 0; h < group; h += 4) {
           const int64_t at = lse_index(a, t, hk * group + h, 0);
-          for (int i = from + static_cast<int>(threadIdx.x); i < t.n; i += 32 * kWeightWarps) {
+          for (int i = from + static_cast<int>(threadIdx.x); i < row_to; i += 32 * kWeightWarps) {
             float g[4], d[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               g[x] = h + x < group ? __ldg(a.g_norm + at + x * a.L + i) : 0.f;
               d[x] = h + x < group ? __ldg(a.delta + at + x * a.L + i) : 0.f;
+              // what a row that sees no key holds does not count
+              if (scattered && h + x < group && __ldg(a.lse + at + x * a.L + i) == neg_inf()) g[x] = d[x] = 0.f;
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -619,9 +680,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int from = 0;
       if (a.causal) from = min(max(max(key - first_of(s), -1) * f.pack - part * 32, 0), 32);
       if (!valid) from = 32;
+      // window: one past the last row of this part that sees the key
+      int upto = 32;
+      if (FORM != kPlain && key >= sink_end) upto = min(max(min(max(key + a.window - first_of(s), 0), f.tile_tokens) * f.pack - part * 32, 0), 32);
       const float4* nl = reinterpret_cast<const float4*>(&s_stat[stage][0][part * 32]);
       const float4* dl = reinterpret_cast<const float4*>(&s_stat[stage][1][part * 32]);
-      const bool masked = __any_sync(0xffffffffu, from > 0);
+      const bool masked = __any_sync(0xffffffffu, from > 0 || (FORM != kPlain && upto < 32));
       tc::wait_ld(p);
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
@@ -636,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (masked) {
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-          if (e < from) p[e] = 0u;
+          if (e < from || (FORM != kPlain && e >= upto)) p[e] = 0u;
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) w[e] = tc::pack2<T>(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]));
@@ -671,8 +735,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // dO V^T of a key that is not there may be NaN
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          if (2 * e < from) w[e] &= 0xffff0000u;
-          if (2 * e + 1 < from) w[e] &= 0x0000ffffu;
+          if (2 * e < from || (FORM != kPlain && 2 * e >= upto)) w[e] &= 0xffff0000u;
+          if (2 * e + 1 < from || (FORM != kPlain && 2 * e + 1 >= upto)) w[e] &= 0x0000ffffu;
         }
       }
       tc::st16(kBeside ? s_addr + 16 : d_addr, w);
@@ -688,14 +752,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (t.first < t.n) {
       const bool live = key < t.n;
       const int c0 = (part & 1) * (DP / 2);  // parts 0, 1: dV, parts 2, 3: dK, half of the columns each
-      if (part < 2) {
-        T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
-        tc::store_rows<T, DP / 2>(t_dv + lanes + c0, out, c0, a.d, kHalf ? kHalfUnit : 1.f, live, f.wide_dv, steps > 0);
+      const uint32_t sums = (part < 2 ? t_dv : t_dk) + lanes + c0;
+      const float mul = part < 2 ? (kHalf ? kHalfUnit : 1.f) : (kHalf ? a.scale * pow2(-unit) : a.scale);
+      const bool first_ones = FORM != kPlain && key >= lo && key < sink_end;
+      const int at = (key - max(t.first, lo)) * 2 * DP + (part < 2 ? 0 : DP) + c0;  // in far_at's
+      if constexpr (FORM == kFar) {
+        if (steps > 0) {
+          float* to = far_at(row_from / f.chunk) + at;
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[16];
+            tc::ld16(sums + 16 * c, o);
+            tc::wait_ld(o);
+            if (first_ones) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<float4*>(to + 16 * c + e) =
+                    make_float4(__uint_as_float(o[e]) * mul, __uint_as_float(o[e + 1]) * mul, __uint_as_float(o[e + 2]) * mul,
+                                __uint_as_float(o[e + 3]) * mul);
+            }
+          }
+        }
       } else {
-        T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
-        tc::store_rows<T, DP / 2>(t_dk + lanes + c0, out, c0, a.d, kHalf ? a.scale * pow2(-unit) : a.scale, live, f.wide_dk, steps > 0);
+        if (FORM == kWindow && steps > 0 && t.first < sink_end && far_from < t.n) {
+          pdl_wait();  // for the far rows' CTAs
+          if (__any_sync(0xffffffffu, first_ones)) {
+            const float back = 1.f / mul;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[16];
+              tc::ld16(sums + 16 * c, o);
+              tc::wait_ld(o);
+              if (first_ones) {
+                for (int chunk = far_from / f.chunk; chunk * f.chunk < t.n; ++chunk) {
+                  const float4* x = reinterpret_cast<const float4*>(far_at(chunk) + at + 16 * c);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const float4 y = __ldcg(x + e);  // written while this kernel may already be there
+                    o[4 * e] = __float_as_uint(fmaf(y.x, back, __uint_as_float(o[4 * e])));
+                    o[4 * e + 1] = __float_as_uint(fmaf(y.y, back, __uint_as_float(o[4 * e + 1])));
+                    o[4 * e + 2] = __float_as_uint(fmaf(y.z, back, __uint_as_float(o[4 * e + 2])));
+                    o[4 * e + 3] = __float_as_uint(fmaf(y.w, back, __uint_as_float(o[4 * e + 3])));
+                  }
+                }
+              }
+              __syncwarp();
+              tc::st16(sums + 16 * c, o);
+            }
+            tc::wait_st();
+          }
+        }
+        if (part < 2) {
+          T* out = static_cast<T*>(a.dv) + t.batch * a.dvs.b + (t.row0 + key) * a.dvs.t + hk * a.dvs.h;
+          tc::store_rows<T, DP / 2>(sums, out, c0, a.d, mul, live, f.wide_dv, steps > 0);
+        } else {
+          T* out = static_cast<T*>(a.dk) + t.batch * a.dks.b + (t.row0 + key) * a.dks.t + hk * a.dks.h;
+          tc::store_rows<T, DP / 2>(sums, out, c0, a.d, mul, live, f.wide_dk, steps > 0);
+        }
       }
-    } else if (a.cu != nullptr && t.n == 0 && part < 2) {
+    } else if (FORM != kFar && a.cu != nullptr && t.n == 0 && part < 2) {
       T* base = static_cast<T*>(part == 0 ? a.dv : a.dk) + hk * (part == 0 ? a.dvs.h : a.dks.h);
       const int64_t st = part == 0 ? a.dvs.t : a.dks.t;
       for (int64_t r = t.row0 + t.tail_index; r < a.L; r += t.tail_count)
@@ -706,6 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
+  if (FORM == kWindow) pdl_wait();  // launched beside the far rows' CTAs; dQ's wait for this kernel's end covers theirs
 }
 
 int64_t count_tiles(AttnArgs& a, int rows) {
@@ -717,24 +833,55 @@ int64_t count_tiles(AttnArgs& a, int rows) {
   return static_cast<int64_t>(a.tiles) * a.nseq;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool WINDOW>
 cudaError_t run(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k, const CUtensorMap& v, BwdArgs f,
                 cudaStream_t st) {
   if (f.a.dk != nullptr) {
+    if constexpr (WINDOW) {
+      if (f.far != nullptr) {
+        const int64_t tiles = count_tiles(f.a, f.chunk);
+        const cudaError_t e = launch_grid<attn_tc_dkv_kernel<T, DP, kFar>>(false, tiles * f.sink_tiles * f.a.Hk, kThreads,
+                                                                           Layout<DP>::kSmemKv, st, q, g, k, v, f);
+        if (e != cudaSuccess) return e;
+      }
+    }
     const int64_t tiles = count_tiles(f.a, kRows);
-    const cudaError_t e =
-        launch_grid<attn_tc_dkv_kernel<T, DP>>(false, tiles * f.a.Hk, kThreads, Layout<DP>::kSmemKv, st, q, g, k, v, f);
+    const cudaError_t e = launch_grid<attn_tc_dkv_kernel<T, DP, WINDOW ? kWindow : kPlain>>(
+        f.far != nullptr, tiles * f.a.Hk, kThreads, Layout<DP>::kSmemKv, st, q, g, k, v, f);
     if (e != cudaSuccess) return e;
   }
   if (f.a.dq == nullptr) return cudaSuccess;
   const int64_t tiles = count_tiles(f.a, f.tile_tokens);
-  return launch_grid<attn_tc_dq_kernel<T, DP>>(f.a.dk != nullptr, tiles * (f.a.H / f.pack), kThreads, Layout<DP>::kSmem,
-                                               st, q, g, k, v, f);
+  return launch_grid<attn_tc_dq_kernel<T, DP, WINDOW>>(f.a.dk != nullptr, tiles * (f.a.H / f.pack), kThreads,
+                                                       Layout<DP>::kSmem, st, q, g, k, v, f);
+}
+
+template <typename T>
+cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k, const CUtensorMap& v, const BwdArgs& f,
+                     cudaStream_t st) {
+  if (f.a.window > 0) return f.a.d <= 64 ? run<T, 64, true>(q, g, k, v, f, st) : run<T, 128, true>(q, g, k, v, f, st);
+  return f.a.d <= 64 ? run<T, 64, false>(q, g, k, v, f, st) : run<T, 128, false>(q, g, k, v, f, st);
+}
+
+int far_sink_tiles(const AttnArgs& a) { return a.mask != nullptr ? (a.sinks + kRows - 2) / kRows + 1 : (a.sinks + kRows - 1) / kRows; }
+int64_t far_bytes_of(const AttnArgs& a, int64_t chunk) {
+  // packed: a sequence has far rows only if it is at least window + kRows long, which tells them apart
+  const int64_t slots = a.cu != nullptr ? (a.L / chunk + 1) + (a.L / (a.window + kRows) + 1)
+                                        : a.nseq * ((a.L + chunk - 1) / chunk);
+  return slots * far_sink_tiles(a) * a.Hk * std::min(a.sinks, kRows) * 2 * (a.d <= 64 ? 64 : 128) * static_cast<int64_t>(sizeof(float));
+}
+// Rows of a far CTA: about as many as the others' windows; more where there would be more than 64 parts in a row, or
+// more than 256 MB of them.
+int far_chunk(const AttnArgs& a) {
+  int64_t rows = std::max<int64_t>(std::max<int64_t>(a.window + kRows, 512), (a.L + 63) / 64);
+  rows = (rows + kRows - 1) / kRows * kRows;
+  while (rows < a.L && far_bytes_of(a, rows) > (256LL << 20)) rows *= 2;
+  return static_cast<int>(rows);
 }
 
 }  // namespace
 
-bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e) {
+bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, void* far, cudaStream_t st, cudaError_t* e) {
   if (dtype == kF32 || a.d % 8 != 0 || a.d > 128 || !(a.scale > 0.f) || (dtype == kF16 && a.g_norm == nullptr)) return false;
   BwdArgs f = {};
   f.a = a;
@@ -750,11 +897,20 @@ bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   f.wide_dq = row_alignment(a.dq, a.dqs, nb, a.H);
   f.wide_dk = row_alignment(a.dk, a.dks, nb, a.Hk);
   f.wide_dv = row_alignment(a.dv, a.dvs, nb, a.Hk);
-  if (dtype == kBF16)
-    *e = a.d <= 64 ? run<__nv_bfloat16, 64>(q, g, k, v, f, st) : run<__nv_bfloat16, 128>(q, g, k, v, f, st);
-  else
-    *e = a.d <= 64 ? run<__half, 64>(q, g, k, v, f, st) : run<__half, 128>(q, g, k, v, f, st);
+  if (far_bytes(a, dtype) > 0 && a.dk != nullptr) {
+    f.far = static_cast<float*>(far);
+    f.chunk = far_chunk(a);
+    f.sink_tiles = far_sink_tiles(a);
+    f.far_keys = std::min(a.sinks, kRows);
+  }
+  *e = dtype == kBF16 ? dispatch<__nv_bfloat16>(q, g, k, v, f, st) : dispatch<__half>(q, g, k, v, f, st);
   return true;
+}
+
+int64_t far_bytes(const AttnArgs& a, int dtype) {
+  // no row lies behind the window of a whole tile
+  if (a.window == 0 || a.sinks == 0 || a.L < a.window + kRows || dtype == kF32 || a.d % 8 != 0 || a.d > 128) return 0;
+  return far_bytes_of(a, far_chunk(a));
 }
 
 int read_device_error_tc_bwd(int clear) {
