@@ -318,6 +318,76 @@ int64_t split_bytes(int workers, int d) {
   return 2LL * workers * 16 * ((d <= 64 ? 64 : 128) + 4) * static_cast<int64_t>(sizeof(float));
 }
 
+// The arguments' pointers and the workspace.
+int paged_pointers(const PagedArgs& a, int quantized, const void* workspace, int64_t workspace_bytes, int64_t need) {
+  // a pool without pages and a table without entries have no address
+  if (a.q == nullptr || a.o == nullptr || (a.n_pages > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
+      (a.table == nullptr && a.table_width > 0) || a.seq_lens == nullptr)
+    return fail(CTA_EINVAL, "null tensor pointer");
+  const int64_t cells = quantized ? 16 : 8;
+  for (int64_t s : {a.q_sT, a.q_sH, a.o_sT, a.o_sH})
+    if (s % 8 != 0) return fail(CTA_EINVAL, "rows must start on 16 bytes");
+  for (int64_t s : {a.kc_sP, a.kc_sS, a.kc_sH, a.vc_sP, a.vc_sS, a.vc_sH})
+    if (s % cells != 0) return fail(CTA_EINVAL, "the cache's rows must start on 16 bytes");
+  for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, workspace})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
+  return CTA_OK;
+}
+
+// Expands the pages of an e4m3 cache that p's table names into `ws`, and points x at them.
+cudaError_t expand_pages(const PagedArgs& p, int dtype, char* ws, PagedArgs& x, cudaStream_t st) {
+  const int64_t pages = static_cast<int64_t>(p.B) * p.table_width, part = pages * p.page * p.Hk * p.d * 2;
+  float* k_res = reinterpret_cast<float*>(ws + 2 * part);
+  float* v_res = k_res + p.B * residue_row(static_cast<int64_t>(p.table_width) * p.page) * p.Hk;
+  const cudaError_t e = launch_cache_expand(p, dtype, ws, ws + part, k_res, v_res, st);
+  x.k_cache = ws;
+  x.v_cache = ws + part;
+  x.k_res = k_res;
+  x.v_res = v_res;
+  x.expanded_pages = pages;
+  return e;
+}
+
+// The plan of a batch with a shared prefix: the prefix in parts on the tensor cores, 256 (row, head) pairs at once, then
+// the sequences' own keys in the split kernel, whose join takes the parts in.
+struct PrefixPlan {
+  int keys = 0;  // 0: the prefix is not used
+  int splits = 0, chunk = 0;
+  int64_t sums = 0, expanded = 0, bytes = 0;  // workspace: the parts, the expanded pages, all with the split kernel's
+};
+
+PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t shared) {
+  PrefixPlan p;
+  const int64_t width = a.table_width, keys = std::min(shared / a.page, width) * a.page;
+  // the split kernel counts groups past the last key, hence 2^30
+  if (a.T < 2 || keys < 1 || width * a.page >= (1LL << 30) || !(a.scale > 0.f) || !tma_can_address(a) || tensor_cores_pay(a) ||
+      a.n_pages < 1)
+    return p;
+  const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
+  // one wave of CTAs, one per SM
+  const int64_t per = (tiles + std::max<int64_t>(1, 148 / ctas) - 1) / std::max<int64_t>(1, 148 / ctas);
+  const int64_t splits = (tiles + per - 1) / per;
+  const int dp = a.d <= 64 ? 64 : 128;
+  const int64_t sums = splits * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));
+  int64_t expanded = 0;
+  if (quantized) {
+    expanded = expanded_bytes(1, keys / a.page, a.page, a.Hk, a.d);
+    if (expanded == 0) return p;
+  }
+  if (sums > (1LL << 30)) return p;
+  PagedArgs x = a;
+  x.skip = static_cast<int>(keys);
+  p.keys = x.skip;
+  p.splits = static_cast<int>(splits);
+  p.chunk = static_cast<int>(per * 128);
+  p.sums = sums;
+  p.expanded = expanded;
+  p.bytes = sums + expanded + split_bytes(paged_split_workers(x, dtype, quantized), a.d);
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -467,21 +537,10 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
   const int rc = paged_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc;
   if (a.T == 0 || a.B == 0) return CTA_OK;
-  // a pool without pages and a table without entries have no address
-  if (a.q == nullptr || a.o == nullptr || (a.n_pages > 0 && (a.k_cache == nullptr || a.v_cache == nullptr)) ||
-      (a.table == nullptr && a.table_width > 0) || a.seq_lens == nullptr)
-    return fail(CTA_EINVAL, "null tensor pointer");
-  const int64_t cells = args->quantized ? 16 : 8;
-  for (int64_t s : {a.q_sT, a.q_sH, a.o_sT, a.o_sH})
-    if (s % 8 != 0) return fail(CTA_EINVAL, "rows must start on 16 bytes");
-  for (int64_t s : {a.kc_sP, a.kc_sS, a.kc_sH, a.vc_sP, a.vc_sS, a.vc_sH})
-    if (s % cells != 0) return fail(CTA_EINVAL, "the cache's rows must start on 16 bytes");
-  for (const void* x : {a.q, static_cast<const void*>(a.o), a.k_cache, a.v_cache, static_cast<const void*>(workspace)})
-    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(CTA_EINVAL, "tensors must start on 16 bytes");
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t need = cta_window_paged_attention_workspace_bytes(args, window, sinks);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-    return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
+  const int prc = paged_pointers(a, args->quantized, workspace, workspace_bytes, need);
+  if (prc != CTA_OK) return prc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (tensor_cores_pay(a)) {
     const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
@@ -491,18 +550,8 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
     }
     if (bytes > 0) {
       PagedArgs x = a;
-      char* k = static_cast<char*>(workspace);
-      const int64_t part = static_cast<int64_t>(a.B) * a.table_width * a.page * a.Hk * a.d * 2;
-      char* v = k + part;
-      float* k_res = reinterpret_cast<float*>(v + part);
-      float* v_res = k_res + a.B * residue_row(static_cast<int64_t>(a.table_width) * a.page) * a.Hk;
-      e = launch_cache_expand(a, args->dtype, k, v, k_res, v_res, st);
+      e = expand_pages(a, args->dtype, static_cast<char*>(workspace), x, st);
       if (e != cudaSuccess) return launched(e, "paged attention launch");
-      x.k_cache = k;
-      x.v_cache = v;
-      x.k_res = k_res;
-      x.v_res = v_res;
-      x.expanded_pages = static_cast<int64_t>(a.B) * a.table_width;
       if (launch_paged_tc(x, args->dtype, st, &e)) return launched(e, "paged attention launch");
       return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");
     }
@@ -515,13 +564,52 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
 
 int64_t cta_prefix_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t shared_prefix) {
   if (shared_prefix < 0) return -fail(CTA_EINVAL, "shared_prefix must not be negative");
-  return cta_window_paged_attention_workspace_bytes(args, 0, 0);
+  PagedArgs a;
+  const int rc = paged_window(args, 0, 0, a);
+  if (rc != CTA_OK) return -rc;
+  const PrefixPlan p = prefix_plan(a, args->dtype, args->quantized, shared_prefix);
+  return p.keys > 0 ? p.bytes : cta_window_paged_attention_workspace_bytes(args, 0, 0);
 }
 
 int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t shared_prefix, void* workspace,
                                int64_t workspace_bytes, void* stream) {
   if (shared_prefix < 0) return fail(CTA_EINVAL, "shared_prefix must not be negative");
-  return cta_window_paged_attention(args, 0, 0, workspace, workspace_bytes, stream);
+  PagedArgs a;
+  const int rc = paged_window(args, 0, 0, a);
+  if (rc != CTA_OK) return rc;
+  const PrefixPlan p = prefix_plan(a, args->dtype, args->quantized, shared_prefix);
+  if (p.keys == 0) return cta_window_paged_attention(args, 0, 0, workspace, workspace_bytes, stream);
+  if (a.T == 0 || a.B == 0) return CTA_OK;
+  const int prc = paged_pointers(a, args->quantized, workspace, workspace_bytes, p.bytes);
+  if (prc != CTA_OK) return prc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const int64_t pairs = static_cast<int64_t>(p.splits) * a.T * a.H;
+  a.skip = p.keys;
+  a.prefix_splits = p.splits;
+  a.prefix_chunk = p.chunk;
+  a.prefix_ml = reinterpret_cast<float*>(ws);
+  a.prefix_o = a.prefix_ml + pairs * 4;
+  cudaError_t e = cudaSuccess;
+  PagedArgs x = a;
+  x.k_scale = x.v_scale = nullptr;
+  if (args->quantized) {
+    // the first row's pages, all of them
+    PagedArgs one = a;
+    one.B = 1;
+    one.table_width = p.keys / a.page;
+    one.seq_lens = nullptr;
+    one.skip = 0;
+    e = expand_pages(one, args->dtype, ws + p.sums, x, st);
+    if (e != cudaSuccess) return launched(e, "paged attention launch");
+  }
+  if (!launch_prefix_tc(x, args->dtype, st, &e))
+    return fail(CTA_EUNSUPPORTED, "paged attention behind a shared prefix: the tensors cannot be addressed by TMA");
+  if (e != cudaSuccess) return launched(e, "paged attention launch");
+  a.workers = paged_split_workers(a, args->dtype, args->quantized);
+  a.part_ml = reinterpret_cast<float*>(ws + p.sums + p.expanded);
+  a.part_o = a.part_ml + 2LL * a.workers * 16 * 4;
+  return launched(launch_paged_split(a, args->dtype, args->quantized, st), "paged attention launch");
 }
 
 }  // extern "C"

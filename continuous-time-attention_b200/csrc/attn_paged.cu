@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
 
     // this run's share of the segment
     const bool whole = count == g.groups;
+    const bool prefix = CUT && a.prefix_splits > 0;
     const int64_t part = 2 * static_cast<int64_t>(worker) + (first ? 0 : 1);
 #pragma unroll
     for (int r = 0; r < NR; ++r)
@@ -572,6 +573,41 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
         const int i = g.tile * ROWS + row, tok = i / group;
         if (tok >= g.rows) continue;
         if (whole) {
+          if (CUT && prefix) {
+            // the keys that all sequences begin with: a part for each run of them, as in the join
+            const int64_t at = (g.row0 + tok) * a.H + hk * group + i - tok * group, step = a.T * a.H;
+            const float4* ml = reinterpret_cast<const float4*>(a.prefix_ml) + at;
+            float top = m[r][e], topv = mv[r][e];
+            for (int x = 0; x < a.prefix_splits; ++x) {
+              const float4 y = __ldg(ml + x * step);
+              top = fmaxf(top, y.x);
+              topv = fmaxf(topv, y.z);
+            }
+            const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
+            sum *= ex2(m[r][e] - base);
+            const float mine = ex2(mv[r][e] - basev);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) o[t][r][e] *= mine, o[t][r][2 + e] *= mine;
+            for (int x = 0; x < a.prefix_splits; ++x) {
+              const float4 y = __ldg(ml + x * step);
+              sum += y.y * ex2(y.x - base);
+              const float theirs = ex2(y.z - basev);
+              const float* po = a.prefix_o + (at + x * step) * DP + VE * oct;
+#pragma unroll
+              for (int z = 0; z < VL; ++z)
+#pragma unroll
+                for (int j = 0; j < VE / 2; j += 2) {
+                  const int t = z * VE / 2 + j;
+                  const float4 v = __ldg(reinterpret_cast<const float4*>(po + 8 * VE * z + 2 * j));
+                  o[t][r][e] = fmaf(v.x, theirs, o[t][r][e]);
+                  o[t][r][2 + e] = fmaf(v.y, theirs, o[t][r][2 + e]);
+                  o[t + 1][r][e] = fmaf(v.z, theirs, o[t + 1][r][e]);
+                  o[t + 1][r][2 + e] = fmaf(v.w, theirs, o[t + 1][r][2 + e]);
+                }
+            }
+            m[r][e] = base;
+            mv[r][e] = basev;
+          }
           float mul = 0.f;
           if (sum > 0.f || sum != sum) mul = __fdividef(ex2((FP8 ? mv[r][e] - m[r][e] : 0.f) - kShift), sum);
           T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (hk * group + i - tok * group) * a.o_sH;
@@ -649,7 +685,7 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   const int64_t workers = active_shares(a, units);
   const int64_t w0 = ((u0 + 1) * workers - 1) / units, w1 = (u1 * workers - 1) / units;
   if (w0 == w1) return;  // one worker held it all and wrote the output
-  const int parts = static_cast<int>(w1 - w0 + 1);
+  const int own = static_cast<int>(w1 - w0 + 1), parts = own + (CUT ? a.prefix_splits : 0);
   auto slot_of = [&](int x) -> int64_t {
     const int64_t w = w0 + x;
     return 2 * (w * a.Hk + hk) + (x == 0 && units * w / workers < u0 ? 1 : 0);
@@ -660,12 +696,14 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   for (int e = 0; e < V; ++e) o[e] = 0.f;
 #pragma unroll 4
   for (int x = warp; x < parts; x += warps) {
-    const int64_t at = slot_of(x) * kPartRows + r;
+    const bool shared = CUT && x >= own;
+    const int64_t at = shared ? ((x - own) * a.T + row) * a.H + h : slot_of(x) * kPartRows + r;
+    const float* part_o = shared ? a.prefix_o : a.part_o;
     // ordinary loads: the parts are written while this kernel may already be there
-    const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml + at * 4));
+    const float4 ml = __ldcg(reinterpret_cast<const float4*>(shared ? a.prefix_ml : a.part_ml) + at);
     float po[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) po[e] = __ldcg(a.part_o + at * DP + lane + 32 * e);
+    for (int e = 0; e < V; ++e) po[e] = __ldcg(part_o + at * DP + lane + 32 * e);
     const float top = fmaxf(m, ml.x), topv = fmaxf(mv, ml.z);
     const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
     l = l * ex2(m - base) + ml.y * ex2(ml.x - base);
@@ -722,7 +760,7 @@ struct Split {
     if (e != cudaSuccess) return e;
     // about as many warps as a segment has parts when all are equally long
     const int64_t segments = static_cast<int64_t>(a.B) * a.Hk;
-    const int64_t parts = a.workers / (segments > 0 ? segments : 1) + 2;
+    const int64_t parts = a.workers / (segments > 0 ? segments : 1) + 2 + (CUT ? a.prefix_splits : 0);
     const int warps = parts <= 4 ? 2 : parts <= 16 ? 4 : parts <= 64 ? 8 : kMaxJoinWarps;
     if (a.T * a.H > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};

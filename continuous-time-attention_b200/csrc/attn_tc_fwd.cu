@@ -78,6 +78,7 @@ struct FwdArgs {
   // shared prefix: `splits` parts of `chunk` keys (whole tiles), whose sums go to part_o [splits, rows, heads, DP] and
   // part_ml [splits, rows, heads, 4] as the split kernel leaves them (attn_paged.cu)
   int splits, chunk, prefix;
+  int64_t most_keys;  // of a sequence
   float* part_o;
   float* part_ml;
 };
@@ -125,8 +126,7 @@ __device__ __forceinline__ int last_key(const FwdArgs& f, int tok) {
     clamp_range(a.cu, b, a.L, begin, rows);
     from = static_cast<int>(begin);
   }
-  const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
-  const int n = static_cast<int>(min(static_cast<int64_t>(max(__ldg(f.seq_lens + b), 0)), most));
+  const int n = static_cast<int>(min(static_cast<int64_t>(max(__ldg(f.seq_lens + b), 0)), f.most_keys));
   return n - rows + tok - from;
 }
 
@@ -282,22 +282,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           x.t.n = static_cast<int>(a.L);
           x.t.first = y / f.splits * 2 * f.tile_tokens;
           x.lo = part * f.chunk;
-          x.n = x.hi = min(f.prefix, x.lo + f.chunk);
+          // what lies behind the longest sequence may hold anything
+          int longest = 0;
+          for (int b = lane; b < a.nseq; b += 32) longest = max(longest, __ldg(f.seq_lens + b));
+          longest = __reduce_max_sync(0xffffffffu, longest);
+          x.n = x.hi = min(min(f.prefix, x.lo + f.chunk), longest);
         } else {
-        x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
-                        f.seq_lens);
-        x.n = x.hi = x.t.n;
-        if constexpr (PAGED) {
-          if (x.t.first < x.t.n) {
-            x.n = __ldg(f.seq_lens + x.t.seq);
-            const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
-            if ((x.n < 0 || x.n > most) && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
-            x.n = x.n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(x.n), most));
+          x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
+                          f.seq_lens);
+          x.n = x.hi = x.t.n;
+          if constexpr (PAGED) {
+            if (x.t.first < x.t.n) {
+              x.n = __ldg(f.seq_lens + x.t.seq);
+              const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
+              if ((x.n < 0 || x.n > most) && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
+              x.n = x.n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(x.n), most));
+            }
+            x.hi = x.n;
+          } else {
+            mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
           }
-          x.hi = x.n;
-        } else {
-          mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
-        }
         }
       }
       if (lane == 0) {
@@ -699,9 +703,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* to = f.part_o + at * DP + half * (DP / 2);
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[16];
-          tc::ld16(o_addr + 16 * c, o);
-          tc::wait_ld(o);
+          uint32_t o[16] = {};
+          if (count > 0) {  // a part behind all sequences has no keys
+            tc::ld16(o_addr + 16 * c, o);
+            tc::wait_ld(o);
+          }
           if (live) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -865,6 +871,8 @@ bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_
   f.splits = p.prefix_splits;
   f.chunk = p.prefix_chunk;
   f.prefix = p.skip;
+  f.table_width = p.skip / p.page;
+  f.most_keys = static_cast<int64_t>(p.table_width) * p.page;
   f.part_o = p.prefix_o;
   f.part_ml = p.prefix_ml;
   const int64_t pieces = prefix_tiles(p) * f.splits;

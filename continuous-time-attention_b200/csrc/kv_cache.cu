@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
     for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i)
       for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
   if (c >= a.d) return;
-  const int n = __ldg(a.seq_lens + b);
+  const int n = a.seq_lens != nullptr ? __ldg(a.seq_lens + b) : 0x7fffffff;  // nullptr: all of the table
   bool there = n >= 0 && j < static_cast<unsigned>(n);
   if (a.window > 0) {
     // Left out where no row's window reaches, but for boxes that the reader loads whole: what lies beside a key that
