@@ -125,8 +125,8 @@ struct PagedArgs {
   int64_t expanded_pages;
   // shared prefix of `skip` keys: its sums over prefix_splits parts of prefix_chunk keys, for every row of q
   int prefix_splits, prefix_chunk;
-  float* prefix_o;   // [splits, T, H, dim rounded up to 64 or 128] fp32
-  float* prefix_ml;  // [splits, T, H, 4] as part_ml
+  float* prefix_o;   // [splits + 1, T, H, dim rounded up to 64 or 128] fp32; last: a row's own keys, if one worker had them
+  float* prefix_ml;  // [splits + 1, T, H, 4] as part_ml
 };
 
 // workers (warps) of the split kernel on the current device, and its launch

@@ -370,7 +370,7 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
   const int64_t per = (tiles + std::max<int64_t>(1, 148 / ctas) - 1) / std::max<int64_t>(1, 148 / ctas);
   const int64_t splits = (tiles + per - 1) / per;
   const int dp = a.d <= 64 ? 64 : 128;
-  const int64_t sums = splits * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));
+  const int64_t sums = (splits + 1) * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));
   int64_t expanded = 0;
   if (quantized) {
     expanded = expanded_bytes(1, keys / a.page, a.page, a.Hk, a.d);
@@ -584,7 +584,7 @@ int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t sha
   if (prc != CTA_OK) return prc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  const int64_t pairs = static_cast<int64_t>(p.splits) * a.T * a.H;
+  const int64_t pairs = (p.splits + 1LL) * a.T * a.H;
   a.skip = p.keys;
   a.prefix_splits = p.splits;
   a.prefix_chunk = p.chunk;

@@ -224,12 +224,11 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
   const int lane = threadIdx.x & 31, quad = lane & 3, oct = lane >> 2;
   const int worker = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const int64_t units = total_units<CUT>(a, ROWS);
-  if (units == 0) return;
   const int shares = active_shares(a, units);
   const int hk = worker % a.Hk, share = worker / a.Hk;
-  if (share >= shares) return;
+  if (!CUT && (units == 0 || share >= shares)) return;
   int64_t u = units * share / shares;
-  const int64_t u_end = units * (share + 1) / shares;
+  const int64_t u_end = share < shares ? units * (share + 1) / shares : u;  // none for the workers left over
   bool first = true;
   const int group = a.H / a.Hk;
 
@@ -560,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
 
     // this run's share of the segment
     const bool whole = count == g.groups;
-    const bool prefix = CUT && a.prefix_splits > 0;
+    const bool prefix = CUT && a.prefix_splits > 0;  // the join has more to add, to whole segments too
     const int64_t part = 2 * static_cast<int64_t>(worker) + (first ? 0 : 1);
 #pragma unroll
     for (int r = 0; r < NR; ++r)
@@ -572,42 +571,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
         const int row = 8 * r + 2 * quad + e;
         const int i = g.tile * ROWS + row, tok = i / group;
         if (tok >= g.rows) continue;
-        if (whole) {
-          if (CUT && prefix) {
-            // the keys that all sequences begin with: a part for each run of them, as in the join
-            const int64_t at = (g.row0 + tok) * a.H + hk * group + i - tok * group, step = a.T * a.H;
-            const float4* ml = reinterpret_cast<const float4*>(a.prefix_ml) + at;
-            float top = m[r][e], topv = mv[r][e];
-            for (int x = 0; x < a.prefix_splits; ++x) {
-              const float4 y = __ldg(ml + x * step);
-              top = fmaxf(top, y.x);
-              topv = fmaxf(topv, y.z);
-            }
-            const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
-            sum *= ex2(m[r][e] - base);
-            const float mine = ex2(mv[r][e] - basev);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) o[t][r][e] *= mine, o[t][r][2 + e] *= mine;
-            for (int x = 0; x < a.prefix_splits; ++x) {
-              const float4 y = __ldg(ml + x * step);
-              sum += y.y * ex2(y.x - base);
-              const float theirs = ex2(y.z - basev);
-              const float* po = a.prefix_o + (at + x * step) * DP + VE * oct;
-#pragma unroll
-              for (int z = 0; z < VL; ++z)
-#pragma unroll
-                for (int j = 0; j < VE / 2; j += 2) {
-                  const int t = z * VE / 2 + j;
-                  const float4 v = __ldg(reinterpret_cast<const float4*>(po + 8 * VE * z + 2 * j));
-                  o[t][r][e] = fmaf(v.x, theirs, o[t][r][e]);
-                  o[t][r][2 + e] = fmaf(v.y, theirs, o[t][r][2 + e]);
-                  o[t + 1][r][e] = fmaf(v.z, theirs, o[t + 1][r][e]);
-                  o[t + 1][r][2 + e] = fmaf(v.w, theirs, o[t + 1][r][2 + e]);
-                }
-            }
-            m[r][e] = base;
-            mv[r][e] = basev;
-          }
+        if (whole && !prefix) {
           float mul = 0.f;
           if (sum > 0.f || sum != sum) mul = __fdividef(ex2((FP8 ? mv[r][e] - m[r][e] : 0.f) - kShift), sum);
           T* out = static_cast<T*>(a.o) + (g.row0 + tok) * a.o_sT + (hk * group + i - tok * group) * a.o_sH;
@@ -627,7 +591,10 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
             }
           }
         } else {
-          float* po = a.part_o + (part * kPartRows + row) * DP;
+          // a worker has two segments in part, and any number whole: those lie behind the prefix's parts
+          const int64_t pair = (a.prefix_splits * a.T + g.row0 + tok) * a.H + hk * group + i - tok * group;
+          float* po = CUT && prefix && whole ? a.prefix_o + pair * DP : a.part_o + (part * kPartRows + row) * DP;
+          float* ml = CUT && prefix && whole ? a.prefix_ml + pair * 4 : a.part_ml + (part * kPartRows + row) * 4;
 #pragma unroll
           for (int x = 0; x < VL; ++x)
 #pragma unroll
@@ -637,12 +604,13 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
                   make_float4(o[t][r][e], o[t][r][2 + e], o[t + 1][r][e], o[t + 1][r][2 + e]);
             }
           if (oct == 0)
-            *reinterpret_cast<float4*>(a.part_ml + (part * kPartRows + row) * 4) = make_float4(m[r][e], sum, mv[r][e], 0.f);
+            *reinterpret_cast<float4*>(ml) = make_float4(m[r][e], sum, mv[r][e], 0.f);
         }
       }
     u += count;
     first = false;
   }
+  if (CUT) pdl_wait();  // launched beside the prefix's sums; the join's wait for this kernel's end covers theirs
 }
 
 // Joins the parts of one (row, head): the warps of the CTA take the parts in turn, then join theirs in order.
@@ -684,8 +652,10 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   const int64_t u0 = before + static_cast<int64_t>(tile) * s.groups, u1 = u0 + s.groups;
   const int64_t workers = active_shares(a, units);
   const int64_t w0 = ((u0 + 1) * workers - 1) / units, w1 = (u1 * workers - 1) / units;
-  if (w0 == w1) return;  // one worker held it all and wrote the output
-  const int own = static_cast<int>(w1 - w0 + 1), parts = own + (CUT ? a.prefix_splits : 0);
+  const bool prefix = CUT && a.prefix_splits > 0;
+  if (w0 == w1 && !prefix) return;  // one worker held it all and wrote the output
+  // prefix: its parts, and behind them the rest if one worker held that
+  const int own = w0 == w1 ? 0 : static_cast<int>(w1 - w0 + 1), parts = own + (prefix ? a.prefix_splits + (w0 == w1) : 0);
   auto slot_of = [&](int x) -> int64_t {
     const int64_t w = w0 + x;
     return 2 * (w * a.Hk + hk) + (x == 0 && units * w / workers < u0 ? 1 : 0);
@@ -754,9 +724,8 @@ struct Split {
   }
   static cudaError_t run(const PagedArgs& a, cudaStream_t st) {
     constexpr bool kHalf = FP8 || std::is_same<T, __half>::value;
-    paged_split_kernel<T, FP8, DP, ROWS, CUT>
-        <<<static_cast<unsigned>((a.workers + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
-    cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_grid<paged_split_kernel<T, FP8, DP, ROWS, CUT>>(
+        CUT && a.prefix_splits > 0, (a.workers + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st, a);
     if (e != cudaSuccess) return e;
     // about as many warps as a segment has parts when all are equally long
     const int64_t segments = static_cast<int64_t>(a.B) * a.Hk;

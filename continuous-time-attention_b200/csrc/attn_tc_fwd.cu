@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  if (FORM == kPrefix) pdl_launch_dependents();  // the split kernel's CTAs, for the sequences' own keys, may follow
 
   if (warp == kSoftmaxWarps) {
     tc::alloc(&s_tmem, 512);
