@@ -370,7 +370,8 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
   const int64_t per = (tiles + std::max<int64_t>(1, 148 / ctas) - 1) / std::max<int64_t>(1, 148 / ctas);
   const int64_t splits = (tiles + per - 1) / per;
   const int dp = a.d <= 64 ? 64 : 128;
-  const int64_t sums = (splits + 1) * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));
+  // the values' rows start on 32 bytes, the workspace on 16
+  const int64_t sums = 32 + (splits + 1) * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));
   int64_t expanded = 0;
   if (quantized) {
     expanded = expanded_bytes(1, keys / a.page, a.page, a.Hk, a.d);
@@ -588,8 +589,8 @@ int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t sha
   a.skip = p.keys;
   a.prefix_splits = p.splits;
   a.prefix_chunk = p.chunk;
-  a.prefix_ml = reinterpret_cast<float*>(ws);
-  a.prefix_o = a.prefix_ml + pairs * 4;
+  a.prefix_o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws) + 31) & ~static_cast<uintptr_t>(31));
+  a.prefix_ml = a.prefix_o + pairs * (a.d <= 64 ? 64 : 128);
   cudaError_t e = cudaSuccess;
   PagedArgs x = a;
   x.k_scale = x.v_scale = nullptr;

@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
 // Joins the parts of one (row, head): the warps of the CTA take the parts in turn, then join theirs in order.
 constexpr int kMaxJoinWarps = 16;
 
-template <typename T, bool HALF, int DP, int ROWS, bool CUT>
+template <typename T, bool HALF, int DP, int ROWS>
 __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   __shared__ float s_ml[kMaxJoinWarps][4];
   __shared__ float s_o[kMaxJoinWarps][DP];
@@ -640,22 +640,20 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   // its segment: units before the sequence, and all units
   int64_t before = 0, units = 0;
   for (int s = lane; s < a.B; s += 32) {
-    const int64_t x = seq_info<CUT>(a, s, ROWS).units;
+    const int64_t x = seq_info<false>(a, s, ROWS).units;
     units += x;
     if (s < b) before += x;
   }
   before = warp_sum(before);
   units = warp_sum(units);
-  const SeqInfo s = seq_info<CUT>(a, b, ROWS);
+  const SeqInfo s = seq_info<false>(a, b, ROWS);
   const int i = first_row * group + (h - hk * group);
   const int tile = i / ROWS, r = i - tile * ROWS;
   const int64_t u0 = before + static_cast<int64_t>(tile) * s.groups, u1 = u0 + s.groups;
   const int64_t workers = active_shares(a, units);
   const int64_t w0 = ((u0 + 1) * workers - 1) / units, w1 = (u1 * workers - 1) / units;
-  const bool prefix = CUT && a.prefix_splits > 0;
-  if (w0 == w1 && !prefix) return;  // one worker held it all and wrote the output
-  // prefix: its parts, and behind them the rest if one worker held that
-  const int own = w0 == w1 ? 0 : static_cast<int>(w1 - w0 + 1), parts = own + (prefix ? a.prefix_splits + (w0 == w1) : 0);
+  if (w0 == w1) return;  // one worker held it all and wrote the output
+  const int parts = static_cast<int>(w1 - w0 + 1);
   auto slot_of = [&](int x) -> int64_t {
     const int64_t w = w0 + x;
     return 2 * (w * a.Hk + hk) + (x == 0 && units * w / workers < u0 ? 1 : 0);
@@ -666,14 +664,12 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
   for (int e = 0; e < V; ++e) o[e] = 0.f;
 #pragma unroll 4
   for (int x = warp; x < parts; x += warps) {
-    const bool shared = CUT && x >= own;
-    const int64_t at = shared ? ((x - own) * a.T + row) * a.H + h : slot_of(x) * kPartRows + r;
-    const float* part_o = shared ? a.prefix_o : a.part_o;
+    const int64_t at = slot_of(x) * kPartRows + r;
     // ordinary loads: the parts are written while this kernel may already be there
-    const float4 ml = __ldcg(reinterpret_cast<const float4*>(shared ? a.prefix_ml : a.part_ml) + at);
+    const float4 ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml + at * 4));
     float po[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) po[e] = __ldcg(part_o + at * DP + lane + 32 * e);
+    for (int e = 0; e < V; ++e) po[e] = __ldcg(a.part_o + at * DP + lane + 32 * e);
     const float top = fmaxf(m, ml.x), topv = fmaxf(mv, ml.z);
     const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
     l = l * ex2(m - base) + ml.y * ex2(ml.x - base);
@@ -709,6 +705,157 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedArgs a) {
     if (lane + 32 * e < a.d) out[lane + 32 * e] = Elem<T>::from_f(o[e] * mul);
 }
 
+// The same for segments of CUT.  A lane takes one part's maxima and sum, so that the weights of 32 parts are known after
+// one load, and then the parts' values are loaded several at a time, a row per load.  The warps take runs of parts and
+// join in order; one warp for a (row, head) where those fill the GPU.  Measured with 16 parts of a shared prefix and 64
+// rows of 32 heads of 128, 18 MB: TODO us.
+template <typename T, bool HALF, int DP, int ROWS>
+__global__ void paged_cut_join_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int V = DP / 32, kDeep = 8;
+  __shared__ float s_ml[kMaxJoinWarps][4];
+  __shared__ float s_o[kMaxJoinWarps][DP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int h = blockIdx.x % a.H;
+  const int64_t row = blockIdx.x / a.H;
+  const int group = a.H / a.Hk, hk = h / group;
+  // the row's sequence and its segment: units before the sequence, and all units
+  int b = static_cast<int>(row), first_row = 0;
+  bool live = true;
+  if (a.cu != nullptr) {
+    int64_t begin;
+    int n;
+    clamp_range(a.cu, 0, a.T, begin, n);
+    live = row >= begin;
+    if (live) {
+      const SeqTile t = find_tile(a.cu, a.B, a.T, static_cast<int>(a.T) + 1, static_cast<int>(row - begin), 1, false, false);
+      live = t.n != 0;  // not behind the last sequence
+      b = t.seq;
+      first_row = t.first;
+    }
+  }
+  int64_t before = 0, units = 0;
+  for (int s = lane; s < a.B; s += 32) {
+    const int64_t x = seq_info<true>(a, s, ROWS).units;
+    units += x;
+    if (s < b) before += x;
+  }
+  before = warp_sum(before);
+  units = warp_sum(units);
+  int parts = 0, own = 0;
+  int64_t w0 = 0, workers = 1, u0 = 0;
+  int r = 0;
+  if (live) {
+    const SeqInfo s = seq_info<true>(a, b, ROWS);
+    const int i = first_row * group + (h - hk * group);
+    const int tile = i / ROWS;
+    r = i - tile * ROWS;
+    u0 = before + static_cast<int64_t>(tile) * s.groups;
+    workers = active_shares(a, units);
+    w0 = ((u0 + 1) * workers - 1) / units;
+    own = static_cast<int>(((u0 + s.groups) * workers - 1) / units - w0) + 1;
+    if (own == 1) own = 0;  // one worker held it all: it wrote the output, or a part of its own behind the prefix's
+    parts = own + (a.prefix_splits > 0 ? a.prefix_splits + (own == 0) : 0);
+  }
+  pdl_wait();
+  if (parts == 0) return;
+  // this warp's parts
+  const int from = parts * warp / warps, to = parts * (warp + 1) / warps;
+  float m = neg_inf(), l = 0.f, mv = neg_inf(), o[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = 0.f;
+  for (int x0 = from; x0 < to; x0 += 32) {
+    const int x = x0 + lane;
+    float4 ml = make_float4(neg_inf(), 0.f, neg_inf(), 0.f);
+    const float* po = nullptr;
+    if (x < to) {
+      // ordinary loads: the parts are written while this kernel may already be there
+      if (x < own) {
+        const int64_t w = w0 + x;
+        const int64_t at = (2 * (w * a.Hk + hk) + (x == 0 && units * w / workers < u0 ? 1 : 0)) * kPartRows + r;
+        ml = __ldcg(reinterpret_cast<const float4*>(a.part_ml) + at);
+        po = a.part_o + at * DP;
+      } else {
+        const int64_t at = ((x - own) * a.T + row) * a.H + h;
+        ml = __ldcg(reinterpret_cast<const float4*>(a.prefix_ml) + at);
+        po = a.prefix_o + at * DP;
+      }
+    }
+    float top = ml.x, topv = ml.z;
+#pragma unroll
+    for (int y = 16; y > 0; y >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+      topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, y));
+    }
+    top = fmaxf(top, m);
+    topv = fmaxf(topv, mv);
+    const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
+    float sum = ml.y * ex2(ml.x - base);
+#pragma unroll
+    for (int y = 16; y > 0; y >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, y);
+    l = l * ex2(m - base) + sum;
+    const float mine = ex2(mv - basev), weight = ex2(ml.z - basev);
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] *= mine;
+    m = top;
+    mv = topv;
+    const int count = min(32, to - x0);
+    for (int y0 = 0; y0 < count; y0 += kDeep) {
+      float v[kDeep][V];
+#pragma unroll
+      for (int y = 0; y < kDeep; ++y) {
+        const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(po), (y0 + y) & 31));
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[y][e] = 0.f;
+        if (y0 + y < count) {
+          if constexpr (V == 4) {
+            const float4 z = __ldcg(reinterpret_cast<const float4*>(p) + lane);
+            v[y][0] = z.x, v[y][1] = z.y, v[y][2] = z.z, v[y][3] = z.w;
+          } else {
+            const float2 z = __ldcg(reinterpret_cast<const float2*>(p) + lane);
+            v[y][0] = z.x, v[y][1] = z.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < kDeep; ++y) {
+        const float w = __shfl_sync(0xffffffffu, weight, (y0 + y) & 31);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = fmaf(v[y][e], w, o[e]);
+      }
+    }
+  }
+  if (warps > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_o[warp][V * lane + e] = o[e];
+    if (lane == 0) s_ml[warp][0] = m, s_ml[warp][1] = l, s_ml[warp][2] = mv;
+    __syncthreads();
+    if (warp != 0) return;
+    float top = neg_inf(), topv = neg_inf();
+    for (int w = 0; w < warps; ++w) top = fmaxf(top, s_ml[w][0]), topv = fmaxf(topv, s_ml[w][2]);
+    const float base = top == neg_inf() ? 0.f : top, basev = topv == neg_inf() ? 0.f : topv;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 0.f;
+    for (int w = 0; w < warps; ++w) {
+      l += s_ml[w][1] * ex2(s_ml[w][0] - base);
+      const float mul = ex2(s_ml[w][2] - basev);
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] += s_o[w][V * lane + e] * mul;
+    }
+    m = top;
+    mv = topv;
+  }
+  const float base = m == neg_inf() ? 0.f : m, basev = mv == neg_inf() ? 0.f : mv;
+  float mul = 0.f;
+  if (l > 0.f || l != l) mul = __fdividef(ex2(basev - base - (HALF ? kHalfShift : 0.f)), l);
+  if (V * lane >= a.d) return;
+  T* out = static_cast<T*>(a.o) + row * a.o_sT + h * a.o_sH + V * lane;
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(o[0] * mul, o[1] * mul), Mma<T>::pack(o[2] * mul, o[3] * mul));
+  else
+    *reinterpret_cast<uint32_t*>(out) = Mma<T>::pack(o[0] * mul, o[1] * mul);
+}
+
 template <typename T, bool FP8, int DP, int ROWS, bool CUT>
 struct Split {
   static int workers() {
@@ -730,7 +877,9 @@ struct Split {
     // about as many warps as a segment has parts when all are equally long
     const int64_t segments = static_cast<int64_t>(a.B) * a.Hk;
     const int64_t parts = a.workers / (segments > 0 ? segments : 1) + 2 + (CUT ? a.prefix_splits : 0);
-    const int warps = parts <= 4 ? 2 : parts <= 16 ? 4 : parts <= 64 ? 8 : kMaxJoinWarps;
+    int warps = parts <= 4 ? 2 : parts <= 16 ? 4 : parts <= 64 ? 8 : kMaxJoinWarps;
+    // CUT: eight parts to a warp, and no more warps than about 16 an SM
+    if (CUT) warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(parts + 7) / 8, 2368 / (a.T * a.H), kMaxJoinWarps})));
     if (a.T * a.H > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.T * a.H));
@@ -741,7 +890,8 @@ struct Split {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kHalf, DP, ROWS, CUT>, a);
+    if constexpr (CUT) return cudaLaunchKernelEx(&cfg, paged_cut_join_kernel<T, kHalf, DP, ROWS>, a);
+    else return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kHalf, DP, ROWS>, a);
   }
 };
 

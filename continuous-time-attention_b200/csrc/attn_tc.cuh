@@ -330,6 +330,50 @@ __device__ __forceinline__ void store_rows(uint32_t taddr, T* out, int col, int 
   }
 }
 
+// The same for fp32 rows that start on 32 bytes: 32 columns at a time, whose four 32-byte pieces four lanes exchange, so
+// that a store writes 128 bytes each of 8 rows.
+template <int N>
+__device__ __forceinline__ void store_floats(uint32_t taddr, float* out, float scale, bool live, bool any) {
+  const int lane = threadIdx.x & 31;
+  const unsigned long long mine = live ? reinterpret_cast<unsigned long long>(out) : 0ull;
+#pragma unroll 1
+  for (int c = 0; c < N / 32; ++c) {
+    uint32_t v[32];
+    if (any) {
+      ld32(taddr + 32 * c, v);
+      wait_ld(v);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * scale);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = 0u;
+    }
+    // piece p of lane l goes to lane p of l's four, as its piece l
+#pragma unroll
+    for (int step = 1; step < 4; step *= 2)
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        if (p & step) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool high = lane & step;
+          const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? v[8 * p + e] : v[8 * (p | step) + e], step);
+          if (high) v[8 * p + e] = got;
+          else v[8 * (p | step) + e] = got;
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const unsigned long long row = __shfl_sync(0xffffffffu, mine, (lane & ~3) + r);
+      if (row == 0) continue;
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + 128 * c + 32 * (lane & 3)),
+                   "r"(v[8 * r]), "r"(v[8 * r + 1]), "r"(v[8 * r + 2]), "r"(v[8 * r + 3]), "r"(v[8 * r + 4]),
+                   "r"(v[8 * r + 5]), "r"(v[8 * r + 6]), "r"(v[8 * r + 7])
+                   : "memory");
+    }
+  }
+}
+
 }  // namespace tc
 
 // Host: the alignment in bytes of a 16-bit tensor's rows that store_rows can use.

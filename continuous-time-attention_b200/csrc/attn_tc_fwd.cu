@@ -701,22 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // codes do not.
         constexpr float kUnit = SCALED && !kWeighted ? 128.f : 1.f;
         const int64_t at = (static_cast<int64_t>(x.lo / f.chunk) * a.L + tok) * a.H + h;
-        float* to = f.part_o + at * DP + half * (DP / 2);
-#pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[16] = {};
-          if (count > 0) {  // a part behind all sequences has no keys
-            tc::ld16(o_addr + 16 * c, o);
-            tc::wait_ld(o);
-          }
-          if (live) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(to + 16 * c + e) =
-                  make_float4(__uint_as_float(o[e]) * kUnit, __uint_as_float(o[e + 1]) * kUnit,
-                              __uint_as_float(o[e + 2]) * kUnit, __uint_as_float(o[e + 3]) * kUnit);
-          }
-        }
+        tc::store_floats<DP / 2>(o_addr, f.part_o + at * DP + half * (DP / 2), kUnit, live, count > 0);  // or the part lies behind all sequences
         if (live && half == 0)
           *reinterpret_cast<float4*>(f.part_ml + at * 4) =
               make_float4(m * c2, kShift == 0.f ? sum : sum * 0x1p-7f, kWeighted ? mv : m * c2, 0.f);
