@@ -366,9 +366,16 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
       a.n_pages < 1)
     return p;
   const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
-  // one wave of CTAs, one per SM
-  const int64_t per = (tiles + std::max<int64_t>(1, 148 / ctas) - 1) / std::max<int64_t>(1, 148 / ctas);
-  const int64_t splits = (tiles + per - 1) / per;
+  // Both kernels run at once: the parts' CTAs, one per SM, leave the split kernel the other SMs, and their own when they
+  // are done.  So there are as many parts as let both end at about the same time.  In SM-microseconds, measured: a part
+  // costs 12 and each of its key tiles 2.5 (e4m3 5, in fp16 7); the own keys, taken as half of what the table holds, what
+  // HBM needs.  64 sequences of 16 to 1024 own keys behind 8192: TODO
+  const double tile_us = !quantized ? 2.5 : dtype == CTA_F16 ? 7. : 5.;
+  const double own_bytes = 0.5 * a.B * static_cast<double>(width * a.page - keys) * 2. * a.Hk * (quantized ? a.d + 4 : 2 * a.d);
+  const double shared_us = static_cast<double>(tiles) * ctas * tile_us, own_us = own_bytes / 44300.;
+  const double parts = shared_us / ((shared_us + own_us) / 148. + 6.) / ctas;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(148 / ctas, static_cast<int64_t>(parts + 0.5)));
+  const int64_t per = (tiles + most - 1) / most, splits = (tiles + per - 1) / per;
   const int dp = a.d <= 64 ? 64 : 128;
   // the values' rows start on 32 bytes, the workspace on 16
   const int64_t sums = 32 + (splits + 1) * a.T * a.H * (dp + 4) * static_cast<int64_t>(sizeof(float));

@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
     u += count;
     first = false;
   }
-  if (CUT) pdl_wait();  // launched beside the prefix's sums; the join's wait for this kernel's end covers theirs
+  if (CUT) wait_beside();  // the prefix's sums; the join's wait for this kernel's end covers theirs
 }
 
 // Joins the parts of one (row, head): the warps of the CTA take the parts in turn, then join theirs in order.

@@ -138,13 +138,13 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, u
 // C[128 x N] (+)= A[tmem, 128 x 128] B[128 x N], B MN-major (rows are the
 // contraction index), its 64-column blocks 16 KB apart.  A lies where the warps
 // that made it left it: GROUP indices at a time at the start of the GROUP columns
-// their fp32 sources took.  One thread.
-template <int GROUP>
+// their fp32 sources took.  STEPS: of 16 contraction indices, from the first.  One thread.
+template <int GROUP, int STEPS = 8>
 __device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, uint32_t id, bool accumulate) {
   const uint32_t bl = desc_low(b, 16384);
   constexpr int kPer = GROUP / 16;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < STEPS; ++k)
     mma_ts(d, a + GROUP * (k / kPer) + 8 * (k % kPer), bl + k * (2048 >> 4), id, accumulate || k > 0);
 }
 

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
-  pdl_wait();  // launched beside dK and dV
+  wait_beside();  // dK and dV
 }
 
 // ---------------------------------------------------------------------------
@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
-  if (FORM == kWindow) pdl_wait();  // launched beside the far rows' CTAs; dQ's wait for this kernel's end covers theirs
+  if (FORM == kWindow) wait_beside();  // the far rows; dQ's wait for this kernel's end covers them
 }
 
 int64_t count_tiles(AttnArgs& a, int rows) {

@@ -228,6 +228,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // first keys that stay visible to all: those before this one
   auto sinks_of = [&](const Item& x) { return FORM == kWindow && a.sinks > 0 ? x.lo + a.sinks : 0; };
+  // A step of first keys alone, up to 32 of them, takes a quarter of the products.  It pays where the softmax skips what
+  // no row of a warp sees, which it does not at dim 128 over 16 bits: each step waits for the other tile there, and the
+  // votes cost more than they save (12 prompts of up to 4096 tokens, 32/8 heads of 128, window 512: 451 and 424 us; 16384
+  // tokens, 8 heads of 64, window 1024: 101 and 104; chunks of 512 over e4m3: 101 and 111).
+  constexpr bool kSkip = FORM == kWindow && (SCALED || DP == 64);
+  auto narrow = [&](int j0, int from, int sink_end) { return kSkip && j0 < from && sink_end - j0 <= 32; };
   // to the next tile
   auto advance = [&](int& j0, int from, const Item& x) {
     j0 += kRows;
@@ -398,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // both tiles those of one tile delayed the other's products (562 instead of 503 us at 8192 keys,
     // 16 heads of 128, 477 instead of 402 at 64).  Both free a key tile.
     const int i = warp == kSoftmaxWarps ? 0 : 1;
-    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_32 = tc::idesc<T>(32, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
     bool ok = true;
     int kv = 0, nq = 0, ns = 0;  // running numbers: tiles, Q loads, steps of this row tile
@@ -416,16 +422,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
       auto kv_wait = [&](int y) { ok = ok && tc::wait(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
       auto kv_addr = [&](int y) { return smem + (2 + (kv + y) % NS) * L::kTile; };
+      const int sink_end = sinks_of(x);
       // scores of step j into the tile's buffer; keys are released by the step's end
-      auto scores = [&](int j) {
-        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), id_s);
+      auto scores = [&](int j, int at) {
+        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), narrow(at, from, sink_end) ? id_32 : id_s);
         tc::commit(&bars.s_full[i]);
         if (j + 1 == mine) tc::commit(&bars.q_empty);
       };
       kv_wait(0);
       tc::fence_after();
       if (ok && leader) {
-        if (mine > 0) scores(0);
+        if (mine > 0) scores(0, j0);
         else tc::commit(&bars.q_empty);
         tc::commit(&bars.kv_empty[kv % NS]);
       }
@@ -447,9 +454,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && tc::wait(&bars.p_full[i], ns & 1);
           tc::fence_after();
           if (ok && leader) {
-            tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
-            if (j + 1 == mine) tc::commit(&bars.o_full[i]);
-            else scores(j + 1);
+            if (narrow(j0, from, sink_end)) tc::product_tn<64, 2>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            else tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            if (j + 1 == mine) {
+              tc::commit(&bars.o_full[i]);
+            } else {
+              int at = j0;
+              advance(at, from, x);
+              scores(j + 1, at);
+            }
           }
           ++ns;
         }
@@ -558,21 +571,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             x[4 * e + 3] = __float_as_uint(hi.y);
           }
         };
-        auto hide = [&](int c, uint32_t (&x)[32]) {
+        // false: none of these 32 keys counts for any row of the warp (kSkip; x is left as it is)
+        auto hide = [&](int c, uint32_t (&x)[32]) -> bool {
           const int left = limit - j0 - 64 * half - 32 * c + 1;
           uint32_t see =
               (half == 0 ? w[c] : w[2 + c]) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
           if constexpr (FORM == kWindow) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - j0 - 64 * half - 32 * c);
+          if constexpr (kSkip) {
+            if (!__any_sync(0xffffffffu, see != 0u)) return false;
+            if (__all_sync(0xffffffffu, see == 0xffffffffu)) return true;
+          }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!((see >> e) & 1u)) x[e] = 0xff800000u;
+          return true;
         };
+        bool some[2] = {true, true};
         float t[4], topv = mv;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t(&x)[32] = s[SCALED ? 0 : c];
           if (SCALED) scale(c, x);
-          if (!whole) hide(c, x);
+          if (!whole) some[c] = hide(c, x);
+          if (kSkip && !some[c]) {
+            t[2 * c] = t[2 * c + 1] = neg_inf();
+            continue;
+          }
           if constexpr (kWeighted) {
             // score + logarithm of the value's scale
             float4 r[8];
@@ -645,6 +669,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t p[16];
           uint32_t(&x)[32] = s[SCALED ? 0 : c];
           float4 r[SCALED ? 8 : 1];
+          if (kSkip && !some[c]) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) p[e] = 0u;
+          } else {
           if constexpr (SCALED) {
             scale(c, x);
             if (!whole) hide(c, x);
@@ -671,6 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             p[e] = tc::pack2<T>(y.x, y.y);
+          }
           }
           // over this half's own scores: the other half may not have read its yet
           tc::st16(s_addr + 16 * c, p);

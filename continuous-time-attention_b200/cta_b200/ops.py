@@ -827,6 +827,19 @@ def _row_strides(t: torch.Tensor):
     return tuple(x if n > 1 else 0 for x, n in zip(t.stride(), t.shape[:-1]))
 
 
+def _placed_rows(t: torch.Tensor):
+    """(t or a copy whose rows start on 16 bytes, address, strides of tokens and heads) of rows [T, heads, dim]."""
+    address = t.data_ptr()
+    if t.is_contiguous() and not address & 15:
+        _, heads, dim = t.shape
+        if not dim & 7:
+            return t, address, heads * dim, dim
+    if not _on16(t):
+        t = _own_rows(t)
+        address = t.data_ptr()
+    return (t, address, *_row_strides(t))
+
+
 def _cache_sizes(k_cache, v_cache, k_scale, v_scale, dtype, like):
     """Checked cache: (pages, page_size, kv_heads, dim, quantized)."""
     shape, kind = k_cache.shape, k_cache.dtype
@@ -966,23 +979,29 @@ def _rotary_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleav
     if cos_sin.dim() != 2 or cos_sin.dtype not in (torch.float32, q.dtype) or cos_sin.get_device() != device:
         raise ValueError(f"cos_sin must have shape (positions, rotary_dim), float32 or {q.dtype} on {q.device}, got "
                          f"{tuple(cos_sin.shape)}, {cos_sin.dtype} on {cos_sin.device}")
-    if not _on16(cos_sin):
+    table = cos_sin.data_ptr()
+    if (table & 15 or not cos_sin.is_contiguous() or cos_sin.shape[1] & 7) and not _on16(cos_sin):
         raise ValueError("cos_sin must have a contiguous last axis and rows that start on 16 bytes")
-    q, k, v = (x if _on16(x) else _own_rows(x) for x in (q, k, v))
+    q, q_at, q_token, q_head = _placed_rows(q)
+    k, k_at, k_token, k_head = _placed_rows(k)
+    v, v_at, v_token, v_head = _placed_rows(v)
     if out is None:
         o = _new(q)
+        o_token, o_head = shape[1] * dim, dim
     else:
         o = _out(out, shape, q)
         if not _on16(o):
             raise ValueError("out must have rows that start on 16 bytes")
+        o_token, o_head = _row_strides(o)
+    angles, rotary_dim = cos_sin.shape
     cache = _lib.KV_CACHE_ARGS.pack(
-        k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
-        slots.data_ptr(), *_row_strides(k), *_row_strides(v), *_row_strides(k_cache), *_row_strides(v_cache), shape[0],
-        kv_heads, dim, pages, page, code, quantized)
+        k_at, v_at, k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale), slots.data_ptr(), k_token,
+        k_head, v_token, v_head, *_row_strides(k_cache), *_row_strides(v_cache), shape[0], kv_heads, dim, pages, page, code,
+        quantized)
     rotary = _lib.ROTARY_ARGS.pack(
-        q.data_ptr(), o.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), *_row_strides(q), *_row_strides(o),
-        cos_sin.stride(0) if cos_sin.shape[0] > 1 else 0, shape[1], cos_sin.shape[1], cos_sin.shape[0],
-        _lib.dtype_code(cos_sin.dtype), bool(interleaved))
+        q_at, o.data_ptr(), positions.data_ptr(), table, q_token, q_head, o_token, o_head,
+        cos_sin.stride(0) if angles > 1 else 0, shape[1], rotary_dim, angles, 0 if cos_sin.dtype == torch.float32 else code,
+        bool(interleaved))
     return q, o, cache, rotary, (k, v, k_cache, v_cache, k_scale, v_scale, slots, positions, cos_sin)
 
 
@@ -1116,18 +1135,19 @@ def _paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows
         cu = _offsets(cu_seqlens, q)
         if cu.shape[0] != batch + 1:
             raise ValueError(f"cu_seqlens must have {batch + 1} entries, got {cu.shape[0]}")
-    if not _on16(q):
-        q = _own_rows(q)
+    q, q_at, q_token, q_head = _placed_rows(q)
     if out is None:
         o = _new(q)
+        o_token, o_head = heads * dim, dim
     else:
-        o = _out(out, q.shape, q)
+        o = _out(out, shape, q)
         if not _on16(o):
             raise ValueError("out must have rows that start on 16 bytes")
+        o_token, o_head = _row_strides(o)
     lib = _lib.load()
     args = _lib.PAGED_ATTENTION_ARGS.pack(
-        q.data_ptr(), o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
-        table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), *_row_strides(q), *_row_strides(o), *_row_strides(k_cache),
+        q_at, o.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
+        table.data_ptr(), lens.data_ptr(), _lib.ptr(cu), q_token, q_head, o_token, o_head, *_row_strides(k_cache),
         *_row_strides(v_cache), table.stride(0), rows, batch, heads, kv_heads, dim, pages, page, tshape[1],
         int(max_rows), code, quantized, dim**-0.5 if scale is None else float(scale), 0.0)
     if reach[0]:
