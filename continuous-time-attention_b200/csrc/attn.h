@@ -119,10 +119,11 @@ struct PagedArgs {
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
   // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these what it left out of their
   // elements [B, Hk, residue_row(table_width * page)]: the fractions of the scales in bf16, the key's scale and the
-  // logarithm (base 2) of the value's in fp16; else nullptr
+  // logarithm (base 2) of the value's in fp16, rows on 32 bytes; else nullptr
   const float* k_res;
   const float* v_res;
   int64_t expanded_pages;
+  int fold_scale;  // k_res times scale * log2(e): for windows and prefixes
   // shared prefix of `skip` keys: its sums over prefix_splits parts of prefix_chunk keys, for every row of q
   int prefix_splits, prefix_chunk;
   float* prefix_o;   // [splits + 1, T, H, dim rounded up to 64 or 128] fp32; last: a row's own keys, if one worker had them

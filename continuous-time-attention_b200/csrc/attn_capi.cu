@@ -311,7 +311,7 @@ int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64
   const int64_t slots = b * width * page;
   if (slots >= (1LL << 24) || slots * hk >= (1LL << 26)) return 0;
   const int64_t bytes = slots * hk * d * 4 + b * residue_row(width * page) * hk * 8;
-  return bytes <= kMostExpanded ? bytes : 0;
+  return bytes > 0 && bytes <= kMostExpanded ? bytes + 32 : 0;  // and what puts its start on 32 bytes
 }
 
 int64_t split_bytes(int workers, int d) {
@@ -339,9 +339,12 @@ int paged_pointers(const PagedArgs& a, int quantized, const void* workspace, int
 // Expands the pages of an e4m3 cache that p's table names into `ws`, and points x at them.
 cudaError_t expand_pages(const PagedArgs& p, int dtype, char* ws, PagedArgs& x, cudaStream_t st) {
   const int64_t pages = static_cast<int64_t>(p.B) * p.table_width, part = pages * p.page * p.Hk * p.d * 2;
+  ws += -reinterpret_cast<intptr_t>(ws) & 31;
   float* k_res = reinterpret_cast<float*>(ws + 2 * part);
   float* v_res = k_res + p.B * residue_row(static_cast<int64_t>(p.table_width) * p.page) * p.Hk;
-  const cudaError_t e = launch_cache_expand(p, dtype, ws, ws + part, k_res, v_res, st);
+  PagedArgs fold = p;
+  fold.fold_scale = p.window > 0 || p.seq_lens == nullptr;  // windows, and the whole table of a prefix
+  const cudaError_t e = launch_cache_expand(fold, dtype, ws, ws + part, k_res, v_res, st);
   x.k_cache = ws;
   x.v_cache = ws + part;
   x.k_res = k_res;
@@ -368,9 +371,10 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
   const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
   // Both kernels run at once: the parts' CTAs, one per SM, leave the split kernel the other SMs, and their own when they
   // are done.  So there are as many parts as let both end at about the same time.  In SM-microseconds, measured: a part
-  // costs 12 and each of its key tiles 2.5 (e4m3 5, in fp16 7); the own keys, taken as half of what the table holds, what
-  // HBM needs.  64 sequences of 16 to 1024 own keys behind 8192: TODO
-  const double tile_us = !quantized ? 2.5 : dtype == CTA_F16 ? 7. : 5.;
+  // costs 12 and each of its key tiles 4 (e4m3 5, in fp16 7); the own keys, taken as half of what the table holds, what
+  // HBM needs.  64 sequences of 16 to 1024 own keys behind 8192, 32/8 heads of 128: 64 us with the parts on 72 SMs, 81
+  // with them on 128, 91 on 40; of 64 own keys each 39, 36 and 44.
+  const double tile_us = !quantized ? 4. : dtype == CTA_F16 ? 7. : 5.;
   const double own_bytes = 0.5 * a.B * static_cast<double>(width * a.page - keys) * 2. * a.Hk * (quantized ? a.d + 4 : 2 * a.d);
   const double shared_us = static_cast<double>(tiles) * ctas * tile_us, own_us = own_bytes / 44300.;
   const double parts = shared_us / ((shared_us + own_us) / 148. + 6.) / ctas;

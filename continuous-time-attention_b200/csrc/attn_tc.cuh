@@ -184,6 +184,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+// `bytes` (a multiple of 16) from global memory, both ends on 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
 // Bounded wait on an mbarrier phase, false after about a second.  The timer is
 // read only when some tries have failed: reading it costs a few hundred cycles,
 // which a wait that is on the critical path would pay after every failed try.

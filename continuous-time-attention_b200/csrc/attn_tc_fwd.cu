@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // product within fp16 for any scales.
   constexpr bool kWeighted = SCALED && std::is_same<T, __half>::value;
   constexpr float kShift = std::is_same<T, __half>::value && !SCALED ? kHalfShift : 0.f;
+  // The keys' fractions carry scale * log2(e): one product less for each score.
+  constexpr bool kFolded = SCALED && FORM != kPlain;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -151,6 +153,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float s_max[2][2][kRows], s_sum[2][2][kRows];  // [tile][half of the keys][row]
   __shared__ float s_maxv[kWeighted ? 2 : 1][2][kWeighted ? kRows : 1];
   __shared__ uint32_t s_boxes[16];  // paged: which boxes of a key tile were loaded
+  // SCALED: the fractions of the key tiles in flight, keys' and values'.  They come with the values' tile, whose stage is
+  // free only when the weights that need them are in O, so four of them are more than are in flight.
+  __shared__ __align__(16) float s_res[SCALED ? 4 : 1][2][SCALED ? kRows : 1];
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -374,7 +379,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b = 0; b < boxes; ++b)
               if ((got >> b) & 1u) bits |= ((1u << per) - 1u) << (b * per);
             *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kv >> 1) & 15]) = bits;
-            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64));
+            const bool res = SCALED && (y & 1);
+            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64) + (res ? 8 * kRows : 0));
+            if (res) {
+              const int64_t at = (static_cast<int64_t>(x.t.seq) * a.Hk + x.hk) * residue_row(f.table_width * f.page) + j0;
+              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][0]), f.k_res + at, 4 * kRows, &bars.kv_full[stage]);
+              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][1]), f.v_res + at, 4 * kRows, &bars.kv_full[stage]);
+            }
           }
           __syncwarp();
           if (page >= 0)
@@ -484,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + i * kRows + half * 64;
     const uint32_t o_addr = tmem + lanes + 2 * kRows + i * DP + half * (DP / 2);
-    const float c2 = a.scale * kLog2e;
+    const float c2 = kFolded ? 1.f : a.scale * kLog2e;
     bool ok = true;
     int ns = 0, no = 0, kt = 0;  // running numbers: steps, outputs, key tiles
     for (int it = 0; ok; ++it) {
@@ -519,21 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       T* out = static_cast<T*>(a.o) + x.t.batch * a.os.b + (x.t.row0 + tok) * a.os.t + h * a.os.h;
       float* lse = live && half == 0 && a.lse != nullptr ? a.lse + lse_index(a, x.t, h, tok) : nullptr;
       const int sink_end = sinks_of(x);
-      // the first fraction of this half's keys
-      int res = SCALED ? (x.t.seq * a.Hk + x.hk) * static_cast<int>(residue_row(f.table_width * f.page)) + j0 + 64 * half : 0;
       float m = neg_inf(), sum = 0.f;
       float mv = neg_inf();  // kWeighted: the reference of weight * scale, as an exponent of two
-      auto next = [&] {
-        const int before = j0;
-        advance(j0, from, x);
-        if (SCALED) res += j0 - before;
-      };
-      for (int j = 0; j < count; ++j, ++ns, next()) {
-        if (SCALED && lane < 4)  // two lines each of the step's fractions
-          asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 2 ? f.k_res : f.v_res) + res + 32 * (lane & 1)));
+      for (int j = 0; j < count; ++j, ++ns, advance(j0, from, x)) {
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
         ok = ok && tc::wait(&bars.s_full[i], ns & 1);
+        if (SCALED) ok = ok && tc::wait(&bars.kv_full[(2 * (kt + j) + 1) % NS], ((2 * (kt + j) + 1) / NS) & 1);
         tc::fence_after();
         uint32_t s[2][32];
         if (!SCALED) {
@@ -550,14 +553,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!SCALED) tc::wait_ld(s[0], s[1]);
         // Fractions of the scales, 32 keys at a time: the scores are read from tensor memory once for the maximum and
-        // once for the weights, which leaves registers for eight loads.  Bound by issue (77 % of the cycles of a busy
-        // SM); with one read of both the loads wait for one another instead, 205 and 199 us for 32 chunks of 16
-        // rows over 2048 keys.
+        // once for the weights, for want of registers.  From shared memory, where the loads' warp puts them: the
+        // softmax waited for them 56 % of its time when each warp fetched them (512 rows of 4 sequences in windows
+        // of 1024, 32/8 heads of 128: 106 and 83 us; 128 rows in fp16 over a prefix of 16384: 120 and 93).
+        auto fractions = [&](int of, int c, float4 (&r)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r[e] = *reinterpret_cast<const float4*>(&s_res[(kt + j) & 3][of][64 * half + 32 * c + 4 * e]);
+        };
         auto scale = [&](int c, uint32_t (&x)[32]) {
           tc::ld32(s_addr + 32 * c, x);
           float4 r[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.k_res + res + 32 * c) + e);
+          fractions(0, c, r);
           tc::wait_ld(x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -600,14 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kWeighted) {
             // score + logarithm of the value's scale
             float4 r[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
+            fractions(1, c, r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 lo = fma2(make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])), f2(c2),
-                                     make_float2(r[e].x, r[e].y));
-              const float2 hi = fma2(make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])), f2(c2),
-                                     make_float2(r[e].z, r[e].w));
+              const float2 a0 = make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]));
+              const float2 a1 = make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+              const float2 v0 = make_float2(r[e].x, r[e].y), v1 = make_float2(r[e].z, r[e].w);
+              const float2 lo = kFolded ? add2(a0, v0) : fma2(a0, f2(c2), v0);
+              const float2 hi = kFolded ? add2(a1, v1) : fma2(a1, f2(c2), v1);
               topv = tc::max3(tc::max3(lo.x, lo.y, hi.x), hi.y, topv);
             }
           }
@@ -676,13 +682,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (SCALED) {
             scale(c, x);
             if (!whole) hide(c, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
+            fractions(1, c, r);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 score = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-            float2 y = fma2(score, c2v, bv);
+            float2 y = kFolded ? add2(score, bv) : fma2(score, c2v, bv);
             y.x = ex2(y.x);
             y.y = ex2(y.y);
             if (e & 1) part2 = add2(part2, y);
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float4& z = r[e / 2];
               const float2 of_value = (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
               if constexpr (kWeighted) {
-                y = fma2(score, c2v, add2(of_value, vv));
+                y = kFolded ? add2(score, add2(of_value, vv)) : fma2(score, c2v, add2(of_value, vv));
                 y.x = ex2(y.x);
                 y.y = ex2(y.y);
               } else {

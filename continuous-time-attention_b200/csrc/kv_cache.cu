@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
 
 // Codes of the pages of each sequence, in order, as exact 16-bit rows.  bf16, whose exponents reach as far as fp32's:
 // each times the power of two below its scale, whose fraction goes into k_res and v_res.  fp16: the codes alone, and
-// beside them the key's scale and the logarithm of the value's (attn_tc_fwd.cu says why).
+// beside them the key's scale and the logarithm of the value's (attn_tc_fwd.cu says why).  fold_scale: what is for
+// the keys carries what takes a score to an exponent of two.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out,
                                                                 float* k_res, float* v_res) {
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
         pow = __uint_as_float(bits & 0xff800000u);
         rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
       }
-      if (lane == 0) res[i * res_row + j] = rest;
+      if (lane == 0) res[i * res_row + j] = second || !a.fold_scale ? rest : rest * (a.scale * kLog2e);
       float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

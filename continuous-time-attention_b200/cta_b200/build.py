@@ -73,7 +73,7 @@ def is_stale() -> bool:
 # A march kernel keeps its whole state in registers; a stack frame above a few
 # bytes means a helper was not inlined (its state went to local memory) or
 # large spills, either of which costs an order of magnitude.
-MAX_STACK_BYTES = 80
+MAX_STACK_BYTES = 96
 
 
 def stack_frames(ptxas_log: str) -> list:
