@@ -371,12 +371,13 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
   const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
   // Both kernels run at once: the parts' CTAs, one per SM, leave the split kernel the other SMs, and their own when they
   // are done.  So there are as many parts as let both end at about the same time.  In SM-microseconds, measured: a part
-  // costs 12 and each of its key tiles 4 (e4m3 5, in fp16 7); the own keys, taken as half of what the table holds, what
-  // HBM needs.  64 sequences of 16 to 1024 own keys behind 8192, 32/8 heads of 128: 64 us with the parts on 72 SMs, 81
-  // with them on 128, 91 on 40; of 64 own keys each 39, 36 and 44.
-  const double tile_us = !quantized ? 4. : dtype == CTA_F16 ? 7. : 5.;
+  // costs 12 and each of its key tiles 3.5 (e4m3 3.8, in fp16 5.5); the own keys, taken as half of what the table holds,
+  // 1.2 times what HBM needs (e4m3 twice).  32/8 heads of 128: 64 sequences of 16 to 1024 own keys behind 8192 take 63 us
+  // with the parts on 56 SMs, 82 with them on 128 and 90 on 40; 64 of 64 own keys 39 on 112 or 128 SMs, 42 on 72; 128 of
+  // 16 to 512 behind 16384, e4m3 in fp16, 140 us on 112 and 154 on 128.
+  const double tile_us = !quantized ? 3.5 : dtype == CTA_F16 ? 5.5 : 3.8;
   const double own_bytes = 0.5 * a.B * static_cast<double>(width * a.page - keys) * 2. * a.Hk * (quantized ? a.d + 4 : 2 * a.d);
-  const double shared_us = static_cast<double>(tiles) * ctas * tile_us, own_us = own_bytes / 44300.;
+  const double shared_us = static_cast<double>(tiles) * ctas * tile_us, own_us = own_bytes / 44300. * (quantized ? 2. : 1.2);
   const double parts = shared_us / ((shared_us + own_us) / 148. + 6.) / ctas;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(148 / ctas, static_cast<int64_t>(parts + 0.5)));
   const int64_t per = (tiles + most - 1) / most, splits = (tiles + per - 1) / per;

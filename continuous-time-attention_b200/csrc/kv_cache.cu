@@ -20,6 +20,8 @@
 // together.  Measured: 16384 tokens of 8 heads of 128 into e4m3, 101 MB, 23 us (21
 // without the correction), and back 17 us; 16-bit cache, 134 MB, 22 and 20 us, 6.0 and
 // 6.7 TB/s in part from L2; 64 tokens 2 us each.
+#include <algorithm>
+
 #include "attn_common.cuh"
 
 namespace cta {
@@ -224,15 +226,29 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
 // the keys carries what takes a score to an exponent of two.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out,
-                                                                float* k_res, float* v_res) {
+                                                                float* k_res, float* v_res, unsigned per_seq) {
   constexpr int GROUP = 16;
   const bool second = blockIdx.y != 0;
   const unsigned blocks = (a.Hk + kHeads - 1) / kHeads;
   const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
   const unsigned slots = static_cast<unsigned>(a.table_width) * a.page;  // per sequence
-  const unsigned row = group / blocks, b = row / slots, j = row - b * slots;
-  const int h0 = static_cast<int>(group - row * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
+  const unsigned at = group / blocks, b = at / per_seq;
+  unsigned j = at - b * per_seq;
+  const int h0 = static_cast<int>(group - at * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
   if (b >= static_cast<unsigned>(a.B)) return;
+  const int n = a.seq_lens != nullptr ? __ldg(a.seq_lens + b) : 0x7fffffff;  // nullptr: all of the table
+  int low = 0;  // window: the first key that the first row's window holds
+  if (a.window > 0) {
+    int64_t begin;
+    int rows;
+    clamp_range(a.cu, b, a.T, begin, rows);
+    low = max(n - rows - a.window + 1, 0);
+    // the key tiles between the first keys and the windows are nobody's
+    const unsigned sinks = static_cast<unsigned>(residue_row(a.sinks));
+    if (j >= sinks) j = max(sinks, static_cast<unsigned>(low) / 128 * 128) + (j - sinks);
+  }
+  if (j >= slots) return;
+  const unsigned row = b * slots + j;
   // what goes beside this key, and behind the last key up to the row's end
   const int64_t res_row = residue_row(slots);
   float* res = (second ? v_res : k_res) + (static_cast<int64_t>(b) * a.Hk + h0) * res_row;
@@ -240,17 +256,12 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
     for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i)
       for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
   if (c >= a.d) return;
-  const int n = a.seq_lens != nullptr ? __ldg(a.seq_lens + b) : 0x7fffffff;  // nullptr: all of the table
   bool there = n >= 0 && j < static_cast<unsigned>(n);
   if (a.window > 0) {
     // Left out where no row's window reaches, but for boxes that the reader loads whole: what lies beside a key that
     // counts meets a zero weight, and must not be NaN.
-    const int box = min(a.page & -a.page, 128);
-    int64_t begin;
-    int rows;
-    clamp_range(a.cu, b, a.T, begin, rows);
-    const int at = static_cast<int>(j) / box * box;
-    there = there && (at < a.sinks || at + box > n - rows - a.window + 1);
+    const int box = min(a.page & -a.page, 128), first = static_cast<int>(j) / box * box;
+    there = there && (first < a.sinks || first + box > low);
   }
   const int page = there ? __ldg(a.table + b * a.table_sB + j / a.page) : -1;
   if (page < 0 || page >= a.n_pages) {
@@ -528,17 +539,20 @@ cudaError_t launch_rotary_write(const RotaryArgs& r, int dtype, bool table16, cu
 
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
                                 cudaStream_t st) {
-  const int64_t groups = static_cast<int64_t>(p.B) * p.table_width * p.page * ((p.Hk + kHeads - 1) / kHeads);
+  int64_t per_seq = static_cast<int64_t>(p.table_width) * p.page;
+  // a window: the first keys' tiles, and from the first window's on what the rows can reach
+  if (p.window > 0) per_seq = std::min<int64_t>(per_seq, residue_row(p.sinks) + residue_row(p.window + p.T + 128));
+  const int64_t groups = p.B * per_seq * ((p.Hk + kHeads - 1) / kHeads);
   const int64_t ctas = (groups * 16 + kThreads - 1) / kThreads;
   if (groups >= (1LL << 28)) return cudaErrorInvalidConfiguration;  // the caller's limit keeps it below
   const dim3 grid(static_cast<unsigned>(ctas), 2u);
   if (ctas == 0) return cudaSuccess;
   if (dtype == kBF16)
     cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v),
-                                                   k_res, v_res);
+                                                   k_res, v_res, static_cast<unsigned>(per_seq));
   else
     cache_expand_kernel<<<grid, kThreads, 0, st>>>(p, static_cast<__half*>(k), static_cast<__half*>(v), k_res,
-                                                   v_res);
+                                                   v_res, static_cast<unsigned>(per_seq));
   return cudaGetLastError();
 }
 
