@@ -138,6 +138,7 @@ cudaError_t launch_paged_split(const PagedArgs& a, int dtype, int quantized, cud
 bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
 // far: far_bytes() of workspace for windows with first keys
 bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, void* far, cudaStream_t st, cudaError_t* e);
+bool launch_attn_tc_bwd_window(const AttnArgs& a, int dtype, void* far, cudaStream_t st, cudaError_t* e);
 int64_t far_bytes(const AttnArgs& a, int dtype);
 int attn_pack(int group);  // heads of a group that one row tile holds: its largest power of two
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
@@ -154,6 +155,7 @@ __host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);
 int read_device_error_tc_bwd(int clear);
+int read_device_error_tc_bwd_window(int clear);
 int read_device_error_cache(int clear);
 
 }  // namespace cta

@@ -337,9 +337,10 @@ int cta_device_error(int clear) {
   const int k = read_device_error_cache(clear);
   const int f = read_device_error_tc_fwd(clear);
   const int b = read_device_error_tc_bwd(clear);
-  for (int e : {a, c, d, p, k, f, b})
+  const int w = read_device_error_tc_bwd_window(clear);
+  for (int e : {a, c, d, p, k, f, b, w})
     if (e < 0) return -1;
-  for (int e : {a, c, d, p, k, f, b})
+  for (int e : {a, c, d, p, k, f, b, w})
     if (e != 0) return e;
   return 0;
 }
