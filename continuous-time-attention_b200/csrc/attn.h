@@ -136,12 +136,14 @@ cudaError_t launch_paged_split(const PagedArgs& a, int dtype, int quantized, cud
 
 // tensor-core forms; false = not for these types, sizes or strides (nothing was launched)
 bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
+bool launch_attn_tc_fwd_window(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e);
 // far: far_bytes() of workspace for windows with first keys
 bool launch_attn_tc_bwd(const AttnArgs& a, int dtype, void* far, cudaStream_t st, cudaError_t* e);
 bool launch_attn_tc_bwd_window(const AttnArgs& a, int dtype, void* far, cudaStream_t st, cudaError_t* e);
 int64_t far_bytes(const AttnArgs& a, int dtype);
 int attn_pack(int group);  // heads of a group that one row tile holds: its largest power of two
 bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
+bool launch_paged_tc_window(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
 // sums of all rows over the first `skip` keys of the table's first row
 int64_t prefix_tiles(const PagedArgs& p);  // CTAs for each part
 bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
@@ -154,6 +156,7 @@ __host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots
 
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);
+int read_device_error_tc_fwd_reach(int clear);
 int read_device_error_tc_bwd(int clear);
 int read_device_error_tc_bwd_window(int clear);
 int read_device_error_cache(int clear);

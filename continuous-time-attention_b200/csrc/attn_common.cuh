@@ -144,9 +144,9 @@ inline int num_sms_here() {
 // Launches a kernel.  `beside`: its CTAs may start as soon as all of the kernel in
 // front of it in the stream have started (that one calls pdl_launch_dependents,
 // and this one reads nothing of it), so that they fill the SMs that its last CTAs
-// leave idle; the last CTA calls wait_beside before it ends, so that the stream goes
-// on only when both are done.  (If all of them did, those that end early would hold
-// their SMs until the kernel in front is done.)
+// leave idle; every CTA calls pdl_wait before it ends, so that the stream goes on
+// only when both are done.  (One that does so is enough: where many end early, all
+// of them would hold their SMs until the kernel in front is done.)
 template <auto Kernel, typename... Args>
 cudaError_t launch_grid(bool beside, int64_t ctas, int threads, int smem, cudaStream_t st, const Args&... args) {
   const cudaError_t e = allow_smem<Kernel>(smem);
@@ -176,10 +176,6 @@ template <> __host__ __device__ constexpr float low_scale<__half>() { return 204
 template <typename T>
 __device__ __forceinline__ float lost(float x) {
   return (x - Elem<T>::to_f(Elem<T>::from_f(x))) * low_scale<T>();
-}
-
-__device__ __forceinline__ void wait_beside() {
-  if (blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // Sets rows behind the last sequence to zero, head h, `d` elements each.

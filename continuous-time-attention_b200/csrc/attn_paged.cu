@@ -610,7 +610,9 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? ((FP8 && !CUT) || DP == 
     u += count;
     first = false;
   }
-  if (CUT) wait_beside();  // the prefix's sums; the join's wait for this kernel's end covers theirs
+  // launched beside the prefix's sums: the join's wait for this kernel's end covers theirs.  By one CTA: the others' SMs
+  // are wanted for those that have not started.
+  if (CUT && blockIdx.x == gridDim.x - 1) pdl_wait();
 }
 
 // Joins the parts of one (row, head): the warps of the CTA take the parts in turn, then join theirs in order.

@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
   const SeqTile t = block_tile(a, blockIdx.x / a.H, kSimtRows, a.causal);
   if (t.first >= t.n) {
     if (a.cu != nullptr) zero_rows<T>(a.dq, a.dqs, t.row0, a.L, h, a.d, t.tail_index, t.tail_count);
-    wait_beside();
+    pdl_wait();
     return;
   }
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
 #pragma unroll
   for (int r = 0; r < R; ++r) mul[r] = a.scale;
   store_rows<T, R, DC>(a.dq, a.dqs, t, h, acc, mul, a.d, ty, tx);
-  wait_beside();  // dK and dV
+  pdl_wait();  // launched beside dK and dV
 }
 
 // owns KT keys of one key/value head; rows of the score tile are keys, columns are queries

@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   if (warp == kWeightWarps) tc::dealloc(tmem, 512);
-  wait_beside();  // dK and dV
+  pdl_wait();  // launched beside dK and dV
 }
 
 // ---------------------------------------------------------------------------

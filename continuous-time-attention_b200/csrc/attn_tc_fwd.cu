@@ -43,7 +43,7 @@
 // 4 chunks of 512 rows over 1500 to 8192 cached keys, 32/8 heads of 128: 162 us.
 #include <algorithm>
 
-#include "attn_tc.cuh"
+#include "attn_tc_fwd.cuh"
 
 namespace cta {
 
@@ -51,19 +51,12 @@ __device__ int g_tc_fwd_error;
 
 namespace {
 
-constexpr int kThreads = 640;  // five warpgroups
-constexpr int kSoftmaxWarps = 16;
-constexpr int kRows = 128;  // rows of a tile, and keys of a step
-constexpr float kLazy = 8.f;
-// fp16 weights carry 2^7, and so stay below 2^15; what is lost to subnormals is below 2^-32 of the reference
-constexpr float kHalfShift = 7.f;
-static_assert(kHalfShift == 7.f, "lse takes 2^-7 of the sum");
+using namespace tcfwd;
 
 struct FwdArgs {
   AttnArgs a;
   int pack;          // heads per tile row block
   int tile_tokens;   // kRows / pack
-  int warp_span;     // tokens from a warp's first row to its last
   int across;        // order of the work, see find_tile
   // paged keys
   const int32_t* table;
@@ -75,62 +68,9 @@ struct FwdArgs {
   const float* k_res;
   const float* v_res;
   int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
-  // shared prefix: `splits` parts of `chunk` keys (whole tiles), whose sums go to part_o [splits, rows, heads, DP] and
-  // part_ml [splits, rows, heads, 4] as the split kernel leaves them (attn_paged.cu)
-  int splits, chunk, prefix;
-  int64_t most_keys;  // of a sequence
-  float* part_o;
-  float* part_ml;
 };
 
-// What the rows see.  kPrefix: all rows of a batch over the pages that it begins with.
-enum Form : int { kPlain = 0, kWindow = 1, kPrefix = 2 };
-
-template <int DP>
-struct Layout {
-  static constexpr int kHalf = kRows * 128;            // one 64-column block of a 128-row tile
-  static constexpr int kTile = kHalf * (DP / 64);
-  static constexpr int kStages = DP == 128 ? 4 : 6;
-  static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
-};
-
-struct Bars {
-  uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t item_full, item_taken, answer;
-};
-
-// One piece of work: two row tiles of one block of heads.
-struct Item {
-  SeqTile t;
-  int h0, hk;  // first query head, key/value head
-  int n;       // keys of the sequence
-  int lo, hi;  // first and one past the last that may be valid
-  bool last;   // there is no more work
-};
-
-// kPrefix: the last key that row `tok` sees, by its own sequence's length; rows behind the last sequence do not count
-__device__ __forceinline__ int last_key(const FwdArgs& f, int tok) {
-  const AttnArgs& a = f.a;
-  int b = tok, from = tok, rows = 1;
-  if (a.cu != nullptr) {
-    // the last sequence that begins at or before the row
-    int lo = 0, hi = a.nseq;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(a.cu + mid + 1) > tok) hi = mid;
-      else lo = mid + 1;
-    }
-    if (lo == a.nseq) return 0x7fffffff;
-    b = lo;
-    int64_t begin;
-    clamp_range(a.cu, b, a.L, begin, rows);
-    from = static_cast<int>(begin);
-  }
-  const int n = static_cast<int>(min(static_cast<int64_t>(max(__ldg(f.seq_lens + b), 0)), f.most_keys));
-  return n - rows + tok - from;
-}
-
-template <typename T, int DP, bool PAGED, bool SCALED, int FORM>
+template <typename T, int DP, bool PAGED, bool SCALED>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_fwd_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ FwdArgs f) {
@@ -143,8 +83,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   // product within fp16 for any scales.
   constexpr bool kWeighted = SCALED && std::is_same<T, __half>::value;
   constexpr float kShift = std::is_same<T, __half>::value && !SCALED ? kHalfShift : 0.f;
-  // The keys' fractions carry scale * log2(e): one product less for each score.
-  constexpr bool kFolded = SCALED && FORM != kPlain;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
@@ -153,13 +91,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float s_max[2][2][kRows], s_sum[2][2][kRows];  // [tile][half of the keys][row]
   __shared__ float s_maxv[kWeighted ? 2 : 1][2][kWeighted ? kRows : 1];
   __shared__ uint32_t s_boxes[16];  // paged: which boxes of a key tile were loaded
-  // SCALED: the fractions of the key tiles in flight, keys' and values'.  They come with the values' tile, whose stage is
-  // free only when the weights that need them are in O, so four of them are more than are in flight.
-  __shared__ __align__(16) float s_res[SCALED ? 4 : 1][2][SCALED ? kRows : 1];
   const AttnArgs& a = f.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  if (FORM == kPrefix) pdl_launch_dependents();  // the split kernel's CTAs, for the sequences' own keys, may follow
 
   if (warp == kSoftmaxWarps) {
     tc::alloc(&s_tmem, 512);
@@ -204,45 +138,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     taken();
     return true;
   };
-  // steps of 128 keys of the two tiles; j0: the first key of the first
-  // kWindow: the tiles between the first keys and `from`, where the windows begin, are passed over
-  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j0, int& from, int& shift) {
-    shift = PAGED && FORM != kPrefix ? x.n - x.t.n : 0;
-    int tile = x.lo / kRows, jump = 1 << 30, gap = 0;
-    from = 0;
-    if constexpr (FORM == kWindow) {
-      const int window_tile = max(tile, max(x.t.first + shift - a.window + 1, 0) / kRows);
-      if (a.sinks == 0) {
-        tile = window_tile;
-      } else {
-        const int sink_tiles = (x.lo + a.sinks + kRows - 1) / kRows;
-        if (window_tile > sink_tiles) jump = sink_tiles - tile, gap = window_tile - sink_tiles;
-      }
-      from = window_tile * kRows;
-    }
-    j0 = tile * kRows;
+  // steps of 128 keys of the two tiles; j_lo: the first
+  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j_lo, int& shift) {
+    shift = PAGED ? x.n - x.t.n : 0;
+    j_lo = x.lo / kRows;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       first[i] = x.t.first + i * f.tile_tokens;
       int end = x.hi;
       if (a.causal) end = min(end, min(first[i] + f.tile_tokens, x.t.n) + shift);
-      int n = (end + kRows - 1) / kRows - tile;
-      if (FORM == kWindow && n > jump) n = max(jump, n - gap);
-      steps[i] = first[i] < x.t.n ? max(0, n) : 0;
+      steps[i] = first[i] < x.t.n ? max(0, (end + kRows - 1) / kRows - j_lo) : 0;
     }
-  };
-  // first keys that stay visible to all: those before this one
-  auto sinks_of = [&](const Item& x) { return FORM == kWindow && a.sinks > 0 ? x.lo + a.sinks : 0; };
-  // A step of first keys alone, up to 32 of them, takes a quarter of the products.  It pays where the softmax skips what
-  // no row of a warp sees, which it does not at dim 128 over 16 bits: each step waits for the other tile there, and the
-  // votes cost more than they save (12 prompts of up to 4096 tokens, 32/8 heads of 128, window 512: 451 and 424 us; 16384
-  // tokens, 8 heads of 64, window 1024: 101 and 104; chunks of 512 over e4m3: 101 and 111).
-  constexpr bool kSkip = FORM == kWindow && (SCALED || DP == 64);
-  auto narrow = [&](int j0, int from, int sink_end) { return kSkip && j0 < from && sink_end - j0 <= 32; };
-  // to the next tile
-  auto advance = [&](int& j0, int from, const Item& x) {
-    j0 += kRows;
-    if (FORM == kWindow && j0 >= sinks_of(x)) j0 = max(j0, from);
   };
   // bit c of word i: key 32 i + c of the tile at j0 is one of the sequence's and valid; `kt`: running number of the tile
   auto key_words = [&](int n, const uint32_t* mask, int j0, int kt, uint32_t (&w)[4]) {
@@ -289,31 +195,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int hb = id % blocks;
         x.h0 = hb * f.pack;
         x.hk = x.h0 / (a.H / a.Hk);
-        if constexpr (FORM == kPrefix) {
-          const int y = id / blocks, part = y % f.splits;
-          x.t.n = static_cast<int>(a.L);
-          x.t.first = y / f.splits * 2 * f.tile_tokens;
-          x.lo = part * f.chunk;
-          // what lies behind the longest sequence may hold anything
-          int longest = 0;
-          for (int b = lane; b < a.nseq; b += 32) longest = max(longest, __ldg(f.seq_lens + b));
-          longest = __reduce_max_sync(0xffffffffu, longest);
-          x.n = x.hi = min(min(f.prefix, x.lo + f.chunk), longest);
-        } else {
-          x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
-                          f.seq_lens);
-          x.n = x.hi = x.t.n;
-          if constexpr (PAGED) {
-            if (x.t.first < x.t.n) {
-              x.n = __ldg(f.seq_lens + x.t.seq);
-              const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
-              if ((x.n < 0 || x.n > most) && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
-              x.n = x.n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(x.n), most));
-            }
-            x.hi = x.n;
-          } else {
-            mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
+        x.t = find_tile(a.cu, a.nseq, a.L, a.tiles, id / blocks, 2 * f.tile_tokens, a.causal, f.across,
+                        f.seq_lens);
+        x.n = x.hi = x.t.n;
+        if constexpr (PAGED) {
+          if (x.t.first < x.t.n) {
+            x.n = __ldg(f.seq_lens + x.t.seq);
+            const int64_t most = static_cast<int64_t>(f.table_width) * f.page;
+            if ((x.n < 0 || x.n > most) && lane == 0) atomicExch(&g_tc_fwd_error, kDevBadIndex);
+            x.n = x.n < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(x.n), most));
           }
+          x.hi = x.n;
+        } else {
+          mask_range(a, x.t.batch, x.t.n, x.lo, x.hi);
         }
       }
       if (lane == 0) {
@@ -332,8 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = read_item(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
       const int all = max(steps[0], steps[1]);
       if (all == 0) {
         taken();
@@ -355,14 +249,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const CUtensorMap* map = (y & 1) ? &vmap : &kmap;
         const uint32_t dst = smem + (2 + stage) * L::kTile;
+        const int j0 = (j_lo + (y >> 1)) * kRows;
         if constexpr (PAGED) {
           // one lane per box; a box outside the sequence or the cache is left out
           const int boxes = kRows / f.box;
           const int key = j0 + lane * f.box;
           int page = -1;
-          // no row's window reaches it: the page may be gone
-          const bool reached = FORM != kWindow || key < a.sinks || key + f.box > x.t.first + shift - a.window + 1;
-          if (lane < boxes && key < x.n && reached) {
+          if (lane < boxes && key < x.n) {
             page = __ldg(f.table + x.t.seq * f.table_sB + key / f.page);
             if (page < 0 || page >= f.n_pages) {
               atomicExch(&g_tc_fwd_error, kDevBadIndex);
@@ -379,13 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b = 0; b < boxes; ++b)
               if ((got >> b) & 1u) bits |= ((1u << per) - 1u) << (b * per);
             *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kv >> 1) & 15]) = bits;
-            const bool res = SCALED && (y & 1);
-            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64) + (res ? 8 * kRows : 0));
-            if (res) {
-              const int64_t at = (static_cast<int64_t>(x.t.seq) * a.Hk + x.hk) * residue_row(f.table_width * f.page) + j0;
-              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][0]), f.k_res + at, 4 * kRows, &bars.kv_full[stage]);
-              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][1]), f.v_res + at, 4 * kRows, &bars.kv_full[stage]);
-            }
+            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64));
           }
           __syncwarp();
           if (page >= 0)
@@ -398,7 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::tma_load_4d(dst + c * L::kHalf, map, &bars.kv_full[stage], 64 * c, x.hk,
                             static_cast<int>(x.t.row0) + j0, x.t.batch);
         }
-        if (y & 1) advance(j0, from, x);
         ++kv;
       }
       taken();
@@ -415,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // both tiles those of one tile delayed the other's products (562 instead of 503 us at 8192 keys,
     // 16 heads of 128, 477 instead of 402 at 64).  Both free a key tile.
     const int i = warp == kSoftmaxWarps ? 0 : 1;
-    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_32 = tc::idesc<T>(32, false), id_o = tc::idesc<T>(DP, true);
+    constexpr uint32_t id_s = tc::idesc<T>(kRows, false), id_o = tc::idesc<T>(DP, true);
     const bool leader = tc::elect_one();
     bool ok = true;
     int kv = 0, nq = 0, ns = 0;  // running numbers: tiles, Q loads, steps of this row tile
@@ -424,8 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
       const int all = max(steps[0], steps[1]), mine = i == 0 ? steps[0] : steps[1];
       if (all == 0) continue;
       ok = tc::wait(&bars.q_full, nq & 1);
@@ -433,28 +319,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
       auto kv_wait = [&](int y) { ok = ok && tc::wait(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
       auto kv_addr = [&](int y) { return smem + (2 + (kv + y) % NS) * L::kTile; };
-      const int sink_end = sinks_of(x);
       // scores of step j into the tile's buffer; keys are released by the step's end
-      auto scores = [&](int j, int at) {
-        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), narrow(at, from, sink_end) ? id_32 : id_s);
+      auto scores = [&](int j) {
+        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), id_s);
         tc::commit(&bars.s_full[i]);
         if (j + 1 == mine) tc::commit(&bars.q_empty);
       };
       kv_wait(0);
       tc::fence_after();
       if (ok && leader) {
-        if (mine > 0) scores(0, j0);
+        if (mine > 0) scores(0);
         else tc::commit(&bars.q_empty);
         tc::commit(&bars.kv_empty[kv % NS]);
       }
       __syncwarp();
-      for (int j = 0; j < all && ok; ++j, advance(j0, from, x)) {
+      for (int j = 0; j < all && ok; ++j) {
         kv_wait(2 * j + 1);
         if (j + 1 < all) kv_wait(2 * j + 2);
         if (!ok) break;
         if (j < mine) {
           // values of keys that are not there or not valid may hold anything
           uint32_t w[4];
+          const int j0 = (j_lo + j) * kRows;
           if (PAGED || mask != nullptr || j0 + kRows > x.n) {
             key_words(x.n, mask, j0, (kv >> 1) + j, w);
             if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
@@ -465,15 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && tc::wait(&bars.p_full[i], ns & 1);
           tc::fence_after();
           if (ok && leader) {
-            if (narrow(j0, from, sink_end)) tc::product_tn<64, 2>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
-            else tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
-            if (j + 1 == mine) {
-              tc::commit(&bars.o_full[i]);
-            } else {
-              int at = j0;
-              advance(at, from, x);
-              scores(j + 1, at);
-            }
+            tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            if (j + 1 == mine) tc::commit(&bars.o_full[i]);
+            else scores(j + 1);
           }
           ++ns;
         }
@@ -495,15 +375,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + i * kRows + half * 64;
     const uint32_t o_addr = tmem + lanes + 2 * kRows + i * DP + half * (DP / 2);
-    const float c2 = kFolded ? 1.f : a.scale * kLog2e;
+    const float c2 = a.scale * kLog2e;
     bool ok = true;
     int ns = 0, no = 0, kt = 0;  // running numbers: steps, outputs, key tiles
     for (int it = 0; ok; ++it) {
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
+      int first[2], steps[2], j_lo, shift;
+      plan(x, first, steps, j_lo, shift);
       const int mine = i == 0 ? first[0] : first[1], count = i == 0 ? steps[0] : steps[1];
       const int all = max(steps[0], steps[1]);
       if (!PAGED && a.cu != nullptr && a.zero_tail && warp < 4 && x.t.n == 0) {
@@ -520,32 +400,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
       const int tok = mine + row / f.pack, h = x.h0 + row % f.pack;
       const bool live = tok < x.t.n;
-      int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
-      int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
-      if constexpr (FORM == kPrefix) {
-        // of its own sequence, which may end here
-        limit = live ? min(n - 1, last_key(f, tok)) : n - 1;
-        limit_all = __reduce_min_sync(0xffffffffu, limit);
-      }
+      const int limit = a.causal ? tok + shift : n - 1;  // last key the row sees
+      const int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // causal: last key all rows of the warp see
       T* out = static_cast<T*>(a.o) + x.t.batch * a.os.b + (x.t.row0 + tok) * a.os.t + h * a.os.h;
       float* lse = live && half == 0 && a.lse != nullptr ? a.lse + lse_index(a, x.t, h, tok) : nullptr;
-      const int sink_end = sinks_of(x);
+      // the first fraction of this half's keys
+      int res = SCALED ? (x.t.seq * a.Hk + x.hk) * static_cast<int>(residue_row(f.table_width * f.page)) +
+                             j_lo * kRows + 64 * half
+                       : 0;
       float m = neg_inf(), sum = 0.f;
       float mv = neg_inf();  // kWeighted: the reference of weight * scale, as an exponent of two
-      for (int j = 0; j < count; ++j, ++ns, advance(j0, from, x)) {
+      for (int j = 0; j < count; ++j, ++ns, res += SCALED ? kRows : 0) {
+        if (SCALED && lane < 4)  // two lines each of the step's fractions
+          asm volatile("prefetch.global.L1 [%0];" ::"l"((lane < 2 ? f.k_res : f.v_res) + res + 32 * (lane & 1)));
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
         ok = ok && tc::wait(&bars.s_full[i], ns & 1);
-        if (SCALED) ok = ok && tc::wait(&bars.kv_full[(2 * (kt + j) + 1) % NS], ((2 * (kt + j) + 1) / NS) & 1);
         tc::fence_after();
+        const int j0 = (j_lo + j) * kRows;
         uint32_t s[2][32];
         if (!SCALED) {
           tc::ld32(s_addr, s[0]);
           tc::ld32(s_addr + 32, s[1]);
         }
         // warp-uniform: every row of the warp sees all keys of the tile
-        bool whole = j0 + kRows <= n && ((FORM != kPrefix && !a.causal) || j0 + kRows - 1 <= limit_all) &&
-                     (FORM != kWindow || j0 > limit_all + f.warp_span - a.window || j0 + kRows <= sink_end);
+        bool whole = j0 + kRows <= n && (!a.causal || j0 + kRows - 1 <= limit_all);
         uint32_t w[4];
         if (PAGED || mask != nullptr || !whole) {
           key_words(n, mask, j0, kt + j, w);
@@ -553,17 +432,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!SCALED) tc::wait_ld(s[0], s[1]);
         // Fractions of the scales, 32 keys at a time: the scores are read from tensor memory once for the maximum and
-        // once for the weights, for want of registers.  From shared memory, where the loads' warp puts them: the
-        // softmax waited for them 56 % of its time when each warp fetched them (512 rows of 4 sequences in windows
-        // of 1024, 32/8 heads of 128: 106 and 83 us; 128 rows in fp16 over a prefix of 16384: 120 and 93).
-        auto fractions = [&](int of, int c, float4 (&r)[8]) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) r[e] = *reinterpret_cast<const float4*>(&s_res[(kt + j) & 3][of][64 * half + 32 * c + 4 * e]);
-        };
+        // once for the weights, which leaves registers for eight loads.  Bound by issue (77 % of the cycles of a busy
+        // SM); with one read of both the loads wait for one another instead, 205 and 199 us for 32 chunks of 16
+        // rows over 2048 keys.
         auto scale = [&](int c, uint32_t (&x)[32]) {
           tc::ld32(s_addr + 32 * c, x);
           float4 r[8];
-          fractions(0, c, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.k_res + res + 32 * c) + e);
           tc::wait_ld(x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -577,43 +453,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             x[4 * e + 3] = __float_as_uint(hi.y);
           }
         };
-        // false: none of these 32 keys counts for any row of the warp (kSkip; x is left as it is)
-        auto hide = [&](int c, uint32_t (&x)[32]) -> bool {
+        auto hide = [&](int c, uint32_t (&x)[32]) {
           const int left = limit - j0 - 64 * half - 32 * c + 1;
-          uint32_t see =
+          const uint32_t see =
               (half == 0 ? w[c] : w[2 + c]) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
-          if constexpr (FORM == kWindow) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - j0 - 64 * half - 32 * c);
-          if constexpr (kSkip) {
-            if (!__any_sync(0xffffffffu, see != 0u)) return false;
-            if (__all_sync(0xffffffffu, see == 0xffffffffu)) return true;
-          }
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!((see >> e) & 1u)) x[e] = 0xff800000u;
-          return true;
         };
-        bool some[2] = {true, true};
         float t[4], topv = mv;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t(&x)[32] = s[SCALED ? 0 : c];
           if (SCALED) scale(c, x);
-          if (!whole) some[c] = hide(c, x);
-          if (kSkip && !some[c]) {
-            t[2 * c] = t[2 * c + 1] = neg_inf();
-            continue;
-          }
+          if (!whole) hide(c, x);
           if constexpr (kWeighted) {
             // score + logarithm of the value's scale
             float4 r[8];
-            fractions(1, c, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float2 a0 = make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]));
-              const float2 a1 = make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
-              const float2 v0 = make_float2(r[e].x, r[e].y), v1 = make_float2(r[e].z, r[e].w);
-              const float2 lo = kFolded ? add2(a0, v0) : fma2(a0, f2(c2), v0);
-              const float2 hi = kFolded ? add2(a1, v1) : fma2(a1, f2(c2), v1);
+              const float2 lo = fma2(make_float2(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1])), f2(c2),
+                                     make_float2(r[e].x, r[e].y));
+              const float2 hi = fma2(make_float2(__uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3])), f2(c2),
+                                     make_float2(r[e].z, r[e].w));
               topv = tc::max3(tc::max3(lo.x, lo.y, hi.x), hi.y, topv);
             }
           }
@@ -675,19 +539,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t p[16];
           uint32_t(&x)[32] = s[SCALED ? 0 : c];
           float4 r[SCALED ? 8 : 1];
-          if (kSkip && !some[c]) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) p[e] = 0u;
-          } else {
           if constexpr (SCALED) {
             scale(c, x);
             if (!whole) hide(c, x);
-            fractions(1, c, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) r[e] = __ldg(reinterpret_cast<const float4*>(f.v_res + res + 32 * c) + e);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 score = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-            float2 y = kFolded ? add2(score, bv) : fma2(score, c2v, bv);
+            float2 y = fma2(score, c2v, bv);
             y.x = ex2(y.x);
             y.y = ex2(y.y);
             if (e & 1) part2 = add2(part2, y);
@@ -696,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float4& z = r[e / 2];
               const float2 of_value = (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
               if constexpr (kWeighted) {
-                y = kFolded ? add2(score, add2(of_value, vv)) : fma2(score, c2v, add2(of_value, vv));
+                y = fma2(score, c2v, add2(of_value, vv));
                 y.x = ex2(y.x);
                 y.y = ex2(y.y);
               } else {
@@ -704,7 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             p[e] = tc::pack2<T>(y.x, y.y);
-          }
           }
           // over this half's own scores: the other half may not have read its yet
           tc::st16(s_addr + 16 * c, p);
@@ -730,18 +590,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         sum += s_sum[i][half ^ 1][row];
       }
-      if constexpr (FORM == kPrefix) {
-        // The part's sums as they are.  The join takes it that values of half products carry 2^7; bf16 weights over e4m3
-        // codes do not.
-        constexpr float kUnit = SCALED && !kWeighted ? 128.f : 1.f;
-        const int64_t at = (static_cast<int64_t>(x.lo / f.chunk) * a.L + tok) * a.H + h;
-        tc::store_floats<DP / 2>(o_addr, f.part_o + at * DP + half * (DP / 2), kUnit, live, count > 0);  // or the part lies behind all sequences
-        if (live && half == 0)
-          *reinterpret_cast<float4*>(f.part_ml + at * 4) =
-              make_float4(m * c2, kShift == 0.f ? sum : sum * 0x1p-7f, kWeighted ? mv : m * c2, 0.f);
-        tc::fence_before();
-        continue;
-      }
       // the factor between the references, which a scale past 2^120 takes out of fp32's range, and fp16's anyway
       const float unit = kWeighted ? ex2(fminf(mv - kHalfShift - m * c2, 127.f)) : 1.f;
       const float inv = sum > 0.f ? unit / sum : sum == 0.f ? 0.f : sum;  // NaN stays
@@ -761,20 +609,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kSoftmaxWarps) tc::dealloc(tmem, 512);
 }
 
-template <typename T, int DP, bool PAGED, bool SCALED, int FORM>
+template <typename T, int DP, bool PAGED, bool SCALED>
 cudaError_t launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int64_t ctas,
                    cudaStream_t st) {
-  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED, SCALED, FORM>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
+  return launch_grid<attn_tc_fwd_kernel<T, DP, PAGED, SCALED>>(false, ctas, kThreads, Layout<DP>::kSmem, st, q, k, v, f);
 }
 
-template <bool PAGED, bool SCALED, int FORM>
+template <bool PAGED, bool SCALED>
 cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const FwdArgs& f, int dtype,
                      int64_t ctas, cudaStream_t st) {
   if (dtype == kBF16)
-    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED, SCALED, FORM>(q, k, v, f, ctas, st)
-                       : launch<__nv_bfloat16, 128, PAGED, SCALED, FORM>(q, k, v, f, ctas, st);
-  return f.a.d <= 64 ? launch<__half, 64, PAGED, SCALED, FORM>(q, k, v, f, ctas, st)
-                     : launch<__half, 128, PAGED, SCALED, FORM>(q, k, v, f, ctas, st);
+    return f.a.d <= 64 ? launch<__nv_bfloat16, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
+                       : launch<__nv_bfloat16, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
+  return f.a.d <= 64 ? launch<__half, 64, PAGED, SCALED>(q, k, v, f, ctas, st)
+                     : launch<__half, 128, PAGED, SCALED>(q, k, v, f, ctas, st);
 }
 
 }  // namespace
@@ -782,12 +630,12 @@ cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorM
 int attn_pack(int group) { return std::min(group & -group, kRows); }
 
 bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError_t* e) {
+  if (a.window > 0) return launch_attn_tc_fwd_window(a, dtype, st, e);
   if (dtype == kF32 || a.d % 8 != 0 || a.d > 128 || !(a.scale > 0.f)) return false;
   FwdArgs f = {};
   f.a = a;
   f.pack = attn_pack(a.H / a.Hk);
   f.tile_tokens = kRows / f.pack;
-  f.warp_span = 31 / f.pack;
   const int64_t nb = a.cu != nullptr ? 1 : a.nseq;
   CUtensorMap q, k, v;
   if (!attn_map(&q, a.q, dtype, nb, a.L, a.H, a.d, a.qs, f.pack, f.tile_tokens) ||
@@ -810,16 +658,14 @@ bool launch_attn_tc_fwd(const AttnArgs& a, int dtype, cudaStream_t st, cudaError
   // the keys' sake (24 such sequences, 32/8 heads, three times the pieces: 281 and 266 us).
   const int64_t pieces = tiles * (a.H / f.pack);
   f.across = a.cu != nullptr || (a.causal && pieces <= 12 * num_sms_here());
-  *e = a.window > 0 ? dispatch<false, false, kWindow>(q, k, v, f, dtype, pieces, st)
-                    : dispatch<false, false, kPlain>(q, k, v, f, dtype, pieces, st);
+  *e = dispatch<false, false>(q, k, v, f, dtype, pieces, st);
   return true;
 }
 
-namespace {
-
-// what chunks and prefixes have in common: the tensors and the pages
-bool paged_maps(const PagedArgs& p, int dtype, FwdArgs& f, CUtensorMap (&maps)[3]) {
-  if (!(p.scale > 0.f)) return false;
+bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
+  if (p.window > 0) return launch_paged_tc_window(p, dtype, st, e);
+  if (!(p.scale > 0.f) || p.cu == nullptr) return false;
+  FwdArgs f = {};
   AttnArgs& a = f.a;
   a.q = p.q;
   a.o = p.o;
@@ -831,73 +677,36 @@ bool paged_maps(const PagedArgs& p, int dtype, FwdArgs& f, CUtensorMap (&maps)[3
   a.H = p.H;
   a.Hk = p.Hk;
   a.d = p.d;
+  a.causal = 1;
   a.scale = p.scale;
   f.pack = attn_pack(p.H / p.Hk);
   f.tile_tokens = kRows / f.pack;
-  f.warp_span = 31 / f.pack;
   f.table = p.table;
   f.table_sB = p.table_sB;
   f.seq_lens = p.seq_lens;
+  f.across = 1;
   f.table_width = p.table_width;
   f.page = p.page;
   f.n_pages = p.n_pages;
   f.k_res = p.k_res;
   f.v_res = p.v_res;
   f.box = std::min(p.page & -p.page, kRows);  // the largest power of two that divides a page
+  f.wide_out = row_alignment(a.o, a.os, 1, a.H);
   // expanded pages are contiguous
-  const int64_t pages = p.k_res != nullptr ? p.expanded_pages : p.n_pages;
+  const int64_t pages = p.k_res != nullptr ? static_cast<int64_t>(p.B) * p.table_width : p.n_pages;
   const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
   const AttnStrides ks = p.k_res != nullptr ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
   const AttnStrides vs = p.k_res != nullptr ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
-  return attn_map(&maps[0], p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) &&
-         attn_map(&maps[1], p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) &&
-         attn_map(&maps[2], p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box);
-}
-
-}  // namespace
-
-bool launch_paged_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
-  if (p.cu == nullptr) return false;
-  FwdArgs f = {};
-  CUtensorMap m[3];
-  if (!paged_maps(p, dtype, f, m)) return false;
-  f.a.causal = 1;
-  f.a.window = p.window;
-  f.a.sinks = p.sinks;
-  f.across = 1;
-  f.wide_out = row_alignment(f.a.o, f.a.os, 1, f.a.H);
+  CUtensorMap q, k, v;
+  if (!attn_map(&q, p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) ||
+      !attn_map(&k, p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) ||
+      !attn_map(&v, p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box))
+    return false;
   const int64_t tiles = packed_tiles(p.T, p.B, 2 * f.tile_tokens);
-  f.a.tiles = static_cast<int>(tiles);
+  a.tiles = static_cast<int>(tiles);
   const int64_t pieces = tiles * (p.H / f.pack);
-  if (p.window > 0)
-    *e = p.k_res != nullptr ? dispatch<true, true, kWindow>(m[0], m[1], m[2], f, dtype, pieces, st)
-                            : dispatch<true, false, kWindow>(m[0], m[1], m[2], f, dtype, pieces, st);
-  else
-    *e = p.k_res != nullptr ? dispatch<true, true, kPlain>(m[0], m[1], m[2], f, dtype, pieces, st)
-                            : dispatch<true, false, kPlain>(m[0], m[1], m[2], f, dtype, pieces, st);
-  return true;
-}
-
-// row tiles of 256 (row, head) pairs
-int64_t prefix_tiles(const PagedArgs& p) {
-  const int64_t rows = 2 * (kRows / attn_pack(p.H / p.Hk));
-  return (p.T + rows - 1) / rows * (p.H / attn_pack(p.H / p.Hk));
-}
-
-bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
-  FwdArgs f = {};
-  CUtensorMap m[3];
-  if (!paged_maps(p, dtype, f, m)) return false;
-  f.splits = p.prefix_splits;
-  f.chunk = p.prefix_chunk;
-  f.prefix = p.skip;
-  f.table_width = p.skip / p.page;
-  f.most_keys = static_cast<int64_t>(p.table_width) * p.page;
-  f.part_o = p.prefix_o;
-  f.part_ml = p.prefix_ml;
-  const int64_t pieces = prefix_tiles(p) * f.splits;
-  *e = p.k_res != nullptr ? dispatch<true, true, kPrefix>(m[0], m[1], m[2], f, dtype, pieces, st)
-                          : dispatch<true, false, kPrefix>(m[0], m[1], m[2], f, dtype, pieces, st);
+  *e = p.k_res != nullptr ? dispatch<true, true>(q, k, v, f, dtype, pieces, st)
+                          : dispatch<true, false>(q, k, v, f, dtype, pieces, st);
   return true;
 }
 

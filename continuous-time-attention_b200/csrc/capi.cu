@@ -337,10 +337,11 @@ int cta_device_error(int clear) {
   const int k = read_device_error_cache(clear);
   const int f = read_device_error_tc_fwd(clear);
   const int b = read_device_error_tc_bwd(clear);
+  const int r = read_device_error_tc_fwd_reach(clear);
   const int w = read_device_error_tc_bwd_window(clear);
-  for (int e : {a, c, d, p, k, f, b, w})
+  for (int e : {a, c, d, p, k, f, b, r, w})
     if (e < 0) return -1;
-  for (int e : {a, c, d, p, k, f, b, w})
+  for (int e : {a, c, d, p, k, f, b, r, w})
     if (e != 0) return e;
   return 0;
 }

@@ -32,8 +32,8 @@ LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = [
     "bld_fwd_bf16_fm.cu", "bld_fwd_f16_fm.cu", "bld_fwd_bf16.cu", "bld_fwd_f16.cu", "bld_fwd_f32.cu",
     "bld_dalpha_bf16_fm.cu", "bld_dalpha_f16_fm.cu", "bld_dalpha_bf16.cu", "bld_dalpha_f16.cu",
-    "bld_dalpha_f32.cu", "stencil_bdl.cu", "attn_simt.cu", "attn_paged.cu", "attn_tc_fwd.cu", "attn_tc_bwd.cu",
-    "attn_tc_bwd_window.cu", "kv_cache.cu",
+    "bld_dalpha_f32.cu", "stencil_bdl.cu", "attn_simt.cu", "attn_paged.cu", "attn_tc_fwd.cu",
+    "attn_tc_fwd_reach.cu", "attn_tc_bwd.cu", "attn_tc_bwd_window.cu", "kv_cache.cu",
     "capi.cu", "attn_capi.cu", "bld_fwd.cu", "bld_dalpha.cu", "noalloc.cu",
 ]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
