@@ -4,7 +4,8 @@
 (``cta_b200.transformers``, ``attention="fused"``) and of packed prefill
 batches, whose output the mixer (``cta_b200.serving_vllm``) refines: padded
 [B, L, heads, dim] with a key mask, or packed [T, heads, dim] with offsets;
-causal or not, or causal within a sliding window whose first tokens stay visible; grouped key/value heads; float32, bfloat16, float16.
+causal or not, or causal within a sliding window whose first tokens stay visible;
+grouped key/value heads; float32, bfloat16, float16.
 """
 from __future__ import annotations
 
@@ -18,9 +19,16 @@ from . import ops
 __all__ = ["prompt_attention"]
 
 
+_EVERY = (0, 0)  # no window
+
+
 class _PromptAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale, reach):
+    def forward(ctx, q, k, v, mask_words, cu_seqlens, causal, scale):
+        # causal: False, True, or the window and sinks of a causal window (each argument costs a call its time)
+        reach = _EVERY
+        if type(causal) is tuple:
+            reach, causal = causal, True
         q, k, v, cu, sizes, code, scale = ops._attention_inputs(q, k, v, cu_seqlens, mask_words, scale)
         out = ops._new(q)
         # what rounding the output loses: delta of rows with few keys needs it
@@ -39,7 +47,7 @@ class _PromptAttention(torch.autograd.Function):
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq, dk, dv = ops._attention_backward(grad_out, q, k, v, out, 0 if low is None else low.data_ptr(), lse, cu,
                                              mask_words, *ctx.plan, need_q, need_k or need_v)
-        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None, None
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
 def _tangents(*tensors: torch.Tensor) -> bool:
@@ -77,7 +85,8 @@ def prompt_attention(
     infinities and NaN included; a NaN or infinity in the k or v of a valid token may
     also reach rows of its sequence that do not see it, one in the q or the output
     gradient of a row the gradients of keys that it does not see.  Forward-mode differentiation raises."""
-    reach = ops._window(window, sinks, causal)
+    if window is not None or sinks:
+        reach = ops._window(window, sinks, causal)
     words = mask_words
     if key_mask is not None:
         if words is not None:
@@ -88,6 +97,6 @@ def prompt_attention(
             raise ValueError(f"key_mask on {key_mask.device}, expected {q.device}")
         words = ops.attention_mask(key_mask)
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _tangents(q, k, v):
-        return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal), scale, reach)
+        return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal) if window is None else reach, scale)
     return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens,
                                  need_lse=False, window=window, sinks=sinks)[0]
