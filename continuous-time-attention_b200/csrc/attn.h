@@ -154,6 +154,7 @@ cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v,
 // entries of k_res and v_res for a sequence and head, in whole key tiles
 __host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots + 127) / 128 * 128; }
 
+int set_prefix_always(int value);  // use shared prefixes where that does not pay too; the value before
 int read_device_error_paged(int clear);
 int read_device_error_tc_fwd(int clear);
 int read_device_error_tc_fwd_reach(int clear);

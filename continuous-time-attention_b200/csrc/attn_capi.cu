@@ -4,6 +4,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
@@ -361,12 +362,21 @@ struct PrefixPlan {
   int64_t sums = 0, expanded = 0, bytes = 0;  // workspace: the parts, the expanded pages, all with the split kernel's
 };
 
+std::atomic<int> g_prefix_always{0};
+
 PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t shared) {
   PrefixPlan p;
   const int64_t width = a.table_width, keys = std::min(shared / a.page, width) * a.page;
   // the split kernel counts groups past the last key, hence 2^30
   if (a.T < 2 || keys < 1 || width * a.page >= (1LL << 30) || !(a.scale > 0.f) || !tma_can_address(a) || tensor_cores_pay(a) ||
       a.n_pages < 1)
+    return p;
+  // It costs a launch, two over e4m3, and the sums' way through memory, about what HBM takes for 40 (e4m3 64) MB.  32/8 heads
+  // of 128, calls with and without it: 16 sequences behind 512 keys, 31 MB read again, 20.9 and 19.3 us, behind 1024, 63
+  // MB, 21.2 and 23.1; e4m3: behind 2048, 65 MB, 27.5 and 27.3, 64 sequences behind 1024, 136 MB, 31.6 and 41.8.
+  const int64_t again = std::max<int64_t>(a.B, (a.T * (a.H / a.Hk) + 15) / 16) - 1;
+  if (again * keys * 2 * a.Hk * (quantized ? a.d + 4 : 2 * a.d) < (quantized ? 64000000 : 40000000) &&
+      g_prefix_always.load(std::memory_order_relaxed) == 0)
     return p;
   const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
   // Both kernels run at once: the parts' CTAs, one per SM, leave the split kernel the other SMs, and their own when they
@@ -402,6 +412,8 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
 }
 
 }  // namespace
+
+int cta::set_prefix_always(int value) { return g_prefix_always.exchange(value != 0 ? 1 : 0); }
 
 extern "C" {
 

@@ -378,6 +378,8 @@ int cta_set_tuning(int key, int value) {
   } else if (key == 5) {
     prev = g_tuning.debug_stall_us;
     g_tuning.debug_stall_us = value > 0 ? std::min(value, 100000) : 0;
+  } else if (key == 6) {
+    prev = set_prefix_always(value);
   }
   return prev;
 }

@@ -62,7 +62,8 @@ int cta_device_error(int clear);
  * (default 0), key 5 = test of the timeout path: the first CTA of every
  * forward march waits this many microseconds (at most 100000) on an mbarrier
  * phase nothing completes, then reports the timeout in the device error word
- * and exits (default 0 = off).  Returns the previous value.  Process-wide, not
+ * and exits (default 0 = off), key 6 = a shared prefix is read once wherever it
+ * can be, not only where that pays (default 0).  Returns the previous value.  Process-wide, not
  * thread-safe against concurrent launches. */
 int cta_set_tuning(int key, int value);
 

@@ -15,9 +15,12 @@ DTYPES = [torch.bfloat16, torch.float16]
 
 @pytest.fixture(autouse=True)
 def no_device_error():
+    """The prefix is read once at these sizes too, where that need not pay."""
     from cta_b200 import _lib
 
+    before = _lib.set_tuning(6, 1)
     yield
+    _lib.set_tuning(6, before)
     assert _lib.device_error() == 0
 
 
@@ -187,6 +190,21 @@ def test_captured_and_replayed_together(quantized):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_where_it_pays(quantized):
+    """Small batches go without it, to the bit; large ones use it."""
+    from cta_b200 import _lib
+
+    _lib.set_tuning(6, 0)
+    s = Setup(512, [600, 530, 513], [1] * 3, 8, 2, 64, 16, torch.bfloat16, quantized, seed=8)
+    assert torch.equal(s.run(), s.run(shared_prefix=0))
+    n = 80
+    s = Setup(3200, [3200 + 1 + b % 7 for b in range(n)], [1] * n, 8, 2, 64, 64, torch.bfloat16, quantized, seed=9)
+    out = s.run()
+    s.check(out)
+    assert not torch.equal(out, s.run(shared_prefix=0))
 
 
 def test_empty():

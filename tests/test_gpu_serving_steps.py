@@ -91,6 +91,7 @@ def test_prompts_chunks_and_decode(window, sinks, heads, kv_heads, dim, rotary, 
 @pytest.mark.parametrize("quantized", [False, True])
 def test_shared_prefix(quantized):
     """A prompt is prefilled once, other sequences go on from its pages."""
+    from cta_b200 import _lib
     from cta_b200.serving_vllm import CtaConfig, CtaPostAttnMixer
 
     mixer = CtaPostAttnMixer(CtaConfig(enabled=False))
@@ -100,9 +101,10 @@ def test_shared_prefix(quantized):
     server.check(mixer.attend(q, k, v, server.kc, server.vc, attn_metadata=md, **kw).view(-1, 8, 128), q, {0: 640})
     for s in range(1, 40):
         server.pages[s], server.k[s], server.v[s] = list(server.pages[0]), server.k[0], server.v[0]
-    for step in range(3):
+    for step in range(4):
         new = {s: (1 if step else 1 + s % 5) for s in range(40)}
         md, q, k, v = server.batch(new, step + 1, padding=2)
+        _lib.set_tuning(6, int(step < 3))
         out = mixer.attend(q, k, v, server.kc, server.vc, attn_metadata=md, shared_prefix=640, **kw)
         server.check(out.view(-1, 8, 128), q, new)
 
