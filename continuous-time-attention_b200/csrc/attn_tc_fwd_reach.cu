@@ -51,8 +51,16 @@ struct FwdArgs {
   float* part_ml;
 };
 
+// what the two tiles of a piece go through
+struct Plan {
+  int first[2], steps[2], stop[2];  // first rows, steps, where the keys end
+  int j0, edge, gap, shift;
+  __device__ __forceinline__ int key(int at) const { return at + (at >= edge ? gap : 0); }
+};
+
 // kPrefix: all rows of a batch over the pages that it begins with
 enum Form : int { kWindow = 0, kPrefix = 1 };
+constexpr int kBox = 32;  // kWindow: keys per TMA box, see plan
 
 // kPrefix: the last key that row `tok` sees, by its own sequence's length; rows behind the last sequence do not count
 __device__ __forceinline__ int last_key(const FwdArgs& f, int tok) {
@@ -150,58 +158,56 @@ __global__ void __launch_bounds__(kThreads, 1)
     taken();
     return true;
   };
-  // steps of 128 keys of the two tiles; j0: the first key of the first
-  // kWindow: the tiles between the first keys and `from`, where the windows begin, are passed over
-  auto plan = [&](const Item& x, int (&first)[2], int (&steps)[2], int& j0, int& from, int& shift) {
-    shift = PAGED && FORM != kPrefix ? x.n - x.t.n : 0;
-    int tile = x.lo / kRows, jump = 1 << 30, gap = 0;
-    from = 0;
+  // Steps of 128 keys of the two tiles, from j0 on.  kWindow: the keys between the first ones and the windows are passed
+  // over: the keys from `edge` on stand for those `gap` further on, so that a step may hold the first keys and where the
+  // windows begin.  Words of 32 keys lie on one side.  (With the first keys in steps of their own, and windows from the
+  // beginning of a whole tile: TODO1.)
+  auto plan = [&](const Item& x) {
+    Plan y;
+    y.shift = PAGED && FORM != kPrefix ? x.n - x.t.n : 0;
+    y.edge = 0x7fffffff;
+    y.gap = 0;
     if constexpr (FORM == kWindow) {
-      const int window_tile = max(tile, max(x.t.first + shift - a.window + 1, 0) / kRows);
-      if (a.sinks == 0) {
-        tile = window_tile;
-      } else {
-        const int sink_tiles = (x.lo + a.sinks + kRows - 1) / kRows;
-        if (window_tile > sink_tiles) jump = sink_tiles - tile, gap = window_tile - sink_tiles;
-      }
-      from = window_tile * kRows;
+      y.j0 = x.lo & ~31;
+      const int from = max(x.lo, x.t.first + y.shift - a.window + 1) & ~31;
+      const int edge = a.sinks == 0 ? y.j0 : (x.lo + a.sinks + 31) & ~31;
+      if (from > edge) y.edge = edge, y.gap = from - edge;
+    } else {
+      y.j0 = x.lo / kRows * kRows;
     }
-    j0 = tile * kRows;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      first[i] = x.t.first + i * f.tile_tokens;
+      y.first[i] = x.t.first + i * f.tile_tokens;
       int end = x.hi;
-      if (FORM == kWindow) end = min(end, min(first[i] + f.tile_tokens, x.t.n) + shift);
-      int n = (end + kRows - 1) / kRows - tile;
-      if (FORM == kWindow && n > jump) n = max(jump, n - gap);
-      steps[i] = first[i] < x.t.n ? max(0, n) : 0;
+      if (FORM == kWindow) end = min(end, min(y.first[i] + f.tile_tokens, x.t.n) + y.shift);
+      if (end > y.edge) end = max(y.edge, end - y.gap);
+      y.stop[i] = end;
+      y.steps[i] = y.first[i] < x.t.n ? max(0, (end - y.j0 + kRows - 1) / kRows) : 0;
     }
+    return y;
   };
   // first keys that stay visible to all: those before this one
   auto sinks_of = [&](const Item& x) { return FORM == kWindow && a.sinks > 0 ? x.lo + a.sinks : 0; };
-  // A step of first keys alone, up to 32 of them, takes a quarter of the products.  It pays where the softmax skips what
-  // no row of a warp sees, which it does not at dim 128 over 16 bits: each step waits for the other tile there, and the
-  // votes cost more than they save (12 prompts of up to 4096 tokens, 32/8 heads of 128, window 512: 451 and 424 us; 16384
+  // A step of up to 32 keys takes a quarter of the products.  It pays where the softmax skips what no row of a warp
+  // sees, which it does not at dim 128 over 16 bits: each step waits for the other tile there, and the votes cost more
+  // than they save (12 prompts of up to 4096 tokens, 32/8 heads of 128, window 512: 451 and 424 us; 16384
   // tokens, 8 heads of 64, window 1024: 101 and 104; chunks of 512 over e4m3: 101 and 111).
   constexpr bool kSkip = FORM == kWindow && (SCALED || DP == 64);
-  auto narrow = [&](int j0, int from, int sink_end) { return kSkip && j0 < from && sink_end - j0 <= 32; };
-  // to the next tile
-  auto advance = [&](int& j0, int from, const Item& x) {
-    j0 += kRows;
-    if (FORM == kWindow && j0 >= sinks_of(x)) j0 = max(j0, from);
-  };
-  // bit c of word i: key 32 i + c of the tile at j0 is one of the sequence's and valid; `kt`: running number of the tile
-  auto key_words = [&](int n, const uint32_t* mask, int j0, int kt, uint32_t (&w)[4]) {
-    tc::first_bits(n - j0, w);
-    if constexpr (PAGED) {
-      const uint32_t boxes = *reinterpret_cast<volatile uint32_t*>(&s_boxes[kt & 15]);
+  auto narrow = [&](int j0, int stop) { return kSkip && stop - j0 <= 32; };
+  // bit c of word i: key c of the 32 that step j0's place 32 i stands for is one of the sequence's and valid; `kt`: running
+  // number of the tile
+  auto key_words = [&](int n, const uint32_t* mask, const Plan& y, int j0, int kt, uint32_t (&w)[4]) {
+    const uint32_t boxes = PAGED ? *reinterpret_cast<volatile uint32_t*>(&s_boxes[kt & 15]) : 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!((boxes >> i) & 1u)) w[i >> 1] &= (i & 1) == 0 ? 0xffff0000u : 0x0000ffffu;
-    } else if (mask != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n - j0 - 32 * i > 0) w[i] &= __ldg(mask + (j0 >> 5) + i);
+    for (int i = 0; i < 4; ++i) {
+      const int at = y.key(j0 + 32 * i);
+      w[i] = ~tc::bits_from(n - at);
+      if constexpr (PAGED) {
+        if (!((boxes >> (2 * i)) & 1u)) w[i] &= 0xffff0000u;
+        if (!((boxes >> (2 * i + 1)) & 1u)) w[i] &= 0x0000ffffu;
+      } else if (mask != nullptr) {
+        if (n - at > 0) w[i] &= __ldg(mask + (at >> 5));
+      }
     }
   };
 
@@ -278,9 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = read_item(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
-      const int all = max(steps[0], steps[1]);
+      const Plan y = plan(x);
+      const int all = max(y.steps[0], y.steps[1]);
       if (all == 0) {
         taken();
         continue;
@@ -292,22 +297,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i)
           for (int c = 0; c < DP / 64; ++c)
             tc::tma_load_4d(smem + i * L::kTile + c * L::kHalf, &qmap, &bars.q_full, 64 * c, x.h0,
-                            static_cast<int>(x.t.row0) + first[i], x.t.batch);
+                            static_cast<int>(x.t.row0) + y.first[i], x.t.batch);
       }
       ++nq;
-      for (int y = 0; y < 2 * all; ++y) {
-        const int stage = kv % NS;
+      for (int step = 0; step < 2 * all; ++step) {
+        const int stage = kv % NS, j0 = y.j0 + step / 2 * kRows;
         if (kv >= NS) ok = tc::wait(&bars.kv_empty[stage], ((kv / NS) - 1) & 1);
         if (!ok) break;
-        const CUtensorMap* map = (y & 1) ? &vmap : &kmap;
+        const CUtensorMap* map = (step & 1) ? &vmap : &kmap;
         const uint32_t dst = smem + (2 + stage) * L::kTile;
+        // one lane per box
+        const int boxes = kRows / f.box, key = y.key(j0 + lane * f.box);
         if constexpr (PAGED) {
-          // one lane per box; a box outside the sequence or the cache is left out
-          const int boxes = kRows / f.box;
-          const int key = j0 + lane * f.box;
+          // a box outside the sequence or the cache is left out
           int page = -1;
           // no row's window reaches it: the page may be gone
-          const bool reached = FORM != kWindow || key < a.sinks || key + f.box > x.t.first + shift - a.window + 1;
+          const bool reached = FORM != kWindow || key < a.sinks || key + f.box > x.t.first + y.shift - a.window + 1;
           if (lane < boxes && key < x.n && reached) {
             page = __ldg(f.table + x.t.seq * f.table_sB + key / f.page);
             if (page < 0 || page >= f.n_pages) {
@@ -318,6 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
+          // SCALED: lanes 0 to 3 fetch the keys' fractions, 32 each, the next four the values', with the values' tile; what
+          // lies behind the row's end counts for nobody
+          int64_t res_at = 0;
+          uint32_t res = 0u;
+          if (SCALED && (step & 1)) {
+            const int64_t res_row = residue_row(static_cast<int64_t>(f.table_width) * f.page);
+            const int res_key = y.key(j0 + (lane & 3) * 32);
+            res_at = (static_cast<int64_t>(x.t.seq) * a.Hk + x.hk) * res_row + res_key;
+            res = __ballot_sync(0xffffffffu, lane < 8 && res_key < res_row);
+          }
           if (lane == 0) {
             // one bit per 16 keys
             uint32_t bits = 0;
@@ -325,26 +340,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b = 0; b < boxes; ++b)
               if ((got >> b) & 1u) bits |= ((1u << per) - 1u) << (b * per);
             *reinterpret_cast<volatile uint32_t*>(&s_boxes[(kv >> 1) & 15]) = bits;
-            const bool res = SCALED && (y & 1);
-            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64) + (res ? 8 * kRows : 0));
-            if (res) {
-              const int64_t at = (static_cast<int64_t>(x.t.seq) * a.Hk + x.hk) * residue_row(f.table_width * f.page) + j0;
-              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][0]), f.k_res + at, 4 * kRows, &bars.kv_full[stage]);
-              tc::bulk_load(smem_addr(s_res[(kv >> 1) & 3][1]), f.v_res + at, 4 * kRows, &bars.kv_full[stage]);
-            }
+            mbar_arrive_expect_tx(&bars.kv_full[stage], __popc(got) * f.box * 128 * (DP / 64) + __popc(res) * 128);
           }
           __syncwarp();
+          if (SCALED && ((res >> lane) & 1u))
+            tc::bulk_load(smem_addr(&s_res[(kv >> 1) & 3][lane >> 2][(lane & 3) * 32]), (lane < 4 ? f.k_res : f.v_res) + res_at,
+                          128, &bars.kv_full[stage]);
           if (page >= 0)
             for (int c = 0; c < DP / 64; ++c)
               tc::tma_load_4d(dst + c * L::kHalf + lane * f.box * 128, map, &bars.kv_full[stage], 64 * c, x.hk,
                               key % f.page, page);
-        } else if (lane == 0) {
-          mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
-          for (int c = 0; c < DP / 64; ++c)
-            tc::tma_load_4d(dst + c * L::kHalf, map, &bars.kv_full[stage], 64 * c, x.hk,
-                            static_cast<int>(x.t.row0) + j0, x.t.batch);
+        } else {
+          if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
+          __syncwarp();
+          if (lane < boxes)
+            for (int c = 0; c < DP / 64; ++c)
+              tc::tma_load_4d(dst + c * L::kHalf + lane * f.box * 128, map, &bars.kv_full[stage], 64 * c, x.hk,
+                              static_cast<int>(x.t.row0) + key, x.t.batch);
         }
-        if (y & 1) advance(j0, from, x);
         ++kv;
       }
       taken();
@@ -370,39 +383,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
-      const int all = max(steps[0], steps[1]), mine = i == 0 ? steps[0] : steps[1];
+      const Plan y = plan(x);
+      const int all = max(y.steps[0], y.steps[1]), mine = i == 0 ? y.steps[0] : y.steps[1];
+      const int stop = i == 0 ? y.stop[0] : y.stop[1];
       if (all == 0) continue;
       ok = tc::wait(&bars.q_full, nq & 1);
       ++nq;
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
-      auto kv_wait = [&](int y) { ok = ok && tc::wait(&bars.kv_full[(kv + y) % NS], ((kv + y) / NS) & 1); };
-      auto kv_addr = [&](int y) { return smem + (2 + (kv + y) % NS) * L::kTile; };
-      const int sink_end = sinks_of(x);
+      auto kv_wait = [&](int z) { ok = ok && tc::wait(&bars.kv_full[(kv + z) % NS], ((kv + z) / NS) & 1); };
+      auto kv_addr = [&](int z) { return smem + (2 + (kv + z) % NS) * L::kTile; };
       // scores of step j into the tile's buffer; keys are released by the step's end
       auto scores = [&](int j, int at) {
-        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), narrow(at, from, sink_end) ? id_32 : id_s);
+        tc::product_nt<DP>(t_s, q, kv_addr(2 * j), narrow(at, stop) ? id_32 : id_s);
         tc::commit(&bars.s_full[i]);
         if (j + 1 == mine) tc::commit(&bars.q_empty);
       };
       kv_wait(0);
       tc::fence_after();
       if (ok && leader) {
-        if (mine > 0) scores(0, j0);
+        if (mine > 0) scores(0, y.j0);
         else tc::commit(&bars.q_empty);
         tc::commit(&bars.kv_empty[kv % NS]);
       }
       __syncwarp();
-      for (int j = 0; j < all && ok; ++j, advance(j0, from, x)) {
+      for (int j = 0, j0 = y.j0; j < all && ok; ++j, j0 += kRows) {
         kv_wait(2 * j + 1);
         if (j + 1 < all) kv_wait(2 * j + 2);
         if (!ok) break;
         if (j < mine) {
           // values of keys that are not there or not valid may hold anything
           uint32_t w[4];
-          if (PAGED || mask != nullptr || j0 + kRows > x.n) {
-            key_words(x.n, mask, j0, (kv >> 1) + j, w);
+          if (PAGED || mask != nullptr || y.key(j0 + kRows - 1) >= x.n) {
+            key_words(x.n, mask, y, j0, (kv >> 1) + j, w);
             if (!tc::all_set(w)) tc::clear_rows<DP / 64>(kv_addr(2 * j + 1), w);
           }
           // (Issuing the products of half the keys ahead of the others was tried: it costs more than it
@@ -411,14 +423,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = ok && tc::wait(&bars.p_full[i], ns & 1);
           tc::fence_after();
           if (ok && leader) {
-            if (narrow(j0, from, sink_end)) tc::product_tn<64, 2>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
+            if (narrow(j0, stop)) tc::product_tn<64, 2>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
             else tc::product_tn<64>(t_o, t_s, kv_addr(2 * j + 1), id_o, j > 0);
             if (j + 1 == mine) {
               tc::commit(&bars.o_full[i]);
             } else {
-              int at = j0;
-              advance(at, from, x);
-              scores(j + 1, at);
+              scores(j + 1, j0 + kRows);
             }
           }
           ++ns;
@@ -448,15 +458,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x;
       ok = take(it, x);
       if (!ok || x.last) break;
-      int first[2], steps[2], j0, from, shift;
-      plan(x, first, steps, j0, from, shift);
-      const int mine = i == 0 ? first[0] : first[1], count = i == 0 ? steps[0] : steps[1];
-      const int all = max(steps[0], steps[1]);
+      const Plan y = plan(x);
+      const int mine = i == 0 ? y.first[0] : y.first[1], count = i == 0 ? y.steps[0] : y.steps[1];
+      const int all = max(y.steps[0], y.steps[1]);
       if (!PAGED && a.cu != nullptr && a.zero_tail && warp < 4 && x.t.n == 0) {
         // a tile behind the last sequence clears rows there
         for (int64_t r = x.t.row0 + x.t.tail_index; r < a.L; r += x.t.tail_count)
-          for (int y = threadIdx.x; y < a.d * f.pack; y += kRows)
-            static_cast<T*>(a.o)[r * a.os.t + (x.h0 + y / a.d) * a.os.h + y % a.d] = Elem<T>::from_f(0.f);
+          for (int c = threadIdx.x; c < a.d * f.pack; c += kRows)
+            static_cast<T*>(a.o)[r * a.os.t + (x.h0 + c / a.d) * a.os.h + c % a.d] = Elem<T>::from_f(0.f);
       }
       if (mine >= x.t.n) {
         kt += all;
@@ -466,8 +475,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t* mask = !PAGED && a.mask != nullptr ? a.mask + x.t.batch * a.mask_words + kMaskHead : nullptr;
       const int tok = mine + row / f.pack, h = x.h0 + row % f.pack;
       const bool live = tok < x.t.n;
-      int limit = tok + shift;                                  // last key the row sees
-      int limit_all = mine + (warp & 3) * 32 / f.pack + shift;  // and that all rows of the warp see
+      int limit = tok + y.shift;                                  // last key the row sees
+      int limit_all = mine + (warp & 3) * 32 / f.pack + y.shift;  // and that all rows of the warp see
       if constexpr (FORM == kPrefix) {
         // of its own sequence, which may end here
         limit = live ? min(n - 1, last_key(f, tok)) : n - 1;
@@ -478,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int sink_end = sinks_of(x);
       float m = neg_inf(), sum = 0.f;
       float mv = neg_inf();  // kWeighted: the reference of weight * scale, as an exponent of two
-      for (int j = 0; j < count; ++j, ++ns, advance(j0, from, x)) {
+      for (int j = 0, j0 = y.j0; j < count; ++j, ++ns, j0 += kRows) {
         // After a wait that ran out a warp goes on without waiting to the end of the piece, so that
         // the named barriers below see all their warps.
         ok = ok && tc::wait(&bars.s_full[i], ns & 1);
@@ -490,11 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::ld32(s_addr + 32, s[1]);
         }
         // warp-uniform: every row of the warp sees all keys of the tile
-        bool whole = j0 + kRows <= n && j0 + kRows - 1 <= limit_all &&
-                     (FORM != kWindow || j0 > limit_all + f.warp_span - a.window || j0 + kRows <= sink_end);
+        const int k0 = y.key(j0), k1 = y.key(j0 + kRows - 1);
+        bool whole = k1 < n && k1 <= limit_all &&
+                     (FORM != kWindow || k0 > limit_all + f.warp_span - a.window || k1 < sink_end);
         uint32_t w[4];
         if (PAGED || mask != nullptr || !whole) {
-          key_words(n, mask, j0, kt + j, w);
+          key_words(n, mask, y, j0, kt + j, w);
           whole = whole && tc::all_set(w);
         }
         if (!SCALED) tc::wait_ld(s[0], s[1]);
@@ -525,10 +535,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         // false: none of these 32 keys counts for any row of the warp (kSkip; x is left as it is)
         auto hide = [&](int c, uint32_t (&x)[32]) -> bool {
-          const int left = limit - j0 - 64 * half - 32 * c + 1;
+          const int at = y.key(j0 + 64 * half + 32 * c), left = limit - at + 1;
           uint32_t see =
               (half == 0 ? w[c] : w[2 + c]) & (left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u);
-          if constexpr (FORM == kWindow) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - j0 - 64 * half - 32 * c);
+          if constexpr (FORM == kWindow) see &= tc::bits_from(left - a.window) | ~tc::bits_from(sink_end - at);
           if constexpr (kSkip) {
             if (!__any_sync(0xffffffffu, see != 0u)) return false;
             if (__all_sync(0xffffffffu, see == 0xffffffffu)) return true;
@@ -564,13 +574,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            float& z = t[2 * c + y];
-            z = __uint_as_float(x[16 * y]);
+          for (int b = 0; b < 2; ++b) {
+            float& z = t[2 * c + b];
+            z = __uint_as_float(x[16 * b]);
 #pragma unroll
             for (int e = 1; e < 15; e += 2)
-              z = tc::max3(z, __uint_as_float(x[16 * y + e]), __uint_as_float(x[16 * y + e + 1]));
-            z = fmaxf(z, __uint_as_float(x[16 * y + 15]));
+              z = tc::max3(z, __uint_as_float(x[16 * b + e]), __uint_as_float(x[16 * b + e + 1]));
+            z = fmaxf(z, __uint_as_float(x[16 * b + 15]));
           }
         }
         float top = tc::max3(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]), m);
@@ -625,32 +635,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) p[e] = 0u;
           } else {
-          if constexpr (SCALED) {
-            scale(c, x);
-            if (!whole) hide(c, x);
-            fractions(1, c, r);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 score = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-            float2 y = kFolded ? add2(score, bv) : fma2(score, c2v, bv);
-            y.x = ex2(y.x);
-            y.y = ex2(y.y);
-            if (e & 1) part2 = add2(part2, y);
-            else part = add2(part, y);
             if constexpr (SCALED) {
-              const float4& z = r[e / 2];
-              const float2 of_value = (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
-              if constexpr (kWeighted) {
-                y = kFolded ? add2(score, add2(of_value, vv)) : fma2(score, c2v, add2(of_value, vv));
-                y.x = ex2(y.x);
-                y.y = ex2(y.y);
-              } else {
-                y = mul2(y, of_value);
-              }
+              scale(c, x);
+              if (!whole) hide(c, x);
+              fractions(1, c, r);
             }
-            p[e] = tc::pack2<T>(y.x, y.y);
-          }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 score = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+              float2 w2 = kFolded ? add2(score, bv) : fma2(score, c2v, bv);
+              w2.x = ex2(w2.x);
+              w2.y = ex2(w2.y);
+              if (e & 1) part2 = add2(part2, w2);
+              else part = add2(part, w2);
+              if constexpr (SCALED) {
+                const float4& z = r[e / 2];
+                const float2 of_value = (e & 1) ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
+                if constexpr (kWeighted) {
+                  w2 = kFolded ? add2(score, add2(of_value, vv)) : fma2(score, c2v, add2(of_value, vv));
+                  w2.x = ex2(w2.x);
+                  w2.y = ex2(w2.y);
+                } else {
+                  w2 = mul2(w2, of_value);
+                }
+              }
+              p[e] = tc::pack2<T>(w2.x, w2.y);
+            }
           }
           // over this half's own scores: the other half may not have read its yet
           tc::st16(s_addr + 16 * c, p);
@@ -732,11 +742,12 @@ bool launch_attn_tc_fwd_window(const AttnArgs& a, int dtype, cudaStream_t st, cu
   f.pack = attn_pack(a.H / a.Hk);
   f.tile_tokens = kRows / f.pack;
   f.warp_span = 31 / f.pack;
+  f.box = kBox;
   const int64_t nb = a.cu != nullptr ? 1 : a.nseq;
   CUtensorMap q, k, v;
   if (!attn_map(&q, a.q, dtype, nb, a.L, a.H, a.d, a.qs, f.pack, f.tile_tokens) ||
-      !attn_map(&k, a.k, dtype, nb, a.L, a.Hk, a.d, a.ks, 1, kRows) ||
-      !attn_map(&v, a.v, dtype, nb, a.L, a.Hk, a.d, a.vs, 1, kRows))
+      !attn_map(&k, a.k, dtype, nb, a.L, a.Hk, a.d, a.ks, 1, kBox) ||
+      !attn_map(&v, a.v, dtype, nb, a.L, a.Hk, a.d, a.vs, 1, kBox))
     return false;
   f.wide_out = row_alignment(a.o, a.os, nb, a.H);
   f.wide_low = row_alignment(a.low, AttnStrides{a.L * a.H * a.d, static_cast<int64_t>(a.H) * a.d, a.d}, nb, a.H);
@@ -761,7 +772,7 @@ bool launch_attn_tc_fwd_window(const AttnArgs& a, int dtype, cudaStream_t st, cu
 namespace {
 
 // what chunks and prefixes have in common: the tensors and the pages
-bool paged_maps(const PagedArgs& p, int dtype, FwdArgs& f, CUtensorMap (&maps)[3]) {
+bool paged_maps(const PagedArgs& p, int dtype, int most_box, FwdArgs& f, CUtensorMap (&maps)[3]) {
   if (!(p.scale > 0.f)) return false;
   AttnArgs& a = f.a;
   a.q = p.q;
@@ -786,7 +797,7 @@ bool paged_maps(const PagedArgs& p, int dtype, FwdArgs& f, CUtensorMap (&maps)[3
   f.n_pages = p.n_pages;
   f.k_res = p.k_res;
   f.v_res = p.v_res;
-  f.box = std::min(p.page & -p.page, kRows);  // the largest power of two that divides a page
+  f.box = std::min(p.page & -p.page, most_box);  // the largest power of two that divides a page
   // expanded pages are contiguous
   const int64_t pages = p.k_res != nullptr ? p.expanded_pages : p.n_pages;
   const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
@@ -803,7 +814,7 @@ bool launch_paged_tc_window(const PagedArgs& p, int dtype, cudaStream_t st, cuda
   if (p.cu == nullptr) return false;
   FwdArgs f = {};
   CUtensorMap m[3];
-  if (!paged_maps(p, dtype, f, m)) return false;
+  if (!paged_maps(p, dtype, kBox, f, m)) return false;
   f.a.causal = 1;
   f.a.window = p.window;
   f.a.sinks = p.sinks;
@@ -826,7 +837,7 @@ int64_t prefix_tiles(const PagedArgs& p) {
 bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e) {
   FwdArgs f = {};
   CUtensorMap m[3];
-  if (!paged_maps(p, dtype, f, m)) return false;
+  if (!paged_maps(p, dtype, kRows, f, m)) return false;
   f.splits = p.prefix_splits;
   f.chunk = p.prefix_chunk;
   f.prefix = p.skip;
