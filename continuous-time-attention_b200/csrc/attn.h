@@ -50,7 +50,9 @@ constexpr int kMaskHead = 4;
 
 // dtype codes as in common.cuh
 cudaError_t launch_attn_simt_fwd(const AttnArgs& a, int dtype, cudaStream_t st);
-cudaError_t launch_attn_simt_bwd(const AttnArgs& a, int dtype, cudaStream_t st);
+// far: simt_far_bytes() of workspace for windows with first keys
+cudaError_t launch_attn_simt_bwd(const AttnArgs& a, int dtype, void* far, cudaStream_t st);
+int64_t simt_far_bytes(const AttnArgs& a);
 cudaError_t launch_attn_delta(const AttnArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_attn_mask_words(const void* mask, int mask_dtype, int64_t sB, int64_t sL, int64_t B, int64_t L,
                                    uint32_t* words, int64_t words_per_batch, cudaStream_t st);

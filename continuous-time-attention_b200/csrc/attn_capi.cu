@@ -448,11 +448,25 @@ int cta_attention_backward(const cta_attention_args* args, void* stream) {
   return cta_window_attention_backward(args, 0, 0, nullptr, 0, stream);
 }
 
+// for either kernel
+static int64_t backward_bytes(const AttnArgs& a, int dtype) {
+  return a.dk != nullptr ? std::max(far_bytes(a, dtype), simt_far_bytes(a)) : 0;
+}
+
+// Up to 16 keys a row: the score gradients' rounding to 16 bits, which the tensor cores need, has few terms to average
+// over, and leaves dQ and dK 1.5 times as far off as the rounding of their own that is nearly all the FP32 pipe leaves (1.1
+// times).  That is slower, 1024 tokens, 8 heads of 64, window 4: 34 and 10 us, so it is for sizes where the call takes
+// longer than that to make.
+static bool few_keys(const AttnArgs& a) {
+  const int64_t tokens = a.cu != nullptr ? a.L : a.L * a.nseq;
+  return a.window > 0 && a.window + a.sinks <= 16 && tokens * a.H * a.d <= (1 << 20);
+}
+
 int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int64_t window, int64_t sinks) {
   AttnArgs a;
   const int rc = prompt_window(args, window, sinks, a);
   if (rc != CTA_OK) return rc == kNothing ? 0 : -rc;
-  return a.dk != nullptr ? far_bytes(a, args->dtype) : 0;
+  return backward_bytes(a, args->dtype);
 }
 
 int cta_window_attention_backward(const cta_attention_args* args, int64_t window, int64_t sinks, void* workspace,
@@ -469,13 +483,14 @@ int cta_window_attention_backward(const cta_attention_args* args, int64_t window
     a.g_norm = a.delta + plane;
     a.v_norm = a.g_norm + plane;
   }
-  const int64_t need = a.dk != nullptr ? far_bytes(a, args->dtype) : 0;
+  const int64_t need = backward_bytes(a, args->dtype);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(CTA_EINVAL, "workspace of %lld bytes needed, got %lld", (long long)need, (long long)workspace_bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CTA_EINVAL, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_attn_delta(a, args->dtype, st);
-  if (e == cudaSuccess && !launch_attn_tc_bwd(a, args->dtype, workspace, st, &e)) e = launch_attn_simt_bwd(a, args->dtype, st);
+  if (e == cudaSuccess && (few_keys(a) || !launch_attn_tc_bwd(a, args->dtype, workspace, st, &e)))
+    e = launch_attn_simt_bwd(a, args->dtype, workspace, st);
   return launched(e, "attention backward launch");
 }
 

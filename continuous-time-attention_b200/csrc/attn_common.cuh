@@ -213,6 +213,19 @@ __device__ __forceinline__ Reach reach_of(const AttnArgs& a, int lo) {
   return Reach{a.window, a.sinks > 0 ? lo + a.sinks : 0};
 }
 
+// A window's far rows, those behind the window of a key tile of `rows` that holds first keys, go in parts of `chunk`; part c
+// of a sequence has the place far_place + c of far_places.  Packed: a sequence has far rows only if it is at least window +
+// rows long, so its place among those, or among all if they are fewer, tells them apart.
+__host__ __device__ __forceinline__ bool far_by_sequence(const AttnArgs& a, int rows) { return a.nseq <= a.L / (a.window + rows); }
+__device__ __forceinline__ int64_t far_place(const AttnArgs& a, const SeqTile& t, int rows, int chunk) {
+  if (a.cu == nullptr) return static_cast<int64_t>(t.batch) * ((a.L + chunk - 1) / chunk);
+  return t.row0 / chunk + (far_by_sequence(a, rows) ? t.seq : t.row0 / (a.window + rows));
+}
+inline int64_t far_places(const AttnArgs& a, int rows, int64_t chunk) {
+  if (a.cu == nullptr) return a.nseq * ((a.L + chunk - 1) / chunk);
+  return a.L / chunk + 1 + (far_by_sequence(a, rows) ? a.nseq : a.L / (a.window + rows) + 1);
+}
+
 __device__ __forceinline__ int64_t lse_index(const AttnArgs& a, const SeqTile& t, int h, int row) {
   return (static_cast<int64_t>(t.batch) * a.H + h) * a.L + t.row0 + row;
 }

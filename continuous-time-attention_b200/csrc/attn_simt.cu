@@ -359,9 +359,21 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const __grid_con
   pdl_wait();  // launched beside dK and dV
 }
 
-// owns KT keys of one key/value head; rows of the score tile are keys, columns are queries
-template <typename T, int DP, bool WINDOW>
-__global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_constant__ AttnArgs a) {
+// A window's first keys are seen by all rows.  Those behind the window of such a key tile, the far ones, are another launch,
+// a CTA per `chunk` rows, which leaves its sums over the first keys in 32 bits; the tile's own CTA adds them in order.  One
+// sequence, 8 heads of 64, window 4 and 4 first keys: 16384 tokens 467 us in fp32, against 3200 (bf16) with the tile's CTA
+// going through all rows; 1024 tokens 71 and 200.
+struct FarRows {
+  float* sums;  // nullptr: there are none
+  int chunk, tiles, keys;  // rows of a CTA; tiles with first keys; first keys of a tile at most
+};
+enum DkvForm : int { kAll = 0, kNear = 1, kFar = 2 };
+
+// owns KT keys of one key/value head; rows of the score tile are keys, columns are queries.  kNear, kFar: with a window.
+template <typename T, int DP, int FORM>
+__global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_constant__ AttnArgs a,
+                                                                 const __grid_constant__ FarRows far) {
+  constexpr bool WINDOW = FORM != kAll;
   constexpr int KT = SimtTile<DP>::KT, QT = KT, C = QT / 8, DC = DP / 32, R = KT / 16;
   extern __shared__ float4 smem_raw[];
   float* K = reinterpret_cast<float*>(smem_raw);
@@ -371,11 +383,13 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   float* P = G + QT * (DP + kPad);
   __shared__ float s_lse[QT], s_delta[QT];
   const int hk = blockIdx.x % a.Hk, group = a.H / a.Hk;
-  pdl_launch_dependents();  // dQ's CTAs may follow
+  pdl_launch_dependents();  // dQ's CTAs may follow; kFar: the others'
   // early keys of a causal sequence meet the most queries: forwards is heaviest first
-  const SeqTile t = block_tile(a, blockIdx.x / a.Hk, KT, false);
+  SeqTile t = FORM == kFar ? block_tile(a, blockIdx.x / a.Hk / far.tiles, far.chunk, false)
+                           : block_tile(a, blockIdx.x / a.Hk, KT, false);
   if (t.first >= t.n) {
-    if (a.cu != nullptr) {
+    if (FORM == kNear) pdl_wait();
+    if (FORM != kFar && a.cu != nullptr) {
       zero_rows<T>(a.dk, a.dks, t.row0, a.L, hk, a.d, t.tail_index, t.tail_count);
       zero_rows<T>(a.dv, a.dvs, t.row0, a.L, hk, a.d, t.tail_index, t.tail_count);
     }
@@ -383,6 +397,28 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
   }
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const uint32_t* mask = a.mask != nullptr ? a.mask + t.batch * a.mask_words : nullptr;
+  int lo, hi;
+  mask_range(a, t.batch, t.n, lo, hi);
+  const Reach reach = reach_of(a, lo);
+  int row_from = a.causal ? t.first : 0, row_to = t.n;
+  if constexpr (WINDOW) {
+    const int chunk_from = t.first;
+    if constexpr (FORM == kFar) t.first = (lo / KT + static_cast<int>(blockIdx.x) / a.Hk % far.tiles) * KT;
+    // rows behind the windows that hold the last of these keys see none of them, unless it is one of the first
+    const int far_from = (min(t.n, t.first + KT - 1 + reach.window) + QT - 1) / QT * QT;
+    if constexpr (FORM == kFar) {
+      row_from = max(chunk_from, far_from);
+      row_to = min(chunk_from + far.chunk, t.n);
+      if (row_from >= row_to || t.first >= min(min(t.n, hi), reach.sink_end)) return;
+    } else if (t.first >= reach.sink_end || far.sums != nullptr) {
+      row_to = min(t.n, far_from);
+    }
+  }
+  // the far rows' sums of chunk c over the first keys of this tile: dV, then dK, [far.keys][2][DP]
+  auto far_at = [&](int c) {
+    const int64_t slot = far_place(a, t, KT, far.chunk) + c;
+    return far.sums + (((slot * far.tiles + (t.first / KT - lo / KT)) * a.Hk + hk) * far.keys - max(t.first, lo)) * 2 * DP;
+  };
   const uint64_t valid = valid_keys<KT>(mask, t.first, t.n);
   load_rows<T, KT, DP>(K, a.k, a.ks, t, hk, t.first, t.n, a.d, valid);
   load_rows<T, KT, DP>(V, a.v, a.vs, t, hk, t.first, t.n, a.d, valid);
@@ -396,15 +432,10 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
     for (int x = 0; x < DC; ++x) dk[r][x] = dv[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float c2 = a.scale * kLog2e;
-  int lo, hi;
-  mask_range(a, t.batch, t.n, lo, hi);
   // rows that see no key, up to the first valid one, may hold anything
   const int from = lo >= hi ? t.n : a.causal ? lo : 0;
-  const Reach reach = reach_of(a, lo);
-  // rows behind the windows that hold the last of these keys see none of them, unless it is one of the first
-  const int end = WINDOW && t.first >= reach.sink_end ? min(t.n, t.first + KT - 1 + reach.window) : t.n;
   for (int h = hk * group; h < (hk + 1) * group; ++h) {
-    for (int i0 = a.causal ? t.first : 0; i0 < end; i0 += QT) {
+    for (int i0 = row_from; i0 < row_to; i0 += QT) {
       if (from >= i0 + QT) continue;
       uint64_t seeing = from > i0 ? ~0ull << (from - i0) : ~0ull;
       if constexpr (WINDOW) {
@@ -448,6 +479,34 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const __grid_co
       __syncwarp();
       mm_nn<R, DC, QT, DP>(dk, P, Q, ty, tx);
     }
+  }
+  if constexpr (WINDOW) {
+    if constexpr (FORM == kNear) pdl_wait();  // launched beside the far rows
+    if (FORM == kFar || (far.sums != nullptr && row_to < t.n && t.first < min(hi, reach.sink_end))) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int j = t.first + ty + 16 * r;
+        if (j < lo || j >= reach.sink_end) continue;
+        const int c1 = FORM == kFar ? row_from / far.chunk + 1 : (t.n + far.chunk - 1) / far.chunk;
+        for (int c = (FORM == kFar ? row_from : row_to) / far.chunk; c < c1; ++c) {
+          float* sums = far_at(c) + static_cast<int64_t>(j) * 2 * DP + 4 * tx;
+#pragma unroll
+          for (int x = 0; x < DC; ++x) {
+            float4* of_v = reinterpret_cast<float4*>(sums + 32 * x);
+            float4* of_k = reinterpret_cast<float4*>(sums + DP + 32 * x);
+            if constexpr (FORM == kFar) {
+              *of_v = dv[r][x];
+              *of_k = dk[r][x];
+            } else {
+              const float4 y = __ldcg(of_v), z = __ldcg(of_k);  // written while this kernel may already be there
+              dv[r][x].x += y.x, dv[r][x].y += y.y, dv[r][x].z += y.z, dv[r][x].w += y.w;
+              dk[r][x].x += z.x, dk[r][x].y += z.y, dk[r][x].z += z.z, dk[r][x].w += z.w;
+            }
+          }
+        }
+      }
+    }
+    if constexpr (FORM == kFar) return;
   }
   float mul[R], one[R];
 #pragma unroll
@@ -589,13 +648,41 @@ cudaError_t fwd(AttnArgs a, cudaStream_t st) {
   return launch_grid<attn_simt_fwd_kernel<T, DP, WINDOW>>(false, tiles * a.H, kThreads, smem, st, a);
 }
 
+int key_tile(int d) { return d > 128 ? SimtTile<256>::KT : SimtTile<64>::KT; }
+int far_tiles(const AttnArgs& a) {
+  const int kt = key_tile(a.d);
+  return a.mask != nullptr ? (a.sinks + kt - 2) / kt + 1 : (a.sinks + kt - 1) / kt;
+}
+int64_t far_bytes_of(const AttnArgs& a, int64_t chunk) {
+  const int kt = key_tile(a.d);
+  return far_places(a, kt, chunk) * far_tiles(a) * a.Hk * std::min(a.sinks, kt) * 2 * (a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256) *
+         static_cast<int64_t>(sizeof(float));
+}
+// Rows of a far CTA: about as many as the others' windows; more where there would be more than 64 parts in a row, or
+// more than 256 MB of them.
+int far_chunk(const AttnArgs& a) {
+  int64_t rows = std::max<int64_t>(std::max<int64_t>(a.window + key_tile(a.d), 128), (a.L + 63) / 64);
+  rows = (rows + 63) / 64 * 64;
+  while (rows < a.L && far_bytes_of(a, rows) > (256LL << 20)) rows *= 2;
+  return static_cast<int>(rows);
+}
+
 template <typename T, int DP, bool WINDOW>
-cudaError_t bwd(AttnArgs a, cudaStream_t st) {
+cudaError_t bwd(AttnArgs a, void* far_sums, cudaStream_t st) {
   constexpr int KT = SimtTile<DP>::KT;
   if (a.dk != nullptr) {
     constexpr int smem = sizeof(float) * (4 * KT * (DP + kPad) + KT * (KT + kPad));
+    FarRows far = {};
+    if (WINDOW && simt_far_bytes(a) > 0) {
+      far = FarRows{static_cast<float*>(far_sums), far_chunk(a), far_tiles(a), std::min(a.sinks, KT)};
+      const int64_t chunks = count_tiles(a, far.chunk);
+      const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP, WINDOW ? kFar : kAll>>(
+          false, chunks * far.tiles * a.Hk, kThreads, smem, st, a, far);
+      if (e != cudaSuccess) return e;
+    }
     const int64_t tiles = count_tiles(a, KT);
-    const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP, WINDOW>>(false, tiles * a.Hk, kThreads, smem, st, a);
+    const cudaError_t e = launch_grid<attn_simt_dkv_kernel<T, DP, WINDOW ? kNear : kAll>>(far.sums != nullptr, tiles * a.Hk,
+                                                                                          kThreads, smem, st, a, far);
     if (e != cudaSuccess) return e;
   }
   if (a.dq == nullptr) return cudaSuccess;
@@ -605,31 +692,37 @@ cudaError_t bwd(AttnArgs a, cudaStream_t st) {
 }
 
 template <typename T, bool WINDOW>
-cudaError_t dispatch_dim(const AttnArgs& a, bool backward, cudaStream_t st) {
-  if (a.d <= 64) return backward ? bwd<T, 64, WINDOW>(a, st) : fwd<T, 64, WINDOW>(a, st);
-  if (a.d <= 128) return backward ? bwd<T, 128, WINDOW>(a, st) : fwd<T, 128, WINDOW>(a, st);
-  return backward ? bwd<T, 256, WINDOW>(a, st) : fwd<T, 256, WINDOW>(a, st);
+cudaError_t dispatch_dim(const AttnArgs& a, bool backward, void* far, cudaStream_t st) {
+  if (a.d <= 64) return backward ? bwd<T, 64, WINDOW>(a, far, st) : fwd<T, 64, WINDOW>(a, st);
+  if (a.d <= 128) return backward ? bwd<T, 128, WINDOW>(a, far, st) : fwd<T, 128, WINDOW>(a, st);
+  return backward ? bwd<T, 256, WINDOW>(a, far, st) : fwd<T, 256, WINDOW>(a, st);
 }
 template <typename T>
-cudaError_t dispatch(const AttnArgs& a, bool backward, cudaStream_t st) {
-  return a.window > 0 ? dispatch_dim<T, true>(a, backward, st) : dispatch_dim<T, false>(a, backward, st);
+cudaError_t dispatch(const AttnArgs& a, bool backward, void* far, cudaStream_t st) {
+  return a.window > 0 ? dispatch_dim<T, true>(a, backward, far, st) : dispatch_dim<T, false>(a, backward, far, st);
 }
 
 }  // namespace
 
+int64_t simt_far_bytes(const AttnArgs& a) {
+  // for few far rows the launch costs as much as it saves (a step over 4 x 512 tokens, window 128: 147 to 157 us with and without)
+  if (a.window == 0 || a.sinks == 0 || a.L < a.window + 8 * key_tile(a.d)) return 0;
+  return far_bytes_of(a, far_chunk(a));
+}
+
 cudaError_t launch_attn_simt_fwd(const AttnArgs& a, int dtype, cudaStream_t st) {
   switch (dtype) {
-    case kF32: return dispatch<float>(a, false, st);
-    case kBF16: return dispatch<__nv_bfloat16>(a, false, st);
-    default: return dispatch<__half>(a, false, st);
+    case kF32: return dispatch<float>(a, false, nullptr, st);
+    case kBF16: return dispatch<__nv_bfloat16>(a, false, nullptr, st);
+    default: return dispatch<__half>(a, false, nullptr, st);
   }
 }
 
-cudaError_t launch_attn_simt_bwd(const AttnArgs& a, int dtype, cudaStream_t st) {
+cudaError_t launch_attn_simt_bwd(const AttnArgs& a, int dtype, void* far, cudaStream_t st) {
   switch (dtype) {
-    case kF32: return dispatch<float>(a, true, st);
-    case kBF16: return dispatch<__nv_bfloat16>(a, true, st);
-    default: return dispatch<__half>(a, true, st);
+    case kF32: return dispatch<float>(a, true, far, st);
+    case kBF16: return dispatch<__nv_bfloat16>(a, true, far, st);
+    default: return dispatch<__half>(a, true, far, st);
   }
 }
 

@@ -554,8 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // the sums of the far rows of chunk c over the first keys of this tile: dV, then dK, [far_keys][2][DP]
   auto far_at = [&](const Plan& p, const SeqTile& t, int chunk) {
-    const int64_t slot = a.cu != nullptr ? (t.row0 + static_cast<int64_t>(chunk) * f.chunk) / f.chunk + t.row0 / (a.window + kRows)
-                                         : static_cast<int64_t>(t.batch) * ((a.L + f.chunk - 1) / f.chunk) + chunk;
+    const int64_t slot = far_place(a, t, kRows, f.chunk) + chunk;
     return f.far + ((slot * f.sink_tiles + (t.first / kRows - p.lo / kRows)) * a.Hk + p.hk) * f.far_keys * 2 * DP;
   };
 
@@ -1000,10 +999,7 @@ cudaError_t dispatch(const CUtensorMap& q, const CUtensorMap& g, const CUtensorM
 
 int far_sink_tiles(const AttnArgs& a) { return a.mask != nullptr ? (a.sinks + kRows - 2) / kRows + 1 : (a.sinks + kRows - 1) / kRows; }
 int64_t far_bytes_of(const AttnArgs& a, int64_t chunk) {
-  // packed: a sequence has far rows only if it is at least window + kRows long, which tells them apart
-  const int64_t slots = a.cu != nullptr ? (a.L / chunk + 1) + (a.L / (a.window + kRows) + 1)
-                                        : a.nseq * ((a.L + chunk - 1) / chunk);
-  return slots * far_sink_tiles(a) * a.Hk * std::min(a.sinks, kRows) * 2 * (a.d <= 64 ? 64 : 128) * static_cast<int64_t>(sizeof(float));
+  return far_places(a, kRows, chunk) * far_sink_tiles(a) * a.Hk * std::min(a.sinks, kRows) * 2 * (a.d <= 64 ? 64 : 128) * static_cast<int64_t>(sizeof(float));
 }
 // Rows of a far CTA: about as many as the others' windows; more where there would be more than 64 parts in a row, or
 // more than 256 MB of them.

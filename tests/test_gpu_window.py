@@ -148,9 +148,21 @@ def test_long(dim, heads, kv_heads, window, sinks, dtype):
         _check_sequence(one, q[0][:, part], k[0][:, h : h + 1], v[0][:, h : h + 1], g[0][:, part], see, dim**-0.5, dtype)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_long_packed(dtype):
-    lens, window, sinks = [3000, 40, 4100, 1500], 300, 20
+@pytest.mark.parametrize("dim,heads,kv_heads,window,sinks,dtype", [(64, 2, 2, 200, 4, torch.float32), (128, 2, 1, 60, 70, torch.float32),
+                                                                  (192, 2, 1, 31, 40, torch.bfloat16), (20, 4, 4, 5, 3, torch.float16)])
+def test_long_without_tensor_cores(dim, heads, kv_heads, window, sinks, dtype):
+    n = 2500
+    q, k, v, g = _inputs((2, n), heads, kv_heads, dim, dtype, seed=9)
+    got = _run(q, k, v, g, causal=True, window=window, sinks=sinks)
+    see = _reach(n, n, window, sinks)
+    for b in range(2):
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], see, dim**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,window,sinks", [([3000, 40, 4100, 1500], 300, 20), ([5] * 40 + [70] * 50 + [600, 0, 411] + [3] * 30, 30, 4),
+                                               ([9, 333, 1200], 12, 4)])
+def test_long_packed(lens, window, sinks, dtype):
     q, k, v, g = _inputs((sum(lens),), 4, 1, 64, dtype, seed=6)
     cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32).cuda()
     got = _run(q, k, v, g, causal=True, cu_seqlens=cu, window=window, sinks=sinks)
@@ -158,10 +170,12 @@ def test_long_packed(dtype):
     for n in lens:
         part = slice(at, at + n)
         at += n
+        if n == 0:
+            continue
         _check_sequence([x[part] for x in got], q[part], k[part], v[part], g[part], _reach(n, n, window, sinks), 0.125, dtype)
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_long_masked(dtype):
     """First tokens in the middle of a key tile, and over the edge of one; their rows far behind."""
     L, window = 3300, 200

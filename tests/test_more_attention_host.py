@@ -49,7 +49,7 @@ def test_window_calls_refuse_what_the_plain_ones_do():
 
 
 def test_backward_workspace():
-    """For the far rows of first keys, on the tensor cores; nothing where there are none."""
+    """For the far rows of first keys; nothing where there are none."""
     from cta_b200 import _lib
 
     lib = _lib.load()
@@ -60,7 +60,7 @@ def test_backward_workspace():
     assert size(100, 4, length=5000) > 0
     assert size(100, 0, length=5000) == 0 and size(0, 0, length=5000) == 0
     assert size(100, 4, length=200) == 0 and size(4996, 4, length=5000) == 0
-    assert size(100, 4, length=5000, dtype=0) == 0 and size(100, 4, length=5000, dim=20) == 0
+    assert size(100, 4, length=5000, dtype=0) > 0 and size(100, 4, length=5000, dim=20) > 0
     no_dk = (16,) * 9 + (0, 0, 0, 0)
     assert size(100, 4, length=5000, pointers=no_dk) == 0
     # many first keys of long rows: bounded, beyond one part for each
