@@ -705,8 +705,9 @@ cudaError_t dispatch(const AttnArgs& a, bool backward, void* far, cudaStream_t s
 }  // namespace
 
 int64_t simt_far_bytes(const AttnArgs& a) {
-  // for few far rows the launch costs as much as it saves (a step over 4 x 512 tokens, window 128: 147 to 157 us with and without)
-  if (a.window == 0 || a.sinks == 0 || a.L < a.window + 8 * key_tile(a.d)) return 0;
+  // A launch pays for a few row tiles.  fp32 backward, 8 heads of 64, 4 first keys, with and without: 4 x 512 tokens, window
+  // 128, 111 and 116 us; 4 x 1024, 212 and 273; 512, window 16, 46 and 100.
+  if (a.window == 0 || a.sinks == 0 || a.L < a.window + 4 * key_tile(a.d)) return 0;
   return far_bytes_of(a, far_chunk(a));
 }
 

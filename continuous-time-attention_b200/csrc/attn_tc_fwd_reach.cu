@@ -3,18 +3,22 @@
 // begin with.  The mathematics, the warps and the pipeline are those of attn_tc_fwd.cu, whose comments hold here too.
 // What is different:
 //
-// * Window: the key tiles between the first keys and the windows of a piece's rows are passed over; pages that no row
-//   of the piece sees are not loaded, nor are their entries in the table trusted.
+// * Window: the keys between the first ones and the windows of a piece's rows are passed over, in words of 32, so that
+//   one step holds the first keys and where the windows begin; pages that no row of the piece sees are not loaded, nor are
+//   their entries in the table trusted.
 // * Prefix: the rows are those of all sequences, 256 (row, head) pairs to a piece, and the keys are cut into parts, so
 //   that pieces fill the SMs; a part leaves its weighted values, maximum and sum in 32 bits for the join of the split
 //   kernel (attn_paged.cu), which runs beside this one over the sequences' own keys.
 // * Over e4m3 caches the scales' fractions come to shared memory with the values, and the keys' carry scale * log2(e).
 //
 // Bound like the forward by a step's chain of product, softmax and product, 2.0 us for the two tiles of a piece at dim
-// 128, and by what a piece costs before and behind its steps, 5 to 6 us: in windows of 512 a piece of 64 tokens has six
-// steps.  Measured, 32/8 heads of 128: 12 prompts of up to 4096 tokens, window 512, 4 first keys 424 us; chunks of 512 of 4
-// sequences, window 1024, over e4m3 83 us; 64 rows over 8192 keys in 7 parts beside the own keys 55 us, alone in 16 parts
-// 25; 16384 tokens, 8 heads of 64, window 1024 102 us.
+// 128, and by what a piece costs before and behind its steps, 5 to 6 us: in windows of 512 a piece of 64 tokens has five
+// steps.  Measured, 32/8 heads of 128: 12 prompts of up to 4096 tokens, window 512, 4 first keys 417 us; chunks of 512 of 4
+// sequences, window 1024, over e4m3 73 to 76 us; 64 rows over 8192 keys in 7 parts beside the own keys 55 us, alone in 16
+// parts 25; 16384 tokens, 8 heads of 64, window 1024 105 us.
+//
+// Scores over e4m3 stay in registers in no variant: read from tensor memory a second time for the weights, chunks take 73 us;
+// kept, with spills of 260 bytes, 94.
 #include <algorithm>
 
 #include "attn_tc_fwd.cuh"

@@ -73,7 +73,9 @@ def is_stale() -> bool:
 
 # A march kernel keeps its whole state in registers; a stack frame above a few
 # bytes means a helper was not inlined (its state went to local memory) or
-# large spills, either of which costs an order of magnitude.
+# large spills, either of which costs an order of magnitude.  The attention
+# kernels' softmax warps, at 96 registers a thread, spill up to 88 bytes of what
+# a piece of work needs once.
 MAX_STACK_BYTES = 96
 
 
