@@ -453,13 +453,13 @@ static int64_t backward_bytes(const AttnArgs& a, int dtype) {
   return a.dk != nullptr ? std::max(far_bytes(a, dtype), simt_far_bytes(a)) : 0;
 }
 
-// Up to 16 keys a row: the score gradients' rounding to 16 bits, which the tensor cores need, has few terms to average
-// over, and leaves dQ and dK 1.5 times as far off as the rounding of their own that is nearly all the FP32 pipe leaves (1.1
-// times).  That is slower, 1024 tokens, 8 heads of 64, window 4: 34 and 10 us, so it is for sizes where the call takes
-// longer than that to make.
-static bool few_keys(const AttnArgs& a) {
-  const int64_t tokens = a.cu != nullptr ? a.L : a.L * a.nseq;
-  return a.window > 0 && a.window + a.sinks <= 16 && tokens * a.H * a.d <= (1 << 20);
+// Where a row sees few keys, the score gradients' rounding to 16 bits, which the tensor cores need, has few terms to average
+// over, and leaves dQ and dK 1.5 to 1.7 times as far off as the rounding of their own that is nearly all the FP32 pipe leaves
+// (1.1 times).  That is slower, 1024 tokens, 8 heads of 64, window 4: 34 and 10 us, so it is for sizes where the call
+// takes longer than that to make.  A window that reaches over a short sequence counts as one.
+static bool few_keys(const AttnArgs& a, int64_t window) {
+  const int64_t tokens = a.cu != nullptr ? a.L : a.L * a.nseq, keys = a.window > 0 ? a.window + a.sinks : a.L;
+  return window > 0 && keys <= 32 && tokens * a.H * a.d <= (1 << 20);
 }
 
 int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int64_t window, int64_t sinks) {
@@ -489,7 +489,7 @@ int cta_window_attention_backward(const cta_attention_args* args, int64_t window
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(CTA_EINVAL, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_attn_delta(a, args->dtype, st);
-  if (e == cudaSuccess && (few_keys(a) || !launch_attn_tc_bwd(a, args->dtype, workspace, st, &e)))
+  if (e == cudaSuccess && (few_keys(a, window) || !launch_attn_tc_bwd(a, args->dtype, workspace, st, &e)))
     e = launch_attn_simt_bwd(a, args->dtype, workspace, st);
   return launched(e, "attention backward launch");
 }

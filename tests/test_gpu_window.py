@@ -132,6 +132,28 @@ def test_window_over_everything_is_none(window, sinks, dtype):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,window,sinks", [([3, 0, 1, 20, 8], 2**40, 0), ([32], 40, 3), ([33], 20, 12), ([700, 31, 2], 1, 31),
+                                               ([300, 9], 2, 0)])
+def test_few_keys(lens, window, sinks, dtype):
+    """Gradients of rows that see few keys, up to the sizes from which the tensor cores compute them and beyond."""
+    for heads, kv_heads, dim in ((2, 1, 40), (16, 4, 128)):
+        total = sum(lens) + 3
+        q, k, v, g = _inputs((total,), heads, kv_heads, dim, dtype, seed=total)
+        cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32).cuda()
+        for x in (q, k, v, g):
+            x[sum(lens):] = float("nan")
+        got = _run(q, k, v, g, causal=True, cu_seqlens=cu, window=window, sinks=sinks)
+        at = 0
+        for n in lens:
+            part = slice(at, at + n)
+            at += n
+            if n > 0:
+                _check_sequence([x[part] for x in got], q[part], k[part], v[part], g[part], _reach(n, n, window, sinks),
+                                dim**-0.5, dtype)
+        assert all((x[at:] == 0).all() for x in got)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim,heads,kv_heads,window,sinks", [(64, 8, 8, 1024, 4), (128, 8, 2, 500, 16), (128, 4, 1, 2000, 300),
                                                             (64, 2, 2, 31, 129)])
