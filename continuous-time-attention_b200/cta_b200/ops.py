@@ -1090,8 +1090,8 @@ def paged_attention(
     the table may hold anything: an engine may have freed them.
 
     `shared_prefix`: the batch's sequences all begin with the same keys, and the rows of
-    block_table name the same pages for the first shared_prefix of them (a page that
-    they fill in part does not count).  Where that pays they are read once for all
+    block_table, also of sequences that end earlier, name the same pages for the first
+    shared_prefix of them (a page that they fill in part does not count).  Where that pays they are read once for all
     rows; it changes what the call costs, and its sums' order, not what it computes.
     With a window it is not used.  A NaN or infinity in the v of a shared key may then also reach
     sequences that end before it."""

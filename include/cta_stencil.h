@@ -466,7 +466,8 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
  * block_table name the same pages for the first shared_prefix keys (>= 0; a last
  * page that they fill in part does not count), and those are read once for all
  * rows where that pays.  It changes the cost and the order of the sums, not what
- * is computed.  Sequences may end within the prefix. */
+ * is computed.  Sequences may end within the prefix; their rows name its pages
+ * all the same. */
 int64_t cta_prefix_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t shared_prefix);
 int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t shared_prefix, void* workspace,
                                int64_t workspace_bytes, void* stream);
