@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
   unsigned j = at - b * per_seq;
   const int h0 = static_cast<int>(group - at * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
   if (b >= static_cast<unsigned>(a.B)) return;
-  const int n = a.seq_lens != nullptr ? __ldg(a.seq_lens + b) : 0x7fffffff;  // nullptr: all of the table
+  // nullptr: all of the table; a length past it ends with it, as for the kernel that reads the pages (and reports it)
+  const int n = a.seq_lens != nullptr ? min(max(__ldg(a.seq_lens + b), 0), static_cast<int>(slots)) : static_cast<int>(slots);
   int low = 0;  // window: the first key that the first row's window holds
   if (a.window > 0) {
     int64_t begin;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
     for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i)
       for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
   if (c >= a.d) return;
-  bool there = n >= 0 && j < static_cast<unsigned>(n);
+  bool there = j < static_cast<unsigned>(n);
   if (a.window > 0) {
     // Left out where no row's window reaches, but for boxes that the reader loads whole: what lies beside a key that
     // counts meets a zero weight, and must not be NaN.

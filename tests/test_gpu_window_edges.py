@@ -1,0 +1,50 @@
+"""Sliding windows at the edges of what a call may hold: lengths past the block table, gradients of very different
+sizes, few keys a row at every size of a call, padding longer than the window; against the definition in 64 bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_paged import Setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    from cta_b200 import _lib
+
+    yield
+    assert _lib.device_error() == 0
+
+
+def _poisoned(s, **kw):
+    """paged_attention of the setup in a workspace of NaN, as an earlier call may have left it."""
+    from cta_b200 import _lib, ops
+
+    q, out, fn, args, nbytes, held = ops._paged_plan(
+        s.q, s.kc, s.vc, s.table, s.seq_lens, s.cu, max(s.rows), None, s.ks, s.vs, None, kw["window"], kw["sinks"])
+    ws = torch.full((nbytes,), 0xFF, dtype=torch.uint8, device="cuda")
+    _lib.enqueue(fn, q, *args, ws.data_ptr(), nbytes)
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("rows", [[1, 1], [40, 200]])
+@pytest.mark.parametrize("past", [1, 17, 100, 1000, 2**31 - 1 - 640])
+def test_lengths_past_the_table(past, rows, quantized, dtype):
+    """Reported, and computed as if the sequence ended with the table: no row holds what nobody wrote."""
+    from cta_b200 import _lib
+
+    s = Setup([640, 640], rows, 32, 8, 64, 16, dtype, quantized, seed=past % 1000)
+    for window, sinks in ((100, 8), (30, 0), (257, 33)):
+        want = _poisoned(s, window=window, sinks=sinks)
+        assert _lib.device_error() == 0 and torch.isfinite(want.float()).all()
+        for b in (0, 1):
+            s.seq_lens[b] = 640 + past
+            got = _poisoned(s, window=window, sinks=sinks)
+            assert _lib.device_error() == 2
+            assert torch.equal(got, want)
+            s.seq_lens[b] = 640
