@@ -134,6 +134,21 @@ cudaError_t allow_smem(int bytes) {
   return e;
 }
 
+// A kernel without shared memory that starts beside one that fills it would find that one's division of each SM, with
+// next to no L1, and keep it to its end; asked for, its own comes with the SMs that are idle.  Once per kernel and device.
+template <auto Kernel>
+cudaError_t prefer_l1() {
+  static std::atomic<uint64_t> done{0};  // one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxL1);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 inline int num_sms_here() {
   int dev = 0, v = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;

@@ -878,6 +878,10 @@ struct Split {
   }
   static cudaError_t run(const PagedArgs& a, cudaStream_t st) {
     constexpr bool kHalf = FP8 || std::is_same<T, __half>::value;
+    if (CUT && a.prefix_splits > 0) {
+      const cudaError_t l1 = prefer_l1<paged_split_kernel<T, FP8, DP, ROWS, CUT>>();
+      if (l1 != cudaSuccess) return l1;
+    }
     const cudaError_t e = launch_grid<paged_split_kernel<T, FP8, DP, ROWS, CUT>>(
         CUT && a.prefix_splits > 0, (a.workers + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, st, a);
     if (e != cudaSuccess) return e;
