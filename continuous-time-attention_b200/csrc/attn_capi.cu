@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
@@ -371,25 +372,32 @@ PrefixPlan prefix_plan(const PagedArgs& a, int dtype, int quantized, int64_t sha
   if (a.T < 2 || keys < 1 || width * a.page >= (1LL << 30) || !(a.scale > 0.f) || !tma_can_address(a) || tensor_cores_pay(a) ||
       a.n_pages < 1)
     return p;
-  // It costs a launch, two over e4m3, and the sums' way through memory, about what HBM takes for 40 (e4m3 64) MB.  32/8 heads
-  // of 128, calls with and without it: 16 sequences behind 512 keys, 31 MB read again, 20.9 and 19.3 us, behind 1024, 63
-  // MB, 21.2 and 23.1; e4m3: behind 2048, 65 MB, 27.5 and 27.3, 64 sequences behind 1024, 136 MB, 31.6 and 41.8.
-  const int64_t again = std::max<int64_t>(a.B, (a.T * (a.H / a.Hk) + 15) / 16) - 1;
-  if (again * keys * 2 * a.Hk * (quantized ? a.d + 4 : 2 * a.d) < (quantized ? 64000000 : 40000000) &&
-      g_prefix_always.load(std::memory_order_relaxed) == 0)
-    return p;
+  // It costs a launch, two over e4m3, the sums' way through memory, and a split kernel whose last workers start when the
+  // parts are done; and what is read again comes from L2 in part.  So it is for calls that spare 120 MB, over e4m3, where
+  // reading is bound by the codes' conversion, 450,000 rows of k and of v (fp16, whose parts take longer, 900,000).  How
+  // many keys of their own the sequences have is not known here (a block table is as wide as its owner's longest
+  // sequence may ever be), so it has to do for few and for many.  GPU time with and without it, 32/8 heads of 128: 16
+  // sequences of 16 to 64, 16 to 1024, 2048 to 4096 own keys behind 2048, 126 MB, 16, 25, 55 and 27, 31, 54 us; 4 behind
+  // 8192, 100 MB, 25, 26, 40 and 30, 30, 36.  e4m3, few and many: 64 behind 1024, 516,000 rows, 22, 127 and 39, 125, in
+  // fp16 24, 129 and 39, 117; 16 behind 2048, 246,000 rows, 21, 55 and 25, 51.  The worst found: 128 of 2048 to 4096 own
+  // keys behind 2048, 8/1 heads, whose prefix L2 holds, 61 and 55.
+  const int64_t rows = (std::max<int64_t>(a.B, (a.T * (a.H / a.Hk) + 15) / 16) - 1) * keys * a.Hk;  // of k and of v, read again
+  const double bytes = static_cast<double>(rows) * 2 * (quantized ? a.d + 4 : 2 * a.d);
+  const bool pays = !quantized ? bytes >= 120e6 : rows >= (dtype == CTA_F16 ? 900000 : 450000);
+  if (!pays && g_prefix_always.load(std::memory_order_relaxed) == 0) return p;
   const int64_t tiles = (keys + 127) / 128, ctas = prefix_tiles(a);
-  // Both kernels run at once: the parts' CTAs, one per SM, leave the split kernel the other SMs, and their own when they
-  // are done.  So there are as many parts as let both end at about the same time.  In SM-microseconds, measured: a part
-  // costs 12 and each of its key tiles 3.5 (e4m3 3.8, in fp16 5.5); the own keys, taken as half of what the table holds,
-  // 1.2 times what HBM needs (e4m3 twice).  32/8 heads of 128: 64 sequences of 16 to 1024 own keys behind 8192 take 63 us
-  // with the parts on 56 SMs, 82 with them on 128 and 90 on 40; 64 of 64 own keys 39 on 112 or 128 SMs, 42 on 72; 128 of
-  // 16 to 512 behind 16384, e4m3 in fp16, 140 us on 112 and 154 on 128.
-  const double tile_us = !quantized ? 3.5 : dtype == CTA_F16 ? 5.5 : 3.8;
-  const double own_bytes = 0.5 * a.B * static_cast<double>(width * a.page - keys) * 2. * a.Hk * (quantized ? a.d + 4 : 2 * a.d);
-  const double shared_us = static_cast<double>(tiles) * ctas * tile_us, own_us = own_bytes / 44300. * (quantized ? 2. : 1.2);
-  const double parts = shared_us / ((shared_us + own_us) / 148. + 6.) / ctas;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(148 / ctas, static_cast<int64_t>(parts + 0.5)));
+  // Both kernels run at once, a part on an SM of its own; the workers that find no room start when a part ends.  Few long
+  // parts keep the call waiting where the own keys are few, many short ones keep their SMs from them where they are many.
+  // A part takes 12 us and 3.5 for each key tile (e4m3 3.8, in fp16 5.5), measured; it is to end within a seventh of what
+  // reading the prefix again would take, and within 16 tiles, on 64 to 112 SMs.  Own keys as above, 64 sequences behind
+  // 8192: 8 parts (64 SMs), the rule's, 41, 63, 165 us, 13 parts 34, 68, 163, 5 parts 55, 60, 174; without 218, 233, 307.
+  // 16 behind 8192: 13 parts, the rule's, 26, 35, 62, 8 parts 33, 36, 69.  4 behind 16384: 13 parts, the rule's, 39, 40, 48, 8
+  // parts 55, 56, 59; without 43, 44, 51.  128 behind 16384, e4m3 in fp16, up to 512 own keys: 7 parts (112 SMs), the rule's,
+  // 134, 8 parts 148, 6 parts 147.
+  const double tile_us = !quantized ? 3.5 : dtype == CTA_F16 ? 5.5 : 3.8, again_us = bytes / 6.5e6;
+  const double longest = std::min(16., std::max(1., (again_us / 7. - 12.) / tile_us));  // key tiles of a part
+  const int64_t few = std::max<int64_t>(1, 64 / ctas), many = std::max<int64_t>(1, 112 / ctas);
+  const int64_t most = std::max(few, std::min(many, static_cast<int64_t>(std::ceil(tiles / longest))));
   const int64_t per = (tiles + most - 1) / most, splits = (tiles + per - 1) / per;
   const int dp = a.d <= 64 ? 64 : 128;
   // the values' rows start on 32 bytes, the workspace on 16

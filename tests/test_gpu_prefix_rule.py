@@ -59,3 +59,12 @@ def test_long_own_keys():
     shared, plain = _both(64, 2048, 2048, 4096)
     # 0.9 of it; 1.5 where it lost its L1.  A clock that changes between the two moves this by a few percent.
     assert shared < 1.2 * plain, (shared, plain)
+
+
+@pytest.mark.parametrize("batch,prefix,low,high", [(16, 8192, 16, 64), (4, 16384, 16, 1024), (16, 8192, 2048, 4096), (64, 8192, 16, 1024),
+                                                  (16, 2048, 2048, 4096)])
+def test_wide_block_tables(batch, prefix, low, high):
+    """Tables of an engine whose sequences may be 131072 keys long."""
+    shared, plain = _both(batch, prefix, low, high, width=131072 // 16)
+    # 0.3 to 1.02 of it; 2 to 6 times as much where the table's width was taken for the sequences'
+    assert shared < 1.2 * plain, (shared, plain)
