@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad
 
 from . import ops
 
@@ -48,13 +47,6 @@ class _PromptAttention(torch.autograd.Function):
         dq, dk, dv = ops._attention_backward(grad_out, q, k, v, out, 0 if low is None else low.data_ptr(), lse, cu,
                                              mask_words, *ctx.plan, need_q, need_k or need_v)
         return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
-
-
-def _tangents(*tensors: torch.Tensor) -> bool:
-    """Whether one carries a forward-mode tangent: such a call goes through the function, which refuses it.
-    Outside of a dual level, a look at its number (unpack_dual takes 0.4 us a tensor)."""
-    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
-        forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def prompt_attention(
@@ -96,7 +88,8 @@ def prompt_attention(
         if key_mask.get_device() != q.get_device():
             raise ValueError(f"key_mask on {key_mask.device}, expected {q.device}")
         words = ops.attention_mask(key_mask)
-    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _tangents(q, k, v):
+    # a call with a tangent goes through the function, which refuses it
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or ops._tangents(q, k, v):
         return _PromptAttention.apply(q, k, v, words, cu_seqlens, bool(causal) if window is None else reach, scale)
     return ops.attention_forward(q, k, v, causal=causal, scale=scale, mask_words=words, cu_seqlens=cu_seqlens,
                                  need_lse=False, window=window, sinks=sinks)[0]

@@ -13,6 +13,7 @@ import operator
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -581,6 +582,13 @@ def attention_mask(key_mask: torch.Tensor) -> torch.Tensor:
     return words
 
 
+def _tangents(*tensors: torch.Tensor) -> bool:
+    """Whether one carries a forward-mode tangent, which a call would drop.
+    Outside of a dual level, a look at its number (unpack_dual takes 0.4 us a tensor)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _attention_inputs(q, k, v, cu_seqlens, mask_words, scale):
     """Checked inputs and sizes: (q, k, v, cu or None, (sequences, length, heads, kv_heads, dim), dtype code, scale)."""
     device = q.get_device()  # plain numbers: comparing device objects costs several times as much
@@ -949,7 +957,13 @@ def rotary_cache_write(
     alone (padding rows; their queries are rotated all the same), the others must be
     distinct.  A slot past the cache is skipped; a token whose position is
     outside of cos_sin has a zero query and is not written.  Both are reported by
-    ``_lib.device_error()``, the position only where the slot is not negative."""
+    ``_lib.device_error()``, the position only where the slot is not negative.
+
+    Not differentiable: where the queries returned would need a gradient (of q or
+    cos_sin) it raises; call it under ``torch.no_grad()`` or on detached tensors.  The
+    cache takes no gradients of k and v, as for ``kv_cache_write``."""
+    if (torch.is_grad_enabled() and (q.requires_grad or cos_sin.requires_grad)) or _tangents(q, cos_sin):
+        raise ValueError("rotary_cache_write has no gradient: q and cos_sin must not require one")
     return _rotary_launch(*_rotary_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved, k_scale,
                                         v_scale, out))
 

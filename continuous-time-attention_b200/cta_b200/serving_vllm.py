@@ -205,8 +205,9 @@ class CtaPostAttnMixer(nn.Module):
         ``max_query_len`` on the host.  The cache is [pages, page_size, kv_heads,
         dim], in q's type or float8_e4m3fn with scales [pages, kv_heads,
         page_size] (``ops.kv_cache_write``, ``ops.paged_attention``).  No device
-        data is read on the host.  Rows behind the last sequence come back
-        undefined, as the mixer leaves them; ``residual`` as for ``forward``.
+        data is read on the host, and no gradients pass through the attention.
+        Rows behind the last sequence come back undefined, as the mixer leaves
+        them; ``residual`` as for ``forward``.
 
         ``positions`` [T] with ``cos_sin`` (and ``interleaved``) rotate q and k by
         their positions on the way (``ops.rotary_cache_write``; q itself is left as
