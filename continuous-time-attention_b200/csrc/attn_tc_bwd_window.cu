@@ -884,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = key < t.n;
         const int c0 = (part & 1) * (DP / 2);  // parts 0, 1: dV, parts 2, 3: dK, half of the columns each
         const uint32_t sums = (part < 2 ? t_dv : t_dk) + lanes + c0;
-        const float mul = part < 2 ? (kHalf ? kHalfUnit : 1.f) : (kHalf ? a.scale * pow2(-unit) : a.scale);
+        float mul = part < 2 ? (kHalf ? kHalfUnit : 1.f) : (kHalf ? a.scale * pow2(-unit) : a.scale);
         const bool first_ones = key >= p.lo && key < p.sink_end;
         const int at = (key - max(t.first, p.lo)) * 2 * DP + (part < 2 ? 0 : DP) + c0;  // in far_at's
         if constexpr (FORM == kFar) {
@@ -908,22 +908,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (p.steps > 0 && t.first < p.sink_end && p.far_from < t.n) {
             pdl_wait();  // for the far rows' CTAs
             if (__any_sync(0xffffffffu, first_ones)) {
-              const float back = 1.f / mul;
+              // In the gradients' own units, not in the near rows': if those have no gradient theirs is 2^100, and a far
+              // sum in it would leave fp32.
 #pragma unroll 1
               for (int c = 0; c < DP / 32; ++c) {
                 uint32_t o[16];
                 tc::ld16(sums + 16 * c, o);
                 tc::wait_ld(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * mul);
                 if (first_ones) {
                   for (int chunk = p.far_from / f.chunk; chunk * f.chunk < t.n; ++chunk) {
                     const float4* x = reinterpret_cast<const float4*>(far_at(p, t, chunk) + at + 16 * c);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                       const float4 y = __ldcg(x + e);  // written while this kernel may already be there
-                      o[4 * e] = __float_as_uint(fmaf(y.x, back, __uint_as_float(o[4 * e])));
-                      o[4 * e + 1] = __float_as_uint(fmaf(y.y, back, __uint_as_float(o[4 * e + 1])));
-                      o[4 * e + 2] = __float_as_uint(fmaf(y.z, back, __uint_as_float(o[4 * e + 2])));
-                      o[4 * e + 3] = __float_as_uint(fmaf(y.w, back, __uint_as_float(o[4 * e + 3])));
+                      o[4 * e] = __float_as_uint(__uint_as_float(o[4 * e]) + y.x);
+                      o[4 * e + 1] = __float_as_uint(__uint_as_float(o[4 * e + 1]) + y.y);
+                      o[4 * e + 2] = __float_as_uint(__uint_as_float(o[4 * e + 2]) + y.z);
+                      o[4 * e + 3] = __float_as_uint(__uint_as_float(o[4 * e + 3]) + y.w);
                     }
                   }
                 }
@@ -931,6 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc::st16(sums + 16 * c, o);
               }
               tc::wait_st();
+              mul = 1.f;
             }
           }
           if (part < 2) {

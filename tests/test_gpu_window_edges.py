@@ -5,7 +5,9 @@ from __future__ import annotations
 import pytest
 import torch
 
+from test_gpu_attention import _check_sequence, _inputs, _run
 from test_gpu_paged import Setup
+from test_gpu_window import _reach
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +50,17 @@ def test_lengths_past_the_table(past, rows, quantized, dtype):
             assert _lib.device_error() == 2
             assert torch.equal(got, want)
             s.seq_lens[b] = 640
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (4, 1, 128)])
+@pytest.mark.parametrize("scale,size", [(2e-6, 1.5e4), (2e-7, 1.5e4), (0.1, 1.0)])
+def test_gradients_far_behind_rows_without(scale, size, heads, kv_heads, dim, dtype):
+    """Only late rows have a gradient, as where a prompt's tokens carry no loss: what reaches the first keys comes from the
+    rows behind their tile alone, and is right for any scale."""
+    n, window, sinks = 3000, 128, 4
+    q, k, v, g = _inputs((1, n), heads, kv_heads, dim, dtype, seed=12)
+    q, g = ((x.float() * size).clamp(-6e4, 6e4).to(dtype) for x in (q, g))  # fp16's largest number is 65504
+    g[:, :500] = 0
+    got = _run(q, k, v, g, causal=True, window=window, sinks=sinks, scale=scale)
+    _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _reach(n, n, window, sinks), scale, dtype)
