@@ -461,13 +461,17 @@ static int64_t backward_bytes(const AttnArgs& a, int dtype) {
   return a.dk != nullptr ? std::max(far_bytes(a, dtype), simt_far_bytes(a)) : 0;
 }
 
-// Where a row sees few keys, the score gradients' rounding to 16 bits, which the tensor cores need, has few terms to average
-// over, and leaves dQ and dK 1.5 to 1.7 times as far off as the rounding of their own that is nearly all the FP32 pipe leaves
-// (1.1 times).  That is slower, 1024 tokens, 8 heads of 64, window 4: 34 and 10 us, so it is for sizes where the call
-// takes longer than that to make.  A window that reaches over a short sequence counts as one.
+// The tensor cores need weights and score gradients in 16 bits, which leaves dQ and dK 1.45 times as far off as the rounding
+// of their own, and 1.5 to 1.8 times where a row sees up to 8 keys, since there are few terms to average over; the FP32
+// pipe 1.05 to 1.2 (1.4 for two keys).  That is a trade of time for it, for calls that a training step does not notice: a CTA
+// walks the heads of its group and two row tiles, or with first keys up to four, so within these limits the backward takes
+// 19 to 105 us against 11 to 28, and a training call in PyTorch takes 130 to make; a captured graph pays the difference.
+// 32/8 heads of 128, past them: 256 tokens, window 4, 208 and 23 us, with 4 first keys 369 and 27; 2048 tokens of 8 heads of 64,
+// with first keys, 104 and 29.  A window that reaches over a short sequence counts as one.
 static bool few_keys(const AttnArgs& a, int64_t window) {
   const int64_t tokens = a.cu != nullptr ? a.L : a.L * a.nseq, keys = a.window > 0 ? a.window + a.sinks : a.L;
-  return window > 0 && keys <= 32 && tokens * a.H * a.d <= (1 << 20);
+  const int chain = a.H / a.Hk * (a.d <= 64 ? 64 : 128) * (a.sinks > 0 ? 2 : 1);
+  return window > 0 && keys <= 8 && chain <= 256 && tokens * a.H * a.d <= (1 << 19);
 }
 
 int64_t cta_window_attention_workspace_bytes(const cta_attention_args* args, int64_t window, int64_t sinks) {

@@ -64,3 +64,49 @@ def test_gradients_far_behind_rows_without(scale, size, heads, kv_heads, dim, dt
     g[:, :500] = 0
     got = _run(q, k, v, g, causal=True, window=window, sinks=sinks, scale=scale)
     _check_sequence([x[0] for x in got], q[0], k[0], v[0], g[0], _reach(n, n, window, sinks), scale, dtype)
+
+
+def _graph_time(call, n=10):
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(n):
+            call()
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) / n)
+    return sorted(times)[3]
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,window,sinks", [(256, 32, 8, 128, 4, 4), (256, 32, 8, 128, 4, 0), (1024, 8, 2, 128, 4, 4),
+                                                                   (2048, 8, 8, 64, 4, 4), (1024, 8, 8, 64, 16, 4)])
+def test_windows_of_few_keys_cost_what_others_do(tokens, heads, kv_heads, dim, window, sinks):
+    """Where the FP32 pipe would take longer than a training call takes to make, or is no more exact, the tensor cores
+    compute the gradients, as under wider windows."""
+    from cta_b200 import ops
+
+    q, k, v, g = _inputs((1, tokens), heads, kv_heads, dim, torch.bfloat16, seed=3)
+    times = []
+    for w in (window, 40):
+        kw = dict(causal=True, window=w, sinks=sinks)
+        low = torch.empty_like(q)
+        out, lse = ops.attention_forward(q, k, v, out_low=low, **kw)
+        times.append(_graph_time(lambda: ops.attention_backward(g, q, k, v, out, lse, out_low=low, **kw)))
+    # the same steps of work, within the few percent of a clock that moves; 2.7 to 14 times on the FP32 pipe
+    assert times[0] < 1.5 * times[1], times
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim", [(300, 4, 4, 64), (300, 4, 1, 128), (9, 6, 2, 96)])
+@pytest.mark.parametrize("window,sinks", [(2, 0), (3, 0), (1, 1), (4, 4), (8, 0), (9, 0), (5, 4)])
+def test_few_keys_on_either_side_of_the_rule(window, sinks, tokens, heads, kv_heads, dim, dtype):
+    q, k, v, g = _inputs((2, tokens), heads, kv_heads, dim, dtype, seed=window)
+    got = _run(q, k, v, g, causal=True, window=window, sinks=sinks)
+    for b in range(2):
+        _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], _reach(tokens, tokens, window, sinks), dim**-0.5, dtype)
