@@ -120,11 +120,14 @@ struct PagedArgs {
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
   // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these what it left out of their
-  // elements [B, Hk, residue_row(table_width * page)]: the fractions of the scales in bf16, the key's scale and the
+  // elements [B, Hk, residue_row(table_width * page)], over a window [Hk, copy_slots]: the fractions of the scales in bf16, the key's scale and the
   // logarithm (base 2) of the value's in fp16, rows on 32 bytes; else nullptr
   const float* k_res;
   const float* v_res;
   int64_t expanded_pages;
+  // over a window the copy is one run of `copy_slots` slots, which holds what the rows can reach, see CopySlots
+  int64_t copy_slots;
+  int copy_stride, copy_dense;
   int fold_scale;  // k_res times scale * log2(e): for windows and prefixes
   // shared prefix of `skip` keys: its sums over prefix_splits parts of prefix_chunk keys, for every row of q
   int prefix_splits, prefix_chunk;
@@ -150,11 +153,14 @@ bool launch_paged_tc_window(const PagedArgs& p, int dtype, cudaStream_t st, cuda
 int64_t prefix_tiles(const PagedArgs& p);  // CTAs for each part
 bool launch_prefix_tc(const PagedArgs& p, int dtype, cudaStream_t st, cudaError_t* e);
 // e4m3 caches: the pages that the table names, as 16-bit rows in page order (page i of sequence b is page
-// b * table_width + i), for the tensor-core kernel
+// b * table_width + i), or with a window the keys of CopySlots, for the tensor-core kernel
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
                                 cudaStream_t st);
 // entries of k_res and v_res for a sequence and head, in whole key tiles
 __host__ __device__ constexpr int64_t residue_row(int64_t slots) { return (slots + 127) / 128 * 128; }
+
+// the copy's slots for a windowed chunk (PagedArgs::copy_*)
+void plan_copy_slots(PagedArgs& p);
 
 int set_prefix_always(int value);  // use shared prefixes where that does not pay too; the value before
 int read_device_error_paged(int clear);

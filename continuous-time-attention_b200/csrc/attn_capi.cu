@@ -309,11 +309,19 @@ bool tensor_cores_pay(const PagedArgs& a) {
 // 16-bit copy of the pages that the table can name, k then v, and what goes beside them; 0 where that is too much to
 // ask for
 constexpr int64_t kMostExpanded = 1LL << 31;
-int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64_t d) {
-  const int64_t slots = b * width * page;
+int64_t copy_bytes(int64_t slots, int64_t beside, int64_t hk, int64_t d) {
   if (slots >= (1LL << 24) || slots * hk >= (1LL << 26)) return 0;
-  const int64_t bytes = slots * hk * d * 4 + b * residue_row(width * page) * hk * 8;
+  const int64_t bytes = slots * hk * d * 4 + beside * hk * 8;
   return bytes > 0 && bytes <= kMostExpanded ? bytes + 32 : 0;  // and what puts its start on 32 bytes
+}
+int64_t expanded_bytes(int64_t b, int64_t width, int64_t page, int64_t hk, int64_t d) {
+  return copy_bytes(b * width * page, b * residue_row(width * page), hk, d);
+}
+// of chunks, and where their keys go under a window
+int64_t chunk_bytes(PagedArgs& a) {
+  if (a.window == 0) return expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
+  plan_copy_slots(a);
+  return copy_bytes(a.copy_slots, a.copy_slots, a.Hk, a.d);
 }
 
 int64_t split_bytes(int workers, int d) {
@@ -340,10 +348,11 @@ int paged_pointers(const PagedArgs& a, int quantized, const void* workspace, int
 
 // Expands the pages of an e4m3 cache that p's table names into `ws`, and points x at them.
 cudaError_t expand_pages(const PagedArgs& p, int dtype, char* ws, PagedArgs& x, cudaStream_t st) {
-  const int64_t pages = static_cast<int64_t>(p.B) * p.table_width, part = pages * p.page * p.Hk * p.d * 2;
+  const int64_t pages = static_cast<int64_t>(p.B) * p.table_width;
+  const int64_t part = (p.window > 0 ? p.copy_slots : pages * p.page) * p.Hk * p.d * 2;
   ws += -reinterpret_cast<intptr_t>(ws) & 31;
   float* k_res = reinterpret_cast<float*>(ws + 2 * part);
-  float* v_res = k_res + p.B * residue_row(static_cast<int64_t>(p.table_width) * p.page) * p.Hk;
+  float* v_res = k_res + (p.window > 0 ? p.copy_slots : p.B * residue_row(static_cast<int64_t>(p.table_width) * p.page)) * p.Hk;
   PagedArgs fold = p;
   fold.fold_scale = p.window > 0 || p.seq_lens == nullptr;  // windows, and the whole table of a prefix
   const cudaError_t e = launch_cache_expand(fold, dtype, ws, ws + part, k_res, v_res, st);
@@ -577,7 +586,7 @@ int64_t cta_window_paged_attention_workspace_bytes(const cta_paged_attention_arg
   if (a.T == 0 || a.B == 0) return 0;
   if (tensor_cores_pay(a)) {
     if (!args->quantized) return 0;
-    const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
+    const int64_t bytes = chunk_bytes(a);
     if (bytes > 0) return bytes;
   }
   return split_bytes(paged_split_workers(a, args->dtype, args->quantized), a.d);
@@ -595,7 +604,7 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (tensor_cores_pay(a)) {
-    const int64_t bytes = expanded_bytes(a.B, a.table_width, a.page, a.Hk, a.d);
+    const int64_t bytes = chunk_bytes(a);
     if (!args->quantized) {
       if (launch_paged_tc(a, args->dtype, st, &e)) return launched(e, "paged attention launch");
       return fail(CTA_EUNSUPPORTED, "paged attention of chunks: the tensors cannot be addressed by TMA");

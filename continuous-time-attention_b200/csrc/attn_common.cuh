@@ -228,6 +228,22 @@ __device__ __forceinline__ Reach reach_of(const AttnArgs& a, int lo) {
   return Reach{a.window, a.sinks > 0 ? lo + a.sinks : 0};
 }
 
+// Where the keys of a sequence lie in the 16-bit copy of an e4m3 cache that a chunk under a window reads.  Dense: whole
+// tiles of 128 keys, those of the first keys and those from the first row's window on, so that the copy's size follows
+// from the window, the first keys and the rows, not from the block table's width.  A sequence has copy_stride slots
+// and one for each of its rows: with tiles of 128 on either side of both, its keys fit.  Where that is no less than the
+// table, every key has a slot.
+struct CopySlots {
+  int base, first, gap;  // key j at base + j, those from `first` on `gap` further down
+  __device__ __forceinline__ int at(int key) const { return base + key - (key >= first ? gap : 0); }
+};
+// of a sequence of n keys (within the table), whose rows begin at `begin`
+__device__ __forceinline__ CopySlots copy_slots(int stride, bool dense, int window, int sinks, int seq, int64_t begin, int rows, int n) {
+  if (!dense) return CopySlots{seq * stride, 0, 0};
+  const int first = static_cast<int>(residue_row(sinks)), low = max(n - rows - window + 1, 0);
+  return CopySlots{seq * stride + static_cast<int>(begin) / 128 * 128, first, max(first, low / 128 * 128) - first};
+}
+
 // A window's far rows, those behind the window of a key tile of `rows` that holds first keys, go in parts of `chunk`; part c
 // of a sequence has the place far_place + c of far_places.  Packed: a sequence has far rows only if it is at least window +
 // rows long, so its place among those, or among all if they are fewer, tells them apart.

@@ -42,10 +42,11 @@ struct FwdArgs {
   int64_t table_sB;
   const int32_t* seq_lens;
   int table_width, page, n_pages, box;  // box: keys per TMA box
-  // SCALED: page i of sequence b is page b * table_width + i (the table still says which are valid), and these are
-  // what the expansion left out of its elements, see launch_cache_expand
+  // SCALED: page i of sequence b is page b * table_width + i, or with a window a key lies where CopySlots says (the table
+  // still says which are valid), and these are what the expansion left out of its elements, see launch_cache_expand
   const float* k_res;
   const float* v_res;
+  int copy_stride, copy_dense, copy_slots;
   int wide_out, wide_low;  // alignment of the outputs' rows, see store_rows
   // shared prefix: `splits` parts of `chunk` keys (whole tiles), whose sums go to part_o [splits, rows, heads, DP] and
   // part_ml [splits, rows, heads, 4] as the split kernel leaves them (attn_paged.cu)
@@ -294,6 +295,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         taken();
         continue;
       }
+      constexpr bool kCopy = SCALED && FORM == kWindow;
+      CopySlots copy = {};
+      if constexpr (kCopy)
+        copy = copy_slots(f.copy_stride, f.copy_dense, a.window, a.sinks, x.t.seq, x.t.row0, x.t.n, x.n);
       if (nq > 0) ok = tc::wait(&bars.q_empty, (nq - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               atomicExch(&g_tc_fwd_reach_error, kDevBadIndex);
               page = -1;
             } else if (SCALED) {
-              page = x.t.seq * f.table_width + key / f.page;
+              page = kCopy ? 0 : x.t.seq * f.table_width + key / f.page;
             }
           }
           const uint32_t got = __ballot_sync(0xffffffffu, page >= 0);
@@ -332,10 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           int64_t res_at = 0;
           uint32_t res = 0u;
           if (SCALED && (step & 1)) {
-            const int64_t res_row = residue_row(static_cast<int64_t>(f.table_width) * f.page);
-            const int res_key = y.key(j0 + (lane & 3) * 32);
-            res_at = (static_cast<int64_t>(x.t.seq) * a.Hk + x.hk) * res_row + res_key;
-            res = __ballot_sync(0xffffffffu, lane < 8 && res_key < res_row);
+            const int64_t res_row = kCopy ? f.copy_slots : residue_row(static_cast<int64_t>(f.table_width) * f.page);
+            const int res_key = y.key(j0 + (lane & 3) * 32), slot = kCopy ? copy.at(res_key) : res_key;
+            res_at = (static_cast<int64_t>(kCopy ? 0 : x.t.seq) * a.Hk + x.hk) * res_row + slot;
+            res = __ballot_sync(0xffffffffu, lane < 8 && slot >= 0 && slot < res_row);
           }
           if (lane == 0) {
             // one bit per 16 keys
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (page >= 0)
             for (int c = 0; c < DP / 64; ++c)
               tc::tma_load_4d(dst + c * L::kHalf + lane * f.box * 128, map, &bars.kv_full[stage], 64 * c, x.hk,
-                              key % f.page, page);
+                              kCopy ? copy.at(key) : key % f.page, page);
         } else {
           if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[stage], L::kTile);
           __syncwarp();
@@ -802,14 +807,18 @@ bool paged_maps(const PagedArgs& p, int dtype, int most_box, FwdArgs& f, CUtenso
   f.k_res = p.k_res;
   f.v_res = p.v_res;
   f.box = std::min(p.page & -p.page, most_box);  // the largest power of two that divides a page
-  // expanded pages are contiguous
-  const int64_t pages = p.k_res != nullptr ? p.expanded_pages : p.n_pages;
-  const AttnStrides dense{static_cast<int64_t>(p.page) * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
+  // expanded pages are contiguous, the keys of a window one page
+  const bool copy = p.k_res != nullptr && p.window > 0;
+  f.copy_stride = p.copy_stride;
+  f.copy_dense = p.copy_dense;
+  f.copy_slots = static_cast<int>(p.copy_slots);
+  const int64_t pages = copy ? 1 : p.k_res != nullptr ? p.expanded_pages : p.n_pages, page = copy ? p.copy_slots : p.page;
+  const AttnStrides dense{page * p.Hk * p.d, static_cast<int64_t>(p.Hk) * p.d, p.d};
   const AttnStrides ks = p.k_res != nullptr ? dense : AttnStrides{p.kc_sP, p.kc_sS, p.kc_sH};
   const AttnStrides vs = p.k_res != nullptr ? dense : AttnStrides{p.vc_sP, p.vc_sS, p.vc_sH};
   return attn_map(&maps[0], p.q, dtype, 1, p.T, p.H, p.d, a.qs, f.pack, f.tile_tokens) &&
-         attn_map(&maps[1], p.k_cache, dtype, pages, p.page, p.Hk, p.d, ks, 1, f.box) &&
-         attn_map(&maps[2], p.v_cache, dtype, pages, p.page, p.Hk, p.d, vs, 1, f.box);
+         attn_map(&maps[1], p.k_cache, dtype, pages, page, p.Hk, p.d, ks, 1, f.box) &&
+         attn_map(&maps[2], p.v_cache, dtype, pages, page, p.Hk, p.d, vs, 1, f.box);
 }
 
 }  // namespace

@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
 // Codes of the pages of each sequence, in order, as exact 16-bit rows.  bf16, whose exponents reach as far as fp32's:
 // each times the power of two below its scale, whose fraction goes into k_res and v_res.  fp16: the codes alone, and
 // beside them the key's scale and the logarithm of the value's (attn_tc_fwd.cu says why).  fold_scale: what is for
-// the keys carries what takes a score to an exponent of two.
+// the keys carries what takes a score to an exponent of two.  Window: `per_seq` is copy_stride, and the groups behind
+// those of all sequences are the slots that they have for their rows.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_constant__ PagedArgs a, T* k_out, T* v_out,
                                                                 float* k_res, float* v_res, unsigned per_seq) {
@@ -232,30 +233,51 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
   const unsigned blocks = (a.Hk + kHeads - 1) / kHeads;
   const unsigned group = (blockIdx.x * kThreads + threadIdx.x) / GROUP;
   const unsigned slots = static_cast<unsigned>(a.table_width) * a.page;  // per sequence
-  const unsigned at = group / blocks, b = at / per_seq;
-  unsigned j = at - b * per_seq;
+  const unsigned at = group / blocks;
+  unsigned b = at / per_seq, j = at - b * per_seq;
   const int h0 = static_cast<int>(group - at * blocks) * kHeads, lane = threadIdx.x % GROUP, c = lane * 8;
-  if (b >= static_cast<unsigned>(a.B)) return;
+  if (a.window > 0 && at >= a.copy_slots) return;
+  if (b >= static_cast<unsigned>(a.B)) {
+    if (a.window == 0 || !a.copy_dense) return;
+    // the last sequence whose rows begin in or before this slot's tile
+    const unsigned t = at - static_cast<unsigned>(a.B) * per_seq;
+    unsigned last = a.B - 1;
+    int64_t begin;
+    int rows;
+    for (b = 0; b < last;) {
+      const unsigned mid = (b + last + 1) / 2;
+      clamp_range(a.cu, mid, a.T, begin, rows);
+      if (static_cast<unsigned>(begin) / 128 * 128 <= t) b = mid;
+      else last = mid - 1;
+    }
+    clamp_range(a.cu, b, a.T, begin, rows);
+    if (t < static_cast<unsigned>(begin) / 128 * 128) return;
+    j = per_seq + t - static_cast<unsigned>(begin) / 128 * 128;
+  }
   // nullptr: all of the table; a length past it ends with it, as for the kernel that reads the pages (and reports it)
   const int n = a.seq_lens != nullptr ? min(max(__ldg(a.seq_lens + b), 0), static_cast<int>(slots)) : static_cast<int>(slots);
   int low = 0;  // window: the first key that the first row's window holds
+  unsigned row = b * slots + j;  // where the key goes
   if (a.window > 0) {
     int64_t begin;
     int rows;
     clamp_range(a.cu, b, a.T, begin, rows);
     low = max(n - rows - a.window + 1, 0);
-    // the key tiles between the first keys and the windows are nobody's
-    const unsigned sinks = static_cast<unsigned>(residue_row(a.sinks));
-    if (j >= sinks) j = max(sinks, static_cast<unsigned>(low) / 128 * 128) + (j - sinks);
+    const CopySlots copy = copy_slots(per_seq, a.copy_dense, a.window, a.sinks, b, begin, rows, n);
+    row = copy.base + j;
+    if (a.copy_dense) {
+      // no further than the rows reach: what follows is the next sequence's
+      if (j >= static_cast<unsigned>(copy.first + residue_row(a.window + rows + 127))) return;
+      if (j >= static_cast<unsigned>(copy.first)) j += copy.gap;
+    }
   }
   if (j >= slots) return;
-  const unsigned row = b * slots + j;
-  // what goes beside this key, and behind the last key up to the row's end
-  const int64_t res_row = residue_row(slots);
-  float* res = (second ? v_res : k_res) + (static_cast<int64_t>(b) * a.Hk + h0) * res_row;
+  // what goes beside this key, and behind the last key up to the tile's end
+  const int64_t res_row = a.window > 0 ? a.copy_slots : residue_row(slots);
+  float* res = (second ? v_res : k_res) + (a.window > 0 ? h0 * res_row + row : (static_cast<int64_t>(b) * a.Hk + h0) * res_row + j);
   if (j + 1 == slots)
     for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i)
-      for (int64_t x = slots + lane; x < res_row; x += GROUP) res[i * res_row + x] = 1.f;
+      for (int x = 1 + lane; x <= residue_row(slots) - slots; x += GROUP) res[i * res_row + x] = 1.f;
   if (c >= a.d) return;
   bool there = j < static_cast<unsigned>(n);
   if (a.window > 0) {
@@ -268,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
   if (page < 0 || page >= a.n_pages) {
     // not there, or reported by the kernel that reads the pages, which leaves it out
     if (lane == 0)
-      for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i) res[i * res_row + j] = 1.f;
+      for (int i = 0; i < kHeads && h0 + i < a.Hk; ++i) res[i * res_row] = 1.f;
     return;
   }
   const unsigned slot = j % a.page;
@@ -297,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) cache_expand_kernel(const __grid_con
         pow = __uint_as_float(bits & 0xff800000u);
         rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
       }
-      if (lane == 0) res[i * res_row + j] = second || !a.fold_scale ? rest : rest * (a.scale * kLog2e);
+      if (lane == 0) res[i * res_row] = second || !a.fold_scale ? rest : rest * (a.scale * kLog2e);
       float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -538,12 +560,18 @@ cudaError_t launch_rotary_write(const RotaryArgs& r, int dtype, bool table16, cu
   return dtype == kBF16 ? launch_rotary<__nv_bfloat16>(r, table16, st) : launch_rotary<__half>(r, table16, st);
 }
 
+void plan_copy_slots(PagedArgs& p) {
+  const int64_t table = residue_row(static_cast<int64_t>(p.table_width) * p.page);
+  const int64_t stride = residue_row(p.sinks) + residue_row(p.window) + 256, dense = p.B * stride + residue_row(p.T);
+  p.copy_dense = dense < p.B * table;
+  p.copy_stride = static_cast<int>(p.copy_dense ? stride : table);
+  p.copy_slots = p.copy_dense ? dense : p.B * table;
+}
+
 cudaError_t launch_cache_expand(const PagedArgs& p, int dtype, void* k, void* v, float* k_res, float* v_res,
                                 cudaStream_t st) {
-  int64_t per_seq = static_cast<int64_t>(p.table_width) * p.page;
-  // a window: the first keys' tiles, and from the first window's on what the rows can reach
-  if (p.window > 0) per_seq = std::min<int64_t>(per_seq, residue_row(p.sinks) + residue_row(p.window + p.T + 128));
-  const int64_t groups = p.B * per_seq * ((p.Hk + kHeads - 1) / kHeads);
+  const int64_t per_seq = p.window > 0 ? p.copy_stride : static_cast<int64_t>(p.table_width) * p.page;
+  const int64_t groups = (p.window > 0 ? p.copy_slots : p.B * per_seq) * ((p.Hk + kHeads - 1) / kHeads);
   const int64_t ctas = (groups * 16 + kThreads - 1) / kThreads;
   if (groups >= (1LL << 28)) return cudaErrorInvalidConfiguration;  // the caller's limit keeps it below
   const dim3 grid(static_cast<unsigned>(ctas), 2u);

@@ -110,3 +110,26 @@ def test_few_keys_on_either_side_of_the_rule(window, sinks, tokens, heads, kv_he
     got = _run(q, k, v, g, causal=True, window=window, sinks=sinks)
     for b in range(2):
         _check_sequence([x[b] for x in got], q[b], k[b], v[b], g[b], _reach(tokens, tokens, window, sinks), dim**-0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (40, 4), (100, 0), (128, 130), (257, 33), (700, 300), (1000, 1)])
+@pytest.mark.parametrize("rows,more", [([40, 200, 1, 0, 64], (0, 77, 900, 3, 1000)), ([130, 1, 127, 129], (1000, 640, 5, 333)),
+                                       ([1, 300, 2, 2, 2, 2, 90, 1], (5, 0, 700, 701, 702, 100, 64, 1500))])
+def test_chunks_with_wide_tables(rows, more, window, sinks, dtype):
+    """An e4m3 cache's copy holds what the rows can reach, however wide the block table: nothing else is read, the results
+    are those of a narrow table bit for bit, and right."""
+    from test_gpu_window import _check_paged
+
+    lens = [r + x for r, x in zip(rows, more)]
+    for heads, kv_heads, dim, page in ((32, 8, 64, 16), (12, 6, 80, 48), (32, 8, 128, 64)):
+        s = Setup(lens, rows, heads, kv_heads, dim, page, dtype, True, seed=window, tail=3)
+        narrow = s.table
+        want = _poisoned(s, window=window, sinks=sinks)
+        wide = torch.full((len(lens), 131072 // page), 2**31 - 1, dtype=torch.int32, device="cuda")
+        wide[:, : narrow.shape[1]] = narrow
+        s.table = wide
+        got = _poisoned(s, window=window, sinks=sinks)
+        total = sum(rows)
+        assert torch.equal(got[:total], want[:total])
+        _check_paged(s, got, window, sinks)
