@@ -365,7 +365,8 @@ cudaError_t expand_pages(const PagedArgs& p, int dtype, char* ws, PagedArgs& x, 
 }
 
 // The plan of a batch with a shared prefix: the prefix in parts on the tensor cores, 256 (row, head) pairs at once, then
-// the sequences' own keys in the split kernel, whose join takes the parts in.
+// the sequences' own keys in the split kernel, whose join takes the parts in.  Not of chunks for the tensor cores, whose
+// kernel goes through each sequence's pages.
 struct PrefixPlan {
   int keys = 0;  // 0: the prefix is not used
   int splits = 0, chunk = 0;

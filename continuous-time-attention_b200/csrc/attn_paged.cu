@@ -38,6 +38,9 @@
 // a shared prefix, whose sums another kernel leaves for the join.  64 sequences of 512 to 8192 keys in windows of 1024, 4
 // first keys, 16 bits: 57 us a call, 53 of them this kernel's, 270 MB at 5.1 TB/s; a worker has 27 groups there, and the
 // ramp up and the rest of the workers' ends weigh more than over whole sequences.
+// Over e4m3 48 us a call, at three CTAs an SM; with four, as over whole sequences, 72 bytes a thread are spilled and it takes 52.
+// Beside the prefix's parts, which fill their SMs' shared memory, it asks for its L1 (prefer_l1): without, 64 sequences of 2048
+// to 4096 own keys take 209 us instead of 132.
 //
 // e4m3: the codes are exact in fp16, so both products run in fp16 whatever the
 // type of q.  A bf16 row is first divided by the power of two at its largest

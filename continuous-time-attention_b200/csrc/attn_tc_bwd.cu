@@ -26,6 +26,9 @@
 // products; dim 64 406 and 537, 1020.  Both in one call, delta included, take 1655 and
 // 941: dQ's CTAs start while the last ones of dK and dV run.  fp16, with its bounds,
 // 1678 and 976.
+//
+// attn_tc_bwd_window.cu has these pipelines again, for windows, and CTAs that go from piece to piece: a change to the barriers
+// or the rings here belongs there too.
 #include <algorithm>
 
 #include "attn_tc_bwd.cuh"

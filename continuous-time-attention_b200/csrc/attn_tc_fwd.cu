@@ -41,6 +41,9 @@
 // 1070 TFLOP/s; 32/8 heads of 128, causal, 457 us, 1203; 16 heads of 64 426 us, 645
 // (runs on other boards: 503 to 510, 445, 400).
 // 4 chunks of 512 rows over 1500 to 8192 cached keys, 32/8 heads of 128: 162 us.
+//
+// attn_tc_fwd_reach.cu has this pipeline again, for rows that do not see every key: a change to the barriers or the rings here
+// belongs there too.
 #include <algorithm>
 
 #include "attn_tc_fwd.cuh"

@@ -1107,7 +1107,7 @@ def paged_attention(
     block_table, also of sequences that end earlier, name the same pages for the first
     shared_prefix of them (a page that they fill in part does not count).  Where that pays they are read once for all
     rows; it changes what the call costs, and its sums' order, not what it computes.
-    With a window it is not used.  A NaN or infinity in the v of a shared key may then also reach
+    It serves single tokens and a few per sequence; chunks of many rows, and calls with a window, are as without it.  A NaN or infinity in the v of a shared key may then also reach
     sequences that end before it."""
     return _paged_launch(*_paged_plan(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, max_rows, scale, k_scale,
                                       v_scale, out, window, sinks, shared_prefix))
