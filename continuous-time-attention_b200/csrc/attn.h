@@ -120,8 +120,8 @@ struct PagedArgs {
   float* part_o;   // [2 * workers, 16, dim rounded up to 64 or 128] fp32
   float* part_ml;  // [2 * workers, 16, 4] maximum, sum, maximum of the weighted values
   // tensor-core kernel: k_cache and v_cache hold launch_cache_expand's pages, and these what it left out of their
-  // elements [B, Hk, residue_row(table_width * page)], over a window [Hk, copy_slots]: the fractions of the scales in bf16, the key's scale and the
-  // logarithm (base 2) of the value's in fp16, rows on 32 bytes; else nullptr
+  // elements [B, Hk, residue_row(table_width * page)], over a window [Hk, copy_slots]: the fractions of the scales in
+  // bf16, the key's scale and the logarithm (base 2) of the value's in fp16, rows on 32 bytes; else nullptr
   const float* k_res;
   const float* v_res;
   int64_t expanded_pages;

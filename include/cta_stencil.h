@@ -467,9 +467,9 @@ int cta_window_paged_attention(const cta_paged_attention_args* args, int64_t win
  * page that they fill in part does not count), and those are read once for all
  * rows where that pays, by a rule on the prefix and the batch (the own keys'
  * number is not known on the host).  Chunks of many rows, which the tensor cores
- * take, go through each sequence's pages as without it.  It changes the cost and the order of the sums, not what
- * is computed.  Sequences may end within the prefix; their rows name its pages
- * all the same. */
+ * take, go through each sequence's pages as without it.  It changes the cost and
+ * the order of the sums, not what is computed.  Sequences may end within the
+ * prefix; their rows name its pages all the same. */
 int64_t cta_prefix_paged_attention_workspace_bytes(const cta_paged_attention_args* args, int64_t shared_prefix);
 int cta_prefix_paged_attention(const cta_paged_attention_args* args, int64_t shared_prefix, void* workspace,
                                int64_t workspace_bytes, void* stream);
